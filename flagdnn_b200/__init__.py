@@ -34,7 +34,8 @@ from .graph import (  # noqa: F401
     graph,
 )
 from .ops import (  # noqa: F401
-    adaptive_avg_pool2d, add, bias_add, conv1d, conv2d, gelu, max_pool2d, mm, mul, relu, sub,
+    adaptive_avg_pool2d, add, bias_add, causal_conv1d, causal_conv1d_step, conv1d, conv2d, gelu, group_norm, group_norm_backward,
+    max_pool2d, mm, mul, relu, selective_scan, selective_scan_step, sub,
 )
 
 __version__ = "0.1.0"

@@ -22,7 +22,7 @@ FDNN_DEVICE_TIMEOUT = 6
 
 F16, BF16, F32, F64 = 0, 1, 2, 3
 ALGO_AUTO, ALGO_DIRECT, ALGO_IGEMM, ALGO_IGEMM_PAIR = 0, 1, 2, 3
-ACT_NONE, ACT_RELU, ACT_GELU, ACT_GELU_TANH = 0, 1, 2, 3
+ACT_NONE, ACT_RELU, ACT_GELU, ACT_GELU_TANH, ACT_SILU = 0, 1, 2, 3, 4
 STREAMK_FLAG_BYTES = 8192
 ALGO_FLAG_STREAM_K = 0x100
 ALGO_FLAG_OUT_F32 = 0x200
@@ -53,6 +53,14 @@ EXPORTED_SYMBOLS = (
     "fdnn_conv2d_fwd_static_scratch",
     "fdnn_static_scratch_bytes",
     "fdnn_static_scratch_last_error",
+    "fdnn_group_norm_workspace_bytes",
+    "fdnn_group_norm_fwd",
+    "fdnn_group_norm_bwd",
+    "fdnn_causal_conv1d_fwd",
+    "fdnn_causal_conv1d_step",
+    "fdnn_selective_scan_workspace_bytes",
+    "fdnn_selective_scan_fwd",
+    "fdnn_selective_scan_step",
 )
 
 
@@ -113,6 +121,23 @@ class PoolDesc(ctypes.Structure):
                [("x_strides", ctypes.c_int64 * 4), ("y_strides", ctypes.c_int64 * 4)]
 
 
+class NormDesc(ctypes.Structure):
+    _fields_ = [(name, ctypes.c_int32) for name in ("dtype", "param_dtype", "n", "c", "h", "w", "groups", "activation")] + \
+               [("eps", ctypes.c_float), ("reserved", ctypes.c_int32)] + \
+               [(name, ctypes.c_int64 * 4) for name in ("x_strides", "y_strides", "dy_strides", "dx_strides")]
+
+
+class CausalConvDesc(ctypes.Structure):
+    _fields_ = [(name, ctypes.c_int32) for name in ("dtype", "n", "l", "c", "width", "activation")] + \
+               [("x_strides", ctypes.c_int64 * 3), ("y_strides", ctypes.c_int64 * 3)]
+
+
+class ScanDesc(ctypes.Structure):
+    _fields_ = [(name, ctypes.c_int32) for name in ("dtype", "n", "l", "c", "s", "groups", "delta_softplus", "reserved")] + \
+               [(name, ctypes.c_int64 * 3) for name in ("u_strides", "delta_strides", "z_strides", "y_strides")] + \
+               [("b_strides", ctypes.c_int64 * 4), ("c_strides", ctypes.c_int64 * 4)]
+
+
 class NativeError(RuntimeError):
     """A non-OK status that maps to RuntimeError in the reference's convention."""
 
@@ -168,6 +193,19 @@ def load() -> ctypes.CDLL:
     lib.fdnn_debug_set_wait_limit.argtypes = [i64, i32]
     lib.fdnn_debug_tensor_map_counters.restype = i32
     lib.fdnn_debug_tensor_map_counters.argtypes = [ctypes.POINTER(ctypes.c_int64), ctypes.POINTER(ctypes.c_int64)]
+    pi64, pnorm, pconv, pscan = (ctypes.POINTER(t) for t in (i64, NormDesc, CausalConvDesc, ScanDesc))
+    for name, args in (
+        ("fdnn_group_norm_workspace_bytes", [pnorm, i32, pi64]),
+        ("fdnn_group_norm_fwd", [pnorm] + [vp] * 7 + [i64, vp]),
+        ("fdnn_group_norm_bwd", [pnorm] + [vp] * 10 + [i64, vp]),
+        ("fdnn_causal_conv1d_fwd", [pconv] + [vp] * 8),
+        ("fdnn_causal_conv1d_step", [pconv] + [vp] * 4 + [i32] + [vp] * 3),
+        ("fdnn_selective_scan_workspace_bytes", [pscan, pi64]),
+        ("fdnn_selective_scan_fwd", [pscan] + [vp] * 13 + [i64, vp]),
+        ("fdnn_selective_scan_step", [pscan] + [vp] * 9 + [i32] + [vp] * 3),
+    ):
+        fn = getattr(lib, name)
+        fn.restype, fn.argtypes = i32, args
     lib.fdnn_device_status.restype = i32
     lib.fdnn_device_status.argtypes = [ctypes.POINTER(ctypes.c_uint32)]
     _lib = lib

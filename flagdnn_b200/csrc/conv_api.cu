@@ -14,6 +14,7 @@
 #include <string>
 
 #include "conv_internal.h"
+#include "sequence_internal.h"
 
 namespace fdnn {
 namespace {
@@ -1150,6 +1151,9 @@ bool launch_overlap_enabled() {
   }();
   return on;
 }
+
+int api_fail(int status, const char* text) { return fail(status, text); }
+int api_fail_cuda(const char* what, cudaError_t e) { return fail_cuda(what, e); }
 
 namespace {
 std::atomic<long long*> g_prof_buffer[64];  // per device ordinal; set through fdnn_debug_set_profile_buffer

@@ -1,0 +1,118 @@
+// Activations, their slopes and small reductions shared by the group norm and state space kernels.  All in fp32.
+#pragma once
+#include <math.h>
+
+#include <type_traits>
+
+#include "../../include/flagdnn_b200.h"
+#include "conv_convert.cuh"
+#include "sm100_ptx.cuh"
+
+namespace fdnn {
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+// 2^v by the special function unit (relative error 2^-22, subnormal results flushed)
+__device__ __forceinline__ float ex2(float v) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+// 1 / (1 + e^-v): the denominator is infinite below -88, which divides to zero
+__device__ __forceinline__ float logistic(float v) { return __fdividef(1.0f, 1.0f + ex2(-kLog2e * v)); }
+__device__ __forceinline__ float silu(float v) { return __fdividef(v, 1.0f + ex2(-kLog2e * v)); }
+// log(1 + e^v) without losing either end: e^-|v| is at most 1
+__device__ __forceinline__ float softplus(float v) { return fmaxf(v, 0.0f) + log1pf(ex2(-kLog2e * fabsf(v))); }
+
+constexpr float kSqrtHalf = 0.70710678118654752f;
+constexpr float kGeluTanhScale = 0.79788456080286536f;   // sqrt(2 / pi)
+constexpr float kGeluTanhCubic = 0.044715f;
+
+template <int ACT>
+__device__ __forceinline__ float activate(float v) {
+  if constexpr (ACT == FDNN_ACT_RELU) return v < 0.0f ? 0.0f : v;   // NaN stays
+  if constexpr (ACT == FDNN_ACT_GELU) return 0.5f * v * erfcf(-kSqrtHalf * v);
+  if constexpr (ACT == FDNN_ACT_GELU_TANH)   // (1 + tanh a) / 2 is the logistic function of 2 a
+    return __fdividef(v, 1.0f + ex2(-2.0f * kLog2e * kGeluTanhScale * (v + kGeluTanhCubic * v * v * v)));
+  if constexpr (ACT == FDNN_ACT_SILU) return silu(v);
+  return v;
+}
+
+// d activate(v) / dv
+template <int ACT>
+__device__ __forceinline__ float slope(float v) {
+  if constexpr (ACT == FDNN_ACT_RELU) return v > 0.0f ? 1.0f : 0.0f;
+  if constexpr (ACT == FDNN_ACT_GELU)
+    return 0.5f * erfcf(-kSqrtHalf * v) + 0.3989422804014327f * v * ex2(-0.5f * kLog2e * v * v);
+  if constexpr (ACT == FDNN_ACT_GELU_TANH) {
+    const float p = logistic(2.0f * kGeluTanhScale * (v + kGeluTanhCubic * v * v * v));
+    const float rest = p * (1.0f - p);   // zero far out, where the cube may have no finite value
+    return p + (rest == 0.0f ? 0.0f : v * rest * (2.0f * kGeluTanhScale) * (1.0f + 3.0f * kGeluTanhCubic * v * v));
+  }
+  if constexpr (ACT == FDNN_ACT_SILU) {
+    const float p = logistic(v);
+    const float rest = 1.0f - p;
+    return p * (1.0f + (rest == 0.0f ? 0.0f : v * rest));
+  }
+  return 1.0f;
+}
+
+// Runs f(std::integral_constant<int, ACT>) for a run-time activation: the branch is taken once, not per element.
+template <typename F>
+__device__ __forceinline__ void with_activation(int act, F&& f) {
+  switch (act) {
+    case FDNN_ACT_RELU: f(std::integral_constant<int, FDNN_ACT_RELU>{}); break;
+    case FDNN_ACT_GELU: f(std::integral_constant<int, FDNN_ACT_GELU>{}); break;
+    case FDNN_ACT_GELU_TANH: f(std::integral_constant<int, FDNN_ACT_GELU_TANH>{}); break;
+    case FDNN_ACT_SILU: f(std::integral_constant<int, FDNN_ACT_SILU>{}); break;
+    default: f(std::integral_constant<int, FDNN_ACT_NONE>{}); break;
+  }
+}
+
+// Mean and sum of squared deviations of two sets together (n_a + n_b > 0).
+struct Moments {
+  float n, mean, m2;
+};
+__device__ __forceinline__ Moments joined(const Moments& a, const Moments& b) {
+  const float n = a.n + b.n, d = b.mean - a.mean, share = b.n / n;
+  return Moments{n, a.mean + d * share, a.m2 + b.m2 + d * d * a.n * share};
+}
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+// Sum over a block of whole warps (at most 32); `scratch` holds 33 floats.  Every thread gets it.
+__device__ __forceinline__ float block_sum(float v, float* scratch) {
+  const int warps = blockDim.x >> 5;
+  v = warp_sum(v);
+  if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    const float t = warp_sum(int(threadIdx.x) < warps ? scratch[threadIdx.x] : 0.0f);
+    if (threadIdx.x == 0) scratch[32] = t;
+  }
+  __syncthreads();
+  const float r = scratch[32];
+  __syncthreads();
+  return r;
+}
+
+template <typename T>
+__device__ __forceinline__ float param(const void* p, int f32, long long i) {
+  return f32 ? static_cast<const float*>(p)[i] : to_f32<T>(static_cast<const T*>(p)[i]);
+}
+template <typename T>
+__device__ __forceinline__ void put_param(void* p, int f32, long long i, float v) {
+  if (f32) static_cast<float*>(p)[i] = v;
+  else static_cast<T*>(p)[i] = from_f32<T>(v);
+}
+
+// One launch after another on a stream without a gap: see griddep_wait().  First statement of every kernel here.
+__device__ __forceinline__ void chained() {
+  griddep_launch_dependents();
+  griddep_wait();
+}
+
+}  // namespace fdnn

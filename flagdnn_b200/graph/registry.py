@@ -277,6 +277,52 @@ def _run_adaptive_avg_pool2d(inputs: list, attrs: dict) -> torch.Tensor:
     return pool_host.adaptive_avg_pool2d(inputs[0], a["output_size"])
 
 
+# -------------------------------------------------------------- group norm
+_GROUP_NORM_ARG_NAMES = ["input", "num_groups", "weight", "bias", "eps", "activation", "return_stats"]
+
+
+def _normalize_group_norm(ctx: Any, args: tuple, kwargs: dict) -> tuple:
+    if len(args) > len(_GROUP_NORM_ARG_NAMES):
+        raise TypeError("group_norm got too many positional args")
+    params = {"weight": None, "bias": None, "eps": 1e-5, "activation": "none", "return_stats": False}
+    params.update(kwargs)
+    for name, arg in zip(_GROUP_NORM_ARG_NAMES, args):
+        if name in kwargs:
+            raise TypeError(f"group_norm got multiple values for {name}")
+        params[name] = arg
+    if params.pop("return_stats"):
+        raise NotImplementedError("graph group_norm returns values only (return_stats=False)")
+    if "input" not in params or "num_groups" not in params:
+        raise TypeError("group_norm expects an input and num_groups")
+    ids = [ctx.as_value(params.pop("input"), "input")]
+    params["operands"] = tuple(name for name in ("weight", "bias") if params[name] is not None)
+    for name in ("weight", "bias"):
+        value = params.pop(name)
+        if value is not None:
+            ids.append(ctx.as_value(value, name))
+    return ids, params
+
+
+def _infer_group_norm(specs: list, attrs: dict) -> TensorSpec:
+    x, groups = specs[0], int(attrs["num_groups"])
+    if not 2 <= len(x.shape) <= 4:
+        raise RuntimeError("graph group_norm expects 2 to 4 dimensions")
+    if groups <= 0 or x.shape[1] % groups != 0:
+        raise RuntimeError("graph group_norm channels must be divisible by num_groups")
+    for spec in specs[1:]:
+        if tuple(spec.shape) != (x.shape[1],):
+            raise RuntimeError("graph group_norm weight and bias must have one value per channel")
+    return _infer_same(specs, attrs)
+
+
+def _run_group_norm(inputs: list, attrs: dict) -> torch.Tensor:
+    from .. import norm_host
+
+    operands = dict(zip(attrs["operands"], inputs[1:]))
+    return norm_host.group_norm(inputs[0], int(attrs["num_groups"]), operands.get("weight"), operands.get("bias"), attrs["eps"],
+                                attrs["activation"])
+
+
 # -------------------------------------------------------------- glue ops
 def _normalize_unary(name: str):
     def normalize(ctx: Any, args: tuple, kwargs: dict) -> tuple:
@@ -379,6 +425,7 @@ def _register_defaults() -> None:
     register_op(OpSchema("max_pool2d", _normalize_max_pool2d, _infer_max_pool2d, _run_max_pool2d))
     register_op(OpSchema("adaptive_avg_pool2d", _normalize_adaptive_avg_pool2d, _infer_adaptive_avg_pool2d,
                          _run_adaptive_avg_pool2d))
+    register_op(OpSchema("group_norm", _normalize_group_norm, _infer_group_norm, _run_group_norm))
     register_op(OpSchema("bias_add", _normalize_binary("bias_add"), _infer_same, _run_bias_add))
     register_op(OpSchema("relu", _normalize_unary("relu"), _infer_same, _run_relu))
     register_op(OpSchema("fused_bias_relu", _normalize_binary("fused_bias_relu"), _infer_same, _run_fused_bias_relu))

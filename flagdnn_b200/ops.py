@@ -12,7 +12,9 @@ from typing import Any
 import torch
 
 from . import conv_host as _conv
+from . import norm_host as _norm
 from . import pool_host as _pool
+from . import sequence_host as _sequence
 from .graph.compiler import current_capture
 
 
@@ -57,9 +59,15 @@ relu = _capturable("relu", _eager_relu)
 gelu = _capturable("gelu", _eager_gelu)
 max_pool2d = _capturable("max_pool2d", _pool.max_pool2d)
 adaptive_avg_pool2d = _capturable("adaptive_avg_pool2d", _pool.adaptive_avg_pool2d)
+group_norm = _capturable("group_norm", _norm.group_norm)
 add = _capturable("add", _eager_binary(torch.add))
 sub = _capturable("sub", _eager_binary(torch.sub))
 mul = _capturable("mul", _eager_binary(torch.mul))
 conv1d = _conv.conv1d  # eager only: the graph registry has no conv1d node, as in the reference
 mm = _conv.mm          # eager only
+group_norm_backward = _norm.group_norm_backward
+causal_conv1d = _sequence.causal_conv1d            # the state space operators are eager only: they carry state
+causal_conv1d_step = _sequence.causal_conv1d_step
+selective_scan = _sequence.selective_scan
+selective_scan_step = _sequence.selective_scan_step
 fused_conv2d_bias_relu = _conv.fused_conv2d_bias_relu

@@ -76,6 +76,7 @@ typedef enum fdnn_status {
 #define FDNN_ACT_RELU 1
 #define FDNN_ACT_GELU 2      /* 0.5 x (1 + erf(x / sqrt 2)), torch's default */
 #define FDNN_ACT_GELU_TANH 3 /* torch's approximate="tanh" form */
+#define FDNN_ACT_SILU 4      /* x / (1 + exp(-x)); group norm and causal convolution only */
 
 /* Problem descriptor.  Replaces the argument list the reference passes to its
  * Triton launches (src/flag_dnn/graph/kernels/fused_conv.py:151-191,
@@ -263,6 +264,90 @@ int fdnn_max_pool2d_fwd(const fdnn_pool_desc* desc, const void* x, void* y,
  * [floor(o*L/O), ceil((o+1)*L/O)), fp32 (fp64) accumulate. */
 int fdnn_adaptive_avg_pool2d_fwd(const fdnn_pool_desc* desc, const void* x,
                                  void* y, void* stream);
+
+/* Group norm with an activation: y = act((x - mean) * rstd * weight + bias), mean and rstd over the
+ * c / groups * h * w values of an image's group, rstd = 1 / sqrt(variance + eps).  Channels-last x is read and
+ * written once; rows of tokens are h = w = 1.  fp32 statistics (no difference of large sums), one rounding.
+ * Channels-last tensors whose pixels lie at one stride (dense, or a slice of the channels) take the fast kernels, other
+ * strides a slower one. */
+typedef struct fdnn_norm_desc {
+  int32_t dtype;               /* FDNN_F16, FDNN_BF16 or FDNN_F32: x, y, dy, dx */
+  int32_t param_dtype;         /* weight, bias and their gradients: dtype or FDNN_F32 */
+  int32_t n, c, h, w, groups;
+  int32_t activation;          /* FDNN_ACT_* */
+  float eps;
+  int32_t reserved;            /* 0 */
+  int64_t x_strides[4];        /* element strides in (n, c, h, w) order */
+  int64_t y_strides[4];
+  int64_t dy_strides[4];       /* backward only */
+  int64_t dx_strides[4];
+} fdnn_norm_desc;
+
+/* Scratch that fdnn_group_norm_fwd (backward = 0) or fdnn_group_norm_bwd (1) needs, 16-byte aligned. */
+int fdnn_group_norm_workspace_bytes(const fdnn_norm_desc* desc, int backward, int64_t* bytes);
+
+/* weight and bias [C] or NULL; mean and rstd [N, groups] float32, both or neither. */
+int fdnn_group_norm_fwd(const fdnn_norm_desc* desc, const void* x, const void* weight, const void* bias, void* y,
+                        float* mean, float* rstd, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* The gradient for dy, from x and the forward call's mean and rstd.  dx, dweight and dbias may each be NULL.  Sums are
+ * made in a fixed order: equal calls give equal bits. */
+int fdnn_group_norm_bwd(const fdnn_norm_desc* desc, const void* dy, const void* x, const float* mean,
+                        const float* rstd, const void* weight, const void* bias, void* dx, void* dweight,
+                        void* dbias, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* The short depthwise convolution in front of a state space scan, over tokens in their order:
+ * y[n, t, c] = act(bias[c] + sum_j weight[c, j] * xs[n, t + j, c]), xs = the width - 1 inputs before the first token
+ * (initial_state [N, width - 1, C] dense, NULL: zeros), then x.  Tokens from lengths[n] on (int32, NULL: none) are padding:
+ * never read, y = 0 there.  final_state (NULL: not wanted) receives the last width - 1 inputs of each row; it must not
+ * overlap initial_state. */
+#define FDNN_CAUSAL_CONV_MAX_WIDTH 8
+typedef struct fdnn_causal_conv_desc {
+  int32_t dtype;               /* FDNN_F16, FDNN_BF16 or FDNN_F32: every tensor */
+  int32_t n, l, c, width;
+  int32_t activation;          /* FDNN_ACT_* */
+  int64_t x_strides[3];        /* element strides in (n, l, c) order */
+  int64_t y_strides[3];
+} fdnn_causal_conv_desc;
+int fdnn_causal_conv1d_fwd(const fdnn_causal_conv_desc* desc, const void* x, const void* weight, const void* bias,
+                           const void* initial_state, const int32_t* lengths, void* y, void* final_state, void* stream);
+
+/* The same for one token of each row (desc->l and the l strides are not read): row n continues state number slots[n] (int32;
+ * NULL: n) of n_slots, [n_slots, width - 1, C] dense, which is updated in place.  A row whose slot is not in [0, n_slots)
+ * is idle: y = 0.  Two rows must not have the same slot. */
+int fdnn_causal_conv1d_step(const fdnn_causal_conv_desc* desc, const void* x, const void* weight, const void* bias,
+                            void* state, int32_t n_slots, const int32_t* slots, void* y, void* stream);
+
+/* The selective state space scan: with dt = delta + delta_bias (softplus of it if delta_softplus),
+ *   h[t] = exp(dt A) h[t-1] + dt u[t] B[t],   y[t] = (sum over the states of C[t] h[t] + D u[t]) * silu(z[t])
+ * for each channel, whose s states are fp32; B and C are shared by the c / groups channels of a group.  A [C, s], D,
+ * delta_bias [C] and the states [N, C, s] are dense float32; D, z, delta_bias, initial_state (zeros), lengths (see above) and
+ * final_state may be NULL.  final_state must not overlap initial_state. */
+#define FDNN_SCAN_MAX_STATES 256
+typedef struct fdnn_scan_desc {
+  int32_t dtype;               /* FDNN_F16, FDNN_BF16 or FDNN_F32: u, delta, B, C, z, y */
+  int32_t n, l, c, s, groups;
+  int32_t delta_softplus;
+  int32_t reserved;            /* 0 */
+  int64_t u_strides[3];        /* element strides in (n, l, c) order */
+  int64_t delta_strides[3];
+  int64_t z_strides[3];
+  int64_t y_strides[3];
+  int64_t b_strides[4];        /* (n, l, group, state) */
+  int64_t c_strides[4];
+} fdnn_scan_desc;
+
+/* Scratch that fdnn_selective_scan_fwd needs, 16-byte aligned: long rows are cut into pieces that run side by side. */
+int fdnn_selective_scan_workspace_bytes(const fdnn_scan_desc* desc, int64_t* bytes);
+int fdnn_selective_scan_fwd(const fdnn_scan_desc* desc, const void* u, const void* delta, const float* A, const void* B,
+                            const void* C, const float* D, const void* z, const float* delta_bias,
+                            const float* initial_state, const int32_t* lengths, void* y, float* final_state,
+                            void* workspace, int64_t workspace_bytes, void* stream);
+
+/* The same for one token of each row (l is not read), states [n_slots, C, s] in place as for fdnn_causal_conv1d_step. */
+int fdnn_selective_scan_step(const fdnn_scan_desc* desc, const void* u, const void* delta, const float* A, const void* B,
+                             const void* C, const float* D, const void* z, const float* delta_bias, float* state,
+                             int32_t n_slots, const int32_t* slots, void* y, void* stream);
 
 /* Every wait inside the kernels is bounded; a wait that runs out records a
  * code in a per-device status word and the kernel returns early.  This call
