@@ -1,4 +1,4 @@
-// Pairs of fp32 values in one 64-bit register (fma.rn.f32x2), shared by the depthwise kernels.
+// Pairs of fp32 values in one 64-bit register (fma.rn.f32x2), shared by the depthwise and scan kernels.
 #pragma once
 #include <stdint.h>
 
@@ -20,5 +20,13 @@ __device__ __forceinline__ F2 f2_fma(F2 a, F2 b, F2 c) {
   F2 d;
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
   return d;
+}
+__device__ __forceinline__ F2 f2_mul(F2 a, F2 b) {
+  F2 d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ F2 f2_pack(float lo, float hi) {
+  return f2_make(__float_as_uint(lo), __float_as_uint(hi));
 }
 }  // namespace fdnn

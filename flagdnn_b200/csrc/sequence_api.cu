@@ -5,6 +5,8 @@ using namespace fdnn;
 
 namespace {
 
+constexpr int32_t kMaxTokens = 0x7fffffff - 1024;   // tiles past a row's end are counted in 32 bits
+
 bool float_type(int dtype) { return dtype == FDNN_F16 || dtype == FDNN_BF16 || dtype == FDNN_F32; }
 
 int norm_params(const fdnn_norm_desc* d, NormParams* p) {
@@ -46,6 +48,7 @@ int causal_params(const fdnn_causal_conv_desc* d, CausalConvParams* p) {
   if (d == nullptr) return api_fail(FDNN_BAD_PARAM, "descriptor is NULL");
   if (!float_type(d->dtype)) return api_fail(FDNN_NOT_SUPPORTED, "Unsupported dtype");
   if (d->n < 0 || d->l < 0 || d->c < 0) return api_fail(FDNN_BAD_PARAM, "negative extent");
+  if (d->l > kMaxTokens) return api_fail(FDNN_NOT_SUPPORTED, "more tokens in a row than the kernels count");
   if (d->width < 1 || d->width > FDNN_CAUSAL_CONV_MAX_WIDTH) return api_fail(FDNN_NOT_SUPPORTED, "the filter must have 1 to 8 taps");
   if (d->activation < FDNN_ACT_NONE || d->activation > FDNN_ACT_SILU) return api_fail(FDNN_BAD_PARAM, "unknown activation");
   p->N = d->n; p->L = d->l; p->C = d->c; p->width = d->width; p->act = d->activation;
@@ -60,6 +63,7 @@ int scan_params(const fdnn_scan_desc* d, ScanParams* p) {
   if (d == nullptr) return api_fail(FDNN_BAD_PARAM, "descriptor is NULL");
   if (!float_type(d->dtype)) return api_fail(FDNN_NOT_SUPPORTED, "Unsupported dtype");
   if (d->n < 0 || d->l < 0 || d->c < 0) return api_fail(FDNN_BAD_PARAM, "negative extent");
+  if (d->l > kMaxTokens) return api_fail(FDNN_NOT_SUPPORTED, "more tokens in a row than the kernels count");
   if (d->s < 1 || d->s > FDNN_SCAN_MAX_STATES) return api_fail(FDNN_NOT_SUPPORTED, "a channel must have 1 to 256 states");
   if (d->groups <= 0 || d->c % d->groups != 0) return api_fail(FDNN_BAD_PARAM, "channels must be divisible by groups");
   p->N = d->n; p->L = d->l; p->C = d->c; p->S = d->s; p->G = d->groups;

@@ -1,6 +1,9 @@
 // Launching the group norm and state space kernels (host side).
 #pragma once
 #include <cuda_runtime.h>
+#include <stdint.h>
+
+#include <atomic>
 
 #include "conv_internal.h"
 
@@ -30,6 +33,19 @@ cudaError_t launch_seq(void (*kernel)(P...), dim3 grid, int threads, int smem, i
   cfg.attrs = attr;
   cfg.numAttrs = unsigned(n);
   return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+}
+
+// Opts a kernel in to `bytes` of dynamic shared memory, once per device (`done`: a bit per device ordinal).
+template <typename K>
+cudaError_t allow_smem(K* kernel, int bytes, std::atomic<uint64_t>& done) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const uint64_t bit = 1ull << (dev & 63);
+  if ((done.load(std::memory_order_acquire) & bit) != 0) return cudaSuccess;
+  e = cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
+  return e;
 }
 
 }  // namespace fdnn

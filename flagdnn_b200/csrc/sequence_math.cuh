@@ -21,8 +21,23 @@ __device__ __forceinline__ float ex2(float v) {
 // 1 / (1 + e^-v): the denominator is infinite below -88, which divides to zero
 __device__ __forceinline__ float logistic(float v) { return __fdividef(1.0f, 1.0f + ex2(-kLog2e * v)); }
 __device__ __forceinline__ float silu(float v) { return __fdividef(v, 1.0f + ex2(-kLog2e * v)); }
-// log(1 + e^v) without losing either end: e^-|v| is at most 1
-__device__ __forceinline__ float softplus(float v) { return fmaxf(v, 0.0f) + log1pf(ex2(-kLog2e * fabsf(v))); }
+// log(1 + e^v) = max(v, 0) + log(1 + e), e = e^-|v| at most 1.  log(1 + e) / e is a polynomial of degree 9, fitted to the
+// smallest relative error on [0, 1] (5e-9; 1.3e-7 in fp32 arithmetic): no result is lost where e is small, and no second call of
+// the special function unit, which bounds the scan.
+__device__ __forceinline__ float softplus(float v) {
+  const float e = ex2(-kLog2e * fabsf(v));
+  float p = -0.0032440070062875748f;
+  p = fmaf(p, e, 0.019851384684443474f);
+  p = fmaf(p, e, -0.056959398090839386f);
+  p = fmaf(p, e, 0.10603642463684082f);
+  p = fmaf(p, e, -0.15305586159229279f);
+  p = fmaf(p, e, 0.19675937294960022f);
+  p = fmaf(p, e, -0.24954132735729218f);
+  p = fmaf(p, e, 0.3332996368408203f);
+  p = fmaf(p, e, -0.4999990165233612f);
+  p = fmaf(p, e, 1.0f);
+  return fmaf(p, e, fmaxf(v, 0.0f));   // NaN stays: e is NaN then
+}
 
 constexpr float kSqrtHalf = 0.70710678118654752f;
 constexpr float kGeluTanhScale = 0.79788456080286536f;   // sqrt(2 / pi)
