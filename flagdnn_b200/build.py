@@ -15,7 +15,8 @@ from pathlib import Path
 PKG_DIR = Path(__file__).resolve().parent
 CSRC = PKG_DIR / "csrc"
 LIB_PATH = PKG_DIR / "libflagdnn_b200.so"
-HOST_SOURCE = CSRC / "host" / "fastcall.cpp"
+HOST_DIR = CSRC / "host"
+HOST_SOURCES = (HOST_DIR / "fastcall.cpp", HOST_DIR / "sequence_fast.cpp")
 HOST_PATH = PKG_DIR / "_fastcall.so"
 
 NVCC_FLAGS = [
@@ -76,13 +77,13 @@ def _host_stale() -> bool:
     if not HOST_PATH.exists():
         return True
     built = HOST_PATH.stat().st_mtime
-    if any(p.stat().st_mtime > built for p in (HOST_SOURCE, header) if p.exists()):
+    if any(p.stat().st_mtime > built for p in (*HOST_DIR.iterdir(), header) if p.is_file()):
         return True
     return (host_tag() + "\0").encode() not in HOST_PATH.read_bytes()
 
 
 def build_host(force: bool = False, verbose: bool = False) -> Path:
-    """Compile the native host path of the eager operators (csrc/host/fastcall.cpp) against the installed torch."""
+    """Compile the native host path of the eager operators (csrc/host) against the installed torch."""
     if not force and not _host_stale():
         return HOST_PATH
     import sysconfig
@@ -98,7 +99,7 @@ def build_host(force: bool = False, verbose: bool = False) -> Path:
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f'-DFDNN_HOST_TAG="{host_tag()}"',
            f"-I{root / 'include'}", f"-I{root / 'include' / 'torch' / 'csrc' / 'api' / 'include'}",
            f"-I{sysconfig.get_paths()['include']}", f"-I{cuda / 'include'}",
-           "-o", str(HOST_PATH), str(HOST_SOURCE), f"-L{root / 'lib'}",
+           "-o", str(HOST_PATH), *map(str, HOST_SOURCES), f"-L{root / 'lib'}",
            "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch", "-ltorch_python", f"-Wl,-rpath,{root / 'lib'}"]
     if verbose:
         print(" ".join(cmd), file=sys.stderr)

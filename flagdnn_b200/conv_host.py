@@ -277,12 +277,21 @@ def _load_fast() -> Any:
             _fastcall.bind(*address, _packed_for_native, lib.fdnn_abi_version(), ctypes.sizeof(nat.ConvDesc),
                            ctypes.sizeof(nat.ConvPlan))
             _fastcall.bind_unpacked(ctypes.cast(lib.fdnn_conv2d_fwd_unpacked, ctypes.c_void_p).value)
+            _fastcall.bind_sequence(*(ctypes.cast(f, ctypes.c_void_p).value for f in (
+                lib.fdnn_group_norm_workspace_bytes, lib.fdnn_group_norm_fwd, lib.fdnn_group_norm_bwd, lib.fdnn_causal_conv1d_fwd,
+                lib.fdnn_causal_conv1d_step, lib.fdnn_selective_scan_workspace_bytes, lib.fdnn_selective_scan_fwd,
+                lib.fdnn_selective_scan_step)), *(ctypes.sizeof(t) for t in (nat.NormDesc, nat.CausalConvDesc, nat.ScanDesc)))
             _fast = _fastcall
         except (ImportError, AttributeError, TypeError) as exc:   # not built, or built against something else
             warnings.warn(f"flagdnn_b200: the native host path is not used, calls take some 15 us longer ({exc}); "
                           "build it with `python -m flagdnn_b200.build`", RuntimeWarning, stacklevel=3)
             _fast = False
     return _fast
+
+
+def native_host() -> Any:
+    """The native host path, or False where there is none."""
+    return _fast if _fast is not None else _load_fast()
 
 
 def fast_conv(input, weight, bias, scale, residual, stride, padding, dilation, groups, act) -> Optional[torch.Tensor]:

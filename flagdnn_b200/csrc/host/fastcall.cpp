@@ -24,9 +24,11 @@
 #include <cstring>
 #include <unordered_map>
 
-#include "../../../include/flagdnn_b200.h"
+#include "host_common.h"
 
 namespace {
+
+using namespace fdnn_host;
 
 using QueryFn = int (*)(const fdnn_conv_desc*, const void*, const void*, const void*, fdnn_conv_plan*);
 using FwdFn = int (*)(const fdnn_conv_desc*, const void*, const void*, const void*, const void*, const void*, const void*,
@@ -72,16 +74,6 @@ std::unordered_map<PlanKey, fdnn_conv_plan, PlanHash>& plans() {   // used with 
   return *m;
 }
 
-// nullptr: not a plain strided CUDA tensor (subclasses and other layouts take the Python route).  The tensors belong to
-// the caller's arguments, which outlive the call.
-const at::Tensor* plain(PyObject* o) {
-  if (!THPVariable_CheckExact(o)) return nullptr;
-  const at::Tensor& t = THPVariable_Unpack(o);
-  if (!t.defined() || !t.is_cuda() || t.layout() != at::kStrided || !t.has_storage() || t.is_conj() || t.is_neg())
-    return nullptr;   // (tensors without storage: wrappers of function transforms)
-  return &t;
-}
-
 // An int, or two of them.
 bool pair_of(PyObject* o, int64_t (&v)[2]) {
   auto one = [](PyObject* p, int64_t* out) {
@@ -102,15 +94,6 @@ bool pair_of(PyObject* o, int64_t (&v)[2]) {
   return one(PyTuple_GET_ITEM(o, 0), &v[0]) && one(PyTuple_GET_ITEM(o, 1), &v[1]);
 }
 
-int dtype_code(at::ScalarType t) {
-  switch (t) {
-    case at::kHalf: return FDNN_F16;
-    case at::kBFloat16: return FDNN_BF16;
-    case at::kFloat: return FDNN_F32;
-    default: return -1;
-  }
-}
-
 int64_t out_dim(int64_t in, int64_t pad, int64_t dil, int64_t k, int64_t stride) {
   const int64_t span = in + 2 * pad - dil * (k - 1) - 1;
   return span < 0 ? 0 : span / stride + 1;
@@ -127,14 +110,6 @@ bool vector_of(PyObject* o, const at::Tensor& x, int64_t k, const void** ptr) {
   *ptr = t->const_data_ptr();
   return true;
 }
-
-PyObject* none() { Py_RETURN_NONE; }
-
-// Other Python threads may run while this one allocates and launches (an allocation can wait for the device).
-struct WithoutGil {
-  PyThreadState* state = PyEval_SaveThread();
-  ~WithoutGil() { PyEval_RestoreThread(state); }
-};
 
 // Runs one planned convolution; `weight_obj` is the tensor the packed-filter cache knows, or nullptr when the filter is
 // a view made for this call (packed into a buffer of this call then).  Returns 0 or the C ABI's status; -1 with a Python
@@ -400,7 +375,14 @@ PyMethodDef kMethods[] = {
     {"conv", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(fast_conv)), METH_FASTCALL, nullptr},
     {"conv1d", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(fast_conv1d)), METH_FASTCALL, nullptr},
     {"mm", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(fast_mm)), METH_FASTCALL, nullptr},
+    {"group_norm", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(fast_group_norm)), METH_FASTCALL, nullptr},
+    {"group_norm_backward", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(fast_group_norm_backward)), METH_FASTCALL, nullptr},
+    {"causal_conv1d", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(fast_causal_conv1d)), METH_FASTCALL, nullptr},
+    {"causal_conv1d_step", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(fast_causal_conv1d_step)), METH_FASTCALL, nullptr},
+    {"selective_scan", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(fast_selective_scan)), METH_FASTCALL, nullptr},
+    {"selective_scan_step", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(fast_selective_scan_step)), METH_FASTCALL, nullptr},
     {"bind", bind, METH_VARARGS, nullptr},
+    {"bind_sequence", bind_sequence, METH_VARARGS, nullptr},
     {"bind_unpacked", bind_unpacked, METH_O, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_fastcall", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};

@@ -12,6 +12,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _native as nat
+from . import conv_host as _conv
 
 _DTYPE_IDS = {torch.float16: nat.F16, torch.bfloat16: nat.BF16, torch.float32: nat.F32}
 ACTIVATIONS = {"none": nat.ACT_NONE, "relu": nat.ACT_RELU, "gelu": nat.ACT_GELU, "gelu_tanh": nat.ACT_GELU_TANH,
@@ -22,6 +23,13 @@ def activation_id(activation: str) -> int:
     if activation not in ACTIVATIONS:
         raise RuntimeError(f"activation must be one of {', '.join(ACTIVATIONS)}, got {activation!r}")
     return ACTIVATIONS[activation]
+
+
+def answered(result):
+    """What the native host path answered: a status is raised."""
+    if result.__class__ is int:
+        nat.check(result)
+    return result
 
 
 def workspace(nbytes: int, device: torch.device) -> Optional[torch.Tensor]:
@@ -156,6 +164,11 @@ def group_norm(input: torch.Tensor, num_groups: int, weight: Optional[torch.Tens
     Weight and bias are of the input's type or float32.  With ``return_stats`` the result is ``(y, mean, rstd)``, the float32
     [N, num_groups] statistics that ``group_norm_backward`` takes.  Differentiable once."""
     act = activation_id(activation)
+    fast = _conv._fast or _conv.native_host()
+    if fast:
+        y = fast.group_norm(input, num_groups, weight, bias, float(eps), act, bool(return_stats))
+        if y is not None:
+            return answered(y)
     _check(input, num_groups, weight, bias)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (input, weight, bias)):
         y, mean, rstd = _GroupNorm.apply(input, weight, bias, num_groups, float(eps), act)
@@ -169,6 +182,11 @@ def group_norm_backward(dy: torch.Tensor, input: torch.Tensor, mean: torch.Tenso
     """The gradient of ``group_norm`` for ``dy``: ``(dx, dweight, dbias)``, None in the place of a parameter that is None.
     ``mean`` and ``rstd`` are what the forward call returned.  The sums are made in a fixed order."""
     act = activation_id(activation)
+    fast = _conv._fast or _conv.native_host()
+    if fast:
+        grads = fast.group_norm_backward(dy, input, mean, rstd, num_groups, weight, bias, act)
+        if grads is not None:
+            return answered(grads)
     _check(input, num_groups, weight, bias)
     if dy.shape != input.shape or dy.dtype != input.dtype or dy.device != input.device:
         raise RuntimeError("dy must have the input's shape, dtype and device")

@@ -16,7 +16,8 @@ from typing import Optional
 import torch
 
 from . import _native as nat
-from .norm_host import _DTYPE_IDS, activation_id, address, workspace
+from . import conv_host as _conv
+from .norm_host import _DTYPE_IDS, activation_id, address, answered, workspace
 
 MAX_WIDTH, MAX_STATES = 8, 256
 
@@ -78,6 +79,11 @@ def causal_conv1d(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Te
     None) followed by ``x`` [N, L, C].  With ``return_final_state`` the result is ``(y, state after the row)``."""
     what = "causal_conv1d"
     act = activation_id(activation)
+    fast = _conv._fast or _conv.native_host()
+    if fast:
+        y = fast.causal_conv1d(x, weight, bias, act, initial_state, lengths, bool(return_final_state))
+        if y is not None:
+            return answered(y)
     _check_input(what, "x", x, 3)
     weight, bias, width = _check_conv(what, x, weight, bias)
     n, length, c = x.shape
@@ -116,6 +122,11 @@ def causal_conv1d_step(x: torch.Tensor, conv_state: torch.Tensor, weight: torch.
     """``causal_conv1d`` of the next token of each row, ``x`` [N, C]; ``conv_state`` [slots, width - 1, C] is updated in place."""
     what = "causal_conv1d_step"
     act = activation_id(activation)
+    fast = _conv._fast or _conv.native_host()
+    if fast:
+        y = fast.causal_conv1d_step(x, conv_state, weight, bias, act, slots)
+        if y is not None:
+            return answered(y)
     _check_input(what, "x", x, 2)
     weight, bias, width = _check_conv(what, x, weight, bias)
     n, c = x.shape
@@ -175,6 +186,12 @@ def selective_scan(u: torch.Tensor, delta: torch.Tensor, A: torch.Tensor, B: tor
     ``A`` [C, S], ``D`` and ``delta_bias`` [C] are float32; ``B`` and ``C`` [N, L, S], or [N, L, groups, S] where each group of
     channels has its own.  ``initial_state`` and the returned state are float32 [N, C, S]."""
     what = "selective_scan"
+    fast = _conv._fast or _conv.native_host()
+    if fast:
+        y = fast.selective_scan(u, delta, A, B, C, D, z, delta_bias, bool(delta_softplus), initial_state, lengths,
+                                bool(return_final_state))
+        if y is not None:
+            return answered(y)
     _check_input(what, "u", u, 3)
     d, A, B, C, D, delta_bias = _check_scan(what, u, delta, A, B, C, D, z, delta_bias)
     n, length, c = u.shape
@@ -205,6 +222,11 @@ def selective_scan_step(u: torch.Tensor, delta: torch.Tensor, A: torch.Tensor, B
     """``selective_scan`` of the next token of each row: ``u``, ``delta``, ``z`` [N, C], ``B`` and ``C`` [N, S] or
     [N, groups, S]; ``state`` [slots, C, S] float32 is updated in place."""
     what = "selective_scan_step"
+    fast = _conv._fast or _conv.native_host()
+    if fast:
+        y = fast.selective_scan_step(u, delta, A, B, C, state, D, z, delta_bias, bool(delta_softplus), slots)
+        if y is not None:
+            return answered(y)
     _check_input(what, "u", u, 2)
     d, A, B, C, D, delta_bias = _check_scan(what, u, delta, A, B, C, D, z, delta_bias)
     n, c = u.shape
