@@ -7,9 +7,7 @@
 // Statistics are a mean and a sum of squared deviations from it, never a difference of two large sums: values whose mean
 // is thousands of times their spread keep their precision.  All sums are fp32 in a fixed order, so that equal calls give
 // equal results.
-#include "sequence_internal.h"
-#include "sequence_launch.h"
-#include "sequence_math.cuh"
+#include "group_norm.cuh"
 
 namespace fdnn {
 namespace {
@@ -162,6 +160,35 @@ norm_channel_sums_kernel(const NormParams p) {
   }
 }
 
+// The same for images of a few pixels: a thread per channel.
+template <typename T>
+__global__ void __launch_bounds__(kThreads)
+norm_channel_sums_thin_kernel(const NormParams p) {
+  chained();
+  float2* sums = static_cast<float2*>(p.workspace);
+  const long long items = (long long)p.N * p.C;
+  with_activation(p.act, [&](auto act) {
+    for (long long item = blockIdx.x * (long long)kThreads + threadIdx.x; item < items; item += (long long)gridDim.x * kThreads) {
+      const int n = int(item / p.C), c = int(item % p.C);
+      const long long ng = (long long)n * p.G + c / (p.C / p.G);
+      const float mean = p.mean[ng], rstd = p.rstd[ng];
+      const float w = p.weight != nullptr ? param<T>(p.weight, p.param_f32, c) : 1.0f;
+      const float b = p.bias != nullptr ? param<T>(p.bias, p.param_f32, c) : 0.0f;
+      const T* x = static_cast<const T*>(p.x) + n * p.x_s[0] + c * p.x_s[1];
+      const T* dy = static_cast<const T*>(p.dy) + n * p.dy_s[0] + c * p.dy_s[1];
+      float2 t = make_float2(0.0f, 0.0f);
+      for (int h = 0; h < p.H; ++h)
+        for (int q = 0; q < p.W; ++q) {
+          const float xh = (to_f32<T>(x[h * p.x_s[2] + q * p.x_s[3]]) - mean) * rstd;
+          const float g = to_f32<T>(dy[h * p.dy_s[2] + q * p.dy_s[3]]) * slope<decltype(act)::value>(xh * w + b);
+          t.x += g * xh;
+          t.y += g;
+        }
+      sums[item] = t;
+    }
+  });
+}
+
 template <typename T, typename I>
 __global__ void __launch_bounds__(kThreads)
 norm_dx_kernel(const NormParams p) {
@@ -204,7 +231,7 @@ norm_dx_kernel(const NormParams p) {
   }
 }
 
-// dweight and dbias from `rows` rows of [C] pairs: 32 channels a block, its eight warps an eighth of the rows each.
+// 32 channels a block, its eight warps an eighth of the rows each (every eighth row, four on their way).
 template <typename T>
 __global__ void __launch_bounds__(256)
 norm_dparams_kernel(const NormParams p, const float2* rows, long long count) {
@@ -213,12 +240,14 @@ norm_dparams_kernel(const NormParams p, const float2* rows, long long count) {
   const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5;
   const int c = blockIdx.x * 32 + lane;
   float2 v = make_float2(0.0f, 0.0f);
-  if (c < p.C)
+  if (c < p.C) {
+#pragma unroll 8
     for (long long r = slice; r < count; r += 8) {
       const float2 q = rows[r * p.C + c];
       v.x += q.x;
       v.y += q.y;
     }
+  }
   part[slice][lane] = v;
   __syncthreads();
   if (slice != 0 || c >= p.C) return;
@@ -242,15 +271,17 @@ cudaError_t forward(const NormParams& p, cudaStream_t stream) {
 
 template <typename T, typename I>
 cudaError_t backward(const NormParams& p, cudaStream_t stream) {
-  cudaError_t e = launch_seq(norm_channel_sums_kernel<T, I>, dim3(grid_of((long long)p.N * p.C)), kThreads, 0, 1, stream, p);
+  const long long channels = (long long)p.N * p.C;
+  cudaError_t e = (long long)p.H * p.W <= 32
+                      ? launch_seq(norm_channel_sums_thin_kernel<T>, dim3(grid_of((channels + kThreads - 1) / kThreads)), kThreads, 0, 1, stream, p)
+                      : launch_seq(norm_channel_sums_kernel<T, I>, dim3(grid_of(channels)), kThreads, 0, 1, stream, p);
   if (e != cudaSuccess) return e;
   if (p.dx != nullptr) {
     e = launch_seq(norm_dx_kernel<T, I>, dim3(grid_of((long long)p.N * p.G * chunks_of(p).count)), kThreads, 0, 1, stream, p);
     if (e != cudaSuccess) return e;
   }
   if (p.dweight == nullptr && p.dbias == nullptr) return cudaSuccess;
-  return launch_seq(norm_dparams_kernel<T>, dim3(unsigned((p.C + 31) / 32)), 256, 0, 1, stream, p,
-                    static_cast<const float2*>(p.workspace), (long long)p.N);
+  return launch_norm_dparams<T>(p, static_cast<const float2*>(p.workspace), p.N, stream);
 }
 
 bool small(const NormParams& p) { return (long long)(p.C / p.G) * p.H * p.W < (1ll << 31); }
@@ -266,13 +297,26 @@ cudaError_t backward_t(const NormParams& p, cudaStream_t stream) {
 
 }  // namespace
 
+template <typename T>
+cudaError_t launch_norm_dparams(const NormParams& p, const float2* rows, long long count, cudaStream_t stream) {
+  return launch_seq(norm_dparams_kernel<T>, dim3(unsigned((p.C + 31) / 32)), 256, 0, 1, stream, p, rows, count);
+}
+template cudaError_t launch_norm_dparams<__half>(const NormParams&, const float2*, long long, cudaStream_t);
+template cudaError_t launch_norm_dparams<__nv_bfloat16>(const NormParams&, const float2*, long long, cudaStream_t);
+template cudaError_t launch_norm_dparams<float>(const NormParams&, const float2*, long long, cudaStream_t);
+
+// Known without the tensors' addresses: the most that any kernel which may take the problem needs.
 long long group_norm_workspace(int dtype, const NormParams& p, bool backward) {
-  (void)dtype;
-  if (backward) return 8ll * p.N * p.C;
-  return 8ll * p.N * p.G * chunks_of(p).count;
+  const long long here = 8ll * p.N * (backward ? p.C : p.G * chunks_of(p).count);
+  if (!norm_rows(p, backward) || p.C / p.G > 512 || (long long)p.H * p.W > (1 << 29)) return here;
+  const long long images = norm_images_workspace(dtype, p, backward);
+  const long long tokens = p.H == 1 && p.W == 1 ? norm_tokens_workspace(dtype, p, backward) : 0;
+  return tokens > images ? tokens : images;
 }
 
 cudaError_t launch_group_norm(int dtype, const NormParams& p, cudaStream_t stream) {
+  if (norm_tokens_take(dtype, p, false)) return launch_norm_tokens(dtype, p, false, stream);
+  if (norm_images_take(dtype, p, false)) return launch_norm_images(dtype, p, false, stream);
   switch (dtype) {
     case FDNN_F16: return forward_t<__half>(p, stream);
     case FDNN_BF16: return forward_t<__nv_bfloat16>(p, stream);
@@ -281,6 +325,8 @@ cudaError_t launch_group_norm(int dtype, const NormParams& p, cudaStream_t strea
 }
 
 cudaError_t launch_group_norm_backward(int dtype, const NormParams& p, cudaStream_t stream) {
+  if (norm_tokens_take(dtype, p, true)) return launch_norm_tokens(dtype, p, true, stream);
+  if (norm_images_take(dtype, p, true)) return launch_norm_images(dtype, p, true, stream);
   switch (dtype) {
     case FDNN_F16: return backward_t<__half>(p, stream);
     case FDNN_BF16: return backward_t<__nv_bfloat16>(p, stream);

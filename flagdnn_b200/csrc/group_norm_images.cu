@@ -1,0 +1,729 @@
+// Group norm over channels-last images, and over rows of tokens whose groups do not fit a warp.
+//
+// Bound by memory: x is read once and y written once, so a group's values have to stay on chip between the statistics and the
+// last pass. They stay in registers: a cluster of up to eight blocks holds all pixels of a slab of neighbouring groups (rows of
+// about 128 bytes), up to sixteen vectors of 16 bytes a thread, loaded at once. Mean first and deviations from it second, both
+// from registers; the blocks' means and squared deviations are joined over distributed shared memory. The gradient holds x and
+// dy the same way, sums g xh and g per channel, and joins those.
+//
+// Slabs that no cluster holds (a 16-bit group of more than half a million values) go in two launches, which read x twice.
+#include <cooperative_groups.h>
+
+#include "group_norm.cuh"
+
+namespace fdnn {
+namespace {
+
+namespace cg = cooperative_groups;
+
+constexpr int kMaxChunks = 64;        // pieces of an image in two launches
+constexpr int kMaxGroups = 512;       // of a slab
+
+struct Slab {
+  NormParams p;
+  int S;                 // pixels
+  int channels, cols;    // of a slab; vectors of channels in a row of it
+  int rows_at_once;      // rows that a block's threads cover
+  int rows;              // of a block (cluster) or a piece (two launches)
+  int slabs, cluster;
+  int slices;            // backward: clusters that share the images
+  int pieces;
+  float2* part;          // forward in two launches: [N, pieces, G] mean and squared deviations
+  float2* sums;          // backward: rows of [C] sums of g xh and g
+};
+
+// A thread's place: a vector of channels and every rows_at_once-th row.
+struct Place {
+  int col, r, cc;        // column, first row, first channel within the slab
+  int c0;                // the slab's first channel
+  int here;              // channels of this slab (the last may have fewer)
+  bool live;
+  __device__ Place(const Slab& s, int slab) {
+    col = threadIdx.x % s.cols;
+    r = threadIdx.x / s.cols;
+    cc = 0;
+    c0 = slab * s.channels;
+    here = min(s.channels, s.p.C - c0);
+    live = r < s.rows_at_once;
+  }
+  template <int V>
+  __device__ void at() {
+    cc = col * V;
+    live = live && cc < here;
+  }
+};
+
+// Sums of v[] over the block by group, into out[]. red: as many floats as threads times V.
+// ONE (everywhere): the channels of a vector are all of one group, whose values are then kept once.
+template <int V, bool ONE>
+__device__ __forceinline__ void sum_by_group(const Slab& s, const Place& at, const float (&v)[V], float* red, float* out) {
+  const int pitch = ONE ? s.cols : s.channels, per = s.p.C / s.p.G / (ONE ? V : 1);
+  if (at.r < s.rows_at_once) {
+    if constexpr (ONE) {
+      float t = 0.0f;
+#pragma unroll
+      for (int j = 0; j < V; ++j) t += v[j];
+      red[at.r * pitch + at.col] = t;
+    } else {
+#pragma unroll
+      for (int j = 0; j < V; ++j) red[at.r * pitch + at.cc + j] = v[j];
+    }
+  }
+  __syncthreads();
+  const int groups = at.here / (s.p.C / s.p.G), lane = threadIdx.x & 31, entries = s.rows_at_once * per;
+  const float inv = 1.0f / float(per);
+  for (int g = threadIdx.x >> 5; g < groups; g += blockDim.x >> 5) {
+    float t = 0.0f;
+    for (int i = lane; i < entries; i += 32) {
+      const int row = int((float(i) + 0.5f) * inv);   // i / per: exact for the few thousand entries there are
+      t += red[row * pitch + g * per + i - row * per];
+    }
+    t = warp_sum(t);
+    if (lane == 0) out[g] = t;
+  }
+  __syncthreads();
+}
+
+template <typename T, int V>
+__device__ __forceinline__ void channel_params(const NormParams& p, int c, bool live, float (&w)[V], float (&b)[V]) {
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    w[j] = live && p.weight != nullptr ? param<T>(p.weight, p.param_f32, c + j) : 1.0f;
+    b[j] = live && p.bias != nullptr ? param<T>(p.bias, p.param_f32, c + j) : 0.0f;
+  }
+}
+
+// Mean and squared deviations of a block's rows by group, from registers: mean[g] and m2[g] in shared memory.
+template <typename T, int V, bool ONE, int R>
+__device__ __forceinline__ void local_moments(const Slab& s, const Place& at, const Pack<T, V> (&x)[R], int rows, float* red,
+                                              float* mean, float* m2) {
+  const int cpg = s.p.C / s.p.G;
+  constexpr int M = ONE ? 1 : V;
+  float v[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) v[j] = 0.0f;
+#pragma unroll
+  for (int k = 0; k < R; ++k)
+#pragma unroll
+    for (int j = 0; j < V; ++j) v[j] += x[k].at(j);        // (rows that are not there hold zeros)
+  sum_by_group<V, ONE>(s, at, v, red, mean);
+  const float inv = 1.0f / (float(rows) * float(cpg));
+  float m[M];
+#pragma unroll
+  for (int j = 0; j < M; ++j) m[j] = at.live ? mean[(at.cc + j) / cpg] * inv : 0.0f;
+#pragma unroll
+  for (int j = 0; j < V; ++j) v[j] = 0.0f;
+#pragma unroll
+  for (int k = 0; k < R; ++k)
+    if (at.live && at.r + k * s.rows_at_once < rows) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const float d = x[k].at(j) - m[ONE ? 0 : j];
+        v[j] += d * d;
+      }
+    }
+  sum_by_group<V, ONE>(s, at, v, red, m2);
+  for (int g = threadIdx.x; g < at.here / cpg; g += blockDim.x) mean[g] *= inv;
+}
+
+template <typename T, int V, bool ONE, int R, int THREADS>
+__global__ void __launch_bounds__(THREADS, THREADS > 256 ? 1 : R > 8 ? 2 : 3)
+norm_images_kernel(const Slab s) {
+  __shared__ float red[THREADS * V];
+  __shared__ float mean[kMaxGroups], m2[kMaxGroups], mean_all[kMaxGroups], rstd_all[kMaxGroups];
+  constexpr int M = ONE ? 1 : V;
+  chained();
+  const NormParams& p = s.p;
+  const cg::cluster_group cluster = cg::this_cluster();
+  const int rank = blockIdx.x % s.cluster, job = blockIdx.x / s.cluster, slab = job % s.slabs, n = job / s.slabs;
+  const int row0 = rank * s.rows, rows = max(0, min(s.rows, s.S - row0)), cpg = p.C / p.G;
+  Place at(s, slab);
+  at.at<V>();
+  const long long pixel = p.W > 1 ? p.x_s[3] : p.x_s[2], out_pixel = p.W > 1 ? p.y_s[3] : p.y_s[2];
+  const T* x0 = static_cast<const T*>(p.x) + n * p.x_s[0] + at.c0 + at.cc + (long long)(row0 + at.r) * pixel;
+  Pack<T, V> x[R];
+#pragma unroll
+  for (int k = 0; k < R; ++k) {
+    x[k].clear();
+    if (at.live && at.r + k * s.rows_at_once < rows) x[k].load(x0 + k * s.rows_at_once * pixel);
+  }
+  local_moments<T, V, ONE>(s, at, x, rows, red, mean, m2);
+  if (s.cluster > 1) cluster.sync();
+  else __syncthreads();
+  const int g0 = at.c0 / cpg;
+  for (int g = threadIdx.x; g < at.here / cpg; g += THREADS) {
+    Moments all{0.0f, 0.0f, 0.0f};
+    for (int q = 0; q < s.cluster; ++q) {
+      const float count = float(max(0, min(s.rows, s.S - q * s.rows))) * float(cpg);
+      const float* mq = s.cluster > 1 ? cluster.map_shared_rank(mean, q) : mean;
+      const float* dq = s.cluster > 1 ? cluster.map_shared_rank(m2, q) : m2;
+      if (count > 0.0f) all = joined(all, Moments{count, mq[g], dq[g]});
+    }
+    const float rstd = rsqrtf(all.m2 / all.n + p.eps);
+    mean_all[g] = all.mean;
+    rstd_all[g] = rstd;
+    if (p.mean != nullptr && rank == 0) {
+      p.mean[(long long)n * p.G + g0 + g] = all.mean;
+      p.rstd[(long long)n * p.G + g0 + g] = rstd;
+    }
+  }
+  if (s.cluster > 1) cluster.barrier_arrive();   // this block has read the others' moments
+  __syncthreads();
+  float w[V], b[V], m[M];
+  channel_params<T, V>(p, at.c0 + at.cc, at.live, w, b);
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    const int g = at.live ? (at.cc + (ONE ? 0 : j)) / cpg : 0;
+    m[ONE ? 0 : j] = mean_all[g];
+    w[j] *= rstd_all[g];
+  }
+  T* y0 = static_cast<T*>(p.y) + n * p.y_s[0] + at.c0 + at.cc + (long long)(row0 + at.r) * out_pixel;
+  with_activation(p.act, [&](auto act) {
+#pragma unroll
+    for (int k = 0; k < R; ++k)
+      if (at.live && at.r + k * s.rows_at_once < rows) {
+        Pack<T, V> y;
+#pragma unroll
+        for (int j = 0; j < V; ++j) y.set(j, activate<decltype(act)::value>((x[k].at(j) - m[ONE ? 0 : j]) * w[j] + b[j]));
+        y.store(y0 + k * s.rows_at_once * out_pixel);
+      }
+  });
+  if (s.cluster > 1) cluster.barrier_wait();     // and the others have read this one's
+}
+
+// Sums over a block's rows of two values per channel: sums[channel of the slab]. red: twice as many floats as threads times V.
+template <int V>
+__device__ __forceinline__ void sum_by_channel(const Slab& s, const Place& at, const float (&a)[V], const float (&b)[V], float2* red,
+                                               float2* sums) {
+  if (at.r < s.rows_at_once) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) red[at.r * s.channels + at.cc + j] = make_float2(a[j], b[j]);
+  }
+  __syncthreads();
+  // the rows in as many parts as there are threads for; the first part's thread adds the parts in their order
+  const int parts = min(s.rows_at_once, max(1, int(blockDim.x) / s.channels));
+  for (int e = threadIdx.x; e < parts * s.channels; e += blockDim.x) {
+    const int part = e / s.channels, c = e - part * s.channels;
+    float2 t = red[part * s.channels + c];
+    for (int row = part + parts; row < s.rows_at_once; row += parts) {
+      const float2 q = red[row * s.channels + c];
+      t.x += q.x;
+      t.y += q.y;
+    }
+    red[part * s.channels + c] = t;
+  }
+  __syncthreads();
+  for (int c = threadIdx.x; c < s.channels; c += blockDim.x) {
+    float2 t = red[c];
+    for (int part = 1; part < parts; ++part) {
+      const float2 q = red[part * s.channels + c];
+      t.x += q.x;
+      t.y += q.y;
+    }
+    sums[c] = t;
+  }
+}
+
+// s1 / m and s2 / m of every group of the slab from its channels' sums.
+template <typename T>
+__device__ __forceinline__ void group_means(const Slab& s, int c0, int here, const float2* sums, float2* means) {
+  const NormParams& p = s.p;
+  const int cpg = p.C / p.G, lane = threadIdx.x & 31;
+  const float inv = 1.0f / (float(s.S) * float(cpg));
+  for (int g = threadIdx.x >> 5; g < here / cpg; g += blockDim.x >> 5) {
+    float s1 = 0.0f, s2 = 0.0f;
+    for (int c = g * cpg + lane; c < (g + 1) * cpg; c += 32) {
+      const float w = p.weight != nullptr ? param<T>(p.weight, p.param_f32, c0 + c) : 1.0f;
+      s2 += w * sums[c].x;
+      s1 += w * sums[c].y;
+    }
+    s1 = warp_sum(s1);
+    s2 = warp_sum(s2);
+    if (lane == 0) means[g] = make_float2(s1 * inv, s2 * inv);
+  }
+}
+
+// Shared memory of the backward kernels: a row of vectors bounds a slab's channels.
+struct BackwardShared {
+  float2 *red, *own, *all, *acc, *means;
+  __device__ BackwardShared(unsigned char* raw, int entries, int channels)
+      : red(reinterpret_cast<float2*>(raw)), own(red + entries), all(own + channels), acc(all + channels), means(acc + channels) {}
+  static int bytes(int entries, int channels) { return 8 * (entries + 3 * channels + kMaxGroups); }
+};
+
+template <typename T, int V, bool ONE, int R, int THREADS>
+__global__ void __launch_bounds__(THREADS, THREADS > 256 ? 1 : 2)
+norm_images_backward_kernel(const Slab s) {
+  extern __shared__ __align__(16) unsigned char raw[];
+  const BackwardShared sh(raw, THREADS * V, s.channels);
+  constexpr int M = ONE ? 1 : V;
+  chained();
+  const NormParams& p = s.p;
+  const cg::cluster_group cluster = cg::this_cluster();
+  const int rank = blockIdx.x % s.cluster, job = blockIdx.x / s.cluster, slab = job % s.slabs, slice = job / s.slabs;
+  const int row0 = rank * s.rows, rows = max(0, min(s.rows, s.S - row0)), cpg = p.C / p.G;
+  Place at(s, slab);
+  at.at<V>();
+  const bool tall = p.W > 1;
+  const long long px = tall ? p.x_s[3] : p.x_s[2], pdy = tall ? p.dy_s[3] : p.dy_s[2], pdx = tall ? p.dx_s[3] : p.dx_s[2];
+  const int c = at.c0 + at.cc, first = row0 + at.r;
+  float w[V], b[V];
+  channel_params<T, V>(p, c, at.live, w, b);
+  for (int i = threadIdx.x; i < s.channels; i += THREADS) sh.acc[i] = make_float2(0.0f, 0.0f);
+  for (int n = slice; n < p.N; n += s.slices) {
+    const T* x0 = static_cast<const T*>(p.x) + n * p.x_s[0] + c + first * px;
+    const T* dy0 = static_cast<const T*>(p.dy) + n * p.dy_s[0] + c + first * pdy;
+    Pack<T, V> x[R], dy[R];
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+      x[k].clear();
+      dy[k].clear();
+      if (at.live && at.r + k * s.rows_at_once < rows) {
+        x[k].load(x0 + k * s.rows_at_once * px);
+        dy[k].load(dy0 + k * s.rows_at_once * pdy);
+      }
+    }
+    float mean[M], rstd[M], gx[V], gs[V];
+#pragma unroll
+    for (int j = 0; j < M; ++j) {
+      const long long g = (long long)n * p.G + (at.live ? (c + j) / cpg : 0);
+      mean[j] = p.mean[g];
+      rstd[j] = p.rstd[g];
+    }
+#pragma unroll
+    for (int j = 0; j < V; ++j) gx[j] = gs[j] = 0.0f;
+    with_activation(p.act, [&](auto act) {
+#pragma unroll
+      for (int k = 0; k < R; ++k)
+        if (at.live && at.r + k * s.rows_at_once < rows) {
+#pragma unroll
+          for (int j = 0; j < V; ++j) {
+            const float xh = (x[k].at(j) - mean[ONE ? 0 : j]) * rstd[ONE ? 0 : j];
+            const float g = dy[k].at(j) * slope<decltype(act)::value>(xh * w[j] + b[j]);
+            gx[j] += g * xh;
+            gs[j] += g;
+          }
+        }
+    });
+    sum_by_channel<V>(s, at, gx, gs, sh.red, sh.own);
+    if (s.cluster > 1) cluster.sync();
+    else __syncthreads();
+    for (int i = threadIdx.x; i < s.channels; i += THREADS) {
+      float2 t = make_float2(0.0f, 0.0f);
+      for (int q = 0; q < s.cluster; ++q) {
+        const float2 v = (s.cluster > 1 ? cluster.map_shared_rank(sh.own, q) : sh.own)[i];
+        t.x += v.x;
+        t.y += v.y;
+      }
+      sh.all[i] = t;
+      sh.acc[i].x += t.x;
+      sh.acc[i].y += t.y;
+    }
+    if (s.cluster > 1) cluster.barrier_arrive();
+    __syncthreads();
+    group_means<T>(s, at.c0, at.here, sh.all, sh.means);
+    __syncthreads();
+    if (p.dx != nullptr) {
+      float s1[M], s2[M];
+#pragma unroll
+      for (int j = 0; j < M; ++j) {
+        const float2 m = sh.means[at.live ? (at.cc + j) / cpg : 0];
+        s1[j] = m.x;
+        s2[j] = m.y;
+      }
+      T* dx0 = static_cast<T*>(p.dx) + n * p.dx_s[0] + c + first * pdx;
+      with_activation(p.act, [&](auto act) {
+#pragma unroll
+        for (int k = 0; k < R; ++k)
+          if (at.live && at.r + k * s.rows_at_once < rows) {
+            Pack<T, V> dx;
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+              const float xh = (x[k].at(j) - mean[ONE ? 0 : j]) * rstd[ONE ? 0 : j];
+              const float g = dy[k].at(j) * slope<decltype(act)::value>(xh * w[j] + b[j]);
+              dx.set(j, rstd[ONE ? 0 : j] * (g * w[j] - s1[ONE ? 0 : j] - xh * s2[ONE ? 0 : j]));
+            }
+            dx.store(dx0 + k * s.rows_at_once * pdx);
+          }
+      });
+    }
+    if (s.cluster > 1) cluster.barrier_wait();   // before sh.own is written again, or the block ends
+  }
+  if (rank == 0)
+    for (int i = threadIdx.x; i < at.here; i += THREADS) s.sums[(long long)slice * p.C + at.c0 + i] = sh.acc[i];
+}
+
+// ---- in two launches: a block takes a piece of an image's pixels of a slab -----------------------------------------
+
+constexpr int kSplitThreads = 256, kSplitRows = 8;
+
+template <typename T, int V, bool ONE>
+__global__ void __launch_bounds__(kSplitThreads)
+norm_split_stats_kernel(const Slab s) {
+  __shared__ float red[kSplitThreads * V];
+  __shared__ float mean[kMaxGroups], m2[kMaxGroups];
+  __shared__ Moments all[kMaxGroups];
+  chained();
+  const NormParams& p = s.p;
+  const int piece = blockIdx.x % s.pieces, job = blockIdx.x / s.pieces, slab = job % s.slabs, n = job / s.slabs;
+  const int row0 = piece * s.rows, end = min(s.S, row0 + s.rows), cpg = p.C / p.G;
+  Place at(s, slab);
+  at.at<V>();
+  const long long pixel = p.W > 1 ? p.x_s[3] : p.x_s[2];
+  for (int g = threadIdx.x; g < at.here / cpg; g += kSplitThreads) all[g] = Moments{0.0f, 0.0f, 0.0f};
+  for (int r0 = row0; r0 < end; r0 += kSplitRows * s.rows_at_once) {
+    const int rows = min(end - r0, kSplitRows * s.rows_at_once);
+    const T* x0 = static_cast<const T*>(p.x) + n * p.x_s[0] + at.c0 + at.cc + (long long)(r0 + at.r) * pixel;
+    Pack<T, V> x[kSplitRows];
+#pragma unroll
+    for (int k = 0; k < kSplitRows; ++k) {
+      x[k].clear();
+      if (at.live && at.r + k * s.rows_at_once < rows) x[k].load(x0 + k * s.rows_at_once * pixel);
+    }
+    local_moments<T, V, ONE>(s, at, x, rows, red, mean, m2);
+    __syncthreads();
+    for (int g = threadIdx.x; g < at.here / cpg; g += kSplitThreads)
+      all[g] = joined(all[g], Moments{float(rows) * float(cpg), mean[g], m2[g]});
+    __syncthreads();
+  }
+  for (int g = threadIdx.x; g < at.here / cpg; g += kSplitThreads)
+    s.part[((long long)n * s.pieces + piece) * p.G + at.c0 / cpg + g] = make_float2(all[g].mean, all[g].m2);
+}
+
+template <typename T, int V, bool ONE>
+__global__ void __launch_bounds__(kSplitThreads)
+norm_split_apply_kernel(const Slab s) {
+  __shared__ float mean_all[kMaxGroups], rstd_all[kMaxGroups];
+  constexpr int M = ONE ? 1 : V;
+  chained();
+  const NormParams& p = s.p;
+  const int piece = blockIdx.x % s.pieces, job = blockIdx.x / s.pieces, slab = job % s.slabs, n = job / s.slabs;
+  const int row0 = piece * s.rows, end = min(s.S, row0 + s.rows), cpg = p.C / p.G;
+  Place at(s, slab);
+  at.at<V>();
+  const int g0 = at.c0 / cpg;
+  for (int g = threadIdx.x; g < at.here / cpg; g += kSplitThreads) {
+    Moments all{0.0f, 0.0f, 0.0f};
+    for (int q = 0; q < s.pieces; ++q) {
+      const float2 v = s.part[((long long)n * s.pieces + q) * p.G + g0 + g];
+      all = joined(all, Moments{float(min(s.S, (q + 1) * s.rows) - q * s.rows) * float(cpg), v.x, v.y});
+    }
+    const float rstd = rsqrtf(all.m2 / all.n + p.eps);
+    mean_all[g] = all.mean;
+    rstd_all[g] = rstd;
+    if (p.mean != nullptr && piece == 0) {
+      p.mean[(long long)n * p.G + g0 + g] = all.mean;
+      p.rstd[(long long)n * p.G + g0 + g] = rstd;
+    }
+  }
+  __syncthreads();
+  if (!at.live) return;
+  const long long px = p.W > 1 ? p.x_s[3] : p.x_s[2], py = p.W > 1 ? p.y_s[3] : p.y_s[2];
+  float w[V], b[V], m[M];
+  channel_params<T, V>(p, at.c0 + at.cc, true, w, b);
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    const int g = (at.cc + (ONE ? 0 : j)) / cpg;
+    m[ONE ? 0 : j] = mean_all[g];
+    w[j] *= rstd_all[g];
+  }
+  const T* x0 = static_cast<const T*>(p.x) + n * p.x_s[0] + at.c0 + at.cc;
+  T* y0 = static_cast<T*>(p.y) + n * p.y_s[0] + at.c0 + at.cc;
+  with_activation(p.act, [&](auto act) {
+#pragma unroll 4
+    for (long long row = row0 + at.r; row < end; row += s.rows_at_once) {
+      Pack<T, V> x, y;
+      x.load(x0 + row * px);
+#pragma unroll
+      for (int j = 0; j < V; ++j) y.set(j, activate<decltype(act)::value>((x.at(j) - m[ONE ? 0 : j]) * w[j] + b[j]));
+      y.store(y0 + row * py);
+    }
+  });
+}
+
+template <typename T, int V, bool ONE>
+__global__ void __launch_bounds__(kSplitThreads)
+norm_split_sums_kernel(const Slab s) {
+  extern __shared__ __align__(16) unsigned char raw[];
+  const BackwardShared sh(raw, kSplitThreads * V, s.channels);
+  constexpr int M = ONE ? 1 : V;
+  chained();
+  const NormParams& p = s.p;
+  const int piece = blockIdx.x % s.pieces, job = blockIdx.x / s.pieces, slab = job % s.slabs, n = job / s.slabs;
+  const int row0 = piece * s.rows, end = min(s.S, row0 + s.rows), cpg = p.C / p.G;
+  Place at(s, slab);
+  at.at<V>();
+  const long long px = p.W > 1 ? p.x_s[3] : p.x_s[2], pdy = p.W > 1 ? p.dy_s[3] : p.dy_s[2];
+  const int c = at.c0 + at.cc;
+  float w[V], b[V], mean[M], rstd[M], gx[V], gs[V];
+  channel_params<T, V>(p, c, at.live, w, b);
+#pragma unroll
+  for (int j = 0; j < M; ++j) {
+    const long long g = (long long)n * p.G + (at.live ? (c + j) / cpg : 0);
+    mean[j] = p.mean[g];
+    rstd[j] = p.rstd[g];
+  }
+#pragma unroll
+  for (int j = 0; j < V; ++j) gx[j] = gs[j] = 0.0f;
+  const T* x0 = static_cast<const T*>(p.x) + n * p.x_s[0] + c;
+  const T* dy0 = static_cast<const T*>(p.dy) + n * p.dy_s[0] + c;
+  if (at.live)
+    with_activation(p.act, [&](auto act) {
+#pragma unroll 4
+      for (long long row = row0 + at.r; row < end; row += s.rows_at_once) {
+        Pack<T, V> x, dy;
+        x.load(x0 + row * px);
+        dy.load(dy0 + row * pdy);
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          const float xh = (x.at(j) - mean[ONE ? 0 : j]) * rstd[ONE ? 0 : j];
+          const float g = dy.at(j) * slope<decltype(act)::value>(xh * w[j] + b[j]);
+          gx[j] += g * xh;
+          gs[j] += g;
+        }
+      }
+    });
+  sum_by_channel<V>(s, at, gx, gs, sh.red, sh.own);
+  __syncthreads();
+  for (int i = threadIdx.x; i < at.here; i += kSplitThreads) s.sums[((long long)n * s.pieces + piece) * p.C + at.c0 + i] = sh.own[i];
+}
+
+template <typename T, int V, bool ONE>
+__global__ void __launch_bounds__(kSplitThreads)
+norm_split_dx_kernel(const Slab s) {
+  extern __shared__ __align__(16) unsigned char raw[];
+  const BackwardShared sh(raw, kSplitThreads * V, s.channels);
+  constexpr int M = ONE ? 1 : V;
+  chained();
+  const NormParams& p = s.p;
+  const int piece = blockIdx.x % s.pieces, job = blockIdx.x / s.pieces, slab = job % s.slabs, n = job / s.slabs;
+  const int row0 = piece * s.rows, end = min(s.S, row0 + s.rows), cpg = p.C / p.G;
+  Place at(s, slab);
+  at.at<V>();
+  for (int i = threadIdx.x; i < at.here; i += kSplitThreads) {
+    float2 t = make_float2(0.0f, 0.0f);
+    for (int q = 0; q < s.pieces; ++q) {
+      const float2 v = s.sums[((long long)n * s.pieces + q) * p.C + at.c0 + i];
+      t.x += v.x;
+      t.y += v.y;
+    }
+    sh.all[i] = t;
+  }
+  __syncthreads();
+  group_means<T>(s, at.c0, at.here, sh.all, sh.means);
+  __syncthreads();
+  if (!at.live) return;
+  const bool tall = p.W > 1;
+  const long long px = tall ? p.x_s[3] : p.x_s[2], pdy = tall ? p.dy_s[3] : p.dy_s[2], pdx = tall ? p.dx_s[3] : p.dx_s[2];
+  const int c = at.c0 + at.cc;
+  float w[V], b[V], mean[M], rstd[M], s1[M], s2[M];
+  channel_params<T, V>(p, c, true, w, b);
+#pragma unroll
+  for (int j = 0; j < M; ++j) {
+    const long long g = (long long)n * p.G + (c + j) / cpg;
+    mean[j] = p.mean[g];
+    rstd[j] = p.rstd[g];
+    const float2 m = sh.means[(at.cc + j) / cpg];
+    s1[j] = m.x;
+    s2[j] = m.y;
+  }
+  const T* x0 = static_cast<const T*>(p.x) + n * p.x_s[0] + c;
+  const T* dy0 = static_cast<const T*>(p.dy) + n * p.dy_s[0] + c;
+  T* dx0 = static_cast<T*>(p.dx) + n * p.dx_s[0] + c;
+  with_activation(p.act, [&](auto act) {
+#pragma unroll 4
+    for (long long row = row0 + at.r; row < end; row += s.rows_at_once) {
+      Pack<T, V> x, dy, dx;
+      x.load(x0 + row * px);
+      dy.load(dy0 + row * pdy);
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const float xh = (x.at(j) - mean[ONE ? 0 : j]) * rstd[ONE ? 0 : j];
+        const float g = dy.at(j) * slope<decltype(act)::value>(xh * w[j] + b[j]);
+        dx.set(j, rstd[ONE ? 0 : j] * (g * w[j] - s1[ONE ? 0 : j] - xh * s2[ONE ? 0 : j]));
+      }
+      dx.store(dx0 + row * pdx);
+    }
+  });
+}
+
+// ---- which slab, how many blocks ------------------------------------------------------------------------------------
+
+struct ImagePlan {
+  Slab s;
+  int V, threads, R;     // R = 0: two launches
+};
+
+int gcd(int a, int b) { return b == 0 ? a : gcd(b, a % b); }
+
+// False: a row of the slab is wider than a block's threads.
+bool slab_of(ImagePlan* plan, const NormParams& p, int V, int threads, int channels) {
+  Slab& s = plan->s;
+  s.p = p;
+  s.S = p.H * p.W;
+  s.channels = channels;
+  s.cols = channels / V;
+  if (s.cols > threads || s.cols < 1) return false;
+  s.rows_at_once = threads / s.cols;
+  s.slabs = (p.C + channels - 1) / channels;
+  s.slices = s.pieces = 1;
+  s.cluster = 1;
+  s.part = nullptr;
+  s.sums = nullptr;
+  plan->V = V;
+  plan->threads = threads;
+  return channels / (p.C / p.G) <= kMaxGroups;
+}
+
+// The slab: whole groups and whole vectors, rows of about 128 bytes (8 vectors: narrower rows waste what a DRAM access brings,
+// wider ones leave too few blocks), narrower where that is what a cluster holds or too few blocks would run.
+// Then the fewest blocks to a cluster that hold it at eight vectors a thread (x and dy: four), sixteen and 512 threads last.
+bool image_plan(int dtype, const NormParams& p, bool backward, ImagePlan* plan) {
+  const int cpg = p.C / p.G;
+  int V = norm_vector(dtype, p, backward, p.C);
+  if (V == 0) return false;
+  if (V == 2 && cpg % 2 != 0) V = 1;
+  const long long S = (long long)p.H * p.W;
+  if (S > 0x3fffffff) return false;
+  const int unit = cpg / gcd(cpg, V) * V, units = p.C / unit;   // whole groups and whole vectors
+  const int sms = current_sm_count();
+  const int tops[2] = {backward ? 8 : 16, backward ? 8 : 16};
+  const long long wide = S < 32 ? 256 / S : 8;                  // (few pixels: wider rows, or threads have none)
+  int k = int(wide * V / unit);
+  if (k < 1) k = 1;
+  if (k > units) k = units;
+  const int widest = k;
+  for (;; k = (k + 1) / 2) {
+    for (int threads = 256; threads <= 512; threads *= 2) {
+      if (!slab_of(plan, p, V, threads, k * unit)) continue;
+      Slab& s = plan->s;
+      const long long at_once = s.rows_at_once;
+      if (8 * at_once * tops[threads > 256] < S) continue;
+      const int want = backward ? 4 : 8;
+      int cluster = 1;
+      while (cluster < 8 && cluster * at_once * want < S) cluster *= 2;
+      // few blocks: more to a cluster, as long as each has rows for its threads
+      while (cluster < 8 && (long long)p.N * s.slabs * cluster < sms && cluster * at_once * 2 <= S) cluster *= 2;
+      const long long need = (S + cluster * at_once - 1) / (cluster * at_once);
+      if (k > 1 && need > want && (long long)p.N * s.slabs < 4ll * sms) break;       // narrower first
+      if (k > 1 && (long long)p.N * s.slabs * cluster < sms && k * unit / V > 4) break;
+      plan->R = need <= 2 ? 2 : need <= 4 ? 4 : need <= 8 ? 8 : 16;
+      s.cluster = cluster;
+      s.rows = int((S + cluster - 1) / cluster);
+      const long long room = 4ll * sms / ((long long)s.slabs * cluster);
+      s.slices = int(p.N < room ? p.N : room < 1 ? 1 : room);
+      return true;
+    }
+    if (k == 1) break;
+  }
+  // no cluster holds a slab
+  for (k = widest; k >= 1; k /= 2)
+    if (slab_of(plan, p, V, kSplitThreads, k * unit)) break;
+  if (k < 1) return false;
+  Slab& s = plan->s;
+  plan->R = 0;
+  long long pieces = (S + 4ll * kSplitRows * s.rows_at_once - 1) / (4ll * kSplitRows * s.rows_at_once);
+  if (pieces > kMaxChunks) pieces = kMaxChunks;
+  s.rows = int((S + pieces - 1) / pieces);
+  s.pieces = int((S + s.rows - 1) / s.rows);
+  return true;
+}
+
+template <typename T, int V, bool ONE>
+cudaError_t forward(ImagePlan& plan, cudaStream_t stream) {
+  Slab& s = plan.s;
+  const NormParams& p = s.p;
+  if (plan.R == 0) {
+    const long long blocks = (long long)p.N * s.slabs * s.pieces;
+    if (blocks > 0x7fffffffll) return cudaErrorInvalidConfiguration;
+    s.part = static_cast<float2*>(p.workspace);
+    const cudaError_t e = launch_seq(norm_split_stats_kernel<T, V, ONE>, dim3(unsigned(blocks)), kSplitThreads, 0, 1, stream, s);
+    if (e != cudaSuccess) return e;
+    return launch_seq(norm_split_apply_kernel<T, V, ONE>, dim3(unsigned(blocks)), kSplitThreads, 0, 1, stream, s);
+  }
+  const long long blocks = (long long)p.N * s.slabs * s.cluster;
+  if (blocks > 0x7fffffffll) return cudaErrorInvalidConfiguration;
+  auto* kernel = plan.threads > 256 ? norm_images_kernel<T, V, ONE, 16, 512>
+                 : plan.R == 2      ? norm_images_kernel<T, V, ONE, 2, 256>
+                 : plan.R <= 8      ? norm_images_kernel<T, V, ONE, 8, 256>
+                                    : norm_images_kernel<T, V, ONE, 16, 256>;
+  return launch_seq(kernel, dim3(unsigned(blocks)), plan.threads, 0, s.cluster, stream, s);
+}
+
+template <typename T, int V, bool ONE, int R, int THREADS>
+cudaError_t run_backward(const Slab& s, long long blocks, cudaStream_t stream) {
+  static std::atomic<uint64_t> done;
+  auto* kernel = norm_images_backward_kernel<T, V, ONE, R, THREADS>;
+  const int smem = BackwardShared::bytes(THREADS * V, s.channels);
+  const cudaError_t e = allow_smem(kernel, BackwardShared::bytes(THREADS * V, THREADS * V), done);
+  if (e != cudaSuccess) return e;
+  return launch_seq(kernel, dim3(unsigned(blocks)), THREADS, smem, s.cluster, stream, s);
+}
+template <typename T, int V, bool ONE>
+cudaError_t run_split(const Slab& s, long long blocks, cudaStream_t stream) {
+  static std::atomic<uint64_t> sums_done, dx_done;
+  const int smem = BackwardShared::bytes(kSplitThreads * V, s.channels), most = BackwardShared::bytes(kSplitThreads * V, kSplitThreads * V);
+  cudaError_t e = allow_smem(norm_split_sums_kernel<T, V, ONE>, most, sums_done);
+  if (e == cudaSuccess) e = allow_smem(norm_split_dx_kernel<T, V, ONE>, most, dx_done);
+  if (e == cudaSuccess) e = launch_seq(norm_split_sums_kernel<T, V, ONE>, dim3(unsigned(blocks)), kSplitThreads, smem, 1, stream, s);
+  if (e == cudaSuccess && s.p.dx != nullptr)
+    e = launch_seq(norm_split_dx_kernel<T, V, ONE>, dim3(unsigned(blocks)), kSplitThreads, smem, 1, stream, s);
+  return e;
+}
+
+template <typename T, int V, bool ONE>
+cudaError_t backward(ImagePlan& plan, cudaStream_t stream) {
+  Slab& s = plan.s;
+  const NormParams& p = s.p;
+  s.sums = static_cast<float2*>(p.workspace);
+  cudaError_t e;
+  long long rows;
+  if (plan.R == 0) {
+    const long long blocks = (long long)p.N * s.slabs * s.pieces;
+    if (blocks > 0x7fffffffll) return cudaErrorInvalidConfiguration;
+    e = run_split<T, V, ONE>(s, blocks, stream);
+    rows = (long long)p.N * s.pieces;
+  } else {
+    const long long blocks = (long long)s.slices * s.slabs * s.cluster;
+    rows = s.slices;
+    e = plan.threads > 256 ? run_backward<T, V, ONE, 8, 512>(s, blocks, stream)
+        : plan.R <= 2      ? run_backward<T, V, ONE, 2, 256>(s, blocks, stream)
+        : plan.R == 4      ? run_backward<T, V, ONE, 4, 256>(s, blocks, stream)
+                           : run_backward<T, V, ONE, 8, 256>(s, blocks, stream);
+  }
+  if (e != cudaSuccess || (p.dweight == nullptr && p.dbias == nullptr)) return e;
+  return launch_norm_dparams<T>(p, s.sums, rows, stream);
+}
+
+}  // namespace
+
+bool norm_images_take(int dtype, const NormParams& p, bool backward) {
+  ImagePlan plan;
+  return image_plan(dtype, p, backward, &plan);
+}
+
+// Upper bounds for any alignment: slices of the images, or pieces of them.
+long long norm_images_workspace(int dtype, const NormParams& p, bool backward) {
+  (void)dtype;
+  const long long S = (long long)p.H * p.W, pieces = S < kMaxChunks ? S : kMaxChunks;
+  const long long slices = 4ll * current_sm_count() < p.N ? 4ll * current_sm_count() : p.N;
+  // two launches: only groups of more than 8 x 256 x 8 values (a cluster of blocks with narrow vectors), and wide ones
+  const bool split = S * (p.C / p.G) > 8 * 256 * 8 || p.C / p.G > 256;
+  const long long rows = split ? (p.N * pieces > slices ? p.N * pieces : slices) : slices;
+  return 8 * rows * (backward ? p.C : split ? p.G : 0);
+}
+
+cudaError_t launch_norm_images(int dtype, const NormParams& p, bool back, cudaStream_t stream) {
+  ImagePlan plan;
+  if (!image_plan(dtype, p, back, &plan)) return cudaErrorInvalidValue;
+  const bool one = p.C / p.G % plan.V == 0;
+  return norm_by_vector(dtype, plan.V, [&](auto type, auto v) {
+    using T = typename decltype(type)::type;
+    constexpr int V = decltype(v)::value;
+    if constexpr (V > 2)
+      if (!one) return back ? backward<T, V, false>(plan, stream) : forward<T, V, false>(plan, stream);
+    return back ? backward<T, V, true>(plan, stream) : forward<T, V, true>(plan, stream);
+  });
+}
+
+}  // namespace fdnn

@@ -1,0 +1,273 @@
+// Group norm over rows of tokens: x [N, C] with its channels together, statistics over the c = C / G values of a group of one row.
+//
+// Bound by memory.  A group is an even share of a warp (up to 32 lanes, up to kEach vectors of 16 bytes a lane), so that a
+// token's groups are reduced by shuffles alone; a lane keeps its channels' parameters and walks over tokens, the values of
+// the next ones on their way.  Mean first, then squared deviations from it, both from registers: x is read once.
+//
+// The gradient's row sums need nothing else.  dweight and dbias are sums over the rows: a lane adds up those of its channels in
+// fp32 over the tokens that it walks, each slice of the tokens leaves one row of [C] pairs, and a last launch adds the slices in
+// their order.
+#include "group_norm.cuh"
+
+namespace fdnn {
+namespace {
+
+constexpr int kThreads = 256, kWarps = kThreads / 32;
+
+struct TokenParams {
+  NormParams p;
+  int units, lanes;      // vectors of a group, lanes that share it (a power of two)
+  int slices;            // of the tokens
+  float2* rows;          // backward: [slices, C]
+};
+
+// Sum over the lanes of a group.
+__device__ __forceinline__ float lane_sum(float v, int lanes) {
+  for (int o = lanes >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// Where a thread works: its group and its vectors of it.
+template <int EACH>
+struct Seat {
+  int g, u0;
+  bool live;
+  __device__ Seat(const TokenParams& t) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, groups = 32 / t.lanes;
+    g = (blockIdx.x * kWarps + warp) * groups + lane / t.lanes;
+    u0 = lane % t.lanes;
+    live = g < t.p.G;
+    if (!live) g = 0;
+  }
+  __device__ bool in(const TokenParams& t, int e) const { return live && u0 + e * t.lanes < t.units; }
+};
+
+template <typename T, int V, int EACH, int TOKENS>
+__global__ void __launch_bounds__(kThreads)
+norm_tokens_kernel(const TokenParams t) {
+  chained();
+  const NormParams& p = t.p;
+  const Seat<EACH> seat(t);
+  const int cpg = p.C / p.G;
+  float w[EACH][V], b[EACH][V];
+  long long at[EACH];
+#pragma unroll
+  for (int e = 0; e < EACH; ++e) {
+    const int c = seat.g * cpg + (seat.u0 + e * t.lanes) * V;
+    at[e] = seat.in(t, e) ? c : 0;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      w[e][j] = seat.in(t, e) && p.weight != nullptr ? param<T>(p.weight, p.param_f32, c + j) : 1.0f;
+      b[e][j] = seat.in(t, e) && p.bias != nullptr ? param<T>(p.bias, p.param_f32, c + j) : 0.0f;
+    }
+  }
+  const float m = float(cpg);
+  with_activation(p.act, [&](auto act) {
+    for (long long n0 = (long long)blockIdx.y * TOKENS; n0 < p.N; n0 += (long long)gridDim.y * TOKENS) {
+      Pack<T, V> x[TOKENS][EACH];
+#pragma unroll
+      for (int k = 0; k < TOKENS; ++k) {
+        const long long n = n0 + k < p.N ? n0 + k : p.N - 1;
+#pragma unroll
+        for (int e = 0; e < EACH; ++e) {
+          x[k][e].clear();
+          if (seat.in(t, e)) x[k][e].load(static_cast<const T*>(p.x) + n * p.x_s[0] + at[e]);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < TOKENS; ++k) {
+        float sum = 0.0f;
+#pragma unroll
+        for (int e = 0; e < EACH; ++e)
+#pragma unroll
+          for (int j = 0; j < V; ++j) sum += x[k][e].at(j);
+        const float mean = lane_sum(sum, t.lanes) / m;
+        float m2 = 0.0f;
+#pragma unroll
+        for (int e = 0; e < EACH; ++e)
+#pragma unroll
+          for (int j = 0; j < V; ++j) {
+            const float d = x[k][e].at(j) - mean;
+            m2 += seat.in(t, e) ? d * d : 0.0f;
+          }
+        const float rstd = rsqrtf(lane_sum(m2, t.lanes) / m + p.eps);
+        if (n0 + k >= p.N) continue;
+        if (p.mean != nullptr && seat.live && seat.u0 == 0) {
+          p.mean[(n0 + k) * p.G + seat.g] = mean;
+          p.rstd[(n0 + k) * p.G + seat.g] = rstd;
+        }
+#pragma unroll
+        for (int e = 0; e < EACH; ++e) {
+          if (!seat.in(t, e)) continue;
+          Pack<T, V> y;
+#pragma unroll
+          for (int j = 0; j < V; ++j) y.set(j, activate<decltype(act)::value>((x[k][e].at(j) - mean) * (rstd * w[e][j]) + b[e][j]));
+          y.store(static_cast<T*>(p.y) + (n0 + k) * p.y_s[0] + at[e]);
+        }
+      }
+    }
+  });
+}
+
+template <typename T, int V, int EACH, int TOKENS>
+__global__ void __launch_bounds__(kThreads)
+norm_tokens_backward_kernel(const TokenParams t) {
+  chained();
+  const NormParams& p = t.p;
+  const Seat<EACH> seat(t);
+  const int cpg = p.C / p.G;
+  float w[EACH][V], b[EACH][V], dw[EACH][V], db[EACH][V];
+  long long at[EACH];
+#pragma unroll
+  for (int e = 0; e < EACH; ++e) {
+    const int c = seat.g * cpg + (seat.u0 + e * t.lanes) * V;
+    at[e] = seat.in(t, e) ? c : 0;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      w[e][j] = seat.in(t, e) && p.weight != nullptr ? param<T>(p.weight, p.param_f32, c + j) : 1.0f;
+      b[e][j] = seat.in(t, e) && p.bias != nullptr ? param<T>(p.bias, p.param_f32, c + j) : 0.0f;
+      dw[e][j] = db[e][j] = 0.0f;
+    }
+  }
+  const float inv = 1.0f / float(cpg);
+  with_activation(p.act, [&](auto act) {
+    for (long long n0 = (long long)blockIdx.y * TOKENS; n0 < p.N; n0 += (long long)gridDim.y * TOKENS) {
+      Pack<T, V> x[TOKENS][EACH], dy[TOKENS][EACH];
+      float mean[TOKENS], rstd[TOKENS];
+#pragma unroll
+      for (int k = 0; k < TOKENS; ++k) {
+        const bool there = n0 + k < p.N;
+        const long long n = there ? n0 + k : p.N - 1;
+        mean[k] = p.mean[n * p.G + seat.g];
+        rstd[k] = p.rstd[n * p.G + seat.g];
+#pragma unroll
+        for (int e = 0; e < EACH; ++e) {
+          x[k][e].clear();
+          dy[k][e].clear();
+          if (seat.in(t, e) && there) {
+            x[k][e].load(static_cast<const T*>(p.x) + n * p.x_s[0] + at[e]);
+            dy[k][e].load(static_cast<const T*>(p.dy) + n * p.dy_s[0] + at[e]);
+          }
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < TOKENS; ++k) {
+        const bool there = n0 + k < p.N;
+        float s1 = 0.0f, s2 = 0.0f, xh[EACH][V], g[EACH][V];
+#pragma unroll
+        for (int e = 0; e < EACH; ++e)
+#pragma unroll
+          for (int j = 0; j < V; ++j) {
+            const bool in = there && seat.in(t, e);
+            xh[e][j] = in ? (x[k][e].at(j) - mean[k]) * rstd[k] : 0.0f;
+            g[e][j] = in ? dy[k][e].at(j) * slope<decltype(act)::value>(xh[e][j] * w[e][j] + b[e][j]) : 0.0f;
+            dw[e][j] += g[e][j] * xh[e][j];
+            db[e][j] += g[e][j];
+            g[e][j] *= w[e][j];
+            s1 += g[e][j];
+            s2 += g[e][j] * xh[e][j];
+          }
+        s1 = lane_sum(s1, t.lanes) * inv;
+        s2 = lane_sum(s2, t.lanes) * inv;
+        if (!there || p.dx == nullptr) continue;
+#pragma unroll
+        for (int e = 0; e < EACH; ++e) {
+          if (!seat.in(t, e)) continue;
+          Pack<T, V> dx;
+#pragma unroll
+          for (int j = 0; j < V; ++j) dx.set(j, rstd[k] * (g[e][j] - s1 - xh[e][j] * s2));
+          dx.store(static_cast<T*>(p.dx) + (n0 + k) * p.dx_s[0] + at[e]);
+        }
+      }
+    }
+  });
+  // the block's part of a row of sums; every channel has one lane
+#pragma unroll
+  for (int e = 0; e < EACH; ++e)
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+      if (seat.in(t, e)) t.rows[(long long)blockIdx.y * p.C + at[e] + j] = make_float2(dw[e][j], db[e][j]);
+}
+
+// How a problem is cut; EACH vectors a lane, 0: a group is larger than a warp holds.
+struct TokenPlan {
+  TokenParams t;
+  int each, blocks;
+};
+TokenPlan plan_of(const NormParams& p, int V, int tokens, int per_sm) {
+  TokenPlan plan;
+  plan.t.p = p;
+  plan.t.units = p.C / p.G / V;
+  plan.t.lanes = 1;
+  while (plan.t.lanes < 32 && plan.t.lanes < plan.t.units) plan.t.lanes *= 2;
+  const int each = (plan.t.units + plan.t.lanes - 1) / plan.t.lanes;
+  plan.each = each <= 1 ? 1 : each <= 2 ? 2 : each <= 4 ? 4 : 0;
+  const int groups = kWarps * (32 / plan.t.lanes);
+  plan.blocks = (p.G + groups - 1) / groups;
+  // enough blocks for every SM; more tokens are walked
+  long long slices = (p.N + tokens - 1) / tokens, room = (long long)per_sm * current_sm_count() / plan.blocks;
+  if (room < 1) room = 1;
+  plan.t.slices = int(slices < room ? slices : room);
+  plan.t.rows = static_cast<float2*>(p.workspace);
+  return plan;
+}
+
+constexpr int kPerSm = 4;          // blocks of 256 threads an SM keeps at these registers
+int tokens_at_once(int each, bool backward) { return each == 1 ? (backward ? 2 : 4) : each == 2 ? (backward ? 1 : 2) : 1; }
+
+template <typename T, int V>
+cudaError_t forward(const NormParams& p, cudaStream_t stream) {
+  TokenPlan plan = plan_of(p, V, 1, 1);
+  plan = plan_of(p, V, tokens_at_once(plan.each, false), kPerSm);
+  const dim3 grid(unsigned(plan.blocks), unsigned(plan.t.slices));
+  switch (plan.each) {
+    case 1: return launch_seq(norm_tokens_kernel<T, V, 1, 4>, grid, kThreads, 0, 1, stream, plan.t);
+    case 2: return launch_seq(norm_tokens_kernel<T, V, 2, 2>, grid, kThreads, 0, 1, stream, plan.t);
+    default: return launch_seq(norm_tokens_kernel<T, V, 4, 1>, grid, kThreads, 0, 1, stream, plan.t);
+  }
+}
+
+template <typename T, int V>
+TokenPlan backward_plan(const NormParams& p) {
+  const TokenPlan plan = plan_of(p, V, 1, 1);
+  return plan_of(p, V, tokens_at_once(plan.each, true), kPerSm);
+}
+
+template <typename T, int V>
+cudaError_t backward(const NormParams& p, cudaStream_t stream) {
+  const TokenPlan plan = backward_plan<T, V>(p);
+  const dim3 grid(unsigned(plan.blocks), unsigned(plan.t.slices));
+  cudaError_t e;
+  switch (plan.each) {
+    case 1: e = launch_seq(norm_tokens_backward_kernel<T, V, 1, 2>, grid, kThreads, 0, 1, stream, plan.t); break;
+    case 2: e = launch_seq(norm_tokens_backward_kernel<T, V, 2, 1>, grid, kThreads, 0, 1, stream, plan.t); break;
+    default: e = launch_seq(norm_tokens_backward_kernel<T, V, 4, 1>, grid, kThreads, 0, 1, stream, plan.t); break;
+  }
+  if (e != cudaSuccess || (p.dweight == nullptr && p.dbias == nullptr)) return e;
+  return launch_norm_dparams<T>(p, plan.t.rows, plan.t.slices, stream);
+}
+
+}  // namespace
+
+// Rows of tokens whose groups fit a warp.
+bool norm_tokens_take(int dtype, const NormParams& p, bool backward) {
+  const int V = norm_vector(dtype, p, backward, p.C / p.G);
+  return V > 0 && p.H == 1 && p.W == 1 && p.C / p.G <= 128 * V;
+}
+
+long long norm_tokens_workspace(int dtype, const NormParams& p, bool backward) {
+  (void)dtype;
+  if (!backward) return 0;
+  // (an upper bound that does not depend on the tensors' alignment)
+  const long long slices = p.N < 65535 ? p.N : 65535, room = (long long)kPerSm * current_sm_count();
+  return 8ll * p.C * (slices < room ? slices : room);
+}
+
+cudaError_t launch_norm_tokens(int dtype, const NormParams& p, bool back, cudaStream_t stream) {
+  return norm_by_vector(dtype, norm_vector(dtype, p, back, p.C / p.G), [&](auto type, auto v) {
+    using T = typename decltype(type)::type;
+    return back ? backward<T, decltype(v)::value>(p, stream) : forward<T, decltype(v)::value>(p, stream);
+  });
+}
+
+}  // namespace fdnn
