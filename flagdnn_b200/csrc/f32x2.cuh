@@ -1,4 +1,4 @@
-// Pairs of fp32 values in one 64-bit register (fma.rn.f32x2), shared by the depthwise and scan kernels.
+// Pairs of fp32 values in one 64-bit register (fma.rn.f32x2), shared by the depthwise, scan and norm kernels.
 #pragma once
 #include <stdint.h>
 
@@ -26,7 +26,18 @@ __device__ __forceinline__ F2 f2_mul(F2 a, F2 b) {
   asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
   return d;
 }
+__device__ __forceinline__ F2 f2_add(F2 a, F2 b) {
+  F2 d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
 __device__ __forceinline__ F2 f2_pack(float lo, float hi) {
   return f2_make(__float_as_uint(lo), __float_as_uint(hi));
+}
+__device__ __forceinline__ F2 f2_both(float v) { return f2_pack(v, v); }
+__device__ __forceinline__ float f2_sum(F2 v) {
+  float lo, hi;
+  f2_split(v, lo, hi);
+  return lo + hi;
 }
 }  // namespace fdnn

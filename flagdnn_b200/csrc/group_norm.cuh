@@ -17,7 +17,52 @@ struct Pack {
   __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<Word*>(p) = q; }
   __device__ __forceinline__ float at(int j) const { return to_f32<T>(reinterpret_cast<const T*>(&q)[j]); }
   __device__ __forceinline__ void set(int j, float v) { reinterpret_cast<T*>(&q)[j] = from_f32<T>(v); }
+  // Values 2 i and 2 i + 1 as fp32 (of a single value: it and zero).
+  static constexpr int kPairs = (V + 1) / 2;
+  __device__ __forceinline__ F2 pair(int i) const {
+    if constexpr (V == 1) {
+      return f2_pack(at(0), 0.0f);
+    } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+      const uint32_t w = reinterpret_cast<const uint32_t*>(&q)[i];
+      return f2_make(w << 16, w & 0xffff0000u);
+    } else {
+      return f2_pack(at(2 * i), at(2 * i + 1));
+    }
+  }
+  __device__ __forceinline__ void set_pair(int i, F2 v) {
+    float lo, hi;
+    f2_split(v, lo, hi);
+    if constexpr (V == 1) {
+      set(0, lo);
+    } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+      const __nv_bfloat162 b = __floats2bfloat162_rn(lo, hi);
+      reinterpret_cast<uint32_t*>(&q)[i] = *reinterpret_cast<const uint32_t*>(&b);
+    } else if constexpr (std::is_same<T, __half>::value) {
+      const __half2 b = __floats2half2_rn(lo, hi);
+      reinterpret_cast<uint32_t*>(&q)[i] = *reinterpret_cast<const uint32_t*>(&b);
+    } else {
+      set(2 * i, lo);
+      set(2 * i + 1, hi);
+    }
+  }
 };
+
+// A thread's parameters as pairs.
+template <typename T, int V>
+__device__ __forceinline__ void norm_params_of(const NormParams& p, int c, bool live, F2 (&w)[Pack<T, V>::kPairs], F2 (&b)[Pack<T, V>::kPairs]) {
+#pragma unroll
+  for (int i = 0; i < Pack<T, V>::kPairs; ++i) {
+    float wv[2], bv[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const bool in = live && 2 * i + j < V;
+      wv[j] = in && p.weight != nullptr ? param<T>(p.weight, p.param_f32, c + 2 * i + j) : 1.0f;
+      bv[j] = in && p.bias != nullptr ? param<T>(p.bias, p.param_f32, c + 2 * i + j) : 0.0f;
+    }
+    w[i] = f2_pack(wv[0], wv[1]);
+    b[i] = f2_pack(bv[0], bv[1]);
+  }
+}
 
 // Whether the channels lie together and the pixels at one stride, in x and in what goes with it.
 inline bool norm_rows(const NormParams& p, bool backward) {

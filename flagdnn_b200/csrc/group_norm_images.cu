@@ -53,85 +53,89 @@ struct Place {
   }
 };
 
-// Sums of v[] over the block by group, into out[]. red: as many floats as threads times V.
-// ONE (everywhere): the channels of a vector are all of one group, whose values are then kept once.
-template <int V, bool ONE>
-__device__ __forceinline__ void sum_by_group(const Slab& s, const Place& at, const float (&v)[V], float* red, float* out) {
-  const int pitch = ONE ? s.cols : s.channels, per = s.p.C / s.p.G / (ONE ? V : 1);
-  if (at.r < s.rows_at_once) {
-    if constexpr (ONE) {
-      float t = 0.0f;
-#pragma unroll
-      for (int j = 0; j < V; ++j) t += v[j];
-      red[at.r * pitch + at.col] = t;
-    } else {
-#pragma unroll
-      for (int j = 0; j < V; ++j) red[at.r * pitch + at.cc + j] = v[j];
-    }
-  }
-  __syncthreads();
-  const int groups = at.here / (s.p.C / s.p.G), lane = threadIdx.x & 31, entries = s.rows_at_once * per;
-  const float inv = 1.0f / float(per);
-  for (int g = threadIdx.x >> 5; g < groups; g += blockDim.x >> 5) {
-    float t = 0.0f;
-    for (int i = lane; i < entries; i += 32) {
-      const int row = int((float(i) + 0.5f) * inv);   // i / per: exact for the few thousand entries there are
-      t += red[row * pitch + g * per + i - row * per];
-    }
-    t = warp_sum(t);
-    if (lane == 0) out[g] = t;
-  }
-  __syncthreads();
-}
+// Rows of a block's threads that its r-th row of threads has.
+__device__ __forceinline__ int rows_of(const Slab& s, int r, int rows) { return r < rows ? (rows - r - 1) / s.rows_at_once + 1 : 0; }
 
-template <typename T, int V>
-__device__ __forceinline__ void channel_params(const NormParams& p, int c, bool live, float (&w)[V], float (&b)[V]) {
-#pragma unroll
-  for (int j = 0; j < V; ++j) {
-    w[j] = live && p.weight != nullptr ? param<T>(p.weight, p.param_f32, c + j) : 1.0f;
-    b[j] = live && p.bias != nullptr ? param<T>(p.bias, p.param_f32, c + j) : 0.0f;
-  }
-}
-
-// Mean and squared deviations of a block's rows by group, from registers: mean[g] and m2[g] in shared memory.
+// Mean and squared deviations of a block's rows by group, from registers: out[g] in shared memory.
+// A thread sums its values' distances from its own first one, and their squares, channel by channel: one pass, and what
+// the squares lose to a first value far from the others is less than 2^-24 of that value's own share of the group's squared
+// deviations, times the thread's rows. Threads and channels are joined by their means.  ONE (everywhere): the channels of a
+// vector are all of one group.
 template <typename T, int V, bool ONE, int R>
-__device__ __forceinline__ void local_moments(const Slab& s, const Place& at, const Pack<T, V> (&x)[R], int rows, float* red,
-                                              float* mean, float* m2) {
-  const int cpg = s.p.C / s.p.G;
-  constexpr int M = ONE ? 1 : V;
-  float v[V];
+__device__ __forceinline__ void local_moments(const Slab& s, const Place& at, const Pack<T, V> (&x)[R], int rows, float2* red,
+                                              float2* out) {
+  const int cpg = s.p.C / s.p.G, count = at.live ? rows_of(s, at.r, rows) : 0;
+  constexpr int P = Pack<T, V>::kPairs;
+  F2 sum[P], square[P];
 #pragma unroll
-  for (int j = 0; j < V; ++j) v[j] = 0.0f;
+  for (int i = 0; i < P; ++i) sum[i] = square[i] = 0;
 #pragma unroll
-  for (int k = 0; k < R; ++k)
+  for (int k = 1; k < R; ++k)
+    if (k < count) {
 #pragma unroll
-    for (int j = 0; j < V; ++j) v[j] += x[k].at(j);        // (rows that are not there hold zeros)
-  sum_by_group<V, ONE>(s, at, v, red, mean);
-  const float inv = 1.0f / (float(rows) * float(cpg));
-  float m[M];
-#pragma unroll
-  for (int j = 0; j < M; ++j) m[j] = at.live ? mean[(at.cc + j) / cpg] * inv : 0.0f;
-#pragma unroll
-  for (int j = 0; j < V; ++j) v[j] = 0.0f;
-#pragma unroll
-  for (int k = 0; k < R; ++k)
-    if (at.live && at.r + k * s.rows_at_once < rows) {
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const float d = x[k].at(j) - m[ONE ? 0 : j];
-        v[j] += d * d;
+      for (int i = 0; i < P; ++i) {
+        const F2 d = f2_fma(x[0].pair(i), f2_both(-1.0f), x[k].pair(i));
+        sum[i] = f2_add(sum[i], d);
+        square[i] = f2_fma(d, d, square[i]);
       }
     }
-  sum_by_group<V, ONE>(s, at, v, red, m2);
-  for (int g = threadIdx.x; g < at.here / cpg; g += blockDim.x) mean[g] *= inv;
+  if (at.r < s.rows_at_once) {
+    const float inv = count > 0 ? 1.0f / float(count) : 0.0f;
+    float mean[2 * P], m2[2 * P];
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      float a[2], q[2], first[2];
+      f2_split(sum[i], a[0], a[1]);
+      f2_split(square[i], q[0], q[1]);
+      f2_split(x[0].pair(i), first[0], first[1]);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        mean[2 * i + j] = first[j] + a[j] * inv;
+        m2[2 * i + j] = fmaxf(q[j] - a[j] * a[j] * inv, q[j] * 0.0f);   // (rounding may leave less than nothing; NaN stays)
+      }
+    }
+    if constexpr (ONE) {
+      float all = 0.0f, dev = 0.0f;
+#pragma unroll
+      for (int j = 0; j < V; ++j) all += mean[j];
+      all *= 1.0f / V;
+#pragma unroll
+      for (int j = 0; j < V; ++j) dev += m2[j] + float(count) * (mean[j] - all) * (mean[j] - all);
+      red[at.r * s.cols + at.col] = make_float2(all, dev);
+    } else {
+#pragma unroll
+      for (int j = 0; j < V; ++j) red[at.r * s.channels + at.cc + j] = make_float2(mean[j], m2[j]);
+    }
+  }
+  __syncthreads();
+  const int pitch = ONE ? s.cols : s.channels, per = cpg / (ONE ? V : 1), groups = at.here / cpg, lane = threadIdx.x & 31;
+  const int entries = s.rows_at_once * per;
+  const float part = 1.0f / float(per);
+  for (int g = threadIdx.x >> 5; g < groups; g += blockDim.x >> 5) {
+    Moments all{0.0f, 0.0f, 0.0f};
+    for (int i = lane; i < entries; i += 32) {
+      const int row = int((float(i) + 0.5f) * part);   // i / per: exact for the few thousand entries there are
+      const float n = float(rows_of(s, row, rows) * (ONE ? V : 1));
+      const float2 v = red[row * pitch + g * per + i - row * per];
+      if (n > 0.0f) all = joined(all, Moments{n, v.x, v.y});
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      const Moments other{__shfl_down_sync(0xffffffffu, all.n, o), __shfl_down_sync(0xffffffffu, all.mean, o),
+                          __shfl_down_sync(0xffffffffu, all.m2, o)};
+      if (other.n > 0.0f) all = joined(all, other);
+    }
+    if (lane == 0) out[g] = make_float2(all.mean, all.m2);
+  }
+  __syncthreads();
 }
 
 template <typename T, int V, bool ONE, int R, int THREADS>
 __global__ void __launch_bounds__(THREADS, THREADS > 256 ? 1 : R > 8 ? 2 : 3)
 norm_images_kernel(const Slab s) {
-  __shared__ float red[THREADS * V];
-  __shared__ float mean[kMaxGroups], m2[kMaxGroups], mean_all[kMaxGroups], rstd_all[kMaxGroups];
-  constexpr int M = ONE ? 1 : V;
+  __shared__ float2 red[ONE ? THREADS : THREADS * V];
+  __shared__ float2 own[kMaxGroups], all_of[kMaxGroups];   // mean and squared deviations; mean and 1 / deviation
+  constexpr int M = ONE ? 1 : Pack<T, V>::kPairs;
   chained();
   const NormParams& p = s.p;
   const cg::cluster_group cluster = cg::this_cluster();
@@ -147,21 +151,18 @@ norm_images_kernel(const Slab s) {
     x[k].clear();
     if (at.live && at.r + k * s.rows_at_once < rows) x[k].load(x0 + k * s.rows_at_once * pixel);
   }
-  local_moments<T, V, ONE>(s, at, x, rows, red, mean, m2);
+  local_moments<T, V, ONE>(s, at, x, rows, red, own);
   if (s.cluster > 1) cluster.sync();
-  else __syncthreads();
   const int g0 = at.c0 / cpg;
   for (int g = threadIdx.x; g < at.here / cpg; g += THREADS) {
     Moments all{0.0f, 0.0f, 0.0f};
     for (int q = 0; q < s.cluster; ++q) {
       const float count = float(max(0, min(s.rows, s.S - q * s.rows))) * float(cpg);
-      const float* mq = s.cluster > 1 ? cluster.map_shared_rank(mean, q) : mean;
-      const float* dq = s.cluster > 1 ? cluster.map_shared_rank(m2, q) : m2;
-      if (count > 0.0f) all = joined(all, Moments{count, mq[g], dq[g]});
+      const float2 v = (s.cluster > 1 ? cluster.map_shared_rank(own, q) : own)[g];
+      if (count > 0.0f) all = joined(all, Moments{count, v.x, v.y});
     }
     const float rstd = rsqrtf(all.m2 / all.n + p.eps);
-    mean_all[g] = all.mean;
-    rstd_all[g] = rstd;
+    all_of[g] = make_float2(all.mean, rstd);
     if (p.mean != nullptr && rank == 0) {
       p.mean[(long long)n * p.G + g0 + g] = all.mean;
       p.rstd[(long long)n * p.G + g0 + g] = rstd;
@@ -169,13 +170,15 @@ norm_images_kernel(const Slab s) {
   }
   if (s.cluster > 1) cluster.barrier_arrive();   // this block has read the others' moments
   __syncthreads();
-  float w[V], b[V], m[M];
-  channel_params<T, V>(p, at.c0 + at.cc, at.live, w, b);
+  constexpr int P = Pack<T, V>::kPairs;
+  F2 w[P], b[P], m[M];                              // m: minus the mean
+  norm_params_of<T, V>(p, at.c0 + at.cc, at.live, w, b);
 #pragma unroll
-  for (int j = 0; j < V; ++j) {
-    const int g = at.live ? (at.cc + (ONE ? 0 : j)) / cpg : 0;
-    m[ONE ? 0 : j] = mean_all[g];
-    w[j] *= rstd_all[g];
+  for (int i = 0; i < P; ++i) {
+    const float2 lo = all_of[at.live ? (at.cc + (ONE ? 0 : 2 * i)) / cpg : 0];
+    const float2 hi = ONE ? lo : all_of[at.live ? (at.cc + min(2 * i + 1, V - 1)) / cpg : 0];
+    m[ONE ? 0 : i] = f2_pack(-lo.x, -hi.x);
+    w[i] = f2_mul(w[i], f2_pack(lo.y, hi.y));
   }
   T* y0 = static_cast<T*>(p.y) + n * p.y_s[0] + at.c0 + at.cc + (long long)(row0 + at.r) * out_pixel;
   with_activation(p.act, [&](auto act) {
@@ -184,7 +187,7 @@ norm_images_kernel(const Slab s) {
       if (at.live && at.r + k * s.rows_at_once < rows) {
         Pack<T, V> y;
 #pragma unroll
-        for (int j = 0; j < V; ++j) y.set(j, activate<decltype(act)::value>((x[k].at(j) - m[ONE ? 0 : j]) * w[j] + b[j]));
+        for (int i = 0; i < P; ++i) y.set_pair(i, activate2<decltype(act)::value>(f2_fma(f2_add(x[k].pair(i), m[ONE ? 0 : i]), w[i], b[i])));
         y.store(y0 + k * s.rows_at_once * out_pixel);
       }
   });
@@ -193,11 +196,17 @@ norm_images_kernel(const Slab s) {
 
 // Sums over a block's rows of two values per channel: sums[channel of the slab]. red: twice as many floats as threads times V.
 template <int V>
-__device__ __forceinline__ void sum_by_channel(const Slab& s, const Place& at, const float (&a)[V], const float (&b)[V], float2* red,
-                                               float2* sums) {
+__device__ __forceinline__ void sum_by_channel(const Slab& s, const Place& at, const F2 (&a)[(V + 1) / 2], const F2 (&b)[(V + 1) / 2],
+                                               float2* red, float2* sums) {
   if (at.r < s.rows_at_once) {
 #pragma unroll
-    for (int j = 0; j < V; ++j) red[at.r * s.channels + at.cc + j] = make_float2(a[j], b[j]);
+    for (int i = 0; i < (V + 1) / 2; ++i) {
+      float x0, x1, y0, y1;
+      f2_split(a[i], x0, x1);
+      f2_split(b[i], y0, y1);
+      red[at.r * s.channels + at.cc + 2 * i] = make_float2(x0, y0);
+      if (V > 1) red[at.r * s.channels + at.cc + 2 * i + 1] = make_float2(x1, y1);
+    }
   }
   __syncthreads();
   // the rows in as many parts as there are threads for; the first part's thread adds the parts in their order
@@ -256,7 +265,7 @@ __global__ void __launch_bounds__(THREADS, THREADS > 256 ? 1 : 2)
 norm_images_backward_kernel(const Slab s) {
   extern __shared__ __align__(16) unsigned char raw[];
   const BackwardShared sh(raw, THREADS * V, s.channels);
-  constexpr int M = ONE ? 1 : V;
+  constexpr int M = ONE ? 1 : Pack<T, V>::kPairs;
   chained();
   const NormParams& p = s.p;
   const cg::cluster_group cluster = cg::this_cluster();
@@ -267,8 +276,9 @@ norm_images_backward_kernel(const Slab s) {
   const bool tall = p.W > 1;
   const long long px = tall ? p.x_s[3] : p.x_s[2], pdy = tall ? p.dy_s[3] : p.dy_s[2], pdx = tall ? p.dx_s[3] : p.dx_s[2];
   const int c = at.c0 + at.cc, first = row0 + at.r;
-  float w[V], b[V];
-  channel_params<T, V>(p, c, at.live, w, b);
+  constexpr int P = Pack<T, V>::kPairs;
+  F2 w[P], b[P];
+  norm_params_of<T, V>(p, c, at.live, w, b);
   for (int i = threadIdx.x; i < s.channels; i += THREADS) sh.acc[i] = make_float2(0.0f, 0.0f);
   for (int n = slice; n < p.N; n += s.slices) {
     const T* x0 = static_cast<const T*>(p.x) + n * p.x_s[0] + c + first * px;
@@ -283,25 +293,26 @@ norm_images_backward_kernel(const Slab s) {
         dy[k].load(dy0 + k * s.rows_at_once * pdy);
       }
     }
-    float mean[M], rstd[M], gx[V], gs[V];
+    F2 mean[M], rstd[M], gx[P], gs[P];               // mean: minus the mean
 #pragma unroll
-    for (int j = 0; j < M; ++j) {
-      const long long g = (long long)n * p.G + (at.live ? (c + j) / cpg : 0);
-      mean[j] = p.mean[g];
-      rstd[j] = p.rstd[g];
+    for (int i = 0; i < M; ++i) {
+      const long long lo = (long long)n * p.G + (at.live ? (c + 2 * i) / cpg : 0);
+      const long long hi = ONE ? lo : (long long)n * p.G + (at.live ? (c + min(2 * i + 1, V - 1)) / cpg : 0);
+      mean[i] = f2_pack(-p.mean[lo], -p.mean[hi]);
+      rstd[i] = f2_pack(p.rstd[lo], p.rstd[hi]);
     }
 #pragma unroll
-    for (int j = 0; j < V; ++j) gx[j] = gs[j] = 0.0f;
+    for (int i = 0; i < P; ++i) gx[i] = gs[i] = 0;
     with_activation(p.act, [&](auto act) {
 #pragma unroll
       for (int k = 0; k < R; ++k)
         if (at.live && at.r + k * s.rows_at_once < rows) {
 #pragma unroll
-          for (int j = 0; j < V; ++j) {
-            const float xh = (x[k].at(j) - mean[ONE ? 0 : j]) * rstd[ONE ? 0 : j];
-            const float g = dy[k].at(j) * slope<decltype(act)::value>(xh * w[j] + b[j]);
-            gx[j] += g * xh;
-            gs[j] += g;
+          for (int i = 0; i < P; ++i) {
+            const F2 xh = f2_mul(f2_add(x[k].pair(i), mean[ONE ? 0 : i]), rstd[ONE ? 0 : i]);
+            const F2 g = f2_mul(dy[k].pair(i), slope2<decltype(act)::value>(f2_fma(xh, w[i], b[i])));
+            gx[i] = f2_fma(g, xh, gx[i]);
+            gs[i] = f2_add(gs[i], g);
           }
         }
     });
@@ -324,12 +335,13 @@ norm_images_backward_kernel(const Slab s) {
     group_means<T>(s, at.c0, at.here, sh.all, sh.means);
     __syncthreads();
     if (p.dx != nullptr) {
-      float s1[M], s2[M];
+      F2 s1[M], s2[M];                               // minus s1 / m, minus s2 / m
 #pragma unroll
-      for (int j = 0; j < M; ++j) {
-        const float2 m = sh.means[at.live ? (at.cc + j) / cpg : 0];
-        s1[j] = m.x;
-        s2[j] = m.y;
+      for (int i = 0; i < M; ++i) {
+        const float2 lo = sh.means[at.live ? (at.cc + 2 * i) / cpg : 0];
+        const float2 hi = ONE ? lo : sh.means[at.live ? (at.cc + min(2 * i + 1, V - 1)) / cpg : 0];
+        s1[i] = f2_pack(-lo.x, -hi.x);
+        s2[i] = f2_pack(-lo.y, -hi.y);
       }
       T* dx0 = static_cast<T*>(p.dx) + n * p.dx_s[0] + c + first * pdx;
       with_activation(p.act, [&](auto act) {
@@ -338,10 +350,10 @@ norm_images_backward_kernel(const Slab s) {
           if (at.live && at.r + k * s.rows_at_once < rows) {
             Pack<T, V> dx;
 #pragma unroll
-            for (int j = 0; j < V; ++j) {
-              const float xh = (x[k].at(j) - mean[ONE ? 0 : j]) * rstd[ONE ? 0 : j];
-              const float g = dy[k].at(j) * slope<decltype(act)::value>(xh * w[j] + b[j]);
-              dx.set(j, rstd[ONE ? 0 : j] * (g * w[j] - s1[ONE ? 0 : j] - xh * s2[ONE ? 0 : j]));
+            for (int i = 0; i < P; ++i) {
+              const F2 xh = f2_mul(f2_add(x[k].pair(i), mean[ONE ? 0 : i]), rstd[ONE ? 0 : i]);
+              const F2 g = f2_mul(dy[k].pair(i), slope2<decltype(act)::value>(f2_fma(xh, w[i], b[i])));
+              dx.set_pair(i, f2_mul(rstd[ONE ? 0 : i], f2_fma(xh, s2[ONE ? 0 : i], f2_fma(g, w[i], s1[ONE ? 0 : i]))));
             }
             dx.store(dx0 + k * s.rows_at_once * pdx);
           }
@@ -360,8 +372,8 @@ constexpr int kSplitThreads = 256, kSplitRows = 8;
 template <typename T, int V, bool ONE>
 __global__ void __launch_bounds__(kSplitThreads)
 norm_split_stats_kernel(const Slab s) {
-  __shared__ float red[kSplitThreads * V];
-  __shared__ float mean[kMaxGroups], m2[kMaxGroups];
+  __shared__ float2 red[ONE ? kSplitThreads : kSplitThreads * V];
+  __shared__ float2 own[kMaxGroups];
   __shared__ Moments all[kMaxGroups];
   chained();
   const NormParams& p = s.p;
@@ -380,10 +392,9 @@ norm_split_stats_kernel(const Slab s) {
       x[k].clear();
       if (at.live && at.r + k * s.rows_at_once < rows) x[k].load(x0 + k * s.rows_at_once * pixel);
     }
-    local_moments<T, V, ONE>(s, at, x, rows, red, mean, m2);
-    __syncthreads();
+    local_moments<T, V, ONE>(s, at, x, rows, red, own);
     for (int g = threadIdx.x; g < at.here / cpg; g += kSplitThreads)
-      all[g] = joined(all[g], Moments{float(rows) * float(cpg), mean[g], m2[g]});
+      all[g] = joined(all[g], Moments{float(rows) * float(cpg), own[g].x, own[g].y});
     __syncthreads();
   }
   for (int g = threadIdx.x; g < at.here / cpg; g += kSplitThreads)
@@ -393,8 +404,8 @@ norm_split_stats_kernel(const Slab s) {
 template <typename T, int V, bool ONE>
 __global__ void __launch_bounds__(kSplitThreads)
 norm_split_apply_kernel(const Slab s) {
-  __shared__ float mean_all[kMaxGroups], rstd_all[kMaxGroups];
-  constexpr int M = ONE ? 1 : V;
+  __shared__ float2 all_of[kMaxGroups];
+  constexpr int M = ONE ? 1 : Pack<T, V>::kPairs;
   chained();
   const NormParams& p = s.p;
   const int piece = blockIdx.x % s.pieces, job = blockIdx.x / s.pieces, slab = job % s.slabs, n = job / s.slabs;
@@ -409,8 +420,7 @@ norm_split_apply_kernel(const Slab s) {
       all = joined(all, Moments{float(min(s.S, (q + 1) * s.rows) - q * s.rows) * float(cpg), v.x, v.y});
     }
     const float rstd = rsqrtf(all.m2 / all.n + p.eps);
-    mean_all[g] = all.mean;
-    rstd_all[g] = rstd;
+    all_of[g] = make_float2(all.mean, rstd);
     if (p.mean != nullptr && piece == 0) {
       p.mean[(long long)n * p.G + g0 + g] = all.mean;
       p.rstd[(long long)n * p.G + g0 + g] = rstd;
@@ -419,13 +429,15 @@ norm_split_apply_kernel(const Slab s) {
   __syncthreads();
   if (!at.live) return;
   const long long px = p.W > 1 ? p.x_s[3] : p.x_s[2], py = p.W > 1 ? p.y_s[3] : p.y_s[2];
-  float w[V], b[V], m[M];
-  channel_params<T, V>(p, at.c0 + at.cc, true, w, b);
+  constexpr int P = Pack<T, V>::kPairs;
+  F2 w[P], b[P], m[M];                              // m: minus the mean
+  norm_params_of<T, V>(p, at.c0 + at.cc, true, w, b);
 #pragma unroll
-  for (int j = 0; j < V; ++j) {
-    const int g = (at.cc + (ONE ? 0 : j)) / cpg;
-    m[ONE ? 0 : j] = mean_all[g];
-    w[j] *= rstd_all[g];
+  for (int i = 0; i < P; ++i) {
+    const float2 lo = all_of[at.live ? (at.cc + (ONE ? 0 : 2 * i)) / cpg : 0];
+    const float2 hi = ONE ? lo : all_of[at.live ? (at.cc + min(2 * i + 1, V - 1)) / cpg : 0];
+    m[ONE ? 0 : i] = f2_pack(-lo.x, -hi.x);
+    w[i] = f2_mul(w[i], f2_pack(lo.y, hi.y));
   }
   const T* x0 = static_cast<const T*>(p.x) + n * p.x_s[0] + at.c0 + at.cc;
   T* y0 = static_cast<T*>(p.y) + n * p.y_s[0] + at.c0 + at.cc;
@@ -435,7 +447,7 @@ norm_split_apply_kernel(const Slab s) {
       Pack<T, V> x, y;
       x.load(x0 + row * px);
 #pragma unroll
-      for (int j = 0; j < V; ++j) y.set(j, activate<decltype(act)::value>((x.at(j) - m[ONE ? 0 : j]) * w[j] + b[j]));
+      for (int i = 0; i < P; ++i) y.set_pair(i, activate2<decltype(act)::value>(f2_fma(f2_add(x.pair(i), m[ONE ? 0 : i]), w[i], b[i])));
       y.store(y0 + row * py);
     }
   });
@@ -446,7 +458,7 @@ __global__ void __launch_bounds__(kSplitThreads)
 norm_split_sums_kernel(const Slab s) {
   extern __shared__ __align__(16) unsigned char raw[];
   const BackwardShared sh(raw, kSplitThreads * V, s.channels);
-  constexpr int M = ONE ? 1 : V;
+  constexpr int M = ONE ? 1 : Pack<T, V>::kPairs;
   chained();
   const NormParams& p = s.p;
   const int piece = blockIdx.x % s.pieces, job = blockIdx.x / s.pieces, slab = job % s.slabs, n = job / s.slabs;
@@ -455,16 +467,18 @@ norm_split_sums_kernel(const Slab s) {
   at.at<V>();
   const long long px = p.W > 1 ? p.x_s[3] : p.x_s[2], pdy = p.W > 1 ? p.dy_s[3] : p.dy_s[2];
   const int c = at.c0 + at.cc;
-  float w[V], b[V], mean[M], rstd[M], gx[V], gs[V];
-  channel_params<T, V>(p, c, at.live, w, b);
+  constexpr int P = Pack<T, V>::kPairs;
+  F2 w[P], b[P], mean[M], rstd[M], gx[P], gs[P];    // mean: minus the mean
+  norm_params_of<T, V>(p, c, at.live, w, b);
 #pragma unroll
-  for (int j = 0; j < M; ++j) {
-    const long long g = (long long)n * p.G + (at.live ? (c + j) / cpg : 0);
-    mean[j] = p.mean[g];
-    rstd[j] = p.rstd[g];
+  for (int i = 0; i < M; ++i) {
+    const long long lo = (long long)n * p.G + (at.live ? (c + 2 * i) / cpg : 0);
+    const long long hi = ONE ? lo : (long long)n * p.G + (at.live ? (c + min(2 * i + 1, V - 1)) / cpg : 0);
+    mean[i] = f2_pack(-p.mean[lo], -p.mean[hi]);
+    rstd[i] = f2_pack(p.rstd[lo], p.rstd[hi]);
   }
 #pragma unroll
-  for (int j = 0; j < V; ++j) gx[j] = gs[j] = 0.0f;
+  for (int i = 0; i < P; ++i) gx[i] = gs[i] = 0;
   const T* x0 = static_cast<const T*>(p.x) + n * p.x_s[0] + c;
   const T* dy0 = static_cast<const T*>(p.dy) + n * p.dy_s[0] + c;
   if (at.live)
@@ -475,11 +489,11 @@ norm_split_sums_kernel(const Slab s) {
         x.load(x0 + row * px);
         dy.load(dy0 + row * pdy);
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-          const float xh = (x.at(j) - mean[ONE ? 0 : j]) * rstd[ONE ? 0 : j];
-          const float g = dy.at(j) * slope<decltype(act)::value>(xh * w[j] + b[j]);
-          gx[j] += g * xh;
-          gs[j] += g;
+        for (int i = 0; i < P; ++i) {
+          const F2 xh = f2_mul(f2_add(x.pair(i), mean[ONE ? 0 : i]), rstd[ONE ? 0 : i]);
+          const F2 g = f2_mul(dy.pair(i), slope2<decltype(act)::value>(f2_fma(xh, w[i], b[i])));
+          gx[i] = f2_fma(g, xh, gx[i]);
+          gs[i] = f2_add(gs[i], g);
         }
       }
     });
@@ -493,7 +507,7 @@ __global__ void __launch_bounds__(kSplitThreads)
 norm_split_dx_kernel(const Slab s) {
   extern __shared__ __align__(16) unsigned char raw[];
   const BackwardShared sh(raw, kSplitThreads * V, s.channels);
-  constexpr int M = ONE ? 1 : V;
+  constexpr int M = ONE ? 1 : Pack<T, V>::kPairs;
   chained();
   const NormParams& p = s.p;
   const int piece = blockIdx.x % s.pieces, job = blockIdx.x / s.pieces, slab = job % s.slabs, n = job / s.slabs;
@@ -516,16 +530,18 @@ norm_split_dx_kernel(const Slab s) {
   const bool tall = p.W > 1;
   const long long px = tall ? p.x_s[3] : p.x_s[2], pdy = tall ? p.dy_s[3] : p.dy_s[2], pdx = tall ? p.dx_s[3] : p.dx_s[2];
   const int c = at.c0 + at.cc;
-  float w[V], b[V], mean[M], rstd[M], s1[M], s2[M];
-  channel_params<T, V>(p, c, true, w, b);
+  constexpr int P = Pack<T, V>::kPairs;
+  F2 w[P], b[P], mean[M], rstd[M], s1[M], s2[M];    // minus the mean, minus s1 / m, minus s2 / m
+  norm_params_of<T, V>(p, c, true, w, b);
 #pragma unroll
-  for (int j = 0; j < M; ++j) {
-    const long long g = (long long)n * p.G + (c + j) / cpg;
-    mean[j] = p.mean[g];
-    rstd[j] = p.rstd[g];
-    const float2 m = sh.means[(at.cc + j) / cpg];
-    s1[j] = m.x;
-    s2[j] = m.y;
+  for (int i = 0; i < M; ++i) {
+    const int glo = (c + 2 * i) / cpg, ghi = ONE ? glo : (c + min(2 * i + 1, V - 1)) / cpg;
+    const long long at_n = (long long)n * p.G;
+    mean[i] = f2_pack(-p.mean[at_n + glo], -p.mean[at_n + ghi]);
+    rstd[i] = f2_pack(p.rstd[at_n + glo], p.rstd[at_n + ghi]);
+    const float2 lo = sh.means[glo - at.c0 / cpg], hi = sh.means[ghi - at.c0 / cpg];
+    s1[i] = f2_pack(-lo.x, -hi.x);
+    s2[i] = f2_pack(-lo.y, -hi.y);
   }
   const T* x0 = static_cast<const T*>(p.x) + n * p.x_s[0] + c;
   const T* dy0 = static_cast<const T*>(p.dy) + n * p.dy_s[0] + c;
@@ -537,10 +553,10 @@ norm_split_dx_kernel(const Slab s) {
       x.load(x0 + row * px);
       dy.load(dy0 + row * pdy);
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const float xh = (x.at(j) - mean[ONE ? 0 : j]) * rstd[ONE ? 0 : j];
-        const float g = dy.at(j) * slope<decltype(act)::value>(xh * w[j] + b[j]);
-        dx.set(j, rstd[ONE ? 0 : j] * (g * w[j] - s1[ONE ? 0 : j] - xh * s2[ONE ? 0 : j]));
+      for (int i = 0; i < P; ++i) {
+        const F2 xh = f2_mul(f2_add(x.pair(i), mean[ONE ? 0 : i]), rstd[ONE ? 0 : i]);
+        const F2 g = f2_mul(dy.pair(i), slope2<decltype(act)::value>(f2_fma(xh, w[i], b[i])));
+        dx.set_pair(i, f2_mul(rstd[ONE ? 0 : i], f2_fma(xh, s2[ONE ? 0 : i], f2_fma(g, w[i], s1[ONE ? 0 : i]))));
       }
       dx.store(dx0 + row * pdx);
     }

@@ -49,17 +49,13 @@ norm_tokens_kernel(const TokenParams t) {
   const NormParams& p = t.p;
   const Seat<EACH> seat(t);
   const int cpg = p.C / p.G;
-  float w[EACH][V], b[EACH][V];
-  long long at[EACH];
+  constexpr int P = Pack<T, V>::kPairs;
+  F2 w[EACH][P], b[EACH][P];
+  int at[EACH];
 #pragma unroll
   for (int e = 0; e < EACH; ++e) {
-    const int c = seat.g * cpg + (seat.u0 + e * t.lanes) * V;
-    at[e] = seat.in(t, e) ? c : 0;
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      w[e][j] = seat.in(t, e) && p.weight != nullptr ? param<T>(p.weight, p.param_f32, c + j) : 1.0f;
-      b[e][j] = seat.in(t, e) && p.bias != nullptr ? param<T>(p.bias, p.param_f32, c + j) : 0.0f;
-    }
+    at[e] = seat.in(t, e) ? seat.g * cpg + (seat.u0 + e * t.lanes) * V : 0;
+    norm_params_of<T, V>(p, at[e], seat.in(t, e), w[e], b[e]);
   }
   const float m = float(cpg);
   with_activation(p.act, [&](auto act) {
@@ -76,21 +72,27 @@ norm_tokens_kernel(const TokenParams t) {
       }
 #pragma unroll
       for (int k = 0; k < TOKENS; ++k) {
-        float sum = 0.0f;
+        F2 sum = 0;
 #pragma unroll
-        for (int e = 0; e < EACH; ++e)
+        for (int e = 0; e < EACH; ++e) {
 #pragma unroll
-          for (int j = 0; j < V; ++j) sum += x[k][e].at(j);
-        const float mean = lane_sum(sum, t.lanes) / m;
+          for (int i = 0; i < P; ++i) sum = f2_add(sum, x[k][e].pair(i));
+        }
+        const float mean = lane_sum(f2_sum(sum), t.lanes) / m;
+        const F2 minus = f2_pack(-mean, V == 1 ? 0.0f : -mean);
         float m2 = 0.0f;
 #pragma unroll
-        for (int e = 0; e < EACH; ++e)
+        for (int e = 0; e < EACH; ++e) {
+          F2 square = 0;
 #pragma unroll
-          for (int j = 0; j < V; ++j) {
-            const float d = x[k][e].at(j) - mean;
-            m2 += seat.in(t, e) ? d * d : 0.0f;
+          for (int i = 0; i < P; ++i) {
+            const F2 d = f2_add(x[k][e].pair(i), minus);
+            square = f2_fma(d, d, square);
           }
+          m2 += seat.in(t, e) ? f2_sum(square) : 0.0f;
+        }
         const float rstd = rsqrtf(lane_sum(m2, t.lanes) / m + p.eps);
+        const F2 scale = f2_both(rstd);
         if (n0 + k >= p.N) continue;
         if (p.mean != nullptr && seat.live && seat.u0 == 0) {
           p.mean[(n0 + k) * p.G + seat.g] = mean;
@@ -101,7 +103,8 @@ norm_tokens_kernel(const TokenParams t) {
           if (!seat.in(t, e)) continue;
           Pack<T, V> y;
 #pragma unroll
-          for (int j = 0; j < V; ++j) y.set(j, activate<decltype(act)::value>((x[k][e].at(j) - mean) * (rstd * w[e][j]) + b[e][j]));
+          for (int i = 0; i < P; ++i)
+            y.set_pair(i, activate2<decltype(act)::value>(f2_fma(f2_mul(f2_add(x[k][e].pair(i), minus), scale), w[e][i], b[e][i])));
           y.store(static_cast<T*>(p.y) + (n0 + k) * p.y_s[0] + at[e]);
         }
       }
@@ -116,18 +119,15 @@ norm_tokens_backward_kernel(const TokenParams t) {
   const NormParams& p = t.p;
   const Seat<EACH> seat(t);
   const int cpg = p.C / p.G;
-  float w[EACH][V], b[EACH][V], dw[EACH][V], db[EACH][V];
-  long long at[EACH];
+  constexpr int P = Pack<T, V>::kPairs;
+  F2 w[EACH][P], b[EACH][P], dw[EACH][P], db[EACH][P];
+  int at[EACH];
 #pragma unroll
   for (int e = 0; e < EACH; ++e) {
-    const int c = seat.g * cpg + (seat.u0 + e * t.lanes) * V;
-    at[e] = seat.in(t, e) ? c : 0;
+    at[e] = seat.in(t, e) ? seat.g * cpg + (seat.u0 + e * t.lanes) * V : 0;
+    norm_params_of<T, V>(p, at[e], seat.in(t, e), w[e], b[e]);
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      w[e][j] = seat.in(t, e) && p.weight != nullptr ? param<T>(p.weight, p.param_f32, c + j) : 1.0f;
-      b[e][j] = seat.in(t, e) && p.bias != nullptr ? param<T>(p.bias, p.param_f32, c + j) : 0.0f;
-      dw[e][j] = db[e][j] = 0.0f;
-    }
+    for (int i = 0; i < P; ++i) dw[e][i] = db[e][i] = 0;
   }
   const float inv = 1.0f / float(cpg);
   with_activation(p.act, [&](auto act) {
@@ -153,20 +153,23 @@ norm_tokens_backward_kernel(const TokenParams t) {
 #pragma unroll
       for (int k = 0; k < TOKENS; ++k) {
         const bool there = n0 + k < p.N;
-        float s1 = 0.0f, s2 = 0.0f, xh[EACH][V], g[EACH][V];
+        const F2 minus = f2_both(-mean[k]), scale = f2_both(rstd[k]);
+        F2 xh[EACH][P], g[EACH][P], t1 = 0, t2 = 0;
 #pragma unroll
-        for (int e = 0; e < EACH; ++e)
+        for (int e = 0; e < EACH; ++e) {
+          const bool in = there && seat.in(t, e);
 #pragma unroll
-          for (int j = 0; j < V; ++j) {
-            const bool in = there && seat.in(t, e);
-            xh[e][j] = in ? (x[k][e].at(j) - mean[k]) * rstd[k] : 0.0f;
-            g[e][j] = in ? dy[k][e].at(j) * slope<decltype(act)::value>(xh[e][j] * w[e][j] + b[e][j]) : 0.0f;
-            dw[e][j] += g[e][j] * xh[e][j];
-            db[e][j] += g[e][j];
-            g[e][j] *= w[e][j];
-            s1 += g[e][j];
-            s2 += g[e][j] * xh[e][j];
+          for (int i = 0; i < P; ++i) {
+            xh[e][i] = in ? f2_mul(f2_add(x[k][e].pair(i), minus), scale) : 0;
+            g[e][i] = in ? f2_mul(dy[k][e].pair(i), slope2<decltype(act)::value>(f2_fma(xh[e][i], w[e][i], b[e][i]))) : 0;
+            dw[e][i] = f2_fma(g[e][i], xh[e][i], dw[e][i]);
+            db[e][i] = f2_add(db[e][i], g[e][i]);
+            g[e][i] = f2_mul(g[e][i], w[e][i]);
+            t1 = f2_add(t1, g[e][i]);
+            t2 = f2_fma(g[e][i], xh[e][i], t2);
           }
+        }
+        float s1 = f2_sum(t1), s2 = f2_sum(t2);
         s1 = lane_sum(s1, t.lanes) * inv;
         s2 = lane_sum(s2, t.lanes) * inv;
         if (!there || p.dx == nullptr) continue;
@@ -175,7 +178,7 @@ norm_tokens_backward_kernel(const TokenParams t) {
           if (!seat.in(t, e)) continue;
           Pack<T, V> dx;
 #pragma unroll
-          for (int j = 0; j < V; ++j) dx.set(j, rstd[k] * (g[e][j] - s1 - xh[e][j] * s2));
+          for (int i = 0; i < P; ++i) dx.set_pair(i, f2_mul(scale, f2_fma(xh[e][i], f2_both(-s2), f2_add(g[e][i], f2_both(-s1)))));
           dx.store(static_cast<T*>(p.dx) + (n0 + k) * p.dx_s[0] + at[e]);
         }
       }
@@ -183,10 +186,18 @@ norm_tokens_backward_kernel(const TokenParams t) {
   });
   // the block's part of a row of sums; every channel has one lane
 #pragma unroll
-  for (int e = 0; e < EACH; ++e)
+  for (int e = 0; e < EACH; ++e) {
+    if (!seat.in(t, e)) continue;
+    float2* to = t.rows + (long long)blockIdx.y * p.C + at[e];
 #pragma unroll
-    for (int j = 0; j < V; ++j)
-      if (seat.in(t, e)) t.rows[(long long)blockIdx.y * p.C + at[e] + j] = make_float2(dw[e][j], db[e][j]);
+    for (int i = 0; i < P; ++i) {
+      float w0, w1, b0, b1;
+      f2_split(dw[e][i], w0, w1);
+      f2_split(db[e][i], b0, b1);
+      to[2 * i] = make_float2(w0, b0);
+      if (V > 1) to[2 * i + 1] = make_float2(w1, b1);
+    }
+  }
 }
 
 // How a problem is cut; EACH vectors a lane, 0: a group is larger than a warp holds.

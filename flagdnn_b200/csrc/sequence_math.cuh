@@ -6,6 +6,7 @@
 
 #include "../../include/flagdnn_b200.h"
 #include "conv_convert.cuh"
+#include "f32x2.cuh"
 #include "sm100_ptx.cuh"
 
 namespace fdnn {
@@ -18,9 +19,15 @@ __device__ __forceinline__ float ex2(float v) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
   return r;
 }
-// 1 / (1 + e^-v): the denominator is infinite below -88, which divides to zero
-__device__ __forceinline__ float logistic(float v) { return __fdividef(1.0f, 1.0f + ex2(-kLog2e * v)); }
-__device__ __forceinline__ float silu(float v) { return __fdividef(v, 1.0f + ex2(-kLog2e * v)); }
+// 1 / v by the special function unit (one unit in the last place)
+__device__ __forceinline__ float rcp(float v) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+// 1 / (1 + e^-v): the denominator is infinite below -88, whose reciprocal is zero
+__device__ __forceinline__ float logistic(float v) { return rcp(1.0f + ex2(-kLog2e * v)); }
+__device__ __forceinline__ float silu(float v) { return v * logistic(v); }
 // log(1 + e^v) = max(v, 0) + log(1 + e), e = e^-|v| at most 1.  log(1 + e) / e is a polynomial of degree 9, fitted to the
 // smallest relative error on [0, 1] (5e-9; 1.3e-7 in fp32 arithmetic): no result is lost where e is small, and no second call of
 // the special function unit, which bounds the scan.
@@ -48,7 +55,7 @@ __device__ __forceinline__ float activate(float v) {
   if constexpr (ACT == FDNN_ACT_RELU) return v < 0.0f ? 0.0f : v;   // NaN stays
   if constexpr (ACT == FDNN_ACT_GELU) return 0.5f * v * erfcf(-kSqrtHalf * v);
   if constexpr (ACT == FDNN_ACT_GELU_TANH)   // (1 + tanh a) / 2 is the logistic function of 2 a
-    return __fdividef(v, 1.0f + ex2(-2.0f * kLog2e * kGeluTanhScale * (v + kGeluTanhCubic * v * v * v)));
+    return v * logistic(2.0f * kGeluTanhScale * (v + kGeluTanhCubic * v * v * v));
   if constexpr (ACT == FDNN_ACT_SILU) return silu(v);
   return v;
 }
@@ -66,10 +73,32 @@ __device__ __forceinline__ float slope(float v) {
   }
   if constexpr (ACT == FDNN_ACT_SILU) {
     const float p = logistic(v);
-    const float rest = 1.0f - p;
-    return p * (1.0f + (rest == 0.0f ? 0.0f : v * rest));
+    return p * (1.0f + v * (1.0f - p));
   }
   return 1.0f;
+}
+
+// The same for two values: the cheap ones stay packed.
+template <int ACT>
+__device__ __forceinline__ F2 activate2(F2 v) {
+  if constexpr (ACT == FDNN_ACT_NONE) return v;
+  float lo, hi;
+  f2_split(v, lo, hi);
+  return f2_pack(activate<ACT>(lo), activate<ACT>(hi));
+}
+template <int ACT>
+__device__ __forceinline__ F2 slope2(F2 v) {
+  if constexpr (ACT == FDNN_ACT_NONE) return f2_both(1.0f);
+  if constexpr (ACT == FDNN_ACT_SILU) {
+    float lo, hi;
+    f2_split(f2_mul(v, f2_both(-kLog2e)), lo, hi);
+    f2_split(f2_add(f2_pack(ex2(lo), ex2(hi)), f2_both(1.0f)), lo, hi);
+    const F2 p = f2_pack(rcp(lo), rcp(hi));
+    return f2_mul(p, f2_fma(v, f2_fma(p, f2_both(-1.0f), f2_both(1.0f)), f2_both(1.0f)));
+  }
+  float lo, hi;
+  f2_split(v, lo, hi);
+  return f2_pack(slope<ACT>(lo), slope<ACT>(hi));
 }
 
 // Runs f(std::integral_constant<int, ACT>) for a run-time activation: the branch is taken once, not per element.
