@@ -263,6 +263,7 @@ unsigned grid_of(long long items) { return unsigned(items < (1ll << 30) ? items 
 
 template <typename T, typename I>
 cudaError_t forward(const NormParams& p, cudaStream_t stream) {
+  if (8ll * p.N * p.G * chunks_of(p).count > p.workspace_bytes) return cudaErrorInvalidValue;
   const long long items = (long long)p.N * p.G * chunks_of(p).count;
   cudaError_t e = launch_seq(norm_stats_kernel<T, I>, dim3(grid_of(items)), kThreads, 0, 1, stream, p);
   if (e != cudaSuccess) return e;
@@ -271,6 +272,7 @@ cudaError_t forward(const NormParams& p, cudaStream_t stream) {
 
 template <typename T, typename I>
 cudaError_t backward(const NormParams& p, cudaStream_t stream) {
+  if (8ll * p.N * p.C > p.workspace_bytes) return cudaErrorInvalidValue;
   const long long channels = (long long)p.N * p.C;
   cudaError_t e = (long long)p.H * p.W <= 32
                       ? launch_seq(norm_channel_sums_thin_kernel<T>, dim3(grid_of((channels + kThreads - 1) / kThreads)), kThreads, 0, 1, stream, p)
@@ -311,7 +313,10 @@ long long group_norm_workspace(int dtype, const NormParams& p, bool backward) {
   if (!norm_rows(p, backward) || p.C / p.G > 512 || (long long)p.H * p.W > (1 << 29)) return here;
   const long long images = norm_images_workspace(dtype, p, backward);
   const long long tokens = p.H == 1 && p.W == 1 ? norm_tokens_workspace(dtype, p, backward) : 0;
-  return tokens > images ? tokens : images;
+  // images of groups that may be wider than the 256 threads of their two-launch form
+  const long long wide = p.C / p.G > 256 && (long long)p.H * p.W > 64 ? here : 0;
+  const long long most = tokens > images ? tokens : images;
+  return most > wide ? most : wide;
 }
 
 cudaError_t launch_group_norm(int dtype, const NormParams& p, cudaStream_t stream) {

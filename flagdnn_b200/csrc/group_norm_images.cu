@@ -591,7 +591,7 @@ bool slab_of(ImagePlan* plan, const NormParams& p, int V, int threads, int chann
   return channels / (p.C / p.G) <= kMaxGroups;
 }
 
-// The slab: whole groups and whole vectors, rows of about 128 bytes (8 vectors: narrower rows waste what a DRAM access brings,
+// The slab: whole groups and whole vectors, rows of about 64 bytes (4 vectors: narrower rows waste what a DRAM access brings,
 // wider ones leave too few blocks), narrower where that is what a cluster holds or too few blocks would run.
 // Then the fewest blocks to a cluster that hold it at eight vectors a thread (x and dy: four), sixteen and 512 threads last.
 bool image_plan(int dtype, const NormParams& p, bool backward, ImagePlan* plan) {
@@ -604,7 +604,7 @@ bool image_plan(int dtype, const NormParams& p, bool backward, ImagePlan* plan) 
   const int unit = cpg / gcd(cpg, V) * V, units = p.C / unit;   // whole groups and whole vectors
   const int sms = current_sm_count();
   const int tops[2] = {backward ? 8 : 16, backward ? 8 : 16};
-  const long long wide = S < 32 ? 256 / S : 8;                  // (few pixels: wider rows, or threads have none)
+  const long long wide = S < 64 ? 256 / S : 4;                  // (few pixels: wider rows, or threads have none)
   int k = int(wide * V / unit);
   if (k < 1) k = 1;
   if (k > units) k = units;
@@ -615,7 +615,7 @@ bool image_plan(int dtype, const NormParams& p, bool backward, ImagePlan* plan) 
       Slab& s = plan->s;
       const long long at_once = s.rows_at_once;
       if (8 * at_once * tops[threads > 256] < S) continue;
-      const int want = backward ? 4 : 8;
+      const int want = backward ? 8 : 16;
       int cluster = 1;
       while (cluster < 8 && cluster * at_once * want < S) cluster *= 2;
       // few blocks: more to a cluster, as long as each has rows for its threads
@@ -652,6 +652,7 @@ cudaError_t forward(ImagePlan& plan, cudaStream_t stream) {
   if (plan.R == 0) {
     const long long blocks = (long long)p.N * s.slabs * s.pieces;
     if (blocks > 0x7fffffffll) return cudaErrorInvalidConfiguration;
+    if (8ll * p.N * s.pieces * p.G > p.workspace_bytes) return cudaErrorInvalidValue;
     s.part = static_cast<float2*>(p.workspace);
     const cudaError_t e = launch_seq(norm_split_stats_kernel<T, V, ONE>, dim3(unsigned(blocks)), kSplitThreads, 0, 1, stream, s);
     if (e != cudaSuccess) return e;
@@ -693,15 +694,14 @@ cudaError_t backward(ImagePlan& plan, cudaStream_t stream) {
   const NormParams& p = s.p;
   s.sums = static_cast<float2*>(p.workspace);
   cudaError_t e;
-  long long rows;
+  const long long rows = plan.R == 0 ? (long long)p.N * s.pieces : s.slices;
+  if (8 * rows * p.C > p.workspace_bytes) return cudaErrorInvalidValue;
   if (plan.R == 0) {
     const long long blocks = (long long)p.N * s.slabs * s.pieces;
     if (blocks > 0x7fffffffll) return cudaErrorInvalidConfiguration;
     e = run_split<T, V, ONE>(s, blocks, stream);
-    rows = (long long)p.N * s.pieces;
   } else {
     const long long blocks = (long long)s.slices * s.slabs * s.cluster;
-    rows = s.slices;
     e = plan.threads > 256 ? run_backward<T, V, ONE, 8, 512>(s, blocks, stream)
         : plan.R <= 2      ? run_backward<T, V, ONE, 2, 256>(s, blocks, stream)
         : plan.R == 4      ? run_backward<T, V, ONE, 4, 256>(s, blocks, stream)

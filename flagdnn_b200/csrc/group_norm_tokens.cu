@@ -247,6 +247,7 @@ TokenPlan backward_plan(const NormParams& p) {
 template <typename T, int V>
 cudaError_t backward(const NormParams& p, cudaStream_t stream) {
   const TokenPlan plan = backward_plan<T, V>(p);
+  if (8ll * p.C * plan.t.slices > p.workspace_bytes) return cudaErrorInvalidValue;
   const dim3 grid(unsigned(plan.blocks), unsigned(plan.t.slices));
   cudaError_t e;
   switch (plan.each) {

@@ -105,14 +105,14 @@ struct Ring {
   uint4 delta[kSlots][kWords][kHalf];
   uint4 bc[kSlots][PIECES > 0 ? PIECES : 1][kWords][kHalf];
 };
-// VEC: asynchronously, zeros where `count` is zero
+// VEC: asynchronously, 16 bytes at a time, zeros past `count` values
 template <bool VEC, typename T>
 __device__ __forceinline__ void fetch(uint4 (&slot)[Eight<T>::kWords][kHalf], int tid, const T* p, long long stride, int count) {
   if constexpr (VEC) {
 #pragma unroll
     for (int w = 0; w < Eight<T>::kWords; ++w)
       asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(uint32_t(__cvta_generic_to_shared(&slot[w][tid]))),
-                   "l"(reinterpret_cast<const uint4*>(p) + w), "r"(count > 0 ? 16 : 0)
+                   "l"(reinterpret_cast<const uint4*>(p) + w), "r"(count > w * 16 / int(sizeof(T)) ? 16 : 0)
                    : "memory");
   } else {
     Eight<T> v;
@@ -286,7 +286,8 @@ scan_kernel(const ScanJob job) {
 #pragma unroll
           for (int k = 0; k < 8; ++k) out.set(k, from_f32<T>(v[k]));
 #pragma unroll
-          for (int w = 0; w < Eight<T>::kWords; ++w) reinterpret_cast<uint4*>(y)[w] = out.q[w];
+          for (int w = 0; w < Eight<T>::kWords; ++w)
+            if (have > w * 16 / int(sizeof(T))) reinterpret_cast<uint4*>(y)[w] = out.q[w];
         } else {
 #pragma unroll
           for (int k = 0; k < 8; ++k)
@@ -501,7 +502,7 @@ Cut cut_of(const ScanParams& p) {
   return best;
 }
 
-// Whether every tensor can be read (and y written) by 16 bytes: eights of channels and of states dense, aligned and whole.
+// Whether every tensor can be read (and y written) by 16 bytes: channels and states dense, aligned and whole numbers of them.
 template <typename T>
 bool by_eights(const ScanParams& p) {
   const int per = 16 / int(sizeof(T));
@@ -511,7 +512,7 @@ bool by_eights(const ScanParams& p) {
       if (i != last && st[i] % per != 0) return false;
     return true;
   };
-  return p.C / p.G % 8 == 0 && p.S % 8 == 0 && (p.S & (p.S - 1)) == 0 && ok(p.u, p.u_s, 2, 3) && ok(p.delta, p.delta_s, 2, 3) &&
+  return p.C / p.G % per == 0 && p.S % 8 == 0 && (p.S & (p.S - 1)) == 0 && ok(p.u, p.u_s, 2, 3) && ok(p.delta, p.delta_s, 2, 3) &&
          ok(p.y, p.y_s, 2, 3) && (p.z == nullptr || ok(p.z, p.z_s, 2, 3)) && ok(p.B, p.b_s, 3, 4) && ok(p.Cm, p.c_s, 3, 4);
 }
 

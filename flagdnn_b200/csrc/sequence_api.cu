@@ -32,6 +32,7 @@ int norm_params(const fdnn_norm_desc* d, NormParams* p) {
   p->y = p->dx = p->dweight = p->dbias = nullptr;
   p->mean = p->rstd = nullptr;
   p->workspace = nullptr;
+  p->workspace_bytes = 0;
   return FDNN_OK;
 }
 
@@ -108,7 +109,7 @@ int fdnn_group_norm_fwd(const fdnn_norm_desc* desc, const void* x, const void* w
   if (x == nullptr || y == nullptr) return api_fail(FDNN_BAD_PARAM, "x and y must not be NULL");
   st = check_workspace(workspace, workspace_bytes, group_norm_workspace(desc->dtype, p, false));
   if (st != FDNN_OK) return st;
-  p.x = x; p.weight = weight; p.bias = bias; p.y = y; p.mean = mean; p.rstd = rstd; p.workspace = workspace;
+  p.x = x; p.weight = weight; p.bias = bias; p.y = y; p.mean = mean; p.rstd = rstd; p.workspace = workspace; p.workspace_bytes = workspace_bytes;
   const cudaError_t e = launch_group_norm(desc->dtype, p, static_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? FDNN_OK : api_fail_cuda("group_norm launch", e);
 }
@@ -134,7 +135,7 @@ int fdnn_group_norm_bwd(const fdnn_norm_desc* desc, const void* dy, const void* 
   st = check_workspace(workspace, workspace_bytes, group_norm_workspace(desc->dtype, p, true));
   if (st != FDNN_OK) return st;
   p.x = x; p.dy = dy; p.weight = weight; p.bias = bias; p.dx = dx; p.dweight = dweight; p.dbias = dbias;
-  p.mean = const_cast<float*>(mean); p.rstd = const_cast<float*>(rstd); p.workspace = workspace;
+  p.mean = const_cast<float*>(mean); p.rstd = const_cast<float*>(rstd); p.workspace = workspace; p.workspace_bytes = workspace_bytes;
   const cudaError_t e = launch_group_norm_backward(desc->dtype, p, s);
   return e == cudaSuccess ? FDNN_OK : api_fail_cuda("group_norm backward launch", e);
 }

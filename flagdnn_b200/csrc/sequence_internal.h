@@ -22,6 +22,7 @@ struct NormParams {
   void *y, *dx, *dweight, *dbias;
   float *mean, *rstd;    // [N, G]; forward: written if not null, backward: read
   void* workspace;
+  long long workspace_bytes;   // every launcher compares it with what it is about to write
 };
 long long group_norm_workspace(int dtype, const NormParams& p, bool backward);
 cudaError_t launch_group_norm(int dtype, const NormParams& p, cudaStream_t stream);

@@ -76,6 +76,10 @@ SHAPES = [   # shape, groups, layout
     ((1, 64, 112, 112), 2, "cl"),         # a group of 401 408 values
     ((1, 16, 260, 260), 1, "cl"),         # larger than a cluster holds
     ((2, 8, 512, 300), 8, "cl"),
+    ((1, 511, 13, 13), 1, "cl"),          # a group wider than a block of the two-launch form
+    ((2, 300, 9, 10), 1, "odd"),
+    ((2, 1026, 3, 3), 2, "cl"),
+    ((3, 700, 1, 1), 1, "odd"),
     ((5, 96, 1, 1), 8, "cl"),             # one pixel
     ((2, 256, 1, 3), 32, "cl"),
     ((2, 48, 17), 6, "cl"),               # [N, C, L]

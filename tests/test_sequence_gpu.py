@@ -138,6 +138,8 @@ SCANS = [   # n, l, c, s, groups, layout, lengths
     (2, 0, 16, 16, 1, "dense", None),
     (5, 129, 256, 16, 1, "dense", [129, 128, 127, 32, 33]),
     (1, 260, 1030, 16, 1, "dense", None),
+    (2, 70, 72, 16, 2, "dense", [70, 40]),             # 36 channels a group: eights and four
+    (2, 45, 40, 8, 2, "slice", None),
     (2, 2500, 40, 16, 1, "dense", [2500, 700]),       # rows in chunks
     (1, 2100, 24, 64, 2, "slice", None),
     (3, 1500, 9, 5, 1, "odd", [0, 1500, 130]),
