@@ -47,6 +47,27 @@ struct Pack {
   }
 };
 
+// A vector on its way into shared memory while the thread works on: zeros where it is not `there` (`from` is then any valid
+// address). What a thread has asked for it may read after async_wait(); nobody else may.
+template <typename T, int V>
+__device__ __forceinline__ void async_load(Pack<T, V>* to, const T* from, bool there) {
+  const uint32_t at = uint32_t(__cvta_generic_to_shared(to));
+  if constexpr (Pack<T, V>::kBytes == 16) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(at), "l"(from), "r"(there ? 16 : 0) : "memory");
+  } else if constexpr (Pack<T, V>::kBytes >= 4) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(at), "l"(from), "n"(Pack<T, V>::kBytes),
+                 "r"(there ? Pack<T, V>::kBytes : 0)
+                 : "memory");
+  } else {   // (two bytes cannot be copied asynchronously)
+    to->clear();
+    if (there) to->load(from);
+  }
+}
+__device__ __forceinline__ void async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// All but the newest N groups of this thread have arrived.
+template <int N>
+__device__ __forceinline__ void async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
 // A thread's parameters as pairs.
 template <typename T, int V>
 __device__ __forceinline__ void norm_params_of(const NormParams& p, int c, bool live, F2 (&w)[Pack<T, V>::kPairs], F2 (&b)[Pack<T, V>::kPairs]) {

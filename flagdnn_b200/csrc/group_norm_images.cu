@@ -18,6 +18,7 @@ namespace cg = cooperative_groups;
 
 constexpr int kMaxChunks = 64;        // pieces of an image in two launches
 constexpr int kMaxGroups = 512;       // of a slab
+constexpr int kMostShared = 220 * 1024;
 
 struct Slab {
   NormParams p;
@@ -130,68 +131,88 @@ __device__ __forceinline__ void local_moments(const Slab& s, const Place& at, co
   __syncthreads();
 }
 
+// Blocks of THREADS that share an SM.
+constexpr int blocks_per_sm(int threads) { return threads > 256 ? 1 : 2; }
+
 template <typename T, int V, bool ONE, int R, int THREADS>
-__global__ void __launch_bounds__(THREADS, THREADS > 256 ? 1 : R > 8 ? 2 : 3)
+__global__ void __launch_bounds__(THREADS, blocks_per_sm(THREADS))
 norm_images_kernel(const Slab s) {
+  extern __shared__ __align__(16) unsigned char raw[];
   __shared__ float2 red[ONE ? THREADS : THREADS * V];
   __shared__ float2 own[kMaxGroups], all_of[kMaxGroups];   // mean and squared deviations; mean and 1 / deviation
-  constexpr int M = ONE ? 1 : Pack<T, V>::kPairs;
+  constexpr int M = ONE ? 1 : Pack<T, V>::kPairs, P = Pack<T, V>::kPairs;
+  Pack<T, V>* next = reinterpret_cast<Pack<T, V>*>(raw) + threadIdx.x;   // this thread's rows of the next job, THREADS apart
   chained();
   const NormParams& p = s.p;
   const cg::cluster_group cluster = cg::this_cluster();
-  const int rank = blockIdx.x % s.cluster, job = blockIdx.x / s.cluster, slab = job % s.slabs, n = job / s.slabs;
-  const int row0 = rank * s.rows, rows = max(0, min(s.rows, s.S - row0)), cpg = p.C / p.G;
-  Place at(s, slab);
-  at.at<V>();
+  const int rank = blockIdx.x % s.cluster, jobs = p.N * s.slabs, cpg = p.C / p.G;
+  const int row0 = rank * s.rows, rows = max(0, min(s.rows, s.S - row0));
   const long long pixel = p.W > 1 ? p.x_s[3] : p.x_s[2], out_pixel = p.W > 1 ? p.y_s[3] : p.y_s[2];
-  const T* x0 = static_cast<const T*>(p.x) + n * p.x_s[0] + at.c0 + at.cc + (long long)(row0 + at.r) * pixel;
-  Pack<T, V> x[R];
+  auto fetch = [&](int job) {
+    if (job < jobs) {
+      const int slab = job % s.slabs, n = job / s.slabs;
+      Place at(s, slab);
+      at.at<V>();
+      const int count = at.live ? rows_of(s, at.r, rows) : 0;
+      const T* x0 = static_cast<const T*>(p.x) + (at.live ? n * p.x_s[0] + at.c0 + at.cc + (long long)(row0 + at.r) * pixel : 0);
 #pragma unroll
-  for (int k = 0; k < R; ++k) {
-    x[k].clear();
-    if (at.live && at.r + k * s.rows_at_once < rows) x[k].load(x0 + k * s.rows_at_once * pixel);
-  }
-  local_moments<T, V, ONE>(s, at, x, rows, red, own);
-  if (s.cluster > 1) cluster.sync();
-  const int g0 = at.c0 / cpg;
-  for (int g = threadIdx.x; g < at.here / cpg; g += THREADS) {
-    Moments all{0.0f, 0.0f, 0.0f};
-    for (int q = 0; q < s.cluster; ++q) {
-      const float count = float(max(0, min(s.rows, s.S - q * s.rows))) * float(cpg);
-      const float2 v = (s.cluster > 1 ? cluster.map_shared_rank(own, q) : own)[g];
-      if (count > 0.0f) all = joined(all, Moments{count, v.x, v.y});
+      for (int k = 0; k < R; ++k)
+        async_load(next + k * THREADS, k < count ? x0 + k * s.rows_at_once * pixel : static_cast<const T*>(p.x), k < count);
     }
-    const float rstd = rsqrtf(all.m2 / all.n + p.eps);
-    all_of[g] = make_float2(all.mean, rstd);
-    if (p.mean != nullptr && rank == 0) {
-      p.mean[(long long)n * p.G + g0 + g] = all.mean;
-      p.rstd[(long long)n * p.G + g0 + g] = rstd;
-    }
-  }
-  if (s.cluster > 1) cluster.barrier_arrive();   // this block has read the others' moments
-  __syncthreads();
-  constexpr int P = Pack<T, V>::kPairs;
-  F2 w[P], b[P], m[M];                              // m: minus the mean
-  norm_params_of<T, V>(p, at.c0 + at.cc, at.live, w, b);
+    async_commit();
+  };
+  const int clusters = gridDim.x / s.cluster;
+  fetch(blockIdx.x / s.cluster);
+  for (int job = blockIdx.x / s.cluster; job < jobs; job += clusters) {
+    const int slab = job % s.slabs, n = job / s.slabs;
+    Place at(s, slab);
+    at.at<V>();
+    Pack<T, V> x[R];
+    async_wait<0>();
 #pragma unroll
-  for (int i = 0; i < P; ++i) {
-    const float2 lo = all_of[at.live ? (at.cc + (ONE ? 0 : 2 * i)) / cpg : 0];
-    const float2 hi = ONE ? lo : all_of[at.live ? (at.cc + min(2 * i + 1, V - 1)) / cpg : 0];
-    m[ONE ? 0 : i] = f2_pack(-lo.x, -hi.x);
-    w[i] = f2_mul(w[i], f2_pack(lo.y, hi.y));
-  }
-  T* y0 = static_cast<T*>(p.y) + n * p.y_s[0] + at.c0 + at.cc + (long long)(row0 + at.r) * out_pixel;
-  with_activation(p.act, [&](auto act) {
-#pragma unroll
-    for (int k = 0; k < R; ++k)
-      if (at.live && at.r + k * s.rows_at_once < rows) {
-        Pack<T, V> y;
-#pragma unroll
-        for (int i = 0; i < P; ++i) y.set_pair(i, activate2<decltype(act)::value>(f2_fma(f2_add(x[k].pair(i), m[ONE ? 0 : i]), w[i], b[i])));
-        y.store(y0 + k * s.rows_at_once * out_pixel);
+    for (int k = 0; k < R; ++k) x[k] = next[k * THREADS];
+    fetch(job + clusters);
+    local_moments<T, V, ONE>(s, at, x, rows, red, own);
+    if (s.cluster > 1) cluster.sync();
+    const int g0 = at.c0 / cpg;
+    for (int g = threadIdx.x; g < at.here / cpg; g += THREADS) {
+      Moments all{0.0f, 0.0f, 0.0f};
+      for (int q = 0; q < s.cluster; ++q) {
+        const float count = float(max(0, min(s.rows, s.S - q * s.rows))) * float(cpg);
+        const float2 v = (s.cluster > 1 ? cluster.map_shared_rank(own, q) : own)[g];
+        if (count > 0.0f) all = joined(all, Moments{count, v.x, v.y});
       }
-  });
-  if (s.cluster > 1) cluster.barrier_wait();     // and the others have read this one's
+      const float rstd = rsqrtf(all.m2 / all.n + p.eps);
+      all_of[g] = make_float2(all.mean, rstd);
+      if (p.mean != nullptr && rank == 0) {
+        p.mean[(long long)n * p.G + g0 + g] = all.mean;
+        p.rstd[(long long)n * p.G + g0 + g] = rstd;
+      }
+    }
+    if (s.cluster > 1) cluster.barrier_arrive();   // this block has read the others' moments
+    __syncthreads();
+    F2 w[P], b[P], m[M];                              // m: minus the mean
+    norm_params_of<T, V>(p, at.c0 + at.cc, at.live, w, b);
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      const float2 lo = all_of[at.live ? (at.cc + (ONE ? 0 : 2 * i)) / cpg : 0];
+      const float2 hi = ONE ? lo : all_of[at.live ? (at.cc + min(2 * i + 1, V - 1)) / cpg : 0];
+      m[ONE ? 0 : i] = f2_pack(-lo.x, -hi.x);
+      w[i] = f2_mul(w[i], f2_pack(lo.y, hi.y));
+    }
+    T* y0 = static_cast<T*>(p.y) + n * p.y_s[0] + at.c0 + at.cc + (long long)(row0 + at.r) * out_pixel;
+    with_activation(p.act, [&](auto act) {
+#pragma unroll
+      for (int k = 0; k < R; ++k)
+        if (at.live && at.r + k * s.rows_at_once < rows) {
+          Pack<T, V> y;
+#pragma unroll
+          for (int i = 0; i < P; ++i) y.set_pair(i, activate2<decltype(act)::value>(f2_fma(f2_add(x[k].pair(i), m[ONE ? 0 : i]), w[i], b[i])));
+          y.store(y0 + k * s.rows_at_once * out_pixel);
+        }
+    });
+    if (s.cluster > 1) cluster.barrier_wait();     // and the others have read this one's
+  }
 }
 
 // Sums over a block's rows of two values per channel: sums[channel of the slab]. red: twice as many floats as threads times V.
@@ -257,11 +278,11 @@ struct BackwardShared {
   float2 *red, *own, *all, *acc, *means;
   __device__ BackwardShared(unsigned char* raw, int entries, int channels)
       : red(reinterpret_cast<float2*>(raw)), own(red + entries), all(own + channels), acc(all + channels), means(acc + channels) {}
-  static int bytes(int entries, int channels) { return 8 * (entries + 3 * channels + kMaxGroups); }
+  static __host__ __device__ int bytes(int entries, int channels) { return (8 * (entries + 3 * channels + kMaxGroups) + 15) / 16 * 16; }
 };
 
 template <typename T, int V, bool ONE, int R, int THREADS>
-__global__ void __launch_bounds__(THREADS, THREADS > 256 ? 1 : 2)
+__global__ void __launch_bounds__(THREADS, blocks_per_sm(THREADS))
 norm_images_backward_kernel(const Slab s) {
   extern __shared__ __align__(16) unsigned char raw[];
   const BackwardShared sh(raw, THREADS * V, s.channels);
@@ -280,19 +301,31 @@ norm_images_backward_kernel(const Slab s) {
   F2 w[P], b[P];
   norm_params_of<T, V>(p, c, at.live, w, b);
   for (int i = threadIdx.x; i < s.channels; i += THREADS) sh.acc[i] = make_float2(0.0f, 0.0f);
-  for (int n = slice; n < p.N; n += s.slices) {
-    const T* x0 = static_cast<const T*>(p.x) + n * p.x_s[0] + c + first * px;
-    const T* dy0 = static_cast<const T*>(p.dy) + n * p.dy_s[0] + c + first * pdy;
-    Pack<T, V> x[R], dy[R];
+  // this thread's rows of the next image, THREADS apart: x, then dy
+  Pack<T, V>* next = reinterpret_cast<Pack<T, V>*>(raw + BackwardShared::bytes(THREADS * V, s.channels)) + threadIdx.x;
+  const int count = at.live ? rows_of(s, at.r, rows) : 0;
+  auto fetch = [&](int n) {
+    if (n < p.N) {
+      const T* x0 = static_cast<const T*>(p.x) + (at.live ? n * p.x_s[0] + c + first * px : 0);
+      const T* dy0 = static_cast<const T*>(p.dy) + (at.live ? n * p.dy_s[0] + c + first * pdy : 0);
 #pragma unroll
-    for (int k = 0; k < R; ++k) {
-      x[k].clear();
-      dy[k].clear();
-      if (at.live && at.r + k * s.rows_at_once < rows) {
-        x[k].load(x0 + k * s.rows_at_once * px);
-        dy[k].load(dy0 + k * s.rows_at_once * pdy);
+      for (int k = 0; k < R; ++k) {
+        async_load(next + k * THREADS, k < count ? x0 + k * s.rows_at_once * px : static_cast<const T*>(p.x), k < count);
+        async_load(next + (R + k) * THREADS, k < count ? dy0 + k * s.rows_at_once * pdy : static_cast<const T*>(p.dy), k < count);
       }
     }
+    async_commit();
+  };
+  fetch(slice);
+  for (int n = slice; n < p.N; n += s.slices) {
+    Pack<T, V> x[R], dy[R];
+    async_wait<0>();
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+      x[k] = next[k * THREADS];
+      dy[k] = next[(R + k) * THREADS];
+    }
+    fetch(n + s.slices);
     F2 mean[M], rstd[M], gx[P], gs[P];               // mean: minus the mean
 #pragma unroll
     for (int i = 0; i < M; ++i) {
@@ -623,11 +656,15 @@ bool image_plan(int dtype, const NormParams& p, bool backward, ImagePlan* plan) 
       const long long need = (S + cluster * at_once - 1) / (cluster * at_once);
       if (k > 1 && need > want && (long long)p.N * s.slabs < 4ll * sms) break;       // narrower first
       if (k > 1 && (long long)p.N * s.slabs * cluster < sms && k * unit / V > 4) break;
-      plan->R = need <= 2 ? 2 : need <= 4 ? 4 : need <= 8 ? 8 : 16;
+      plan->R = need <= 2 ? 2 : need <= 4 && threads == 256 ? 4 : need <= 8 ? 8 : 16;
+      if (backward && BackwardShared::bytes(threads * V, s.channels) + 2 * plan->R * threads * 16 > kMostShared) continue;
       s.cluster = cluster;
       s.rows = int((S + cluster - 1) / cluster);
-      const long long room = 4ll * sms / ((long long)s.slabs * cluster);
-      s.slices = int(p.N < room ? p.N : room < 1 ? 1 : room);
+      // backward: as many clusters as the SMs hold at once, or fewer that have equally many images each
+      long long room = (long long)blocks_per_sm(threads) * sms / ((long long)s.slabs * cluster);
+      if (room < 1) room = 1;
+      const long long rounds = (p.N + room - 1) / room;
+      s.slices = int((p.N + rounds - 1) / rounds);
       return true;
     }
     if (k == 1) break;
@@ -645,6 +682,19 @@ bool image_plan(int dtype, const NormParams& p, bool backward, ImagePlan* plan) 
   return true;
 }
 
+template <typename T, int V, bool ONE, int R, int THREADS>
+cudaError_t run_forward(const Slab& s, cudaStream_t stream) {
+  static std::atomic<uint64_t> done;
+  auto* kernel = norm_images_kernel<T, V, ONE, R, THREADS>;
+  constexpr int kSmem = R * THREADS * Pack<T, V>::kBytes;
+  const cudaError_t e = allow_smem(kernel, kSmem, done);
+  if (e != cudaSuccess) return e;
+  // as many clusters as the SMs hold at once, or fewer that have equally many jobs each
+  const long long jobs = (long long)s.p.N * s.slabs, room = (long long)blocks_per_sm(THREADS) * current_sm_count() / s.cluster;
+  const long long rounds = (jobs + room - 1) / room, clusters = (jobs + rounds - 1) / rounds;
+  return launch_seq(kernel, dim3(unsigned(clusters * s.cluster)), THREADS, kSmem, s.cluster, stream, s);
+}
+
 template <typename T, int V, bool ONE>
 cudaError_t forward(ImagePlan& plan, cudaStream_t stream) {
   Slab& s = plan.s;
@@ -658,21 +708,21 @@ cudaError_t forward(ImagePlan& plan, cudaStream_t stream) {
     if (e != cudaSuccess) return e;
     return launch_seq(norm_split_apply_kernel<T, V, ONE>, dim3(unsigned(blocks)), kSplitThreads, 0, 1, stream, s);
   }
-  const long long blocks = (long long)p.N * s.slabs * s.cluster;
-  if (blocks > 0x7fffffffll) return cudaErrorInvalidConfiguration;
-  auto* kernel = plan.threads > 256 ? norm_images_kernel<T, V, ONE, 16, 512>
-                 : plan.R == 2      ? norm_images_kernel<T, V, ONE, 2, 256>
-                 : plan.R <= 8      ? norm_images_kernel<T, V, ONE, 8, 256>
-                                    : norm_images_kernel<T, V, ONE, 16, 256>;
-  return launch_seq(kernel, dim3(unsigned(blocks)), plan.threads, 0, s.cluster, stream, s);
+  if ((long long)p.N * s.slabs > 0x3fffffffll) return cudaErrorInvalidConfiguration;
+  return plan.threads > 256 ? run_forward<T, V, ONE, 16, 512>(s, stream)
+         : plan.R == 2      ? run_forward<T, V, ONE, 2, 256>(s, stream)
+         : plan.R <= 8      ? run_forward<T, V, ONE, 8, 256>(s, stream)
+                            : run_forward<T, V, ONE, 16, 256>(s, stream);
 }
 
 template <typename T, int V, bool ONE, int R, int THREADS>
 cudaError_t run_backward(const Slab& s, long long blocks, cudaStream_t stream) {
   static std::atomic<uint64_t> done;
   auto* kernel = norm_images_backward_kernel<T, V, ONE, R, THREADS>;
-  const int smem = BackwardShared::bytes(THREADS * V, s.channels);
-  const cudaError_t e = allow_smem(kernel, BackwardShared::bytes(THREADS * V, THREADS * V), done);
+  constexpr int kRing = 2 * R * THREADS * Pack<T, V>::kBytes;
+  const int smem = BackwardShared::bytes(THREADS * V, s.channels) + kRing;
+  const int most = BackwardShared::bytes(THREADS * V, THREADS * V) + kRing;
+  const cudaError_t e = allow_smem(kernel, most < kMostShared ? most : kMostShared, done);
   if (e != cudaSuccess) return e;
   return launch_seq(kernel, dim3(unsigned(blocks)), THREADS, smem, s.cluster, stream, s);
 }
@@ -702,7 +752,7 @@ cudaError_t backward(ImagePlan& plan, cudaStream_t stream) {
     e = run_split<T, V, ONE>(s, blocks, stream);
   } else {
     const long long blocks = (long long)s.slices * s.slabs * s.cluster;
-    e = plan.threads > 256 ? run_backward<T, V, ONE, 8, 512>(s, blocks, stream)
+    e = plan.threads > 256 ? (plan.R == 2 ? run_backward<T, V, ONE, 2, 512>(s, blocks, stream) : run_backward<T, V, ONE, 8, 512>(s, blocks, stream))
         : plan.R <= 2      ? run_backward<T, V, ONE, 2, 256>(s, blocks, stream)
         : plan.R == 4      ? run_backward<T, V, ONE, 4, 256>(s, blocks, stream)
                            : run_backward<T, V, ONE, 8, 256>(s, blocks, stream);

@@ -80,6 +80,11 @@ SHAPES = [   # shape, groups, layout
     ((2, 300, 9, 10), 1, "odd"),
     ((2, 1026, 3, 3), 2, "cl"),
     ((3, 700, 1, 1), 1, "odd"),
+    ((3, 4096, 1, 1), 1, "cl"),           # slabs as wide as they get
+    ((2, 4096, 3, 5), 8, "cl"),
+    ((2, 3968, 6, 6), 1, "cl"),
+    ((40, 64, 28, 28), 8, "cl"),          # several images to a cluster
+    ((700, 32, 4, 4), 4, "cl"),
     ((5, 96, 1, 1), 8, "cl"),             # one pixel
     ((2, 256, 1, 3), 32, "cl"),
     ((2, 48, 17), 6, "cl"),               # [N, C, L]
