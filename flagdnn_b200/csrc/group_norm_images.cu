@@ -27,35 +27,39 @@ struct Slab {
   int rows_at_once;      // rows that a block's threads cover
   int rows;              // of a block (cluster) or a piece (two launches)
   int slabs, cluster;
-  int slices;            // backward: clusters that share the images
+  int slices;            // clusters that share the images
   int pieces;
   float2* part;          // forward in two launches: [N, pieces, G] mean and squared deviations
   float2* sums;          // backward: rows of [C] sums of g xh and g
 };
 
-// A thread's place: a vector of channels and every rows_at_once-th row.
+// A thread's place: a vector of channels and every rows_at_once-th row.  (All that takes a division is taken once.)
 struct Place {
   int col, r, cc;        // column, first row, first channel within the slab
   int c0;                // the slab's first channel
   int here;              // channels of this slab (the last may have fewer)
+  int groups;            // and groups
   bool live;
-  __device__ Place(const Slab& s, int slab) {
-    col = threadIdx.x % s.cols;
-    r = threadIdx.x / s.cols;
-    cc = 0;
-    c0 = slab * s.channels;
-    here = min(s.channels, s.p.C - c0);
-    live = r < s.rows_at_once;
-  }
   template <int V>
-  __device__ void at() {
-    cc = col * V;
-    live = live && cc < here;
+  static __device__ Place of(const Slab& s, int slab) {
+    Place at;
+    at.r = int(threadIdx.x) / s.cols;
+    at.col = int(threadIdx.x) - at.r * s.cols;
+    at.cc = at.col * V;
+    at.c0 = slab * s.channels;
+    at.here = min(s.channels, s.p.C - at.c0);
+    at.groups = at.here / (s.p.C / s.p.G);
+    at.live = at.r < s.rows_at_once && at.cc < at.here;
+    return at;
   }
 };
 
-// Rows of a block's threads that its r-th row of threads has.
-__device__ __forceinline__ int rows_of(const Slab& s, int r, int rows) { return r < rows ? (rows - r - 1) / s.rows_at_once + 1 : 0; }
+// Rows that each of a block's rows of threads has: `each` of them, the first `more` one more.
+struct Rows {
+  int all, each, more;
+  __device__ Rows(const Slab& s, int rows) : all(rows), each(rows / s.rows_at_once), more(rows - each * s.rows_at_once) {}
+  __device__ int of(int r) const { return each + (r < more ? 1 : 0); }
+};
 
 // Mean and squared deviations of a block's rows by group, from registers: out[g] in shared memory.
 // A thread sums its values' distances from its own first one, and their squares, channel by channel: one pass, and what
@@ -63,9 +67,9 @@ __device__ __forceinline__ int rows_of(const Slab& s, int r, int rows) { return 
 // deviations, times the thread's rows. Threads and channels are joined by their means.  ONE (everywhere): the channels of a
 // vector are all of one group.
 template <typename T, int V, bool ONE, int R>
-__device__ __forceinline__ void local_moments(const Slab& s, const Place& at, const Pack<T, V> (&x)[R], int rows, float2* red,
+__device__ __forceinline__ void local_moments(const Slab& s, const Place& at, const Pack<T, V> (&x)[R], const Rows& rows, float2* red,
                                               float2* out) {
-  const int cpg = s.p.C / s.p.G, count = at.live ? rows_of(s, at.r, rows) : 0;
+  const int cpg = s.p.C / s.p.G, count = at.live ? rows.of(at.r) : 0;
   constexpr int P = Pack<T, V>::kPairs;
   F2 sum[P], square[P];
 #pragma unroll
@@ -81,7 +85,7 @@ __device__ __forceinline__ void local_moments(const Slab& s, const Place& at, co
       }
     }
   if (at.r < s.rows_at_once) {
-    const float inv = count > 0 ? 1.0f / float(count) : 0.0f;
+    const float inv = count > 0 ? __fdividef(1.0f, float(count)) : 0.0f;
     float mean[2 * P], m2[2 * P];
 #pragma unroll
     for (int i = 0; i < P; ++i) {
@@ -109,24 +113,27 @@ __device__ __forceinline__ void local_moments(const Slab& s, const Place& at, co
     }
   }
   __syncthreads();
-  const int pitch = ONE ? s.cols : s.channels, per = cpg / (ONE ? V : 1), groups = at.here / cpg, lane = threadIdx.x & 31;
+  // a warp takes a group: the mean of its threads' means first, then their deviations from it
+  const int pitch = ONE ? s.cols : s.channels, per = cpg / (ONE ? V : 1), lane = threadIdx.x & 31;
   const int entries = s.rows_at_once * per;
-  const float part = 1.0f / float(per);
-  for (int g = threadIdx.x >> 5; g < groups; g += blockDim.x >> 5) {
-    Moments all{0.0f, 0.0f, 0.0f};
+  const float part = __fdividef(1.0f, float(per)), inv = __fdividef(1.0f, float(rows.all) * float(cpg)), each = ONE ? V : 1;
+  for (int g = threadIdx.x >> 5; g < at.groups; g += blockDim.x >> 5) {
+    const float2* from = red + g * per;
+    const float first = from[0].x;
+    float t = 0.0f;
     for (int i = lane; i < entries; i += 32) {
-      const int row = int((float(i) + 0.5f) * part);   // i / per: exact for the few thousand entries there are
-      const float n = float(rows_of(s, row, rows) * (ONE ? V : 1));
-      const float2 v = red[row * pitch + g * per + i - row * per];
-      if (n > 0.0f) all = joined(all, Moments{n, v.x, v.y});
+      const int row = per == 1 ? i : int((float(i) + 0.5f) * part);   // i / per: exact for the few thousand entries there are
+      t += float(rows.of(row)) * (rows.of(row) > 0 ? from[row * pitch + i - row * per].x - first : 0.0f);
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      const Moments other{__shfl_down_sync(0xffffffffu, all.n, o), __shfl_down_sync(0xffffffffu, all.mean, o),
-                          __shfl_down_sync(0xffffffffu, all.m2, o)};
-      if (other.n > 0.0f) all = joined(all, other);
+    const float mean = first + warp_sum(t) * each * inv;
+    t = 0.0f;
+    for (int i = lane; i < entries; i += 32) {
+      const int row = per == 1 ? i : int((float(i) + 0.5f) * part);
+      const float2 v = from[row * pitch + i - row * per];
+      if (rows.of(row) > 0) t += v.y + float(rows.of(row)) * each * (v.x - mean) * (v.x - mean);
     }
-    if (lane == 0) out[g] = make_float2(all.mean, all.m2);
+    t = warp_sum(t);
+    if (lane == 0) out[g] = make_float2(mean, t);
   }
   __syncthreads();
 }
@@ -141,74 +148,91 @@ norm_images_kernel(const Slab s) {
   __shared__ float2 red[ONE ? THREADS : THREADS * V];
   __shared__ float2 own[kMaxGroups], all_of[kMaxGroups];   // mean and squared deviations; mean and 1 / deviation
   constexpr int M = ONE ? 1 : Pack<T, V>::kPairs, P = Pack<T, V>::kPairs;
-  Pack<T, V>* next = reinterpret_cast<Pack<T, V>*>(raw) + threadIdx.x;   // this thread's rows of the next job, THREADS apart
+  Pack<T, V>* next = reinterpret_cast<Pack<T, V>*>(raw) + threadIdx.x;   // this thread's rows of the next image, THREADS apart
   chained();
   const NormParams& p = s.p;
   const cg::cluster_group cluster = cg::this_cluster();
-  const int rank = blockIdx.x % s.cluster, jobs = p.N * s.slabs, cpg = p.C / p.G;
-  const int row0 = rank * s.rows, rows = max(0, min(s.rows, s.S - row0));
+  const int rank = blockIdx.x % s.cluster, job = blockIdx.x / s.cluster, slab = job % s.slabs, slice = job / s.slabs;
+  const int row0 = rank * s.rows, cpg = p.C / p.G;
+  const Rows rows(s, max(0, min(s.rows, s.S - row0)));
+  const Place at = Place::of<V>(s, slab);
+  const int count = at.live ? rows.of(at.r) : 0, c = at.c0 + at.cc, g0 = at.c0 / cpg;
   const long long pixel = p.W > 1 ? p.x_s[3] : p.x_s[2], out_pixel = p.W > 1 ? p.y_s[3] : p.y_s[2];
-  auto fetch = [&](int job) {
-    if (job < jobs) {
-      const int slab = job % s.slabs, n = job / s.slabs;
-      Place at(s, slab);
-      at.at<V>();
-      const int count = at.live ? rows_of(s, at.r, rows) : 0;
-      const T* x0 = static_cast<const T*>(p.x) + (at.live ? n * p.x_s[0] + at.c0 + at.cc + (long long)(row0 + at.r) * pixel : 0);
+  const T* x0 = static_cast<const T*>(p.x) + (count > 0 ? c + (long long)(row0 + at.r) * pixel : 0);
+  T* y0 = static_cast<T*>(p.y) + (count > 0 ? c + (long long)(row0 + at.r) * out_pixel : 0);
+  const long long x_step = s.rows_at_once * pixel, y_step = s.rows_at_once * out_pixel;
+  int group[M][2];                                  // of a pair's two channels, within the slab
 #pragma unroll
-      for (int k = 0; k < R; ++k)
-        async_load(next + k * THREADS, k < count ? x0 + k * s.rows_at_once * pixel : static_cast<const T*>(p.x), k < count);
+  for (int i = 0; i < M; ++i) {
+    group[i][0] = at.live ? (at.cc + (ONE ? 0 : 2 * i)) / cpg : 0;
+    group[i][1] = ONE || !at.live ? group[i][0] : (at.cc + min(2 * i + 1, V - 1)) / cpg;
+  }
+  F2 w[P], b[P];
+  norm_params_of<T, V>(p, c, at.live, w, b);
+  auto fetch = [&](int n) {
+    if (n < p.N) {
+      const T* from = x0 + (count > 0 ? n * p.x_s[0] : 0);
+#pragma unroll
+      for (int k = 0; k < R; ++k) {
+        async_load(next + k * THREADS, from, k < count);
+        if (k + 1 < count) from += x_step;
+      }
     }
     async_commit();
   };
-  const int clusters = gridDim.x / s.cluster;
-  fetch(blockIdx.x / s.cluster);
-  for (int job = blockIdx.x / s.cluster; job < jobs; job += clusters) {
-    const int slab = job % s.slabs, n = job / s.slabs;
-    Place at(s, slab);
-    at.at<V>();
+  fetch(slice);
+  for (int n = slice; n < p.N; n += s.slices) {
     Pack<T, V> x[R];
     async_wait<0>();
 #pragma unroll
     for (int k = 0; k < R; ++k) x[k] = next[k * THREADS];
-    fetch(job + clusters);
+    fetch(n + s.slices);
     local_moments<T, V, ONE>(s, at, x, rows, red, own);
     if (s.cluster > 1) cluster.sync();
-    const int g0 = at.c0 / cpg;
-    for (int g = threadIdx.x; g < at.here / cpg; g += THREADS) {
-      Moments all{0.0f, 0.0f, 0.0f};
-      for (int q = 0; q < s.cluster; ++q) {
-        const float count = float(max(0, min(s.rows, s.S - q * s.rows))) * float(cpg);
-        const float2 v = (s.cluster > 1 ? cluster.map_shared_rank(own, q) : own)[g];
-        if (count > 0.0f) all = joined(all, Moments{count, v.x, v.y});
+    for (int g = threadIdx.x; g < at.groups; g += THREADS) {
+      float2 all = own[g];
+      if (s.cluster > 1) {
+        float2 v[8];
+        float n_of[8], t = 0.0f;
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+          n_of[q] = q < s.cluster ? float(max(0, min(s.rows, s.S - q * s.rows))) * float(cpg) : 0.0f;
+          v[q] = n_of[q] > 0.0f ? cluster.map_shared_rank(own, q)[g] : make_float2(0.0f, 0.0f);
+        }
+        const float inv = __fdividef(1.0f, float(s.S) * float(cpg));
+#pragma unroll
+        for (int q = 1; q < 8; ++q) t += n_of[q] > 0.0f ? n_of[q] * (v[q].x - v[0].x) : 0.0f;
+        all = make_float2(v[0].x + t * inv, 0.0f);
+#pragma unroll
+        for (int q = 0; q < 8; ++q) all.y += n_of[q] > 0.0f ? v[q].y + n_of[q] * (v[q].x - all.x) * (v[q].x - all.x) : 0.0f;
       }
-      const float rstd = rsqrtf(all.m2 / all.n + p.eps);
-      all_of[g] = make_float2(all.mean, rstd);
+      const float rstd = rsqrtf(all.y / (float(s.S) * float(cpg)) + p.eps);
+      all_of[g] = make_float2(all.x, rstd);
       if (p.mean != nullptr && rank == 0) {
-        p.mean[(long long)n * p.G + g0 + g] = all.mean;
+        p.mean[(long long)n * p.G + g0 + g] = all.x;
         p.rstd[(long long)n * p.G + g0 + g] = rstd;
       }
     }
     if (s.cluster > 1) cluster.barrier_arrive();   // this block has read the others' moments
     __syncthreads();
-    F2 w[P], b[P], m[M];                              // m: minus the mean
-    norm_params_of<T, V>(p, at.c0 + at.cc, at.live, w, b);
+    F2 m[M], scale[P];                                // m: minus the mean
 #pragma unroll
     for (int i = 0; i < P; ++i) {
-      const float2 lo = all_of[at.live ? (at.cc + (ONE ? 0 : 2 * i)) / cpg : 0];
-      const float2 hi = ONE ? lo : all_of[at.live ? (at.cc + min(2 * i + 1, V - 1)) / cpg : 0];
+      const float2 lo = all_of[group[ONE ? 0 : i][0]], hi = ONE ? lo : all_of[group[ONE ? 0 : i][1]];
       m[ONE ? 0 : i] = f2_pack(-lo.x, -hi.x);
-      w[i] = f2_mul(w[i], f2_pack(lo.y, hi.y));
+      scale[i] = f2_mul(w[i], f2_pack(lo.y, hi.y));
     }
-    T* y0 = static_cast<T*>(p.y) + n * p.y_s[0] + at.c0 + at.cc + (long long)(row0 + at.r) * out_pixel;
+    T* to = y0 + (count > 0 ? n * p.y_s[0] : 0);
     with_activation(p.act, [&](auto act) {
 #pragma unroll
       for (int k = 0; k < R; ++k)
-        if (at.live && at.r + k * s.rows_at_once < rows) {
+        if (k < count) {
           Pack<T, V> y;
 #pragma unroll
-          for (int i = 0; i < P; ++i) y.set_pair(i, activate2<decltype(act)::value>(f2_fma(f2_add(x[k].pair(i), m[ONE ? 0 : i]), w[i], b[i])));
-          y.store(y0 + k * s.rows_at_once * out_pixel);
+          for (int i = 0; i < P; ++i)
+            y.set_pair(i, activate2<decltype(act)::value>(f2_fma(f2_add(x[k].pair(i), m[ONE ? 0 : i]), scale[i], b[i])));
+          y.store(to);
+          to += y_step;
         }
     });
     if (s.cluster > 1) cluster.barrier_wait();     // and the others have read this one's
@@ -291,27 +315,38 @@ norm_images_backward_kernel(const Slab s) {
   const NormParams& p = s.p;
   const cg::cluster_group cluster = cg::this_cluster();
   const int rank = blockIdx.x % s.cluster, job = blockIdx.x / s.cluster, slab = job % s.slabs, slice = job / s.slabs;
-  const int row0 = rank * s.rows, rows = max(0, min(s.rows, s.S - row0)), cpg = p.C / p.G;
-  Place at(s, slab);
-  at.at<V>();
+  const int row0 = rank * s.rows, cpg = p.C / p.G;
+  const Rows rows(s, max(0, min(s.rows, s.S - row0)));
+  const Place at = Place::of<V>(s, slab);
   const bool tall = p.W > 1;
   const long long px = tall ? p.x_s[3] : p.x_s[2], pdy = tall ? p.dy_s[3] : p.dy_s[2], pdx = tall ? p.dx_s[3] : p.dx_s[2];
-  const int c = at.c0 + at.cc, first = row0 + at.r;
+  const int c = at.c0 + at.cc, first = row0 + at.r, g0 = at.c0 / cpg;
   constexpr int P = Pack<T, V>::kPairs;
   F2 w[P], b[P];
   norm_params_of<T, V>(p, c, at.live, w, b);
+  int group[M][2];                                  // of a pair's two channels, within the slab
+#pragma unroll
+  for (int i = 0; i < M; ++i) {
+    group[i][0] = at.live ? (at.cc + (ONE ? 0 : 2 * i)) / cpg : 0;
+    group[i][1] = ONE || !at.live ? group[i][0] : (at.cc + min(2 * i + 1, V - 1)) / cpg;
+  }
   for (int i = threadIdx.x; i < s.channels; i += THREADS) sh.acc[i] = make_float2(0.0f, 0.0f);
   // this thread's rows of the next image, THREADS apart: x, then dy
   Pack<T, V>* next = reinterpret_cast<Pack<T, V>*>(raw + BackwardShared::bytes(THREADS * V, s.channels)) + threadIdx.x;
-  const int count = at.live ? rows_of(s, at.r, rows) : 0;
+  const int count = at.live ? rows.of(at.r) : 0;
+  const long long x_step = s.rows_at_once * px, dy_step = s.rows_at_once * pdy, dx_step = s.rows_at_once * pdx;
   auto fetch = [&](int n) {
     if (n < p.N) {
-      const T* x0 = static_cast<const T*>(p.x) + (at.live ? n * p.x_s[0] + c + first * px : 0);
-      const T* dy0 = static_cast<const T*>(p.dy) + (at.live ? n * p.dy_s[0] + c + first * pdy : 0);
+      const T* x0 = static_cast<const T*>(p.x) + (count > 0 ? n * p.x_s[0] + c + first * px : 0);
+      const T* dy0 = static_cast<const T*>(p.dy) + (count > 0 ? n * p.dy_s[0] + c + first * pdy : 0);
 #pragma unroll
       for (int k = 0; k < R; ++k) {
-        async_load(next + k * THREADS, k < count ? x0 + k * s.rows_at_once * px : static_cast<const T*>(p.x), k < count);
-        async_load(next + (R + k) * THREADS, k < count ? dy0 + k * s.rows_at_once * pdy : static_cast<const T*>(p.dy), k < count);
+        async_load(next + k * THREADS, x0, k < count);
+        async_load(next + (R + k) * THREADS, dy0, k < count);
+        if (k + 1 < count) {
+          x0 += x_step;
+          dy0 += dy_step;
+        }
       }
     }
     async_commit();
@@ -329,8 +364,7 @@ norm_images_backward_kernel(const Slab s) {
     F2 mean[M], rstd[M], gx[P], gs[P];               // mean: minus the mean
 #pragma unroll
     for (int i = 0; i < M; ++i) {
-      const long long lo = (long long)n * p.G + (at.live ? (c + 2 * i) / cpg : 0);
-      const long long hi = ONE ? lo : (long long)n * p.G + (at.live ? (c + min(2 * i + 1, V - 1)) / cpg : 0);
+      const long long lo = (long long)n * p.G + g0 + group[i][0], hi = (long long)n * p.G + g0 + group[i][1];
       mean[i] = f2_pack(-p.mean[lo], -p.mean[hi]);
       rstd[i] = f2_pack(p.rstd[lo], p.rstd[hi]);
     }
@@ -339,7 +373,7 @@ norm_images_backward_kernel(const Slab s) {
     with_activation(p.act, [&](auto act) {
 #pragma unroll
       for (int k = 0; k < R; ++k)
-        if (at.live && at.r + k * s.rows_at_once < rows) {
+        if (k < count) {
 #pragma unroll
           for (int i = 0; i < P; ++i) {
             const F2 xh = f2_mul(f2_add(x[k].pair(i), mean[ONE ? 0 : i]), rstd[ONE ? 0 : i]);
@@ -371,16 +405,15 @@ norm_images_backward_kernel(const Slab s) {
       F2 s1[M], s2[M];                               // minus s1 / m, minus s2 / m
 #pragma unroll
       for (int i = 0; i < M; ++i) {
-        const float2 lo = sh.means[at.live ? (at.cc + 2 * i) / cpg : 0];
-        const float2 hi = ONE ? lo : sh.means[at.live ? (at.cc + min(2 * i + 1, V - 1)) / cpg : 0];
+        const float2 lo = sh.means[group[i][0]], hi = sh.means[group[i][1]];
         s1[i] = f2_pack(-lo.x, -hi.x);
         s2[i] = f2_pack(-lo.y, -hi.y);
       }
-      T* dx0 = static_cast<T*>(p.dx) + n * p.dx_s[0] + c + first * pdx;
+      T* dx0 = static_cast<T*>(p.dx) + (count > 0 ? n * p.dx_s[0] + c + first * pdx : 0);
       with_activation(p.act, [&](auto act) {
 #pragma unroll
         for (int k = 0; k < R; ++k)
-          if (at.live && at.r + k * s.rows_at_once < rows) {
+          if (k < count) {
             Pack<T, V> dx;
 #pragma unroll
             for (int i = 0; i < P; ++i) {
@@ -388,7 +421,8 @@ norm_images_backward_kernel(const Slab s) {
               const F2 g = f2_mul(dy[k].pair(i), slope2<decltype(act)::value>(f2_fma(xh, w[i], b[i])));
               dx.set_pair(i, f2_mul(rstd[ONE ? 0 : i], f2_fma(xh, s2[ONE ? 0 : i], f2_fma(g, w[i], s1[ONE ? 0 : i]))));
             }
-            dx.store(dx0 + k * s.rows_at_once * pdx);
+            dx.store(dx0);
+            dx0 += dx_step;
           }
       });
     }
@@ -412,25 +446,24 @@ norm_split_stats_kernel(const Slab s) {
   const NormParams& p = s.p;
   const int piece = blockIdx.x % s.pieces, job = blockIdx.x / s.pieces, slab = job % s.slabs, n = job / s.slabs;
   const int row0 = piece * s.rows, end = min(s.S, row0 + s.rows), cpg = p.C / p.G;
-  Place at(s, slab);
-  at.at<V>();
+  const Place at = Place::of<V>(s, slab);
   const long long pixel = p.W > 1 ? p.x_s[3] : p.x_s[2];
-  for (int g = threadIdx.x; g < at.here / cpg; g += kSplitThreads) all[g] = Moments{0.0f, 0.0f, 0.0f};
+  for (int g = threadIdx.x; g < at.groups; g += kSplitThreads) all[g] = Moments{0.0f, 0.0f, 0.0f};
   for (int r0 = row0; r0 < end; r0 += kSplitRows * s.rows_at_once) {
-    const int rows = min(end - r0, kSplitRows * s.rows_at_once);
+    const Rows rows(s, min(end - r0, kSplitRows * s.rows_at_once));
     const T* x0 = static_cast<const T*>(p.x) + n * p.x_s[0] + at.c0 + at.cc + (long long)(r0 + at.r) * pixel;
     Pack<T, V> x[kSplitRows];
 #pragma unroll
     for (int k = 0; k < kSplitRows; ++k) {
       x[k].clear();
-      if (at.live && at.r + k * s.rows_at_once < rows) x[k].load(x0 + k * s.rows_at_once * pixel);
+      if (at.live && k < rows.of(at.r)) x[k].load(x0 + k * s.rows_at_once * pixel);
     }
     local_moments<T, V, ONE>(s, at, x, rows, red, own);
-    for (int g = threadIdx.x; g < at.here / cpg; g += kSplitThreads)
-      all[g] = joined(all[g], Moments{float(rows) * float(cpg), own[g].x, own[g].y});
+    for (int g = threadIdx.x; g < at.groups; g += kSplitThreads)
+      all[g] = joined(all[g], Moments{float(rows.all) * float(cpg), own[g].x, own[g].y});
     __syncthreads();
   }
-  for (int g = threadIdx.x; g < at.here / cpg; g += kSplitThreads)
+  for (int g = threadIdx.x; g < at.groups; g += kSplitThreads)
     s.part[((long long)n * s.pieces + piece) * p.G + at.c0 / cpg + g] = make_float2(all[g].mean, all[g].m2);
 }
 
@@ -443,10 +476,9 @@ norm_split_apply_kernel(const Slab s) {
   const NormParams& p = s.p;
   const int piece = blockIdx.x % s.pieces, job = blockIdx.x / s.pieces, slab = job % s.slabs, n = job / s.slabs;
   const int row0 = piece * s.rows, end = min(s.S, row0 + s.rows), cpg = p.C / p.G;
-  Place at(s, slab);
-  at.at<V>();
+  const Place at = Place::of<V>(s, slab);
   const int g0 = at.c0 / cpg;
-  for (int g = threadIdx.x; g < at.here / cpg; g += kSplitThreads) {
+  for (int g = threadIdx.x; g < at.groups; g += kSplitThreads) {
     Moments all{0.0f, 0.0f, 0.0f};
     for (int q = 0; q < s.pieces; ++q) {
       const float2 v = s.part[((long long)n * s.pieces + q) * p.G + g0 + g];
@@ -496,8 +528,7 @@ norm_split_sums_kernel(const Slab s) {
   const NormParams& p = s.p;
   const int piece = blockIdx.x % s.pieces, job = blockIdx.x / s.pieces, slab = job % s.slabs, n = job / s.slabs;
   const int row0 = piece * s.rows, end = min(s.S, row0 + s.rows), cpg = p.C / p.G;
-  Place at(s, slab);
-  at.at<V>();
+  const Place at = Place::of<V>(s, slab);
   const long long px = p.W > 1 ? p.x_s[3] : p.x_s[2], pdy = p.W > 1 ? p.dy_s[3] : p.dy_s[2];
   const int c = at.c0 + at.cc;
   constexpr int P = Pack<T, V>::kPairs;
@@ -545,8 +576,7 @@ norm_split_dx_kernel(const Slab s) {
   const NormParams& p = s.p;
   const int piece = blockIdx.x % s.pieces, job = blockIdx.x / s.pieces, slab = job % s.slabs, n = job / s.slabs;
   const int row0 = piece * s.rows, end = min(s.S, row0 + s.rows), cpg = p.C / p.G;
-  Place at(s, slab);
-  at.at<V>();
+  const Place at = Place::of<V>(s, slab);
   for (int i = threadIdx.x; i < at.here; i += kSplitThreads) {
     float2 t = make_float2(0.0f, 0.0f);
     for (int q = 0; q < s.pieces; ++q) {
@@ -660,7 +690,7 @@ bool image_plan(int dtype, const NormParams& p, bool backward, ImagePlan* plan) 
       if (backward && BackwardShared::bytes(threads * V, s.channels) + 2 * plan->R * threads * 16 > kMostShared) continue;
       s.cluster = cluster;
       s.rows = int((S + cluster - 1) / cluster);
-      // backward: as many clusters as the SMs hold at once, or fewer that have equally many images each
+      // as many clusters as the SMs hold at once, or fewer that have equally many images each
       long long room = (long long)blocks_per_sm(threads) * sms / ((long long)s.slabs * cluster);
       if (room < 1) room = 1;
       const long long rounds = (p.N + room - 1) / room;
@@ -689,10 +719,7 @@ cudaError_t run_forward(const Slab& s, cudaStream_t stream) {
   constexpr int kSmem = R * THREADS * Pack<T, V>::kBytes;
   const cudaError_t e = allow_smem(kernel, kSmem, done);
   if (e != cudaSuccess) return e;
-  // as many clusters as the SMs hold at once, or fewer that have equally many jobs each
-  const long long jobs = (long long)s.p.N * s.slabs, room = (long long)blocks_per_sm(THREADS) * current_sm_count() / s.cluster;
-  const long long rounds = (jobs + room - 1) / room, clusters = (jobs + rounds - 1) / rounds;
-  return launch_seq(kernel, dim3(unsigned(clusters * s.cluster)), THREADS, kSmem, s.cluster, stream, s);
+  return launch_seq(kernel, dim3(unsigned((long long)s.slices * s.slabs * s.cluster)), THREADS, kSmem, s.cluster, stream, s);
 }
 
 template <typename T, int V, bool ONE>
@@ -708,7 +735,6 @@ cudaError_t forward(ImagePlan& plan, cudaStream_t stream) {
     if (e != cudaSuccess) return e;
     return launch_seq(norm_split_apply_kernel<T, V, ONE>, dim3(unsigned(blocks)), kSplitThreads, 0, 1, stream, s);
   }
-  if ((long long)p.N * s.slabs > 0x3fffffffll) return cudaErrorInvalidConfiguration;
   return plan.threads > 256 ? run_forward<T, V, ONE, 16, 512>(s, stream)
          : plan.R == 2      ? run_forward<T, V, ONE, 2, 256>(s, stream)
          : plan.R <= 8      ? run_forward<T, V, ONE, 8, 256>(s, stream)
