@@ -310,11 +310,11 @@ template cudaError_t launch_norm_dparams<float>(const NormParams&, const float2*
 // Known without the tensors' addresses: the most that any kernel which may take the problem needs.
 long long group_norm_workspace(int dtype, const NormParams& p, bool backward) {
   const long long here = 8ll * p.N * (backward ? p.C : p.G * chunks_of(p).count);
-  if (!norm_rows(p, backward) || p.C / p.G > 512 || (long long)p.H * p.W > (1 << 29)) return here;
+  if (!norm_rows(p, backward) || (long long)p.H * p.W > 0x1fffffff) return here;
   const long long images = norm_images_workspace(dtype, p, backward);
   const long long tokens = p.H == 1 && p.W == 1 ? norm_tokens_workspace(dtype, p, backward) : 0;
-  // images of groups that may be wider than the 256 threads of their two-launch form
-  const long long wide = p.C / p.G > 256 && (long long)p.H * p.W > 64 ? here : 0;
+  // groups that may be wider than a block of the images' kernels has threads
+  const long long wide = p.C / p.G > 256 ? here : 0;
   const long long most = tokens > images ? tokens : images;
   return most > wide ? most : wide;
 }

@@ -1,12 +1,16 @@
 // Group norm over channels-last images, and over rows of tokens whose groups do not fit a warp.
 //
 // Bound by memory: x is read once and y written once, so a group's values have to stay on chip between the statistics and the
-// last pass. They stay in registers: a cluster of up to eight blocks holds all pixels of a slab of neighbouring groups (rows of
-// about 128 bytes), up to sixteen vectors of 16 bytes a thread, loaded at once. Mean first and deviations from it second, both
-// from registers; the blocks' means and squared deviations are joined over distributed shared memory. The gradient holds x and
-// dy the same way, sums g xh and g per channel, and joins those.
+// last pass. They stay in shared memory: a cluster of up to eight blocks holds all pixels of a slab of neighbouring groups (rows
+// of about 64 bytes). Every thread copies its own rows there asynchronously and nobody else reads them, so that nothing waits
+// for anything but sums; as soon as a row has gone through the last pass, the next image's row is on its way into its place.
+// The sums are taken in one pass (see local_moments) and joined over the block and, by distributed shared memory, the cluster.
+// The gradient holds x and dy the same way, sums g xh and g per channel, and joins those.
 //
-// Slabs that no cluster holds (a 16-bit group of more than half a million values) go in two launches, which read x twice.
+// (With the rows in registers, sixteen vectors a thread and copies a buffer ahead, the same took 37 us on 32 x 256 x 56 x 56 bf16:
+// two blocks an SM, and unrolled code that the instruction cache did not hold.)
+//
+// Slabs that no cluster holds go in two launches, which read x twice.
 #include <cooperative_groups.h>
 
 #include "group_norm.cuh"
@@ -18,7 +22,7 @@ namespace cg = cooperative_groups;
 
 constexpr int kMaxChunks = 64;        // pieces of an image in two launches
 constexpr int kMaxGroups = 512;       // of a slab
-constexpr int kMostShared = 220 * 1024;
+constexpr int kMostShared = 224 * 1024, kSharedOfSm = 228 * 1024;
 
 struct Slab {
   NormParams p;
@@ -27,6 +31,7 @@ struct Slab {
   int rows_at_once;      // rows that a block's threads cover
   int rows;              // of a block (cluster) or a piece (two launches)
   int slabs, cluster;
+  int held;              // rows of a thread
   int slices;            // clusters that share the images
   int pieces;
   float2* part;          // forward in two launches: [N, pieces, G] mean and squared deviations
@@ -66,24 +71,29 @@ struct Rows {
 // the squares lose to a first value far from the others is less than 2^-24 of that value's own share of the group's squared
 // deviations, times the thread's rows. Threads and channels are joined by their means.  ONE (everywhere): the channels of a
 // vector are all of one group.
-template <typename T, int V, bool ONE, int R>
-__device__ __forceinline__ void local_moments(const Slab& s, const Place& at, const Pack<T, V> (&x)[R], const Rows& rows, float2* red,
-                                              float2* out) {
+template <typename T, int V, bool ONE, typename F>
+__device__ __forceinline__ void local_moments(const Slab& s, const Place& at, F&& row, const Rows& rows, float2* red, float2* out) {
   const int cpg = s.p.C / s.p.G, count = at.live ? rows.of(at.r) : 0;
   constexpr int P = Pack<T, V>::kPairs;
-  F2 sum[P], square[P];
+  F2 sum[P], square[P], minus[P];
+  Pack<T, V> x0;
+  x0.clear();
+  if (count > 0) x0 = row(0);
 #pragma unroll
-  for (int i = 0; i < P; ++i) sum[i] = square[i] = 0;
+  for (int i = 0; i < P; ++i) {
+    sum[i] = square[i] = 0;
+    minus[i] = f2_mul(x0.pair(i), f2_both(-1.0f));
+  }
+#pragma unroll 4
+  for (int k = 1; k < count; ++k) {
+    const Pack<T, V> x = row(k);
 #pragma unroll
-  for (int k = 1; k < R; ++k)
-    if (k < count) {
-#pragma unroll
-      for (int i = 0; i < P; ++i) {
-        const F2 d = f2_fma(x[0].pair(i), f2_both(-1.0f), x[k].pair(i));
-        sum[i] = f2_add(sum[i], d);
-        square[i] = f2_fma(d, d, square[i]);
-      }
+    for (int i = 0; i < P; ++i) {
+      const F2 d = f2_add(x.pair(i), minus[i]);
+      sum[i] = f2_add(sum[i], d);
+      square[i] = f2_fma(d, d, square[i]);
     }
+  }
   if (at.r < s.rows_at_once) {
     const float inv = count > 0 ? __fdividef(1.0f, float(count)) : 0.0f;
     float mean[2 * P], m2[2 * P];
@@ -92,7 +102,7 @@ __device__ __forceinline__ void local_moments(const Slab& s, const Place& at, co
       float a[2], q[2], first[2];
       f2_split(sum[i], a[0], a[1]);
       f2_split(square[i], q[0], q[1]);
-      f2_split(x[0].pair(i), first[0], first[1]);
+      f2_split(x0.pair(i), first[0], first[1]);
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         mean[2 * i + j] = first[j] + a[j] * inv;
@@ -138,17 +148,24 @@ __device__ __forceinline__ void local_moments(const Slab& s, const Place& at, co
   __syncthreads();
 }
 
-// Blocks of THREADS that share an SM.
-constexpr int blocks_per_sm(int threads) { return threads > 256 ? 1 : 2; }
+constexpr int kThreads = 256;
 
-template <typename T, int V, bool ONE, int R, int THREADS>
-__global__ void __launch_bounds__(THREADS, blocks_per_sm(THREADS))
+// The cluster's barrier, after a __syncthreads(): what the block's threads wrote (or read) before that is ordered by the first
+// warp's release; a fence in each of the others would cost as much again and order nothing more.
+__device__ __forceinline__ void cluster_arrive() {
+  if (threadIdx.x < 32) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  else asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+
+template <typename T, int V, bool ONE>
+__global__ void __launch_bounds__(kThreads, 3)
 norm_images_kernel(const Slab s) {
   extern __shared__ __align__(16) unsigned char raw[];
-  __shared__ float2 red[ONE ? THREADS : THREADS * V];
+  __shared__ float2 red[ONE ? kThreads : kThreads * V];
   __shared__ float2 own[kMaxGroups], all_of[kMaxGroups];   // mean and squared deviations; mean and 1 / deviation
   constexpr int M = ONE ? 1 : Pack<T, V>::kPairs, P = Pack<T, V>::kPairs;
-  Pack<T, V>* next = reinterpret_cast<Pack<T, V>*>(raw) + threadIdx.x;   // this thread's rows of the next image, THREADS apart
+  Pack<T, V>* held = reinterpret_cast<Pack<T, V>*>(raw) + threadIdx.x;   // this thread's rows, kThreads apart
   chained();
   const NormParams& p = s.p;
   const cg::cluster_group cluster = cg::this_cluster();
@@ -169,27 +186,19 @@ norm_images_kernel(const Slab s) {
   }
   F2 w[P], b[P];
   norm_params_of<T, V>(p, c, at.live, w, b);
-  auto fetch = [&](int n) {
-    if (n < p.N) {
-      const T* from = x0 + (count > 0 ? n * p.x_s[0] : 0);
-#pragma unroll
-      for (int k = 0; k < R; ++k) {
-        async_load(next + k * THREADS, from, k < count);
-        if (k + 1 < count) from += x_step;
-      }
-    }
-    async_commit();
-  };
-  fetch(slice);
+  if (slice < p.N) {
+    const T* from = x0 + (count > 0 ? slice * p.x_s[0] : 0);
+    for (int k = 0; k < count; ++k) async_load(held + k * kThreads, from + k * x_step, true);
+  }
   for (int n = slice; n < p.N; n += s.slices) {
-    Pack<T, V> x[R];
+    async_commit();
     async_wait<0>();
-#pragma unroll
-    for (int k = 0; k < R; ++k) x[k] = next[k * THREADS];
-    fetch(n + s.slices);
-    local_moments<T, V, ONE>(s, at, x, rows, red, own);
-    if (s.cluster > 1) cluster.sync();
-    for (int g = threadIdx.x; g < at.groups; g += THREADS) {
+    local_moments<T, V, ONE>(s, at, [&](int k) { return held[k * kThreads]; }, rows, red, own);
+    if (s.cluster > 1) {
+      cluster_arrive();
+      cluster_wait();
+    }
+    for (int g = threadIdx.x; g < at.groups; g += kThreads) {
       float2 all = own[g];
       if (s.cluster > 1) {
         float2 v[8];
@@ -213,8 +222,8 @@ norm_images_kernel(const Slab s) {
         p.rstd[(long long)n * p.G + g0 + g] = rstd;
       }
     }
-    if (s.cluster > 1) cluster.barrier_arrive();   // this block has read the others' moments
     __syncthreads();
+    if (s.cluster > 1) cluster_arrive();           // this block has read the others' moments
     F2 m[M], scale[P];                                // m: minus the mean
 #pragma unroll
     for (int i = 0; i < P; ++i) {
@@ -223,19 +232,21 @@ norm_images_kernel(const Slab s) {
       scale[i] = f2_mul(w[i], f2_pack(lo.y, hi.y));
     }
     T* to = y0 + (count > 0 ? n * p.y_s[0] : 0);
+    const bool more = n + s.slices < p.N;
+    const T* from = x0 + (count > 0 && more ? (n + s.slices) * p.x_s[0] : 0);
     with_activation(p.act, [&](auto act) {
+#pragma unroll 4
+      for (int k = 0; k < count; ++k) {
+        const Pack<T, V> x = held[k * kThreads];
+        Pack<T, V> y;
 #pragma unroll
-      for (int k = 0; k < R; ++k)
-        if (k < count) {
-          Pack<T, V> y;
-#pragma unroll
-          for (int i = 0; i < P; ++i)
-            y.set_pair(i, activate2<decltype(act)::value>(f2_fma(f2_add(x[k].pair(i), m[ONE ? 0 : i]), scale[i], b[i])));
-          y.store(to);
-          to += y_step;
-        }
+        for (int i = 0; i < P; ++i)
+          y.set_pair(i, activate2<decltype(act)::value>(f2_fma(f2_add(x.pair(i), m[ONE ? 0 : i]), scale[i], b[i])));
+        y.store(to + k * y_step);
+        if (more) async_load(held + k * kThreads, from + k * x_step, true);
+      }
     });
-    if (s.cluster > 1) cluster.barrier_wait();     // and the others have read this one's
+    if (s.cluster > 1) cluster_wait();             // and the others have read this one's
   }
 }
 
@@ -305,11 +316,11 @@ struct BackwardShared {
   static __host__ __device__ int bytes(int entries, int channels) { return (8 * (entries + 3 * channels + kMaxGroups) + 15) / 16 * 16; }
 };
 
-template <typename T, int V, bool ONE, int R, int THREADS>
-__global__ void __launch_bounds__(THREADS, blocks_per_sm(THREADS))
+template <typename T, int V, bool ONE>
+__global__ void __launch_bounds__(kThreads, 2)
 norm_images_backward_kernel(const Slab s) {
   extern __shared__ __align__(16) unsigned char raw[];
-  const BackwardShared sh(raw, THREADS * V, s.channels);
+  const BackwardShared sh(raw, kThreads * V, s.channels);
   constexpr int M = ONE ? 1 : Pack<T, V>::kPairs;
   chained();
   const NormParams& p = s.p;
@@ -330,37 +341,22 @@ norm_images_backward_kernel(const Slab s) {
     group[i][0] = at.live ? (at.cc + (ONE ? 0 : 2 * i)) / cpg : 0;
     group[i][1] = ONE || !at.live ? group[i][0] : (at.cc + min(2 * i + 1, V - 1)) / cpg;
   }
-  for (int i = threadIdx.x; i < s.channels; i += THREADS) sh.acc[i] = make_float2(0.0f, 0.0f);
-  // this thread's rows of the next image, THREADS apart: x, then dy
-  Pack<T, V>* next = reinterpret_cast<Pack<T, V>*>(raw + BackwardShared::bytes(THREADS * V, s.channels)) + threadIdx.x;
+  for (int i = threadIdx.x; i < s.channels; i += kThreads) sh.acc[i] = make_float2(0.0f, 0.0f);
+  // this thread's rows, kThreads apart: x, then dy
+  Pack<T, V>* held = reinterpret_cast<Pack<T, V>*>(raw + BackwardShared::bytes(kThreads * V, s.channels)) + threadIdx.x;
+  Pack<T, V>* held_dy = held + s.held * kThreads;
   const int count = at.live ? rows.of(at.r) : 0;
   const long long x_step = s.rows_at_once * px, dy_step = s.rows_at_once * pdy, dx_step = s.rows_at_once * pdx;
-  auto fetch = [&](int n) {
-    if (n < p.N) {
-      const T* x0 = static_cast<const T*>(p.x) + (count > 0 ? n * p.x_s[0] + c + first * px : 0);
-      const T* dy0 = static_cast<const T*>(p.dy) + (count > 0 ? n * p.dy_s[0] + c + first * pdy : 0);
-#pragma unroll
-      for (int k = 0; k < R; ++k) {
-        async_load(next + k * THREADS, x0, k < count);
-        async_load(next + (R + k) * THREADS, dy0, k < count);
-        if (k + 1 < count) {
-          x0 += x_step;
-          dy0 += dy_step;
-        }
-      }
-    }
-    async_commit();
-  };
-  fetch(slice);
+  const T* x0 = static_cast<const T*>(p.x) + (count > 0 ? c + first * px : 0);
+  const T* dy0 = static_cast<const T*>(p.dy) + (count > 0 ? c + first * pdy : 0);
+  T* dx0 = static_cast<T*>(p.dx) + (count > 0 ? c + first * pdx : 0);
+  for (int k = 0; k < count; ++k) {
+    async_load(held + k * kThreads, x0 + slice * p.x_s[0] + k * x_step, true);
+    async_load(held_dy + k * kThreads, dy0 + slice * p.dy_s[0] + k * dy_step, true);
+  }
   for (int n = slice; n < p.N; n += s.slices) {
-    Pack<T, V> x[R], dy[R];
+    async_commit();
     async_wait<0>();
-#pragma unroll
-    for (int k = 0; k < R; ++k) {
-      x[k] = next[k * THREADS];
-      dy[k] = next[(R + k) * THREADS];
-    }
-    fetch(n + s.slices);
     F2 mean[M], rstd[M], gx[P], gs[P];               // mean: minus the mean
 #pragma unroll
     for (int i = 0; i < M; ++i) {
@@ -371,22 +367,25 @@ norm_images_backward_kernel(const Slab s) {
 #pragma unroll
     for (int i = 0; i < P; ++i) gx[i] = gs[i] = 0;
     with_activation(p.act, [&](auto act) {
+#pragma unroll 2
+      for (int k = 0; k < count; ++k) {
+        const Pack<T, V> x = held[k * kThreads], dy = held_dy[k * kThreads];
 #pragma unroll
-      for (int k = 0; k < R; ++k)
-        if (k < count) {
-#pragma unroll
-          for (int i = 0; i < P; ++i) {
-            const F2 xh = f2_mul(f2_add(x[k].pair(i), mean[ONE ? 0 : i]), rstd[ONE ? 0 : i]);
-            const F2 g = f2_mul(dy[k].pair(i), slope2<decltype(act)::value>(f2_fma(xh, w[i], b[i])));
-            gx[i] = f2_fma(g, xh, gx[i]);
-            gs[i] = f2_add(gs[i], g);
-          }
+        for (int i = 0; i < P; ++i) {
+          const F2 xh = f2_mul(f2_add(x.pair(i), mean[ONE ? 0 : i]), rstd[ONE ? 0 : i]);
+          const F2 g = f2_mul(dy.pair(i), slope2<decltype(act)::value>(f2_fma(xh, w[i], b[i])));
+          gx[i] = f2_fma(g, xh, gx[i]);
+          gs[i] = f2_add(gs[i], g);
         }
+      }
     });
     sum_by_channel<V>(s, at, gx, gs, sh.red, sh.own);
-    if (s.cluster > 1) cluster.sync();
-    else __syncthreads();
-    for (int i = threadIdx.x; i < s.channels; i += THREADS) {
+    __syncthreads();
+    if (s.cluster > 1) {
+      cluster_arrive();
+      cluster_wait();
+    }
+    for (int i = threadIdx.x; i < s.channels; i += kThreads) {
       float2 t = make_float2(0.0f, 0.0f);
       for (int q = 0; q < s.cluster; ++q) {
         const float2 v = (s.cluster > 1 ? cluster.map_shared_rank(sh.own, q) : sh.own)[i];
@@ -397,78 +396,72 @@ norm_images_backward_kernel(const Slab s) {
       sh.acc[i].x += t.x;
       sh.acc[i].y += t.y;
     }
-    if (s.cluster > 1) cluster.barrier_arrive();
     __syncthreads();
+    if (s.cluster > 1) cluster_arrive();
     group_means<T>(s, at.c0, at.here, sh.all, sh.means);
     __syncthreads();
-    if (p.dx != nullptr) {
-      F2 s1[M], s2[M];                               // minus s1 / m, minus s2 / m
+    F2 s1[M], s2[M];                                 // minus s1 / m, minus s2 / m
 #pragma unroll
-      for (int i = 0; i < M; ++i) {
-        const float2 lo = sh.means[group[i][0]], hi = sh.means[group[i][1]];
-        s1[i] = f2_pack(-lo.x, -hi.x);
-        s2[i] = f2_pack(-lo.y, -hi.y);
-      }
-      T* dx0 = static_cast<T*>(p.dx) + (count > 0 ? n * p.dx_s[0] + c + first * pdx : 0);
-      with_activation(p.act, [&](auto act) {
-#pragma unroll
-        for (int k = 0; k < R; ++k)
-          if (k < count) {
-            Pack<T, V> dx;
-#pragma unroll
-            for (int i = 0; i < P; ++i) {
-              const F2 xh = f2_mul(f2_add(x[k].pair(i), mean[ONE ? 0 : i]), rstd[ONE ? 0 : i]);
-              const F2 g = f2_mul(dy[k].pair(i), slope2<decltype(act)::value>(f2_fma(xh, w[i], b[i])));
-              dx.set_pair(i, f2_mul(rstd[ONE ? 0 : i], f2_fma(xh, s2[ONE ? 0 : i], f2_fma(g, w[i], s1[ONE ? 0 : i]))));
-            }
-            dx.store(dx0);
-            dx0 += dx_step;
-          }
-      });
+    for (int i = 0; i < M; ++i) {
+      const float2 lo = sh.means[group[i][0]], hi = sh.means[group[i][1]];
+      s1[i] = f2_pack(-lo.x, -hi.x);
+      s2[i] = f2_pack(-lo.y, -hi.y);
     }
-    if (s.cluster > 1) cluster.barrier_wait();   // before sh.own is written again, or the block ends
+    const bool more = n + s.slices < p.N;
+    const T* next_x = x0 + (more ? (n + s.slices) * p.x_s[0] : 0);
+    const T* next_dy = dy0 + (more ? (n + s.slices) * p.dy_s[0] : 0);
+    with_activation(p.act, [&](auto act) {
+#pragma unroll 2
+      for (int k = 0; k < count; ++k) {
+        const Pack<T, V> x = held[k * kThreads], dy = held_dy[k * kThreads];
+        if (p.dx != nullptr) {
+          Pack<T, V> dx;
+#pragma unroll
+          for (int i = 0; i < P; ++i) {
+            const F2 xh = f2_mul(f2_add(x.pair(i), mean[ONE ? 0 : i]), rstd[ONE ? 0 : i]);
+            const F2 g = f2_mul(dy.pair(i), slope2<decltype(act)::value>(f2_fma(xh, w[i], b[i])));
+            dx.set_pair(i, f2_mul(rstd[ONE ? 0 : i], f2_fma(xh, s2[ONE ? 0 : i], f2_fma(g, w[i], s1[ONE ? 0 : i]))));
+          }
+          dx.store(dx0 + n * p.dx_s[0] + k * dx_step);
+        }
+        if (more) {
+          async_load(held + k * kThreads, next_x + k * x_step, true);
+          async_load(held_dy + k * kThreads, next_dy + k * dy_step, true);
+        }
+      }
+    });
+    if (s.cluster > 1) cluster_wait();           // before sh.own is written again, or the block ends
   }
   if (rank == 0)
-    for (int i = threadIdx.x; i < at.here; i += THREADS) s.sums[(long long)slice * p.C + at.c0 + i] = sh.acc[i];
+    for (int i = threadIdx.x; i < at.here; i += kThreads) s.sums[(long long)slice * p.C + at.c0 + i] = sh.acc[i];
 }
 
 // ---- in two launches: a block takes a piece of an image's pixels of a slab -----------------------------------------
 
-constexpr int kSplitThreads = 256, kSplitRows = 8;
+constexpr int kSplitRows = 32;        // rows of a thread
 
 template <typename T, int V, bool ONE>
-__global__ void __launch_bounds__(kSplitThreads)
+__global__ void __launch_bounds__(kThreads)
 norm_split_stats_kernel(const Slab s) {
-  __shared__ float2 red[ONE ? kSplitThreads : kSplitThreads * V];
+  __shared__ float2 red[ONE ? kThreads : kThreads * V];
   __shared__ float2 own[kMaxGroups];
-  __shared__ Moments all[kMaxGroups];
   chained();
   const NormParams& p = s.p;
   const int piece = blockIdx.x % s.pieces, job = blockIdx.x / s.pieces, slab = job % s.slabs, n = job / s.slabs;
-  const int row0 = piece * s.rows, end = min(s.S, row0 + s.rows), cpg = p.C / p.G;
+  const int row0 = piece * s.rows, cpg = p.C / p.G;
   const Place at = Place::of<V>(s, slab);
   const long long pixel = p.W > 1 ? p.x_s[3] : p.x_s[2];
-  for (int g = threadIdx.x; g < at.groups; g += kSplitThreads) all[g] = Moments{0.0f, 0.0f, 0.0f};
-  for (int r0 = row0; r0 < end; r0 += kSplitRows * s.rows_at_once) {
-    const Rows rows(s, min(end - r0, kSplitRows * s.rows_at_once));
-    const T* x0 = static_cast<const T*>(p.x) + n * p.x_s[0] + at.c0 + at.cc + (long long)(r0 + at.r) * pixel;
-    Pack<T, V> x[kSplitRows];
-#pragma unroll
-    for (int k = 0; k < kSplitRows; ++k) {
-      x[k].clear();
-      if (at.live && k < rows.of(at.r)) x[k].load(x0 + k * s.rows_at_once * pixel);
-    }
-    local_moments<T, V, ONE>(s, at, x, rows, red, own);
-    for (int g = threadIdx.x; g < at.groups; g += kSplitThreads)
-      all[g] = joined(all[g], Moments{float(rows.all) * float(cpg), own[g].x, own[g].y});
-    __syncthreads();
-  }
-  for (int g = threadIdx.x; g < at.groups; g += kSplitThreads)
-    s.part[((long long)n * s.pieces + piece) * p.G + at.c0 / cpg + g] = make_float2(all[g].mean, all[g].m2);
+  const T* x0 = static_cast<const T*>(p.x) + n * p.x_s[0] + at.c0 + at.cc + (long long)(row0 + at.r) * pixel;
+  local_moments<T, V, ONE>(s, at, [&](int k) {
+    Pack<T, V> x;
+    x.load(x0 + (long long)k * s.rows_at_once * pixel);
+    return x;
+  }, Rows(s, min(s.S - row0, s.rows)), red, own);
+  for (int g = threadIdx.x; g < at.groups; g += kThreads) s.part[((long long)n * s.pieces + piece) * p.G + at.c0 / cpg + g] = own[g];
 }
 
 template <typename T, int V, bool ONE>
-__global__ void __launch_bounds__(kSplitThreads)
+__global__ void __launch_bounds__(kThreads)
 norm_split_apply_kernel(const Slab s) {
   __shared__ float2 all_of[kMaxGroups];
   constexpr int M = ONE ? 1 : Pack<T, V>::kPairs;
@@ -478,7 +471,7 @@ norm_split_apply_kernel(const Slab s) {
   const int row0 = piece * s.rows, end = min(s.S, row0 + s.rows), cpg = p.C / p.G;
   const Place at = Place::of<V>(s, slab);
   const int g0 = at.c0 / cpg;
-  for (int g = threadIdx.x; g < at.groups; g += kSplitThreads) {
+  for (int g = threadIdx.x; g < at.groups; g += kThreads) {
     Moments all{0.0f, 0.0f, 0.0f};
     for (int q = 0; q < s.pieces; ++q) {
       const float2 v = s.part[((long long)n * s.pieces + q) * p.G + g0 + g];
@@ -519,10 +512,10 @@ norm_split_apply_kernel(const Slab s) {
 }
 
 template <typename T, int V, bool ONE>
-__global__ void __launch_bounds__(kSplitThreads)
+__global__ void __launch_bounds__(kThreads)
 norm_split_sums_kernel(const Slab s) {
   extern __shared__ __align__(16) unsigned char raw[];
-  const BackwardShared sh(raw, kSplitThreads * V, s.channels);
+  const BackwardShared sh(raw, kThreads * V, s.channels);
   constexpr int M = ONE ? 1 : Pack<T, V>::kPairs;
   chained();
   const NormParams& p = s.p;
@@ -563,21 +556,21 @@ norm_split_sums_kernel(const Slab s) {
     });
   sum_by_channel<V>(s, at, gx, gs, sh.red, sh.own);
   __syncthreads();
-  for (int i = threadIdx.x; i < at.here; i += kSplitThreads) s.sums[((long long)n * s.pieces + piece) * p.C + at.c0 + i] = sh.own[i];
+  for (int i = threadIdx.x; i < at.here; i += kThreads) s.sums[((long long)n * s.pieces + piece) * p.C + at.c0 + i] = sh.own[i];
 }
 
 template <typename T, int V, bool ONE>
-__global__ void __launch_bounds__(kSplitThreads)
+__global__ void __launch_bounds__(kThreads)
 norm_split_dx_kernel(const Slab s) {
   extern __shared__ __align__(16) unsigned char raw[];
-  const BackwardShared sh(raw, kSplitThreads * V, s.channels);
+  const BackwardShared sh(raw, kThreads * V, s.channels);
   constexpr int M = ONE ? 1 : Pack<T, V>::kPairs;
   chained();
   const NormParams& p = s.p;
   const int piece = blockIdx.x % s.pieces, job = blockIdx.x / s.pieces, slab = job % s.slabs, n = job / s.slabs;
   const int row0 = piece * s.rows, end = min(s.S, row0 + s.rows), cpg = p.C / p.G;
   const Place at = Place::of<V>(s, slab);
-  for (int i = threadIdx.x; i < at.here; i += kSplitThreads) {
+  for (int i = threadIdx.x; i < at.here; i += kThreads) {
     float2 t = make_float2(0.0f, 0.0f);
     for (int q = 0; q < s.pieces; ++q) {
       const float2 v = s.sums[((long long)n * s.pieces + q) * p.C + at.c0 + i];
@@ -630,137 +623,119 @@ norm_split_dx_kernel(const Slab s) {
 
 struct ImagePlan {
   Slab s;
-  int V, threads, R;     // R = 0: two launches
+  int V;
+  bool split;            // two launches
+  int smem;              // else: a block's
 };
 
 int gcd(int a, int b) { return b == 0 ? a : gcd(b, a % b); }
 
 // False: a row of the slab is wider than a block's threads.
-bool slab_of(ImagePlan* plan, const NormParams& p, int V, int threads, int channels) {
+bool slab_of(ImagePlan* plan, const NormParams& p, int V, int channels) {
   Slab& s = plan->s;
   s.p = p;
   s.S = p.H * p.W;
   s.channels = channels;
   s.cols = channels / V;
-  if (s.cols > threads || s.cols < 1) return false;
-  s.rows_at_once = threads / s.cols;
+  if (s.cols > kThreads || s.cols < 1) return false;
+  s.rows_at_once = kThreads / s.cols;
   s.slabs = (p.C + channels - 1) / channels;
-  s.slices = s.pieces = 1;
-  s.cluster = 1;
+  s.slices = s.pieces = s.cluster = 1;
+  s.held = 0;
   s.part = nullptr;
   s.sums = nullptr;
   plan->V = V;
-  plan->threads = threads;
+  plan->split = false;
   return channels / (p.C / p.G) <= kMaxGroups;
 }
 
 // The slab: whole groups and whole vectors, rows of about 64 bytes (4 vectors: narrower rows waste what a DRAM access brings,
-// wider ones leave too few blocks), narrower where that is what a cluster holds or too few blocks would run.
-// Then the fewest blocks to a cluster that hold it at eight vectors a thread (x and dy: four), sixteen and 512 threads last.
+// wider ones leave too few blocks), narrower where no cluster holds it; few pixels take wider rows, or threads have none.
+// The cluster: the fewest blocks that hold the slab with three (gradient: two) to an SM, more where SMs would be idle, and with
+// one to an SM where eight blocks are too few.
 bool image_plan(int dtype, const NormParams& p, bool backward, ImagePlan* plan) {
-  const int cpg = p.C / p.G;
+  const int cpg = p.C / p.G, es = dtype == FDNN_F32 ? 4 : 2, sms = current_sm_count();
   int V = norm_vector(dtype, p, backward, p.C);
   if (V == 0) return false;
   if (V == 2 && cpg % 2 != 0) V = 1;
   const long long S = (long long)p.H * p.W;
-  if (S > 0x3fffffff) return false;
+  if (S > 0x1fffffff) return false;
   const int unit = cpg / gcd(cpg, V) * V, units = p.C / unit;   // whole groups and whole vectors
-  const int sms = current_sm_count();
-  const int tops[2] = {backward ? 8 : 16, backward ? 8 : 16};
-  const long long wide = S < 64 ? 256 / S : 4;                  // (few pixels: wider rows, or threads have none)
+  const long long wide = S < 64 ? kThreads / S : 4;
   int k = int(wide * V / unit);
   if (k < 1) k = 1;
   if (k > units) k = units;
-  const int widest = k;
-  for (;; k = (k + 1) / 2) {
-    for (int threads = 256; threads <= 512; threads *= 2) {
-      if (!slab_of(plan, p, V, threads, k * unit)) continue;
-      Slab& s = plan->s;
-      const long long at_once = s.rows_at_once;
-      if (8 * at_once * tops[threads > 256] < S) continue;
-      const int want = backward ? 8 : 16;
-      int cluster = 1;
-      while (cluster < 8 && cluster * at_once * want < S) cluster *= 2;
-      // few blocks: more to a cluster, as long as each has rows for its threads
-      while (cluster < 8 && (long long)p.N * s.slabs * cluster < sms && cluster * at_once * 2 <= S) cluster *= 2;
-      const long long need = (S + cluster * at_once - 1) / (cluster * at_once);
-      if (k > 1 && need > want && (long long)p.N * s.slabs < 4ll * sms) break;       // narrower first
-      if (k > 1 && (long long)p.N * s.slabs * cluster < sms && k * unit / V > 4) break;
-      plan->R = need <= 2 ? 2 : need <= 4 && threads == 256 ? 4 : need <= 8 ? 8 : 16;
-      if (backward && BackwardShared::bytes(threads * V, s.channels) + 2 * plan->R * threads * 16 > kMostShared) continue;
-      s.cluster = cluster;
-      s.rows = int((S + cluster - 1) / cluster);
-      // as many clusters as the SMs hold at once, or fewer that have equally many images each
-      long long room = (long long)blocks_per_sm(threads) * sms / ((long long)s.slabs * cluster);
-      if (room < 1) room = 1;
-      const long long rounds = (p.N + room - 1) / room;
-      s.slices = int((p.N + rounds - 1) / rounds);
-      return true;
+  Slab& s = plan->s;
+  for (;; k /= 2) {
+    if (!slab_of(plan, p, V, k * unit)) {
+      if (k == 1) return false;
+      continue;
     }
-    if (k == 1) break;
+    const int fixed = backward ? BackwardShared::bytes(kThreads * V, s.channels) : 0;
+    const int row = kThreads * V * es * (backward ? 2 : 1);       // bytes of a row of a block's threads
+    // (forward: beside 10 to 24 KB of static shared memory)
+    const int few = ((backward ? 112 : 74) * 1024 - (backward ? fixed : (cpg % V == 0 ? 11 : 25) * 1024)) / row;
+    const int most = (kMostShared - (backward ? fixed : 24 * 1024)) / row;
+    const long long at_once = s.rows_at_once;
+    int cluster = 1;
+    while (cluster < 8 && cluster * at_once * few < S) cluster *= 2;
+    while (cluster < 8 && (long long)p.N * s.slabs * cluster < sms && cluster * at_once * 2 <= S) cluster *= 2;
+    const long long need = (S + cluster * at_once - 1) / (cluster * at_once);
+    if (need > most || (k * unit / V > 2 && k > 1 && need > few)) {   // (not under 32 bytes to have three blocks: 64 x 64 x 112 x 112)
+      if (k > 1) continue;                                         // narrower
+      break;
+    }
+    s.cluster = cluster;
+    s.rows = int((S + cluster - 1) / cluster);
+    s.held = int((s.rows + at_once - 1) / at_once);
+    plan->smem = fixed + s.held * row;
+    // as many clusters as the SMs hold at once, or fewer that have equally many images each
+    int per_sm = kSharedOfSm / (plan->smem + 1024 + (backward ? 0 : (cpg % V == 0 ? 10 : 24) * 1024));
+    if (per_sm > (backward ? 2 : 3)) per_sm = backward ? 2 : 3;
+    long long room = (long long)per_sm * sms / ((long long)s.slabs * cluster);
+    if (room < 1) room = 1;
+    const long long rounds = (p.N + room - 1) / room;
+    s.slices = int((p.N + rounds - 1) / rounds);
+    return true;
   }
   // no cluster holds a slab
-  for (k = widest; k >= 1; k /= 2)
-    if (slab_of(plan, p, V, kSplitThreads, k * unit)) break;
-  if (k < 1) return false;
-  Slab& s = plan->s;
-  plan->R = 0;
-  long long pieces = (S + 4ll * kSplitRows * s.rows_at_once - 1) / (4ll * kSplitRows * s.rows_at_once);
+  plan->split = true;
+  long long pieces = (S + (long long)kSplitRows * s.rows_at_once - 1) / ((long long)kSplitRows * s.rows_at_once);
   if (pieces > kMaxChunks) pieces = kMaxChunks;
   s.rows = int((S + pieces - 1) / pieces);
   s.pieces = int((S + s.rows - 1) / s.rows);
   return true;
 }
 
-template <typename T, int V, bool ONE, int R, int THREADS>
-cudaError_t run_forward(const Slab& s, cudaStream_t stream) {
-  static std::atomic<uint64_t> done;
-  auto* kernel = norm_images_kernel<T, V, ONE, R, THREADS>;
-  constexpr int kSmem = R * THREADS * Pack<T, V>::kBytes;
-  const cudaError_t e = allow_smem(kernel, kSmem, done);
-  if (e != cudaSuccess) return e;
-  return launch_seq(kernel, dim3(unsigned((long long)s.slices * s.slabs * s.cluster)), THREADS, kSmem, s.cluster, stream, s);
-}
-
 template <typename T, int V, bool ONE>
 cudaError_t forward(ImagePlan& plan, cudaStream_t stream) {
   Slab& s = plan.s;
   const NormParams& p = s.p;
-  if (plan.R == 0) {
+  if (plan.split) {
     const long long blocks = (long long)p.N * s.slabs * s.pieces;
     if (blocks > 0x7fffffffll) return cudaErrorInvalidConfiguration;
     if (8ll * p.N * s.pieces * p.G > p.workspace_bytes) return cudaErrorInvalidValue;
     s.part = static_cast<float2*>(p.workspace);
-    const cudaError_t e = launch_seq(norm_split_stats_kernel<T, V, ONE>, dim3(unsigned(blocks)), kSplitThreads, 0, 1, stream, s);
+    const cudaError_t e = launch_seq(norm_split_stats_kernel<T, V, ONE>, dim3(unsigned(blocks)), kThreads, 0, 1, stream, s);
     if (e != cudaSuccess) return e;
-    return launch_seq(norm_split_apply_kernel<T, V, ONE>, dim3(unsigned(blocks)), kSplitThreads, 0, 1, stream, s);
+    return launch_seq(norm_split_apply_kernel<T, V, ONE>, dim3(unsigned(blocks)), kThreads, 0, 1, stream, s);
   }
-  return plan.threads > 256 ? run_forward<T, V, ONE, 16, 512>(s, stream)
-         : plan.R == 2      ? run_forward<T, V, ONE, 2, 256>(s, stream)
-         : plan.R <= 8      ? run_forward<T, V, ONE, 8, 256>(s, stream)
-                            : run_forward<T, V, ONE, 16, 256>(s, stream);
+  static std::atomic<uint64_t> done;
+  auto* kernel = norm_images_kernel<T, V, ONE>;
+  const cudaError_t e = allow_smem(kernel, kMostShared - 24 * 1024, done);   // (beside the static part)
+  if (e != cudaSuccess) return e;
+  return launch_seq(kernel, dim3(unsigned((long long)s.slices * s.slabs * s.cluster)), kThreads, plan.smem, s.cluster, stream, s);
 }
 
-template <typename T, int V, bool ONE, int R, int THREADS>
-cudaError_t run_backward(const Slab& s, long long blocks, cudaStream_t stream) {
-  static std::atomic<uint64_t> done;
-  auto* kernel = norm_images_backward_kernel<T, V, ONE, R, THREADS>;
-  constexpr int kRing = 2 * R * THREADS * Pack<T, V>::kBytes;
-  const int smem = BackwardShared::bytes(THREADS * V, s.channels) + kRing;
-  const int most = BackwardShared::bytes(THREADS * V, THREADS * V) + kRing;
-  const cudaError_t e = allow_smem(kernel, most < kMostShared ? most : kMostShared, done);
-  if (e != cudaSuccess) return e;
-  return launch_seq(kernel, dim3(unsigned(blocks)), THREADS, smem, s.cluster, stream, s);
-}
 template <typename T, int V, bool ONE>
 cudaError_t run_split(const Slab& s, long long blocks, cudaStream_t stream) {
   static std::atomic<uint64_t> sums_done, dx_done;
-  const int smem = BackwardShared::bytes(kSplitThreads * V, s.channels), most = BackwardShared::bytes(kSplitThreads * V, kSplitThreads * V);
+  const int smem = BackwardShared::bytes(kThreads * V, s.channels), most = BackwardShared::bytes(kThreads * V, kThreads * V);
   cudaError_t e = allow_smem(norm_split_sums_kernel<T, V, ONE>, most, sums_done);
   if (e == cudaSuccess) e = allow_smem(norm_split_dx_kernel<T, V, ONE>, most, dx_done);
-  if (e == cudaSuccess) e = launch_seq(norm_split_sums_kernel<T, V, ONE>, dim3(unsigned(blocks)), kSplitThreads, smem, 1, stream, s);
+  if (e == cudaSuccess) e = launch_seq(norm_split_sums_kernel<T, V, ONE>, dim3(unsigned(blocks)), kThreads, smem, 1, stream, s);
   if (e == cudaSuccess && s.p.dx != nullptr)
-    e = launch_seq(norm_split_dx_kernel<T, V, ONE>, dim3(unsigned(blocks)), kSplitThreads, smem, 1, stream, s);
+    e = launch_seq(norm_split_dx_kernel<T, V, ONE>, dim3(unsigned(blocks)), kThreads, smem, 1, stream, s);
   return e;
 }
 
@@ -769,19 +744,19 @@ cudaError_t backward(ImagePlan& plan, cudaStream_t stream) {
   Slab& s = plan.s;
   const NormParams& p = s.p;
   s.sums = static_cast<float2*>(p.workspace);
-  cudaError_t e;
-  const long long rows = plan.R == 0 ? (long long)p.N * s.pieces : s.slices;
+  const long long rows = plan.split ? (long long)p.N * s.pieces : s.slices;
   if (8 * rows * p.C > p.workspace_bytes) return cudaErrorInvalidValue;
-  if (plan.R == 0) {
+  cudaError_t e;
+  if (plan.split) {
     const long long blocks = (long long)p.N * s.slabs * s.pieces;
     if (blocks > 0x7fffffffll) return cudaErrorInvalidConfiguration;
     e = run_split<T, V, ONE>(s, blocks, stream);
   } else {
-    const long long blocks = (long long)s.slices * s.slabs * s.cluster;
-    e = plan.threads > 256 ? (plan.R == 2 ? run_backward<T, V, ONE, 2, 512>(s, blocks, stream) : run_backward<T, V, ONE, 8, 512>(s, blocks, stream))
-        : plan.R <= 2      ? run_backward<T, V, ONE, 2, 256>(s, blocks, stream)
-        : plan.R == 4      ? run_backward<T, V, ONE, 4, 256>(s, blocks, stream)
-                           : run_backward<T, V, ONE, 8, 256>(s, blocks, stream);
+    static std::atomic<uint64_t> done;
+    auto* kernel = norm_images_backward_kernel<T, V, ONE>;
+    e = allow_smem(kernel, kMostShared, done);
+    if (e == cudaSuccess)
+      e = launch_seq(kernel, dim3(unsigned((long long)s.slices * s.slabs * s.cluster)), kThreads, plan.smem, s.cluster, stream, s);
   }
   if (e != cudaSuccess || (p.dweight == nullptr && p.dbias == nullptr)) return e;
   return launch_norm_dparams<T>(p, s.sums, rows, stream);
@@ -799,8 +774,8 @@ long long norm_images_workspace(int dtype, const NormParams& p, bool backward) {
   (void)dtype;
   const long long S = (long long)p.H * p.W, pieces = S < kMaxChunks ? S : kMaxChunks;
   const long long slices = 4ll * current_sm_count() < p.N ? 4ll * current_sm_count() : p.N;
-  // two launches: only groups of more than 8 x 256 x 8 values (a cluster of blocks with narrow vectors), and wide ones
-  const bool split = S * (p.C / p.G) > 8 * 256 * 8 || p.C / p.G > 256;
+  // two launches: only groups of more than 8 x 256 x 8 values (less than what eight blocks of the narrowest vectors hold)
+  const bool split = S * (p.C / p.G) > 8 * 256 * 8;
   const long long rows = split ? (p.N * pieces > slices ? p.N * pieces : slices) : slices;
   return 8 * rows * (backward ? p.C : split ? p.G : 0);
 }
