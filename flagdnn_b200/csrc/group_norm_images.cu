@@ -22,6 +22,7 @@ namespace cg = cooperative_groups;
 
 constexpr int kMaxChunks = 64;        // pieces of an image in two launches
 constexpr int kMaxGroups = 512;       // of a slab
+constexpr int kThreads = 256;
 constexpr int kMostShared = 224 * 1024, kSharedOfSm = 228 * 1024;
 
 struct Slab {
@@ -148,8 +149,6 @@ __device__ __forceinline__ void local_moments(const Slab& s, const Place& at, F&
   __syncthreads();
 }
 
-constexpr int kThreads = 256;
-
 // The cluster's barrier, after a __syncthreads(): what the block's threads wrote (or read) before that is ordered by the first
 // warp's release; a fence in each of the others would cost as much again and order nothing more.
 __device__ __forceinline__ void cluster_arrive() {
@@ -265,42 +264,41 @@ __device__ __forceinline__ void sum_by_channel(const Slab& s, const Place& at, c
     }
   }
   __syncthreads();
-  // the rows in as many parts as there are threads for; the first part's thread adds the parts in their order
-  const int parts = min(s.rows_at_once, max(1, int(blockDim.x) / s.channels));
-  for (int e = threadIdx.x; e < parts * s.channels; e += blockDim.x) {
-    const int part = e / s.channels, c = e - part * s.channels;
-    float2 t = red[part * s.channels + c];
-    for (int row = part + parts; row < s.rows_at_once; row += parts) {
+  // the rows in as many parts as there are threads for, each thread a channel's; then the parts in their order
+  const int parts = s.channels <= kThreads ? min(s.rows_at_once, kThreads / s.channels) : 1;
+  const int part = s.channels <= kThreads ? int(threadIdx.x) / s.channels : 0;
+  for (int c = int(threadIdx.x) - part * s.channels; c < s.channels && part < parts; c += kThreads) {
+    float2 t = make_float2(0.0f, 0.0f);
+#pragma unroll 4
+    for (int row = part; row < s.rows_at_once; row += parts) {
       const float2 q = red[row * s.channels + c];
       t.x += q.x;
       t.y += q.y;
     }
-    red[part * s.channels + c] = t;
+    red[part * s.channels + c] = t;      // (of the rows that this thread alone has read)
   }
   __syncthreads();
-  for (int c = threadIdx.x; c < s.channels; c += blockDim.x) {
+  for (int c = threadIdx.x; c < s.channels; c += kThreads) {
     float2 t = red[c];
-    for (int part = 1; part < parts; ++part) {
-      const float2 q = red[part * s.channels + c];
-      t.x += q.x;
-      t.y += q.y;
+#pragma unroll 4
+    for (int q = 1; q < parts; ++q) {
+      const float2 v = red[q * s.channels + c];
+      t.x += v.x;
+      t.y += v.y;
     }
     sums[c] = t;
   }
 }
 
 // s1 / m and s2 / m of every group of the slab from its channels' sums.
-template <typename T>
-__device__ __forceinline__ void group_means(const Slab& s, int c0, int here, const float2* sums, float2* means) {
-  const NormParams& p = s.p;
-  const int cpg = p.C / p.G, lane = threadIdx.x & 31;
-  const float inv = 1.0f / (float(s.S) * float(cpg));
-  for (int g = threadIdx.x >> 5; g < here / cpg; g += blockDim.x >> 5) {
+__device__ __forceinline__ void group_means(const Slab& s, const Place& at, const float* weight, const float2* sums, float2* means) {
+  const int cpg = s.p.C / s.p.G, lane = threadIdx.x & 31;
+  const float inv = __fdividef(1.0f, float(s.S) * float(cpg));
+  for (int g = threadIdx.x >> 5; g < at.groups; g += kThreads / 32) {
     float s1 = 0.0f, s2 = 0.0f;
     for (int c = g * cpg + lane; c < (g + 1) * cpg; c += 32) {
-      const float w = p.weight != nullptr ? param<T>(p.weight, p.param_f32, c0 + c) : 1.0f;
-      s2 += w * sums[c].x;
-      s1 += w * sums[c].y;
+      s2 += weight[c] * sums[c].x;
+      s1 += weight[c] * sums[c].y;
     }
     s1 = warp_sum(s1);
     s2 = warp_sum(s2);
@@ -311,10 +309,19 @@ __device__ __forceinline__ void group_means(const Slab& s, int c0, int here, con
 // Shared memory of the backward kernels: a row of vectors bounds a slab's channels.
 struct BackwardShared {
   float2 *red, *own, *all, *acc, *means;
+  float* weight;
   __device__ BackwardShared(unsigned char* raw, int entries, int channels)
-      : red(reinterpret_cast<float2*>(raw)), own(red + entries), all(own + channels), acc(all + channels), means(acc + channels) {}
-  static __host__ __device__ int bytes(int entries, int channels) { return (8 * (entries + 3 * channels + kMaxGroups) + 15) / 16 * 16; }
+      : red(reinterpret_cast<float2*>(raw)), own(red + entries), all(own + channels), acc(all + channels), means(acc + channels),
+        weight(reinterpret_cast<float*>(means + kMaxGroups)) {}
+  static __host__ __device__ int bytes(int entries, int channels) {
+    return (8 * (entries + 3 * channels + kMaxGroups) + 4 * channels + 15) / 16 * 16;
+  }
 };
+template <typename T>
+__device__ __forceinline__ void stage_weights(const NormParams& p, const Place& at, float* weight) {
+  for (int i = threadIdx.x; i < at.here; i += kThreads)
+    weight[i] = p.weight != nullptr ? param<T>(p.weight, p.param_f32, at.c0 + i) : 1.0f;
+}
 
 template <typename T, int V, bool ONE>
 __global__ void __launch_bounds__(kThreads, 2)
@@ -342,6 +349,7 @@ norm_images_backward_kernel(const Slab s) {
     group[i][1] = ONE || !at.live ? group[i][0] : (at.cc + min(2 * i + 1, V - 1)) / cpg;
   }
   for (int i = threadIdx.x; i < s.channels; i += kThreads) sh.acc[i] = make_float2(0.0f, 0.0f);
+  stage_weights<T>(p, at, sh.weight);
   // this thread's rows, kThreads apart: x, then dy
   Pack<T, V>* held = reinterpret_cast<Pack<T, V>*>(raw + BackwardShared::bytes(kThreads * V, s.channels)) + threadIdx.x;
   Pack<T, V>* held_dy = held + s.held * kThreads;
@@ -386,11 +394,17 @@ norm_images_backward_kernel(const Slab s) {
       cluster_wait();
     }
     for (int i = threadIdx.x; i < s.channels; i += kThreads) {
-      float2 t = make_float2(0.0f, 0.0f);
-      for (int q = 0; q < s.cluster; ++q) {
-        const float2 v = (s.cluster > 1 ? cluster.map_shared_rank(sh.own, q) : sh.own)[i];
-        t.x += v.x;
-        t.y += v.y;
+      float2 t = sh.own[i];
+      if (s.cluster > 1) {
+        float2 v[8];
+#pragma unroll
+        for (int q = 0; q < 8; ++q) v[q] = q < s.cluster ? cluster.map_shared_rank(sh.own, q)[i] : make_float2(0.0f, 0.0f);
+        t = v[0];
+#pragma unroll
+        for (int q = 1; q < 8; ++q) {
+          t.x += v[q].x;
+          t.y += v[q].y;
+        }
       }
       sh.all[i] = t;
       sh.acc[i].x += t.x;
@@ -398,7 +412,7 @@ norm_images_backward_kernel(const Slab s) {
     }
     __syncthreads();
     if (s.cluster > 1) cluster_arrive();
-    group_means<T>(s, at.c0, at.here, sh.all, sh.means);
+    group_means(s, at, sh.weight, sh.all, sh.means);
     __syncthreads();
     F2 s1[M], s2[M];                                 // minus s1 / m, minus s2 / m
 #pragma unroll
@@ -579,8 +593,9 @@ norm_split_dx_kernel(const Slab s) {
     }
     sh.all[i] = t;
   }
+  stage_weights<T>(p, at, sh.weight);
   __syncthreads();
-  group_means<T>(s, at.c0, at.here, sh.all, sh.means);
+  group_means(s, at, sh.weight, sh.all, sh.means);
   __syncthreads();
   if (!at.live) return;
   const bool tall = p.W > 1;
@@ -681,8 +696,11 @@ bool image_plan(int dtype, const NormParams& p, bool backward, ImagePlan* plan) 
     while (cluster < 8 && cluster * at_once * few < S) cluster *= 2;
     while (cluster < 8 && (long long)p.N * s.slabs * cluster < sms && cluster * at_once * 2 <= S) cluster *= 2;
     const long long need = (S + cluster * at_once - 1) / (cluster * at_once);
-    if (need > most || (k * unit / V > 2 && k > 1 && need > few)) {   // (not under 32 bytes to have three blocks: 64 x 64 x 112 x 112)
-      if (k > 1) continue;                                         // narrower
+    // (not under 32 bytes to have three blocks to an SM, 64 x 64 x 112 x 112 bf16 97 us and 209; the gradient goes in two launches
+    // rather than with one block to an SM, 195 us and 345)
+    if (need > most || (need > few && (backward || (k > 1 && k * unit / V > 2)))) {
+      if (k > 1 && k * unit / V > 2) continue;                     // narrower
+      if (k > 1 && !backward) continue;
       break;
     }
     s.cluster = cluster;
@@ -774,8 +792,9 @@ long long norm_images_workspace(int dtype, const NormParams& p, bool backward) {
   (void)dtype;
   const long long S = (long long)p.H * p.W, pieces = S < kMaxChunks ? S : kMaxChunks;
   const long long slices = 4ll * current_sm_count() < p.N ? 4ll * current_sm_count() : p.N;
-  // two launches: only groups of more than 8 x 256 x 8 values (less than what eight blocks of the narrowest vectors hold)
-  const bool split = S * (p.C / p.G) > 8 * 256 * 8;
+  // Two launches: only where a cluster's eight blocks, which hold at least 50 rows of vectors (forward) or 4 (backward, beside the
+  // sums of 2048 channels) for each of their threads, and at least 129 of a row's 256 threads have work, are too few.
+  const bool split = S * (p.C / p.G) > (backward ? 8 * 4 * 128 : 8 * 50 * 128);
   const long long rows = split ? (p.N * pieces > slices ? p.N * pieces : slices) : slices;
   return 8 * rows * (backward ? p.C : split ? p.G : 0);
 }

@@ -80,6 +80,10 @@ SHAPES = [   # shape, groups, layout
     ((2, 300, 9, 10), 1, "odd"),
     ((2, 1026, 3, 3), 2, "cl"),
     ((3, 700, 1, 1), 1, "odd"),
+    ((1, 2040, 6, 6), 8, "cl"),           # 255 channels a group: eight groups to a slab
+    ((2, 2040, 1, 33), 8, "cl"),
+    ((1, 1032, 12, 12), 8, "cl"),
+    ((2, 1032, 13, 13), 8, "cl"),
     ((3, 4096, 1, 1), 1, "cl"),           # slabs as wide as they get
     ((2, 4096, 3, 5), 8, "cl"),
     ((2, 3968, 6, 6), 1, "cl"),
