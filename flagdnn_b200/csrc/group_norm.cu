@@ -231,18 +231,18 @@ norm_dx_kernel(const NormParams p) {
   }
 }
 
-// 32 channels a block, its eight warps an eighth of the rows each (every eighth row, four on their way).
+// 32 channels a block, each of its 32 warps every 32nd row; then the warps' sums in their order.
 template <typename T>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(1024)
 norm_dparams_kernel(const NormParams p, const float2* rows, long long count) {
   chained();
-  __shared__ float2 part[8][32];
+  __shared__ float2 part[32][32];
   const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5;
   const int c = blockIdx.x * 32 + lane;
   float2 v = make_float2(0.0f, 0.0f);
   if (c < p.C) {
 #pragma unroll 8
-    for (long long r = slice; r < count; r += 8) {
+    for (long long r = slice; r < count; r += 32) {
       const float2 q = rows[r * p.C + c];
       v.x += q.x;
       v.y += q.y;
@@ -251,7 +251,8 @@ norm_dparams_kernel(const NormParams p, const float2* rows, long long count) {
   part[slice][lane] = v;
   __syncthreads();
   if (slice != 0 || c >= p.C) return;
-  for (int k = 1; k < 8; ++k) {
+#pragma unroll 8
+  for (int k = 1; k < 32; ++k) {
     v.x += part[k][lane].x;
     v.y += part[k][lane].y;
   }
@@ -301,7 +302,7 @@ cudaError_t backward_t(const NormParams& p, cudaStream_t stream) {
 
 template <typename T>
 cudaError_t launch_norm_dparams(const NormParams& p, const float2* rows, long long count, cudaStream_t stream) {
-  return launch_seq(norm_dparams_kernel<T>, dim3(unsigned((p.C + 31) / 32)), 256, 0, 1, stream, p, rows, count);
+  return launch_seq(norm_dparams_kernel<T>, dim3(unsigned((p.C + 31) / 32)), 1024, 0, 1, stream, p, rows, count);
 }
 template cudaError_t launch_norm_dparams<__half>(const NormParams&, const float2*, long long, cudaStream_t);
 template cudaError_t launch_norm_dparams<__nv_bfloat16>(const NormParams&, const float2*, long long, cudaStream_t);

@@ -703,6 +703,8 @@ bool image_plan(int dtype, const NormParams& p, bool backward, ImagePlan* plan) 
       if (k > 1 && !backward) continue;
       break;
     }
+    // a few large images: the two launches cut them finer (one of 208 x 104 x 103 in slabs of 104 channels 46 us, not cut)
+    if (2ll * p.N * s.slabs * cluster <= sms && need > 16) break;
     s.cluster = cluster;
     s.rows = int((S + cluster - 1) / cluster);
     s.held = int((s.rows + at_once - 1) / at_once);
@@ -718,7 +720,10 @@ bool image_plan(int dtype, const NormParams& p, bool backward, ImagePlan* plan) 
   }
   // no cluster holds a slab
   plan->split = true;
-  long long pieces = (S + (long long)kSplitRows * s.rows_at_once - 1) / ((long long)kSplitRows * s.rows_at_once);
+  // up to 32 rows a thread, fewer (down to 4) where that leaves SMs without blocks
+  long long rows = (long long)p.N * s.slabs * S / (2ll * sms * s.rows_at_once);
+  rows = rows > kSplitRows ? kSplitRows : rows < 4 ? 4 : rows;
+  long long pieces = (S + rows * s.rows_at_once - 1) / (rows * s.rows_at_once);
   if (pieces > kMaxChunks) pieces = kMaxChunks;
   s.rows = int((S + pieces - 1) / pieces);
   s.pieces = int((S + s.rows - 1) / s.rows);
@@ -792,9 +797,9 @@ long long norm_images_workspace(int dtype, const NormParams& p, bool backward) {
   (void)dtype;
   const long long S = (long long)p.H * p.W, pieces = S < kMaxChunks ? S : kMaxChunks;
   const long long slices = 4ll * current_sm_count() < p.N ? 4ll * current_sm_count() : p.N;
-  // Two launches: only where a cluster's eight blocks, which hold at least 50 rows of vectors (forward) or 4 (backward, beside the
-  // sums of 2048 channels) for each of their threads, and at least 129 of a row's 256 threads have work, are too few.
-  const bool split = S * (p.C / p.G) > (backward ? 8 * 4 * 128 : 8 * 50 * 128);
+  // Two launches: only where eight blocks do not hold 16 rows of vectors (backward 4, beside the sums of 2048 channels) for each of
+  // their threads, of which at least 129 have work.
+  const bool split = S * (p.C / p.G) > (backward ? 8 * 4 * 128 : 8 * 16 * 128);
   const long long rows = split ? (p.N * pieces > slices ? p.N * pieces : slices) : slices;
   return 8 * rows * (backward ? p.C : split ? p.G : 0);
 }

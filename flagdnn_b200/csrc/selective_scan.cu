@@ -29,7 +29,7 @@ namespace fdnn {
 namespace {
 
 
-constexpr int kHalf = 128;                 // threads of each half of a block
+constexpr int kScan = 128, kFill = 128;    // threads that scan, threads that fill
 
 struct Cut {
   int chunks, tokens;                      // chunks of a row, tokens of each (the last may have fewer)
@@ -47,12 +47,11 @@ __device__ __forceinline__ int length_of(const int* lengths, int n, int L) {
   return lengths == nullptr ? L : min(max(lengths[n], 0), L);
 }
 template <int ID>
-__device__ __forceinline__ void bar_sync(int which) { asm volatile("bar.sync %0, %1;" ::"r"(ID + which), "n"(2 * kHalf) : "memory"); }
+__device__ __forceinline__ void bar_sync(int which) { asm volatile("bar.sync %0, %1;" ::"r"(ID + which), "n"(kScan + kFill) : "memory"); }
+// (Orders this thread's accesses to shared memory before those behind the others' bar_sync: the producer's half of the PTX
+// manual's own example. A fence in front of it would wait for the stores of y.)
 template <int ID>
-__device__ __forceinline__ void bar_arrive(int which) {
-  __threadfence_block();
-  asm volatile("bar.arrive %0, %1;" ::"r"(ID + which), "n"(2 * kHalf) : "memory");
-}
+__device__ __forceinline__ void bar_arrive(int which) { asm volatile("bar.arrive %0, %1;" ::"r"(ID + which), "n"(kScan + kFill) : "memory"); }
 constexpr int kFull = 1, kDone = 3;
 
 // Eight neighbouring values (of channels or of states), as loaded.
@@ -79,12 +78,13 @@ struct Eight {
   }
 };
 
+// A tile is eight channels of a token for each filling thread.
 template <int NPT, int LANES>
 struct Tile {
-  static constexpr int kChannels = kHalf / LANES;
+  static constexpr int kChannels = kScan / LANES;
   static constexpr int kChunks = kChannels / 8;                      // eights of channels
   static constexpr int kStates = NPT * LANES;
-  static constexpr int kTokens = 8 * LANES < kHalf / 4 ? 8 * LANES : kHalf / 4;
+  static constexpr int kTokens = 8 * kFill / kChannels < kFill / 4 ? 8 * kFill / kChannels : kFill / 4;
   static constexpr int kPieces = 2 * kStates / 8;                    // eights of a token's B and C
   // Sixteen threads of a warp store their k-th channels at once, and the scanning lanes read eight neighbours: channel k of an
   // eight lies at k ^ turn, so that neither meets a bank twice.
@@ -100,29 +100,27 @@ constexpr int kPrefetch = 3, kSlots = kPrefetch + 1, kLongSlots = kPrefetch + 3;
 template <typename T, int PIECES>
 struct Ring {
   static constexpr int kWords = Eight<T>::kWords;
-  uint4 u[kLongSlots][kWords][kHalf];
-  uint4 z[kLongSlots][kWords][kHalf];
-  uint4 delta[kSlots][kWords][kHalf];
-  uint4 bc[kSlots][PIECES > 0 ? PIECES : 1][kWords][kHalf];
+  uint4 u[kLongSlots][kWords][kFill];
+  uint4 z[kLongSlots][kWords][kFill];
+  uint4 delta[kSlots][kWords][kFill];
+  uint4 bc[kSlots][PIECES > 0 ? PIECES : 1][kWords][kFill];
 };
-// VEC: asynchronously, 16 bytes at a time, zeros past `count` values
-template <bool VEC, typename T>
-__device__ __forceinline__ void fetch(uint4 (&slot)[Eight<T>::kWords][kHalf], int tid, const T* p, long long stride, int count) {
-  if constexpr (VEC) {
+// Asynchronously, 16 bytes at a time, zeros past `count` values.
+template <typename T>
+__device__ __forceinline__ void fetch(uint4 (&slot)[Eight<T>::kWords][kFill], int tid, const T* p, int count) {
 #pragma unroll
-    for (int w = 0; w < Eight<T>::kWords; ++w)
-      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(uint32_t(__cvta_generic_to_shared(&slot[w][tid]))),
-                   "l"(reinterpret_cast<const uint4*>(p) + w), "r"(count > w * 16 / int(sizeof(T)) ? 16 : 0)
-                   : "memory");
-  } else {
-    Eight<T> v;
-    v.template load<false>(p, stride, count);
-#pragma unroll
-    for (int w = 0; w < Eight<T>::kWords; ++w) slot[w][tid] = v.q[w];
-  }
+  for (int w = 0; w < Eight<T>::kWords; ++w)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(uint32_t(__cvta_generic_to_shared(&slot[w][tid]))),
+                 "l"(reinterpret_cast<const uint4*>(p) + w), "r"(count > w * 16 / int(sizeof(T)) ? 16 : 0)
+                 : "memory");
 }
 template <typename T>
-__device__ __forceinline__ Eight<T> fetched(const uint4 (&slot)[Eight<T>::kWords][kHalf], int tid) {
+__device__ __forceinline__ void put(uint4 (&slot)[Eight<T>::kWords][kFill], int tid, const Eight<T>& v) {
+#pragma unroll
+  for (int w = 0; w < Eight<T>::kWords; ++w) slot[w][tid] = v.q[w];
+}
+template <typename T>
+__device__ __forceinline__ Eight<T> fetched(const uint4 (&slot)[Eight<T>::kWords][kFill], int tid) {
   Eight<T> v;
 #pragma unroll
   for (int w = 0; w < Eight<T>::kWords; ++w) v.q[w] = slot[w][tid];
@@ -133,15 +131,16 @@ template <typename T, int NPT, int LANES>
 struct Loads {
   using Buf = Tile<NPT, LANES>;
   static constexpr int kTable = Buf::kTokens * Buf::kPieces;          // eights of a tile's B and C
-  static constexpr int kMine = (kTable + kHalf - 1) / kHalf;          // of a filling thread
+  static constexpr int kMine = (kTable + kFill - 1) / kFill;            // of a filling thread
   static constexpr bool kFetched = Buf::kStates >= 8 && kMine <= 4;
   using R = Ring<T, kFetched ? kMine : 0>;
   static constexpr int kSmem = 2 * int(sizeof(Buf)) + int(sizeof(R));
 };
 
-// ENDS: the first launch of a row in chunks (end states and sums of dt, no y).  VEC: every tensor can be read by 16 bytes.
-template <typename T, int NPT, int LANES, bool ENDS, bool VEC>
-__global__ void __launch_bounds__(2 * kHalf)
+// ENDS: the first launch of a row in chunks (end states and sums of dt, no y).  VEC: every tensor can be read by 16 bytes.  ALONE:
+// no other block on the SM.
+template <typename T, int NPT, int LANES, bool ALONE, bool ENDS, bool VEC>
+__global__ void __launch_bounds__(kScan + kFill)
 scan_kernel(const ScanJob job) {
   using Buf = Tile<NPT, LANES>;
   using Load = Loads<T, NPT, LANES>;
@@ -158,9 +157,9 @@ scan_kernel(const ScanJob job) {
   const int t0 = chunk * job.cut.tokens, t1 = min(t0 + job.cut.tokens, p.L), te = min(t1, len);
   const int tiles = te > t0 ? (te - t0 + Buf::kTokens - 1) / Buf::kTokens : 0;
 
-  if (threadIdx.x >= kHalf) {
+  if (threadIdx.x >= kScan) {
     // A filling thread has one token of a tile and eight channels.
-    const int tid = threadIdx.x - kHalf;
+    const int tid = threadIdx.x - kScan;
     const int dt0 = tid / Buf::kChunks, eight = tid % Buf::kChunks;
     const int c = c0 + eight * 8;
     const int have = dt0 < Buf::kTokens ? min(max(c1 - c, 0), 8) : 0;   // channels of this thread
@@ -179,7 +178,7 @@ scan_kernel(const ScanJob job) {
     constexpr int kMine = Load::kMine;
     auto& ring = *reinterpret_cast<typename Load::R*>(smem_raw + 2 * sizeof(Buf));
     auto source = [&](int i, int m, const T*& from, long long& stride) -> int {
-      const int e = tid + m * kHalf, dt = e / Buf::kPieces, j = e % Buf::kPieces * 8, t = t0 + i * Buf::kTokens + dt;
+      const int e = tid + m * kFill, dt = e / Buf::kPieces, j = e % Buf::kPieces * 8, t = t0 + i * Buf::kTokens + dt;
       const bool is_c = j >= Buf::kStates;
       const int s = is_c ? j - Buf::kStates : j;
       const bool in = e < Load::kTable && t < te && s < p.S && !(ENDS && is_c);
@@ -188,28 +187,48 @@ scan_kernel(const ScanJob job) {
       from = static_cast<const T*>(is_c ? p.Cm : p.B) + (in ? n * st[0] + t * st[1] + g * st[2] + s * st[3] : 0);
       return in ? min(p.S - s, 8) : 0;
     };
-    auto put = [&](int i, int m, const Eight<T>& v) {
-      const int e = tid + m * kHalf;
+    auto tabulate = [&](int i, int m, const Eight<T>& v) {
+      const int e = tid + m * kFill;
       if (e >= Load::kTable) return;
       float4* to = reinterpret_cast<float4*>(&buf[i & 1].bc[e / Buf::kPieces][e % Buf::kPieces * 8]);
       to[0] = make_float4(v.at(0), v.at(1), v.at(2), v.at(3));
       to[1] = make_float4(v.at(4), v.at(5), v.at(6), v.at(7));
     };
+    // values that cannot be copied asynchronously wait in registers until the next tile is asked for
+    constexpr int kEights = Load::kFetched ? kMine : 1;
+    Eight<T> wait_u, wait_d, wait_z, wait_bc[kEights];
+    auto settle = [&](int i) {
+      if (i < 0 || i >= tiles) return;
+      put(ring.u[i % kLongSlots], tid, wait_u);
+      put(ring.delta[i % kSlots], tid, wait_d);
+      if (!ENDS && p.z != nullptr) put(ring.z[i % kLongSlots], tid, wait_z);
+      if constexpr (Load::kFetched) {
+#pragma unroll
+        for (int m = 0; m < kMine; ++m) put(ring.bc[i % kSlots][m], tid, wait_bc[m]);
+      }
+    };
     auto load = [&](int i) {
+      if constexpr (!VEC) settle(i - 1);
       if (i < tiles) {
         const int got = first + (long long)i * Buf::kTokens < te ? have : 0;
-        const long long at = got > 0 ? (long long)i * Buf::kTokens : 0;   // (an address inside the row, read or not)
-        fetch<VEC, T>(ring.u[i % kLongSlots], tid, got > 0 ? u + at * p.u_s[1] : static_cast<const T*>(p.u), p.u_s[2], got);
-        fetch<VEC, T>(ring.delta[i % kSlots], tid, got > 0 ? delta + at * p.delta_s[1] : static_cast<const T*>(p.delta), p.delta_s[2], got);
-        if (!ENDS && p.z != nullptr)
-          fetch<VEC, T>(ring.z[i % kLongSlots], tid, got > 0 ? z + at * p.z_s[1] : static_cast<const T*>(p.z), p.z_s[2], got);
+        const long long at = got > 0 ? (long long)i * Buf::kTokens : 0;
+        if constexpr (VEC) {   // (an address inside the tensor, read or not)
+          fetch<T>(ring.u[i % kLongSlots], tid, got > 0 ? u + at * p.u_s[1] : static_cast<const T*>(p.u), got);
+          fetch<T>(ring.delta[i % kSlots], tid, got > 0 ? delta + at * p.delta_s[1] : static_cast<const T*>(p.delta), got);
+          if (!ENDS && p.z != nullptr) fetch<T>(ring.z[i % kLongSlots], tid, got > 0 ? z + at * p.z_s[1] : static_cast<const T*>(p.z), got);
+        } else {
+          wait_u.template load<false>(u + at * p.u_s[1], p.u_s[2], got);
+          wait_d.template load<false>(delta + at * p.delta_s[1], p.delta_s[2], got);
+          if (!ENDS && p.z != nullptr) wait_z.template load<false>(z + at * p.z_s[1], p.z_s[2], got);
+        }
         if constexpr (Load::kFetched) {
 #pragma unroll
           for (int m = 0; m < kMine; ++m) {
             const T* from;
             long long stride;
             const int count = source(i, m, from, stride);
-            fetch<VEC, T>(ring.bc[i % kSlots][m], tid, from, stride, count);
+            if constexpr (VEC) fetch<T>(ring.bc[i % kSlots][m], tid, from, count);
+            else wait_bc[m].template load<false>(from, stride, count);
           }
         }
       }
@@ -220,7 +239,7 @@ scan_kernel(const ScanJob job) {
       if constexpr (VEC) asm volatile("cp.async.wait_group %0;" ::"n"(kPrefetch - 1) : "memory");
       if constexpr (Load::kFetched) {
 #pragma unroll
-        for (int m = 0; m < kMine; ++m) put(i, m, fetched<T>(ring.bc[i % kSlots][m], tid));
+        for (int m = 0; m < kMine; ++m) tabulate(i, m, fetched<T>(ring.bc[i % kSlots][m], tid));
       } else if constexpr (Buf::kStates >= 8) {
         for (int m = 0; m < kMine; m += 4) {
           Eight<T> v[4];
@@ -233,7 +252,7 @@ scan_kernel(const ScanJob job) {
             else v[q].clear();
           }
 #pragma unroll
-          for (int q = 0; q < 4; ++q) put(i, m + q, v[q]);
+          for (int q = 0; q < 4; ++q) tabulate(i, m + q, v[q]);
         }
       } else {
         const int t = t0 + i * Buf::kTokens + tid;                       // at most four states: an eight is a token's B and C
@@ -248,7 +267,7 @@ scan_kernel(const ScanJob job) {
               v.set(k, (static_cast<const T*>(k >= Buf::kStates ? p.Cm : p.B) + n * st[0] + t * st[1] + g * st[2])[s * st[3]]);
           }
         }
-        put(i, 0, v);
+        tabulate(i, 0, v);
       }
       if (dt0 < Buf::kTokens) {
         const int got = first + (long long)i * Buf::kTokens < te ? have : 0, turn = Buf::turn(dt0, eight);
@@ -314,7 +333,7 @@ scan_kernel(const ScanJob job) {
       // padding
       T* row = static_cast<T*>(p.y) + n * p.y_s[0];
       const int span = min(c1 - c0, Buf::kChannels);
-      for (long long e = tid; e < (long long)(t1 - max(t0, len)) * span; e += kHalf)
+      for (long long e = tid; e < (long long)(t1 - max(t0, len)) * span; e += kFill)
         row[(max(t0, len) + e / span) * p.y_s[1] + (c0 + e % span) * p.y_s[2]] = from_f32<T>(0.0f);
     }
     return;
@@ -415,9 +434,84 @@ scan_kernel(const ScanJob job) {
       for (int q = 0; q < kKeep; ++q)
         if (part < kQ) to[(at + q) * 8] = v[q];
     };
-    if constexpr (NPT <= 4) {
-      // A warp alone on its SM quarter has only itself to hide latencies behind: the decays of kQ tokens are taken while the
-      // states go through the kQ before them, and sums are exchanged kQ tokens late.
+    if constexpr (ALONE) {
+      // One scanning warp to an SM quarter has only itself to hide latencies behind: what it reads of four tokens, and their decays,
+      // are on their way, in this order, while the states go through the four before them (8192 x 4096: 284 us, 304 as below).
+      struct Ahead {
+        float dt[kQ], du[kQ];
+        F2 B[kQ][kPairs], C[kQ][kPairs];
+      };
+      auto lds2 = [](const void* p, float& a, float& b) {
+        asm volatile("ld.shared.v2.f32 {%0,%1}, [%2];" : "=f"(a), "=f"(b) : "r"(uint32_t(__cvta_generic_to_shared(p))));
+      };
+      auto lds4 = [](const void* p, F2& a, F2& b) {
+        asm volatile("ld.shared.v2.b64 {%0,%1}, [%2];" : "=l"(a), "=l"(b) : "r"(uint32_t(__cvta_generic_to_shared(p))));
+      };
+      auto vex2 = [](float v) {
+        float r;
+        asm volatile("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+        return r;
+      };
+      auto ahead = [&](int t, Ahead& n) {
+#pragma unroll
+        for (int q = 0; q < kQ; ++q) lds2(&b.step[t + q][eight * 8 + (in_eight ^ Buf::turn(t + q, eight))], n.dt[q], n.du[q]);
+#pragma unroll
+        for (int q = 0; q < kQ; ++q) {
+#pragma unroll
+          for (int s = 0; s < kPairs; s += 2) {
+            lds4(&b.bc[t + q][s0 + 2 * s], n.B[q][s], n.B[q][s + 1]);
+            if constexpr (!ENDS) lds4(&b.bc[t + q][Buf::kStates + s0 + 2 * s], n.C[q][s], n.C[q][s + 1]);
+          }
+        }
+      };
+      Ahead now, next;
+      F2 e[kQ][kPairs], f[kQ][kPairs];
+      float v[kQ], w[kQ];
+      ahead(0, now);
+#pragma unroll
+      for (int q = 0; q < kQ; ++q) {
+        if constexpr (ENDS) sum += now.dt[q];
+#pragma unroll
+        for (int s = 0; s < kPairs; ++s) {
+          float x0, x1;
+          f2_split(f2_mul(f2_pack(now.dt[q], now.dt[q]), a[s]), x0, x1);
+          e[q][s] = f2_pack(vex2(x0), vex2(x1));
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < Buf::kTokens; t += kQ) {
+        const bool more = t + kQ < Buf::kTokens;
+        if (more) ahead(t + kQ, next);
+#pragma unroll
+        for (int q = 0; q < kQ; ++q) {
+          F2 y2 = 0;
+#pragma unroll
+          for (int s = 0; s < kPairs; ++s) {
+            if (more) {
+              float x0, x1;
+              f2_split(f2_mul(f2_pack(next.dt[q], next.dt[q]), a[s]), x0, x1);
+              f[q][s] = f2_pack(vex2(x0), vex2(x1));
+            }
+            h[s] = f2_fma(h[s], e[q][s], f2_mul(f2_pack(now.du[q], now.du[q]), now.B[q][s]));
+            if constexpr (!ENDS) y2 = s == 0 ? f2_mul(h[s], now.C[q][s]) : f2_fma(h[s], now.C[q][s], y2);
+          }
+          if constexpr (ENDS) { if (more) sum += next.dt[q]; }
+          float y0, y1;
+          f2_split(y2, y0, y1);
+          w[q] = y0 + y1;
+        }
+        if (!ENDS && t > 0) give(t - kQ, v);
+#pragma unroll
+        for (int q = 0; q < kQ; ++q) {
+          v[q] = w[q];
+#pragma unroll
+          for (int s = 0; s < kPairs; ++s) e[q][s] = f[q][s];
+        }
+        now = next;
+      }
+      if constexpr (!ENDS) give(Buf::kTokens - kQ, v);
+    } else if constexpr (NPT <= 4) {
+      // The decays of kQ tokens are taken while the states go through the kQ before them, and sums are exchanged kQ tokens late.
       F2 e[kQ][kPairs];
       float v[kQ], du[kQ];
 #pragma unroll
@@ -476,16 +570,17 @@ scan_kernel(const ScanJob job) {
 }
 
 // Threads of a channel.
-int lanes_of(int S) { return S <= 4 ? 1 : S <= 8 ? 2 : S <= 64 ? 4 : S <= 128 ? 8 : 16; }
+int lanes_of(int S) { return S <= 4 ? 1 : S <= 8 ? 2 : S <= 32 ? 4 : S <= 128 ? 8 : 16; }
 
 // How many chunks a row is cut into: the fewest clocks by what was measured for 16 states. A token costs the m blocks that
 // share an SM 57 m + 16 clocks (73 for one alone, where latencies show), the first launch of a row in chunks 0.65 of that for
 // all but the last chunk, and there is some 4 us in a second launch. 8192 x 1024: 310 us whole, 158 in 4, 121 in 16 chunks;
 // 8192 x 4096: 317 us whole, 389 in 4, 360 in 16.
 Cut cut_of(const ScanParams& p) {
-  const int channels = 128 / lanes_of(p.S), per_group = p.C / p.G, sms = current_sm_count();
+  const int channels = kScan / lanes_of(p.S), per_group = p.C / p.G, sms = current_sm_count();
   const double blocks = double(p.N) * p.G * ((per_group + channels - 1) / channels);
-  auto token = [&](double b) { return 57.0 * ceil(b / sms) + 16.0; };
+  const double states = p.S <= 16 ? 1.0 : p.S <= 32 ? 1.5 : p.S <= 64 ? 1.9 : 3.8;   // what a block's token costs with more states
+  auto token = [&](double b) { return (57.0 * ceil(b / sms) + 16.0) * states; };
   Cut best{1, p.L};
   double least = p.L * token(blocks);
   for (int k = 2; k <= 16; ++k) {
@@ -516,17 +611,25 @@ bool by_eights(const ScanParams& p) {
          ok(p.y, p.y_s, 2, 3) && (p.z == nullptr || ok(p.z, p.z_s, 2, 3)) && ok(p.B, p.b_s, 3, 4) && ok(p.Cm, p.c_s, 3, 4);
 }
 
-template <typename T, int NPT, int LANES, bool ENDS, bool VEC>
-cudaError_t run(const ScanJob& job, cudaStream_t stream) {
+template <typename T, int NPT, int LANES, bool ALONE, bool ENDS, bool VEC>
+cudaError_t run(const ScanJob& job, long long blocks, cudaStream_t stream) {
   static std::atomic<uint64_t> done;
   // No more blocks than SMs: each asks for more than half of an SM's shared memory, or two may share one beside an idle one.
   constexpr int kAlone = 116 * 1024, kNeeds = Loads<T, NPT, LANES>::kSmem, kMost = kNeeds > kAlone ? kNeeds : kAlone;
-  auto* kernel = scan_kernel<T, NPT, LANES, ENDS, VEC>;
+  auto* kernel = scan_kernel<T, NPT, LANES, ALONE, ENDS, VEC>;
   const cudaError_t e = allow_smem(kernel, kMost, done);
   if (e != cudaSuccess) return e;
+  return launch_seq(kernel, dim3(unsigned(blocks)), kScan + kFill, blocks <= current_sm_count() ? kMost : kNeeds, 1, stream, job);
+}
+
+template <typename T, int NPT, int LANES, bool ENDS>
+cudaError_t run(const ScanJob& job, bool vec, cudaStream_t stream) {
   const long long blocks = (long long)job.p.N * (ENDS ? job.cut.chunks - 1 : job.cut.chunks) * job.p.G * job.blocks_per_group;
   if (blocks > 0x7fffffffll) return cudaErrorInvalidConfiguration;
-  return launch_seq(kernel, dim3(unsigned(blocks)), 2 * kHalf, blocks <= current_sm_count() ? kMost : kNeeds, 1, stream, job);
+  if constexpr (NPT == 4)
+    if (vec && blocks <= current_sm_count()) return run<T, NPT, LANES, true, ENDS, NPT * LANES >= 8>(job, blocks, stream);
+  constexpr bool kVec = NPT * LANES >= 8;
+  return vec ? run<T, NPT, LANES, false, ENDS, kVec>(job, blocks, stream) : run<T, NPT, LANES, false, ENDS, false>(job, blocks, stream);
 }
 
 template <typename T, int NPT, int LANES>
@@ -534,17 +637,16 @@ cudaError_t go(const ScanParams& p, cudaStream_t stream) {
   ScanJob job;
   job.p = p;
   job.cut = cut_of(p);
-  const int per_group = p.C / p.G, channels = kHalf / LANES;
+  const int per_group = p.C / p.G, channels = kScan / LANES;
   job.blocks_per_group = (per_group + channels - 1) / channels;
   job.ends = static_cast<float*>(p.workspace);
   job.sums = job.ends == nullptr ? nullptr : job.ends + (long long)p.N * (job.cut.chunks - 1) * p.C * p.S;
-  constexpr bool kVec = NPT * LANES >= 8;
-  const bool vec = kVec && by_eights<T>(p);
+  const bool vec = NPT * LANES >= 8 && by_eights<T>(p);
   if (job.cut.chunks > 1) {
-    const cudaError_t e = vec ? run<T, NPT, LANES, true, kVec>(job, stream) : run<T, NPT, LANES, true, false>(job, stream);
+    const cudaError_t e = run<T, NPT, LANES, true>(job, vec, stream);
     if (e != cudaSuccess) return e;
   }
-  return vec ? run<T, NPT, LANES, false, kVec>(job, stream) : run<T, NPT, LANES, false, false>(job, stream);
+  return run<T, NPT, LANES, false>(job, vec, stream);
 }
 
 template <typename T>
@@ -553,7 +655,7 @@ cudaError_t scan(const ScanParams& p, cudaStream_t stream) {
   if (p.S <= 8) return go<T, 4, 2>(p, stream);
   if (p.S <= 16) return go<T, 4, 4>(p, stream);
   if (p.S <= 32) return go<T, 8, 4>(p, stream);
-  if (p.S <= 64) return go<T, 16, 4>(p, stream);
+  if (p.S <= 64) return go<T, 8, 8>(p, stream);
   if (p.S <= 128) return go<T, 16, 8>(p, stream);
   return go<T, 16, 16>(p, stream);
 }
