@@ -5,16 +5,16 @@
 // Tokens lie one after another with their channels together ([N, L, C], as a product of tokens with a weight matrix leaves
 // them); the state between calls is the last width - 1 inputs, [N, width - 1, C].
 //
-// Bound by memory. A thread takes a vector of 16 bytes of channels and walks a run of tokens, four at a time: their vectors are
-// loaded at once, the width - 1 before them are still in its registers, and every value is widened to fp32 once. What a run reads
-// of its predecessor's tokens is in the cache.
+// Bound by memory. A thread takes a vector of 16 bytes of channels and walks a run of tokens, four at a time: the width - 1 before
+// them are still in its registers, and every value is widened to fp32 once. The next twelve tokens' vectors are on their way
+// into slots of shared memory that are the thread's own. What a run reads of its predecessor's tokens is in the cache.
 #include "group_norm.cuh"
 
 namespace fdnn {
 namespace {
 
 constexpr int kThreads = 256, kLanes = 32;      // a block: 32 vectors of channels x 8 runs
-constexpr int kStep = 4;                        // tokens at a time
+constexpr int kStep = 4, kAhead = 3;            // tokens at a time, and how many times that is on its way
 
 __device__ __forceinline__ int length_of(const int* lengths, int n, int L) {
   return lengths == nullptr ? L : min(max(lengths[n], 0), L);
@@ -66,6 +66,7 @@ __device__ __forceinline__ void taps_of(const CausalConvParams& p, int c, F2 (&w
 template <typename T, int V, int W>
 __global__ void __launch_bounds__(kThreads, 2)
 causal_conv_kernel(const ConvJob job) {
+  extern __shared__ __align__(16) unsigned char raw[];
   chained();
   const CausalConvParams& p = job.p;
   constexpr int P = Pack<T, V>::kPairs;
@@ -88,16 +89,26 @@ causal_conv_kernel(const ConvJob job) {
     F2 w[W][P], b[P];
     taps_of<T, V, W>(p, c, w, b);
     Pack<T, V> x[W - 1 + kStep];
+    const T* from = static_cast<const T*>(p.x) + n * p.x_s[0] + c * p.x_s[2];
+    Pack<T, V>* slot = reinterpret_cast<Pack<T, V>*>(raw) + threadIdx.x;   // this thread's, kThreads apart
+    auto ask = [&](int t, int at) {
+#pragma unroll
+      for (int q = 0; q < kStep; ++q)
+        async_load(slot + (at + q) * kThreads, from + (t + q < te ? (long long)(t + q) * p.x_s[1] : 0), t + q < te);
+      async_commit();
+    };
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) ask(t0 + k * kStep, k * kStep);
 #pragma unroll
     for (int j = 0; j < W - 1; ++j) x[j] = input_at<T, V, W>(p, n, t0 + j, c);
-    const T* from = static_cast<const T*>(p.x) + n * p.x_s[0] + c * p.x_s[2];
+    int at = 0;
     with_activation(p.act, [&](auto act) {
       for (int t = t0; t < te; t += kStep) {
+        async_wait<kAhead - 1>();
 #pragma unroll
-        for (int q = 0; q < kStep; ++q) {
-          x[W - 1 + q].clear();
-          if (t + q < te) x[W - 1 + q].load(from + (long long)(t + q) * p.x_s[1]);
-        }
+        for (int q = 0; q < kStep; ++q) x[W - 1 + q] = slot[(at + q) * kThreads];
+        ask(t + kAhead * kStep, at);
+        at = at == (kAhead - 1) * kStep ? 0 : at + kStep;
         Pack<T, V> out[kStep];
 #pragma unroll
         for (int i = 0; i < P; ++i) {
@@ -189,7 +200,8 @@ cudaError_t go(const CausalConvParams& p, cudaStream_t stream) {
   if (job.items == 0) return cudaSuccess;
   const long long blocks = (job.items + kThreads / kLanes - 1) / (kThreads / kLanes) * tiles;
   if (blocks > 0x7fffffffll) return cudaErrorInvalidConfiguration;
-  return launch_seq(causal_conv_kernel<T, V, W>, dim3(unsigned(blocks)), kThreads, 0, 1, stream, job);
+  return launch_seq(causal_conv_kernel<T, V, W>, dim3(unsigned(blocks)), kThreads, kAhead * kStep * kThreads * Pack<T, V>::kBytes, 1, stream,
+                    job);
 }
 
 template <typename T, int V, int W>
