@@ -359,7 +359,7 @@ scan_kernel(const ScanJob job) {
         const float sum = job.sums[at];
 #pragma unroll
         for (int s = 0; s < NPT; ++s)
-          if (s0 + s < p.S) hv[s] = hv[s] * ex2(sum * av[s]) + job.ends[at * p.S + s0 + s];
+          if (s0 + s < p.S) hv[s] = hv[s] * decay_of(sum, av[s]) + job.ends[at * p.S + s0 + s];
       }
     }
 #pragma unroll
@@ -368,6 +368,7 @@ scan_kernel(const ScanJob job) {
       h[s] = f2_pack(hv[2 * s], hv[2 * s + 1]);
     }
   }
+  const F2 middle = f2_both(kDecayMiddle);
   const int eight = cl / 8, in_eight = cl % 8;
   float sum = 0.0f;
   for (int i = 0; i < tiles; ++i) {
@@ -380,7 +381,7 @@ scan_kernel(const ScanJob job) {
 #pragma unroll
       for (int s = 0; s < kPairs; ++s) {
         float x0, x1;
-        f2_split(f2_mul(f2_pack(st.x, st.x), a[s]), x0, x1);
+        f2_split(f2_fma(f2_pack(st.x, st.x), a[s], middle), x0, x1);
         e[s] = f2_pack(ex2(x0), ex2(x1));
       }
     };
@@ -474,7 +475,7 @@ scan_kernel(const ScanJob job) {
 #pragma unroll
         for (int s = 0; s < kPairs; ++s) {
           float x0, x1;
-          f2_split(f2_mul(f2_pack(now.dt[q], now.dt[q]), a[s]), x0, x1);
+          f2_split(f2_fma(f2_pack(now.dt[q], now.dt[q]), a[s], middle), x0, x1);
           e[q][s] = f2_pack(vex2(x0), vex2(x1));
         }
       }
@@ -489,7 +490,7 @@ scan_kernel(const ScanJob job) {
           for (int s = 0; s < kPairs; ++s) {
             if (more) {
               float x0, x1;
-              f2_split(f2_mul(f2_pack(next.dt[q], next.dt[q]), a[s]), x0, x1);
+              f2_split(f2_fma(f2_pack(next.dt[q], next.dt[q]), a[s], middle), x0, x1);
               f[q][s] = f2_pack(vex2(x0), vex2(x1));
             }
             h[s] = f2_fma(h[s], e[q][s], f2_mul(f2_pack(now.du[q], now.du[q]), now.B[q][s]));

@@ -95,10 +95,10 @@ scan_step_kernel(const ScanParams p, float* state, int n_slots, const int* slots
       for (int k = 0; k < CHUNKS; ++k) {
         const int s = (k * LANES + part) * 4;
         float4 v;
-        v.x = h[r][k].x * ex2(d * a[k].x) + du * b[r][k].at(0);
-        v.y = h[r][k].y * ex2(d * a[k].y) + du * b[r][k].at(1);
-        v.z = h[r][k].z * ex2(d * a[k].z) + du * b[r][k].at(2);
-        v.w = h[r][k].w * ex2(d * a[k].w) + du * b[r][k].at(3);
+        v.x = h[r][k].x * decay_of(d, a[k].x) + du * b[r][k].at(0);
+        v.y = h[r][k].y * decay_of(d, a[k].y) + du * b[r][k].at(1);
+        v.z = h[r][k].z * decay_of(d, a[k].z) + du * b[r][k].at(2);
+        v.w = h[r][k].w * decay_of(d, a[k].w) + du * b[r][k].at(3);
         // (states past S: b and m are zero, but zero times an infinite du is not)
         if (WHOLE ? s < p.S : s + 3 < p.S) {
           y += v.x * m[r][k].at(0) + v.y * m[r][k].at(1) + v.z * m[r][k].at(2) + v.w * m[r][k].at(3);

@@ -2,8 +2,8 @@
 
 Tolerances.  Outputs are rounded once to their type (unit roundoff 2^-8 bf16, 2^-11 f16, 2^-24 f32).  A convolution adds up to
 eight fp32 products: 2e-5 of the sum of their sizes, taken as 2e-5 (1 + |y|).  A scan multiplies a state by one rounded decay
-a token (relative error 2^-21 with its exponent's rounding), up to 400 tokens here: 400 * 2^-21 = 2e-4 of the state, at most, and
-the same of an output's sum of terms."""
+a token (relative error 2^-21 with its exponent's rounding): l * 2^-21 of the state, at most, and the same of an output's sum of
+terms; 2e-4 (l = 400), more for longer prompts."""
 import pytest
 import torch
 
@@ -172,6 +172,25 @@ def test_selective_scan(fd, case, dtype):
         y, got_final = fd.selective_scan(v["u"], delta, v["A"], *flat, return_final_state=True)
         near(got_final, final, torch.float32, tol)
         near(y, want, dtype, tol * s ** 0.5)
+
+
+@pytest.mark.parametrize("steps", [False, True], ids=["prompt", "steps"])
+def test_decays_have_no_drift(fd, steps):
+    """Roundings of a slow decay cancel out over many steps: a mean error of 2e-8 a step, a cut one's, is 1e-6 after 50, which
+    8192 states' mean shows (their scatter: sqrt(50) * 5e-8 / sqrt(8192) = 4e-9)."""
+    l, c, s = 50, 512, 16
+    g = torch.Generator().manual_seed(11)
+    delta = torch.empty(1, l, c).uniform_(0.01, 0.03, generator=g).cuda()
+    a = torch.empty(c, s).uniform_(-1.5, -0.5, generator=g).cuda()
+    u, bc, state = torch.zeros(1, l, c, device="cuda"), torch.ones(1, l, s, device="cuda"), torch.ones(1, c, s, device="cuda")
+    if steps:
+        for t in range(l):
+            fd.selective_scan_step(u[:, t], delta[:, t], a, bc[:, t], bc[:, t], state)
+    else:
+        state = fd.selective_scan(u, delta, a, bc, bc, initial_state=state, return_final_state=True)[1]
+    want = torch.exp(delta.double().sum(1)[..., None] * a.double())
+    drift = float((state.double() / want - 1).mean())
+    assert abs(drift) < l * 1e-8, drift
 
 
 def test_a_long_prompt_equals_its_parts(fd):
