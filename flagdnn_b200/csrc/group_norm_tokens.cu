@@ -1,7 +1,7 @@
 // Group norm over rows of tokens: x [N, C] with its channels together, statistics over the c = C / G values of a group of one row.
 //
-// Bound by memory.  A group is an even share of a warp (up to 32 lanes, up to kEach vectors of 16 bytes a lane), so that a
-// token's groups are reduced by shuffles alone; a lane keeps its channels' parameters and walks over tokens, the values of
+// Bound by memory.  A group is an even share of a warp (up to 32 lanes, as many vectors of 16 bytes a lane as registers
+// hold), so that a token's groups are reduced by shuffles alone; a lane keeps its channels' parameters and walks over tokens, the values of
 // the next ones on their way.  Mean first, then squared deviations from it, both from registers: x is read once.
 //
 // The gradient's row sums need nothing else.  dweight and dbias are sums over the rows: a lane adds up those of its channels in
@@ -17,6 +17,7 @@ constexpr int kThreads = 256, kWarps = kThreads / 32;
 struct TokenParams {
   NormParams p;
   int units, lanes;      // vectors of a group, lanes that share it (a power of two)
+  int side;              // tokens of a block side by side, where all groups leave room for more (else 1)
   int slices;            // of the tokens
   float2* rows;          // backward: [slices, C]
 };
@@ -27,27 +28,33 @@ __device__ __forceinline__ float lane_sum(float v, int lanes) {
   return v;
 }
 
-// Where a thread works: its group and its vectors of it.
-template <int EACH>
+// Where a thread works: its token of those side by side (SIDE), its group and its vectors of it.
+template <int EACH, bool SIDE>
 struct Seat {
-  int g, u0;
+  int token, g, u0;
   bool live;
   __device__ Seat(const TokenParams& t) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, groups = 32 / t.lanes;
     g = (blockIdx.x * kWarps + warp) * groups + lane / t.lanes;
+    token = 0;
+    if (SIDE) {
+      token = g / t.p.G;
+      g -= token * t.p.G;
+    }
     u0 = lane % t.lanes;
-    live = g < t.p.G;
-    if (!live) g = 0;
+    live = g < t.p.G && (!SIDE || token < t.side);
+    if (!live) g = token = 0;
   }
   __device__ bool in(const TokenParams& t, int e) const { return live && u0 + e * t.lanes < t.units; }
 };
 
-template <typename T, int V, int EACH, int TOKENS>
+template <typename T, int V, int EACH, int TOKENS, bool SIDE = false>
 __global__ void __launch_bounds__(kThreads)
 norm_tokens_kernel(const TokenParams t) {
   chained();
   const NormParams& p = t.p;
-  const Seat<EACH> seat(t);
+  const Seat<EACH, SIDE> seat(t);
+  const int side = SIDE ? t.side : 1;
   const int cpg = p.C / p.G;
   constexpr int P = Pack<T, V>::kPairs;
   F2 w[EACH][P], b[EACH][P];
@@ -59,11 +66,13 @@ norm_tokens_kernel(const TokenParams t) {
   }
   const float m = float(cpg);
   with_activation(p.act, [&](auto act) {
-    for (long long n0 = (long long)blockIdx.y * TOKENS; n0 < p.N; n0 += (long long)gridDim.y * TOKENS) {
+    // tokens n0, n0 + side, ...: the same number of rounds for all of a warp, whose lanes sum together
+    for (long long first = (long long)blockIdx.y * TOKENS * side; first < p.N; first += (long long)gridDim.y * TOKENS * side) {
+      const long long n0 = first + seat.token;
       Pack<T, V> x[TOKENS][EACH];
 #pragma unroll
       for (int k = 0; k < TOKENS; ++k) {
-        const long long n = n0 + k < p.N ? n0 + k : p.N - 1;
+        const long long n = n0 + k * side < p.N ? n0 + k * side : p.N - 1;
 #pragma unroll
         for (int e = 0; e < EACH; ++e) {
           x[k][e].clear();
@@ -93,10 +102,11 @@ norm_tokens_kernel(const TokenParams t) {
         }
         const float rstd = rsqrtf(lane_sum(m2, t.lanes) / m + p.eps);
         const F2 scale = f2_both(rstd);
-        if (n0 + k >= p.N) continue;
+        const long long n = n0 + k * side;
+        if (n >= p.N) continue;
         if (p.mean != nullptr && seat.live && seat.u0 == 0) {
-          p.mean[(n0 + k) * p.G + seat.g] = mean;
-          p.rstd[(n0 + k) * p.G + seat.g] = rstd;
+          p.mean[n * p.G + seat.g] = mean;
+          p.rstd[n * p.G + seat.g] = rstd;
         }
 #pragma unroll
         for (int e = 0; e < EACH; ++e) {
@@ -105,19 +115,20 @@ norm_tokens_kernel(const TokenParams t) {
 #pragma unroll
           for (int i = 0; i < P; ++i)
             y.set_pair(i, activate2<decltype(act)::value>(f2_fma(f2_mul(f2_add(x[k][e].pair(i), minus), scale), w[e][i], b[e][i])));
-          y.store(static_cast<T*>(p.y) + (n0 + k) * p.y_s[0] + at[e]);
+          y.store(static_cast<T*>(p.y) + n * p.y_s[0] + at[e]);
         }
       }
     }
   });
 }
 
-template <typename T, int V, int EACH, int TOKENS>
+template <typename T, int V, int EACH, int TOKENS, bool SIDE = false>
 __global__ void __launch_bounds__(kThreads)
 norm_tokens_backward_kernel(const TokenParams t) {
   chained();
   const NormParams& p = t.p;
-  const Seat<EACH> seat(t);
+  const Seat<EACH, SIDE> seat(t);
+  const int side = SIDE ? t.side : 1;
   const int cpg = p.C / p.G;
   constexpr int P = Pack<T, V>::kPairs;
   F2 w[EACH][P], b[EACH][P], dw[EACH][P], db[EACH][P];
@@ -131,13 +142,15 @@ norm_tokens_backward_kernel(const TokenParams t) {
   }
   const float inv = 1.0f / float(cpg);
   with_activation(p.act, [&](auto act) {
-    for (long long n0 = (long long)blockIdx.y * TOKENS; n0 < p.N; n0 += (long long)gridDim.y * TOKENS) {
+    // tokens n0, n0 + side, ...: the same number of rounds for all of a warp, whose lanes sum together
+    for (long long first = (long long)blockIdx.y * TOKENS * side; first < p.N; first += (long long)gridDim.y * TOKENS * side) {
+      const long long n0 = first + seat.token;
       Pack<T, V> x[TOKENS][EACH], dy[TOKENS][EACH];
       float mean[TOKENS], rstd[TOKENS];
 #pragma unroll
       for (int k = 0; k < TOKENS; ++k) {
-        const bool there = n0 + k < p.N;
-        const long long n = there ? n0 + k : p.N - 1;
+        const bool there = n0 + k * side < p.N;
+        const long long n = there ? n0 + k * side : p.N - 1;
         mean[k] = p.mean[n * p.G + seat.g];
         rstd[k] = p.rstd[n * p.G + seat.g];
 #pragma unroll
@@ -152,7 +165,7 @@ norm_tokens_backward_kernel(const TokenParams t) {
       }
 #pragma unroll
       for (int k = 0; k < TOKENS; ++k) {
-        const bool there = n0 + k < p.N;
+        const bool there = n0 + k * side < p.N;
         const F2 minus = f2_both(-mean[k]), scale = f2_both(rstd[k]);
         F2 xh[EACH][P], g[EACH][P], t1 = 0, t2 = 0;
 #pragma unroll
@@ -179,32 +192,48 @@ norm_tokens_backward_kernel(const TokenParams t) {
           Pack<T, V> dx;
 #pragma unroll
           for (int i = 0; i < P; ++i) dx.set_pair(i, f2_mul(scale, f2_fma(xh[e][i], f2_both(-s2), f2_add(g[e][i], f2_both(-s1)))));
-          dx.store(static_cast<T*>(p.dx) + (n0 + k) * p.dx_s[0] + at[e]);
+          dx.store(static_cast<T*>(p.dx) + (n0 + k * side) * p.dx_s[0] + at[e]);
         }
       }
     }
   });
-  // the block's part of a row of sums; every channel has one lane
+  // the block's part of a row of sums; every channel has one lane, or one for each of the tokens side by side
+  float2* row = t.rows + (long long)blockIdx.y * p.C;
+  extern __shared__ __align__(16) unsigned char raw[];
+  float2* to = SIDE ? reinterpret_cast<float2*>(raw) + seat.token * p.C : row;
 #pragma unroll
   for (int e = 0; e < EACH; ++e) {
     if (!seat.in(t, e)) continue;
-    float2* to = t.rows + (long long)blockIdx.y * p.C + at[e];
 #pragma unroll
     for (int i = 0; i < P; ++i) {
       float w0, w1, b0, b1;
       f2_split(dw[e][i], w0, w1);
       f2_split(db[e][i], b0, b1);
-      to[2 * i] = make_float2(w0, b0);
-      if (V > 1) to[2 * i + 1] = make_float2(w1, b1);
+      to[at[e] + 2 * i] = make_float2(w0, b0);
+      if (V > 1) to[at[e] + 2 * i + 1] = make_float2(w1, b1);
     }
+  }
+  if (!SIDE) return;
+  __syncthreads();
+  for (int c = threadIdx.x; c < p.C; c += kThreads) {
+    float2 v = make_float2(0.0f, 0.0f);
+    for (int k = 0; k < side; ++k) {
+      const float2 q = reinterpret_cast<const float2*>(raw)[k * p.C + c];
+      v.x += q.x;
+      v.y += q.y;
+    }
+    row[c] = v;
   }
 }
 
-// How a problem is cut; EACH vectors a lane, 0: a group is larger than a warp holds.
+// How a problem is cut; EACH vectors a lane.
 struct TokenPlan {
   TokenParams t;
   int each, blocks;
 };
+// Vectors a lane may have: what its registers hold.
+constexpr int most_each(int V, bool backward) { return V >= 8 ? 4 : backward ? (V == 4 ? 4 : V == 2 ? 8 : 16) : V == 4 ? 8 : 16; }
+
 TokenPlan plan_of(const NormParams& p, int V, int tokens, int per_sm) {
   TokenPlan plan;
   plan.t.p = p;
@@ -212,11 +241,17 @@ TokenPlan plan_of(const NormParams& p, int V, int tokens, int per_sm) {
   plan.t.lanes = 1;
   while (plan.t.lanes < 32 && plan.t.lanes < plan.t.units) plan.t.lanes *= 2;
   const int each = (plan.t.units + plan.t.lanes - 1) / plan.t.lanes;
-  plan.each = each <= 1 ? 1 : each <= 2 ? 2 : each <= 4 ? 4 : 0;
+  for (plan.each = 1; plan.each < each;) plan.each *= 2;
   const int groups = kWarps * (32 / plan.t.lanes);
   plan.blocks = (p.G + groups - 1) / groups;
+  // few groups: several tokens to a block, as far as their sums of the parameters' gradients fit a block's 48 KB
+  plan.t.side = groups / p.G;
+  if (plan.t.side > 49152 / 8 / p.C) plan.t.side = 49152 / 8 / p.C;
+  if (plan.t.side > p.N) plan.t.side = p.N;
+  if (plan.t.side < 1) plan.t.side = 1;
   // enough blocks for every SM; more tokens are walked
-  long long slices = (p.N + tokens - 1) / tokens, room = (long long)per_sm * current_sm_count() / plan.blocks;
+  const long long at_once = (long long)tokens * plan.t.side;
+  long long slices = (p.N + at_once - 1) / at_once, room = (long long)per_sm * current_sm_count() / plan.blocks;
   if (room < 1) room = 1;
   plan.t.slices = int(slices < room ? slices : room);
   plan.t.rows = static_cast<float2*>(p.workspace);
@@ -233,16 +268,38 @@ constexpr int tokens_at_once(int each, bool backward) {
   return each == 1 ? (sizeof(T) == 2 && !backward ? 2 : 4) : each == 2 && !backward ? 2 : 1;
 }
 
+// One token at a time of each block's, or several side by side.
+template <typename T, int V, int EACH>
+cudaError_t forward_as(const TokenPlan& plan, cudaStream_t stream) {
+  constexpr int tokens = tokens_at_once<T>(EACH, false);
+  const dim3 grid(unsigned(plan.blocks), unsigned(plan.t.slices));
+  if (plan.t.side == 1) return launch_seq(norm_tokens_kernel<T, V, EACH, tokens>, grid, kThreads, 0, 1, stream, plan.t);
+  return launch_seq(norm_tokens_kernel<T, V, EACH, tokens, true>, grid, kThreads, 0, 1, stream, plan.t);
+}
+
+template <typename T, int V, int EACH>
+cudaError_t backward_as(const TokenPlan& plan, cudaStream_t stream) {
+  constexpr int tokens = tokens_at_once<T>(EACH, true);
+  const dim3 grid(unsigned(plan.blocks), unsigned(plan.t.slices));
+  if (plan.t.side == 1) return launch_seq(norm_tokens_backward_kernel<T, V, EACH, tokens>, grid, kThreads, 0, 1, stream, plan.t);
+  return launch_seq(norm_tokens_backward_kernel<T, V, EACH, tokens, true>, grid, kThreads, 8 * plan.t.side * plan.t.p.C, 1, stream, plan.t);
+}
+
 template <typename T, int V>
 cudaError_t forward(const NormParams& p, cudaStream_t stream) {
   TokenPlan plan = plan_of(p, V, 1, 1);
   plan = plan_of(p, V, tokens_at_once<T>(plan.each, false), per_sm<T>(false));
-  const dim3 grid(unsigned(plan.blocks), unsigned(plan.t.slices));
   switch (plan.each) {
-    case 1: return launch_seq(norm_tokens_kernel<T, V, 1, tokens_at_once<T>(1, false)>, grid, kThreads, 0, 1, stream, plan.t);
-    case 2: return launch_seq(norm_tokens_kernel<T, V, 2, 2>, grid, kThreads, 0, 1, stream, plan.t);
-    default: return launch_seq(norm_tokens_kernel<T, V, 4, 1>, grid, kThreads, 0, 1, stream, plan.t);
+    case 1: return forward_as<T, V, 1>(plan, stream);
+    case 2: return forward_as<T, V, 2>(plan, stream);
+    case 4: return forward_as<T, V, 4>(plan, stream);
+    default: break;
   }
+  if constexpr (most_each(V, false) >= 8)
+    if (plan.each == 8) return forward_as<T, V, 8>(plan, stream);
+  if constexpr (most_each(V, false) >= 16)
+    if (plan.each == 16) return forward_as<T, V, 16>(plan, stream);
+  return cudaErrorInvalidValue;
 }
 
 template <typename T, int V>
@@ -255,13 +312,17 @@ template <typename T, int V>
 cudaError_t backward(const NormParams& p, cudaStream_t stream) {
   const TokenPlan plan = backward_plan<T, V>(p);
   if (8ll * p.C * plan.t.slices > p.workspace_bytes) return cudaErrorInvalidValue;
-  const dim3 grid(unsigned(plan.blocks), unsigned(plan.t.slices));
-  cudaError_t e;
+  cudaError_t e = cudaErrorInvalidValue;
   switch (plan.each) {
-    case 1: e = launch_seq(norm_tokens_backward_kernel<T, V, 1, tokens_at_once<T>(1, true)>, grid, kThreads, 0, 1, stream, plan.t); break;
-    case 2: e = launch_seq(norm_tokens_backward_kernel<T, V, 2, 1>, grid, kThreads, 0, 1, stream, plan.t); break;
-    default: e = launch_seq(norm_tokens_backward_kernel<T, V, 4, 1>, grid, kThreads, 0, 1, stream, plan.t); break;
+    case 1: e = backward_as<T, V, 1>(plan, stream); break;
+    case 2: e = backward_as<T, V, 2>(plan, stream); break;
+    case 4: e = backward_as<T, V, 4>(plan, stream); break;
+    default: break;
   }
+  if constexpr (most_each(V, true) >= 8)
+    if (plan.each == 8) e = backward_as<T, V, 8>(plan, stream);
+  if constexpr (most_each(V, true) >= 16)
+    if (plan.each == 16) e = backward_as<T, V, 16>(plan, stream);
   if (e != cudaSuccess || (p.dweight == nullptr && p.dbias == nullptr)) return e;
   return launch_norm_dparams<T>(p, plan.t.rows, plan.t.slices, stream);
 }
@@ -271,7 +332,7 @@ cudaError_t backward(const NormParams& p, cudaStream_t stream) {
 // Rows of tokens whose groups fit a warp.
 bool norm_tokens_take(int dtype, const NormParams& p, bool backward) {
   const int V = norm_vector(dtype, p, backward, p.C / p.G);
-  return V > 0 && p.H == 1 && p.W == 1 && p.C / p.G <= 128 * V;
+  return V > 0 && p.H == 1 && p.W == 1 && p.C / p.G <= 32 * most_each(V, backward) * V;
 }
 
 long long norm_tokens_workspace(int dtype, const NormParams& p, bool backward) {

@@ -105,6 +105,17 @@ SHAPES = [   # shape, groups, layout
     ((9, 12000), 1, "cl"),                # a group larger than a warp holds
     ((7, 6000), 5, "cl"),
     ((65, 100), 100, "cl"),
+    ((1000, 128), 4, "cl"),               # several tokens to a block
+    ((6455, 8), 1, "cl"),
+    ((77, 12), 3, "cl"),
+    ((3, 24), 2, "cl"),
+    ((301, 1916), 4, "cl"),               # four groups of 479 channels: two tokens to a block
+    ((123, 1024), 2, "cl"),
+    ((21, 64 * 477), 64, "cl"),           # as long, and more of them than a block has warps
+    ((61, 1024), 1, "cl"),
+    ((5, 429), 1, "cl"),                  # an odd number of channels, more than a lane's of a warp
+    ((40, 906), 3, "cl"),
+    ((9, 1020), 1, "cl"),
     ((12, 36), 3, "t"),
     ((300, 640), 20, "slice"),
 ]
