@@ -22,10 +22,13 @@ struct TokenParams {
   float2* rows;          // backward: [slices, C]
 };
 
-// Sum over the lanes of a group.
-__device__ __forceinline__ float lane_sum(float v, int lanes) {
-  for (int o = lanes >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
+// Sums over the lanes of a group, of several values at once: their shuffles do not wait for one another.
+template <int K>
+__device__ __forceinline__ void lane_sums(float (&v)[K], int lanes) {
+  for (int o = lanes >> 1; o > 0; o >>= 1) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
+  }
 }
 
 // Where a thread works: its token of those side by side (SIDE), its group and its vectors of it.
@@ -49,7 +52,7 @@ struct Seat {
 };
 
 template <typename T, int V, int EACH, int TOKENS, bool SIDE = false>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, EACH == 1 ? 4 : 1)
 norm_tokens_kernel(const TokenParams t) {
   chained();
   const NormParams& p = t.p;
@@ -64,21 +67,24 @@ norm_tokens_kernel(const TokenParams t) {
     at[e] = seat.in(t, e) ? seat.g * cpg + (seat.u0 + e * t.lanes) * V : 0;
     norm_params_of<T, V>(p, at[e], seat.in(t, e), w[e], b[e]);
   }
-  const float m = float(cpg);
+  const float inv = 1.0f / float(cpg);
+  const int step = gridDim.y * TOKENS * side;
   with_activation(p.act, [&](auto act) {
-    // tokens n0, n0 + side, ...: the same number of rounds for all of a warp, whose lanes sum together
-    for (long long first = (long long)blockIdx.y * TOKENS * side; first < p.N; first += (long long)gridDim.y * TOKENS * side) {
-      const long long n0 = first + seat.token;
+    // tokens n, n + side, ...: the same number of rounds for all of a warp, whose lanes sum together
+    for (long long first = (long long)blockIdx.y * TOKENS * side; first < p.N; first += step) {
+      const int n0 = int(first) + seat.token;
       Pack<T, V> x[TOKENS][EACH];
 #pragma unroll
       for (int k = 0; k < TOKENS; ++k) {
-        const long long n = n0 + k * side < p.N ? n0 + k * side : p.N - 1;
+        const int n = n0 + k * side < p.N ? n0 + k * side : p.N - 1;
+        const T* from = static_cast<const T*>(p.x) + n * p.x_s[0];
 #pragma unroll
         for (int e = 0; e < EACH; ++e) {
           x[k][e].clear();
-          if (seat.in(t, e)) x[k][e].load(static_cast<const T*>(p.x) + n * p.x_s[0] + at[e]);
+          if (seat.in(t, e)) x[k][e].load(from + at[e]);
         }
       }
+      float mean[TOKENS], rstd[TOKENS];
 #pragma unroll
       for (int k = 0; k < TOKENS; ++k) {
         F2 sum = 0;
@@ -87,9 +93,14 @@ norm_tokens_kernel(const TokenParams t) {
 #pragma unroll
           for (int i = 0; i < P; ++i) sum = f2_add(sum, x[k][e].pair(i));
         }
-        const float mean = lane_sum(f2_sum(sum), t.lanes) / m;
-        const F2 minus = f2_pack(-mean, V == 1 ? 0.0f : -mean);
-        float m2 = 0.0f;
+        mean[k] = f2_sum(sum);
+      }
+      lane_sums(mean, t.lanes);
+#pragma unroll
+      for (int k = 0; k < TOKENS; ++k) {
+        mean[k] *= inv;
+        const F2 minus = f2_pack(-mean[k], V == 1 ? 0.0f : -mean[k]);
+        rstd[k] = 0.0f;
 #pragma unroll
         for (int e = 0; e < EACH; ++e) {
           F2 square = 0;
@@ -98,24 +109,30 @@ norm_tokens_kernel(const TokenParams t) {
             const F2 d = f2_add(x[k][e].pair(i), minus);
             square = f2_fma(d, d, square);
           }
-          m2 += seat.in(t, e) ? f2_sum(square) : 0.0f;
+          rstd[k] += seat.in(t, e) ? f2_sum(square) : 0.0f;
         }
-        const float rstd = rsqrtf(lane_sum(m2, t.lanes) / m + p.eps);
-        const F2 scale = f2_both(rstd);
-        const long long n = n0 + k * side;
-        if (n >= p.N) continue;
-        if (p.mean != nullptr && seat.live && seat.u0 == 0) {
-          p.mean[n * p.G + seat.g] = mean;
-          p.rstd[n * p.G + seat.g] = rstd;
-        }
+      }
+      lane_sums(rstd, t.lanes);
 #pragma unroll
-        for (int e = 0; e < EACH; ++e) {
-          if (!seat.in(t, e)) continue;
-          Pack<T, V> y;
+      for (int k = 0; k < TOKENS; ++k) {
+        rstd[k] = rsqrtf(rstd[k] * inv + p.eps);
+        const F2 minus = f2_both(-mean[k]), scale = f2_both(rstd[k]);
+        const int n = n0 + k * side;
+        if (n < p.N) {
+          if (p.mean != nullptr && seat.live && seat.u0 == 0) {
+            p.mean[(long long)n * p.G + seat.g] = mean[k];
+            p.rstd[(long long)n * p.G + seat.g] = rstd[k];
+          }
+          T* to = static_cast<T*>(p.y) + n * p.y_s[0];
 #pragma unroll
-          for (int i = 0; i < P; ++i)
-            y.set_pair(i, activate2<decltype(act)::value>(f2_fma(f2_mul(f2_add(x[k][e].pair(i), minus), scale), w[e][i], b[e][i])));
-          y.store(static_cast<T*>(p.y) + n * p.y_s[0] + at[e]);
+          for (int e = 0; e < EACH; ++e) {
+            if (!seat.in(t, e)) continue;
+            Pack<T, V> y;
+#pragma unroll
+            for (int i = 0; i < P; ++i)
+              y.set_pair(i, activate2<decltype(act)::value>(f2_fma(f2_mul(f2_add(x[k][e].pair(i), minus), scale), w[e][i], b[e][i])));
+            y.store(to + at[e]);
+          }
         }
       }
     }
@@ -123,7 +140,7 @@ norm_tokens_kernel(const TokenParams t) {
 }
 
 template <typename T, int V, int EACH, int TOKENS, bool SIDE = false>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, EACH == 1 ? 2 : 1)
 norm_tokens_backward_kernel(const TokenParams t) {
   chained();
   const NormParams& p = t.p;
@@ -141,58 +158,66 @@ norm_tokens_backward_kernel(const TokenParams t) {
     for (int i = 0; i < P; ++i) dw[e][i] = db[e][i] = 0;
   }
   const float inv = 1.0f / float(cpg);
+  const int step = gridDim.y * TOKENS * side;
   with_activation(p.act, [&](auto act) {
-    // tokens n0, n0 + side, ...: the same number of rounds for all of a warp, whose lanes sum together
-    for (long long first = (long long)blockIdx.y * TOKENS * side; first < p.N; first += (long long)gridDim.y * TOKENS * side) {
-      const long long n0 = first + seat.token;
+    for (long long first = (long long)blockIdx.y * TOKENS * side; first < p.N; first += step) {
+      const int n0 = int(first) + seat.token;
       Pack<T, V> x[TOKENS][EACH], dy[TOKENS][EACH];
-      float mean[TOKENS], rstd[TOKENS];
+      float mean[TOKENS], rstd[TOKENS], s[2 * TOKENS];
 #pragma unroll
       for (int k = 0; k < TOKENS; ++k) {
         const bool there = n0 + k * side < p.N;
-        const long long n = there ? n0 + k * side : p.N - 1;
-        mean[k] = p.mean[n * p.G + seat.g];
-        rstd[k] = p.rstd[n * p.G + seat.g];
+        const int n = there ? n0 + k * side : p.N - 1;
+        mean[k] = p.mean[(long long)n * p.G + seat.g];
+        rstd[k] = p.rstd[(long long)n * p.G + seat.g];
+        const T *xn = static_cast<const T*>(p.x) + n * p.x_s[0], *dyn = static_cast<const T*>(p.dy) + n * p.dy_s[0];
 #pragma unroll
         for (int e = 0; e < EACH; ++e) {
           x[k][e].clear();
           dy[k][e].clear();
           if (seat.in(t, e) && there) {
-            x[k][e].load(static_cast<const T*>(p.x) + n * p.x_s[0] + at[e]);
-            dy[k][e].load(static_cast<const T*>(p.dy) + n * p.dy_s[0] + at[e]);
+            x[k][e].load(xn + at[e]);
+            dy[k][e].load(dyn + at[e]);
           }
         }
       }
+      F2 xh[TOKENS][EACH][P], g[TOKENS][EACH][P];
 #pragma unroll
       for (int k = 0; k < TOKENS; ++k) {
-        const bool there = n0 + k * side < p.N;
         const F2 minus = f2_both(-mean[k]), scale = f2_both(rstd[k]);
-        F2 xh[EACH][P], g[EACH][P], t1 = 0, t2 = 0;
+        F2 t1 = 0, t2 = 0;
 #pragma unroll
         for (int e = 0; e < EACH; ++e) {
-          const bool in = there && seat.in(t, e);
+          const bool in = n0 + k * side < p.N && seat.in(t, e);
 #pragma unroll
           for (int i = 0; i < P; ++i) {
-            xh[e][i] = in ? f2_mul(f2_add(x[k][e].pair(i), minus), scale) : 0;
-            g[e][i] = in ? f2_mul(dy[k][e].pair(i), slope2<decltype(act)::value>(f2_fma(xh[e][i], w[e][i], b[e][i]))) : 0;
-            dw[e][i] = f2_fma(g[e][i], xh[e][i], dw[e][i]);
-            db[e][i] = f2_add(db[e][i], g[e][i]);
-            g[e][i] = f2_mul(g[e][i], w[e][i]);
-            t1 = f2_add(t1, g[e][i]);
-            t2 = f2_fma(g[e][i], xh[e][i], t2);
+            xh[k][e][i] = in ? f2_mul(f2_add(x[k][e].pair(i), minus), scale) : 0;
+            g[k][e][i] = in ? f2_mul(dy[k][e].pair(i), slope2<decltype(act)::value>(f2_fma(xh[k][e][i], w[e][i], b[e][i]))) : 0;
+            dw[e][i] = f2_fma(g[k][e][i], xh[k][e][i], dw[e][i]);
+            db[e][i] = f2_add(db[e][i], g[k][e][i]);
+            g[k][e][i] = f2_mul(g[k][e][i], w[e][i]);
+            t1 = f2_add(t1, g[k][e][i]);
+            t2 = f2_fma(g[k][e][i], xh[k][e][i], t2);
           }
         }
-        float s1 = f2_sum(t1), s2 = f2_sum(t2);
-        s1 = lane_sum(s1, t.lanes) * inv;
-        s2 = lane_sum(s2, t.lanes) * inv;
-        if (!there || p.dx == nullptr) continue;
+        s[2 * k] = f2_sum(t1);
+        s[2 * k + 1] = f2_sum(t2);
+      }
+      lane_sums(s, t.lanes);
 #pragma unroll
-        for (int e = 0; e < EACH; ++e) {
-          if (!seat.in(t, e)) continue;
-          Pack<T, V> dx;
+      for (int k = 0; k < TOKENS; ++k) {
+        const F2 m1 = f2_both(-s[2 * k] * inv), m2 = f2_both(-s[2 * k + 1] * inv), scale = f2_both(rstd[k]);
+        const int n = n0 + k * side;
+        if (n < p.N && p.dx != nullptr) {
+          T* to = static_cast<T*>(p.dx) + n * p.dx_s[0];
 #pragma unroll
-          for (int i = 0; i < P; ++i) dx.set_pair(i, f2_mul(scale, f2_fma(xh[e][i], f2_both(-s2), f2_add(g[e][i], f2_both(-s1)))));
-          dx.store(static_cast<T*>(p.dx) + (n0 + k * side) * p.dx_s[0] + at[e]);
+          for (int e = 0; e < EACH; ++e) {
+            if (!seat.in(t, e)) continue;
+            Pack<T, V> dx;
+#pragma unroll
+            for (int i = 0; i < P; ++i) dx.set_pair(i, f2_mul(scale, f2_fma(xh[k][e][i], m2, f2_add(g[k][e][i], m1))));
+            dx.store(to + at[e]);
+          }
         }
       }
     }
@@ -258,15 +283,14 @@ TokenPlan plan_of(const NormParams& p, int V, int tokens, int per_sm) {
   return plan;
 }
 
-// Blocks an SM is given (they walk the tokens) and tokens a lane loads at once, as measured for one vector a lane: two tokens
-// and four blocks for 16-bit values (16384 x 4096 bf16 56 us; four tokens 70, one 69), four and eight for fp32 (4096 x 2048
-// 14.2 us; two tokens 15.9), four and four backward (96 us; two tokens 105, eight blocks 105).
+// Blocks an SM is given (they walk the tokens) and tokens a lane holds at once, as measured for one vector a lane.  Four tokens
+// and as many blocks as the registers leave room for: 16384 x 4096 bf16 46.5 us (two tokens 52.4, five blocks 62, three 49), the
+// gradient with two blocks 78.3 (two tokens 91, three blocks of them 85, one block 111).  fp32 takes fewer registers: eight blocks,
+// 4096 x 2048 11.5 us (four 12.1).  A second round of blocks that do not fit costs most: 78 us.
 template <typename T>
-constexpr int per_sm(bool backward) { return sizeof(T) == 4 && !backward ? 8 : 4; }
+constexpr int per_sm(bool backward) { return backward ? 2 : sizeof(T) == 4 ? 8 : 4; }
 template <typename T>
-constexpr int tokens_at_once(int each, bool backward) {
-  return each == 1 ? (sizeof(T) == 2 && !backward ? 2 : 4) : each == 2 && !backward ? 2 : 1;
-}
+constexpr int tokens_at_once(int each, bool backward) { return each == 1 ? 4 : each == 2 && !backward ? 2 : 1; }
 
 // One token at a time of each block's, or several side by side.
 template <typename T, int V, int EACH>

@@ -10,7 +10,7 @@
 // quarter), beside three packed multiplications; the bytes of 8192 x 4096 values of bf16 take 41 us, their 16 exponentials
 // each 118.  So a block keeps one half of its warps on nothing but the recurrence and has the other half do the rest:
 //
-//   warps 4-7 (fill)  load u, delta, z, B, C of the next 32 tokens, take softplus and the gate, leave (dt, dt, dt u, dt u)
+//   warps 4-7 (fill)  load u, delta, z, B, C of the next 32 tokens, take softplus and the gate, leave (dt, dt u)
 //                     and fp32 B, C in shared memory, two tiles deep; later add D u, gate and store what the scan left
 //   warps 0-3 (scan)  LANES neighbouring parts of a channel's states per channel, NPT states a thread in registers, packed
 //                     in pairs; a tile's sums over the states are exchanged between the lanes four tokens at a time
@@ -575,8 +575,8 @@ int lanes_of(int S) { return S <= 4 ? 1 : S <= 8 ? 2 : S <= 32 ? 4 : S <= 128 ? 
 
 // How many chunks a row is cut into: the fewest clocks by what was measured for 16 states. A token costs the m blocks that
 // share an SM 57 m + 16 clocks (73 for one alone, where latencies show), the first launch of a row in chunks 0.65 of that for
-// all but the last chunk, and there is some 4 us in a second launch. 8192 x 1024: 310 us whole, 158 in 4, 121 in 16 chunks;
-// 8192 x 4096: 317 us whole, 389 in 4, 360 in 16.
+// all but the last chunk, and there is some 4 us in a second launch. 8192 x 1024: 280 us whole, 145 in 4, 116 in 12 chunks;
+// 8192 x 4096: 284 us whole, 380 in 4, 361 in 12; 2048 x 256: 73 whole, 19 in 16.
 Cut cut_of(const ScanParams& p) {
   const int channels = kScan / lanes_of(p.S), per_group = p.C / p.G, sms = current_sm_count();
   const double blocks = double(p.N) * p.G * ((per_group + channels - 1) / channels);
