@@ -25,6 +25,8 @@ constexpr int kMaxChunks = 64;        // pieces of an image in two launches
 constexpr int kMaxGroups = 512;       // of a slab
 constexpr int kThreads = 256;
 constexpr int kMostShared = 224 * 1024, kSharedOfSm = 228 * 1024;
+constexpr int kRowVectors = 4;        // of a slab's row, where groups are narrower and pixels not few
+constexpr int kFewRows = 16;          // of a thread, more of which have a few large images cut finer
 
 struct Slab {
   NormParams p;
@@ -677,7 +679,7 @@ bool image_plan(int dtype, const NormParams& p, bool backward, ImagePlan* plan) 
   const long long S = (long long)p.H * p.W;
   if (S > 0x1fffffff) return false;
   const int unit = cpg / gcd(cpg, V) * V, units = p.C / unit;   // whole groups and whole vectors
-  const long long wide = S < 64 ? kThreads / S : 4;
+  const long long wide = S < 64 ? kThreads / S : kRowVectors;
   int k = int(wide * V / unit);
   if (k < 1) k = 1;
   if (k > units) k = units;
@@ -705,7 +707,7 @@ bool image_plan(int dtype, const NormParams& p, bool backward, ImagePlan* plan) 
       break;
     }
     // a few large images: the two launches cut them finer (one of 208 x 104 x 103 in slabs of 104 channels 46 us, not cut)
-    if (2ll * p.N * s.slabs * cluster <= sms && need > 16) break;
+    if (2ll * p.N * s.slabs * cluster <= sms && need > kFewRows) break;
     s.cluster = cluster;
     s.rows = int((S + cluster - 1) / cluster);
     s.held = int((s.rows + at_once - 1) / at_once);
@@ -798,9 +800,11 @@ long long norm_images_workspace(int dtype, const NormParams& p, bool backward) {
   (void)dtype;
   const long long S = (long long)p.H * p.W, pieces = S < kMaxChunks ? S : kMaxChunks;
   const long long slices = 4ll * current_sm_count() < p.N ? 4ll * current_sm_count() : p.N;
-  // Two launches: only where eight blocks do not hold 16 rows of vectors (backward 4, beside the sums of 2048 channels) for each of
-  // their threads, of which at least 129 have work.
-  const bool split = S * (p.C / p.G) > (backward ? 8 * 4 * 128 : 8 * 16 * 128);
+  // Two launches: only where eight blocks do not hold kFewRows rows of vectors (backward 4, beside the sums of 2048 channels) for each
+  // of their threads, of which at least 129 have work. A row has as many vectors as a group has channels, at most, or kRowVectors (of
+  // several narrow groups; the wider rows of images of a few pixels are held by one block).
+  const long long cols = p.C / p.G > kRowVectors ? p.C / p.G : kRowVectors;
+  const bool split = S * cols > (backward ? 8 * 4 * 128 : 8 * kFewRows * 128);
   const long long rows = split ? (p.N * pieces > slices ? p.N * pieces : slices) : slices;
   return 8 * rows * (backward ? p.C : split ? p.G : 0);
 }
