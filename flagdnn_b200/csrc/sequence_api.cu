@@ -6,6 +6,8 @@ using namespace fdnn;
 namespace {
 
 constexpr int32_t kMaxTokens = 0x7fffffff - 1024;   // tiles past a row's end are counted in 32 bits
+// Rows (images) past the last are counted in 32 bits: at most 1024 side by side in a block, or a stride of sixteen blocks an SM.
+constexpr int32_t kMaxRows = 0x7fffffff - 65536;
 
 bool float_type(int dtype) { return dtype == FDNN_F16 || dtype == FDNN_BF16 || dtype == FDNN_F32; }
 
@@ -15,6 +17,7 @@ int norm_params(const fdnn_norm_desc* d, NormParams* p) {
   if (d->param_dtype != d->dtype && d->param_dtype != FDNN_F32)
     return api_fail(FDNN_NOT_SUPPORTED, "weight and bias must be of the input's type or float32");
   if (d->n < 0 || d->c <= 0 || d->h < 0 || d->w < 0) return api_fail(FDNN_BAD_PARAM, "negative extent");
+  if (d->n > kMaxRows) return api_fail(FDNN_NOT_SUPPORTED, "more rows than the kernels count");
   if (d->groups <= 0 || d->c % d->groups != 0) return api_fail(FDNN_BAD_PARAM, "channels must be divisible by groups");
   if (d->activation < FDNN_ACT_NONE || d->activation > FDNN_ACT_SILU) return api_fail(FDNN_BAD_PARAM, "unknown activation");
   if (!(d->eps >= 0.0f)) return api_fail(FDNN_BAD_PARAM, "eps must not be negative");
@@ -204,6 +207,7 @@ int fdnn_selective_scan_step(const fdnn_scan_desc* desc, const void* u, const vo
   const int st = scan_params(desc, &p);
   if (st != FDNN_OK) return st;
   if (p.N == 0 || p.C == 0) return FDNN_OK;
+  if (p.N > kMaxRows) return api_fail(FDNN_NOT_SUPPORTED, "more rows than the kernels count");
   if (n_slots < 0 || (slots == nullptr && n_slots < p.N)) return api_fail(FDNN_BAD_PARAM, "fewer states than rows");
   if (u == nullptr || delta == nullptr || A == nullptr || B == nullptr || C == nullptr || y == nullptr || (state == nullptr && n_slots > 0))
     return api_fail(FDNN_BAD_PARAM, "u, delta, A, B, C, state and y must not be NULL");

@@ -269,7 +269,7 @@ int fdnn_adaptive_avg_pool2d_fwd(const fdnn_pool_desc* desc, const void* x,
  * c / groups * h * w values of an image's group, rstd = 1 / sqrt(variance + eps).  Channels-last x is read and
  * written once; rows of tokens are h = w = 1.  fp32 statistics (no difference of large sums), one rounding.
  * Channels-last tensors whose pixels lie at one stride (dense, or a slice of the channels) take the fast kernels, other
- * strides a slower one. */
+ * strides a slower one.  n is at most 2^31 - 65537 (more: FDNN_NOT_SUPPORTED). */
 typedef struct fdnn_norm_desc {
   int32_t dtype;               /* FDNN_F16, FDNN_BF16 or FDNN_F32: x, y, dy, dx */
   int32_t param_dtype;         /* weight, bias and their gradients: dtype or FDNN_F32 */
@@ -344,7 +344,8 @@ int fdnn_selective_scan_fwd(const fdnn_scan_desc* desc, const void* u, const voi
                             const float* initial_state, const int32_t* lengths, void* y, float* final_state,
                             void* workspace, int64_t workspace_bytes, void* stream);
 
-/* The same for one token of each row (l is not read), states [n_slots, C, s] in place as for fdnn_causal_conv1d_step. */
+/* The same for one token of each row (l is not read; n at most 2^31 - 65537), states [n_slots, C, s] in place as for
+ * fdnn_causal_conv1d_step. */
 int fdnn_selective_scan_step(const fdnn_scan_desc* desc, const void* u, const void* delta, const float* A, const void* B,
                              const void* C, const float* D, const void* z, const float* delta_bias, float* state,
                              int32_t n_slots, const int32_t* slots, void* y, void* stream);
