@@ -23,9 +23,18 @@ class MixerState:
     scan: torch.Tensor    # [slots, inner, states] float32
 
     def put(self, slots: torch.Tensor, other: "MixerState") -> None:
-        """Row n of ``other`` into slot ``slots[n]``, as after the prompts that begin there."""
-        self.conv[slots.long()] = other.conv
-        self.scan[slots.long()] = other.scan
+        """Row n of ``other`` into slot ``slots[n]``, as after the prompts that begin there; a slot outside the cache marks an
+        idle row, which is not written."""
+        if slots.numel() == 0 or self.conv.shape[0] == 0:
+            return
+        # an idle row writes once more what the first other one does (or what slot 0 has, where all are idle): the host need not
+        # know which rows those are
+        live = (slots >= 0) & (slots < self.conv.shape[0])
+        first, any_live = live.to(torch.uint8).argmax(), live.any()
+        rows = torch.where(live, torch.arange(slots.numel(), device=slots.device), first)
+        at = torch.where(any_live, slots[rows], 0).long()
+        self.conv[at] = torch.where(any_live, other.conv[rows], self.conv[at])
+        self.scan[at] = torch.where(any_live, other.scan[rows], self.scan[at])
 
 
 class StateSpaceMixer:
