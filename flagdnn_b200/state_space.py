@@ -78,9 +78,11 @@ class StateSpaceMixer:
     @torch.no_grad()
     def forward(self, x: torch.Tensor, state: Optional[MixerState] = None,
                 lengths: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, MixerState]:
-        """Prompts x [N, L, model], behind ``state`` if given (row n at slot n), ragged by ``lengths``: the outputs (of padding
-        tokens: those of a zero) and the state behind each row."""
+        """Prompts x [N, L, model], behind ``state`` if given (row n at slot n of N slots or more), ragged by ``lengths``: the
+        outputs (of padding tokens: those of a zero) and the state behind each row."""
         n, length, _ = x.shape
+        if state is not None:
+            state = MixerState(state.conv[:n], state.scan[:n])
         both = conv_host.mm(x.reshape(n * length, self.model), self.w_in).view(n, length, 2 * self.inner)
         v, conv_state = sequence_host.causal_conv1d(both[..., :self.inner], self.w_conv, self.b_conv, "silu",
                                                     None if state is None else state.conv, lengths, True)
