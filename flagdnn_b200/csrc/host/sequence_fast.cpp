@@ -274,6 +274,7 @@ PyObject* fast_group_norm_backward(PyObject*, PyObject* const* a, Py_ssize_t n) 
   if (dy == nullptr || mean == nullptr || rstd == nullptr || !norm_call(k, a[1], a[4], a[5], a[6], a[7])) return none();
   if (dy->sizes() != k.x->sizes() || dy->scalar_type() != k.x->scalar_type() || dy->device() != k.x->device()) return none();
   if (!dense(mean, at::kFloat, {k.d.n, k.d.groups}, *k.x) || !dense(rstd, at::kFloat, {k.d.n, k.d.groups}, *k.x)) return none();
+  if (any_grad({dy, k.x, mean, rstd, k.weight, k.bias})) return none();
   c10::DeviceGuard guard(k.x->device());
   at::Tensor dx, dw, db, scratch;
   int st;

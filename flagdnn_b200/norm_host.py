@@ -32,6 +32,11 @@ def answered(result):
     return result
 
 
+def refuse_grad(what: str, *tensors: Optional[torch.Tensor]) -> None:
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise NotImplementedError(f"flag_dnn {what} computes no gradients: call it under torch.no_grad()")
+
+
 def workspace(nbytes: int, device: torch.device) -> Optional[torch.Tensor]:
     return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
 
@@ -180,7 +185,8 @@ def group_norm(input: torch.Tensor, num_groups: int, weight: Optional[torch.Tens
 def group_norm_backward(dy: torch.Tensor, input: torch.Tensor, mean: torch.Tensor, rstd: torch.Tensor, num_groups: int,
                         weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None, activation: str = "none"):
     """The gradient of ``group_norm`` for ``dy``: ``(dx, dweight, dbias)``, None in the place of a parameter that is None.
-    ``mean`` and ``rstd`` are what the forward call returned.  The sums are made in a fixed order."""
+    ``mean`` and ``rstd`` are what the forward call returned.  The sums are made in a fixed order.  Not differentiable itself:
+    tensors that ask for a gradient are refused outside of ``torch.no_grad()``."""
     act = activation_id(activation)
     fast = _conv._fast or _conv.native_host()
     if fast:
@@ -193,4 +199,5 @@ def group_norm_backward(dy: torch.Tensor, input: torch.Tensor, mean: torch.Tenso
     for name, t in (("mean", mean), ("rstd", rstd)):
         if tuple(t.shape) != (input.shape[0], num_groups) or t.dtype != torch.float32 or t.device != input.device:
             raise RuntimeError(f"{name} must be a float32 tensor of shape ({input.shape[0]}, {num_groups}) on the input's device")
+    refuse_grad("group_norm_backward", dy, input, mean, rstd, weight, bias)
     return _backward(dy, input, mean.contiguous(), rstd.contiguous(), num_groups, weight, bias, act)

@@ -17,7 +17,7 @@ import torch
 
 from . import _native as nat
 from . import conv_host as _conv
-from .norm_host import _DTYPE_IDS, activation_id, address, answered, workspace
+from .norm_host import _DTYPE_IDS, activation_id, address, answered, refuse_grad, workspace
 
 MAX_WIDTH, MAX_STATES = 8, 256
 
@@ -42,11 +42,6 @@ def _check_like(what: str, name: str, t: Optional[torch.Tensor], shape: tuple, d
         raise RuntimeError(f"{what}: {name} must be {dtype}, got {t.dtype}")
     if t.device != device:
         raise RuntimeError(f"{what}: {name} must be on {device}, got {t.device}")
-
-
-def _refuse_grad(what: str, *tensors: Optional[torch.Tensor]) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise NotImplementedError(f"flag_dnn {what} computes no gradients: call it under torch.no_grad()")
 
 
 def _dense(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
@@ -89,7 +84,7 @@ def causal_conv1d(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Te
     n, length, c = x.shape
     _check_like(what, "initial_state", initial_state, (n, width - 1, c), x.dtype, x.device)
     _check_like(what, "lengths", lengths, (n,), torch.int32, x.device)
-    _refuse_grad(what, x, weight, bias, initial_state)
+    refuse_grad(what, x, weight, bias, initial_state)
     initial_state, lengths = _dense(initial_state), _dense(lengths)
     y = torch.empty((n, length, c), dtype=x.dtype, device=x.device)
     final = torch.empty((n, width - 1, c), dtype=x.dtype, device=x.device) if return_final_state else None
@@ -131,7 +126,7 @@ def causal_conv1d_step(x: torch.Tensor, conv_state: torch.Tensor, weight: torch.
     weight, bias, width = _check_conv(what, x, weight, bias)
     n, c = x.shape
     _check_cache(what, "conv_state", conv_state, (width - 1, c), x.dtype, x, slots)
-    _refuse_grad(what, x, weight, bias, conv_state)
+    refuse_grad(what, x, weight, bias, conv_state)
     slots = _dense(slots)
     y = torch.empty((n, c), dtype=x.dtype, device=x.device)
     d = nat.CausalConvDesc()
@@ -197,7 +192,7 @@ def selective_scan(u: torch.Tensor, delta: torch.Tensor, A: torch.Tensor, B: tor
     n, length, c = u.shape
     _check_like(what, "initial_state", initial_state, (n, c, d.s), torch.float32, u.device)
     _check_like(what, "lengths", lengths, (n,), torch.int32, u.device)
-    _refuse_grad(what, u, delta, A, B, C, D, z, delta_bias, initial_state)
+    refuse_grad(what, u, delta, A, B, C, D, z, delta_bias, initial_state)
     initial_state, lengths = _dense(initial_state), _dense(lengths)
     d.delta_softplus = int(bool(delta_softplus))
     y = torch.empty((n, length, c), dtype=u.dtype, device=u.device)
@@ -231,7 +226,7 @@ def selective_scan_step(u: torch.Tensor, delta: torch.Tensor, A: torch.Tensor, B
     d, A, B, C, D, delta_bias = _check_scan(what, u, delta, A, B, C, D, z, delta_bias)
     n, c = u.shape
     _check_cache(what, "state", state, (c, d.s), torch.float32, u, slots)
-    _refuse_grad(what, u, delta, A, B, C, D, z, delta_bias, state)
+    refuse_grad(what, u, delta, A, B, C, D, z, delta_bias, state)
     slots = _dense(slots)
     d.delta_softplus = int(bool(delta_softplus))
     y = torch.empty((n, c), dtype=u.dtype, device=u.device)
