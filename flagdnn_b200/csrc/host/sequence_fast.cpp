@@ -6,6 +6,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAStream.h>
@@ -57,10 +58,11 @@ bool dense(const at::Tensor* t, at::ScalarType type, at::IntArrayRef sizes, cons
 const void* ptr(const at::Tensor* t) { return t == nullptr ? nullptr : t->const_data_ptr(); }
 const float* f32(const at::Tensor* t) { return static_cast<const float*>(ptr(t)); }
 const int32_t* i32(const at::Tensor* t) { return static_cast<const int32_t*>(ptr(t)); }
+// Whether one of them asks for a gradient or has a tangent of forward-mode differentiation: Python differentiates or refuses.
 bool any_grad(std::initializer_list<const at::Tensor*> ts) {
-  if (!c10::GradMode::is_enabled()) return false;
+  const bool back = c10::GradMode::is_enabled(), forward = c10::AutogradState::get_tls_state().get_fw_grad_mode();
   for (const at::Tensor* t : ts)
-    if (t != nullptr && t->requires_grad()) return true;
+    if (t != nullptr && ((back && t->requires_grad()) || (forward && t->_fw_grad(0).defined()))) return true;
   return false;
 }
 bool small(const at::Tensor& t) {

@@ -10,6 +10,7 @@ import ctypes
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd.forward_ad import unpack_dual
 
 from . import _native as nat
 from . import conv_host as _conv
@@ -32,7 +33,14 @@ def answered(result):
     return result
 
 
+def refuse_tangents(what: str, *tensors: Optional[torch.Tensor]) -> None:
+    """Forward-mode differentiation: a result without a tangent would count as a constant."""
+    if not torch.is_inference_mode_enabled() and any(t is not None and unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"flag_dnn {what} computes no forward-mode derivatives")
+
+
 def refuse_grad(what: str, *tensors: Optional[torch.Tensor]) -> None:
+    refuse_tangents(what, *tensors)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         raise NotImplementedError(f"flag_dnn {what} computes no gradients: call it under torch.no_grad()")
 
@@ -167,7 +175,8 @@ def group_norm(input: torch.Tensor, num_groups: int, weight: Optional[torch.Tens
     [N, C], [N, C, L] or [N, C, H, W] (f16, bf16, f32); activations: none, relu, gelu, gelu_tanh, silu.
 
     Weight and bias are of the input's type or float32.  With ``return_stats`` the result is ``(y, mean, rstd)``, the float32
-    [N, num_groups] statistics that ``group_norm_backward`` takes.  Differentiable once."""
+    [N, num_groups] statistics that ``group_norm_backward`` takes.  Differentiable once, backwards; tensors with a tangent of
+    forward-mode differentiation are refused."""
     act = activation_id(activation)
     fast = _conv._fast or _conv.native_host()
     if fast:
@@ -175,6 +184,7 @@ def group_norm(input: torch.Tensor, num_groups: int, weight: Optional[torch.Tens
         if y is not None:
             return answered(y)
     _check(input, num_groups, weight, bias)
+    refuse_tangents("group_norm", input, weight, bias)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (input, weight, bias)):
         y, mean, rstd = _GroupNorm.apply(input, weight, bias, num_groups, float(eps), act)
     else:
