@@ -65,6 +65,11 @@ bool any_grad(std::initializer_list<const at::Tensor*> ts) {
     if (t != nullptr && ((back && t->requires_grad()) || (forward && t->_fw_grad(0).defined()))) return true;
   return false;
 }
+// A state that a kernel has written through its address: autograd's check of saved tensors goes by their versions.  (Tensors made in
+// inference mode have none.)
+void written(const at::Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
 bool small(const at::Tensor& t) {
   for (int64_t s : t.sizes())
     if (s > kMost) return false;
@@ -348,6 +353,7 @@ PyObject* fast_causal_conv1d_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
     st = g_conv_step(&d, x->const_data_ptr(), w->const_data_ptr(), ptr(bias), state->mutable_data_ptr(), int32_t(cache), i32(slots),
                      y.mutable_data_ptr(), stream_of(*x));
   }
+  if (st == FDNN_OK) written(*state);
   return answer(st, std::move(y));
   END_HANDLE_TH_ERRORS
 }
@@ -409,6 +415,7 @@ PyObject* fast_selective_scan_step(PyObject*, PyObject* const* a, Py_ssize_t n) 
     st = g_scan_step(&k.d, u.const_data_ptr(), k.delta->const_data_ptr(), f32(k.A), k.B->const_data_ptr(), k.C->const_data_ptr(), f32(k.D),
                      ptr(k.z), f32(k.bias), state->mutable_data_ptr<float>(), int32_t(cache), i32(slots), y.mutable_data_ptr(), stream_of(u));
   }
+  if (st == FDNN_OK) written(*state);
   return answer(st, std::move(y));
   END_HANDLE_TH_ERRORS
 }

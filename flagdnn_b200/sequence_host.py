@@ -14,6 +14,7 @@ import ctypes
 from typing import Optional
 
 import torch
+from torch.autograd.graph import increment_version
 
 from . import _native as nat
 from . import conv_host as _conv
@@ -137,6 +138,7 @@ def causal_conv1d_step(x: torch.Tensor, conv_state: torch.Tensor, weight: torch.
         nat.check(nat.load().fdnn_causal_conv1d_step(
             ctypes.byref(d), x.data_ptr(), weight.data_ptr(), address(bias), conv_state.data_ptr(), conv_state.shape[0],
             address(slots), y.data_ptr(), torch.cuda.current_stream().cuda_stream))
+    increment_version(conv_state)
     return y
 
 
@@ -236,4 +238,5 @@ def selective_scan_step(u: torch.Tensor, delta: torch.Tensor, A: torch.Tensor, B
             ctypes.byref(d), u.data_ptr(), delta.data_ptr(), A.data_ptr(), B.data_ptr(), C.data_ptr(), address(D), address(z),
             address(delta_bias), state.data_ptr(), state.shape[0], address(slots), y.data_ptr(),
             torch.cuda.current_stream().cuda_stream))
+    increment_version(state)
     return y
