@@ -282,8 +282,13 @@ _GROUP_NORM_ARG_NAMES = ["input", "num_groups", "weight", "bias", "eps", "activa
 
 
 def _normalize_group_norm(ctx: Any, args: tuple, kwargs: dict) -> tuple:
+    from ..norm_host import activation_id
+
     if len(args) > len(_GROUP_NORM_ARG_NAMES):
         raise TypeError("group_norm got too many positional args")
+    for name in kwargs:
+        if name not in _GROUP_NORM_ARG_NAMES:
+            raise TypeError(f"group_norm got an unexpected keyword argument {name!r}")
     params = {"weight": None, "bias": None, "eps": 1e-5, "activation": "none", "return_stats": False}
     params.update(kwargs)
     for name, arg in zip(_GROUP_NORM_ARG_NAMES, args):
@@ -294,6 +299,7 @@ def _normalize_group_norm(ctx: Any, args: tuple, kwargs: dict) -> tuple:
         raise NotImplementedError("graph group_norm returns values only (return_stats=False)")
     if "input" not in params or "num_groups" not in params:
         raise TypeError("group_norm expects an input and num_groups")
+    activation_id(params["activation"])
     ids = [ctx.as_value(params.pop("input"), "input")]
     params["operands"] = tuple(name for name in ("weight", "bias") if params[name] is not None)
     for name in ("weight", "bias"):
@@ -309,9 +315,13 @@ def _infer_group_norm(specs: list, attrs: dict) -> TensorSpec:
         raise RuntimeError("graph group_norm expects 2 to 4 dimensions")
     if groups <= 0 or x.shape[1] % groups != 0:
         raise RuntimeError("graph group_norm channels must be divisible by num_groups")
-    for spec in specs[1:]:
+    for name, spec in zip(attrs["operands"], specs[1:]):
         if tuple(spec.shape) != (x.shape[1],):
             raise RuntimeError("graph group_norm weight and bias must have one value per channel")
+        if spec.dtype not in (x.dtype, "float32"):
+            raise RuntimeError(f"graph group_norm {name} must be of the input's type or float32, got {spec.dtype}")
+    if len({spec.dtype for spec in specs[1:]}) > 1:
+        raise RuntimeError("graph group_norm weight and bias must have the same dtype")
     return _infer_same(specs, attrs)
 
 
