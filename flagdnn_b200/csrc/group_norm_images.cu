@@ -110,7 +110,8 @@ __device__ __forceinline__ void local_moments(const Slab& s, const Place& at, F&
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         mean[2 * i + j] = first[j] + a[j] * inv;
-        m2[2 * i + j] = fmaxf(q[j] - a[j] * a[j] * inv, q[j] * 0.0f);   // (rounding may leave less than nothing; NaN stays)
+        // (a^2 may be no number where a^2 / n is one; rounding may leave less than nothing; NaN stays)
+        m2[2 * i + j] = fmaxf(q[j] - a[j] * (a[j] * inv), q[j] * 0.0f);
       }
     }
     if constexpr (ONE) {

@@ -1,0 +1,29 @@
+"""group_norm at values whose squares come near the ends of fp32."""
+import pytest
+import torch
+
+from oracle import sequence_oracle as so
+from test_group_norm_gpu import fd, make  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+def near(got, want, rtol=2e-5, atol=2e-5):
+    got = got.double().cpu()
+    assert got.shape == want.shape
+    bad = ~((got - want).abs() <= rtol * want.abs() + atol)   # (a NaN is not near)
+    worst = ((got - want).abs() / want.abs().clamp_min(1e-300)).max()
+    assert not bad.any(), f"{int(bad.sum())} of {bad.numel()} off, {int(torch.isnan(got).sum())} NaN, worst {float(worst):.3g} of its size"
+
+
+def test_an_outlier_whose_squares_are_near_the_largest_number(fd):  # noqa: F811
+    """8e18 among small values: its square, 6.4e37, is a number, and so is the variance; the square of five values' distances
+    from it, added up, is not.  All of it is fp32 arithmetic on numbers, at the tolerances of other values."""
+    x = make((160, 8, 24, 24), torch.float32, "cl")
+    x[:, 0, 0, 0] = 8e18
+    x[:, 4, 5, 3] = -8e18
+    want, mean, rstd = so.group_norm(x, 2)
+    y, got_mean, got_rstd = fd.group_norm(x, 2, return_stats=True)
+    near(got_rstd, rstd, rtol=5e-5, atol=0.0)
+    near(got_mean, mean)
+    near(y, want)
