@@ -70,14 +70,18 @@ struct Rows {
   __device__ int of(int r) const { return each + (r < more ? 1 : 0); }
 };
 
-// Mean and squared deviations of a block's rows by group, from registers: out[g] in shared memory.
-// A thread sums its values' distances from its own first one, and their squares, channel by channel: one pass, and what
-// the squares lose to a first value far from the others is less than 2^-24 of that value's own share of the group's squared
-// deviations, times the thread's rows. Threads and channels are joined by their means.  ONE (everywhere): the channels of a
-// vector are all of one group.
-template <typename T, int V, bool ONE, typename F>
+// Mean and squared deviations of a block's rows by group: out[g] in shared memory.
+// A thread sums its values' distances from its own first one, and their squares, channel by channel, in one pass. Where that first
+// value lies D from n - 1 others, the sums grow to n D and n D^2 and are rounded on the way to 2^-24 of what they have come to: the
+// thread's squared deviations are off by up to 1.5 n^2 2^-24 D^2, and the group's are D^2 at least. n is a thread's rows, up to 50 of a
+// block that holds them.  LONG rows, of which a thread may have thousands, are summed in runs: the first kRun from the first value (off by
+// up to 9.2e-5 of the group's), then as many again as there were from the mean so far. Such a run of n that lies D from it brings the group
+// n / 2 times D^2, of which 3 n 2^-24 may be lost: as much at kMostRun.  Runs, threads and channels are joined by their means.
+// ONE (everywhere): the channels of a vector are all of one group.
+constexpr int kRun = 32, kMostRun = 512;
+template <typename T, int V, bool ONE, bool LONG, typename F>
 __device__ __forceinline__ void local_moments(const Slab& s, const Place& at, F&& row, const Rows& rows, float2* red, float2* out) {
-  const int cpg = s.p.C / s.p.G, count = at.live ? rows.of(at.r) : 0;
+  const int cpg = s.p.C / s.p.G, count = at.live ? rows.of(at.r) : 0, run = LONG ? min(count, kRun) : count;
   constexpr int P = Pack<T, V>::kPairs;
   F2 sum[P], square[P], minus[P];
   Pack<T, V> x0;
@@ -89,7 +93,7 @@ __device__ __forceinline__ void local_moments(const Slab& s, const Place& at, F&
     minus[i] = f2_mul(x0.pair(i), f2_both(-1.0f));
   }
 #pragma unroll 4
-  for (int k = 1; k < count; ++k) {
+  for (int k = 1; k < run; ++k) {
     const Pack<T, V> x = row(k);
 #pragma unroll
     for (int i = 0; i < P; ++i) {
@@ -99,7 +103,7 @@ __device__ __forceinline__ void local_moments(const Slab& s, const Place& at, F&
     }
   }
   if (at.r < s.rows_at_once) {
-    const float inv = count > 0 ? __fdividef(1.0f, float(count)) : 0.0f;
+    const float inv = count > 0 ? __fdividef(1.0f, float(run)) : 0.0f;
     float mean[2 * P], m2[2 * P];
 #pragma unroll
     for (int i = 0; i < P; ++i) {
@@ -112,6 +116,39 @@ __device__ __forceinline__ void local_moments(const Slab& s, const Place& at, F&
         mean[2 * i + j] = first[j] + a[j] * inv;
         // (a^2 may be no number where a^2 / n is one; rounding may leave less than nothing; NaN stays)
         m2[2 * i + j] = fmaxf(q[j] - a[j] * (a[j] * inv), q[j] * 0.0f);
+      }
+    }
+    if constexpr (LONG) {
+      for (int begin = kRun, end; begin < count; begin = end) {
+        end = min(count, begin + min(begin, kMostRun));
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+          sum[i] = square[i] = 0;
+          minus[i] = f2_pack(-mean[2 * i], -mean[2 * i + 1]);
+        }
+#pragma unroll 8
+        for (int k = begin; k < end; ++k) {
+          const Pack<T, V> x = row(k);
+#pragma unroll
+          for (int i = 0; i < P; ++i) {
+            const F2 d = f2_add(x.pair(i), minus[i]);
+            sum[i] = f2_add(sum[i], d);
+            square[i] = f2_fma(d, d, square[i]);
+          }
+        }
+        const float each = __fdividef(1.0f, float(end - begin)), share = __fdividef(float(end - begin), float(end));
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+          float a[2], q[2];
+          f2_split(sum[i], a[0], a[1]);
+          f2_split(square[i], q[0], q[1]);
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const float d = a[j] * each;
+            m2[2 * i + j] += fmaxf(q[j] - a[j] * d, q[j] * 0.0f) + d * (d * (float(begin) * share));
+            mean[2 * i + j] += d * share;
+          }
+        }
       }
     }
     if constexpr (ONE) {
@@ -196,7 +233,7 @@ norm_images_kernel(const Slab s) {
   for (int n = slice; n < p.N; n += s.slices) {
     async_commit();
     async_wait<0>();
-    local_moments<T, V, ONE>(s, at, [&](int k) { return held[k * kThreads]; }, rows, red, own);
+    local_moments<T, V, ONE, false>(s, at, [&](int k) { return held[k * kThreads]; }, rows, red, own);
     if (s.cluster > 1) {
       cluster_arrive();
       cluster_wait();
@@ -470,7 +507,7 @@ norm_split_stats_kernel(const Slab s) {
   const Place at = Place::of<V>(s, slab);
   const long long pixel = p.W > 1 ? p.x_s[3] : p.x_s[2];
   const T* x0 = static_cast<const T*>(p.x) + n * p.x_s[0] + at.c0 + at.cc + (long long)(row0 + at.r) * pixel;
-  local_moments<T, V, ONE>(s, at, [&](int k) {
+  local_moments<T, V, ONE, true>(s, at, [&](int k) {
     Pack<T, V> x;
     x.load(x0 + (long long)k * s.rows_at_once * pixel);
     return x;

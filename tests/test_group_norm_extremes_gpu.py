@@ -1,4 +1,4 @@
-"""group_norm at values whose squares come near the ends of fp32."""
+"""group_norm at values whose squares come near the ends of fp32, and over long runs of pixels behind an outlier."""
 import pytest
 import torch
 
@@ -27,3 +27,17 @@ def test_an_outlier_whose_squares_are_near_the_largest_number(fd):  # noqa: F811
     near(got_rstd, rstd, rtol=5e-5, atol=0.0)
     near(got_mean, mean)
     near(y, want)
+
+
+def test_a_long_run_behind_an_outlier(fd):  # noqa: F811
+    """A thread of the two-launch form sums distances from a first value D away from the others.  Over 32 values each of the
+    two sums is rounded 31 times, to 16 D (16 D^2) on average: 1000 and 500 times 2^-24 of D^2, which is a part of the group's
+    squared deviations; 9e-5 of the variance and half of it of its root, at most.  (A run of a thousand values: a thousand times that.)"""
+    x = torch.randn(1, 4096, 4096, 4, device="cuda", generator=torch.Generator("cuda").manual_seed(0)).permute(0, 3, 1, 2)
+    x[:, 0, 0, 0] = 1e5
+    all_of = x.double()
+    mean = all_of.mean()
+    rstd = ((all_of - mean).square().mean() + 1e-5).rsqrt()
+    _, got_mean, got_rstd = fd.group_norm(x, 1, return_stats=True)
+    near(got_mean[0, 0], mean.cpu())
+    near(got_rstd[0, 0], rstd.cpu(), rtol=4.5e-5, atol=0.0)
