@@ -350,7 +350,7 @@ scan_kernel(const ScanJob job) {
 #pragma unroll
     for (int s = 0; s < NPT; ++s) {
       const bool in = live && s0 + s < p.S;
-      av[s] = in ? p.A[(long long)c * p.S + s0 + s] * kLog2e : 0.0f;
+      av[s] = in ? rate_of(p.A[(long long)c * p.S + s0 + s]) : 0.0f;
       hv[s] = !ENDS && in && p.initial != nullptr ? p.initial[row * p.S + s0 + s] : 0.0f;
     }
     if constexpr (!ENDS) {

@@ -33,7 +33,7 @@ scan_step_kernel(const ScanParams p, float* state, int n_slots, const int* slots
   for (int k = 0; k < CHUNKS; ++k) {
     const int s = (k * LANES + part) * 4;
     a[k] = s < p.S ? four_states<WHOLE>(p.A + (long long)cc * p.S + s, p.S - s) : make_float4(0, 0, 0, 0);
-    a[k].x *= kLog2e; a[k].y *= kLog2e; a[k].z *= kLog2e; a[k].w *= kLog2e;
+    a[k] = make_float4(rate_of(a[k].x), rate_of(a[k].y), rate_of(a[k].z), rate_of(a[k].w));
   }
   const float D = p.D != nullptr ? p.D[cc] : 0.0f, bias = p.delta_bias != nullptr ? p.delta_bias[cc] : 0.0f;
   const T* u0 = static_cast<const T*>(p.u) + cc * p.u_s[2];

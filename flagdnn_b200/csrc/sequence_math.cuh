@@ -19,11 +19,18 @@ __device__ __forceinline__ float ex2(float v) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
   return r;
 }
-// A step's decay e^(dt A), for A log2 e.  The unit cuts its argument and its result downwards: between -0.1 and 0 the mean error
+// A step's decay e^(dt A), for a = A log2 e.  The unit cuts its argument and its result downwards: between -0.1 and 0 the mean error
 // is -1.2e-8 to -2.3e-8 of the decay, which a state that forgets slowly adds up over hundreds of steps (-1.8e-6 of it after 300).
 // An argument larger by kDecayMiddle has a mean error within 1e-8 of zero there; 2^kDecayMiddle is 1, so a step of no time leaves a
 // state as it is.
 constexpr float kDecayMiddle = 2.5e-8f;
+// (A as decay_of takes it. Minus infinity becomes the lowest number: e^(dt A) is zero all the same, but for a step of no time, which past
+// a row's end stands for no step and would make the state NaN.)
+__device__ __forceinline__ float rate_of(float A) {
+  float a;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(a) : "f"(A * kLog2e), "f"(-3.402823466e38f));   // (NaN stays)
+  return a;
+}
 __device__ __forceinline__ float decay_of(float dt, float a) { return ex2(fmaf(dt, a, kDecayMiddle)); }
 // 1 / v by the special function unit (one unit in the last place)
 __device__ __forceinline__ float rcp(float v) {
