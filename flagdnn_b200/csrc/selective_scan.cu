@@ -359,7 +359,8 @@ scan_kernel(const ScanJob job) {
         const float sum = job.sums[at];
 #pragma unroll
         for (int s = 0; s < NPT; ++s)
-          if (s0 + s < p.S) hv[s] = hv[s] * decay_of(sum, av[s]) + job.ends[at * p.S + s0 + s];
+          if (s0 + s < p.S)   // (a state of nothing stays nothing, even if e^(A sum dt) is no number)
+            hv[s] = hv[s] * decay_of(hv[s] == 0.0f ? 0.0f : sum, av[s]) + job.ends[at * p.S + s0 + s];
       }
     }
 #pragma unroll

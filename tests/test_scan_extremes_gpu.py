@@ -1,4 +1,4 @@
-"""selective_scan where a step of no time meets an infinity."""
+"""selective_scan where a step of no time, or a state of zeros, meets an infinity."""
 import pytest
 import torch
 
@@ -33,3 +33,15 @@ def test_states_that_forget_at_once(fd, l, c, lengths, s):  # noqa: F811
     tol = max(2e-4, l * 2.0 ** -21)
     near(got, final, tol)
     near(y, want, tol * s ** 0.5)
+
+
+def test_states_of_zeros_before_growing_ones(fd):  # noqa: F811
+    """A rate above zero over a piece of a long row: e^(A sum dt) is no number, and zero states stay zero all the same."""
+    l, c, s = 4000, 40, 16
+    u, delta = torch.zeros(1, l, c, device="cuda"), torch.ones(1, l, c, device="cuda")
+    a, bc = torch.ones(c, s, device="cuda"), torch.ones(1, l, s, device="cuda")
+    u[:, -2:] = 1.0
+    y, final = fd.selective_scan(u, delta, a, bc, bc, return_final_state=True)
+    want, end = so.selective_scan(u, delta, a, bc[:, :, None], bc[:, :, None])
+    near(final, end, 2e-5)
+    near(y, want, 2e-5 * s ** 0.5)
