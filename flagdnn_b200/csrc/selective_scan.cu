@@ -293,8 +293,10 @@ scan_kernel(const ScanJob job) {
         const float4 lo = from[0], hi = from[1];
         float v[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
         const Eight<T> ku = fetched<T>(ring.u[i % kLongSlots], tid);
+        if (p.D != nullptr) {   // (zero times an infinite u is not nothing)
 #pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] += D[k] * ku.at(k);
+          for (int k = 0; k < 8; ++k) v[k] += D[k] * ku.at(k);
+        }
         if (p.z != nullptr) {
           const Eight<T> kz = fetched<T>(ring.z[i % kLongSlots], tid);
 #pragma unroll

@@ -120,7 +120,7 @@ scan_step_kernel(const ScanParams p, float* state, int n_slots, const int* slots
 #pragma unroll
       for (int o = LANES / 2; o > 0; o >>= 1) y += __shfl_xor_sync(0xffffffffu, y, o);
       if (live && part == 0 && n < p.N) {
-        y += D * uv;
+        if (p.D != nullptr) y += D * uv;   // (zero times an infinite u is not nothing)
         if (p.z != nullptr) y *= silu(to_f32<T>(z[r]));
         static_cast<T*>(p.y)[n * p.y_s[0] + c * p.y_s[2]] = from_f32<T>(at[r] != nullptr ? y : 0.0f);
       }

@@ -1,11 +1,12 @@
-"""selective_scan where a step of no time, or a state of zeros, meets an infinity."""
+"""selective_scan where a step of no time, a state of zeros or a missing skip meets an infinity."""
 import pytest
 import torch
 
 from oracle import sequence_oracle as so
-from test_sequence_gpu import fd, scan_inputs  # noqa: F401
+from test_sequence_gpu import DTYPES, IDS, fd, scan_inputs  # noqa: F401
 
 pytestmark = pytest.mark.gpu
+SEQUENCES = ("u", "delta", "z", "B", "C")
 
 
 def near(got, want, tol):
@@ -45,3 +46,23 @@ def test_states_of_zeros_before_growing_ones(fd):  # noqa: F811
     want, end = so.selective_scan(u, delta, a, bc[:, :, None], bc[:, :, None])
     near(final, end, 2e-5)
     near(y, want, 2e-5 * s ** 0.5)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("s", [4, 16, 64])
+def test_an_infinite_input_without_a_skip(fd, s, dtype):  # noqa: F811
+    """Without D nothing but the states meets u: an infinite one makes them, and the outputs from there on, infinite."""
+    g = torch.Generator().manual_seed(s)
+    v = scan_inputs(g, 2, 40, 24, s, 1, dtype)
+    v["B"], v["C"], v["D"] = v["B"].abs() + 0.5, v["C"].abs() + 0.5, None
+    v["A"] = v["A"] * 0.01
+    v["u"][1, 7, 3] = float("inf")
+    v["z"] = v["z"].abs() + 0.5
+    y = fd.selective_scan(**v, delta_softplus=True)
+    bad = torch.zeros(2, 40, 24, dtype=torch.bool)
+    bad[1, 7:, 3] = True
+    assert torch.equal(torch.isinf(y).cpu(), bad) and not torch.isnan(y).any()
+    state = torch.zeros(2, 24, s, device="cuda")
+    token = {k: (t[:, 7] if k in SEQUENCES else t) for k, t in v.items()}
+    step = fd.selective_scan_step(**token, state=state, delta_softplus=True)
+    assert torch.equal(torch.isinf(step).cpu(), bad[:, 7]) and not torch.isnan(step).any()
