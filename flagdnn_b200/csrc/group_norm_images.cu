@@ -74,8 +74,9 @@ struct Rows {
 // A thread sums its values' distances from its own first one, and their squares, channel by channel, in one pass. Where that first
 // value lies D from n - 1 others, the sums grow to n D and n D^2 and are rounded on the way to 2^-24 of what they have come to: the
 // thread's squared deviations are off by up to 1.5 n^2 2^-24 D^2, and the group's are D^2 at least. n is a thread's rows, up to 50 of a
-// block that holds them.  LONG rows, of which a thread may have thousands, are summed in runs: the first kRun from the first value (off by
-// up to 9.2e-5 of the group's), then as many again as there were from the mean so far. Such a run of n that lies D from it brings the group
+// block that holds them as vectors of 16 bytes.  LONG rows, of which a thread may have hundreds (narrow vectors) or thousands (two
+// launches), are summed in runs: the first kRun from the first value (off by up to 9.2e-5 of the group's), then as many again as there
+// were from the mean so far. Such a run of n that lies D from it brings the group
 // n / 2 times D^2, of which 3 n 2^-24 may be lost: as much at kMostRun.  Runs, threads and channels are joined by their means.
 // ONE (everywhere): the channels of a vector are all of one group.
 constexpr int kRun = 32, kMostRun = 512;
@@ -233,7 +234,7 @@ norm_images_kernel(const Slab s) {
   for (int n = slice; n < p.N; n += s.slices) {
     async_commit();
     async_wait<0>();
-    local_moments<T, V, ONE, false>(s, at, [&](int k) { return held[k * kThreads]; }, rows, red, own);
+    local_moments<T, V, ONE, V <= 2>(s, at, [&](int k) { return held[k * kThreads]; }, rows, red, own);
     if (s.cluster > 1) {
       cluster_arrive();
       cluster_wait();

@@ -41,3 +41,17 @@ def test_a_long_run_behind_an_outlier(fd):  # noqa: F811
     _, got_mean, got_rstd = fd.group_norm(x, 1, return_stats=True)
     near(got_mean[0, 0], mean.cpu())
     near(got_rstd[0, 0], rstd.cpu(), rtol=4.5e-5, atol=0.0)
+
+
+@pytest.mark.parametrize("shape,dtype", [((10, 1, 900, 900), torch.bfloat16), ((10, 3, 590, 600), torch.float32)], ids=["bf16", "f32"])
+def test_a_long_run_that_one_launch_holds(fd, shape, dtype):  # noqa: F811
+    """The same for vectors of one value, of which a block holds hundreds for each of its threads."""
+    n, c, h, w = shape
+    x = torch.randn(n, h, w, c, device="cuda", generator=torch.Generator("cuda").manual_seed(0)).to(dtype).permute(0, 3, 1, 2)
+    x[:, :, 0, 0] = 1e5
+    rows = x.double().flatten(2)
+    mean = rows.mean(2)
+    rstd = ((rows - mean[..., None]).square().mean(2) + 1e-5).rsqrt()
+    _, got_mean, got_rstd = fd.group_norm(x, c, return_stats=True)
+    near(got_mean, mean.cpu())
+    near(got_rstd, rstd.cpu(), rtol=4.5e-5, atol=0.0)
