@@ -26,7 +26,8 @@ constexpr int kMaxGroups = 512;       // of a slab
 constexpr int kThreads = 256;
 constexpr int kMostShared = 224 * 1024, kSharedOfSm = 228 * 1024;
 constexpr int kRowVectors = 4;        // of a slab's row, where groups are narrower and pixels not few
-constexpr int kFewRows = 16;          // of a thread, more of which have a few large images cut finer
+constexpr int kStatic = 24 * 1024;    // shared memory that the forward kernel has beside its rows, at most
+constexpr int kMostRows = (kMostShared - kStatic) / (kThreads * 16);   // rows of 16-byte vectors that a thread may then hold: 50
 
 struct Slab {
   NormParams p;
@@ -732,7 +733,7 @@ bool image_plan(int dtype, const NormParams& p, bool backward, ImagePlan* plan) 
     const int row = kThreads * V * es * (backward ? 2 : 1);       // bytes of a row of a block's threads
     // (forward: beside 10 to 24 KB of static shared memory)
     const int few = ((backward ? 112 : 74) * 1024 - (backward ? fixed : (cpg % V == 0 ? 11 : 25) * 1024)) / row;
-    const int most = (kMostShared - (backward ? fixed : 24 * 1024)) / row;
+    const int most = (kMostShared - (backward ? fixed : kStatic)) / row;
     const long long at_once = s.rows_at_once;
     int cluster = 1;
     while (cluster < 8 && cluster * at_once * few < S) cluster *= 2;
@@ -745,8 +746,10 @@ bool image_plan(int dtype, const NormParams& p, bool backward, ImagePlan* plan) 
       if (k > 1 && !backward) continue;
       break;
     }
-    // a few large images: the two launches cut them finer (one of 208 x 104 x 103 in slabs of 104 channels 46 us, not cut)
-    if (2ll * p.N * s.slabs * cluster <= sms && need > kFewRows) break;
+    // The gradient of a few large images goes in two launches, which cut them finer: 1 x 4 x 163 x 170 bf16 in 4 groups 14.3 us, held by
+    // clusters 20.2 (but 3 x 4 x 147 x 150 in one group 13.9 and 12.2; most are not held as it is). Forward the one launch is ahead on
+    // 35 of 37 such shapes: 1 x 128 x 177 x 170 bf16 in 16 groups 13.5 us, cut 28.6; 1 x 16 x 194 x 189 in one 13.8 and 12.8.
+    if (backward && 2ll * p.N * s.slabs * cluster <= sms && need > 16) break;
     s.cluster = cluster;
     s.rows = int((S + cluster - 1) / cluster);
     s.held = int((s.rows + at_once - 1) / at_once);
@@ -787,7 +790,7 @@ cudaError_t forward(ImagePlan& plan, cudaStream_t stream) {
   }
   static std::atomic<uint64_t> done;
   auto* kernel = norm_images_kernel<T, V, ONE>;
-  const cudaError_t e = allow_smem(kernel, kMostShared - 24 * 1024, done);   // (beside the static part)
+  const cudaError_t e = allow_smem(kernel, kMostShared - kStatic, done);   // (beside the static part)
   if (e != cudaSuccess) return e;
   return launch_seq(kernel, dim3(unsigned((long long)s.slices * s.slabs * s.cluster)), kThreads, plan.smem, s.cluster, stream, s);
 }
@@ -839,11 +842,11 @@ long long norm_images_workspace(int dtype, const NormParams& p, bool backward) {
   (void)dtype;
   const long long S = (long long)p.H * p.W, pieces = S < kMaxChunks ? S : kMaxChunks;
   const long long slices = 4ll * current_sm_count() < p.N ? 4ll * current_sm_count() : p.N;
-  // Two launches: only where eight blocks do not hold kFewRows rows of vectors (backward 4, beside the sums of 2048 channels) for each
+  // Two launches: only where eight blocks do not hold kMostRows rows of vectors (backward 4, beside the sums of 2048 channels) for each
   // of their threads, of which at least 129 have work. A row has as many vectors as a group has channels, at most, or kRowVectors (of
   // several narrow groups; the wider rows of images of a few pixels are held by one block).
   const long long cols = p.C / p.G > kRowVectors ? p.C / p.G : kRowVectors;
-  const bool split = S * cols > (backward ? 8 * 4 * 128 : 8 * kFewRows * 128);
+  const bool split = S * cols > 8 * 128 * (backward ? 4 : kMostRows);
   const long long rows = split ? (p.N * pieces > slices ? p.N * pieces : slices) : slices;
   return 8 * rows * (backward ? p.C : split ? p.G : 0);
 }
