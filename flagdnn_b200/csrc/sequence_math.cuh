@@ -42,7 +42,7 @@ __device__ __forceinline__ float rcp(float v) {
 __device__ __forceinline__ float logistic(float v) { return rcp(1.0f + ex2(-kLog2e * v)); }
 __device__ __forceinline__ float silu(float v) { return v * logistic(v); }
 // log(1 + e^v) = max(v, 0) + log(1 + e), e = e^-|v| at most 1.  log(1 + e) / e is a polynomial of degree 9, fitted to the
-// smallest relative error on [0, 1] (5e-9; 1.3e-7 in fp32 arithmetic): no result is lost where e is small, and no second call of
+// smallest relative error on [0, 1] (4.8e-8 with these fp32 coefficients; 1.3e-7 in fp32 arithmetic): no result is lost where e is small, and no second call of
 // the special function unit, which bounds the scan.
 __device__ __forceinline__ float softplus(float v) {
   const float e = ex2(-kLog2e * fabsf(v));

@@ -6,7 +6,8 @@ slice of the columns of a wider projection needs no copy).  ``lengths`` (int32 [
 ``lengths[n]`` on are padding, are never read and give zeros.  States are the caller's: the convolution's is the last
 ``width - 1`` inputs, ``[N, width - 1, C]`` in the inputs' type, the scan's ``[N, C, S]`` float32.  The step functions update a
 cache of states in place, at ``slots`` (int32 [N]; a slot outside the cache marks an idle row, whose output is zero; two rows
-must not share one).  These are operators of the forward pass.
+must not share one); it counts as written for autograd's check of saved tensors.  These are operators of the forward pass:
+tensors that ask for a gradient, or carry a tangent, are refused.
 """
 from __future__ import annotations
 

@@ -267,7 +267,8 @@ int fdnn_adaptive_avg_pool2d_fwd(const fdnn_pool_desc* desc, const void* x,
 
 /* Group norm with an activation: y = act((x - mean) * rstd * weight + bias), mean and rstd over the
  * c / groups * h * w values of an image's group, rstd = 1 / sqrt(variance + eps).  Channels-last x is read and
- * written once; rows of tokens are h = w = 1.  fp32 statistics (no difference of large sums), one rounding.
+ * written once; rows of tokens are h = w = 1.  fp32 statistics, taken as distances from values of the
+ * group (never from sums of raw squares); one rounding.
  * Channels-last tensors whose pixels lie at one stride (dense, or a slice of the channels) take the fast kernels, other
  * strides a slower one.  n is at most 2^31 - 65537 (more: FDNN_NOT_SUPPORTED). */
 typedef struct fdnn_norm_desc {
