@@ -23,18 +23,25 @@ class MixerState:
     scan: torch.Tensor    # [slots, inner, states] float32
 
     def put(self, slots: torch.Tensor, other: "MixerState") -> None:
-        """Row n of ``other`` into slot ``slots[n]``, as after the prompts that begin there; a slot outside the cache marks an
-        idle row, which is not written."""
-        if slots.numel() == 0 or self.conv.shape[0] == 0:
+        """Row n of ``other`` (or its only one) into slot ``slots[n]``, as after the prompts that begin there; a slot outside the
+        cache marks an idle row, which is not written."""
+        n = slots.numel()
+        if slots.dim() != 1 or any(t.shape[0] not in (n, 1) for t in (other.conv, other.scan)):
+            raise RuntimeError(f"put: {tuple(slots.shape)} slots for {other.conv.shape[0]} and {other.scan.shape[0]} rows")
+        if self.conv.shape[0] != self.scan.shape[0]:
+            raise RuntimeError(f"put: a cache of {self.conv.shape[0]} and {self.scan.shape[0]} slots")
+        if n == 0 or self.conv.shape[0] == 0:
             return
+        slots = slots.to(self.conv.device)
+        conv, scan = (t.expand(n, *t.shape[1:]) for t in (other.conv, other.scan))
         # an idle row writes once more what the first other one does (or what slot 0 has, where all are idle): the host need not
         # know which rows those are
         live = (slots >= 0) & (slots < self.conv.shape[0])
         first, any_live = live.to(torch.uint8).argmax(), live.any()
-        rows = torch.where(live, torch.arange(slots.numel(), device=slots.device), first)
+        rows = torch.where(live, torch.arange(n, device=slots.device), first)
         at = torch.where(any_live, slots[rows], 0).long()
-        self.conv[at] = torch.where(any_live, other.conv[rows], self.conv[at])
-        self.scan[at] = torch.where(any_live, other.scan[rows], self.scan[at])
+        self.conv[at] = torch.where(any_live, conv[rows], self.conv[at])
+        self.scan[at] = torch.where(any_live, scan[rows], self.scan[at])
 
 
 class StateSpaceMixer:

@@ -29,3 +29,18 @@ def test_nothing_to_put():
     empty, rows = states(0, 0), states(2, 1)
     empty.put(torch.tensor([0, -1], dtype=torch.int32), rows)
     assert empty.conv.shape[0] == 0
+
+
+def test_rows_that_do_not_go_with_the_slots():
+    cache = states(5, 0)
+    conv = cache.conv.clone()
+    for slots in (torch.tensor([0, 1, 2, 3]), torch.tensor([0, 1]), torch.tensor([[0, 1, 2]])):
+        with pytest.raises(RuntimeError, match="put"):
+            cache.put(slots.int(), states(3, 1))
+    assert torch.equal(cache.conv, conv)
+    with pytest.raises(RuntimeError, match="put"):
+        MixerState(cache.conv, cache.scan[:4]).put(torch.tensor([0, 1, 4]), states(3, 1))
+    one = states(1, 2)                        # one row for several slots
+    cache.put(torch.tensor([4, -1, 2], dtype=torch.int32), one)
+    conv[[4, 2]] = one.conv
+    assert torch.equal(cache.conv, conv)
