@@ -61,6 +61,9 @@ EXPORTED_SYMBOLS = (
     "fdnn_selective_scan_workspace_bytes",
     "fdnn_selective_scan_fwd",
     "fdnn_selective_scan_step",
+    "fdnn_gated_delta_rule_workspace_bytes",
+    "fdnn_gated_delta_rule_fwd",
+    "fdnn_gated_delta_rule_step",
 )
 
 
@@ -138,6 +141,14 @@ class ScanDesc(ctypes.Structure):
                [("b_strides", ctypes.c_int64 * 4), ("c_strides", ctypes.c_int64 * 4)]
 
 
+class DeltaRuleDesc(ctypes.Structure):
+    _fields_ = [(name, ctypes.c_int32) for name in ("dtype", "gate_dtype", "n", "l", "key_heads", "heads", "dk", "dv", "delta_softplus",
+                                                    "beta_sigmoid", "qk_norm")] + \
+               [("scale", ctypes.c_float)] + \
+               [(name, ctypes.c_int64 * 4) for name in ("q_strides", "k_strides", "v_strides", "y_strides")] + \
+               [("delta_strides", ctypes.c_int64 * 3), ("beta_strides", ctypes.c_int64 * 3)]
+
+
 class NativeError(RuntimeError):
     """A non-OK status that maps to RuntimeError in the reference's convention."""
 
@@ -193,7 +204,7 @@ def load() -> ctypes.CDLL:
     lib.fdnn_debug_set_wait_limit.argtypes = [i64, i32]
     lib.fdnn_debug_tensor_map_counters.restype = i32
     lib.fdnn_debug_tensor_map_counters.argtypes = [ctypes.POINTER(ctypes.c_int64), ctypes.POINTER(ctypes.c_int64)]
-    pi64, pnorm, pconv, pscan = (ctypes.POINTER(t) for t in (i64, NormDesc, CausalConvDesc, ScanDesc))
+    pi64, pnorm, pconv, pscan, pdelta = (ctypes.POINTER(t) for t in (i64, NormDesc, CausalConvDesc, ScanDesc, DeltaRuleDesc))
     for name, args in (
         ("fdnn_group_norm_workspace_bytes", [pnorm, i32, pi64]),
         ("fdnn_group_norm_fwd", [pnorm] + [vp] * 7 + [i64, vp]),
@@ -203,6 +214,9 @@ def load() -> ctypes.CDLL:
         ("fdnn_selective_scan_workspace_bytes", [pscan, pi64]),
         ("fdnn_selective_scan_fwd", [pscan] + [vp] * 13 + [i64, vp]),
         ("fdnn_selective_scan_step", [pscan] + [vp] * 9 + [i32] + [vp] * 3),
+        ("fdnn_gated_delta_rule_workspace_bytes", [pdelta, pi64]),
+        ("fdnn_gated_delta_rule_fwd", [pdelta] + [vp] * 12 + [i64, vp]),
+        ("fdnn_gated_delta_rule_step", [pdelta] + [vp] * 8 + [i32] + [vp] * 3),
     ):
         fn = getattr(lib, name)
         fn.restype, fn.argtypes = i32, args

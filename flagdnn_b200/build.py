@@ -16,7 +16,7 @@ PKG_DIR = Path(__file__).resolve().parent
 CSRC = PKG_DIR / "csrc"
 LIB_PATH = PKG_DIR / "libflagdnn_b200.so"
 HOST_DIR = CSRC / "host"
-HOST_SOURCES = (HOST_DIR / "fastcall.cpp", HOST_DIR / "sequence_fast.cpp")
+HOST_SOURCES = (HOST_DIR / "fastcall.cpp", HOST_DIR / "sequence_fast.cpp", HOST_DIR / "delta_fast.cpp")
 HOST_PATH = PKG_DIR / "_fastcall.so"
 
 NVCC_FLAGS = [

@@ -281,6 +281,9 @@ def _load_fast() -> Any:
                 lib.fdnn_group_norm_workspace_bytes, lib.fdnn_group_norm_fwd, lib.fdnn_group_norm_bwd, lib.fdnn_causal_conv1d_fwd,
                 lib.fdnn_causal_conv1d_step, lib.fdnn_selective_scan_workspace_bytes, lib.fdnn_selective_scan_fwd,
                 lib.fdnn_selective_scan_step)), *(ctypes.sizeof(t) for t in (nat.NormDesc, nat.CausalConvDesc, nat.ScanDesc)))
+            _fastcall.bind_delta_rule(*(ctypes.cast(f, ctypes.c_void_p).value for f in (
+                lib.fdnn_gated_delta_rule_workspace_bytes, lib.fdnn_gated_delta_rule_fwd, lib.fdnn_gated_delta_rule_step)),
+                ctypes.sizeof(nat.DeltaRuleDesc))
             _fast = _fastcall
         except (ImportError, AttributeError, TypeError) as exc:   # not built, or built against something else
             warnings.warn(f"flagdnn_b200: the native host path is not used, calls take some 15 us longer ({exc}); "

@@ -381,7 +381,10 @@ PyMethodDef kMethods[] = {
     {"causal_conv1d_step", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(fast_causal_conv1d_step)), METH_FASTCALL, nullptr},
     {"selective_scan", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(fast_selective_scan)), METH_FASTCALL, nullptr},
     {"selective_scan_step", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(fast_selective_scan_step)), METH_FASTCALL, nullptr},
+    {"gated_delta_rule", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(fast_gated_delta_rule)), METH_FASTCALL, nullptr},
+    {"gated_delta_rule_step", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(fast_gated_delta_rule_step)), METH_FASTCALL, nullptr},
     {"bind", bind, METH_VARARGS, nullptr},
+    {"bind_delta_rule", bind_delta_rule, METH_VARARGS, nullptr},
     {"bind_sequence", bind_sequence, METH_VARARGS, nullptr},
     {"bind_unpacked", bind_unpacked, METH_O, nullptr},
     {nullptr, nullptr, 0, nullptr}};

@@ -6,10 +6,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
-#include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
-#include <c10/core/GradMode.h>
-#include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
 
 #include <cstring>
@@ -41,67 +38,6 @@ ConvStepFn g_conv_step = nullptr;
 BytesFn g_scan_bytes = nullptr;
 ScanFn g_scan = nullptr;
 ScanStepFn g_scan_step = nullptr;
-
-constexpr int64_t kMost = 0x7fffffff;
-
-// An optional operand: false if it is there but not a plain tensor.
-bool optional(PyObject* o, const at::Tensor** t) {
-  *t = nullptr;
-  if (o == Py_None) return true;
-  *t = plain(o);
-  return *t != nullptr;
-}
-// A dense tensor of this type and these sizes on x's device (absent ones are fine).
-bool dense(const at::Tensor* t, at::ScalarType type, at::IntArrayRef sizes, const at::Tensor& x) {
-  return t == nullptr || (t->scalar_type() == type && t->sizes() == sizes && t->device() == x.device() && t->is_contiguous());
-}
-const void* ptr(const at::Tensor* t) { return t == nullptr ? nullptr : t->const_data_ptr(); }
-const float* f32(const at::Tensor* t) { return static_cast<const float*>(ptr(t)); }
-const int32_t* i32(const at::Tensor* t) { return static_cast<const int32_t*>(ptr(t)); }
-// Whether one of them asks for a gradient or has a tangent of forward-mode differentiation: Python differentiates or refuses.
-bool any_grad(std::initializer_list<const at::Tensor*> ts) {
-  const bool back = c10::GradMode::is_enabled(), forward = c10::AutogradState::get_tls_state().get_fw_grad_mode();
-  for (const at::Tensor* t : ts)
-    if (t != nullptr && ((back && t->requires_grad()) || (forward && t->_fw_grad(0).defined()))) return true;
-  return false;
-}
-// A state that a kernel has written through its address: autograd's check of saved tensors goes by their versions.  (Tensors made in
-// inference mode have none.)
-void written(const at::Tensor& t) {
-  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
-}
-bool small(const at::Tensor& t) {
-  for (int64_t s : t.sizes())
-    if (s > kMost) return false;
-  return true;
-}
-void* stream_of(const at::Tensor& x) { return c10::cuda::getCurrentCUDAStream(x.get_device()).stream(); }
-
-PyObject* answer(int status, at::Tensor&& y) {
-  if (status != FDNN_OK) return PyLong_FromLong(status);
-  return THPVariable_Wrap(std::move(y));
-}
-PyObject* answer(int status, std::initializer_list<at::Tensor> ts) {
-  if (status != FDNN_OK) return PyLong_FromLong(status);
-  PyObject* tuple = PyTuple_New(Py_ssize_t(ts.size()));
-  if (tuple == nullptr) return nullptr;
-  Py_ssize_t i = 0;
-  for (const at::Tensor& t : ts) {
-    PyObject* o = nullptr;
-    if (t.defined()) {
-      o = THPVariable_Wrap(t);
-      if (o == nullptr) {
-        Py_DECREF(tuple);
-        return nullptr;
-      }
-    } else {
-      o = Py_None;
-      Py_INCREF(o);
-    }
-    PyTuple_SET_ITEM(tuple, i++, o);
-  }
-  return tuple;
-}
 
 void strides4(const at::Tensor& t, int64_t* s) {
   s[0] = t.stride(0);

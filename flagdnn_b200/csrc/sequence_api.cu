@@ -1,4 +1,4 @@
-// C-ABI front end of the group norm and state space operators: validation and launches.  See include/flagdnn_b200.h.
+// C-ABI front end of the group norm, state space and delta rule operators: validation and launches.  See include/flagdnn_b200.h.
 #include "sequence_internal.h"
 
 using namespace fdnn;
@@ -81,6 +81,41 @@ int scan_params(const fdnn_scan_desc* d, ScanParams* p) {
   for (int i = 0; i < 4; ++i) {
     p->b_s[i] = d->b_strides[i];
     p->c_s[i] = d->c_strides[i];
+  }
+  p->initial = nullptr;
+  p->lengths = nullptr;
+  p->final_state = nullptr;
+  p->workspace = nullptr;
+  return FDNN_OK;
+}
+
+int delta_params(const fdnn_delta_rule_desc* d, DeltaParams* p) {
+  if (d == nullptr) return api_fail(FDNN_BAD_PARAM, "descriptor is NULL");
+  if (!float_type(d->dtype)) return api_fail(FDNN_NOT_SUPPORTED, "Unsupported dtype");
+  if (d->gate_dtype != d->dtype && d->gate_dtype != FDNN_F32)
+    return api_fail(FDNN_NOT_SUPPORTED, "delta and beta must be of the input's type or float32");
+  if (d->n < 0 || d->l < 0 || d->heads < 0) return api_fail(FDNN_BAD_PARAM, "negative extent");
+  if (d->l > kMaxTokens) return api_fail(FDNN_NOT_SUPPORTED, "more tokens in a row than the kernels count");
+  if (d->n > kMaxRows) return api_fail(FDNN_NOT_SUPPORTED, "more rows than the kernels count");
+  if (d->dk < 1 || d->dk > FDNN_DELTA_RULE_MAX_DK) return api_fail(FDNN_NOT_SUPPORTED, "a key must have 1 to 256 channels");
+  if (d->dv < 1 || d->dv > FDNN_DELTA_RULE_MAX_DV) return api_fail(FDNN_NOT_SUPPORTED, "a value must have 1 to 1024 channels");
+  if (d->heads > FDNN_DELTA_RULE_MAX_HEADS) return api_fail(FDNN_NOT_SUPPORTED, "more heads than the kernels count");
+  if (d->key_heads <= 0 || d->heads % d->key_heads != 0) return api_fail(FDNN_BAD_PARAM, "heads must be divisible by key heads");
+  p->N = d->n; p->L = d->l; p->G = d->key_heads; p->H = d->heads; p->K = d->dk; p->V = d->dv;
+  p->gate_f32 = d->gate_dtype == FDNN_F32;
+  p->softplus = d->delta_softplus != 0;
+  p->sigmoid = d->beta_sigmoid != 0;
+  p->norm = d->qk_norm != 0;
+  p->scale = d->scale;
+  for (int i = 0; i < 4; ++i) {
+    p->q_s[i] = d->q_strides[i];
+    p->k_s[i] = d->k_strides[i];
+    p->v_s[i] = d->v_strides[i];
+    p->y_s[i] = d->y_strides[i];
+  }
+  for (int i = 0; i < 3; ++i) {
+    p->delta_s[i] = d->delta_strides[i];
+    p->beta_s[i] = d->beta_strides[i];
   }
   p->initial = nullptr;
   p->lengths = nullptr;
@@ -214,6 +249,50 @@ int fdnn_selective_scan_step(const fdnn_scan_desc* desc, const void* u, const vo
   p.u = u; p.delta = delta; p.A = A; p.B = B; p.Cm = C; p.D = D; p.z = z; p.delta_bias = delta_bias; p.y = y;
   const cudaError_t e = launch_selective_scan_step(desc->dtype, p, state, n_slots, slots, static_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? FDNN_OK : api_fail_cuda("selective_scan_step launch", e);
+}
+
+int fdnn_gated_delta_rule_workspace_bytes(const fdnn_delta_rule_desc* desc, int64_t* bytes) {
+  if (bytes == nullptr) return api_fail(FDNN_BAD_PARAM, "bytes is NULL");
+  DeltaParams p;
+  const int st = delta_params(desc, &p);
+  if (st != FDNN_OK) return st;
+  *bytes = p.N == 0 || p.H == 0 || p.L == 0 ? 0 : delta_rule_workspace(desc->dtype, p);
+  return FDNN_OK;
+}
+
+int fdnn_gated_delta_rule_fwd(const fdnn_delta_rule_desc* desc, const void* q, const void* k, const void* v, const void* delta,
+                              const void* beta, const float* A, const float* delta_bias, const float* initial_state,
+                              const int32_t* lengths, void* y, float* final_state, void* workspace, int64_t workspace_bytes,
+                              void* stream) {
+  DeltaParams p;
+  int st = delta_params(desc, &p);
+  if (st != FDNN_OK) return st;
+  if (p.N == 0 || p.H == 0) return FDNN_OK;
+  if (p.L > 0) {
+    if (q == nullptr || k == nullptr || v == nullptr || delta == nullptr || beta == nullptr || y == nullptr)
+      return api_fail(FDNN_BAD_PARAM, "q, k, v, delta, beta and y must not be NULL");
+    st = check_workspace(workspace, workspace_bytes, delta_rule_workspace(desc->dtype, p));
+    if (st != FDNN_OK) return st;
+  }
+  p.q = q; p.k = k; p.v = v; p.delta = delta; p.beta = beta; p.A = A; p.delta_bias = delta_bias;
+  p.initial = initial_state; p.lengths = lengths; p.y = y; p.final_state = final_state; p.workspace = workspace;
+  const cudaError_t e = launch_delta_rule(desc->dtype, p, static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? FDNN_OK : api_fail_cuda("gated_delta_rule launch", e);
+}
+
+int fdnn_gated_delta_rule_step(const fdnn_delta_rule_desc* desc, const void* q, const void* k, const void* v, const void* delta,
+                               const void* beta, const float* A, const float* delta_bias, float* state, int32_t n_slots,
+                               const int32_t* slots, void* y, void* stream) {
+  DeltaParams p;
+  const int st = delta_params(desc, &p);
+  if (st != FDNN_OK) return st;
+  if (p.N == 0 || p.H == 0) return FDNN_OK;
+  if (n_slots < 0 || (slots == nullptr && n_slots < p.N)) return api_fail(FDNN_BAD_PARAM, "fewer states than rows");
+  if (q == nullptr || k == nullptr || v == nullptr || delta == nullptr || beta == nullptr || y == nullptr || (state == nullptr && n_slots > 0))
+    return api_fail(FDNN_BAD_PARAM, "q, k, v, delta, beta, state and y must not be NULL");
+  p.q = q; p.k = k; p.v = v; p.delta = delta; p.beta = beta; p.A = A; p.delta_bias = delta_bias; p.y = y;
+  const cudaError_t e = launch_delta_rule_step(desc->dtype, p, state, n_slots, slots, static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? FDNN_OK : api_fail_cuda("gated_delta_rule_step launch", e);
 }
 
 }  // extern "C"

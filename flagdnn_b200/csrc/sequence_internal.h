@@ -1,4 +1,4 @@
-// Internal declarations of the group norm and state space operators (group_norm*.cu, causal_conv.cu, selective_scan.cu),
+// Internal declarations of the group norm and state space operators (group_norm*.cu, causal_conv.cu, selective_scan*.cu, delta_rule*.cu),
 // shared with their C-ABI front end (sequence_api.cu).  Nothing here is exported.
 #pragma once
 #include <cuda_runtime.h>
@@ -59,5 +59,26 @@ cudaError_t launch_selective_scan(int dtype, const ScanParams& p, cudaStream_t s
 // One token a row (l strides unused): state [n_slots, C, S] in place.
 cudaError_t launch_selective_scan_step(int dtype, const ScanParams& p, float* state, int n_slots, const int* slots,
                                        cudaStream_t stream);
+
+struct DeltaParams {
+  int N, L, G, H, K, V;                           // G key heads, H heads; K = dk, V = dv
+  int gate_f32;                                   // 1: delta and beta are float32, 0: of q's type
+  int softplus, sigmoid, norm;
+  float scale;
+  long long q_s[4], k_s[4], v_s[4], y_s[4];       // element strides in (n, l, head, channel) order
+  long long delta_s[3], beta_s[3];                // (n, l, head)
+  const void *q, *k, *v, *delta, *beta;
+  const float *A, *delta_bias;                    // [H] or null
+  const float* initial;                           // [N, H, V, K] or null (zeros)
+  const int* lengths;                             // [N] or null
+  void* y;
+  float* final_state;                             // [N, H, V, K] or null
+  void* workspace;
+};
+long long delta_rule_workspace(int dtype, const DeltaParams& p);
+cudaError_t launch_delta_rule(int dtype, const DeltaParams& p, cudaStream_t stream);
+// One token a row (l strides unused): state [n_slots, H, V, K] in place.
+cudaError_t launch_delta_rule_step(int dtype, const DeltaParams& p, float* state, int n_slots, const int* slots,
+                                   cudaStream_t stream);
 
 }  // namespace fdnn

@@ -12,6 +12,7 @@ from typing import Any
 import torch
 
 from . import conv_host as _conv
+from . import delta_host as _delta
 from . import norm_host as _norm
 from . import pool_host as _pool
 from . import sequence_host as _sequence
@@ -70,4 +71,6 @@ causal_conv1d = _sequence.causal_conv1d            # the state space operators a
 causal_conv1d_step = _sequence.causal_conv1d_step
 selective_scan = _sequence.selective_scan
 selective_scan_step = _sequence.selective_scan_step
+gated_delta_rule = _delta.gated_delta_rule
+gated_delta_rule_step = _delta.gated_delta_rule_step
 fused_conv2d_bias_relu = _conv.fused_conv2d_bias_relu

@@ -351,6 +351,45 @@ int fdnn_selective_scan_step(const fdnn_scan_desc* desc, const void* u, const vo
                              const void* C, const float* D, const void* z, const float* delta_bias, float* state,
                              int32_t n_slots, const int32_t* slots, void* y, void* stream);
 
+/* The gated delta rule: a head's state S, [dv, dk] in fp32, forgets by a decay, and what it answers to a key is moved towards
+ * a value.  With dt = delta + delta_bias (softplus of it if delta_softplus), a = exp(A dt) (A NULL: exp(dt)) and b = beta (its
+ * logistic function if beta_sigmoid), for each token
+ *   S <- a S,   S <- S + b (v - S k) k^T,   y = S q * scale
+ * Head h has the keys and queries of key head h / (heads / key_heads); with qk_norm they are divided by
+ * sqrt(sum of their squares + 1e-6) first.  A and delta_bias [heads] and the states [N, heads, dv, dk] are dense float32;
+ * delta_bias, A, initial_state (zeros), lengths (see above) and final_state may be NULL.  final_state must not overlap
+ * initial_state.  Longer prompts are taken in chunks of 64 tokens: a q, k, v, delta or beta that is not finite can make the whole chunk
+ * that it lies in not finite, its earlier tokens too. */
+#define FDNN_DELTA_RULE_MAX_DK 256
+#define FDNN_DELTA_RULE_MAX_DV 1024
+#define FDNN_DELTA_RULE_MAX_HEADS 65535
+typedef struct fdnn_delta_rule_desc {
+  int32_t dtype;               /* FDNN_F16, FDNN_BF16 or FDNN_F32: q, k, v, y */
+  int32_t gate_dtype;          /* delta and beta: dtype or FDNN_F32 */
+  int32_t n, l, key_heads, heads, dk, dv;
+  int32_t delta_softplus, beta_sigmoid, qk_norm;
+  float scale;
+  int64_t q_strides[4];        /* element strides in (n, l, key head, dk) order */
+  int64_t k_strides[4];
+  int64_t v_strides[4];        /* (n, l, head, dv) */
+  int64_t y_strides[4];
+  int64_t delta_strides[3];    /* (n, l, head) */
+  int64_t beta_strides[3];
+} fdnn_delta_rule_desc;
+
+/* Scratch that fdnn_gated_delta_rule_fwd needs, 16-byte aligned. */
+int fdnn_gated_delta_rule_workspace_bytes(const fdnn_delta_rule_desc* desc, int64_t* bytes);
+int fdnn_gated_delta_rule_fwd(const fdnn_delta_rule_desc* desc, const void* q, const void* k, const void* v,
+                              const void* delta, const void* beta, const float* A, const float* delta_bias,
+                              const float* initial_state, const int32_t* lengths, void* y, float* final_state,
+                              void* workspace, int64_t workspace_bytes, void* stream);
+
+/* The same for one token of each row (l and the l strides are not read; n at most 2^31 - 65537), states
+ * [n_slots, heads, dv, dk] in place as for fdnn_causal_conv1d_step. */
+int fdnn_gated_delta_rule_step(const fdnn_delta_rule_desc* desc, const void* q, const void* k, const void* v,
+                               const void* delta, const void* beta, const float* A, const float* delta_bias, float* state,
+                               int32_t n_slots, const int32_t* slots, void* y, void* stream);
+
 /* Every wait inside the kernels is bounded; a wait that runs out records a
  * code in a per-device status word and the kernel returns early.  This call
  * synchronises the current device, returns the word in *word (0 = no
