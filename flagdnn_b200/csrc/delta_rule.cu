@@ -25,7 +25,7 @@ namespace {
 
 constexpr int kChunk = 64;
 constexpr int kChunkKeys = 128;      // the widest key that the chunks' kernels take
-constexpr int kFactors = 6 * kChunk; // floats a chunk and head: a, b, d, t, p, and e^(G_64)
+constexpr int kFactors = 6 * kChunk; // floats a chunk and head: -a, b, d, t, p, and e^(G_64)
 constexpr int kSquare = kChunk * kChunk * 2;   // bytes of a 64 x 64 part
 
 // How many 16-bit parts: of keys and queries, of S and P in what only y sees.
@@ -43,6 +43,12 @@ __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint3
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// D = A B.
+__device__ __forceinline__ void mma_first(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+               : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
 }
 // The same of 16 x 8 x 8 in TF32: A at (row, k = lane % 4), (row + 8, k), (row, k + 4), (row + 8, k + 4), B at k = lane % 4, + 4.
 __device__ __forceinline__ void mma_tf32(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -100,20 +106,36 @@ __device__ __forceinline__ void row_scales(const float (&c)[TILES][4], float& lo
   lower = raise(quad_max(m0));
   upper = raise(quad_max(m1));
 }
-// Accumulator tiles 2 s and 2 s + 1 as the A operand of k-step s.
-__device__ __forceinline__ void operand(const float (&x)[4], const float (&y)[4], float s0, float s1, uint32_t (&hi)[4], uint32_t (&lo)[4]) {
-  const float v[8] = {x[0] * s0, x[1] * s0, x[2] * s1, x[3] * s1, y[0] * s0, y[1] * s0, y[2] * s1, y[3] * s1};
+// The two rows of an accumulator tile, as pairs.
+__device__ __forceinline__ F2 first_row(const float (&c)[4]) { return f2_pack(c[0], c[1]); }
+__device__ __forceinline__ F2 second_row(const float (&c)[4]) { return f2_pack(c[2], c[3]); }
+__device__ __forceinline__ void set_rows(float (&c)[4], F2 first, F2 second) {
+  f2_split(first, c[0], c[1]);
+  f2_split(second, c[2], c[3]);
+}
+__device__ __forceinline__ uint32_t high(F2 v) {
+  float x, y;
+  f2_split(v, x, y);
+  return high(x, y);
+}
+__device__ __forceinline__ uint32_t low(F2 v, uint32_t hi) {
+  const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+  return high(f2_fma(f2_pack(h.x, h.y), f2_both(-1.0f), v));
+}
+// Accumulator tiles 2 s and 2 s + 1, their rows scaled, as the A operand of k-step s: high parts, and low ones.
+__device__ __forceinline__ void operand(const float (&x)[4], const float (&y)[4], F2 s0, F2 s1, uint32_t (&hi)[4], uint32_t (&lo)[4]) {
+  const F2 v[4] = {f2_mul(first_row(x), s0), f2_mul(second_row(x), s1), f2_mul(first_row(y), s0), f2_mul(second_row(y), s1)};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    hi[i] = high(v[2 * i], v[2 * i + 1]);
-    lo[i] = low(v[2 * i], v[2 * i + 1], hi[i]);
+    hi[i] = high(v[i]);
+    lo[i] = low(v[i], hi[i]);
   }
 }
-__device__ __forceinline__ void operand(const float (&x)[4], const float (&y)[4], float s0, float s1, uint32_t (&hi)[4]) {
-  hi[0] = high(x[0] * s0, x[1] * s0);
-  hi[1] = high(x[2] * s1, x[3] * s1);
-  hi[2] = high(y[0] * s0, y[1] * s0);
-  hi[3] = high(y[2] * s1, y[3] * s1);
+__device__ __forceinline__ void operand(const float (&x)[4], const float (&y)[4], F2 s0, F2 s1, uint32_t (&hi)[4]) {
+  hi[0] = high(f2_mul(first_row(x), s0));
+  hi[1] = high(f2_mul(second_row(x), s1));
+  hi[2] = high(f2_mul(first_row(y), s0));
+  hi[3] = high(f2_mul(second_row(y), s1));
 }
 
 // Tiles of 16-bit operands: rows of COLS values, whose 16-byte pieces lie at piece ^ (row % 8), so that eight rows of a piece
@@ -387,7 +409,7 @@ delta_prepare_kernel(const DeltaParams p) {
     float* factors = reinterpret_cast<float*>(out + (2 + Parts<T>::kOut) * kSquare);
     if (tid < kChunk) {
       const float hi = s.sum_hi[tid], lo = s.sum_lo[tid], since = expf(hi + lo);
-      factors[tid] = since * s.key_scale[tid];
+      factors[tid] = -since * s.key_scale[tid];
       factors[kChunk + tid] = since * s.query_scale[tid];
       factors[2 * kChunk + tid] = expf((s.sum_hi[kChunk - 1] - hi) + (s.sum_lo[kChunk - 1] - lo)) * s.key_scale[tid];
       if (tid == kChunk - 1) factors[5 * kChunk] = since;
@@ -464,17 +486,21 @@ delta_prepare_kernel(const DeltaParams p) {
 
 // ---- the chunks in order -------------------------------------------------------------------------------------------
 
-constexpr int kLoaders = 2;   // warps that copy operands; the others hold 16 rows of the state each
+constexpr int kMostSlices = 4;           // 16 rows of the state each, two warps to a slice
+constexpr int kExchange = 2 * 16 * 512;  // bytes through which two warps add up their halves
 
 template <typename T>
-__host__ __device__ constexpr int value_pitch(int warps) { return 16 * warps * int(sizeof(T)) + 16; }   // bytes; eight rows in different banks
+__host__ __device__ constexpr int value_pitch(int slices) { return 16 * slices * int(sizeof(T)) + 16; }   // bytes; eight rows in different banks
 
-// Output tile of a chunk: o[token tile][..] holds rows (value channels) lane / 4, + 8 and tokens 2 (lane % 4), + 1.
+__device__ __forceinline__ void pair_barrier(int id) { asm volatile("bar.sync %0, 64;" ::"r"(id) : "memory"); }
+__device__ __forceinline__ F2 pair_at(const float* p) { return *reinterpret_cast<const F2*>(p); }
+
+// Two output tiles: o[i][..] holds rows (value channels) lane / 4, + 8 and tokens 8 i + 2 (lane % 4), + 1.
 template <typename T, bool WHOLE>
-__device__ __forceinline__ void put_outputs(const DeltaParams& p, T* y, const float (&o)[8][4], int tokens, int channels) {
+__device__ __forceinline__ void put_outputs(const DeltaParams& p, T* y, const float (&o)[2][4], int tokens, int channels) {
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
 #pragma unroll
-  for (int n = 0; n < 8; ++n) {
+  for (int n = 0; n < 2; ++n) {
     if constexpr (sizeof(T) == 2) {
       const uint32_t lower = transposed(pack2(from_f32<T>(o[n][0]), from_f32<T>(o[n][1])));
       const uint32_t upper = transposed(pack2(from_f32<T>(o[n][2]), from_f32<T>(o[n][3])));
@@ -505,294 +531,292 @@ __device__ __forceinline__ void put_outputs(const DeltaParams& p, T* y, const fl
 
 // WHOLE: 16 bytes of neighbouring value channels are copied at once, and pairs stored.
 template <typename T, int KEYS, bool WHOLE>
-__global__ void __launch_bounds__(192)
-delta_chunks_kernel(const DeltaParams p, int slices, int stages) {
+__global__ void __launch_bounds__(2 * kMostSlices * 32, 1)
+delta_chunks_kernel(const DeltaParams p, int blocks_a_head, int stages) {
   extern __shared__ __align__(128) uint8_t smem_raw[];
   chained();
   using W = Work<T, KEYS>;
-  constexpr int kKeyPart = kChunk * KEYS * 2;
+  constexpr int kKeyPart = kChunk * KEYS * 2, kHalf = KEYS / 2;
   const Layout w = layout_of<T, KEYS>(p);
-  const int warps = (blockDim.x >> 5) - kLoaders, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int slice = int(blockIdx.x % slices), h = int(blockIdx.x / slices % p.H);
-  const long long n = blockIdx.x / slices / p.H;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, slices = blockDim.x >> 6;
+  const int h = int(blockIdx.x / blocks_a_head % p.H);
+  const long long n = blockIdx.x / blocks_a_head / p.H;
   const int end = row_end(p, n), chunks = (end + kChunk - 1) / kChunk;
-  const int first = slice * warps * 16;   // the block's first value channel
-  const int pitch = value_pitch<T>(warps), stage_bytes = W::kStage + kChunk * pitch;
+  const int first = int(blockIdx.x % blocks_a_head) * slices * 16;   // the block's first value channel
+  const int pitch = value_pitch<T>(slices), stage_bytes = W::kStage + kChunk * pitch;
   const uint32_t smem = smem_u32(smem_raw);
 
-  if (warp >= warps) {
-    // ---- loaders: chunk c + 1 while the others are at chunk c, where there is room for two
-    const int tid = threadIdx.x - warps * 32;
-    constexpr int kStep = kLoaders * 32;
-    const uint8_t* keys = w.keys + (n * p.G + h / (p.H / p.G)) * w.chunks * (2ll * W::kKeyBytes);
-    const uint8_t* heads = w.heads + (n * p.H + h) * w.chunks * (long long)W::kHeadBytes;
-    const T* v0 = static_cast<const T*>(p.v) + n * p.v_s[0] + h * p.v_s[2] + first * p.v_s[3];
-    auto ask = [&](int c) {
-      const uint32_t to = smem + (c % stages) * stage_bytes;
-      const uint8_t* from = keys + c * (2ll * W::kKeyBytes);
+  const uint8_t* keys_from = w.keys + (n * p.G + h / (p.H / p.G)) * w.chunks * (2ll * W::kKeyBytes);
+  const uint8_t* heads_from = w.heads + (n * p.H + h) * w.chunks * (long long)W::kHeadBytes;
+  const T* v0 = static_cast<const T*>(p.v) + n * p.v_s[0] + h * p.v_s[2] + first * p.v_s[3];
+  auto ask = [&](int c) {   // a chunk's operands, by all threads
+    const int tid = threadIdx.x, step = blockDim.x;
+    const uint32_t to = smem + (c % stages) * stage_bytes;
+    const uint8_t* from = keys_from + c * (2ll * W::kKeyBytes);
 #pragma unroll 8
-      for (int i = tid; i < 2 * W::kKeyBytes / 16; i += kStep) copy16(to + i * 16, from + i * 16, 16);
-      from = heads + c * (long long)W::kHeadBytes;
+    for (int i = tid; i < 2 * W::kKeyBytes / 16; i += step) copy16(to + i * 16, from + i * 16, 16);
+    from = heads_from + c * (long long)W::kHeadBytes;
 #pragma unroll 8
-      for (int i = tid; i < W::kHeadBytes / 16; i += kStep) copy16(to + 2 * W::kKeyBytes + i * 16, from + i * 16, 16);
-      const int here = min(warps * 16, p.V - first), tokens = min(end - c * kChunk, kChunk);
-      const uint32_t values = to + W::kStage;
-      if constexpr (WHOLE) {
-        constexpr int kV = 16 / sizeof(T);
-        const int pieces = warps * 16 / kV;
-        for (int i = tid; i < kChunk * pieces; i += kStep) {
-          const int r = i / pieces, at = i % pieces * kV, bytes = r < tokens ? min(max(here - at, 0), kV) * int(sizeof(T)) : 0;
-          copy16(values + r * pitch + at * int(sizeof(T)), bytes > 0 ? v0 + (c * kChunk + r) * p.v_s[1] + at : v0, bytes);
-        }
-      } else {
-        T* to_v = reinterpret_cast<T*>(smem_raw + (c % stages) * stage_bytes + W::kStage);
-        for (int i = tid; i < kChunk * warps * 16; i += kStep) {
-          const int r = i / (warps * 16), at = i % (warps * 16);
-          to_v[r * (pitch / int(sizeof(T))) + at] =
-              r < tokens && at < here ? v0[(c * kChunk + r) * p.v_s[1] + at * p.v_s[3]] : from_f32<T>(0.0f);
-        }
+    for (int i = tid; i < W::kHeadBytes / 16; i += step) copy16(to + 2 * W::kKeyBytes + i * 16, from + i * 16, 16);
+    const int here = min(slices * 16, p.V - first), tokens = min(end - c * kChunk, kChunk);
+    const uint32_t values = to + W::kStage;
+    if constexpr (WHOLE) {
+      constexpr int kV = 16 / sizeof(T);
+      const int pieces = slices * 16 / kV;   // a thread keeps its column: 64 slices threads are a multiple of it
+      const int at = tid % pieces * kV, bytes = min(max(here - at, 0), kV) * int(sizeof(T));
+#pragma unroll 4
+      for (int r = tid / pieces; r < kChunk; r += step / pieces) {
+        const bool there = r < tokens && bytes > 0;
+        copy16(values + r * pitch + at * int(sizeof(T)), there ? v0 + (c * kChunk + r) * p.v_s[1] + at : v0, there ? bytes : 0);
       }
-      async_commit();
-    };
-    if (chunks > 0) ask(0);
-    for (int c = 0; c < chunks; ++c) {
-      async_wait<0>();
-      __syncthreads();                 // chunk c is there, and the others are done with chunk c - 1
-      if (stages > 1 && c + 1 < chunks) ask(c + 1);
-      if (stages == 1) {
-        __syncthreads();               // .. and with chunk c
-        if (c + 1 < chunks) ask(c + 1);
+    } else {
+      T* to_v = reinterpret_cast<T*>(smem_raw + (c % stages) * stage_bytes + W::kStage);
+      for (int i = tid; i < kChunk * slices * 16; i += step) {
+        const int r = i / (slices * 16), at = i % (slices * 16);
+        to_v[r * (pitch / int(sizeof(T))) + at] =
+            r < tokens && at < here ? v0[(c * kChunk + r) * p.v_s[1] + at * p.v_s[3]] : from_f32<T>(0.0f);
       }
     }
-    return;
-  }
+    async_commit();
+  };
+  if (chunks > 0) ask(0);
 
-  // ---- 16 rows of the state, as the accumulators of S^T's transposed product: s[j]: rows lane / 4, + 8, keys' channels 8 j + 2 (lane % 4), + 1
+  // Two warps hold 16 rows of the state, half of the keys' channels each: s[j] rows lane / 4, + 8, channels 8 j + 2 (lane % 4), + 1.
   const int g = lane >> 2, t = lane & 3, m = lane >> 3, r = lane & 7;
-  const int row0 = first + warp * 16, channels = min(16, p.V - row0);
+  const int slice = warp >> 1, half = warp & 1;
+  const int row0 = first + slice * 16, channels = min(16, p.V - row0);
   const long long state_at = ((n * p.H + h) * p.V + row0) * (long long)p.K;
-  float s[KEYS / 8][4];
+  // what a warp leaves for the other one: its 8 tiles of S k, and its 8 of S q
+  float4* const exchange = reinterpret_cast<float4*>(smem_raw + stages * stage_bytes + slice * kExchange) + lane;
+  float4 *const mine = exchange + half * 16 * 32, *const theirs = exchange + (half ^ 1) * 16 * 32;
+  float s[kHalf / 8][4];
 #pragma unroll
-  for (int j = 0; j < KEYS / 8; ++j)
+  for (int j = 0; j < kHalf / 8; ++j)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int row = g + (i >> 1) * 8, at = j * 8 + 2 * t + (i & 1);
+      const int row = g + (i >> 1) * 8, at = half * kHalf + j * 8 + 2 * t + (i & 1);
       s[j][i] = p.initial != nullptr && row < channels && at < p.K ? p.initial[state_at + (long long)row * p.K + at] : 0.0f;
     }
   T* y = static_cast<T*>(p.y) + n * p.y_s[0] + h * p.y_s[2] + row0 * p.y_s[3];
+  // y of 16-token blocks 0 and 3 is finished by the first of the two warps, of 1 and 2 by the second: P is lower triangular
+  const int own[2] = {half, 3 - half};
 
   for (int c = 0; c < chunks; ++c) {
-    __syncthreads();
+    async_wait<0>();
+    __syncthreads();   // chunk c is there, and all are done with chunk c - 1
+    if (stages > 1 && c + 1 < chunks) ask(c + 1);
     const int base_at = (c % stages) * stage_bytes;
     const uint32_t keys = smem + base_at, queries = keys + W::kKeyBytes, square = queries + W::kKeyBytes;
-    const float* factors = reinterpret_cast<const float*>(smem_raw + base_at + 2 * W::kKeyBytes + (2 + Parts<T>::kOut) * kSquare);
-    // S k and S q
-    float s0, s1;
-    row_scales<KEYS / 8>(s, s0, s1);
-    float x[8][4] = {}, o[8][4] = {};
+    const float* factors = reinterpret_cast<const float*>(smem_raw + base_at + 2 * W::kKeyBytes + (2 + Parts<T>::kOut) * kSquare) + 2 * t;
+    float x[8][4];
+    {   // S k and S q, of this warp's channels
+      float s0, s1, o[8][4];
+      row_scales<kHalf / 8>(s, s0, s1);
+      const F2 up0 = f2_both(s0), up1 = f2_both(s1);
 #pragma unroll
-    for (int k = 0; k < KEYS / 16; ++k) {
-      uint32_t hi[4], lo[4];
-      operand(s[2 * k], s[2 * k + 1], s0, s1, hi, lo);
+      for (int k = 0; k < kHalf / 16; ++k) {
+        uint32_t hi[4], lo[4];
+        operand(s[2 * k], s[2 * k + 1], up0, up1, hi, lo);
+        const int at = half * (kHalf / 8) + 2 * k + (m & 1);
+        uint32_t b[4][4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int at = piece<KEYS>(j * 16 + (m >> 1) * 8 + r, 2 * k + (m & 1));
-        uint32_t b[4];
-        ldmatrix(b, keys + at);
+        for (int j = 0; j < 4; ++j) ldmatrix(b[j], keys + piece<KEYS>(j * 16 + (m >> 1) * 8 + r, at));
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          mma(x[2 * j + i], hi, b[2 * i], b[2 * i + 1]);
-          mma(x[2 * j + i], lo, b[2 * i], b[2 * i + 1]);
+        for (int j = 0; j < 8; ++j) {
+          if (k == 0) mma_first(x[j], hi, b[j >> 1][2 * (j & 1)], b[j >> 1][2 * (j & 1) + 1]);
+          else mma(x[j], hi, b[j >> 1][2 * (j & 1)], b[j >> 1][2 * (j & 1) + 1]);
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) mma(x[j], lo, b[j >> 1][2 * (j & 1)], b[j >> 1][2 * (j & 1) + 1]);
+        if constexpr (Parts<T>::kKey == 2) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) ldmatrix(b[j], keys + kKeyPart + piece<KEYS>(j * 16 + (m >> 1) * 8 + r, at));
+#pragma unroll
+          for (int j = 0; j < 8; ++j) mma(x[j], hi, b[j >> 1][2 * (j & 1)], b[j >> 1][2 * (j & 1) + 1]);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) ldmatrix(b[j], queries + piece<KEYS>(j * 16 + (m >> 1) * 8 + r, at));
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          if (k == 0) mma_first(o[j], hi, b[j >> 1][2 * (j & 1)], b[j >> 1][2 * (j & 1) + 1]);
+          else mma(o[j], hi, b[j >> 1][2 * (j & 1)], b[j >> 1][2 * (j & 1) + 1]);
+        }
+        if constexpr (Parts<T>::kOut == 2) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) mma(o[j], lo, b[j >> 1][2 * (j & 1)], b[j >> 1][2 * (j & 1) + 1]);
         }
         if constexpr (Parts<T>::kKey == 2) {
-          uint32_t bl[4];
-          ldmatrix(bl, keys + kKeyPart + at);
 #pragma unroll
-          for (int i = 0; i < 2; ++i) mma(x[2 * j + i], hi, bl[2 * i], bl[2 * i + 1]);
-        }
-        ldmatrix(b, queries + at);
+          for (int j = 0; j < 4; ++j) ldmatrix(b[j], queries + kKeyPart + piece<KEYS>(j * 16 + (m >> 1) * 8 + r, at));
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          mma(o[2 * j + i], hi, b[2 * i], b[2 * i + 1]);
-          if constexpr (Parts<T>::kOut == 2) mma(o[2 * j + i], lo, b[2 * i], b[2 * i + 1]);
-        }
-        if constexpr (Parts<T>::kKey == 2) {
-          uint32_t bl[4];
-          ldmatrix(bl, queries + kKeyPart + at);
-#pragma unroll
-          for (int i = 0; i < 2; ++i) mma(o[2 * j + i], hi, bl[2 * i], bl[2 * i + 1]);
+          for (int j = 0; j < 8; ++j) mma(o[j], hi, b[j >> 1][2 * (j & 1)], b[j >> 1][2 * (j & 1) + 1]);
         }
       }
+      const F2 down0 = f2_both(inverse_of_power(s0)), down1 = f2_both(inverse_of_power(s1));
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        set_rows(x[j], f2_mul(first_row(x[j]), down0), f2_mul(second_row(x[j]), down1));
+        set_rows(o[j], f2_mul(first_row(o[j]), down0), f2_mul(second_row(o[j]), down1));
+        mine[j * 32] = make_float4(x[j][0], x[j][1], x[j][2], x[j][3]);
+        mine[(8 + j) * 32] = make_float4(o[j][0], o[j][1], o[j][2], o[j][3]);
+      }
     }
-    // v - e^G S k
-    const float i0 = inverse_of_power(s0), i1 = inverse_of_power(s1);
+    pair_barrier(1 + slice);
+    // v - e^G S k (the factors are negative)
     const uint32_t values = smem + base_at + W::kStage;
 #pragma unroll
     for (int j = 0; j < 8; j += 2) {
       float v[2][4];
       if constexpr (sizeof(T) == 2) {
         uint32_t b[4];   // channels 0 .. 7 and 8 .. 15 of tokens 8 j .., then of 8 (j + 1) ..
-        ldmatrix_t(b, values + (j * 8 + (m >> 1) * 8 + r) * pitch + (warp * 16 + (m & 1) * 8) * 2);
+        ldmatrix_t(b, values + (j * 8 + (m >> 1) * 8 + r) * pitch + (slice * 16 + (m & 1) * 8) * 2);
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i >> 2][i & 3] = to_f32<T>(reinterpret_cast<const T*>(b)[i]);
       } else {
         const float* f = reinterpret_cast<const float*>(smem_raw + base_at + W::kStage);
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-          v[i >> 2][i & 3] = f[((j + (i >> 2)) * 8 + 2 * t + (i & 1)) * (pitch / 4) + warp * 16 + g + ((i >> 1) & 1) * 8];
+          v[i >> 2][i & 3] = f[((j + (i >> 2)) * 8 + 2 * t + (i & 1)) * (pitch / 4) + slice * 16 + g + ((i >> 1) & 1) * 8];
       }
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const float2 a = *reinterpret_cast<const float2*>(factors + (j + i) * 8 + 2 * t);
-        x[j + i][0] = v[i][0] - a.x * (x[j + i][0] * i0);
-        x[j + i][1] = v[i][1] - a.y * (x[j + i][1] * i0);
-        x[j + i][2] = v[i][2] - a.x * (x[j + i][2] * i1);
-        x[j + i][3] = v[i][3] - a.y * (x[j + i][3] * i1);
+        const F2 a = pair_at(factors + (j + i) * 8);
+        const float4 other = theirs[(j + i) * 32];
+        set_rows(x[j + i], f2_fma(a, f2_add(first_row(x[j + i]), f2_pack(other.x, other.y)), first_row(v[i])),
+                 f2_fma(a, f2_add(second_row(x[j + i]), f2_pack(other.z, other.w)), second_row(v[i])));
       }
     }
-    // y's part of S: scaled back
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float2 b = *reinterpret_cast<const float2*>(factors + kChunk + j * 8 + 2 * t);
-      o[j][0] = b.x * (o[j][0] * i0);
-      o[j][1] = b.y * (o[j][1] * i0);
-      o[j][2] = b.x * (o[j][2] * i1);
-      o[j][3] = b.y * (o[j][3] * i1);
-    }
-    // U = (v - ..) T^T
-    float u[8][4] = {};
+    // U = (v - ..) T^T, by both warps
+    float u[8][4];
     {
       float r0, r1;
       row_scales<8>(x, r0, r1);
+      const F2 up0 = f2_both(r0), up1 = f2_both(r1);
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        uint32_t hi[4], lo[4];
-        operand(x[2 * k], x[2 * k + 1], r0, r1, hi, lo);
+        uint32_t hi[4], lo[4], b[4][4], bl[4][4];
+        operand(x[2 * k], x[2 * k + 1], up0, up1, hi, lo);
 #pragma unroll
         for (int j = k; j < 4; ++j) {   // (T is lower triangular)
           const uint32_t at = square + piece<kChunk>(j * 16 + (m >> 1) * 8 + r, 2 * k + (m & 1));
-          uint32_t b[4], bl[4];
-          ldmatrix(b, at);
-          ldmatrix(bl, at + kSquare);
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            mma(u[2 * j + i], hi, b[2 * i], b[2 * i + 1]);
-            mma(u[2 * j + i], hi, bl[2 * i], bl[2 * i + 1]);
-            mma(u[2 * j + i], lo, b[2 * i], b[2 * i + 1]);
-          }
+          ldmatrix(b[j], at);
+          ldmatrix(bl[j], at + kSquare);
         }
+#pragma unroll
+        for (int j = 2 * k; j < 8; ++j) {
+          if (k == 0) mma_first(u[j], hi, b[j >> 1][2 * (j & 1)], b[j >> 1][2 * (j & 1) + 1]);
+          else mma(u[j], hi, b[j >> 1][2 * (j & 1)], b[j >> 1][2 * (j & 1) + 1]);
+        }
+#pragma unroll
+        for (int j = 2 * k; j < 8; ++j) mma(u[j], lo, b[j >> 1][2 * (j & 1)], b[j >> 1][2 * (j & 1) + 1]);
+#pragma unroll
+        for (int j = 2 * k; j < 8; ++j) mma(u[j], hi, bl[j >> 1][2 * (j & 1)], bl[j >> 1][2 * (j & 1) + 1]);
       }
-      r0 = inverse_of_power(r0);
-      r1 = inverse_of_power(r1);
+      const F2 down0 = f2_both(inverse_of_power(r0)), down1 = f2_both(inverse_of_power(r1));
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const float2 f = *reinterpret_cast<const float2*>(factors + 3 * kChunk + j * 8 + 2 * t);
-        u[j][0] = f.x * (u[j][0] * r0);
-        u[j][1] = f.y * (u[j][1] * r0);
-        u[j][2] = f.x * (u[j][2] * r1);
-        u[j][3] = f.y * (u[j][3] * r1);
+        const F2 f = pair_at(factors + 3 * kChunk + j * 8);
+        set_rows(u[j], f2_mul(f, f2_mul(first_row(u[j]), down0)), f2_mul(f, f2_mul(second_row(u[j]), down1)));
       }
     }
-    // y = .. + U P^T
-    {
-      float u0, u1, z[8][4] = {};
+    {   // y = e^G S q + U P^T
+      float u0, u1, z[2][2][4] = {};
       row_scales<8>(u, u0, u1);
+      const F2 up0 = f2_both(u0), up1 = f2_both(u1);
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         uint32_t hi[4], lo[4];
-        if constexpr (Parts<T>::kOut == 2) operand(u[2 * k], u[2 * k + 1], u0, u1, hi, lo);
-        else operand(u[2 * k], u[2 * k + 1], u0, u1, hi);
+        if constexpr (Parts<T>::kOut == 2) operand(u[2 * k], u[2 * k + 1], up0, up1, hi, lo);
+        else operand(u[2 * k], u[2 * k + 1], up0, up1, hi);
 #pragma unroll
-        for (int j = k; j < 4; ++j) {
-          const uint32_t at = square + 2 * kSquare + piece<kChunk>(j * 16 + (m >> 1) * 8 + r, 2 * k + (m & 1));
-          uint32_t b[4];
-          ldmatrix(b, at);
+        for (int i = 0; i < 2; ++i)
+          if (k <= own[i]) {
+            const uint32_t at = square + 2 * kSquare + piece<kChunk>(own[i] * 16 + (m >> 1) * 8 + r, 2 * k + (m & 1));
+            uint32_t b[4];
+            ldmatrix(b, at);
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            mma(z[2 * j + i], hi, b[2 * i], b[2 * i + 1]);
-            if constexpr (Parts<T>::kOut == 2) mma(z[2 * j + i], lo, b[2 * i], b[2 * i + 1]);
+            for (int j = 0; j < 2; ++j) {
+              mma(z[i][j], hi, b[2 * j], b[2 * j + 1]);
+              if constexpr (Parts<T>::kOut == 2) mma(z[i][j], lo, b[2 * j], b[2 * j + 1]);
+            }
+            if constexpr (Parts<T>::kOut == 2) {
+              ldmatrix(b, at + kSquare);
+#pragma unroll
+              for (int j = 0; j < 2; ++j) mma(z[i][j], hi, b[2 * j], b[2 * j + 1]);
+            }
           }
-          if constexpr (Parts<T>::kOut == 2) {
-            ldmatrix(b, at + kSquare);
-#pragma unroll
-            for (int i = 0; i < 2; ++i) mma(z[2 * j + i], hi, b[2 * i], b[2 * i + 1]);
-          }
-        }
       }
-      u0 = inverse_of_power(u0);
-      u1 = inverse_of_power(u1);
+      const F2 down0 = f2_both(inverse_of_power(u0)), down1 = f2_both(inverse_of_power(u1));
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float2 f = *reinterpret_cast<const float2*>(factors + 4 * kChunk + j * 8 + 2 * t);
-        o[j][0] += f.x * (z[j][0] * u0);
-        o[j][1] += f.y * (z[j][1] * u0);
-        o[j][2] += f.x * (z[j][2] * u1);
-        o[j][3] += f.y * (z[j][3] * u1);
+      for (int i = 0; i < 2; ++i) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int tile = own[i] * 2 + j;
+          const F2 b = pair_at(factors + kChunk + tile * 8), f = pair_at(factors + 4 * kChunk + tile * 8);
+          const float4 o = mine[(8 + tile) * 32], other = theirs[(8 + tile) * 32];
+          const F2 q0 = f2_mul(b, f2_add(f2_pack(o.x, o.y), f2_pack(other.x, other.y)));
+          const F2 q1 = f2_mul(b, f2_add(f2_pack(o.z, o.w), f2_pack(other.z, other.w)));
+          set_rows(z[i][j], f2_fma(f, f2_mul(first_row(z[i][j]), down0), q0), f2_fma(f, f2_mul(second_row(z[i][j]), down1), q1));
+        }
+        const int token = c * kChunk + own[i] * 16;
+        put_outputs<T, WHOLE>(p, y + token * p.y_s[1], z[i], end - token, channels);
       }
     }
-    put_outputs<T, WHOLE>(p, y + (long long)c * kChunk * p.y_s[1], o, end - c * kChunk, channels);
-    // S = e^(G_64) S + (e^(G_64 - G) U) k
+    // S = e^(G_64) S + (e^(G_64 - G) U) k, of this warp's channels
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const float2 f = *reinterpret_cast<const float2*>(factors + 2 * kChunk + j * 8 + 2 * t);
-      u[j][0] *= f.x;
-      u[j][1] *= f.y;
-      u[j][2] *= f.x;
-      u[j][3] *= f.y;
+      const F2 f = pair_at(factors + 2 * kChunk + j * 8);
+      set_rows(u[j], f2_mul(first_row(u[j]), f), f2_mul(second_row(u[j]), f));
     }
     {
-      const float keep = factors[5 * kChunk];
-      float u0, u1;
+      const F2 keep = f2_both(factors[5 * kChunk - 2 * t]);
+      float u0, u1, z[kHalf / 8][4];
       row_scales<8>(u, u0, u1);
-      uint32_t hi[4][4], lo[4][4];
+      const F2 up0 = f2_both(u0), up1 = f2_both(u1);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) operand(u[2 * k], u[2 * k + 1], u0, u1, hi[k], lo[k]);
-      u0 = inverse_of_power(u0);
-      u1 = inverse_of_power(u1);
+      for (int k = 0; k < 4; ++k) {
+        uint32_t hi[4], lo[4], b[kHalf / 16][4];
+        operand(u[2 * k], u[2 * k + 1], up0, up1, hi, lo);
 #pragma unroll
-      for (int j0 = 0; j0 < KEYS / 16; j0 += 4) {
-        float z[8][4] = {};
+        for (int j = 0; j < kHalf / 16; ++j)
+          ldmatrix_t(b[j], keys + piece<KEYS>(k * 16 + (m & 1) * 8 + r, half * (kHalf / 8) + 2 * j + (m >> 1)));
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
+        for (int j = 0; j < kHalf / 8; ++j) {
+          if (k == 0) mma_first(z[j], hi, b[j >> 1][2 * (j & 1)], b[j >> 1][2 * (j & 1) + 1]);
+          else mma(z[j], hi, b[j >> 1][2 * (j & 1)], b[j >> 1][2 * (j & 1) + 1]);
+        }
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int at = piece<KEYS>(k * 16 + (m & 1) * 8 + r, 2 * (j0 + j) + (m >> 1));
-            uint32_t b[4];
-            ldmatrix_t(b, keys + at);
+        for (int j = 0; j < kHalf / 8; ++j) mma(z[j], lo, b[j >> 1][2 * (j & 1)], b[j >> 1][2 * (j & 1) + 1]);
+        if constexpr (Parts<T>::kKey == 2) {
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              mma(z[2 * j + i], hi[k], b[2 * i], b[2 * i + 1]);
-              mma(z[2 * j + i], lo[k], b[2 * i], b[2 * i + 1]);
-            }
-            if constexpr (Parts<T>::kKey == 2) {
-              ldmatrix_t(b, keys + kKeyPart + at);
+          for (int j = 0; j < kHalf / 16; ++j)
+            ldmatrix_t(b[j], keys + kKeyPart + piece<KEYS>(k * 16 + (m & 1) * 8 + r, half * (kHalf / 8) + 2 * j + (m >> 1)));
 #pragma unroll
-              for (int i = 0; i < 2; ++i) mma(z[2 * j + i], hi[k], b[2 * i], b[2 * i + 1]);
-            }
-          }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          s[2 * j0 + j][0] = keep * s[2 * j0 + j][0] + z[j][0] * u0;
-          s[2 * j0 + j][1] = keep * s[2 * j0 + j][1] + z[j][1] * u0;
-          s[2 * j0 + j][2] = keep * s[2 * j0 + j][2] + z[j][2] * u1;
-          s[2 * j0 + j][3] = keep * s[2 * j0 + j][3] + z[j][3] * u1;
+          for (int j = 0; j < kHalf / 8; ++j) mma(z[j], hi, b[j >> 1][2 * (j & 1)], b[j >> 1][2 * (j & 1) + 1]);
         }
       }
+      const F2 down0 = f2_both(inverse_of_power(u0)), down1 = f2_both(inverse_of_power(u1));
+#pragma unroll
+      for (int j = 0; j < kHalf / 8; ++j)
+        set_rows(s[j], f2_fma(keep, first_row(s[j]), f2_mul(first_row(z[j]), down0)), f2_fma(keep, second_row(s[j]), f2_mul(second_row(z[j]), down1)));
     }
-    if (stages == 1) __syncthreads();
+    if (stages == 1) {
+      __syncthreads();
+      if (c + 1 < chunks) ask(c + 1);
+    }
   }
 
   if (p.final_state != nullptr) {
 #pragma unroll
-    for (int j = 0; j < KEYS / 8; ++j)
+    for (int j = 0; j < kHalf / 8; ++j)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int row = g + (i >> 1) * 8, at = j * 8 + 2 * t + (i & 1);
+        const int row = g + (i >> 1) * 8, at = half * kHalf + j * 8 + 2 * t + (i & 1);
         if (row < channels && at < p.K) p.final_state[state_at + (long long)row * p.K + at] = s[j][i];
       }
   }
   // tokens behind the row's end
-  for (long long i = end * 16ll + lane; i < p.L * 16ll; i += 32)
+  for (long long i = end * 16ll + half * 32 + lane; i < p.L * 16ll; i += 64)
     if (i % 16 < channels) y[i / 16 * p.y_s[1] + i % 16 * p.y_s[3]] = from_f32<T>(0.0f);
 }
 
@@ -822,20 +846,26 @@ cudaError_t run(const DeltaParams& p, cudaStream_t stream) {
   if (e != cudaSuccess) return e;
 
   const int most = (p.V + 15) / 16;
-  int warps = most < 4 ? most : 4;
-  while (warps > 1 && (long long)p.N * p.H * ((most + warps - 1) / warps) < current_sm_count()) warps = (warps + 1) / 2;
-  const int slices = (most + warps - 1) / warps;
-  const long long blocks = (long long)p.N * p.H * slices;
-  if (blocks > 0x7fffffffll) return cudaErrorInvalidConfiguration;
-  const int stage = Work<T, KEYS>::kStage + kChunk * value_pitch<T>(warps);
+  auto blocks_of = [&](int slices) { return (long long)p.N * p.H * ((most + slices - 1) / slices); };
+  auto smem_of = [&](int slices, int stages) {
+    return stages * (Work<T, KEYS>::kStage + kChunk * value_pitch<T>(slices)) + slices * kExchange;
+  };
   constexpr int kMostSmem = 227 * 1024;
-  const int stages = 2 * stage <= kMostSmem ? 2 : 1;
+  // Four slices to a block put two warps on a quarter of an SM: a chunk takes longer, but twice the rows
+  int slices = most < 2 ? most : 2;
+  if (most > 2 && 5 * ((blocks_of(4) + current_sm_count() - 1) / current_sm_count()) < 3 * ((blocks_of(2) + current_sm_count() - 1) / current_sm_count()))
+    slices = most < 4 ? most : 4;
+  while (slices > 1 && smem_of(slices, 2) > kMostSmem) --slices;
+  const int stages = smem_of(slices, 2) <= kMostSmem ? 2 : 1;
+  const long long blocks = blocks_of(slices);
+  if (blocks > 0x7fffffffll) return cudaErrorInvalidConfiguration;
   const bool values_whole = eights<T>(p.v, p.v_s) && p.V % 2 == 0 && p.y_s[3] == 1 && p.y_s[0] % 2 == 0 && p.y_s[1] % 2 == 0 &&
                             p.y_s[2] % 2 == 0 && (reinterpret_cast<uintptr_t>(p.y) & 3u) == 0;
   auto* kernel = values_whole ? delta_chunks_kernel<T, KEYS, true> : delta_chunks_kernel<T, KEYS, false>;
   e = allow_smem(kernel, kMostSmem, done[2 + values_whole]);
   if (e != cudaSuccess) return e;
-  return launch_seq(kernel, dim3(unsigned(blocks)), (warps + kLoaders) * 32, stages * stage, 1, stream, p, slices, stages);
+  return launch_seq(kernel, dim3(unsigned(blocks)), 2 * slices * 32, smem_of(slices, stages), 1, stream, p,
+                    (most + slices - 1) / slices, stages);
 }
 
 // f(TypeOf<T>, integral_constant<int, KEYS>)
