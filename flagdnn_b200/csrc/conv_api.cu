@@ -1202,6 +1202,17 @@ uint32_t* device_status_word() {
   return static_cast<uint32_t*>(p);
 }
 
+void bounded_wait_of(uint32_t** status, long long* limit) {
+  static std::atomic<uint32_t*> words[64];
+  const long long set = g_wait_limit.load(std::memory_order_relaxed);
+  *limit = set > 0 ? set : default_wait_limit_cycles();
+  *status = nullptr;
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return;
+  *status = words[dev].load(std::memory_order_acquire);
+  if (*status == nullptr) words[dev].store(*status = device_status_word(), std::memory_order_release);
+}
+
 }  // namespace fdnn
 
 namespace fdnn {

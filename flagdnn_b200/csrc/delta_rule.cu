@@ -26,7 +26,7 @@ namespace {
 constexpr int kChunk = 64;
 constexpr int kChunkKeys = 128;      // the widest key that the chunks' kernels take
 constexpr int kFactors = 6 * kChunk; // floats a chunk and head: -a, b, d, t, p, and e^(G_64)
-constexpr int kSquare = kChunk * kChunk * 2;   // bytes of a 64 x 64 part
+constexpr int kLower = 10 * 512;     // bytes of a part of T or P
 
 // How many 16-bit parts: of keys and queries, of S and P in what only y sees.
 template <typename T>
@@ -86,10 +86,6 @@ __device__ __forceinline__ uint32_t high(float x, float y) {
   const __half2 h = __floats2half2_rn(x, y);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
-__device__ __forceinline__ uint32_t low(float x, float y, uint32_t hi) {
-  const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&hi));
-  return high(x - h.x, y - h.y);
-}
 __device__ __forceinline__ float quad_max(float v) {
   v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
   return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
@@ -138,17 +134,22 @@ __device__ __forceinline__ void operand(const float (&x)[4], const float (&y)[4]
   hi[3] = high(f2_mul(second_row(y), s1));
 }
 
-// Tiles of 16-bit operands: rows of COLS values, whose 16-byte pieces lie at piece ^ (row % 8), so that eight rows of a piece
-// (one matrix of ldmatrix) are in different banks.  Byte offset of a piece.
-template <int COLS>
-__device__ __forceinline__ int piece(int row, int at) { return row * COLS * 2 + ((at ^ (row & 7)) << 4); }
+// 16-bit operands lie in blocks of 16 x 16 values, a block as its four 8 x 8 matrices (upper left, upper right, lower left, lower
+// right) of eight 16-byte rows: what one ldmatrix reads is 512 bytes in a run, in no bank twice.  Byte offset of 16 bytes of a tile whose
+// rows have `blocks` blocks: `at` counts 8 columns.
+constexpr int kBlock = 512;
+__host__ __device__ constexpr int piece(int row, int at, int blocks) {
+  return ((row >> 4) * blocks + (at >> 1)) * kBlock + (((row >> 3) & 1) * 2 + (at & 1)) * 128 + (row & 7) * 16;
+}
+// Of a lower triangular 64 x 64 tile only the blocks (i, j <= i) are there.
+__host__ __device__ constexpr int lower_block(int i, int j) { return i * (i + 1) / 2 + j; }
 
 // ---- where things lie in the workspace -----------------------------------------------------------------------------
 
 template <typename T, int KEYS>
 struct Work {
   static constexpr int kKeyBytes = Parts<T>::kKey * kChunk * KEYS * 2;   // keys, and as many for the queries
-  static constexpr int kHeadBytes = (2 + Parts<T>::kOut) * kSquare + kFactors * 4;
+  static constexpr int kHeadBytes = (2 + Parts<T>::kOut) * kLower + kFactors * 4;
   static constexpr int kStage = 2 * kKeyBytes + kHeadBytes;
 };
 struct Layout {
@@ -177,82 +178,100 @@ __device__ __forceinline__ int row_end(const DeltaParams& p, long long n) {
 constexpr int kPrepThreads = 128;
 constexpr int kPitch = kChunk + 4;   // floats between rows of A, T
 
+struct HeadGates {
+  float hi[kChunk], lo[kChunk], beta[kChunk];   // sums of log2 decays in two parts
+};
 template <typename T, int KEYS>
 struct PrepShared {
-  uint8_t keys[2 * Work<T, KEYS>::kKeyBytes];   // and the queries
-  float a[kChunk][kPitch], t[kChunk][kPitch], part[4][16][20];
-  float key_scale[kChunk], query_scale[kChunk], sum_hi[kChunk], sum_lo[kChunk], beta[kChunk];
-  float end_hi, end_lo;
+  union {
+    uint8_t keys[2 * Work<T, KEYS>::kKeyBytes];   // and the queries
+    struct {
+      float a[kChunk][kPitch], t[kChunk][kPitch], part[4][16][20];
+    } solve;
+  };
+  float key_scale[kChunk], query_scale[kChunk];
+  HeadGates gates[4];
 };
 
-// A token's key or query: eight neighbouring channels of a row to their place, as parts, scaled; the factor that takes the operand
-// back (with the norm, if asked, and `scale`).
+// Keys or queries of a chunk to their places, as parts, scaled; the factors that take the operands back (with the norm, if asked, and
+// `scale`).  A warp takes 8 rows at once, four lanes a row, so that what they write is 128 bytes in a run.
 template <typename T, int KEYS, bool WHOLE>
 __device__ __forceinline__ void stage_rows(const DeltaParams& p, const T* x, const long long* s, int tokens, float scale, uint8_t* to,
                                            float* factor) {
-  constexpr int kLanes = KEYS / 8, kRows = kPrepThreads / kLanes;
-  const int at = threadIdx.x % kLanes;
+  constexpr int kPieces = KEYS / 32;   // of eight channels, to a lane
+  const int lane = threadIdx.x & 31, part = lane >> 3;
 #pragma unroll
-  for (int r0 = 0; r0 < kChunk; r0 += kRows) {
-    const int r = r0 + threadIdx.x / kLanes;
-    float v[8];
-    if constexpr (WHOLE) {
-      constexpr int kV = 16 / sizeof(T);
+  for (int pass = 0; pass < 2; ++pass) {
+    const int r = (pass * 4 + (threadIdx.x >> 5)) * 8 + (lane & 7);
+    float v[kPieces][8];
 #pragma unroll
-      for (int i = 0; i < 8 / kV; ++i) {
-        Pack<T, kV> q;
-        q.clear();
-        if (r < tokens && at * 8 + i * kV < p.K) q.load(x + r * s[1] + at * 8 + i * kV);
+    for (int n = 0; n < kPieces; ++n) {
+      const int at = (n * 4 + part) * 8;
+      if constexpr (WHOLE) {
+        constexpr int kV = 16 / sizeof(T);
 #pragma unroll
-        for (int j = 0; j < kV; ++j) v[i * kV + j] = q.at(j);
+        for (int i = 0; i < 8 / kV; ++i) {
+          Pack<T, kV> q;
+          q.clear();
+          if (r < tokens && at + i * kV < p.K) q.load(x + r * s[1] + at + i * kV);
+#pragma unroll
+          for (int j = 0; j < kV; ++j) v[n][i * kV + j] = q.at(j);
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[n][j] = r < tokens && at + j < p.K ? to_f32<T>(x[r * s[1] + (at + j) * s[3]]) : 0.0f;
       }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = r < tokens && at * 8 + j < p.K ? to_f32<T>(x[r * s[1] + (at * 8 + j) * s[3]]) : 0.0f;
     }
     float most = 0.0f, squares = 0.0f;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      most = fmaxf(most, fabsf(v[j]));
-      squares += v[j] * v[j];
-    }
+    for (int n = 0; n < kPieces; ++n)
 #pragma unroll
-    for (int o = kLanes / 2; o > 0; o >>= 1) {
+      for (int j = 0; j < 8; ++j) {
+        most = fmaxf(most, fabsf(v[n][j]));
+        squares += v[n][j] * v[n][j];
+      }
+#pragma unroll
+    for (int o = 8; o < 32; o <<= 1) {
       most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
       squares += __shfl_xor_sync(0xffffffffu, squares, o);
     }
     const float up = raise(most);
-    uint4 hi, lo;
-    uint32_t* h = reinterpret_cast<uint32_t*>(&hi);
-    uint32_t* l = reinterpret_cast<uint32_t*>(&lo);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      h[j] = high(v[2 * j] * up, v[2 * j + 1] * up);
-      l[j] = low(v[2 * j] * up, v[2 * j + 1] * up, h[j]);
+    for (int n = 0; n < kPieces; ++n) {
+      uint4 hi, lo;
+      uint32_t* h = reinterpret_cast<uint32_t*>(&hi);
+      uint32_t* l = reinterpret_cast<uint32_t*>(&lo);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const F2 x2 = f2_pack(v[n][2 * j] * up, v[n][2 * j + 1] * up);
+        h[j] = high(x2);
+        if constexpr (Parts<T>::kKey == 2) l[j] = low(x2, h[j]);
+      }
+      const int at = piece(r, n * 4 + part, KEYS / 16);
+      *reinterpret_cast<uint4*>(to + at) = hi;
+      if constexpr (Parts<T>::kKey == 2) *reinterpret_cast<uint4*>(to + kChunk * KEYS * 2 + at) = lo;
     }
-    *reinterpret_cast<uint4*>(to + piece<KEYS>(r, at)) = hi;
-    if constexpr (Parts<T>::kKey == 2) *reinterpret_cast<uint4*>(to + kChunk * KEYS * 2 + piece<KEYS>(r, at)) = lo;
-    if (at == 0) factor[r] = r < tokens ? scale * inverse_of_power(up) * (p.norm ? 1.0f / sqrtf(squares + kKeyEps) : 1.0f) : 0.0f;
+    if (part == 0) factor[r] = r < tokens ? scale * inverse_of_power(up) * (p.norm ? 1.0f / sqrtf(squares + kKeyEps) : 1.0f) : 0.0f;
   }
 }
 
-// c += the products of 16 rows of `x` (from row0) with the first `tiles` x 8 rows of `y`, over KEYS channels.
+// c += the products of row block `i` of `x` with the row blocks up to it of `y`, over KEYS channels.
 template <typename T, int KEYS>
-__device__ __forceinline__ void dots(float (&c)[8][4], const uint8_t* x, const uint8_t* y, int row0, int pairs) {
+__device__ __forceinline__ void dots(float (&c)[8][4], const uint8_t* x, const uint8_t* y, int i) {
   const int lane = threadIdx.x & 31, m = lane >> 3, r = lane & 7;
-  const uint32_t xs = smem_u32(x), ys = smem_u32(y);
+  const uint32_t xs = smem_u32(x) + i * (KEYS / 16) * kBlock + ((m & 1) * 2 + (m >> 1)) * 128 + r * 16, ys = smem_u32(y) + lane * 16;
   constexpr int kPart = kChunk * KEYS * 2;
 #pragma unroll
   for (int s = 0; s < KEYS / 16; ++s) {
     uint32_t a[Parts<T>::kKey][4];
 #pragma unroll
-    for (int i = 0; i < Parts<T>::kKey; ++i) ldmatrix(a[i], xs + i * kPart + piece<KEYS>(row0 + (m & 1) * 8 + r, 2 * s + (m >> 1)));
+    for (int k = 0; k < Parts<T>::kKey; ++k) ldmatrix(a[k], xs + k * kPart + s * kBlock);
 #pragma unroll
     for (int n = 0; n < 4; ++n)
-      if (n < pairs) {
+      if (n <= i) {
         uint32_t b[Parts<T>::kKey][4];
 #pragma unroll
-        for (int i = 0; i < Parts<T>::kKey; ++i) ldmatrix(b[i], ys + i * kPart + piece<KEYS>(n * 16 + (m >> 1) * 8 + r, 2 * s + (m & 1)));
+        for (int k = 0; k < Parts<T>::kKey; ++k) ldmatrix(b[k], ys + k * kPart + (n * (KEYS / 16) + s) * kBlock);
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           mma(c[2 * n + j], a[0], b[0][2 * j], b[0][2 * j + 1]);
@@ -264,6 +283,41 @@ __device__ __forceinline__ void dots(float (&c)[8][4], const uint8_t* x, const u
       }
   }
 }
+
+// Sums of a head's log2 decays and its step sizes, by one warp, two tokens a lane.
+template <typename T>
+__device__ __forceinline__ void sum_gates(const DeltaParams& p, HeadGates& to, long long n, int begin, int tokens, int h) {
+  const int lane = threadIdx.x & 31;
+  const float A = p.A != nullptr ? p.A[h] : 1.0f, bias = p.delta_bias != nullptr ? p.delta_bias[h] : 0.0f;
+  double v[2];
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int i = 2 * lane + j;
+    float g = 0.0f, b = 0.0f;
+    if (i < tokens) {
+      g = log_decay(p, gate_at<T>(p, p.delta, n * p.delta_s[0] + (begin + i) * p.delta_s[1] + h * p.delta_s[2]), bias, A);
+      b = step_size(p, gate_at<T>(p, p.beta, n * p.beta_s[0] + (begin + i) * p.beta_s[1] + h * p.beta_s[2]));
+      g = g < -1e5f ? -1e5f : g;   // a decay of zero, whose difference to itself is a number; NaN stays
+    }
+    v[j] = double(g) * 1.4426950408889634;
+    to.beta[i] = b;
+  }
+  double sum = v[0] + v[1];
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const double other = __shfl_up_sync(0xffffffffu, sum, o);
+    if (lane >= o) sum += other;
+  }
+  const double each[2] = {sum - v[1], sum};
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const float hi = float(each[j]);
+    to.hi[2 * lane + j] = hi;
+    to.lo[2 * lane + j] = float(each[j] - double(hi));
+  }
+}
+// 2^(hi + lo) to fp32's last place but two: what a state keeps over many chunks has no drift.
+__device__ __forceinline__ float exp2_of(float hi, float lo) { return exp2f(hi) * fmaf(lo, 0.6931471805599453f, 1.0f); }
 
 // d += x y of 16 x 16 blocks in fp32, by 3 x TF32 (a high part is the number cut to TF32, what it leaves is exact; 2^-21).
 __device__ __forceinline__ void block_product(float (&d)[2][4], const float* x, int x_pitch, const float* y, int y_pitch) {
@@ -345,7 +399,7 @@ __device__ __forceinline__ void invert(const float (&a)[kChunk][kPitch], float (
 }
 
 template <typename T, int KEYS, bool WHOLE>
-__global__ void __launch_bounds__(kPrepThreads)
+__global__ void __launch_bounds__(kPrepThreads, 4)
 delta_prepare_kernel(const DeltaParams p) {
   extern __shared__ __align__(128) uint8_t smem_raw[];
   PrepShared<T, KEYS>& s = *reinterpret_cast<PrepShared<T, KEYS>*>(smem_raw);
@@ -358,6 +412,8 @@ delta_prepare_kernel(const DeltaParams p) {
   if (tokens <= 0) return;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, q = lane >> 2, t = lane & 3;
   uint8_t* const queries = s.keys + W::kKeyBytes;
+  const int group = p.H / p.G, h0 = g * group;
+  if (warp < group) sum_gates<T>(p, s.gates[warp], n, begin, tokens, h0 + warp);
   stage_rows<T, KEYS, WHOLE>(p, static_cast<const T*>(p.k) + n * p.k_s[0] + begin * p.k_s[1] + g * p.k_s[2], p.k_s, tokens, 1.0f, s.keys,
                              s.key_scale);
   stage_rows<T, KEYS, WHOLE>(p, static_cast<const T*>(p.q) + n * p.q_s[0] + begin * p.q_s[1] + g * p.q_s[2], p.q_s, tokens, p.scale, queries,
@@ -370,114 +426,106 @@ delta_prepare_kernel(const DeltaParams p) {
     for (int i = tid; i < 2 * W::kKeyBytes / 16; i += kPrepThreads) to[i] = from[i];
   }
   float kk[8][4] = {}, qk[8][4] = {};
-  dots<T, KEYS>(kk, s.keys, s.keys, warp * 16, warp + 1);
-  dots<T, KEYS>(qk, queries, s.keys, warp * 16, warp + 1);
-
-  const int group = p.H / p.G;
-  for (int h = g * group; h < (g + 1) * group; ++h) {
-    if (warp == 0) {   // two tokens a lane
-      const float A = p.A != nullptr ? p.A[h] : 1.0f, bias = p.delta_bias != nullptr ? p.delta_bias[h] : 0.0f;
-      double v[2];
+  dots<T, KEYS>(kk, s.keys, s.keys, warp);
+  dots<T, KEYS>(qk, queries, s.keys, warp);
+  const int r0 = warp * 16 + q;
+  {   // the factors of the rows and columns
+    const float k0 = s.key_scale[r0], k1 = s.key_scale[r0 + 8], q0 = s.query_scale[r0], q1 = s.query_scale[r0 + 8];
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int i = 2 * lane + j;
-        float gl = 0.0f, b = 0.0f;
-        if (i < tokens) {
-          gl = log_decay(p, gate_at<T>(p, p.delta, n * p.delta_s[0] + (begin + i) * p.delta_s[1] + h * p.delta_s[2]), bias, A);
-          b = step_size(p, gate_at<T>(p, p.beta, n * p.beta_s[0] + (begin + i) * p.beta_s[1] + h * p.beta_s[2]));
-          gl = gl < -1e5f ? -1e5f : gl;   // a decay of zero, whose difference to itself is a number; NaN stays
-        }
-        v[j] = double(gl);
-        s.beta[i] = b;
-      }
-      double sum = v[0] + v[1];
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const double other = __shfl_up_sync(0xffffffffu, sum, o);
-        if (lane >= o) sum += other;
-      }
-      const double each[2] = {sum - v[1], sum};
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const float hi = float(each[j]);
-        s.sum_hi[2 * lane + j] = hi;
-        s.sum_lo[2 * lane + j] = float(each[j] - double(hi));
-      }
+    for (int m = 0; m < 8; ++m) {
+      const float2 f = *reinterpret_cast<const float2*>(&s.key_scale[m * 8 + 2 * t]);
+      kk[m][0] *= k0 * f.x, kk[m][1] *= k0 * f.y, kk[m][2] *= k1 * f.x, kk[m][3] *= k1 * f.y;
+      qk[m][0] *= q0 * f.x, qk[m][1] *= q0 * f.y, qk[m][2] *= q1 * f.x, qk[m][3] *= q1 * f.y;
     }
-    __syncthreads();
-    uint8_t* out = w.heads + ((n * p.H + h) * w.chunks + c) * (long long)W::kHeadBytes;
-    float* factors = reinterpret_cast<float*>(out + (2 + Parts<T>::kOut) * kSquare);
+  }
+  __syncthreads();   // the operands' place is taken by a and t
+
+  for (int i = 0; i < group; ++i) {
+    if (i > 0 && (i & 3) == 0) {
+      if (i + warp < group) sum_gates<T>(p, s.gates[warp], n, begin, tokens, h0 + i + warp);
+      __syncthreads();
+    }
+    const HeadGates& gates = s.gates[i & 3];
+    uint8_t* out = w.heads + ((n * p.H + h0 + i) * w.chunks + c) * (long long)W::kHeadBytes;
+    float* factors = reinterpret_cast<float*>(out + (2 + Parts<T>::kOut) * kLower);
     if (tid < kChunk) {
-      const float hi = s.sum_hi[tid], lo = s.sum_lo[tid], since = expf(hi + lo);
+      const float hi = gates.hi[tid], lo = gates.lo[tid], since = exp2_of(hi, lo);
       factors[tid] = -since * s.key_scale[tid];
       factors[kChunk + tid] = since * s.query_scale[tid];
-      factors[2 * kChunk + tid] = expf((s.sum_hi[kChunk - 1] - hi) + (s.sum_lo[kChunk - 1] - lo)) * s.key_scale[tid];
+      factors[2 * kChunk + tid] = exp2_of(gates.hi[kChunk - 1] - hi, gates.lo[kChunk - 1] - lo) * s.key_scale[tid];
       if (tid == kChunk - 1) factors[5 * kChunk] = since;
     }
     // a and P, from this warp's 16 rows
-    const int r0 = warp * 16 + q;
-    float hi[2], lo[2], beta[2], most[2] = {0.0f, 0.0f};
+    {
+      float hi[2], lo[2], beta[2], most[2] = {0.0f, 0.0f}, pm[8][4];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      hi[i] = s.sum_hi[r0 + 8 * i];
-      lo[i] = s.sum_lo[r0 + 8 * i];
-      beta[i] = s.beta[r0 + 8 * i] * s.key_scale[r0 + 8 * i];
-    }
-    float pm[8][4];
-#pragma unroll
-    for (int m = 0; m < 8; ++m)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int row = r0 + (i >> 1) * 8, col = m * 8 + 2 * t + (i & 1);
-        float av = 0.0f, pv = 0.0f;
-        if (m < 2 * (warp + 1) && col <= row) {
-          const float d = expf((hi[i >> 1] - s.sum_hi[col]) + (lo[i >> 1] - s.sum_lo[col])) * s.key_scale[col];
-          if (col < row) av = kk[m][i] * beta[i >> 1] * d;
-          pv = qk[m][i] * s.query_scale[row] * d;
-        }
-        s.a[row][col] = av;
-        pm[m][i] = pv;
-        most[i >> 1] = fmaxf(most[i >> 1], fabsf(pv));
+      for (int j = 0; j < 2; ++j) {
+        hi[j] = gates.hi[r0 + 8 * j];
+        lo[j] = gates.lo[r0 + 8 * j];
+        beta[j] = gates.beta[r0 + 8 * j];
       }
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const float up = raise(quad_max(most[i]));
-      if (t == 0) factors[4 * kChunk + r0 + 8 * i] = inverse_of_power(up);
+      for (int m = 0; m < 8; ++m)
+        if (m < 2 * (warp + 1)) {
+          const int col = m * 8 + 2 * t;
+          const float2 chi = *reinterpret_cast<const float2*>(&gates.hi[col]), clo = *reinterpret_cast<const float2*>(&gates.lo[col]);
+          float av[4];
 #pragma unroll
-      for (int m = 0; m < 8; ++m) {
-        const float x = pm[m][2 * i] * up, y = pm[m][2 * i + 1] * up;
-        const uint32_t h16 = high(x, y);
-        uint8_t* at = out + 2 * kSquare + piece<kChunk>(r0 + 8 * i, m) + t * 4;
-        *reinterpret_cast<uint32_t*>(at) = h16;
-        if constexpr (Parts<T>::kOut == 2) *reinterpret_cast<uint32_t*>(at + kSquare) = low(x, y, h16);
+          for (int j = 0; j < 4; ++j) {
+            const int row = r0 + (j >> 1) * 8, at = col + (j & 1);
+            const float d = ex2((hi[j >> 1] - ((j & 1) ? chi.y : chi.x)) + (lo[j >> 1] - ((j & 1) ? clo.y : clo.x)));
+            av[j] = at < row ? kk[m][j] * (beta[j >> 1] * d) : 0.0f;
+            pm[m][j] = at <= row ? qk[m][j] * d : 0.0f;
+            most[j >> 1] = fmaxf(most[j >> 1], fabsf(pm[m][j]));
+          }
+          *reinterpret_cast<float2*>(&s.solve.a[r0][col]) = make_float2(av[0], av[1]);
+          *reinterpret_cast<float2*>(&s.solve.a[r0 + 8][col]) = make_float2(av[2], av[3]);
+        }
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const float up = raise(quad_max(most[j]));
+        if (t == 0) factors[4 * kChunk + r0 + 8 * j] = inverse_of_power(up);
+#pragma unroll
+        for (int m = 0; m < 8; ++m)
+          if (m < 2 * (warp + 1)) {
+            const F2 x = f2_mul(f2_pack(pm[m][2 * j], pm[m][2 * j + 1]), f2_both(up));
+            const uint32_t h16 = high(x);
+            uint8_t* at = out + 2 * kLower + lower_block(warp, m >> 1) * kBlock + (j * 2 + (m & 1)) * 128 + lane * 4;
+            *reinterpret_cast<uint32_t*>(at) = h16;
+            if constexpr (Parts<T>::kOut == 2) *reinterpret_cast<uint32_t*>(at + kLower) = low(x, h16);
+          }
       }
     }
     __syncthreads();
-    invert(s.a, s.t, s.part);
-    {   // T = t diag(beta), two threads a row
-      const int row = tid >> 1, from = (tid & 1) * 32;
-      float v[32], top = 0.0f;
+    invert(s.solve.a, s.solve.t, s.solve.part);
+    {   // T = t diag(beta), this warp's 16 rows
+      float v[8][4], most[2] = {0.0f, 0.0f};
 #pragma unroll
-      for (int j = 0; j < 32; ++j) {
-        v[j] = from + j <= row ? s.t[row][from + j] * s.beta[from + j] : 0.0f;
-        top = fmaxf(top, fabsf(v[j]));
-      }
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      const float up = raise(top);
-      if (from == 0) factors[3 * kChunk + row] = inverse_of_power(up);
+      for (int m = 0; m < 8; ++m)
+        if (m < 2 * (warp + 1)) {
+          const int col = m * 8 + 2 * t;
+          const float2 beta = *reinterpret_cast<const float2*>(&gates.beta[col]);
 #pragma unroll
-      for (int m = 0; m < 4; ++m) {
-        uint4 h4, l4;
-        uint32_t *hp = reinterpret_cast<uint32_t*>(&h4), *lp = reinterpret_cast<uint32_t*>(&l4);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float x = v[m * 8 + 2 * j] * up, y = v[m * 8 + 2 * j + 1] * up;
-          hp[j] = high(x, y);
-          lp[j] = low(x, y, hp[j]);
+          for (int j = 0; j < 2; ++j) {
+            const float2 x = *reinterpret_cast<const float2*>(&s.solve.t[r0 + 8 * j][col]);
+            v[m][2 * j] = x.x * beta.x;
+            v[m][2 * j + 1] = x.y * beta.y;
+            most[j] = fmaxf(most[j], fmaxf(fabsf(v[m][2 * j]), fabsf(v[m][2 * j + 1])));
+          }
         }
-        uint8_t* at = out + piece<kChunk>(row, from / 8 + m);
-        *reinterpret_cast<uint4*>(at) = h4;
-        *reinterpret_cast<uint4*>(at + kSquare) = l4;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const float up = raise(quad_max(most[j]));
+        if (t == 0) factors[3 * kChunk + r0 + 8 * j] = inverse_of_power(up);
+#pragma unroll
+        for (int m = 0; m < 8; ++m)
+          if (m < 2 * (warp + 1)) {
+            const F2 x = f2_mul(f2_pack(v[m][2 * j], v[m][2 * j + 1]), f2_both(up));
+            const uint32_t h16 = high(x);
+            uint8_t* at = out + lower_block(warp, m >> 1) * kBlock + (j * 2 + (m & 1)) * 128 + lane * 4;
+            *reinterpret_cast<uint32_t*>(at) = h16;
+            *reinterpret_cast<uint32_t*>(at + kLower) = low(x, h16);
+          }
       }
     }
     __syncthreads();
@@ -486,16 +534,25 @@ delta_prepare_kernel(const DeltaParams p) {
 
 // ---- the chunks in order -------------------------------------------------------------------------------------------
 
-constexpr int kMostSlices = 4;           // 16 rows of the state each, two warps to a slice
-constexpr int kExchange = 2 * 16 * 512;  // bytes through which two warps add up their halves
+constexpr int kMostSlices = 4;   // of 16 rows of the state; three warps each: two that carry it on, one that makes y
+// What the warps of a slice leave for each other: S k of either half (8 tiles of 512 bytes each), S as operands (each half's, the high parts,
+// then the low ones), U (8 tiles in fp32), the scales of the operands.
+template <typename T, int KEYS>
+struct Exchange {
+  static constexpr int kState = 2 * 8 * 512, kStatePart = KEYS / 32 * 512, kStateHalf = Parts<T>::kOut * kStatePart;
+  static constexpr int kWritten = kState + 2 * kStateHalf, kScales = kWritten + 8 * 512, kBytes = kScales + 2 * 32 * 8;
+};
 
 template <typename T>
 __host__ __device__ constexpr int value_pitch(int slices) { return 16 * slices * int(sizeof(T)) + 16; }   // bytes; eight rows in different banks
 
-__device__ __forceinline__ void pair_barrier(int id) { asm volatile("bar.sync %0, 64;" ::"r"(id) : "memory"); }
+template <int THREADS>
+__device__ __forceinline__ void barrier(int id) { asm volatile("bar.sync %0, %1;" ::"r"(id), "n"(THREADS) : "memory"); }
+template <int THREADS>
+__device__ __forceinline__ void barrier_arrive(int id) { asm volatile("bar.arrive %0, %1;" ::"r"(id), "n"(THREADS) : "memory"); }
 __device__ __forceinline__ F2 pair_at(const float* p) { return *reinterpret_cast<const F2*>(p); }
 
-// Two output tiles: o[i][..] holds rows (value channels) lane / 4, + 8 and tokens 8 i + 2 (lane % 4), + 1.
+// An output block: o[i][..] holds rows (value channels) lane / 4, + 8 and tokens 8 i + 2 (lane % 4), + 1; `y` is at its first token.
 template <typename T, bool WHOLE>
 __device__ __forceinline__ void put_outputs(const DeltaParams& p, T* y, const float (&o)[2][4], int tokens, int channels) {
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -529,66 +586,194 @@ __device__ __forceinline__ void put_outputs(const DeltaParams& p, T* y, const fl
   }
 }
 
+// d (+)= a b for the column tiles from FROM on, whose operands are b[tile / 2][2 (tile % 2)] and the next.
+template <int TILES, int FROM = 0, int PAIRS>
+__device__ __forceinline__ void mma_row(float (&d)[TILES][4], const uint32_t (&a)[4], const uint32_t (&b)[PAIRS][4], bool first = false) {
+#pragma unroll
+  for (int j = FROM; j < TILES; ++j) {
+    if (first) mma_first(d[j], a, b[j >> 1][2 * (j & 1)], b[j >> 1][2 * (j & 1) + 1]);
+    else mma(d[j], a, b[j >> 1][2 * (j & 1)], b[j >> 1][2 * (j & 1) + 1]);
+  }
+}
+
 // WHOLE: 16 bytes of neighbouring value channels are copied at once, and pairs stored.
 template <typename T, int KEYS, bool WHOLE>
-__global__ void __launch_bounds__(2 * kMostSlices * 32, 1)
-delta_chunks_kernel(const DeltaParams p, int blocks_a_head, int stages) {
+__global__ void __launch_bounds__(3 * kMostSlices * 32, 1)
+delta_chunks_kernel(const DeltaParams p, int blocks_a_head, int stages, uint32_t* status, long long wait_limit) {
   extern __shared__ __align__(128) uint8_t smem_raw[];
-  chained();
+  __shared__ uint64_t full[2];
+  __shared__ uint32_t abort_word;
   using W = Work<T, KEYS>;
-  constexpr int kKeyPart = kChunk * KEYS * 2, kHalf = KEYS / 2;
+  using E = Exchange<T, KEYS>;
+  constexpr int kKeyPart = kChunk * KEYS * 2, kHalf = KEYS / 2, kSteps = KEYS / 16;
+  if (threadIdx.x == 0) {
+    mbar_init(&full[0], 1);
+    mbar_init(&full[1], 1);
+    abort_word = 0;
+    fence_barrier_init();
+  }
+  __syncthreads();
+  chained();
   const Layout w = layout_of<T, KEYS>(p);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, slices = blockDim.x >> 6;
+  const int lane = threadIdx.x & 31, slices = blockDim.x / 96;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
   const int h = int(blockIdx.x / blocks_a_head % p.H);
   const long long n = blockIdx.x / blocks_a_head / p.H;
   const int end = row_end(p, n), chunks = (end + kChunk - 1) / kChunk;
   const int first = int(blockIdx.x % blocks_a_head) * slices * 16;   // the block's first value channel
   const int pitch = value_pitch<T>(slices), stage_bytes = W::kStage + kChunk * pitch;
   const uint32_t smem = smem_u32(smem_raw);
+  const int g = lane >> 2, t = lane & 3, m = lane >> 3, r = lane & 7;
+  const bool outputs = warp >= 2 * slices;
+  const int slice = outputs ? warp - 2 * slices : warp >> 1, half = warp & 1;
+  const int row0 = first + slice * 16, channels = min(16, p.V - row0);
+  uint8_t* const exchange = smem_raw + stages * stage_bytes + slice * E::kBytes;
+  const int pair_id = 1 + slice, state_id = 1 + kMostSlices + slice, written_id = 1 + 2 * kMostSlices + slice;   // named barriers
+  // All threads, at the top of chunk c: it is there, and all are done with chunk c - 1.
+  auto arrive_at = [&](int c) {
+    __syncthreads();
+    mbar_wait_warp(&full[c % stages], uint32_t(c / stages) & 1u, &abort_word, status, kIncidentDeltaWait, wait_limit);
+  };
 
-  const uint8_t* keys_from = w.keys + (n * p.G + h / (p.H / p.G)) * w.chunks * (2ll * W::kKeyBytes);
-  const uint8_t* heads_from = w.heads + (n * p.H + h) * w.chunks * (long long)W::kHeadBytes;
-  const T* v0 = static_cast<const T*>(p.v) + n * p.v_s[0] + h * p.v_s[2] + first * p.v_s[3];
-  auto ask = [&](int c) {   // a chunk's operands, by all threads
-    const int tid = threadIdx.x, step = blockDim.x;
-    const uint32_t to = smem + (c % stages) * stage_bytes;
-    const uint8_t* from = keys_from + c * (2ll * W::kKeyBytes);
-#pragma unroll 8
-    for (int i = tid; i < 2 * W::kKeyBytes / 16; i += step) copy16(to + i * 16, from + i * 16, 16);
-    from = heads_from + c * (long long)W::kHeadBytes;
-#pragma unroll 8
-    for (int i = tid; i < W::kHeadBytes / 16; i += step) copy16(to + 2 * W::kKeyBytes + i * 16, from + i * 16, 16);
-    const int here = min(slices * 16, p.V - first), tokens = min(end - c * kChunk, kChunk);
-    const uint32_t values = to + W::kStage;
-    if constexpr (WHOLE) {
-      constexpr int kV = 16 / sizeof(T);
-      const int pieces = slices * 16 / kV;   // a thread keeps its column: 64 slices threads are a multiple of it
-      const int at = tid % pieces * kV, bytes = min(max(here - at, 0), kV) * int(sizeof(T));
-#pragma unroll 4
-      for (int r = tid / pieces; r < kChunk; r += step / pieces) {
-        const bool there = r < tokens && bytes > 0;
-        copy16(values + r * pitch + at * int(sizeof(T)), there ? v0 + (c * kChunk + r) * p.v_s[1] + at : v0, there ? bytes : 0);
+  if (outputs) {
+    // ---- y, and the copies: chunk c + 1 is asked for at chunk c, where there is room for two
+    const int tid = threadIdx.x - 2 * slices * 32, step = slices * 32;
+    const uint8_t* keys_from = w.keys + (n * p.G + h / (p.H / p.G)) * w.chunks * (2ll * W::kKeyBytes);
+    const uint8_t* heads_from = w.heads + (n * p.H + h) * w.chunks * (long long)W::kHeadBytes;
+    const T* v0 = static_cast<const T*>(p.v) + n * p.v_s[0] + h * p.v_s[2] + first * p.v_s[3];
+    auto ask = [&](int c) {
+      uint8_t* const to = smem_raw + (c % stages) * stage_bytes;
+      if (tid == 0) {
+        uint64_t* bar = &full[c % stages];
+        mbar_arrive_expect_tx(bar, W::kStage);
+        bulk_load_1d(to, keys_from + c * (2ll * W::kKeyBytes), 2 * W::kKeyBytes, bar);
+        bulk_load_1d(to + 2 * W::kKeyBytes, heads_from + c * (long long)W::kHeadBytes, W::kHeadBytes, bar);
       }
-    } else {
-      T* to_v = reinterpret_cast<T*>(smem_raw + (c % stages) * stage_bytes + W::kStage);
-      for (int i = tid; i < kChunk * slices * 16; i += step) {
-        const int r = i / (slices * 16), at = i % (slices * 16);
-        to_v[r * (pitch / int(sizeof(T))) + at] =
-            r < tokens && at < here ? v0[(c * kChunk + r) * p.v_s[1] + at * p.v_s[3]] : from_f32<T>(0.0f);
+      const int here = min(slices * 16, p.V - first), tokens = min(end - c * kChunk, kChunk);
+      if constexpr (WHOLE) {
+        constexpr int kV = 16 / sizeof(T);
+        const int pieces = slices * 16 / kV;   // a thread keeps its column: `step` is a multiple of it
+        const int at = tid % pieces * kV, bytes = min(max(here - at, 0), kV) * int(sizeof(T));
+        const uint32_t values = smem_u32(to + W::kStage) + at * int(sizeof(T));
+#pragma unroll 4
+        for (int i = tid / pieces; i < kChunk; i += step / pieces) {
+          const bool there = i < tokens && bytes > 0;
+          copy16(values + i * pitch, there ? v0 + ((long long)c * kChunk + i) * p.v_s[1] + at : v0, there ? bytes : 0);
+        }
+      } else {
+        T* values = reinterpret_cast<T*>(to + W::kStage);
+        for (int i = tid; i < kChunk * slices * 16; i += step) {
+          const int row = i / (slices * 16), at = i % (slices * 16);
+          values[row * (pitch / int(sizeof(T))) + at] =
+              row < tokens && at < here ? v0[((long long)c * kChunk + row) * p.v_s[1] + at * p.v_s[3]] : from_f32<T>(0.0f);
+        }
+      }
+      async_commit();
+    };
+    T* y = static_cast<T*>(p.y) + n * p.y_s[0] + h * p.y_s[2] + row0 * p.y_s[3];
+    if (chunks > 0) ask(0);
+    for (int c = 0; c < chunks; ++c) {
+      async_wait<0>();
+      arrive_at(c);
+      if (stages > 1 && c + 1 < chunks) ask(c + 1);
+      const uint8_t* const base = smem_raw + (c % stages) * stage_bytes;
+      const uint32_t queries = smem_u32(base) + W::kKeyBytes + lane * 16, weights = smem_u32(base) + 2 * W::kKeyBytes + 2 * kLower + lane * 16;
+      const float* factors = reinterpret_cast<const float*>(base + 2 * W::kKeyBytes + (2 + Parts<T>::kOut) * kLower) + 2 * t;
+      float o[8][4];
+      barrier<96>(state_id);
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {   // S q
+        float z[8][4];
+        const uint4* from = reinterpret_cast<const uint4*>(exchange + E::kState + half * E::kStateHalf) + lane;
+#pragma unroll
+        for (int k = 0; k < kSteps / 2; ++k) {
+          uint32_t hi[4], lo[4], b[4][4];
+          const uint4 f = from[k * 32];
+          hi[0] = f.x, hi[1] = f.y, hi[2] = f.z, hi[3] = f.w;
+          if constexpr (Parts<T>::kOut == 2) {
+            const uint4 l = from[(kSteps / 2 + k) * 32];
+            lo[0] = l.x, lo[1] = l.y, lo[2] = l.z, lo[3] = l.w;
+          }
+#pragma unroll
+          for (int j = 0; j < 4; ++j) ldmatrix(b[j], queries + (j * kSteps + half * (kSteps / 2) + k) * kBlock);
+          mma_row<8>(z, hi, b, k == 0);
+          if constexpr (Parts<T>::kOut == 2) mma_row<8>(z, lo, b);
+          if constexpr (Parts<T>::kKey == 2) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) ldmatrix(b[j], queries + kKeyPart + (j * kSteps + half * (kSteps / 2) + k) * kBlock);
+            mma_row<8>(z, hi, b);
+          }
+        }
+        const float2 down = reinterpret_cast<const float2*>(exchange + E::kScales)[half * 32 + lane];
+        const F2 down0 = f2_both(down.x), down1 = f2_both(down.y);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          if (half == 0) set_rows(o[j], f2_mul(first_row(z[j]), down0), f2_mul(second_row(z[j]), down1));
+          else set_rows(o[j], f2_fma(first_row(z[j]), down0, first_row(o[j])), f2_fma(second_row(z[j]), down1, second_row(o[j])));
+        }
+      }
+      barrier<96>(written_id);
+      float u[8][4], z[8][4];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float4 f = reinterpret_cast<const float4*>(exchange + E::kWritten)[j * 32 + lane];
+        u[j][0] = f.x, u[j][1] = f.y, u[j][2] = f.z, u[j][3] = f.w;
+      }
+      float u0, u1;
+      row_scales<8>(u, u0, u1);
+      const F2 up0 = f2_both(u0), up1 = f2_both(u1);
+      auto step_of = [&](auto kc) {   // U P^T, a lower triangle of blocks
+        constexpr int k = decltype(kc)::value;
+        uint32_t hi[4], lo[4], b[4][4];
+        if constexpr (Parts<T>::kOut == 2) operand(u[2 * k], u[2 * k + 1], up0, up1, hi, lo);
+        else operand(u[2 * k], u[2 * k + 1], up0, up1, hi);
+#pragma unroll
+        for (int j = k; j < 4; ++j) ldmatrix(b[j], weights + lower_block(j, k) * kBlock);
+        mma_row<8, 2 * k>(z, hi, b, k == 0);
+        if constexpr (Parts<T>::kOut == 2) {
+          mma_row<8, 2 * k>(z, lo, b);
+#pragma unroll
+          for (int j = k; j < 4; ++j) ldmatrix(b[j], weights + kLower + lower_block(j, k) * kBlock);
+          mma_row<8, 2 * k>(z, hi, b);
+        }
+      };
+      step_of(std::integral_constant<int, 0>{});
+      step_of(std::integral_constant<int, 1>{});
+      step_of(std::integral_constant<int, 2>{});
+      step_of(std::integral_constant<int, 3>{});
+      const F2 down0 = f2_both(inverse_of_power(u0)), down1 = f2_both(inverse_of_power(u1));
+      T* to = y + (long long)c * kChunk * p.y_s[1];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float out[2][4];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int tile = 2 * i + j;
+          const F2 b = pair_at(factors + kChunk + tile * 8), f = pair_at(factors + 4 * kChunk + tile * 8);
+          set_rows(out[j], f2_fma(f, f2_mul(first_row(z[tile]), down0), f2_mul(b, first_row(o[tile]))),
+                   f2_fma(f, f2_mul(second_row(z[tile]), down1), f2_mul(b, second_row(o[tile]))));
+        }
+        put_outputs<T, WHOLE>(p, to + i * 16 * p.y_s[1], out, end - c * kChunk - i * 16, channels);
+      }
+      if (stages == 1) {
+        __syncthreads();
+        if (c + 1 < chunks) ask(c + 1);
       }
     }
-    async_commit();
-  };
-  if (chunks > 0) ask(0);
+    // tokens behind the row's end
+    for (long long i = end * 16ll + lane; i < p.L * 16ll; i += 32)
+      if (i % 16 < channels) y[i / 16 * p.y_s[1] + i % 16 * p.y_s[3]] = from_f32<T>(0.0f);
+    if (*static_cast<volatile uint32_t*>(&abort_word) != 0 && tid == 0) {   // after an incident: give the copies in flight time to land
+      volatile uint32_t never = 0;
+      for (int c = max(0, chunks - 2); c < chunks; ++c)
+        mbar_wait_bounded(&full[c % stages], uint32_t(c / stages) & 1u, &never, status, kIncidentDrainWait, kWaitLimitCycles / 16);
+    }
+    return;
+  }
 
-  // Two warps hold 16 rows of the state, half of the keys' channels each: s[j] rows lane / 4, + 8, channels 8 j + 2 (lane % 4), + 1.
-  const int g = lane >> 2, t = lane & 3, m = lane >> 3, r = lane & 7;
-  const int slice = warp >> 1, half = warp & 1;
-  const int row0 = first + slice * 16, channels = min(16, p.V - row0);
+  // ---- two warps hold 16 rows of the state, half of the keys' channels each: s[j] rows lane / 4, + 8, channels 8 j + 2 (lane % 4), + 1
   const long long state_at = ((n * p.H + h) * p.V + row0) * (long long)p.K;
-  // what a warp leaves for the other one: its 8 tiles of S k, and its 8 of S q
-  float4* const exchange = reinterpret_cast<float4*>(smem_raw + stages * stage_bytes + slice * kExchange) + lane;
-  float4 *const mine = exchange + half * 16 * 32, *const theirs = exchange + (half ^ 1) * 16 * 32;
+  float4 *const mine = reinterpret_cast<float4*>(exchange + half * 8 * 512) + lane, *const theirs = reinterpret_cast<float4*>(exchange + (half ^ 1) * 8 * 512) + lane;
   float s[kHalf / 8][4];
 #pragma unroll
   for (int j = 0; j < kHalf / 8; ++j)
@@ -597,83 +782,56 @@ delta_chunks_kernel(const DeltaParams p, int blocks_a_head, int stages) {
       const int row = g + (i >> 1) * 8, at = half * kHalf + j * 8 + 2 * t + (i & 1);
       s[j][i] = p.initial != nullptr && row < channels && at < p.K ? p.initial[state_at + (long long)row * p.K + at] : 0.0f;
     }
-  T* y = static_cast<T*>(p.y) + n * p.y_s[0] + h * p.y_s[2] + row0 * p.y_s[3];
-  // y of 16-token blocks 0 and 3 is finished by the first of the two warps, of 1 and 2 by the second: P is lower triangular
-  const int own[2] = {half, 3 - half};
 
   for (int c = 0; c < chunks; ++c) {
-    async_wait<0>();
-    __syncthreads();   // chunk c is there, and all are done with chunk c - 1
-    if (stages > 1 && c + 1 < chunks) ask(c + 1);
-    const int base_at = (c % stages) * stage_bytes;
-    const uint32_t keys = smem + base_at, queries = keys + W::kKeyBytes, square = queries + W::kKeyBytes;
-    const float* factors = reinterpret_cast<const float*>(smem_raw + base_at + 2 * W::kKeyBytes + (2 + Parts<T>::kOut) * kSquare) + 2 * t;
+    arrive_at(c);
+    const uint8_t* const base = smem_raw + (c % stages) * stage_bytes;
+    const uint32_t keys = smem_u32(base) + half * (kSteps / 2) * kBlock, solve = smem_u32(base) + 2 * W::kKeyBytes + lane * 16;
+    const float* factors = reinterpret_cast<const float*>(base + 2 * W::kKeyBytes + (2 + Parts<T>::kOut) * kLower) + 2 * t;
     float x[8][4];
-    {   // S k and S q, of this warp's channels
-      float s0, s1, o[8][4];
+    {   // S k, of this warp's channels
+      float s0, s1;
       row_scales<kHalf / 8>(s, s0, s1);
       const F2 up0 = f2_both(s0), up1 = f2_both(s1);
+      uint4* const left = reinterpret_cast<uint4*>(exchange + E::kState + half * E::kStateHalf) + lane;
 #pragma unroll
-      for (int k = 0; k < kHalf / 16; ++k) {
-        uint32_t hi[4], lo[4];
+      for (int k = 0; k < kSteps / 2; ++k) {
+        uint32_t hi[4], lo[4], b[4][4];
         operand(s[2 * k], s[2 * k + 1], up0, up1, hi, lo);
-        const int at = half * (kHalf / 8) + 2 * k + (m & 1);
-        uint32_t b[4][4];
+        left[k * 32] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        if constexpr (Parts<T>::kOut == 2) left[(kSteps / 2 + k) * 32] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) ldmatrix(b[j], keys + piece<KEYS>(j * 16 + (m >> 1) * 8 + r, at));
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          if (k == 0) mma_first(x[j], hi, b[j >> 1][2 * (j & 1)], b[j >> 1][2 * (j & 1) + 1]);
-          else mma(x[j], hi, b[j >> 1][2 * (j & 1)], b[j >> 1][2 * (j & 1) + 1]);
-        }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) mma(x[j], lo, b[j >> 1][2 * (j & 1)], b[j >> 1][2 * (j & 1) + 1]);
+        for (int j = 0; j < 4; ++j) ldmatrix(b[j], keys + lane * 16 + (j * kSteps + k) * kBlock);
+        mma_row<8>(x, hi, b, k == 0);
+        mma_row<8>(x, lo, b);
         if constexpr (Parts<T>::kKey == 2) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) ldmatrix(b[j], keys + kKeyPart + piece<KEYS>(j * 16 + (m >> 1) * 8 + r, at));
-#pragma unroll
-          for (int j = 0; j < 8; ++j) mma(x[j], hi, b[j >> 1][2 * (j & 1)], b[j >> 1][2 * (j & 1) + 1]);
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) ldmatrix(b[j], queries + piece<KEYS>(j * 16 + (m >> 1) * 8 + r, at));
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          if (k == 0) mma_first(o[j], hi, b[j >> 1][2 * (j & 1)], b[j >> 1][2 * (j & 1) + 1]);
-          else mma(o[j], hi, b[j >> 1][2 * (j & 1)], b[j >> 1][2 * (j & 1) + 1]);
-        }
-        if constexpr (Parts<T>::kOut == 2) {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) mma(o[j], lo, b[j >> 1][2 * (j & 1)], b[j >> 1][2 * (j & 1) + 1]);
-        }
-        if constexpr (Parts<T>::kKey == 2) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) ldmatrix(b[j], queries + kKeyPart + piece<KEYS>(j * 16 + (m >> 1) * 8 + r, at));
-#pragma unroll
-          for (int j = 0; j < 8; ++j) mma(o[j], hi, b[j >> 1][2 * (j & 1)], b[j >> 1][2 * (j & 1) + 1]);
+          for (int j = 0; j < 4; ++j) ldmatrix(b[j], keys + kKeyPart + lane * 16 + (j * kSteps + k) * kBlock);
+          mma_row<8>(x, hi, b);
         }
       }
-      const F2 down0 = f2_both(inverse_of_power(s0)), down1 = f2_both(inverse_of_power(s1));
+      const float i0 = inverse_of_power(s0), i1 = inverse_of_power(s1);
+      reinterpret_cast<float2*>(exchange + E::kScales)[half * 32 + lane] = make_float2(i0, i1);
+      barrier_arrive<96>(state_id);
+      const F2 down0 = f2_both(i0), down1 = f2_both(i1);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         set_rows(x[j], f2_mul(first_row(x[j]), down0), f2_mul(second_row(x[j]), down1));
-        set_rows(o[j], f2_mul(first_row(o[j]), down0), f2_mul(second_row(o[j]), down1));
         mine[j * 32] = make_float4(x[j][0], x[j][1], x[j][2], x[j][3]);
-        mine[(8 + j) * 32] = make_float4(o[j][0], o[j][1], o[j][2], o[j][3]);
       }
     }
-    pair_barrier(1 + slice);
+    barrier<64>(pair_id);
     // v - e^G S k (the factors are negative)
-    const uint32_t values = smem + base_at + W::kStage;
 #pragma unroll
     for (int j = 0; j < 8; j += 2) {
       float v[2][4];
       if constexpr (sizeof(T) == 2) {
         uint32_t b[4];   // channels 0 .. 7 and 8 .. 15 of tokens 8 j .., then of 8 (j + 1) ..
-        ldmatrix_t(b, values + (j * 8 + (m >> 1) * 8 + r) * pitch + (slice * 16 + (m & 1) * 8) * 2);
+        ldmatrix_t(b, smem_u32(base) + W::kStage + (j * 8 + (m >> 1) * 8 + r) * pitch + (slice * 16 + (m & 1) * 8) * 2);
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i >> 2][i & 3] = to_f32<T>(reinterpret_cast<const T*>(b)[i]);
       } else {
-        const float* f = reinterpret_cast<const float*>(smem_raw + base_at + W::kStage);
+        const float* f = reinterpret_cast<const float*>(base + W::kStage);
 #pragma unroll
         for (int i = 0; i < 8; ++i)
           v[i >> 2][i & 3] = f[((j + (i >> 2)) * 8 + 2 * t + (i & 1)) * (pitch / 4) + slice * 16 + g + ((i >> 1) & 1) * 8];
@@ -692,75 +850,31 @@ delta_chunks_kernel(const DeltaParams p, int blocks_a_head, int stages) {
       float r0, r1;
       row_scales<8>(x, r0, r1);
       const F2 up0 = f2_both(r0), up1 = f2_both(r1);
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
+      auto step_of = [&](auto kc) {
+        constexpr int k = decltype(kc)::value;
         uint32_t hi[4], lo[4], b[4][4], bl[4][4];
         operand(x[2 * k], x[2 * k + 1], up0, up1, hi, lo);
 #pragma unroll
-        for (int j = k; j < 4; ++j) {   // (T is lower triangular)
-          const uint32_t at = square + piece<kChunk>(j * 16 + (m >> 1) * 8 + r, 2 * k + (m & 1));
-          ldmatrix(b[j], at);
-          ldmatrix(bl[j], at + kSquare);
+        for (int j = k; j < 4; ++j) {
+          ldmatrix(b[j], solve + lower_block(j, k) * kBlock);
+          ldmatrix(bl[j], solve + kLower + lower_block(j, k) * kBlock);
         }
-#pragma unroll
-        for (int j = 2 * k; j < 8; ++j) {
-          if (k == 0) mma_first(u[j], hi, b[j >> 1][2 * (j & 1)], b[j >> 1][2 * (j & 1) + 1]);
-          else mma(u[j], hi, b[j >> 1][2 * (j & 1)], b[j >> 1][2 * (j & 1) + 1]);
-        }
-#pragma unroll
-        for (int j = 2 * k; j < 8; ++j) mma(u[j], lo, b[j >> 1][2 * (j & 1)], b[j >> 1][2 * (j & 1) + 1]);
-#pragma unroll
-        for (int j = 2 * k; j < 8; ++j) mma(u[j], hi, bl[j >> 1][2 * (j & 1)], bl[j >> 1][2 * (j & 1) + 1]);
-      }
+        mma_row<8, 2 * k>(u, hi, b, k == 0);
+        mma_row<8, 2 * k>(u, lo, b);
+        mma_row<8, 2 * k>(u, hi, bl);
+      };
+      step_of(std::integral_constant<int, 0>{});
+      step_of(std::integral_constant<int, 1>{});
+      step_of(std::integral_constant<int, 2>{});
+      step_of(std::integral_constant<int, 3>{});
       const F2 down0 = f2_both(inverse_of_power(r0)), down1 = f2_both(inverse_of_power(r1));
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const F2 f = pair_at(factors + 3 * kChunk + j * 8);
         set_rows(u[j], f2_mul(f, f2_mul(first_row(u[j]), down0)), f2_mul(f, f2_mul(second_row(u[j]), down1)));
+        if ((j >> 2) == half) reinterpret_cast<float4*>(exchange + E::kWritten)[j * 32 + lane] = make_float4(u[j][0], u[j][1], u[j][2], u[j][3]);
       }
-    }
-    {   // y = e^G S q + U P^T
-      float u0, u1, z[2][2][4] = {};
-      row_scales<8>(u, u0, u1);
-      const F2 up0 = f2_both(u0), up1 = f2_both(u1);
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        uint32_t hi[4], lo[4];
-        if constexpr (Parts<T>::kOut == 2) operand(u[2 * k], u[2 * k + 1], up0, up1, hi, lo);
-        else operand(u[2 * k], u[2 * k + 1], up0, up1, hi);
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-          if (k <= own[i]) {
-            const uint32_t at = square + 2 * kSquare + piece<kChunk>(own[i] * 16 + (m >> 1) * 8 + r, 2 * k + (m & 1));
-            uint32_t b[4];
-            ldmatrix(b, at);
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              mma(z[i][j], hi, b[2 * j], b[2 * j + 1]);
-              if constexpr (Parts<T>::kOut == 2) mma(z[i][j], lo, b[2 * j], b[2 * j + 1]);
-            }
-            if constexpr (Parts<T>::kOut == 2) {
-              ldmatrix(b, at + kSquare);
-#pragma unroll
-              for (int j = 0; j < 2; ++j) mma(z[i][j], hi, b[2 * j], b[2 * j + 1]);
-            }
-          }
-      }
-      const F2 down0 = f2_both(inverse_of_power(u0)), down1 = f2_both(inverse_of_power(u1));
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const int tile = own[i] * 2 + j;
-          const F2 b = pair_at(factors + kChunk + tile * 8), f = pair_at(factors + 4 * kChunk + tile * 8);
-          const float4 o = mine[(8 + tile) * 32], other = theirs[(8 + tile) * 32];
-          const F2 q0 = f2_mul(b, f2_add(f2_pack(o.x, o.y), f2_pack(other.x, other.y)));
-          const F2 q1 = f2_mul(b, f2_add(f2_pack(o.z, o.w), f2_pack(other.z, other.w)));
-          set_rows(z[i][j], f2_fma(f, f2_mul(first_row(z[i][j]), down0), q0), f2_fma(f, f2_mul(second_row(z[i][j]), down1), q1));
-        }
-        const int token = c * kChunk + own[i] * 16;
-        put_outputs<T, WHOLE>(p, y + token * p.y_s[1], z[i], end - token, channels);
-      }
+      barrier_arrive<96>(written_id);
     }
     // S = e^(G_64) S + (e^(G_64 - G) U) k, of this warp's channels
 #pragma unroll
@@ -773,26 +887,19 @@ delta_chunks_kernel(const DeltaParams p, int blocks_a_head, int stages) {
       float u0, u1, z[kHalf / 8][4];
       row_scales<8>(u, u0, u1);
       const F2 up0 = f2_both(u0), up1 = f2_both(u1);
+      const uint32_t columns = keys + ((m & 1) * 2 + (m >> 1)) * 128 + r * 16;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        uint32_t hi[4], lo[4], b[kHalf / 16][4];
+        uint32_t hi[4], lo[4], b[kSteps / 2][4];
         operand(u[2 * k], u[2 * k + 1], up0, up1, hi, lo);
 #pragma unroll
-        for (int j = 0; j < kHalf / 16; ++j)
-          ldmatrix_t(b[j], keys + piece<KEYS>(k * 16 + (m & 1) * 8 + r, half * (kHalf / 8) + 2 * j + (m >> 1)));
-#pragma unroll
-        for (int j = 0; j < kHalf / 8; ++j) {
-          if (k == 0) mma_first(z[j], hi, b[j >> 1][2 * (j & 1)], b[j >> 1][2 * (j & 1) + 1]);
-          else mma(z[j], hi, b[j >> 1][2 * (j & 1)], b[j >> 1][2 * (j & 1) + 1]);
-        }
-#pragma unroll
-        for (int j = 0; j < kHalf / 8; ++j) mma(z[j], lo, b[j >> 1][2 * (j & 1)], b[j >> 1][2 * (j & 1) + 1]);
+        for (int j = 0; j < kSteps / 2; ++j) ldmatrix_t(b[j], columns + (k * kSteps + j) * kBlock);
+        mma_row<kHalf / 8>(z, hi, b, k == 0);
+        mma_row<kHalf / 8>(z, lo, b);
         if constexpr (Parts<T>::kKey == 2) {
 #pragma unroll
-          for (int j = 0; j < kHalf / 16; ++j)
-            ldmatrix_t(b[j], keys + kKeyPart + piece<KEYS>(k * 16 + (m & 1) * 8 + r, half * (kHalf / 8) + 2 * j + (m >> 1)));
-#pragma unroll
-          for (int j = 0; j < kHalf / 8; ++j) mma(z[j], hi, b[j >> 1][2 * (j & 1)], b[j >> 1][2 * (j & 1) + 1]);
+          for (int j = 0; j < kSteps / 2; ++j) ldmatrix_t(b[j], columns + kKeyPart + (k * kSteps + j) * kBlock);
+          mma_row<kHalf / 8>(z, hi, b);
         }
       }
       const F2 down0 = f2_both(inverse_of_power(u0)), down1 = f2_both(inverse_of_power(u1));
@@ -800,10 +907,7 @@ delta_chunks_kernel(const DeltaParams p, int blocks_a_head, int stages) {
       for (int j = 0; j < kHalf / 8; ++j)
         set_rows(s[j], f2_fma(keep, first_row(s[j]), f2_mul(first_row(z[j]), down0)), f2_fma(keep, second_row(s[j]), f2_mul(second_row(z[j]), down1)));
     }
-    if (stages == 1) {
-      __syncthreads();
-      if (c + 1 < chunks) ask(c + 1);
-    }
+    if (stages == 1) __syncthreads();
   }
 
   if (p.final_state != nullptr) {
@@ -815,9 +919,6 @@ delta_chunks_kernel(const DeltaParams p, int blocks_a_head, int stages) {
         if (row < channels && at < p.K) p.final_state[state_at + (long long)row * p.K + at] = s[j][i];
       }
   }
-  // tokens behind the row's end
-  for (long long i = end * 16ll + half * 32 + lane; i < p.L * 16ll; i += 64)
-    if (i % 16 < channels) y[i / 16 * p.y_s[1] + i % 16 * p.y_s[3]] = from_f32<T>(0.0f);
 }
 
 // ---- launching -----------------------------------------------------------------------------------------------------
@@ -848,9 +949,9 @@ cudaError_t run(const DeltaParams& p, cudaStream_t stream) {
   const int most = (p.V + 15) / 16;
   auto blocks_of = [&](int slices) { return (long long)p.N * p.H * ((most + slices - 1) / slices); };
   auto smem_of = [&](int slices, int stages) {
-    return stages * (Work<T, KEYS>::kStage + kChunk * value_pitch<T>(slices)) + slices * kExchange;
+    return stages * (Work<T, KEYS>::kStage + kChunk * value_pitch<T>(slices)) + slices * Exchange<T, KEYS>::kBytes;
   };
-  constexpr int kMostSmem = 227 * 1024;
+  constexpr int kMostSmem = 227 * 1024 - 256;   // (and the barriers)
   // Four slices to a block put two warps on a quarter of an SM: a chunk takes longer, but twice the rows
   int slices = most < 2 ? most : 2;
   if (most > 2 && 5 * ((blocks_of(4) + current_sm_count() - 1) / current_sm_count()) < 3 * ((blocks_of(2) + current_sm_count() - 1) / current_sm_count()))
@@ -864,8 +965,12 @@ cudaError_t run(const DeltaParams& p, cudaStream_t stream) {
   auto* kernel = values_whole ? delta_chunks_kernel<T, KEYS, true> : delta_chunks_kernel<T, KEYS, false>;
   e = allow_smem(kernel, kMostSmem, done[2 + values_whole]);
   if (e != cudaSuccess) return e;
-  return launch_seq(kernel, dim3(unsigned(blocks)), 2 * slices * 32, smem_of(slices, stages), 1, stream, p,
-                    (most + slices - 1) / slices, stages);
+  uint32_t* status;
+  long long wait_limit;
+  bounded_wait_of(&status, &wait_limit);
+  if (status == nullptr) return cudaErrorInvalidSymbol;
+  return launch_seq(kernel, dim3(unsigned(blocks)), 3 * slices * 32, smem_of(slices, stages), 1, stream, p, (most + slices - 1) / slices, stages,
+                    status, wait_limit);
 }
 
 // f(TypeOf<T>, integral_constant<int, KEYS>)

@@ -18,7 +18,8 @@ enum : uint32_t {
   kIncidentDrainWait = 5,      // teardown: outstanding copies never landed
   kIncidentPartialWait = 6,    // epilogue of a split tile: another pair's partial sums never arrived
   kIncidentResidualWait = 7,   // epilogue: the residual box never landed in the staging buffer
-  kIncidentDepthwiseWait = 8   // depthwise: an input row never landed in its ring slot
+  kIncidentDepthwiseWait = 8,  // depthwise: an input row never landed in its ring slot
+  kIncidentDeltaWait = 9       // gated delta rule: a chunk's operands never landed
 };
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
