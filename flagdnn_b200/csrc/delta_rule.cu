@@ -64,11 +64,9 @@ __device__ __forceinline__ void ldmatrix_t(uint32_t (&r)[4], uint32_t at) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
 }
-// An 8 x 8 matrix of 16-bit values held as accumulators are, transposed.
-__device__ __forceinline__ uint32_t transposed(uint32_t v) {
-  uint32_t r;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
-  return r;
+// Four 8 x 8 matrices of 16-bit values, held as accumulators are, transposed to shared memory: 16-byte rows at each lane's address.
+__device__ __forceinline__ void stmatrix_t(uint32_t at, uint32_t r0, uint32_t r1, uint32_t r2, uint32_t r3) {
+  asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(r0), "r"(r1), "r"(r2), "r"(r3) : "memory");
 }
 __device__ __forceinline__ void copy16(uint32_t to, const void* from, int bytes) {   // the rest of the 16 is zeros
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
@@ -534,13 +532,17 @@ delta_prepare_kernel(const DeltaParams p) {
 
 // ---- the chunks in order -------------------------------------------------------------------------------------------
 
-constexpr int kMostSlices = 4;   // of 16 rows of the state; three warps each: two that carry it on, one that makes y
+// A block has SLICES slices of 16 rows of the state or fewer. Each has two warps that carry the state on and OUTS that make y.  Two slices
+// with two of them leave each quarter of an SM one warp of either kind; four with one fill it.
+constexpr int kMostSlices = 4;
+__host__ __device__ constexpr int outs_of(int slices) { return slices <= 2 ? 2 : 1; }
 // What the warps of a slice leave for each other: S k of either half (8 tiles of 512 bytes each), S as operands (each half's, the high parts,
-// then the low ones), U (8 tiles in fp32), the scales of the operands.
+// then the low ones), U (8 tiles in fp32), the scales of the operands; and y on its way out.
 template <typename T, int KEYS>
 struct Exchange {
   static constexpr int kState = 2 * 8 * 512, kStatePart = KEYS / 32 * 512, kStateHalf = Parts<T>::kOut * kStatePart;
-  static constexpr int kWritten = kState + 2 * kStateHalf, kScales = kWritten + 8 * 512, kBytes = kScales + 2 * 32 * 8;
+  static constexpr int kWritten = kState + 2 * kStateHalf, kScales = kWritten + 8 * 512, kStage = kScales + 2 * 32 * 8,
+                       kBytes = kStage + (sizeof(T) == 2 ? 2048 : 0);
 };
 
 template <typename T>
@@ -552,37 +554,39 @@ template <int THREADS>
 __device__ __forceinline__ void barrier_arrive(int id) { asm volatile("bar.arrive %0, %1;" ::"r"(id), "n"(THREADS) : "memory"); }
 __device__ __forceinline__ F2 pair_at(const float* p) { return *reinterpret_cast<const F2*>(p); }
 
-// An output block: o[i][..] holds rows (value channels) lane / 4, + 8 and tokens 8 i + 2 (lane % 4), + 1; `y` is at its first token.
-template <typename T, bool WHOLE>
-__device__ __forceinline__ void put_outputs(const DeltaParams& p, T* y, const float (&o)[2][4], int tokens, int channels) {
+// Outputs of BLOCKS x 16 tokens: o[i][..] holds rows (value channels) lane / 4, + 8 and tokens 8 i + 2 (lane % 4), + 1; `y` is at the first
+// token.  16-bit ones go through `stage` (32 bytes a token) to 16-byte stores.
+template <typename T, bool WHOLE, int BLOCKS>
+__device__ __forceinline__ void put_outputs(const DeltaParams& p, T* y, const float (&o)[2 * BLOCKS][4], uint8_t* stage, int tokens, int channels) {
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  if constexpr (sizeof(T) == 2) {
+    const uint32_t to = smem_u32(stage) + (lane >> 4) * 256 + (lane & 7) * 32 + ((lane >> 3) & 1) * 16;
 #pragma unroll
-  for (int n = 0; n < 2; ++n) {
-    if constexpr (sizeof(T) == 2) {
-      const uint32_t lower = transposed(pack2(from_f32<T>(o[n][0]), from_f32<T>(o[n][1])));
-      const uint32_t upper = transposed(pack2(from_f32<T>(o[n][2]), from_f32<T>(o[n][3])));
-      const int token = n * 8 + g;
-      if (token < tokens) {
-        T* at = y + token * p.y_s[1];
-        if constexpr (WHOLE) {   // pairs of channels lie together and are whole
-          if (2 * t < channels) *reinterpret_cast<uint32_t*>(at + 2 * t) = lower;
-          if (8 + 2 * t < channels) *reinterpret_cast<uint32_t*>(at + 8 + 2 * t) = upper;
-        } else {
-          const T *l = reinterpret_cast<const T*>(&lower), *u = reinterpret_cast<const T*>(&upper);
+    for (int i = 0; i < BLOCKS; ++i)   // channels 0 .. 7 and 8 .. 15 of eight tokens, then of the next eight
+      stmatrix_t(to + i * 512, pack2(from_f32<T>(o[2 * i][0]), from_f32<T>(o[2 * i][1])), pack2(from_f32<T>(o[2 * i][2]), from_f32<T>(o[2 * i][3])),
+                 pack2(from_f32<T>(o[2 * i + 1][0]), from_f32<T>(o[2 * i + 1][1])), pack2(from_f32<T>(o[2 * i + 1][2]), from_f32<T>(o[2 * i + 1][3])));
+    __syncwarp();
+    if constexpr (WHOLE) {   // eight channels are whole, and 16 bytes
+      const int token = lane >> 1, channel = (lane & 1) * 8;
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            if (2 * t + j < channels) at[(2 * t + j) * p.y_s[3]] = l[j];
-            if (8 + 2 * t + j < channels) at[(8 + 2 * t + j) * p.y_s[3]] = u[j];
-          }
-        }
+      for (int i = 0; i < BLOCKS; ++i) {
+        const uint4 v = *reinterpret_cast<const uint4*>(stage + i * 512 + lane * 16);
+        if (i * 16 + token < tokens && channel < channels) *reinterpret_cast<uint4*>(y + (i * 16 + token) * p.y_s[1] + channel) = v;
       }
     } else {
+      const int channel = lane & 15;
+      for (int token = lane >> 4; token < min(BLOCKS * 16, tokens); token += 2)
+        if (channel < channels) y[token * p.y_s[1] + channel * p.y_s[3]] = reinterpret_cast<const T*>(stage)[token * 16 + channel];
+    }
+    __syncwarp();
+  } else {
+#pragma unroll
+    for (int n = 0; n < 2 * BLOCKS; ++n)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int token = n * 8 + 2 * t + (i & 1), channel = g + (i >> 1) * 8;
         if (token < tokens && channel < channels) y[token * p.y_s[1] + channel * p.y_s[3]] = from_f32<T>(o[n][i]);
       }
-    }
   }
 }
 
@@ -596,16 +600,16 @@ __device__ __forceinline__ void mma_row(float (&d)[TILES][4], const uint32_t (&a
   }
 }
 
-// WHOLE: 16 bytes of neighbouring value channels are copied at once, and pairs stored.
-template <typename T, int KEYS, bool WHOLE>
-__global__ void __launch_bounds__(3 * kMostSlices * 32, 1)
+// WHOLE: 16 bytes of neighbouring value channels are copied and stored at once.
+template <typename T, int KEYS, int SLICES, bool WHOLE>
+__global__ void __launch_bounds__((2 + outs_of(SLICES)) * SLICES * 32, 1)
 delta_chunks_kernel(const DeltaParams p, int blocks_a_head, int stages, uint32_t* status, long long wait_limit) {
   extern __shared__ __align__(128) uint8_t smem_raw[];
   __shared__ uint64_t full[2];
   __shared__ uint32_t abort_word;
   using W = Work<T, KEYS>;
   using E = Exchange<T, KEYS>;
-  constexpr int kKeyPart = kChunk * KEYS * 2, kHalf = KEYS / 2, kSteps = KEYS / 16;
+  constexpr int kKeyPart = kChunk * KEYS * 2, kHalf = KEYS / 2, kSteps = KEYS / 16, kOuts = outs_of(SLICES), kShare = 64 + 32 * kOuts;
   if (threadIdx.x == 0) {
     mbar_init(&full[0], 1);
     mbar_init(&full[1], 1);
@@ -615,7 +619,7 @@ delta_chunks_kernel(const DeltaParams p, int blocks_a_head, int stages, uint32_t
   __syncthreads();
   chained();
   const Layout w = layout_of<T, KEYS>(p);
-  const int lane = threadIdx.x & 31, slices = blockDim.x / 96;
+  const int lane = threadIdx.x & 31, slices = blockDim.x / kShare;
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
   const int h = int(blockIdx.x / blocks_a_head % p.H);
   const long long n = blockIdx.x / blocks_a_head / p.H;
@@ -625,7 +629,7 @@ delta_chunks_kernel(const DeltaParams p, int blocks_a_head, int stages, uint32_t
   const uint32_t smem = smem_u32(smem_raw);
   const int g = lane >> 2, t = lane & 3, m = lane >> 3, r = lane & 7;
   const bool outputs = warp >= 2 * slices;
-  const int slice = outputs ? warp - 2 * slices : warp >> 1, half = warp & 1;
+  const int slice = outputs ? (warp - 2 * slices) / kOuts : warp >> 1, half = warp & 1;
   const int row0 = first + slice * 16, channels = min(16, p.V - row0);
   uint8_t* const exchange = smem_raw + stages * stage_bytes + slice * E::kBytes;
   const int pair_id = 1 + slice, state_id = 1 + kMostSlices + slice, written_id = 1 + 2 * kMostSlices + slice;   // named barriers
@@ -637,7 +641,7 @@ delta_chunks_kernel(const DeltaParams p, int blocks_a_head, int stages, uint32_t
 
   if (outputs) {
     // ---- y, and the copies: chunk c + 1 is asked for at chunk c, where there is room for two
-    const int tid = threadIdx.x - 2 * slices * 32, step = slices * 32;
+    const int tid = threadIdx.x - 2 * slices * 32, step = kOuts * slices * 32;
     const uint8_t* keys_from = w.keys + (n * p.G + h / (p.H / p.G)) * w.chunks * (2ll * W::kKeyBytes);
     const uint8_t* heads_from = w.heads + (n * p.H + h) * w.chunks * (long long)W::kHeadBytes;
     const T* v0 = static_cast<const T*>(p.v) + n * p.v_s[0] + h * p.v_s[2] + first * p.v_s[3];
@@ -677,17 +681,21 @@ delta_chunks_kernel(const DeltaParams p, int blocks_a_head, int stages, uint32_t
       arrive_at(c);
       if (stages > 1 && c + 1 < chunks) ask(c + 1);
       const uint8_t* const base = smem_raw + (c % stages) * stage_bytes;
-      const uint32_t queries = smem_u32(base) + W::kKeyBytes + lane * 16, weights = smem_u32(base) + 2 * W::kKeyBytes + 2 * kLower + lane * 16;
-      const float* factors = reinterpret_cast<const float*>(base + 2 * W::kKeyBytes + (2 + Parts<T>::kOut) * kLower) + 2 * t;
-      float o[8][4];
-      barrier<96>(state_id);
+      // this warp's tokens: all of the chunk's, or its first or last 32
+      constexpr int kTiles = 8 / kOuts;
+      const int tile0 = kOuts == 2 ? (warp & 1) * kTiles : 0;
+      const uint32_t queries = smem_u32(base) + W::kKeyBytes + tile0 / 2 * kSteps * kBlock + lane * 16;
+      const uint32_t weights = smem_u32(base) + 2 * W::kKeyBytes + 2 * kLower + lane * 16;
+      const float* factors = reinterpret_cast<const float*>(base + 2 * W::kKeyBytes + (2 + Parts<T>::kOut) * kLower) + tile0 * 8 + 2 * t;
+      float o[kTiles][4];
+      barrier<kShare>(state_id);
 #pragma unroll
       for (int half = 0; half < 2; ++half) {   // S q
-        float z[8][4];
+        float z[kTiles][4];
         const uint4* from = reinterpret_cast<const uint4*>(exchange + E::kState + half * E::kStateHalf) + lane;
 #pragma unroll
         for (int k = 0; k < kSteps / 2; ++k) {
-          uint32_t hi[4], lo[4], b[4][4];
+          uint32_t hi[4], lo[4], b[kTiles / 2][4];
           const uint4 f = from[k * 32];
           hi[0] = f.x, hi[1] = f.y, hi[2] = f.z, hi[3] = f.w;
           if constexpr (Parts<T>::kOut == 2) {
@@ -695,73 +703,87 @@ delta_chunks_kernel(const DeltaParams p, int blocks_a_head, int stages, uint32_t
             lo[0] = l.x, lo[1] = l.y, lo[2] = l.z, lo[3] = l.w;
           }
 #pragma unroll
-          for (int j = 0; j < 4; ++j) ldmatrix(b[j], queries + (j * kSteps + half * (kSteps / 2) + k) * kBlock);
-          mma_row<8>(z, hi, b, k == 0);
-          if constexpr (Parts<T>::kOut == 2) mma_row<8>(z, lo, b);
+          for (int j = 0; j < kTiles / 2; ++j) ldmatrix(b[j], queries + (j * kSteps + half * (kSteps / 2) + k) * kBlock);
+          mma_row<kTiles>(z, hi, b, k == 0);
+          if constexpr (Parts<T>::kOut == 2) mma_row<kTiles>(z, lo, b);
           if constexpr (Parts<T>::kKey == 2) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) ldmatrix(b[j], queries + kKeyPart + (j * kSteps + half * (kSteps / 2) + k) * kBlock);
-            mma_row<8>(z, hi, b);
+            for (int j = 0; j < kTiles / 2; ++j) ldmatrix(b[j], queries + kKeyPart + (j * kSteps + half * (kSteps / 2) + k) * kBlock);
+            mma_row<kTiles>(z, hi, b);
           }
         }
         const float2 down = reinterpret_cast<const float2*>(exchange + E::kScales)[half * 32 + lane];
         const F2 down0 = f2_both(down.x), down1 = f2_both(down.y);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
+        for (int j = 0; j < kTiles; ++j) {
           if (half == 0) set_rows(o[j], f2_mul(first_row(z[j]), down0), f2_mul(second_row(z[j]), down1));
           else set_rows(o[j], f2_fma(first_row(z[j]), down0, first_row(o[j])), f2_fma(second_row(z[j]), down1, second_row(o[j])));
         }
       }
-      barrier<96>(written_id);
-      float u[8][4], z[8][4];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float4 f = reinterpret_cast<const float4*>(exchange + E::kWritten)[j * 32 + lane];
-        u[j][0] = f.x, u[j][1] = f.y, u[j][2] = f.z, u[j][3] = f.w;
+      for (int j = 0; j < kTiles; ++j) {
+        const F2 b = pair_at(factors + kChunk + j * 8);
+        set_rows(o[j], f2_mul(b, first_row(o[j])), f2_mul(b, second_row(o[j])));
       }
-      float u0, u1;
-      row_scales<8>(u, u0, u1);
-      const F2 up0 = f2_both(u0), up1 = f2_both(u1);
-      auto step_of = [&](auto kc) {   // U P^T, a lower triangle of blocks
-        constexpr int k = decltype(kc)::value;
-        uint32_t hi[4], lo[4], b[4][4];
-        if constexpr (Parts<T>::kOut == 2) operand(u[2 * k], u[2 * k + 1], up0, up1, hi, lo);
-        else operand(u[2 * k], u[2 * k + 1], up0, up1, hi);
+      barrier<kShare>(written_id);
+      {   // U P^T, a lower triangle of blocks: the blocks on and next to the diagonal, and with the last tokens a square before them
+        float u[kTiles][4], v[8 - kTiles + 1][4] = {}, z[kTiles][4] = {}, u0, u1, v0, v1;
+        auto load = [&](float (&to)[4], int tile) {
+          const float4 f = reinterpret_cast<const float4*>(exchange + E::kWritten)[tile * 32 + lane];
+          to[0] = f.x, to[1] = f.y, to[2] = f.z, to[3] = f.w;
+        };
 #pragma unroll
-        for (int j = k; j < 4; ++j) ldmatrix(b[j], weights + lower_block(j, k) * kBlock);
-        mma_row<8, 2 * k>(z, hi, b, k == 0);
-        if constexpr (Parts<T>::kOut == 2) {
-          mma_row<8, 2 * k>(z, lo, b);
+        for (int j = 0; j < kTiles; ++j) load(u[j], tile0 + j);
+        row_scales<kTiles>(u, u0, u1);
+        if (tile0 != 0) {
 #pragma unroll
-          for (int j = k; j < 4; ++j) ldmatrix(b[j], weights + kLower + lower_block(j, k) * kBlock);
-          mma_row<8, 2 * k>(z, hi, b);
+          for (int j = 0; j < 8 - kTiles; ++j) load(v[j], j);
+          row_scales<8 - kTiles + 1>(v, v0, v1);
+          u0 = fminf(u0, v0);
+          u1 = fminf(u1, v1);
         }
-      };
-      step_of(std::integral_constant<int, 0>{});
-      step_of(std::integral_constant<int, 1>{});
-      step_of(std::integral_constant<int, 2>{});
-      step_of(std::integral_constant<int, 3>{});
-      const F2 down0 = f2_both(inverse_of_power(u0)), down1 = f2_both(inverse_of_power(u1));
-      T* to = y + (long long)c * kChunk * p.y_s[1];
+        const F2 up0 = f2_both(u0), up1 = f2_both(u1);
+        auto products = [&](const float (&x)[4], const float (&y)[4], int k, auto from) {   // tokens 16 k ..: what they wrote, to blocks from .. on
+          constexpr int j0 = decltype(from)::value;
+          uint32_t hi[4], lo[4], b[kTiles / 2][4];
+          if constexpr (Parts<T>::kOut == 2) operand(x, y, up0, up1, hi, lo);
+          else operand(x, y, up0, up1, hi);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float out[2][4];
+          for (int j = j0; j < kTiles / 2; ++j) ldmatrix(b[j], weights + lower_block(tile0 / 2 + j, k) * kBlock);
+          mma_row<kTiles, 2 * j0>(z, hi, b);
+          if constexpr (Parts<T>::kOut == 2) {
+            mma_row<kTiles, 2 * j0>(z, lo, b);
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const int tile = 2 * i + j;
-          const F2 b = pair_at(factors + kChunk + tile * 8), f = pair_at(factors + 4 * kChunk + tile * 8);
-          set_rows(out[j], f2_fma(f, f2_mul(first_row(z[tile]), down0), f2_mul(b, first_row(o[tile]))),
-                   f2_fma(f, f2_mul(second_row(z[tile]), down1), f2_mul(b, second_row(o[tile]))));
+            for (int j = j0; j < kTiles / 2; ++j) ldmatrix(b[j], weights + kLower + lower_block(tile0 / 2 + j, k) * kBlock);
+            mma_row<kTiles, 2 * j0>(z, hi, b);
+          }
+        };
+        products(u[0], u[1], tile0 / 2, std::integral_constant<int, 0>{});
+        products(u[2], u[3], tile0 / 2 + 1, std::integral_constant<int, 1>{});
+        if constexpr (kOuts == 1) {
+          products(u[4], u[5], 2, std::integral_constant<int, 2>{});
+          products(u[6], u[7], 3, std::integral_constant<int, 3>{});
+        } else if (tile0 != 0) {
+          products(v[0], v[1], 0, std::integral_constant<int, 0>{});
+          products(v[2], v[3], 1, std::integral_constant<int, 0>{});
         }
-        put_outputs<T, WHOLE>(p, to + i * 16 * p.y_s[1], out, end - c * kChunk - i * 16, channels);
+        const F2 down0 = f2_both(inverse_of_power(u0)), down1 = f2_both(inverse_of_power(u1));
+#pragma unroll
+        for (int j = 0; j < kTiles; ++j) {
+          const F2 f = pair_at(factors + 4 * kChunk + j * 8);
+          set_rows(o[j], f2_fma(f, f2_mul(first_row(z[j]), down0), first_row(o[j])), f2_fma(f, f2_mul(second_row(z[j]), down1), second_row(o[j])));
+        }
       }
+      uint8_t* const stage = exchange + E::kStage + tile0 * 256;
+      const int token = c * kChunk + tile0 * 8;
+      put_outputs<T, WHOLE, kTiles / 2>(p, y + (long long)token * p.y_s[1], o, stage, end - token, channels);
       if (stages == 1) {
         __syncthreads();
         if (c + 1 < chunks) ask(c + 1);
       }
     }
     // tokens behind the row's end
-    for (long long i = end * 16ll + lane; i < p.L * 16ll; i += 32)
+    for (long long i = end * 16ll + (kOuts == 2 ? (warp & 1) * 32 : 0) + lane; i < p.L * 16ll; i += 32 * kOuts)
       if (i % 16 < channels) y[i / 16 * p.y_s[1] + i % 16 * p.y_s[3]] = from_f32<T>(0.0f);
     if (*static_cast<volatile uint32_t*>(&abort_word) != 0 && tid == 0) {   // after an incident: give the copies in flight time to land
       volatile uint32_t never = 0;
@@ -812,7 +834,7 @@ delta_chunks_kernel(const DeltaParams p, int blocks_a_head, int stages, uint32_t
       }
       const float i0 = inverse_of_power(s0), i1 = inverse_of_power(s1);
       reinterpret_cast<float2*>(exchange + E::kScales)[half * 32 + lane] = make_float2(i0, i1);
-      barrier_arrive<96>(state_id);
+      barrier_arrive<kShare>(state_id);
       const F2 down0 = f2_both(i0), down1 = f2_both(i1);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
@@ -874,7 +896,7 @@ delta_chunks_kernel(const DeltaParams p, int blocks_a_head, int stages, uint32_t
         set_rows(u[j], f2_mul(f, f2_mul(first_row(u[j]), down0)), f2_mul(f, f2_mul(second_row(u[j]), down1)));
         if ((j >> 2) == half) reinterpret_cast<float4*>(exchange + E::kWritten)[j * 32 + lane] = make_float4(u[j][0], u[j][1], u[j][2], u[j][3]);
       }
-      barrier_arrive<96>(written_id);
+      barrier_arrive<kShare>(written_id);
     }
     // S = e^(G_64) S + (e^(G_64 - G) U) k, of this warp's channels
 #pragma unroll
@@ -940,7 +962,7 @@ cudaError_t run(const DeltaParams& p, cudaStream_t stream) {
   const bool keys_whole = p.K % (16 / int(sizeof(T))) == 0 && eights<T>(p.k, p.k_s) && eights<T>(p.q, p.q_s);
   constexpr int kPrepSmem = int(sizeof(PrepShared<T, KEYS>));
   auto* prep = keys_whole ? delta_prepare_kernel<T, KEYS, true> : delta_prepare_kernel<T, KEYS, false>;
-  static std::atomic<uint64_t> done[4];
+  static std::atomic<uint64_t> done[2];
   cudaError_t e = allow_smem(prep, kPrepSmem, done[keys_whole]);
   if (e != cudaSuccess) return e;
   e = launch_seq(prep, dim3(unsigned(prep_blocks)), kPrepThreads, kPrepSmem, 1, stream, p);
@@ -952,25 +974,30 @@ cudaError_t run(const DeltaParams& p, cudaStream_t stream) {
     return stages * (Work<T, KEYS>::kStage + kChunk * value_pitch<T>(slices)) + slices * Exchange<T, KEYS>::kBytes;
   };
   constexpr int kMostSmem = 227 * 1024 - 256;   // (and the barriers)
-  // Four slices to a block put two warps on a quarter of an SM: a chunk takes longer, but twice the rows
+  // Four slices to a block: a chunk takes half as long again as with two, for twice the rows
+  const int sms = current_sm_count();
+  auto rounds = [&](int slices) { return (blocks_of(slices) + sms - 1) / sms; };
   int slices = most < 2 ? most : 2;
-  if (most > 2 && 5 * ((blocks_of(4) + current_sm_count() - 1) / current_sm_count()) < 3 * ((blocks_of(2) + current_sm_count() - 1) / current_sm_count()))
-    slices = most < 4 ? most : 4;
+  if (most > 2 && 3 * rounds(4) < 2 * rounds(2)) slices = most < 4 ? most : 4;
   while (slices > 1 && smem_of(slices, 2) > kMostSmem) --slices;
   const int stages = smem_of(slices, 2) <= kMostSmem ? 2 : 1;
   const long long blocks = blocks_of(slices);
   if (blocks > 0x7fffffffll) return cudaErrorInvalidConfiguration;
-  const bool values_whole = eights<T>(p.v, p.v_s) && p.V % 2 == 0 && p.y_s[3] == 1 && p.y_s[0] % 2 == 0 && p.y_s[1] % 2 == 0 &&
-                            p.y_s[2] % 2 == 0 && (reinterpret_cast<uintptr_t>(p.y) & 3u) == 0;
-  auto* kernel = values_whole ? delta_chunks_kernel<T, KEYS, true> : delta_chunks_kernel<T, KEYS, false>;
-  e = allow_smem(kernel, kMostSmem, done[2 + values_whole]);
-  if (e != cudaSuccess) return e;
-  uint32_t* status;
-  long long wait_limit;
-  bounded_wait_of(&status, &wait_limit);
-  if (status == nullptr) return cudaErrorInvalidSymbol;
-  return launch_seq(kernel, dim3(unsigned(blocks)), 3 * slices * 32, smem_of(slices, stages), 1, stream, p, (most + slices - 1) / slices, stages,
-                    status, wait_limit);
+  const bool values_whole = p.V % (16 / int(sizeof(T))) == 0 && eights<T>(p.v, p.v_s) && eights<T>(p.y, p.y_s);
+  auto go = [&](auto* kernel, std::atomic<uint64_t>& allowed, int most_slices) -> cudaError_t {
+    cudaError_t err = allow_smem(kernel, kMostSmem, allowed);
+    if (err != cudaSuccess) return err;
+    uint32_t* status;
+    long long wait_limit;
+    bounded_wait_of(&status, &wait_limit);
+    if (status == nullptr) return cudaErrorInvalidSymbol;
+    return launch_seq(kernel, dim3(unsigned(blocks)), (2 + outs_of(most_slices)) * slices * 32, smem_of(slices, stages), 1, stream, p,
+                      (most + slices - 1) / slices, stages, status, wait_limit);
+  };
+  static std::atomic<uint64_t> allowed[4];
+  if (slices <= 2)
+    return values_whole ? go(delta_chunks_kernel<T, KEYS, 2, true>, allowed[0], 2) : go(delta_chunks_kernel<T, KEYS, 2, false>, allowed[1], 2);
+  return values_whole ? go(delta_chunks_kernel<T, KEYS, 4, true>, allowed[2], 4) : go(delta_chunks_kernel<T, KEYS, 4, false>, allowed[3], 4);
 }
 
 // f(TypeOf<T>, integral_constant<int, KEYS>)
