@@ -191,67 +191,65 @@ struct PrepShared {
   HeadGates gates[4];
 };
 
-// Keys or queries of a chunk to their places, as parts, scaled; the factors that take the operands back (with the norm, if asked, and
-// `scale`).  A warp takes 8 rows at once, four lanes a row, so that what they write is 128 bytes in a run.
+// Keys or queries of a chunk, on their way to shared memory.  A warp takes 8 rows at once, four lanes a row, so that what they write is 128
+// bytes in a run; two passes make 64 rows.  All loads of a chunk are on their way before the first is waited for.
 template <typename T, int KEYS, bool WHOLE>
-__device__ __forceinline__ void stage_rows(const DeltaParams& p, const T* x, const long long* s, int tokens, float scale, uint8_t* to,
-                                           float* factor) {
-  constexpr int kPieces = KEYS / 32;   // of eight channels, to a lane
-  const int lane = threadIdx.x & 31, part = lane >> 3;
+struct Rows {
+  static constexpr int kPieces = KEYS / 32, kV = WHOLE ? 16 / int(sizeof(T)) : 1;   // pieces of eight channels, to a lane
+  Pack<T, kV> raw[2][kPieces][8 / kV];
+  static __device__ __forceinline__ int row(int pass) { return (pass * 4 + (threadIdx.x >> 5)) * 8 + (threadIdx.x & 7); }
+  static __device__ __forceinline__ int channel(int n) { return (n * 4 + ((threadIdx.x & 31) >> 3)) * 8; }
+  __device__ __forceinline__ void load(const T* x, const long long* s, int tokens, int K) {
 #pragma unroll
-  for (int pass = 0; pass < 2; ++pass) {
-    const int r = (pass * 4 + (threadIdx.x >> 5)) * 8 + (lane & 7);
-    float v[kPieces][8];
+    for (int pass = 0; pass < 2; ++pass)
 #pragma unroll
-    for (int n = 0; n < kPieces; ++n) {
-      const int at = (n * 4 + part) * 8;
-      if constexpr (WHOLE) {
-        constexpr int kV = 16 / sizeof(T);
+      for (int n = 0; n < kPieces; ++n)
 #pragma unroll
         for (int i = 0; i < 8 / kV; ++i) {
-          Pack<T, kV> q;
-          q.clear();
-          if (r < tokens && at + i * kV < p.K) q.load(x + r * s[1] + at + i * kV);
-#pragma unroll
-          for (int j = 0; j < kV; ++j) v[n][i * kV + j] = q.at(j);
+          const int at = channel(n) + i * kV;
+          raw[pass][n][i].clear();
+          if (row(pass) < tokens && at < K) raw[pass][n][i].load(x + row(pass) * s[1] + (WHOLE ? (long long)at : at * s[3]));
         }
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[n][j] = r < tokens && at + j < p.K ? to_f32<T>(x[r * s[1] + (at + j) * s[3]]) : 0.0f;
-      }
-    }
-    float most = 0.0f, squares = 0.0f;
-#pragma unroll
-    for (int n = 0; n < kPieces; ++n)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        most = fmaxf(most, fabsf(v[n][j]));
-        squares += v[n][j] * v[n][j];
-      }
-#pragma unroll
-    for (int o = 8; o < 32; o <<= 1) {
-      most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-      squares += __shfl_xor_sync(0xffffffffu, squares, o);
-    }
-    const float up = raise(most);
-#pragma unroll
-    for (int n = 0; n < kPieces; ++n) {
-      uint4 hi, lo;
-      uint32_t* h = reinterpret_cast<uint32_t*>(&hi);
-      uint32_t* l = reinterpret_cast<uint32_t*>(&lo);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const F2 x2 = f2_pack(v[n][2 * j] * up, v[n][2 * j + 1] * up);
-        h[j] = high(x2);
-        if constexpr (Parts<T>::kKey == 2) l[j] = low(x2, h[j]);
-      }
-      const int at = piece(r, n * 4 + part, KEYS / 16);
-      *reinterpret_cast<uint4*>(to + at) = hi;
-      if constexpr (Parts<T>::kKey == 2) *reinterpret_cast<uint4*>(to + kChunk * KEYS * 2 + at) = lo;
-    }
-    if (part == 0) factor[r] = r < tokens ? scale * inverse_of_power(up) * (p.norm ? 1.0f / sqrtf(squares + kKeyEps) : 1.0f) : 0.0f;
   }
-}
+  // To their places, as parts, scaled; the factors that take the operands back (with the norm, if asked, and `scale`).
+  __device__ __forceinline__ void stage(uint8_t* to, float* factor, int tokens, bool norm, float scale) const {
+#pragma unroll
+    for (int pass = 0; pass < 2; ++pass) {
+      float most = 0.0f, squares = 0.0f;
+#pragma unroll
+      for (int n = 0; n < kPieces; ++n)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float v = raw[pass][n][j / kV].at(j % kV);
+          most = fmaxf(most, fabsf(v));
+          squares += v * v;
+        }
+#pragma unroll
+      for (int o = 8; o < 32; o <<= 1) {
+        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+        squares += __shfl_xor_sync(0xffffffffu, squares, o);
+      }
+      const float up = raise(most);
+      const int r = row(pass);
+#pragma unroll
+      for (int n = 0; n < kPieces; ++n) {
+        uint4 hi, lo;
+        uint32_t* h = reinterpret_cast<uint32_t*>(&hi);
+        uint32_t* l = reinterpret_cast<uint32_t*>(&lo);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const F2 x = f2_mul(f2_pack(raw[pass][n][2 * j / kV].at(2 * j % kV), raw[pass][n][(2 * j + 1) / kV].at((2 * j + 1) % kV)), f2_both(up));
+          h[j] = high(x);
+          if constexpr (Parts<T>::kKey == 2) l[j] = low(x, h[j]);
+        }
+        const int at = piece(r, channel(n) / 8, KEYS / 16);
+        *reinterpret_cast<uint4*>(to + at) = hi;
+        if constexpr (Parts<T>::kKey == 2) *reinterpret_cast<uint4*>(to + kChunk * KEYS * 2 + at) = lo;
+      }
+      if ((threadIdx.x & 31) < 8) factor[r] = r < tokens ? scale * inverse_of_power(up) * (norm ? 1.0f / sqrtf(squares + kKeyEps) : 1.0f) : 0.0f;
+    }
+  }
+};
 
 // c += the products of row block `i` of `x` with the row blocks up to it of `y`, over KEYS channels.
 template <typename T, int KEYS>
@@ -397,25 +395,38 @@ __device__ __forceinline__ void invert(const float (&a)[kChunk][kPitch], float (
 }
 
 template <typename T, int KEYS, bool WHOLE>
-__global__ void __launch_bounds__(kPrepThreads, 4)
+__global__ void __launch_bounds__(kPrepThreads, 3)
 delta_prepare_kernel(const DeltaParams p) {
   extern __shared__ __align__(128) uint8_t smem_raw[];
   PrepShared<T, KEYS>& s = *reinterpret_cast<PrepShared<T, KEYS>*>(smem_raw);
   chained();
   using W = Work<T, KEYS>;
   const Layout w = layout_of<T, KEYS>(p);
-  const int c = int(blockIdx.x % w.chunks), g = int(blockIdx.x / w.chunks % p.G);
-  const long long n = blockIdx.x / w.chunks / p.G;
+  const int g = int(blockIdx.x % p.G), c = int(blockIdx.x / p.G % w.chunks);   // (heads of a token lie together)
+  const long long n = blockIdx.x / p.G / w.chunks;
   const int begin = c * kChunk, tokens = min(row_end(p, n) - begin, kChunk);
   if (tokens <= 0) return;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, q = lane >> 2, t = lane & 3;
   uint8_t* const queries = s.keys + W::kKeyBytes;
   const int group = p.H / p.G, h0 = g * group;
-  if (warp < group) sum_gates<T>(p, s.gates[warp], n, begin, tokens, h0 + warp);
-  stage_rows<T, KEYS, WHOLE>(p, static_cast<const T*>(p.k) + n * p.k_s[0] + begin * p.k_s[1] + g * p.k_s[2], p.k_s, tokens, 1.0f, s.keys,
-                             s.key_scale);
-  stage_rows<T, KEYS, WHOLE>(p, static_cast<const T*>(p.q) + n * p.q_s[0] + begin * p.q_s[1] + g * p.q_s[2], p.q_s, tokens, p.scale, queries,
-                             s.query_scale);
+  {
+    const T* kp = static_cast<const T*>(p.k) + n * p.k_s[0] + begin * p.k_s[1] + g * p.k_s[2];
+    const T* qp = static_cast<const T*>(p.q) + n * p.q_s[0] + begin * p.q_s[1] + g * p.q_s[2];
+    Rows<T, KEYS, WHOLE> rows;
+    rows.load(kp, p.k_s, tokens, p.K);
+    if constexpr (sizeof(T) == 2 && WHOLE) {   // (the queries' registers, too)
+      Rows<T, KEYS, WHOLE> more;
+      more.load(qp, p.q_s, tokens, p.K);
+      if (warp < group) sum_gates<T>(p, s.gates[warp], n, begin, tokens, h0 + warp);
+      rows.stage(s.keys, s.key_scale, tokens, p.norm, 1.0f);
+      more.stage(queries, s.query_scale, tokens, p.norm, p.scale);
+    } else {
+      if (warp < group) sum_gates<T>(p, s.gates[warp], n, begin, tokens, h0 + warp);
+      rows.stage(s.keys, s.key_scale, tokens, p.norm, 1.0f);
+      rows.load(qp, p.q_s, tokens, p.K);
+      rows.stage(queries, s.query_scale, tokens, p.norm, p.scale);
+    }
+  }
   __syncthreads();
   {
     uint4* to = reinterpret_cast<uint4*>(w.keys + ((n * p.G + g) * w.chunks + c) * (2ll * W::kKeyBytes));
@@ -534,7 +545,7 @@ delta_prepare_kernel(const DeltaParams p) {
 
 // A block has SLICES slices of 16 rows of the state or fewer. Each has two warps that carry the state on and OUTS that make y.  Two slices
 // with two of them leave each quarter of an SM one warp of either kind; four with one fill it.
-constexpr int kMostSlices = 4;
+constexpr int kMostSlices = 4, kMostStages = 3;
 __host__ __device__ constexpr int outs_of(int slices) { return slices <= 2 ? 2 : 1; }
 // What the warps of a slice leave for each other: S k of either half (8 tiles of 512 bytes each), S as operands (each half's, the high parts,
 // then the low ones), U (8 tiles in fp32), the scales of the operands; and y on its way out.
@@ -605,14 +616,13 @@ template <typename T, int KEYS, int SLICES, bool WHOLE>
 __global__ void __launch_bounds__((2 + outs_of(SLICES)) * SLICES * 32, 1)
 delta_chunks_kernel(const DeltaParams p, int blocks_a_head, int stages, uint32_t* status, long long wait_limit) {
   extern __shared__ __align__(128) uint8_t smem_raw[];
-  __shared__ uint64_t full[2];
+  __shared__ uint64_t full[kMostStages];
   __shared__ uint32_t abort_word;
   using W = Work<T, KEYS>;
   using E = Exchange<T, KEYS>;
   constexpr int kKeyPart = kChunk * KEYS * 2, kHalf = KEYS / 2, kSteps = KEYS / 16, kOuts = outs_of(SLICES), kShare = 64 + 32 * kOuts;
   if (threadIdx.x == 0) {
-    mbar_init(&full[0], 1);
-    mbar_init(&full[1], 1);
+    for (int i = 0; i < kMostStages; ++i) mbar_init(&full[i], 1);
     abort_word = 0;
     fence_barrier_init();
   }
@@ -640,7 +650,7 @@ delta_chunks_kernel(const DeltaParams p, int blocks_a_head, int stages, uint32_t
   };
 
   if (outputs) {
-    // ---- y, and the copies: chunk c + 1 is asked for at chunk c, where there is room for two
+    // ---- y, and the copies: chunk c + stages - 1 is asked for at chunk c, where there is room for more than one
     const int tid = threadIdx.x - 2 * slices * 32, step = kOuts * slices * 32;
     const uint8_t* keys_from = w.keys + (n * p.G + h / (p.H / p.G)) * w.chunks * (2ll * W::kKeyBytes);
     const uint8_t* heads_from = w.heads + (n * p.H + h) * w.chunks * (long long)W::kHeadBytes;
@@ -675,11 +685,18 @@ delta_chunks_kernel(const DeltaParams p, int blocks_a_head, int stages, uint32_t
       async_commit();
     };
     T* y = static_cast<T*>(p.y) + n * p.y_s[0] + h * p.y_s[2] + row0 * p.y_s[3];
-    if (chunks > 0) ask(0);
+    for (int c = 0; c < max(1, stages - 1); ++c) {
+      if (c < chunks) ask(c);
+      else async_commit();
+    }
     for (int c = 0; c < chunks; ++c) {
-      async_wait<0>();
+      if (stages == 3) async_wait<1>();   // (a thread's groups: one a chunk, empty ones behind the last)
+      else async_wait<0>();
       arrive_at(c);
-      if (stages > 1 && c + 1 < chunks) ask(c + 1);
+      if (stages > 1) {
+        if (c + stages - 1 < chunks) ask(c + stages - 1);
+        else async_commit();
+      }
       const uint8_t* const base = smem_raw + (c % stages) * stage_bytes;
       // this warp's tokens: all of the chunk's, or its first or last 32
       constexpr int kTiles = 8 / kOuts;
@@ -787,7 +804,7 @@ delta_chunks_kernel(const DeltaParams p, int blocks_a_head, int stages, uint32_t
       if (i % 16 < channels) y[i / 16 * p.y_s[1] + i % 16 * p.y_s[3]] = from_f32<T>(0.0f);
     if (*static_cast<volatile uint32_t*>(&abort_word) != 0 && tid == 0) {   // after an incident: give the copies in flight time to land
       volatile uint32_t never = 0;
-      for (int c = max(0, chunks - 2); c < chunks; ++c)
+      for (int c = max(0, chunks - stages); c < chunks; ++c)
         mbar_wait_bounded(&full[c % stages], uint32_t(c / stages) & 1u, &never, status, kIncidentDrainWait, kWaitLimitCycles / 16);
     }
     return;
@@ -810,27 +827,37 @@ delta_chunks_kernel(const DeltaParams p, int blocks_a_head, int stages, uint32_t
     const uint8_t* const base = smem_raw + (c % stages) * stage_bytes;
     const uint32_t keys = smem_u32(base) + half * (kSteps / 2) * kBlock, solve = smem_u32(base) + 2 * W::kKeyBytes + lane * 16;
     const float* factors = reinterpret_cast<const float*>(base + 2 * W::kKeyBytes + (2 + Parts<T>::kOut) * kLower) + 2 * t;
+    auto load_keys = [&](uint32_t (&b)[4][4], int k, int part) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) ldmatrix(b[j], keys + part * kKeyPart + lane * 16 + (j * kSteps + k) * kBlock);
+    };
     float x[8][4];
+    uint32_t values[4][4];   // 16-bit: channels 0 .. 7 and 8 .. 15 of tokens 16 i .., then of 16 i + 8 ..
     {   // S k, of this warp's channels
+      uint32_t b[2][4][4];
+      load_keys(b[0], 0, 0);
       float s0, s1;
       row_scales<kHalf / 8>(s, s0, s1);
       const F2 up0 = f2_both(s0), up1 = f2_both(s1);
       uint4* const left = reinterpret_cast<uint4*>(exchange + E::kState + half * E::kStateHalf) + lane;
 #pragma unroll
       for (int k = 0; k < kSteps / 2; ++k) {
-        uint32_t hi[4], lo[4], b[4][4];
+        uint32_t hi[4], lo[4];
+        if (k + 1 < kSteps / 2) load_keys(b[(k + 1) & 1], k + 1, 0);
         operand(s[2 * k], s[2 * k + 1], up0, up1, hi, lo);
         left[k * 32] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
         if constexpr (Parts<T>::kOut == 2) left[(kSteps / 2 + k) * 32] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) ldmatrix(b[j], keys + lane * 16 + (j * kSteps + k) * kBlock);
-        mma_row<8>(x, hi, b, k == 0);
-        mma_row<8>(x, lo, b);
+        mma_row<8>(x, hi, b[k & 1], k == 0);
+        mma_row<8>(x, lo, b[k & 1]);
         if constexpr (Parts<T>::kKey == 2) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) ldmatrix(b[j], keys + kKeyPart + lane * 16 + (j * kSteps + k) * kBlock);
-          mma_row<8>(x, hi, b);
+          load_keys(b[k & 1], k, 1);
+          mma_row<8>(x, hi, b[k & 1]);
         }
+      }
+      if constexpr (sizeof(T) == 2) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          ldmatrix_t(values[i], smem_u32(base) + W::kStage + (i * 16 + (m >> 1) * 8 + r) * pitch + (slice * 16 + (m & 1) * 8) * 2);
       }
       const float i0 = inverse_of_power(s0), i1 = inverse_of_power(s1);
       reinterpret_cast<float2*>(exchange + E::kScales)[half * 32 + lane] = make_float2(i0, i1);
@@ -842,86 +869,105 @@ delta_chunks_kernel(const DeltaParams p, int blocks_a_head, int stages, uint32_t
         mine[j * 32] = make_float4(x[j][0], x[j][1], x[j][2], x[j][3]);
       }
     }
+    F2 since[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) since[j] = pair_at(factors + j * 8);
     barrier<64>(pair_id);
     // v - e^G S k (the factors are negative)
 #pragma unroll
-    for (int j = 0; j < 8; j += 2) {
-      float v[2][4];
+    for (int j = 0; j < 8; ++j) {
+      const float4 other = theirs[j * 32];
+      float v[4];
       if constexpr (sizeof(T) == 2) {
-        uint32_t b[4];   // channels 0 .. 7 and 8 .. 15 of tokens 8 j .., then of 8 (j + 1) ..
-        ldmatrix_t(b, smem_u32(base) + W::kStage + (j * 8 + (m >> 1) * 8 + r) * pitch + (slice * 16 + (m & 1) * 8) * 2);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i >> 2][i & 3] = to_f32<T>(reinterpret_cast<const T*>(b)[i]);
+        for (int i = 0; i < 4; ++i) v[i] = to_f32<T>(reinterpret_cast<const T*>(values[j >> 1])[(j & 1) * 4 + i]);
       } else {
         const float* f = reinterpret_cast<const float*>(base + W::kStage);
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          v[i >> 2][i & 3] = f[((j + (i >> 2)) * 8 + 2 * t + (i & 1)) * (pitch / 4) + slice * 16 + g + ((i >> 1) & 1) * 8];
+        for (int i = 0; i < 4; ++i) v[i] = f[(j * 8 + 2 * t + (i & 1)) * (pitch / 4) + slice * 16 + g + (i >> 1) * 8];
       }
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const F2 a = pair_at(factors + (j + i) * 8);
-        const float4 other = theirs[(j + i) * 32];
-        set_rows(x[j + i], f2_fma(a, f2_add(first_row(x[j + i]), f2_pack(other.x, other.y)), first_row(v[i])),
-                 f2_fma(a, f2_add(second_row(x[j + i]), f2_pack(other.z, other.w)), second_row(v[i])));
-      }
+      set_rows(x[j], f2_fma(since[j], f2_add(first_row(x[j]), f2_pack(other.x, other.y)), first_row(v)),
+               f2_fma(since[j], f2_add(second_row(x[j]), f2_pack(other.z, other.w)), second_row(v)));
     }
-    // U = (v - ..) T^T, by both warps
-    float u[8][4];
+    // U = (v - ..) T^T: blocks 0 and 3 of 16 tokens by the first of the two warps, 1 and 2 by the second (T is lower triangular)
     {
-      float r0, r1;
+      const int own[2] = {half, 3 - half};
+      const uint32_t rows[2] = {solve + lower_block(own[0], 0) * kBlock, solve + lower_block(own[1], 0) * kBlock};
+      float z[2][2][4], r0, r1;
+      uint32_t b[2][4], bl[2][4];
+      auto load = [&](int i, int k) {
+        ldmatrix(b[i], rows[i] + k * kBlock);
+        ldmatrix(bl[i], rows[i] + kLower + k * kBlock);
+      };
+      load(0, 0);
+      load(1, 0);
       row_scales<8>(x, r0, r1);
       const F2 up0 = f2_both(r0), up1 = f2_both(r1);
-      auto step_of = [&](auto kc) {
-        constexpr int k = decltype(kc)::value;
-        uint32_t hi[4], lo[4], b[4][4], bl[4][4];
-        operand(x[2 * k], x[2 * k + 1], up0, up1, hi, lo);
+      auto products = [&](int i, int k, const uint32_t (&hi)[4], const uint32_t (&lo)[4]) {
 #pragma unroll
-        for (int j = k; j < 4; ++j) {
-          ldmatrix(b[j], solve + lower_block(j, k) * kBlock);
-          ldmatrix(bl[j], solve + kLower + lower_block(j, k) * kBlock);
+        for (int j = 0; j < 2; ++j) {
+          if (k == 0) mma_first(z[i][j], hi, b[i][2 * j], b[i][2 * j + 1]);
+          else mma(z[i][j], hi, b[i][2 * j], b[i][2 * j + 1]);
         }
-        mma_row<8, 2 * k>(u, hi, b, k == 0);
-        mma_row<8, 2 * k>(u, lo, b);
-        mma_row<8, 2 * k>(u, hi, bl);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) mma(z[i][j], lo, b[i][2 * j], b[i][2 * j + 1]);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) mma(z[i][j], hi, bl[i][2 * j], bl[i][2 * j + 1]);
       };
-      step_of(std::integral_constant<int, 0>{});
-      step_of(std::integral_constant<int, 1>{});
-      step_of(std::integral_constant<int, 2>{});
-      step_of(std::integral_constant<int, 3>{});
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        uint32_t hi[4], lo[4];
+        operand(x[2 * k], x[2 * k + 1], up0, up1, hi, lo);
+        if (k == 0 || (k == 1 && half != 0)) products(0, k, hi, lo);
+        if (k == 0 && half != 0) load(0, 1);
+        if (k < 3 || half == 0) products(1, k, hi, lo);
+        if (k < 2 || (k == 2 && half == 0)) load(1, k + 1);
+      }
       const F2 down0 = f2_both(inverse_of_power(r0)), down1 = f2_both(inverse_of_power(r1));
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const F2 f = pair_at(factors + 3 * kChunk + j * 8);
-        set_rows(u[j], f2_mul(f, f2_mul(first_row(u[j]), down0)), f2_mul(f, f2_mul(second_row(u[j]), down1)));
-        if ((j >> 2) == half) reinterpret_cast<float4*>(exchange + E::kWritten)[j * 32 + lane] = make_float4(u[j][0], u[j][1], u[j][2], u[j][3]);
-      }
-      barrier_arrive<kShare>(written_id);
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int tile = 2 * own[i] + j;
+          const F2 f = pair_at(factors + 3 * kChunk + tile * 8);
+          float out[4];
+          set_rows(out, f2_mul(f, f2_mul(first_row(z[i][j]), down0)), f2_mul(f, f2_mul(second_row(z[i][j]), down1)));
+          reinterpret_cast<float4*>(exchange + E::kWritten)[tile * 32 + lane] = make_float4(out[0], out[1], out[2], out[3]);
+        }
     }
     // S = e^(G_64) S + (e^(G_64 - G) U) k, of this warp's channels
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const F2 f = pair_at(factors + 2 * kChunk + j * 8);
-      set_rows(u[j], f2_mul(first_row(u[j]), f), f2_mul(second_row(u[j]), f));
-    }
     {
+      const uint32_t columns = keys + ((m & 1) * 2 + (m >> 1)) * 128 + r * 16;
+      auto load_columns = [&](uint32_t (&b)[kSteps / 2][4], int k, int part) {
+#pragma unroll
+        for (int j = 0; j < kSteps / 2; ++j) ldmatrix_t(b[j], columns + part * kKeyPart + (k * kSteps + j) * kBlock);
+      };
+      uint32_t b[2][kSteps / 2][4];
+      load_columns(b[0], 0, 0);
+      float u[8][4];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) since[j] = pair_at(factors + 2 * kChunk + j * 8);
       const F2 keep = f2_both(factors[5 * kChunk - 2 * t]);
+      barrier<64>(pair_id);
+      barrier_arrive<kShare>(written_id);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float4 f = reinterpret_cast<const float4*>(exchange + E::kWritten)[j * 32 + lane];
+        set_rows(u[j], f2_mul(f2_pack(f.x, f.y), since[j]), f2_mul(f2_pack(f.z, f.w), since[j]));
+      }
       float u0, u1, z[kHalf / 8][4];
       row_scales<8>(u, u0, u1);
       const F2 up0 = f2_both(u0), up1 = f2_both(u1);
-      const uint32_t columns = keys + ((m & 1) * 2 + (m >> 1)) * 128 + r * 16;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        uint32_t hi[4], lo[4], b[kSteps / 2][4];
+        uint32_t hi[4], lo[4];
+        if (k < 3) load_columns(b[(k + 1) & 1], k + 1, 0);
         operand(u[2 * k], u[2 * k + 1], up0, up1, hi, lo);
-#pragma unroll
-        for (int j = 0; j < kSteps / 2; ++j) ldmatrix_t(b[j], columns + (k * kSteps + j) * kBlock);
-        mma_row<kHalf / 8>(z, hi, b, k == 0);
-        mma_row<kHalf / 8>(z, lo, b);
+        mma_row<kHalf / 8>(z, hi, b[k & 1], k == 0);
+        mma_row<kHalf / 8>(z, lo, b[k & 1]);
         if constexpr (Parts<T>::kKey == 2) {
-#pragma unroll
-          for (int j = 0; j < kSteps / 2; ++j) ldmatrix_t(b[j], columns + kKeyPart + (k * kSteps + j) * kBlock);
-          mma_row<kHalf / 8>(z, hi, b);
+          load_columns(b[k & 1], k, 1);
+          mma_row<kHalf / 8>(z, hi, b[k & 1]);
         }
       }
       const F2 down0 = f2_both(inverse_of_power(u0)), down1 = f2_both(inverse_of_power(u1));
@@ -980,7 +1026,7 @@ cudaError_t run(const DeltaParams& p, cudaStream_t stream) {
   int slices = most < 2 ? most : 2;
   if (most > 2 && 3 * rounds(4) < 2 * rounds(2)) slices = most < 4 ? most : 4;
   while (slices > 1 && smem_of(slices, 2) > kMostSmem) --slices;
-  const int stages = smem_of(slices, 2) <= kMostSmem ? 2 : 1;
+  const int stages = smem_of(slices, 3) <= kMostSmem ? 3 : smem_of(slices, 2) <= kMostSmem ? 2 : 1;
   const long long blocks = blocks_of(slices);
   if (blocks > 0x7fffffffll) return cudaErrorInvalidConfiguration;
   const bool values_whole = p.V % (16 / int(sizeof(T))) == 0 && eights<T>(p.v, p.v_s) && eights<T>(p.y, p.y_s);
