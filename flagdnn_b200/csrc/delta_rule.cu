@@ -84,6 +84,12 @@ __device__ __forceinline__ uint32_t high(float x, float y) {
   const __half2 h = __floats2half2_rn(x, y);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
+// The largest of m, |x| and |y| (NaN is passed over).
+__device__ __forceinline__ float most_of(float m, float x, float y) {
+  float r;
+  asm("max.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(m), "f"(x), "f"(y));
+  return r;
+}
 __device__ __forceinline__ float quad_max(float v) {
   v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
   return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
@@ -91,14 +97,14 @@ __device__ __forceinline__ float quad_max(float v) {
 // The scales of an accumulator block's two rows (lane / 4, + 8).
 template <int TILES>
 __device__ __forceinline__ void row_scales(const float (&c)[TILES][4], float& lower, float& upper) {
-  float m0 = 0.0f, m1 = 0.0f;
+  float m[2][2] = {};
 #pragma unroll
   for (int i = 0; i < TILES; ++i) {
-    m0 = fmaxf(m0, fmaxf(fabsf(c[i][0]), fabsf(c[i][1])));
-    m1 = fmaxf(m1, fmaxf(fabsf(c[i][2]), fabsf(c[i][3])));
+    m[0][i & 1] = most_of(m[0][i & 1], c[i][0], c[i][1]);
+    m[1][i & 1] = most_of(m[1][i & 1], c[i][2], c[i][3]);
   }
-  lower = raise(quad_max(m0));
-  upper = raise(quad_max(m1));
+  lower = raise(quad_max(fmaxf(m[0][0], m[0][1])));
+  upper = raise(quad_max(fmaxf(m[1][0], m[1][1])));
 }
 // The two rows of an accumulator tile, as pairs.
 __device__ __forceinline__ F2 first_row(const float (&c)[4]) { return f2_pack(c[0], c[1]); }
@@ -616,13 +622,16 @@ template <typename T, int KEYS, int SLICES, bool WHOLE>
 __global__ void __launch_bounds__((2 + outs_of(SLICES)) * SLICES * 32, 1)
 delta_chunks_kernel(const DeltaParams p, int blocks_a_head, int stages, uint32_t* status, long long wait_limit) {
   extern __shared__ __align__(128) uint8_t smem_raw[];
-  __shared__ uint64_t full[kMostStages];
+  __shared__ uint64_t full[kMostStages], empty[kMostStages];   // a stage's operands have landed; all warps are done with them
   __shared__ uint32_t abort_word;
   using W = Work<T, KEYS>;
   using E = Exchange<T, KEYS>;
   constexpr int kKeyPart = kChunk * KEYS * 2, kHalf = KEYS / 2, kSteps = KEYS / 16, kOuts = outs_of(SLICES), kShare = 64 + 32 * kOuts;
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kMostStages; ++i) mbar_init(&full[i], 1);
+    for (int i = 0; i < kMostStages; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], blockDim.x / 32);
+    }
     abort_word = 0;
     fence_barrier_init();
   }
@@ -642,50 +651,61 @@ delta_chunks_kernel(const DeltaParams p, int blocks_a_head, int stages, uint32_t
   const int slice = outputs ? (warp - 2 * slices) / kOuts : warp >> 1, half = warp & 1;
   const int row0 = first + slice * 16, channels = min(16, p.V - row0);
   uint8_t* const exchange = smem_raw + stages * stage_bytes + slice * E::kBytes;
-  const int pair_id = 1 + slice, state_id = 1 + kMostSlices + slice, written_id = 1 + 2 * kMostSlices + slice;   // named barriers
-  // All threads, at the top of chunk c: it is there, and all are done with chunk c - 1.
+  // named barriers of the slice's own: slices run at their own pace, `stages` chunks apart at most
+  const int top_id = slice, pair_id = kMostSlices + slice, state_id = 2 * kMostSlices + slice, written_id = 3 * kMostSlices + slice;
+  // The slice's warps, at the top of chunk c: it is there, and they are done with chunk c - 1.
   auto arrive_at = [&](int c) {
-    __syncthreads();
+    barrier<kShare>(top_id);
     mbar_wait_warp(&full[c % stages], uint32_t(c / stages) & 1u, &abort_word, status, kIncidentDeltaWait, wait_limit);
+  };
+  auto leave = [&](int c) {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&empty[c % stages]);
   };
 
   if (outputs) {
-    // ---- y, and the copies: chunk c + stages - 1 is asked for at chunk c, where there is room for more than one
-    const int tid = threadIdx.x - 2 * slices * 32, step = kOuts * slices * 32;
+    // ---- y, and the copies, stages - 1 chunks ahead: the first of these warps asks for the operands of all, each for its slice's values
+    const int tid = kOuts == 2 ? threadIdx.x & 63 : lane;
+    constexpr int kStep = 32 * kOuts;
+    const bool loader = threadIdx.x == 2u * slices * 32;
     const uint8_t* keys_from = w.keys + (n * p.G + h / (p.H / p.G)) * w.chunks * (2ll * W::kKeyBytes);
     const uint8_t* heads_from = w.heads + (n * p.H + h) * w.chunks * (long long)W::kHeadBytes;
-    const T* v0 = static_cast<const T*>(p.v) + n * p.v_s[0] + h * p.v_s[2] + first * p.v_s[3];
+    const T* v0 = static_cast<const T*>(p.v) + n * p.v_s[0] + h * p.v_s[2] + row0 * p.v_s[3];
+    int asked = 0;   // chunks, by the loader
     auto ask = [&](int c) {
       uint8_t* const to = smem_raw + (c % stages) * stage_bytes;
-      if (tid == 0) {
+      if (loader && asked == c) {
         uint64_t* bar = &full[c % stages];
-        mbar_arrive_expect_tx(bar, W::kStage);
-        bulk_load_1d(to, keys_from + c * (2ll * W::kKeyBytes), 2 * W::kKeyBytes, bar);
-        bulk_load_1d(to + 2 * W::kKeyBytes, heads_from + c * (long long)W::kHeadBytes, W::kHeadBytes, bar);
+        if (c < stages || mbar_wait_bounded(&empty[c % stages], uint32_t(c / stages - 1) & 1u, &abort_word, status, kIncidentDeltaWait, wait_limit)) {
+          mbar_arrive_expect_tx(bar, W::kStage);
+          bulk_load_1d(to, keys_from + c * (2ll * W::kKeyBytes), 2 * W::kKeyBytes, bar);
+          bulk_load_1d(to + 2 * W::kKeyBytes, heads_from + c * (long long)W::kHeadBytes, W::kHeadBytes, bar);
+          ++asked;
+        }
       }
-      const int here = min(slices * 16, p.V - first), tokens = min(end - c * kChunk, kChunk);
+      __syncwarp();
+      const int tokens = min(end - c * kChunk, kChunk);
+      uint8_t* const values = to + W::kStage + slice * 16 * int(sizeof(T));
       if constexpr (WHOLE) {
-        constexpr int kV = 16 / sizeof(T);
-        const int pieces = slices * 16 / kV;   // a thread keeps its column: `step` is a multiple of it
-        const int at = tid % pieces * kV, bytes = min(max(here - at, 0), kV) * int(sizeof(T));
-        const uint32_t values = smem_u32(to + W::kStage) + at * int(sizeof(T));
+        constexpr int kV = 16 / sizeof(T), kPieces = 16 / kV;
+        const int at = tid % kPieces * kV, bytes = at < channels ? 16 : 0;
+        const uint32_t first_row = smem_u32(values) + at * int(sizeof(T));
 #pragma unroll 4
-        for (int i = tid / pieces; i < kChunk; i += step / pieces) {
+        for (int i = tid / kPieces; i < kChunk; i += kStep / kPieces) {
           const bool there = i < tokens && bytes > 0;
-          copy16(values + i * pitch, there ? v0 + ((long long)c * kChunk + i) * p.v_s[1] + at : v0, there ? bytes : 0);
+          copy16(first_row + i * pitch, there ? v0 + ((long long)c * kChunk + i) * p.v_s[1] + at : static_cast<const T*>(p.v), there ? bytes : 0);
         }
       } else {
-        T* values = reinterpret_cast<T*>(to + W::kStage);
-        for (int i = tid; i < kChunk * slices * 16; i += step) {
-          const int row = i / (slices * 16), at = i % (slices * 16);
-          values[row * (pitch / int(sizeof(T))) + at] =
-              row < tokens && at < here ? v0[((long long)c * kChunk + row) * p.v_s[1] + at * p.v_s[3]] : from_f32<T>(0.0f);
+        for (int i = tid; i < kChunk * 16; i += kStep) {
+          const int row = i / 16, at = i % 16;
+          reinterpret_cast<T*>(values + row * pitch)[at] =
+              row < tokens && at < channels ? v0[((long long)c * kChunk + row) * p.v_s[1] + at * p.v_s[3]] : from_f32<T>(0.0f);
         }
       }
       async_commit();
     };
     T* y = static_cast<T*>(p.y) + n * p.y_s[0] + h * p.y_s[2] + row0 * p.y_s[3];
-    for (int c = 0; c < max(1, stages - 1); ++c) {
+    for (int c = 0; c < stages - 1; ++c) {
       if (c < chunks) ask(c);
       else async_commit();
     }
@@ -693,10 +713,8 @@ delta_chunks_kernel(const DeltaParams p, int blocks_a_head, int stages, uint32_t
       if (stages == 3) async_wait<1>();   // (a thread's groups: one a chunk, empty ones behind the last)
       else async_wait<0>();
       arrive_at(c);
-      if (stages > 1) {
-        if (c + stages - 1 < chunks) ask(c + stages - 1);
-        else async_commit();
-      }
+      if (c + stages - 1 < chunks) ask(c + stages - 1);
+      else async_commit();
       const uint8_t* const base = smem_raw + (c % stages) * stage_bytes;
       // this warp's tokens: all of the chunk's, or its first or last 32
       constexpr int kTiles = 8 / kOuts;
@@ -794,17 +812,14 @@ delta_chunks_kernel(const DeltaParams p, int blocks_a_head, int stages, uint32_t
       uint8_t* const stage = exchange + E::kStage + tile0 * 256;
       const int token = c * kChunk + tile0 * 8;
       put_outputs<T, WHOLE, kTiles / 2>(p, y + (long long)token * p.y_s[1], o, stage, end - token, channels);
-      if (stages == 1) {
-        __syncthreads();
-        if (c + 1 < chunks) ask(c + 1);
-      }
+      leave(c);
     }
     // tokens behind the row's end
     for (long long i = end * 16ll + (kOuts == 2 ? (warp & 1) * 32 : 0) + lane; i < p.L * 16ll; i += 32 * kOuts)
       if (i % 16 < channels) y[i / 16 * p.y_s[1] + i % 16 * p.y_s[3]] = from_f32<T>(0.0f);
-    if (*static_cast<volatile uint32_t*>(&abort_word) != 0 && tid == 0) {   // after an incident: give the copies in flight time to land
+    if (loader && *static_cast<volatile uint32_t*>(&abort_word) != 0) {   // after an incident: give the copies in flight time to land
       volatile uint32_t never = 0;
-      for (int c = max(0, chunks - stages); c < chunks; ++c)
+      for (int c = max(0, asked - stages); c < asked; ++c)
         mbar_wait_bounded(&full[c % stages], uint32_t(c / stages) & 1u, &never, status, kIncidentDrainWait, kWaitLimitCycles / 16);
     }
     return;
@@ -893,7 +908,7 @@ delta_chunks_kernel(const DeltaParams p, int blocks_a_head, int stages, uint32_t
     {
       const int own[2] = {half, 3 - half};
       const uint32_t rows[2] = {solve + lower_block(own[0], 0) * kBlock, solve + lower_block(own[1], 0) * kBlock};
-      float z[2][2][4], r0, r1;
+      float z[2][2][4], z2[2][2][4], r0, r1;
       uint32_t b[2][4], bl[2][4];
       auto load = [&](int i, int k) {
         ldmatrix(b[i], rows[i] + k * kBlock);
@@ -910,7 +925,10 @@ delta_chunks_kernel(const DeltaParams p, int blocks_a_head, int stages, uint32_t
           else mma(z[i][j], hi, b[i][2 * j], b[i][2 * j + 1]);
         }
 #pragma unroll
-        for (int j = 0; j < 2; ++j) mma(z[i][j], lo, b[i][2 * j], b[i][2 * j + 1]);
+        for (int j = 0; j < 2; ++j) {
+          if (k == 0) mma_first(z2[i][j], lo, b[i][2 * j], b[i][2 * j + 1]);
+          else mma(z2[i][j], lo, b[i][2 * j], b[i][2 * j + 1]);
+        }
 #pragma unroll
         for (int j = 0; j < 2; ++j) mma(z[i][j], hi, bl[i][2 * j], bl[i][2 * j + 1]);
       };
@@ -931,7 +949,8 @@ delta_chunks_kernel(const DeltaParams p, int blocks_a_head, int stages, uint32_t
           const int tile = 2 * own[i] + j;
           const F2 f = pair_at(factors + 3 * kChunk + tile * 8);
           float out[4];
-          set_rows(out, f2_mul(f, f2_mul(first_row(z[i][j]), down0)), f2_mul(f, f2_mul(second_row(z[i][j]), down1)));
+          set_rows(out, f2_mul(f, f2_mul(f2_add(first_row(z[i][j]), first_row(z2[i][j])), down0)),
+                   f2_mul(f, f2_mul(f2_add(second_row(z[i][j]), second_row(z2[i][j])), down1)));
           reinterpret_cast<float4*>(exchange + E::kWritten)[tile * 32 + lane] = make_float4(out[0], out[1], out[2], out[3]);
         }
     }
@@ -975,7 +994,7 @@ delta_chunks_kernel(const DeltaParams p, int blocks_a_head, int stages, uint32_t
       for (int j = 0; j < kHalf / 8; ++j)
         set_rows(s[j], f2_fma(keep, first_row(s[j]), f2_mul(first_row(z[j]), down0)), f2_fma(keep, second_row(s[j]), f2_mul(second_row(z[j]), down1)));
     }
-    if (stages == 1) __syncthreads();
+    leave(c);
   }
 
   if (p.final_state != nullptr) {
@@ -1026,7 +1045,8 @@ cudaError_t run(const DeltaParams& p, cudaStream_t stream) {
   int slices = most < 2 ? most : 2;
   if (most > 2 && 3 * rounds(4) < 2 * rounds(2)) slices = most < 4 ? most : 4;
   while (slices > 1 && smem_of(slices, 2) > kMostSmem) --slices;
-  const int stages = smem_of(slices, 3) <= kMostSmem ? 3 : smem_of(slices, 2) <= kMostSmem ? 2 : 1;
+  const int stages = smem_of(slices, 3) <= kMostSmem ? 3 : 2;
+  static_assert(2 * (Work<T, KEYS>::kStage + kChunk * value_pitch<T>(1)) + Exchange<T, KEYS>::kBytes <= kMostSmem, "one slice has two stages");
   const long long blocks = blocks_of(slices);
   if (blocks > 0x7fffffffll) return cudaErrorInvalidConfiguration;
   const bool values_whole = p.V % (16 / int(sizeof(T))) == 0 && eights<T>(p.v, p.v_s) && eights<T>(p.y, p.y_s);
