@@ -287,22 +287,33 @@ __device__ __forceinline__ void dots(float (&c)[8][4], const uint8_t* x, const u
 }
 
 // Sums of a head's log2 decays and its step sizes, by one warp, two tokens a lane.
+struct RawGates {
+  float delta[2], beta[2], A, bias;
+};
 template <typename T>
-__device__ __forceinline__ void sum_gates(const DeltaParams& p, HeadGates& to, long long n, int begin, int tokens, int h) {
+__device__ __forceinline__ void load_gates(const DeltaParams& p, RawGates& x, long long n, int begin, int tokens, int h) {
+  x.A = p.A != nullptr ? p.A[h] : 1.0f;
+  x.bias = p.delta_bias != nullptr ? p.delta_bias[h] : 0.0f;
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int i = 2 * (threadIdx.x & 31) + j;
+    x.delta[j] = x.beta[j] = 0.0f;
+    if (i < tokens) {
+      x.delta[j] = gate_at<T>(p, p.delta, n * p.delta_s[0] + (begin + i) * p.delta_s[1] + h * p.delta_s[2]);
+      x.beta[j] = gate_at<T>(p, p.beta, n * p.beta_s[0] + (begin + i) * p.beta_s[1] + h * p.beta_s[2]);
+    }
+  }
+}
+__device__ __forceinline__ void sum_gates(const DeltaParams& p, const RawGates& x, HeadGates& to, int tokens) {
   const int lane = threadIdx.x & 31;
-  const float A = p.A != nullptr ? p.A[h] : 1.0f, bias = p.delta_bias != nullptr ? p.delta_bias[h] : 0.0f;
   double v[2];
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
     const int i = 2 * lane + j;
-    float g = 0.0f, b = 0.0f;
-    if (i < tokens) {
-      g = log_decay(p, gate_at<T>(p, p.delta, n * p.delta_s[0] + (begin + i) * p.delta_s[1] + h * p.delta_s[2]), bias, A);
-      b = step_size(p, gate_at<T>(p, p.beta, n * p.beta_s[0] + (begin + i) * p.beta_s[1] + h * p.beta_s[2]));
-      g = g < -1e5f ? -1e5f : g;   // a decay of zero, whose difference to itself is a number; NaN stays
-    }
+    float g = log_decay(p, x.delta[j], x.bias, x.A);
+    g = i < tokens ? (g < -1e5f ? -1e5f : g) : 0.0f;   // a decay of zero, whose difference to itself is a number; NaN stays
     v[j] = double(g) * 1.4426950408889634;
-    to.beta[i] = b;
+    to.beta[i] = i < tokens ? step_size(p, x.beta[j]) : 0.0f;
   }
   double sum = v[0] + v[1];
 #pragma unroll
@@ -418,27 +429,28 @@ delta_prepare_kernel(const DeltaParams p) {
   {
     const T* kp = static_cast<const T*>(p.k) + n * p.k_s[0] + begin * p.k_s[1] + g * p.k_s[2];
     const T* qp = static_cast<const T*>(p.q) + n * p.q_s[0] + begin * p.q_s[1] + g * p.q_s[2];
+    RawGates gates;
+    if (warp < group) load_gates<T>(p, gates, n, begin, tokens, h0 + warp);
     Rows<T, KEYS, WHOLE> rows;
     rows.load(kp, p.k_s, tokens, p.K);
     if constexpr (sizeof(T) == 2 && WHOLE) {   // (the queries' registers, too)
       Rows<T, KEYS, WHOLE> more;
       more.load(qp, p.q_s, tokens, p.K);
-      if (warp < group) sum_gates<T>(p, s.gates[warp], n, begin, tokens, h0 + warp);
+      if (warp < group) sum_gates(p, gates, s.gates[warp], tokens);
       rows.stage(s.keys, s.key_scale, tokens, p.norm, 1.0f);
       more.stage(queries, s.query_scale, tokens, p.norm, p.scale);
     } else {
-      if (warp < group) sum_gates<T>(p, s.gates[warp], n, begin, tokens, h0 + warp);
+      if (warp < group) sum_gates(p, gates, s.gates[warp], tokens);
       rows.stage(s.keys, s.key_scale, tokens, p.norm, 1.0f);
       rows.load(qp, p.q_s, tokens, p.K);
       rows.stage(queries, s.query_scale, tokens, p.norm, p.scale);
     }
   }
+  fence_proxy_async_smem();
   __syncthreads();
-  {
-    uint4* to = reinterpret_cast<uint4*>(w.keys + ((n * p.G + g) * w.chunks + c) * (2ll * W::kKeyBytes));
-    const uint4* from = reinterpret_cast<const uint4*>(s.keys);
-#pragma unroll 4
-    for (int i = tid; i < 2 * W::kKeyBytes / 16; i += kPrepThreads) to[i] = from[i];
+  if (tid == 0) {
+    bulk_store_1d(w.keys + ((n * p.G + g) * w.chunks + c) * (2ll * W::kKeyBytes), s.keys, 2 * W::kKeyBytes);
+    bulk_commit_group();
   }
   float kk[8][4] = {}, qk[8][4] = {};
   dots<T, KEYS>(kk, s.keys, s.keys, warp);
@@ -453,11 +465,16 @@ delta_prepare_kernel(const DeltaParams p) {
       qk[m][0] *= q0 * f.x, qk[m][1] *= q0 * f.y, qk[m][2] *= q1 * f.x, qk[m][3] *= q1 * f.y;
     }
   }
+  if (tid == 0) bulk_wait_group_read0();
   __syncthreads();   // the operands' place is taken by a and t
 
   for (int i = 0; i < group; ++i) {
     if (i > 0 && (i & 3) == 0) {
-      if (i + warp < group) sum_gates<T>(p, s.gates[warp], n, begin, tokens, h0 + i + warp);
+      if (i + warp < group) {
+        RawGates raw;
+        load_gates<T>(p, raw, n, begin, tokens, h0 + i + warp);
+        sum_gates(p, raw, s.gates[warp], tokens);
+      }
       __syncthreads();
     }
     const HeadGates& gates = s.gates[i & 3];
@@ -545,6 +562,7 @@ delta_prepare_kernel(const DeltaParams p) {
     }
     __syncthreads();
   }
+  if (tid == 0) bulk_wait_group0();
 }
 
 // ---- the chunks in order -------------------------------------------------------------------------------------------
