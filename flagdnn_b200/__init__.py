@@ -35,7 +35,7 @@ from .graph import (  # noqa: F401
 )
 from .ops import (  # noqa: F401
     adaptive_avg_pool2d, add, bias_add, causal_conv1d, causal_conv1d_step, conv1d, conv2d, gated_delta_rule,
-    gated_delta_rule_step, gelu, group_norm, group_norm_backward, max_pool2d, mm, mul, relu, selective_scan, selective_scan_step, sub,
+    gated_delta_rule_step, gelu, group_norm, group_norm_backward, max_pool2d, mm, mm_bias_act, mul, relu, selective_scan, selective_scan_step, sub,
 )
 
 __version__ = "0.1.0"

@@ -64,6 +64,8 @@ EXPORTED_SYMBOLS = (
     "fdnn_gated_delta_rule_workspace_bytes",
     "fdnn_gated_delta_rule_fwd",
     "fdnn_gated_delta_rule_step",
+    "fdnn_mm_rows_preferred",
+    "fdnn_mm_rows_fwd",
 )
 
 
@@ -149,6 +151,11 @@ class DeltaRuleDesc(ctypes.Structure):
                [("delta_strides", ctypes.c_int64 * 3), ("beta_strides", ctypes.c_int64 * 3)]
 
 
+class MmDesc(ctypes.Structure):
+    _fields_ = [(name, ctypes.c_int32) for name in ("dtype", "m", "n", "k", "activation", "reserved")] + \
+               [(name, ctypes.c_int64 * 2) for name in ("a_strides", "b_strides", "residual_strides", "y_strides")]
+
+
 class NativeError(RuntimeError):
     """A non-OK status that maps to RuntimeError in the reference's convention."""
 
@@ -204,7 +211,7 @@ def load() -> ctypes.CDLL:
     lib.fdnn_debug_set_wait_limit.argtypes = [i64, i32]
     lib.fdnn_debug_tensor_map_counters.restype = i32
     lib.fdnn_debug_tensor_map_counters.argtypes = [ctypes.POINTER(ctypes.c_int64), ctypes.POINTER(ctypes.c_int64)]
-    pi64, pnorm, pconv, pscan, pdelta = (ctypes.POINTER(t) for t in (i64, NormDesc, CausalConvDesc, ScanDesc, DeltaRuleDesc))
+    pi64, pnorm, pconv, pscan, pdelta, pmm = (ctypes.POINTER(t) for t in (i64, NormDesc, CausalConvDesc, ScanDesc, DeltaRuleDesc, MmDesc))
     for name, args in (
         ("fdnn_group_norm_workspace_bytes", [pnorm, i32, pi64]),
         ("fdnn_group_norm_fwd", [pnorm] + [vp] * 7 + [i64, vp]),
@@ -217,6 +224,8 @@ def load() -> ctypes.CDLL:
         ("fdnn_gated_delta_rule_workspace_bytes", [pdelta, pi64]),
         ("fdnn_gated_delta_rule_fwd", [pdelta] + [vp] * 12 + [i64, vp]),
         ("fdnn_gated_delta_rule_step", [pdelta] + [vp] * 8 + [i32] + [vp] * 3),
+        ("fdnn_mm_rows_preferred", [pmm, ctypes.POINTER(ctypes.c_int32)]),
+        ("fdnn_mm_rows_fwd", [pmm] + [vp] * 6),
     ):
         fn = getattr(lib, name)
         fn.restype, fn.argtypes = i32, args

@@ -284,6 +284,8 @@ def _load_fast() -> Any:
             _fastcall.bind_delta_rule(*(ctypes.cast(f, ctypes.c_void_p).value for f in (
                 lib.fdnn_gated_delta_rule_workspace_bytes, lib.fdnn_gated_delta_rule_fwd, lib.fdnn_gated_delta_rule_step)),
                 ctypes.sizeof(nat.DeltaRuleDesc))
+            _fastcall.bind_mm_rows(*(ctypes.cast(f, ctypes.c_void_p).value for f in (lib.fdnn_mm_rows_preferred, lib.fdnn_mm_rows_fwd)),
+                                   ctypes.sizeof(nat.MmDesc))
             _fast = _fastcall
         except (ImportError, AttributeError, TypeError) as exc:   # not built, or built against something else
             warnings.warn(f"flagdnn_b200: the native host path is not used, calls take some 15 us longer ({exc}); "
@@ -698,4 +700,85 @@ def mm(
     if out is not None and y is not out:
         out.copy_(y)
         return out
+    return y
+
+
+_MOST_ROWS = 1 << 22     # of a product to one call of fdnn_mm_rows_fwd
+
+
+def mm_bias_act(
+    input: torch.Tensor,
+    mat2: torch.Tensor,
+    bias: Optional[torch.Tensor] = None,
+    *,
+    residual: Optional[torch.Tensor] = None,
+    activation: str = "none",
+) -> torch.Tensor:
+    """``activation(input @ mat2 + bias + residual)``, summed in fp32 and rounded once: ``mm`` with the epilogue of
+    ``conv2d_bias_act``.  ``input`` [M, K] and ``mat2`` [K, N] may have any strides (a linear layer's weight [N, K] goes in as
+    ``weight.t()``), ``bias`` is [N], ``residual`` [M, N]; all fp16, bf16 or fp32.  Few rows are a reading of ``mat2`` by a kernel of
+    their own, more run as a 1x1 convolution.  It computes no gradients: tensors that ask for one are refused."""
+    if activation not in _ACTIVATIONS:
+        raise RuntimeError(f"activation must be one of {', '.join(_ACTIVATIONS)}, got {activation!r}")
+    act = _ACTIVATIONS[activation]
+    fast = _fast or _load_fast()
+    if fast and not _STREAM_K:
+        y = fast.mm_bias_act(input, mat2, bias, residual, act, _FORCED_ALGO)
+        if y.__class__ is int:
+            nat.check(y)
+        if y is not None:
+            return y
+    from .norm_host import _DTYPE_IDS, address, refuse_grad
+
+    what = "mm_bias_act"
+    for name, t in (("input", input), ("mat2", mat2)):
+        if t.dim() != 2:
+            raise RuntimeError(f"{what}: {name} must be a matrix, got {t.dim()} dimensions")
+    if input.shape[1] != mat2.shape[0]:
+        raise RuntimeError(f"{what}: shapes cannot be multiplied ({input.shape[0]}x{input.shape[1]} and {mat2.shape[0]}x{mat2.shape[1]})")
+    if input.dtype not in _DTYPE_IDS:
+        raise NotImplementedError(f"flag_dnn {what} does not support dtype={input.dtype}")
+    m, k = input.shape
+    n = mat2.shape[1]
+    if max(k, n) > 0x7fffffff - 1024 or m > 0x7fffffff:
+        raise RuntimeError(f"{what}: an extent is too large")
+    for name, t, shape in (("mat2", mat2, (k, n)), ("bias", bias, (n,)), ("residual", residual, (m, n))):
+        if t is None:
+            continue
+        if tuple(t.shape) != shape:
+            raise RuntimeError(f"{what}: {name} must have shape {shape}, got {tuple(t.shape)}")
+        if t.dtype != input.dtype:
+            raise RuntimeError(f"{what}: {name} must be {input.dtype}, got {t.dtype}")
+        if t.device != input.device:
+            raise RuntimeError(f"{what}: {name} must be on {input.device}, got {t.device}")
+    if any(t is not None and t.layout != torch.strided for t in (input, mat2, bias, residual)):
+        raise NotImplementedError(f"flag_dnn {what} supports dense strided tensors only")
+    if not input.is_cuda:
+        raise NotImplementedError(f"flag_dnn {what} CUDA implementation requires CUDA input")
+    refuse_grad(what, input, mat2, bias, residual)
+    y = torch.empty((m, n), dtype=input.dtype, device=input.device)
+    if y.numel() == 0:
+        return y
+    bias = None if bias is None else bias.contiguous()
+    lib = nat.load()
+    d = nat.MmDesc()
+    d.dtype, d.m, d.n, d.k, d.activation = _DTYPE_IDS[input.dtype], min(m, _MOST_ROWS), n, k, act
+    for field, t in ((d.a_strides, input), (d.b_strides, mat2), (d.residual_strides, residual), (d.y_strides, y)):
+        if t is not None:
+            field[0], field[1] = t.stride()
+    preferred = ctypes.c_int32()
+    nat.check(lib.fdnn_mm_rows_preferred(ctypes.byref(d), ctypes.byref(preferred)))
+    if preferred.value:
+        with torch.cuda.device(input.device):
+            for first in range(0, m, _MOST_ROWS):
+                rows = slice(first, first + _MOST_ROWS)
+                d.m = y[rows].shape[0]
+                nat.check(lib.fdnn_mm_rows_fwd(ctypes.byref(d), input[rows].data_ptr(), mat2.data_ptr(), address(bias),
+                                               None if residual is None else residual[rows].data_ptr(), y[rows].data_ptr(),
+                                               _current_stream(input.device)))
+        return y
+    if residual is not None and (not residual.is_contiguous() or residual.data_ptr() % 16 != 0):
+        residual = residual.clone(memory_format=torch.contiguous_format)     # the epilogue adds what lies as y does
+    _run(input.t().unsqueeze(0).unsqueeze(2), mat2.t().unsqueeze(-1).unsqueeze(-1), bias, None, (1, 1), (0, 0, 0, 0), (1, 1), 1, act,
+         None if residual is None else residual.t().unsqueeze(0).unsqueeze(2), out=y.t().unsqueeze(0).unsqueeze(2))
     return y

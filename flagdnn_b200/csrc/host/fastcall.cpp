@@ -303,7 +303,30 @@ PyObject* fast_conv1d(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// mm(a [M, K], b [K, N], algo): a 1x1 convolution over one row of M pixels whose filter is b transposed
+// A product a [M, K] b [K, N] as a 1x1 convolution over one row of M pixels whose filter is b transposed; y is dense.
+fdnn_conv_desc mm_desc(const at::Tensor& x, const at::Tensor& w, int dtype, int algo) {
+  const int64_t m = x.size(0), k = x.size(1), nn = w.size(1);
+  fdnn_conv_desc d;
+  std::memset(&d, 0, sizeof d);
+  d.dtype = dtype;
+  d.n = 1; d.c = int(k); d.h = 1; d.w = int(m);
+  d.k = int(nn); d.r = 1; d.s = 1;
+  d.stride_h = d.stride_w = d.dil_h = d.dil_w = 1;
+  d.groups = 1;
+  d.algo = algo;
+  d.x_strides[0] = d.x_strides[2] = m * x.stride(0);
+  d.x_strides[1] = x.stride(1);
+  d.x_strides[3] = x.stride(0);
+  d.w_strides[0] = w.stride(1);
+  d.w_strides[1] = w.stride(0);
+  d.w_strides[2] = d.w_strides[3] = 1;
+  d.y_strides[0] = d.y_strides[2] = m * nn;
+  d.y_strides[1] = 1;
+  d.y_strides[3] = nn;
+  return d;
+}
+
+// mm(a [M, K], b [K, N], algo)
 PyObject* fast_mm(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS   // C++ exceptions leave as the Python types torch gives them (torch.OutOfMemoryError among them)
   if (n != 3 || g_fwd_unpacked == nullptr) return none();
@@ -320,26 +343,79 @@ PyObject* fast_mm(PyObject*, PyObject* const* a, Py_ssize_t n) {
       WithoutGil free;
       y = at::empty({m, nn}, x->options().requires_grad(false));
     }
-    fdnn_conv_desc d;
-    std::memset(&d, 0, sizeof d);
-    d.dtype = dtype;
-    d.n = 1; d.c = int(k); d.h = 1; d.w = int(m);
-    d.k = int(nn); d.r = 1; d.s = 1;
-    d.stride_h = d.stride_w = d.dil_h = d.dil_w = 1;
-    d.groups = 1;
-    d.algo = int(algo);
-    d.x_strides[0] = d.x_strides[2] = m * x->stride(0);
-    d.x_strides[1] = x->stride(1);
-    d.x_strides[3] = x->stride(0);
-    d.w_strides[0] = w->stride(1);
-    d.w_strides[1] = w->stride(0);
-    d.w_strides[2] = d.w_strides[3] = 1;
-    d.y_strides[0] = d.y_strides[2] = m * nn;
-    d.y_strides[1] = 1;
-    d.y_strides[3] = nn;
-    const int st = launch(d, *x, *w, nullptr, nullptr, nullptr, nullptr, FDNN_ACT_NONE, y);
+    const int st = launch(mm_desc(*x, *w, dtype, int(algo)), *x, *w, nullptr, nullptr, nullptr, nullptr, FDNN_ACT_NONE, y);
     return finish(st, std::move(y));
   END_HANDLE_TH_ERRORS
+}
+
+using MmPreferredFn = int (*)(const fdnn_mm_desc*, int32_t*);
+using MmRowsFn = int (*)(const fdnn_mm_desc*, const void*, const void*, const void*, const void*, void*, void*);
+MmPreferredFn g_mm_preferred = nullptr;
+MmRowsFn g_mm_rows = nullptr;
+
+// mm_bias_act(a [M, K], b [K, N], bias, residual, activation, algo)
+PyObject* fast_mm_bias_act(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 6 || g_fwd_unpacked == nullptr || g_mm_rows == nullptr) return none();
+  const at::Tensor *x = plain(a[0]), *w = plain(a[1]), *bias, *residual;
+  if (x == nullptr || w == nullptr || !optional(a[2], &bias) || !optional(a[3], &residual) || x->dim() != 2 || w->dim() != 2) return none();
+  const int dtype = dtype_code(x->scalar_type());
+  if (dtype < 0 || w->scalar_type() != x->scalar_type() || w->device() != x->device()) return none();
+  const int64_t m = x->size(0), k = x->size(1), nn = w->size(1);
+  if (w->size(0) != k || m < 1 || k < 1 || nn < 1 || m > 1 << 22 || k > kMost - 1024 || nn > kMost - 1024) return none();
+  if (!dense(bias, x->scalar_type(), {nn}, *x)) return none();
+  if (residual != nullptr && (residual->scalar_type() != x->scalar_type() || residual->device() != x->device() || residual->dim() != 2 ||
+                              residual->size(0) != m || residual->size(1) != nn))
+    return none();
+  if (any_grad({x, w, bias, residual}) || !PyLong_CheckExact(a[4])) return none();
+  const int act = int(PyLong_AsLong(a[4]));
+  const int64_t algo = PyLong_AsLongLong(a[5]);
+  fdnn_mm_desc r;
+  std::memset(&r, 0, sizeof r);
+  r.dtype = dtype;
+  r.m = int(m);
+  r.n = int(nn);
+  r.k = int(k);
+  r.activation = act;
+  for (int i = 0; i < 2; ++i) {
+    r.a_strides[i] = x->stride(i);
+    r.b_strides[i] = w->stride(i);
+    if (residual != nullptr) r.residual_strides[i] = residual->stride(i);
+  }
+  r.y_strides[0] = nn;
+  r.y_strides[1] = 1;
+  int32_t preferred = 0;
+  int st = g_mm_preferred(&r, &preferred);
+  if (st != FDNN_OK) return PyLong_FromLong(st);
+  // (what the convolution's epilogue cannot add as it lies is made dense in Python)
+  if (!preferred && residual != nullptr && (!residual->is_contiguous() || reinterpret_cast<uintptr_t>(residual->const_data_ptr()) % 16 != 0))
+    return none();
+  c10::DeviceGuard guard(x->device());
+  at::Tensor y;
+  {
+    WithoutGil free;
+    y = at::empty({m, nn}, x->options().requires_grad(false));
+    if (preferred)
+      st = g_mm_rows(&r, x->const_data_ptr(), w->const_data_ptr(), ptr(bias), ptr(residual), y.mutable_data_ptr(), stream_of(*x));
+  }
+  if (preferred) return finish(st, std::move(y));
+  const fdnn_conv_desc d = mm_desc(*x, *w, dtype, int(algo));
+  st = launch(d, *x, *w, nullptr, ptr(bias), nullptr, ptr(residual), act, y);
+  return finish(st, std::move(y));
+  END_HANDLE_TH_ERRORS
+}
+
+// bind_mm_rows(addresses of fdnn_mm_rows_preferred and fdnn_mm_rows_fwd, the descriptor's size as the caller knows it)
+PyObject* bind_mm_rows(PyObject*, PyObject* args) {
+  unsigned long long preferred, rows, bytes;
+  if (!PyArg_ParseTuple(args, "KKK", &preferred, &rows, &bytes)) return nullptr;
+  if (bytes != sizeof(fdnn_mm_desc)) {
+    PyErr_SetString(PyExc_ImportError, "compiled for other descriptors of the C ABI");
+    return nullptr;
+  }
+  g_mm_preferred = reinterpret_cast<MmPreferredFn>(uintptr_t(preferred));
+  g_mm_rows = reinterpret_cast<MmRowsFn>(uintptr_t(rows));
+  return none();
 }
 
 // bind(query, pack, fwd: addresses of the C ABI's functions, packed_weight: callback, version of the loaded library and the
@@ -383,7 +459,9 @@ PyMethodDef kMethods[] = {
     {"selective_scan_step", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(fast_selective_scan_step)), METH_FASTCALL, nullptr},
     {"gated_delta_rule", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(fast_gated_delta_rule)), METH_FASTCALL, nullptr},
     {"gated_delta_rule_step", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(fast_gated_delta_rule_step)), METH_FASTCALL, nullptr},
+    {"mm_bias_act", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(fast_mm_bias_act)), METH_FASTCALL, nullptr},
     {"bind", bind, METH_VARARGS, nullptr},
+    {"bind_mm_rows", bind_mm_rows, METH_VARARGS, nullptr},
     {"bind_delta_rule", bind_delta_rule, METH_VARARGS, nullptr},
     {"bind_sequence", bind_sequence, METH_VARARGS, nullptr},
     {"bind_unpacked", bind_unpacked, METH_O, nullptr},

@@ -1,0 +1,259 @@
+// A product of few rows with its epilogue: y = act(a b + bias + residual).
+//
+// With one to some dozens of rows a product is a reading of b.  A block takes 64 columns of b and, with the others of its cluster, a share
+// of the reduction; b's tiles come through a ring of asynchronous copies, all of a block's first ones on their way at once.  On the tensor
+// cores columns are the M side (16 a warp) and rows the N side (8 at a time), so that a single row fills an eighth of an
+// instruction and not a 128th.  The blocks of a cluster add up their sums through each other's shared memory, in their order, and finish
+// a share of the columns each: no workspace, no atomics.
+//
+// Sums are fp32; fp32 operands go in as 3 x TF32 (a high part, cut to TF32, and what it leaves: 2^-21); one rounding at the end.
+#include "group_norm.cuh"
+#include "mm_rows.h"
+
+namespace fdnn {
+namespace {
+
+constexpr int kThreads = 128;
+constexpr int kCols = 64;                 // columns of b to a block, 16 a warp
+constexpr int kTileBytes = 128;           // of the reduction, a step of the ring
+constexpr int kPitch = kTileBytes + 16;   // eight rows of 16 bytes lie in different banks
+constexpr int kColTile = kCols * kPitch;  // bytes of a tile of b, in either order
+// Steps of the ring: some 90 KB, two blocks to an SM.
+__host__ __device__ constexpr int stages_of(int rows) { return rows <= 16 ? 8 : rows <= 32 ? 6 : 5; }
+
+__device__ __forceinline__ void copy16(uint32_t to, const void* from, int bytes) {   // the rest of the 16 is zeros
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copy4(uint32_t to, const void* from, bool there) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(from), "r"(there ? 4 : 0) : "memory");
+}
+template <bool TRANS>
+__device__ __forceinline__ void ldmatrix(uint32_t (&r)[4], uint32_t at) {
+  if constexpr (TRANS)
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+  else
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+template <typename T>
+__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (std::is_same<T, __half>::value)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else if constexpr (std::is_same<T, __nv_bfloat16>::value)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// fp32 as a TF32 number and the rest.
+__device__ __forceinline__ void two_parts(float v, uint32_t& hi, uint32_t& lo) {
+  hi = __float_as_uint(v) & 0xffffe000u;
+  lo = __float_as_uint(v - __uint_as_float(hi));
+}
+__device__ __forceinline__ float cluster_f32(uint32_t at) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+  return v;
+}
+
+enum class Order { kReduction, kColumns, kAny };   // what lies together in b, in 16-byte pieces; kAny: value by value
+
+// ROWS: of a, 16, 32 or 64 to a block.  A_WHOLE: 16 bytes of a row of a are copied at once.
+template <typename T, int ROWS, Order ORDER, bool A_WHOLE>
+__global__ void __launch_bounds__(kThreads)
+mm_rows_kernel(const MmRowsParams p, int split) {
+  extern __shared__ __align__(128) uint8_t smem_raw[];
+  chained();
+  constexpr int kV = 16 / int(sizeof(T)), kStep = kTileBytes / int(sizeof(T)), kStages = stages_of(ROWS);
+  constexpr int kStage = kColTile + ROWS * kPitch;
+  // columns together: rows of 64 columns, a step of the reduction apart
+  constexpr int kColPitch = ORDER == Order::kColumns ? kCols * int(sizeof(T)) + (sizeof(T) == 2 ? 16 : 32) : kPitch;
+  static_assert(ORDER != Order::kColumns || kStep * kColPitch <= kColTile, "fits the tile's place");
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3, m = lane >> 3, r = lane & 7;
+  const int rank = int(blockIdx.x % split), col0 = int(blockIdx.x / split) * kCols, row0 = int(blockIdx.y) * ROWS;
+  const int steps = (p.K + kStep - 1) / kStep;
+  const int from = int((long long)steps * rank / split), to = int((long long)steps * (rank + 1) / split);
+  const uint32_t smem = smem_u32(smem_raw);
+  const T *a0 = static_cast<const T*>(p.a) + row0 * p.a_s[0], *b0 = static_cast<const T*>(p.b) + col0 * p.b_s[1];
+
+  auto ask = [&](int step) {
+    if (step < to) {
+      const int at = (step - from) % kStages * kStage, k0 = step * kStep;
+      if constexpr (ORDER == Order::kReduction) {
+#pragma unroll
+        for (int i = tid; i < kCols * 8; i += kThreads) {
+          const int c = i / 8, k = k0 + i % 8 * kV;
+          const bool there = col0 + c < p.N && k < p.K;
+          copy16(smem + at + c * kPitch + i % 8 * 16, there ? b0 + c * p.b_s[1] + k : b0, there ? 16 : 0);
+        }
+      } else if constexpr (ORDER == Order::kColumns) {
+        constexpr int kPieces = kCols / kV;
+#pragma unroll
+        for (int i = tid; i < kStep * kPieces; i += kThreads) {
+          const int k = i / kPieces, c = i % kPieces * kV;
+          const bool there = col0 + c < p.N && k0 + k < p.K;
+          copy16(smem + at + k * kColPitch + i % kPieces * 16, there ? b0 + (k0 + k) * p.b_s[0] + c : b0, there ? 16 : 0);
+        }
+      } else {
+        const bool along = p.b_s[0] != 1;   // threads side by side along what lies together
+#pragma unroll 8
+        for (int i = tid; i < kCols * kStep; i += kThreads) {
+          const int c = along ? i % kCols : i / kStep, k = along ? i / kCols : i % kStep;
+          const bool there = col0 + c < p.N && k0 + k < p.K;
+          const T* src = there ? b0 + c * p.b_s[1] + (k0 + k) * p.b_s[0] : b0;
+          if constexpr (sizeof(T) == 4) copy4(smem + at + c * kPitch + k * 4, src, there);
+          else reinterpret_cast<T*>(smem_raw + at + c * kPitch)[k] = there ? *src : from_f32<T>(0.0f);
+        }
+      }
+      const int a_at = at + kColTile;
+      if constexpr (A_WHOLE) {
+#pragma unroll
+        for (int i = tid; i < ROWS * 8; i += kThreads) {
+          const int row = i / 8, k = k0 + i % 8 * kV;
+          const bool there = row0 + row < p.M && k < p.K;
+          copy16(smem + a_at + row * kPitch + i % 8 * 16, there ? a0 + row * p.a_s[0] + k : static_cast<const T*>(p.a), there ? 16 : 0);
+        }
+      } else {
+#pragma unroll 4
+        for (int i = tid; i < ROWS * kStep; i += kThreads) {
+          const int row = i / kStep, k = i % kStep;
+          const bool there = row0 + row < p.M && k0 + k < p.K;
+          const T* src = there ? a0 + row * p.a_s[0] + (k0 + k) * p.a_s[1] : static_cast<const T*>(p.a);
+          if constexpr (sizeof(T) == 4) copy4(smem + a_at + row * kPitch + k * 4, src, there);
+          else reinterpret_cast<T*>(smem_raw + a_at + row * kPitch)[k] = there ? *src : from_f32<T>(0.0f);
+        }
+      }
+    }
+    async_commit();
+  };
+
+  float d[ROWS / 8][4] = {};
+#pragma unroll
+  for (int i = 0; i < kStages - 1; ++i) ask(from + i);
+  for (int step = from; step < to; ++step) {
+    async_wait<kStages - 2>();
+    __syncthreads();
+    ask(step + kStages - 1);
+    const int at = (step - from) % kStages * kStage;
+    if constexpr (sizeof(T) == 2) {
+      const uint32_t cols = smem + at, rows = smem + at + kColTile;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        uint32_t a[4];
+        if constexpr (ORDER == Order::kColumns) ldmatrix<true>(a, cols + (k * 16 + (m >> 1) * 8 + r) * kColPitch + (warp * 16 + (m & 1) * 8) * 2);
+        else ldmatrix<false>(a, cols + (warp * 16 + (m & 1) * 8 + r) * kPitch + (k * 16 + (m >> 1) * 8) * 2);
+#pragma unroll
+        for (int j = 0; j < ROWS / 16; ++j) {
+          uint32_t b[4];
+          ldmatrix<false>(b, rows + (j * 16 + (m >> 1) * 8 + r) * kPitch + (k * 16 + (m & 1) * 8) * 2);
+          mma<T>(d[2 * j], a, b[0], b[1]);
+          mma<T>(d[2 * j + 1], a, b[2], b[3]);
+        }
+      }
+    } else {
+      const float *cols = reinterpret_cast<const float*>(smem_raw + at), *rows = reinterpret_cast<const float*>(smem_raw + at + kColTile);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        uint32_t a[4], al[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int c = warp * 16 + g + (i & 1) * 8, kk = k * 8 + t + (i >> 1) * 4;
+          two_parts(ORDER == Order::kColumns ? cols[kk * (kColPitch / 4) + c] : cols[c * (kPitch / 4) + kk], a[i], al[i]);
+        }
+#pragma unroll
+        for (int j = 0; j < ROWS / 8; ++j) {
+          uint32_t b[2], bl[2];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) two_parts(rows[(j * 8 + g) * (kPitch / 4) + k * 8 + t + i * 4], b[i], bl[i]);
+          mma<T>(d[j], a, bl[0], bl[1]);
+          mma<T>(d[j], al, b[0], b[1]);
+          mma<T>(d[j], a, b[0], b[1]);
+        }
+      }
+    }
+  }
+  async_wait<0>();
+  __syncthreads();
+  // sums to shared memory, [row][column]; then every block of the cluster finishes its share of the columns
+  constexpr int kSumPitch = kCols + 4;
+  float* sums = reinterpret_cast<float*>(smem_raw);
+#pragma unroll
+  for (int j = 0; j < ROWS / 8; ++j)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sums[(j * 8 + 2 * t + (i & 1)) * kSumPitch + warp * 16 + g + (i >> 1) * 8] = d[j][i];
+  if (split > 1) cluster_sync_all();
+  else __syncthreads();
+  const int share = kCols / split, rows = min(ROWS, p.M - row0);
+  with_activation(p.act, [&](auto act) {
+    for (int i = tid; i < rows * share; i += kThreads) {
+      const int row = i / share, c = rank * share + i % share;
+      const uint32_t at = smem + uint32_t(row * kSumPitch + c) * 4;
+      float v = 0.0f;
+      if (split > 1) {
+        for (int q = 0; q < split; ++q) v += cluster_f32(map_to_cta(at, uint32_t(q)));
+      } else {
+        v = sums[row * kSumPitch + c];
+      }
+      if (col0 + c >= p.N) continue;
+      const long long y_row = row0 + row;
+      if (p.bias != nullptr) v += to_f32<T>(static_cast<const T*>(p.bias)[col0 + c]);
+      if (p.residual != nullptr) v += to_f32<T>(static_cast<const T*>(p.residual)[y_row * p.residual_s[0] + (col0 + c) * p.residual_s[1]]);
+      static_cast<T*>(p.y)[y_row * p.y_s[0] + (col0 + c) * p.y_s[1]] = from_f32<T>(activate<decltype(act)::value>(v));
+    }
+  });
+  if (split > 1) cluster_sync_all();   // (the others have read this block's sums)
+}
+
+template <typename T, int ROWS, Order ORDER, bool A_WHOLE>
+cudaError_t go(const MmRowsParams& p, cudaStream_t stream) {
+  constexpr int kSmem = stages_of(ROWS) * (kColTile + ROWS * kPitch);
+  static_assert(ROWS * (kCols + 4) * 4 <= kSmem, "the sums fit");
+  static std::atomic<uint64_t> done;
+  auto* kernel = mm_rows_kernel<T, ROWS, ORDER, A_WHOLE>;
+  const cudaError_t e = allow_smem(kernel, kSmem, done);
+  if (e != cudaSuccess) return e;
+  const long long tiles = (p.N + kCols - 1) / kCols, row_blocks = (p.M + ROWS - 1) / ROWS;
+  const int steps = (p.K + kTileBytes / int(sizeof(T)) - 1) / (kTileBytes / int(sizeof(T)));
+  // two blocks an SM, as long as each has two steps
+  int split = 1;
+  while (split < 8 && tiles * row_blocks * split < 2 * current_sm_count() && steps >= 4 * split) split *= 2;
+  if (tiles * split > 0x7fffffffll || row_blocks > 65535) return cudaErrorInvalidConfiguration;
+  return launch_seq(kernel, dim3(unsigned(tiles * split), unsigned(row_blocks)), kThreads, kSmem, split, stream, p, split);
+}
+
+template <typename T>
+cudaError_t by_layout(const MmRowsParams& p, cudaStream_t stream) {
+  constexpr int kV = 16 / int(sizeof(T));
+  auto whole = [&](const void* q, long long along, long long across, long long extent) {
+    return along == 1 && (reinterpret_cast<uintptr_t>(q) & 15u) == 0 && across % kV == 0 && extent % kV == 0;
+  };
+  const bool a_whole = whole(p.a, p.a_s[1], p.a_s[0], p.K);
+  const Order order = whole(p.b, p.b_s[0], p.b_s[1], p.K) ? Order::kReduction : whole(p.b, p.b_s[1], p.b_s[0], p.N) ? Order::kColumns : Order::kAny;
+  auto rows = [&](auto count) -> cudaError_t {
+    constexpr int R = decltype(count)::value;
+    if (order == Order::kReduction) return a_whole ? go<T, R, Order::kReduction, true>(p, stream) : go<T, R, Order::kReduction, false>(p, stream);
+    if (order == Order::kColumns) return a_whole ? go<T, R, Order::kColumns, true>(p, stream) : go<T, R, Order::kColumns, false>(p, stream);
+    return a_whole ? go<T, R, Order::kAny, true>(p, stream) : go<T, R, Order::kAny, false>(p, stream);
+  };
+  if (p.M <= 16) return rows(std::integral_constant<int, 16>{});
+  if (p.M <= 32) return rows(std::integral_constant<int, 32>{});
+  return rows(std::integral_constant<int, 64>{});
+}
+
+}  // namespace
+
+// (Fewer than eight terms fill no 16 bytes: the convolution's paths for few channels take steps of their own.)
+bool mm_rows_preferred(int, const MmRowsParams& p) { return p.M <= 64 || p.K < 8; }
+
+cudaError_t launch_mm_rows(int dtype, const MmRowsParams& p, cudaStream_t stream) {
+  switch (dtype) {
+    case FDNN_F16: return by_layout<__half>(p, stream);
+    case FDNN_BF16: return by_layout<__nv_bfloat16>(p, stream);
+    default: return by_layout<float>(p, stream);
+  }
+}
+
+}  // namespace fdnn

@@ -1,4 +1,5 @@
-// C-ABI front end of the group norm, state space and delta rule operators: validation and launches.  See include/flagdnn_b200.h.
+// C-ABI front end of the group norm, state space and delta rule operators and of products of few rows: validation and launches.  See include/flagdnn_b200.h.
+#include "mm_rows.h"
 #include "sequence_internal.h"
 
 using namespace fdnn;
@@ -121,6 +122,22 @@ int delta_params(const fdnn_delta_rule_desc* d, DeltaParams* p) {
   p->lengths = nullptr;
   p->final_state = nullptr;
   p->workspace = nullptr;
+  return FDNN_OK;
+}
+
+int mm_params(const fdnn_mm_desc* d, MmRowsParams* p) {
+  if (d == nullptr) return api_fail(FDNN_BAD_PARAM, "descriptor is NULL");
+  if (!float_type(d->dtype)) return api_fail(FDNN_NOT_SUPPORTED, "Unsupported dtype");
+  if (d->m < 0 || d->n < 0 || d->k < 0) return api_fail(FDNN_BAD_PARAM, "negative extent");
+  if (d->activation < FDNN_ACT_NONE || d->activation > FDNN_ACT_GELU_TANH) return api_fail(FDNN_BAD_PARAM, "unknown activation");
+  if (d->m > 1 << 22 || d->n > kMaxTokens || d->k > kMaxTokens) return api_fail(FDNN_NOT_SUPPORTED, "an extent is more than the kernels count");
+  p->M = d->m; p->N = d->n; p->K = d->k; p->act = d->activation;
+  for (int i = 0; i < 2; ++i) {
+    p->a_s[i] = d->a_strides[i];
+    p->b_s[i] = d->b_strides[i];
+    p->residual_s[i] = d->residual_strides[i];
+    p->y_s[i] = d->y_strides[i];
+  }
   return FDNN_OK;
 }
 
@@ -293,6 +310,27 @@ int fdnn_gated_delta_rule_step(const fdnn_delta_rule_desc* desc, const void* q, 
   p.q = q; p.k = k; p.v = v; p.delta = delta; p.beta = beta; p.A = A; p.delta_bias = delta_bias; p.y = y;
   const cudaError_t e = launch_delta_rule_step(desc->dtype, p, state, n_slots, slots, static_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? FDNN_OK : api_fail_cuda("gated_delta_rule_step launch", e);
+}
+
+int fdnn_mm_rows_preferred(const fdnn_mm_desc* desc, int32_t* preferred) {
+  if (preferred == nullptr) return api_fail(FDNN_BAD_PARAM, "preferred is NULL");
+  MmRowsParams p;
+  const int st = mm_params(desc, &p);
+  if (st != FDNN_OK) return st;
+  *preferred = mm_rows_preferred(desc->dtype, p);
+  return FDNN_OK;
+}
+
+int fdnn_mm_rows_fwd(const fdnn_mm_desc* desc, const void* a, const void* b, const void* bias, const void* residual, void* y,
+                     void* stream) {
+  MmRowsParams p;
+  const int st = mm_params(desc, &p);
+  if (st != FDNN_OK) return st;
+  if (p.M == 0 || p.N == 0) return FDNN_OK;
+  if (y == nullptr || (p.K > 0 && (a == nullptr || b == nullptr))) return api_fail(FDNN_BAD_PARAM, "a, b and y must not be NULL");
+  p.a = a; p.b = b; p.bias = bias; p.residual = residual; p.y = y;
+  const cudaError_t e = launch_mm_rows(desc->dtype, p, static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? FDNN_OK : api_fail_cuda("mm_rows launch", e);
 }
 
 }  // extern "C"

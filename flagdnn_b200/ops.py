@@ -66,6 +66,7 @@ sub = _capturable("sub", _eager_binary(torch.sub))
 mul = _capturable("mul", _eager_binary(torch.mul))
 conv1d = _conv.conv1d  # eager only: the graph registry has no conv1d node, as in the reference
 mm = _conv.mm          # eager only
+mm_bias_act = _conv.mm_bias_act
 group_norm_backward = _norm.group_norm_backward
 causal_conv1d = _sequence.causal_conv1d            # the state space operators are eager only: they carry state
 causal_conv1d_step = _sequence.causal_conv1d_step

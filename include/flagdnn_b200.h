@@ -390,6 +390,23 @@ int fdnn_gated_delta_rule_step(const fdnn_delta_rule_desc* desc, const void* q, 
                                const void* delta, const void* beta, const float* A, const float* delta_bias, float* state,
                                int32_t n_slots, const int32_t* slots, void* y, void* stream);
 
+/* A product of few rows with its epilogue: y = act(a b + bias + residual), a [m, k], b [k, n] of any strides, bias [n] dense or NULL,
+ * residual [m, n] or NULL; fp32 sums, one rounding.  fdnn_mm_rows_fwd takes any m (at most 2^22), but is made for a reading of b:
+ * fdnn_mm_rows_preferred says whether it is ahead of the product as a 1x1 convolution (fdnn_conv2d_fwd_residual on a row of m pixels). */
+typedef struct fdnn_mm_desc {
+  int32_t dtype;               /* FDNN_F16, FDNN_BF16 or FDNN_F32: every tensor */
+  int32_t m, n, k;
+  int32_t activation;          /* FDNN_ACT_NONE .. FDNN_ACT_GELU_TANH */
+  int32_t reserved;            /* 0 */
+  int64_t a_strides[2];        /* (row, reduction), elements */
+  int64_t b_strides[2];        /* (reduction, column) */
+  int64_t residual_strides[2];
+  int64_t y_strides[2];
+} fdnn_mm_desc;
+int fdnn_mm_rows_preferred(const fdnn_mm_desc* desc, int32_t* preferred);
+int fdnn_mm_rows_fwd(const fdnn_mm_desc* desc, const void* a, const void* b, const void* bias, const void* residual, void* y,
+                     void* stream);
+
 /* Every wait inside the kernels is bounded; a wait that runs out records a
  * code in a per-device status word and the kernel returns early.  This call
  * synchronises the current device, returns the word in *word (0 = no
