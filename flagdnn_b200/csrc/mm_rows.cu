@@ -98,14 +98,21 @@ mm_rows_kernel(const MmRowsParams p, int split) {
           copy16(smem + at + k * kColPitch + i % kPieces * 16, there ? b0 + (k0 + k) * p.b_s[0] + c : b0, there ? 16 : 0);
         }
       } else {
-        const bool along = p.b_s[0] != 1;   // threads side by side along what lies together
+        // value by value, threads side by side along what lies together: each keeps its column, or its place in the step
+        const bool along = p.b_s[0] != 1;
+        const int fixed = along ? tid % kCols : tid % kStep, first = along ? tid / kCols : tid / kStep, by = kThreads / (along ? kCols : kStep);
+        const int c0 = along ? fixed : first, kk0 = along ? first : fixed;
+        const bool in = along ? col0 + fixed < p.N : k0 + fixed < p.K;
+        const int most = along ? p.K - k0 : p.N - col0;
+        const T* src = b0 + c0 * p.b_s[1] + (k0 + kk0) * p.b_s[0];
+        const long long next = by * (along ? p.b_s[0] : p.b_s[1]);
+        int dst = at + c0 * kPitch + kk0 * int(sizeof(T));
+        const int dst_next = by * (along ? int(sizeof(T)) : kPitch);
 #pragma unroll 8
-        for (int i = tid; i < kCols * kStep; i += kThreads) {
-          const int c = along ? i % kCols : i / kStep, k = along ? i / kCols : i % kStep;
-          const bool there = col0 + c < p.N && k0 + k < p.K;
-          const T* src = there ? b0 + c * p.b_s[1] + (k0 + k) * p.b_s[0] : b0;
-          if constexpr (sizeof(T) == 4) copy4(smem + at + c * kPitch + k * 4, src, there);
-          else reinterpret_cast<T*>(smem_raw + at + c * kPitch)[k] = there ? *src : from_f32<T>(0.0f);
+        for (int i = first; i < (along ? kStep : kCols); i += by, src += next, dst += dst_next) {
+          const bool there = in && i < most;
+          if constexpr (sizeof(T) == 4) copy4(smem + dst, there ? src : b0, there);
+          else *reinterpret_cast<T*>(smem_raw + dst) = there ? *src : from_f32<T>(0.0f);
         }
       }
       const int a_at = at + kColTile;
@@ -117,13 +124,14 @@ mm_rows_kernel(const MmRowsParams p, int split) {
           copy16(smem + a_at + row * kPitch + i % 8 * 16, there ? a0 + row * p.a_s[0] + k : static_cast<const T*>(p.a), there ? 16 : 0);
         }
       } else {
-#pragma unroll 4
-        for (int i = tid; i < ROWS * kStep; i += kThreads) {
-          const int row = i / kStep, k = i % kStep;
-          const bool there = row0 + row < p.M && k0 + k < p.K;
-          const T* src = there ? a0 + row * p.a_s[0] + (k0 + k) * p.a_s[1] : static_cast<const T*>(p.a);
-          if constexpr (sizeof(T) == 4) copy4(smem + a_at + row * kPitch + k * 4, src, there);
-          else reinterpret_cast<T*>(smem_raw + a_at + row * kPitch)[k] = there ? *src : from_f32<T>(0.0f);
+        const int kk = tid % kStep, by = kThreads / kStep, most = k0 + kk < p.K ? p.M - row0 : 0;
+        const T* src = a0 + tid / kStep * p.a_s[0] + (k0 + kk) * p.a_s[1];
+        int dst = a_at + tid / kStep * kPitch + kk * int(sizeof(T));
+#pragma unroll 8
+        for (int i = tid / kStep; i < ROWS; i += by, src += by * p.a_s[0], dst += by * kPitch) {
+          const bool there = i < most;
+          if constexpr (sizeof(T) == 4) copy4(smem + dst, there ? src : static_cast<const T*>(p.a), there);
+          else *reinterpret_cast<T*>(smem_raw + dst) = there ? *src : from_f32<T>(0.0f);
         }
       }
     }
@@ -217,9 +225,10 @@ cudaError_t go(const MmRowsParams& p, cudaStream_t stream) {
   if (e != cudaSuccess) return e;
   const long long tiles = (p.N + kCols - 1) / kCols, row_blocks = (p.M + ROWS - 1) / ROWS;
   const int steps = (p.K + kTileBytes / int(sizeof(T)) - 1) / (kTileBytes / int(sizeof(T)));
-  // two blocks an SM, as long as each has two steps
+  // up to two blocks an SM, which all run at once, as long as each has two steps: 2048 x 4096 bf16, one row, 9.8 / 8.1 / 6.1 / 9.0 us in
+  // 1 / 2 / 4 / 8 parts (64 to 512 blocks), 4096 x 8192 20.8 / 16.0 / 18.5 / 23.4 (128 to 1024)
   int split = 1;
-  while (split < 8 && tiles * row_blocks * split < 2 * current_sm_count() && steps >= 4 * split) split *= 2;
+  while (split < 8 && tiles * row_blocks * split <= current_sm_count() && steps >= 4 * split) split *= 2;
   if (tiles * split > 0x7fffffffll || row_blocks > 65535) return cudaErrorInvalidConfiguration;
   return launch_seq(kernel, dim3(unsigned(tiles * split), unsigned(row_blocks)), kThreads, kSmem, split, stream, p, split);
 }
@@ -245,8 +254,17 @@ cudaError_t by_layout(const MmRowsParams& p, cudaStream_t stream) {
 
 }  // namespace
 
-// (Fewer than eight terms fill no 16 bytes: the convolution's paths for few channels take steps of their own.)
-bool mm_rows_preferred(int, const MmRowsParams& p) { return p.M <= 64 || p.K < 8; }
+// Its time goes with N K and, slowly, with M; the convolution's, on tiles of 128 rows, with K alone as long as they run at once.  16-bit,
+// us here and there: 4096 x 2048 64 rows 12.4 and 15.6, 96 rows 22.3 and 15.6; 2048 x 4096 16 rows 7.9 and 14.0, 32 rows 9.5 and
+// 9.6; 4096 x 8192 16 rows 18.9 and 17.6; 1024 x 1024 32 rows 5.4 and 6.1, 48 rows 6.6 and 6.1; 512 x 4096 16 rows 5.3 and 5.5, 32
+// rows 6.5 and 5.4.  fp32, whose operands the convolution splits first: 2048 x 4096 64 rows 37 and 50, 1024 x 1024 128 rows 12.6 and 21.9,
+// 4096 x 2048 96 rows 61 and 79, 4096 x 8192 96 rows 220 and 143; with b's reduction together, which it packs value by value, 256 rows
+// of 4096 x 2048 136 and 179.  (Fewer than eight terms fill no 16 bytes: its paths for few channels add a residual in a step of its own.)
+bool mm_rows_preferred(int dtype, const MmRowsParams& p) {
+  if (p.K < 8 || p.M <= 16) return true;
+  if (dtype == FDNN_F32) return p.M <= 64 || (p.M <= 256 && p.b_s[0] == 1);
+  return p.M <= 64 && (long long)p.M * p.N <= 32ll * p.K;
+}
 
 cudaError_t launch_mm_rows(int dtype, const MmRowsParams& p, cudaStream_t stream) {
   switch (dtype) {
