@@ -1,10 +1,11 @@
-"""A state space mixer: the block of a sequence model whose tokens meet through a selective scan instead of attention.
+"""Mixers: blocks of a sequence model whose tokens meet through a recurrence instead of attention.
 
-    x -> mm (in) -> causal_conv1d (silu) -> mm (delta, B, C) -> selective_scan (gated) -> group_norm per token -> mm (out)
+    StateSpaceMixer  x -> mm (in) -> causal_conv1d (silu) -> mm (delta, B, C) -> selective_scan (gated) -> group_norm per token -> mm (out)
+    DeltaMixer       x -> mm (in) -> causal_conv1d (silu) of q, k, v -> gated_delta_rule -> group_norm per head -> mm (out) + x
 
-Prompts run through :meth:`StateSpaceMixer.forward`, which returns the state behind them; the next tokens through
-:meth:`StateSpaceMixer.step`, which continues states in place, each row at its slot of a cache. Everything is computed by this
-library's kernels; what the products leave is read in place (delta, B and C are columns of one product's result).
+Prompts run through ``forward``, which returns the state behind them; the next tokens through ``step``, which continues states in
+place, each row at its slot of a cache. Everything is computed by this library's kernels; what the products leave is read in place
+(delta, B and C, or q, k, v, delta and beta, are columns of one product's result).
 """
 from __future__ import annotations
 
@@ -13,14 +14,14 @@ from typing import Optional, Tuple
 
 import torch
 
-from . import conv_host, norm_host, sequence_host
+from . import conv_host, delta_host, norm_host, sequence_host
 
 
 @dataclass
 class MixerState:
-    """What a row carries from token to token: the convolution's last inputs and the scan's states."""
+    """What a row carries from token to token: the convolution's last inputs and the recurrence's states."""
     conv: torch.Tensor    # [slots, width - 1, inner]
-    scan: torch.Tensor    # [slots, inner, states] float32
+    scan: torch.Tensor    # float32: [slots, inner, states] of a scan, [slots, heads, values, keys] of the delta rule
 
     def put(self, slots: torch.Tensor, other: "MixerState") -> None:
         """Row n of ``other`` (or its only one) into slot ``slots[n]``, as after the prompts that begin there; a slot outside the
@@ -109,3 +110,66 @@ class StateSpaceMixer:
         y = sequence_host.selective_scan_step(v, delta, self.A, B, C, state.scan, self.D, both[:, self.inner:], self.delta_bias, True,
                                               slots)
         return self._out(y)
+
+
+class DeltaMixer:
+    """Random-init parameters; ``heads`` heads of ``keys`` x ``values`` channels, whose keys and queries come from ``key_heads``. The
+    result is added to what goes in, in the last product's epilogue."""
+
+    def __init__(self, model: int, heads: int, key_heads: int, keys: int = 128, values: int = 128, width: int = 4, device="cuda",
+                 dtype: torch.dtype = torch.bfloat16, seed: int = 0):
+        g = torch.Generator().manual_seed(seed)
+        self.model, self.heads, self.key_heads, self.keys, self.values, self.width = model, heads, key_heads, keys, values, width
+        self.device, self.dtype = torch.device(device), dtype
+        self.mixed = 2 * key_heads * keys + heads * values                     # channels of the convolution: q, k, v
+
+        def weight(rows, cols):
+            return (torch.randn(rows, cols, generator=g) * rows ** -0.5).to(dtype).to(device)
+
+        self.w_in = weight(model, self.mixed + 2 * heads)
+        self.w_out = weight(heads * values, model)
+        self.w_conv = (torch.randn(self.mixed, width, generator=g) * width ** -0.5).to(dtype).to(device)
+        self.b_conv = (torch.randn(self.mixed, generator=g) * 0.1).to(dtype).to(device)
+        self.A = -(torch.rand(heads, generator=g) * 15 + 1).to(device)
+        dt = torch.exp(torch.rand(heads, generator=g) * 4.6 - 6.9)             # steps of 0.001 .. 0.1
+        self.delta_bias = (dt + torch.log(-torch.expm1(-dt))).to(device)
+        self.w_norm = torch.ones(heads * values, dtype=dtype, device=device)
+        self.b_norm = torch.zeros(heads * values, dtype=dtype, device=device)
+
+    def new_state(self, slots: int) -> MixerState:
+        return MixerState(torch.zeros(slots, self.width - 1, self.mixed, dtype=self.dtype, device=self.device),
+                          torch.zeros(slots, self.heads, self.values, self.keys, device=self.device))
+
+    def _operands(self, mixed: torch.Tensor, gates: torch.Tensor) -> Tuple[torch.Tensor, ...]:
+        """q, k, v, delta and beta as the rule takes them, all views."""
+        n = self.key_heads * self.keys
+        heads = lambda t, h: t.unflatten(-1, (h, -1))  # noqa: E731
+        return (heads(mixed[..., :n], self.key_heads), heads(mixed[..., n:2 * n], self.key_heads), heads(mixed[..., 2 * n:], self.heads),
+                gates[..., :self.heads], gates[..., self.heads:])
+
+    def _out(self, y: torch.Tensor, x: torch.Tensor) -> torch.Tensor:
+        return conv_host.mm_bias_act(norm_host.group_norm(y, self.heads, self.w_norm, self.b_norm), self.w_out, residual=x)
+
+    @torch.no_grad()
+    def forward(self, x: torch.Tensor, state: Optional[MixerState] = None,
+                lengths: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, MixerState]:
+        """Prompts x [N, L, model], behind ``state`` if given (row n at slot n of N slots or more), ragged by ``lengths`` (what comes
+        out for padding tokens is of no use): the outputs and the state behind each row."""
+        n, length, _ = x.shape
+        rows = x.reshape(n * length, self.model)
+        both = conv_host.mm_bias_act(rows, self.w_in).view(n, length, self.mixed + 2 * self.heads)
+        mixed, conv_state = sequence_host.causal_conv1d(both[..., :self.mixed], self.w_conv, self.b_conv, "silu",
+                                                        None if state is None else state.conv[:n], lengths, True)
+        y, scan_state = delta_host.gated_delta_rule(*self._operands(mixed, both[..., self.mixed:]), self.A, self.delta_bias, True, True,
+                                                    True, None, None if state is None else state.scan[:n], lengths, True)
+        out = self._out(y.view(n * length, self.heads * self.values), rows)
+        return out.view(n, length, self.model), MixerState(conv_state, scan_state)
+
+    @torch.no_grad()
+    def step(self, x: torch.Tensor, state: MixerState, slots: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """The next token of each row, x [N, model]; row n continues slot ``slots[n]`` (default n) of ``state`` in place."""
+        both = conv_host.mm_bias_act(x, self.w_in)
+        mixed = sequence_host.causal_conv1d_step(both[:, :self.mixed], state.conv, self.w_conv, self.b_conv, "silu", slots)
+        y = delta_host.gated_delta_rule_step(*self._operands(mixed, both[:, self.mixed:]), state.scan, self.A, self.delta_bias, True, True,
+                                             True, None, slots)
+        return self._out(y.view(-1, self.heads * self.values), x)
