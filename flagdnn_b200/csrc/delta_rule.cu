@@ -332,7 +332,12 @@ __device__ __forceinline__ void sum_gates(const DeltaParams& p, const RawGates& 
 // 2^(hi + lo) to fp32's last place but two: what a state keeps over many chunks has no drift.
 __device__ __forceinline__ float exp2_of(float hi, float lo) { return exp2f(hi) * fmaf(lo, 0.6931471805599453f, 1.0f); }
 
-// d += x y of 16 x 16 blocks in fp32, by 3 x TF32 (a high part is the number cut to TF32, what it leaves is exact; 2^-21).
+// fp32 as a TF32 number, rounded to nearest, and what it leaves.
+__device__ __forceinline__ void two_parts(float v, uint32_t& hi, uint32_t& lo) {
+  hi = (__float_as_uint(v) + 0x1000u) & 0xffffe000u;
+  lo = __float_as_uint(v - __uint_as_float(hi));
+}
+// d += x y of 16 x 16 blocks in fp32, by 3 x TF32 (2^-22).
 __device__ __forceinline__ void block_product(float (&d)[2][4], const float* x, int x_pitch, const float* y, int y_pitch) {
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
 #pragma unroll
@@ -340,19 +345,13 @@ __device__ __forceinline__ void block_product(float (&d)[2][4], const float* x, 
     uint32_t a[4], al[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float v = x[(g + (i & 1) * 8) * x_pitch + s * 8 + t + (i >> 1) * 4];
-      a[i] = __float_as_uint(v) & 0xffffe000u;
-      al[i] = __float_as_uint(v - __uint_as_float(a[i]));
+      two_parts(x[(g + (i & 1) * 8) * x_pitch + s * 8 + t + (i >> 1) * 4], a[i], al[i]);
     }
 #pragma unroll
     for (int n = 0; n < 2; ++n) {
       uint32_t b[2], bl[2];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const float v = y[(s * 8 + t + i * 4) * y_pitch + n * 8 + g];
-        b[i] = __float_as_uint(v) & 0xffffe000u;
-        bl[i] = __float_as_uint(v - __uint_as_float(b[i]));
-      }
+      for (int i = 0; i < 2; ++i) two_parts(y[(s * 8 + t + i * 4) * y_pitch + n * 8 + g], b[i], bl[i]);
       mma_tf32(d[n], a, bl[0], bl[1]);
       mma_tf32(d[n], al, b[0], b[1]);
       mma_tf32(d[n], a, b[0], b[1]);

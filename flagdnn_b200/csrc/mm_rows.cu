@@ -1,12 +1,15 @@
 // A product of few rows with its epilogue: y = act(a b + bias + residual).
 //
-// With one to some dozens of rows a product is a reading of b.  A block takes 64 columns of b and, with the others of its cluster, a share
-// of the reduction; b's tiles come through a ring of asynchronous copies, all of a block's first ones on their way at once.  On the tensor
+// With one to some dozens of rows a product is a reading of b.  A block takes 64 columns of b (or 128) and, with the others of its cluster, a
+// share of the reduction; b's tiles come through a ring of asynchronous copies, all of a block's first ones on their way at once.  On the tensor
 // cores columns are the M side (16 a warp) and rows the N side (8 at a time), so that a single row fills an eighth of an
 // instruction and not a 128th.  The blocks of a cluster add up their sums through each other's shared memory, in their order, and finish
 // a share of the columns each: no workspace, no atomics.
 //
-// Sums are fp32; fp32 operands go in as 3 x TF32 (a high part, cut to TF32, and what it leaves: 2^-21); one rounding at the end.
+// Sums are fp32; fp32 operands go in as 3 x TF32 (a high part, and what it leaves: 2^-22); one rounding at the end.  The tensor cores cut
+// what they add to an accumulator, always towards zero: a sum of 4096 fp32 products that stays in one is 3e-5 too small.  Each step of the
+// ring (32 or 64 products) therefore has accumulators of its own, which are added to the sums in fp32 (5e-7).  That is why fp32 products
+// of any size come here: many rows in blocks of 64 x 128, whose operands are split once for eight or four products each.
 #include "group_norm.cuh"
 #include "mm_rows.h"
 
@@ -14,12 +17,11 @@ namespace fdnn {
 namespace {
 
 constexpr int kThreads = 128;
-constexpr int kCols = 64;                 // columns of b to a block, 16 a warp
+constexpr int kWarps = kThreads / 32;
 constexpr int kTileBytes = 128;           // of the reduction, a step of the ring
 constexpr int kPitch = kTileBytes + 16;   // eight rows of 16 bytes lie in different banks
-constexpr int kColTile = kCols * kPitch;  // bytes of a tile of b, in either order
 // Steps of the ring: some 90 KB, two blocks to an SM.
-__host__ __device__ constexpr int stages_of(int rows) { return rows <= 16 ? 8 : rows <= 32 ? 6 : 5; }
+__host__ __device__ constexpr int stages_of(int rows, int cols) { return cols == 128 ? 4 : rows <= 16 ? 8 : rows <= 32 ? 6 : 5; }
 
 __device__ __forceinline__ void copy16(uint32_t to, const void* from, int bytes) {   // the rest of the 16 is zeros
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
@@ -48,9 +50,10 @@ __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint3
     asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// fp32 as a TF32 number and the rest.
+// fp32 as a TF32 number, rounded to nearest (by the integer unit: the conversion's instruction takes as long as the products), and what it
+// leaves, of either sign, whose last bits the tensor core does not read.
 __device__ __forceinline__ void two_parts(float v, uint32_t& hi, uint32_t& lo) {
-  hi = __float_as_uint(v) & 0xffffe000u;
+  hi = (__float_as_uint(v) + 0x1000u) & 0xffffe000u;
   lo = __float_as_uint(v - __uint_as_float(hi));
 }
 __device__ __forceinline__ float cluster_f32(uint32_t at) {
@@ -61,14 +64,14 @@ __device__ __forceinline__ float cluster_f32(uint32_t at) {
 
 enum class Order { kReduction, kColumns, kAny };   // what lies together in b, in 16-byte pieces; kAny: value by value
 
-// ROWS: of a, 16, 32 or 64 to a block.  A_WHOLE: 16 bytes of a row of a are copied at once.
-template <typename T, int ROWS, Order ORDER, bool A_WHOLE>
+// ROWS: of a, 16, 32 or 64 to a block.  WIDE: 16 columns to a warp, times this.  A_WHOLE: 16 bytes of a row of a are copied at once.
+template <typename T, int ROWS, int WIDE, Order ORDER, bool A_WHOLE>
 __global__ void __launch_bounds__(kThreads)
 mm_rows_kernel(const MmRowsParams p, int split) {
   extern __shared__ __align__(128) uint8_t smem_raw[];
   chained();
-  constexpr int kV = 16 / int(sizeof(T)), kStep = kTileBytes / int(sizeof(T)), kStages = stages_of(ROWS);
-  constexpr int kStage = kColTile + ROWS * kPitch;
+  constexpr int kV = 16 / int(sizeof(T)), kStep = kTileBytes / int(sizeof(T)), kCols = 16 * WIDE * kWarps, kStages = stages_of(ROWS, kCols);
+  constexpr int kColTile = kCols * kPitch, kStage = kColTile + ROWS * kPitch;   // (b's tile takes that in either order)
   // columns together: rows of 64 columns, a step of the reduction apart
   constexpr int kColPitch = ORDER == Order::kColumns ? kCols * int(sizeof(T)) + (sizeof(T) == 2 ? 16 : 32) : kPitch;
   static_assert(ORDER != Order::kColumns || kStep * kColPitch <= kColTile, "fits the tile's place");
@@ -138,7 +141,7 @@ mm_rows_kernel(const MmRowsParams p, int split) {
     async_commit();
   };
 
-  float d[ROWS / 8][4] = {};
+  float sum[WIDE][ROWS / 8][4] = {};
 #pragma unroll
   for (int i = 0; i < kStages - 1; ++i) ask(from + i);
   for (int step = from; step < to; ++step) {
@@ -146,7 +149,9 @@ mm_rows_kernel(const MmRowsParams p, int split) {
     __syncthreads();
     ask(step + kStages - 1);
     const int at = (step - from) % kStages * kStage;
+    float d[WIDE][ROWS / 8][4] = {};
     if constexpr (sizeof(T) == 2) {
+      static_assert(WIDE == 1, "wide blocks are fp32's");
       const uint32_t cols = smem + at, rows = smem + at + kColTile;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
@@ -157,31 +162,48 @@ mm_rows_kernel(const MmRowsParams p, int split) {
         for (int j = 0; j < ROWS / 16; ++j) {
           uint32_t b[4];
           ldmatrix<false>(b, rows + (j * 16 + (m >> 1) * 8 + r) * kPitch + (k * 16 + (m & 1) * 8) * 2);
-          mma<T>(d[2 * j], a, b[0], b[1]);
-          mma<T>(d[2 * j + 1], a, b[2], b[3]);
+          mma<T>(d[0][2 * j], a, b[0], b[1]);
+          mma<T>(d[0][2 * j + 1], a, b[2], b[3]);
         }
       }
     } else {
       const float *cols = reinterpret_cast<const float*>(smem_raw + at), *rows = reinterpret_cast<const float*>(smem_raw + at + kColTile);
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        uint32_t a[4], al[4];
+        uint32_t a[WIDE][4], al[WIDE][4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int c = warp * 16 + g + (i & 1) * 8, kk = k * 8 + t + (i >> 1) * 4;
-          two_parts(ORDER == Order::kColumns ? cols[kk * (kColPitch / 4) + c] : cols[c * (kPitch / 4) + kk], a[i], al[i]);
-        }
+        for (int n = 0; n < WIDE; ++n)
 #pragma unroll
-        for (int j = 0; j < ROWS / 8; ++j) {
-          uint32_t b[2], bl[2];
+          for (int i = 0; i < 4; ++i) {
+            const int c = (warp * WIDE + n) * 16 + g + (i & 1) * 8, kk = k * 8 + t + (i >> 1) * 4;
+            two_parts(ORDER == Order::kColumns ? cols[kk * (kColPitch / 4) + c] : cols[c * (kPitch / 4) + kk], a[n][i], al[n][i]);
+          }
+uint32_t b[ROWS / 8][2], bl[ROWS / 8][2];
 #pragma unroll
-          for (int i = 0; i < 2; ++i) two_parts(rows[(j * 8 + g) * (kPitch / 4) + k * 8 + t + i * 4], b[i], bl[i]);
-          mma<T>(d[j], a, bl[0], bl[1]);
-          mma<T>(d[j], al, b[0], b[1]);
-          mma<T>(d[j], a, b[0], b[1]);
-        }
+        for (int j = 0; j < ROWS / 8; ++j)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) two_parts(rows[(j * 8 + g) * (kPitch / 4) + k * 8 + t + i * 4], b[j][i], bl[j][i]);
+        // (a product waits for the one before it on the same accumulator: all of one kind, then all of the next)
+#pragma unroll
+        for (int n = 0; n < WIDE; ++n)
+#pragma unroll
+          for (int j = 0; j < ROWS / 8; ++j) mma<T>(d[n][j], a[n], bl[j][0], bl[j][1]);
+#pragma unroll
+        for (int n = 0; n < WIDE; ++n)
+#pragma unroll
+          for (int j = 0; j < ROWS / 8; ++j) mma<T>(d[n][j], al[n], b[j][0], b[j][1]);
+#pragma unroll
+        for (int n = 0; n < WIDE; ++n)
+#pragma unroll
+          for (int j = 0; j < ROWS / 8; ++j) mma<T>(d[n][j], a[n], b[j][0], b[j][1]);
       }
     }
+#pragma unroll
+    for (int n = 0; n < WIDE; ++n)
+#pragma unroll
+      for (int j = 0; j < ROWS / 8; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum[n][j][i] += d[n][j][i];
   }
   async_wait<0>();
   __syncthreads();
@@ -189,9 +211,11 @@ mm_rows_kernel(const MmRowsParams p, int split) {
   constexpr int kSumPitch = kCols + 4;
   float* sums = reinterpret_cast<float*>(smem_raw);
 #pragma unroll
-  for (int j = 0; j < ROWS / 8; ++j)
+  for (int n = 0; n < WIDE; ++n)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) sums[(j * 8 + 2 * t + (i & 1)) * kSumPitch + warp * 16 + g + (i >> 1) * 8] = d[j][i];
+    for (int j = 0; j < ROWS / 8; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sums[(j * 8 + 2 * t + (i & 1)) * kSumPitch + (warp * WIDE + n) * 16 + g + (i >> 1) * 8] = sum[n][j][i];
   if (split > 1) cluster_sync_all();
   else __syncthreads();
   const int share = kCols / split, rows = min(ROWS, p.M - row0);
@@ -215,12 +239,12 @@ mm_rows_kernel(const MmRowsParams p, int split) {
   if (split > 1) cluster_sync_all();   // (the others have read this block's sums)
 }
 
-template <typename T, int ROWS, Order ORDER, bool A_WHOLE>
+template <typename T, int ROWS, int WIDE, Order ORDER, bool A_WHOLE>
 cudaError_t go(const MmRowsParams& p, cudaStream_t stream) {
-  constexpr int kSmem = stages_of(ROWS) * (kColTile + ROWS * kPitch);
+  constexpr int kCols = 16 * WIDE * kWarps, kSmem = stages_of(ROWS, kCols) * (kCols + ROWS) * kPitch;
   static_assert(ROWS * (kCols + 4) * 4 <= kSmem, "the sums fit");
   static std::atomic<uint64_t> done;
-  auto* kernel = mm_rows_kernel<T, ROWS, ORDER, A_WHOLE>;
+  auto* kernel = mm_rows_kernel<T, ROWS, WIDE, ORDER, A_WHOLE>;
   const cudaError_t e = allow_smem(kernel, kSmem, done);
   if (e != cudaSuccess) return e;
   const long long tiles = (p.N + kCols - 1) / kCols, row_blocks = (p.M + ROWS - 1) / ROWS;
@@ -241,15 +265,19 @@ cudaError_t by_layout(const MmRowsParams& p, cudaStream_t stream) {
   };
   const bool a_whole = whole(p.a, p.a_s[1], p.a_s[0], p.K);
   const Order order = whole(p.b, p.b_s[0], p.b_s[1], p.K) ? Order::kReduction : whole(p.b, p.b_s[1], p.b_s[0], p.N) ? Order::kColumns : Order::kAny;
-  auto rows = [&](auto count) -> cudaError_t {
-    constexpr int R = decltype(count)::value;
-    if (order == Order::kReduction) return a_whole ? go<T, R, Order::kReduction, true>(p, stream) : go<T, R, Order::kReduction, false>(p, stream);
-    if (order == Order::kColumns) return a_whole ? go<T, R, Order::kColumns, true>(p, stream) : go<T, R, Order::kColumns, false>(p, stream);
-    return a_whole ? go<T, R, Order::kAny, true>(p, stream) : go<T, R, Order::kAny, false>(p, stream);
+  auto rows = [&](auto count, auto wide) -> cudaError_t {
+    constexpr int R = decltype(count)::value, W = decltype(wide)::value;
+    if (order == Order::kReduction) return a_whole ? go<T, R, W, Order::kReduction, true>(p, stream) : go<T, R, W, Order::kReduction, false>(p, stream);
+    if (order == Order::kColumns) return a_whole ? go<T, R, W, Order::kColumns, true>(p, stream) : go<T, R, W, Order::kColumns, false>(p, stream);
+    return a_whole ? go<T, R, W, Order::kAny, true>(p, stream) : go<T, R, W, Order::kAny, false>(p, stream);
   };
-  if (p.M <= 16) return rows(std::integral_constant<int, 16>{});
-  if (p.M <= 32) return rows(std::integral_constant<int, 32>{});
-  return rows(std::integral_constant<int, 64>{});
+  constexpr std::integral_constant<int, 1> one{};
+  if (p.M <= 16) return rows(std::integral_constant<int, 16>{}, one);
+  if (p.M <= 32) return rows(std::integral_constant<int, 32>{}, one);
+  if constexpr (sizeof(T) == 4) {
+    if (p.M > 64) return rows(std::integral_constant<int, 64>{}, std::integral_constant<int, 2>{});
+  }
+  return rows(std::integral_constant<int, 64>{}, one);
 }
 
 }  // namespace
@@ -257,13 +285,10 @@ cudaError_t by_layout(const MmRowsParams& p, cudaStream_t stream) {
 // Its time goes with N K and, slowly, with M; the convolution's, on tiles of 128 rows, with K alone as long as they run at once.  16-bit,
 // us here and there: 4096 x 2048 64 rows 12.4 and 15.6, 96 rows 22.3 and 15.6; 2048 x 4096 16 rows 7.9 and 14.0, 32 rows 9.5 and
 // 9.6; 4096 x 8192 16 rows 18.9 and 17.6; 1024 x 1024 32 rows 5.4 and 6.1, 48 rows 6.6 and 6.1; 512 x 4096 16 rows 5.3 and 5.5, 32
-// rows 6.5 and 5.4.  fp32, whose operands the convolution splits first: 2048 x 4096 64 rows 37 and 50, 1024 x 1024 128 rows 12.6 and 21.9,
-// 4096 x 2048 96 rows 61 and 79, 4096 x 8192 96 rows 220 and 143; with b's reduction together, which it packs value by value, 256 rows
-// of 4096 x 2048 136 and 179.  (Fewer than eight terms fill no 16 bytes: its paths for few channels add a residual in a step of its own.)
+// rows 6.5 and 5.4.  Fewer than eight terms fill no 16 bytes: its paths for few channels add a residual in a step of its own.  Its fp32
+// sums stay in one accumulator (see above).
 bool mm_rows_preferred(int dtype, const MmRowsParams& p) {
-  if (p.K < 8 || p.M <= 16) return true;
-  if (dtype == FDNN_F32) return p.M <= 64 || (p.M <= 256 && p.b_s[0] == 1);
-  return p.M <= 64 && (long long)p.M * p.N <= 32ll * p.K;
+  return p.K < 8 || p.M <= 16 || dtype == FDNN_F32 || (p.M <= 64 && (long long)p.M * p.N <= 32ll * p.K);
 }
 
 cudaError_t launch_mm_rows(int dtype, const MmRowsParams& p, cudaStream_t stream) {

@@ -107,7 +107,7 @@ def test_which_products_are_of_few_rows(native_lib):
 
     assert preferred(m=1, n=8192, k=64) and preferred(m=16, n=8192, k=64) and preferred(m=500, n=8192, k=7)
     assert preferred(m=64, n=2048, k=4096) and not preferred(m=64, n=4096, k=2048) and not preferred(m=65, n=64, k=4096)
-    assert preferred(m=64, n=8192, k=64, dtype=nat.F32) and not preferred(m=65, n=64, k=4096, dtype=nat.F32)
+    assert preferred(m=5000, n=8192, k=64, dtype=nat.F32)      # whose sums a convolution keeps in one accumulator
 
 
 def test_cpu_tensors_are_refused():

@@ -91,6 +91,16 @@ def test_nothing_to_multiply(fd, dtype):
     assert fd.mm_bias_act(torch.ones(3, 4, dtype=dtype, device="cuda"), torch.ones(4, 0, dtype=dtype, device="cuda")).shape == (3, 0)
 
 
+def test_long_sums_do_not_drift(fd):
+    """fp32 sums of many products of one sign: cut at every step they would be 1e-5 too small; rounded ones scatter."""
+    g = torch.Generator().manual_seed(5)
+    for m in (3, 40, 200):
+        a, b = torch.rand(m, 8192, generator=g).cuda(), torch.rand(8192, 96, generator=g).cuda()
+        want = a.double() @ b.double()
+        drift = float((fd.mm_bias_act(a, b).double() / want - 1).mean())
+        assert abs(drift) < 1e-6, drift
+
+
 def test_infinite_columns_stay_in_their_columns(fd):
     """What stands beside a product's columns, rows and reduction is not multiplied."""
     g = torch.Generator().manual_seed(1)
