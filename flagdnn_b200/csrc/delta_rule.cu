@@ -25,6 +25,7 @@ namespace {
 
 constexpr int kChunk = 64;
 constexpr int kChunkKeys = 128;      // the widest key that the chunks' kernels take
+constexpr int kMostSegments = 32;    // that a row is cut into
 constexpr int kFactors = 6 * kChunk; // floats a chunk and head: -a, b, d, t, p, and e^(G_64)
 constexpr int kLower = 10 * 512;     // bytes of a part of T or P
 
@@ -170,7 +171,7 @@ __host__ __device__ inline Layout layout_of(const DeltaParams& p) {
 }
 template <typename T, int KEYS>
 long long bytes_of(const DeltaParams& p) {
-  const long long chunks = (p.L + kChunk - 1) / kChunk;
+  const long long chunks = ((long long)p.L + kChunk - 1) / kChunk;
   return (long long)p.N * chunks * ((long long)p.G * 2 * Work<T, KEYS>::kKeyBytes + (long long)p.H * Work<T, KEYS>::kHeadBytes);
 }
 __device__ __forceinline__ int row_end(const DeltaParams& p, long long n) {
@@ -634,10 +635,21 @@ __device__ __forceinline__ void mma_row(float (&d)[TILES][4], const uint32_t (&a
   }
 }
 
+// A launch over the chunks.  Where few rows and heads leave SMs idle, a row is cut into segments of `per` chunks, which run side by side: first
+// for their `ends` alone, from nothing, with the K rows of a unit matrix as further rows (the end of a segment is its start times their end
+// plus the end from nothing: delta_join_kernel), then from their `starts`.
+struct Run {
+  int blocks_a_head, stages, per, segments;
+  const float* starts;   // [N, H, segments - 1, V, K]: of all but the first
+  float* ends;           // null, or [N, H, segments - 1, V rounded up to 16 + K, K]: of all but the last
+  uint32_t* status;
+  long long wait_limit;
+};
+
 // WHOLE: 16 bytes of neighbouring value channels are copied and stored at once.
 template <typename T, int KEYS, int SLICES, bool WHOLE>
 __global__ void __launch_bounds__((2 + outs_of(SLICES)) * SLICES * 32, 1)
-delta_chunks_kernel(const DeltaParams p, int blocks_a_head, int stages, uint32_t* status, long long wait_limit) {
+delta_chunks_kernel(const DeltaParams p, const Run run) {
   extern __shared__ __align__(128) uint8_t smem_raw[];
   __shared__ uint64_t full[kMostStages], empty[kMostStages];   // a stage's operands have landed; all warps are done with them
   __shared__ uint32_t abort_word;
@@ -657,23 +669,31 @@ delta_chunks_kernel(const DeltaParams p, int blocks_a_head, int stages, uint32_t
   const Layout w = layout_of<T, KEYS>(p);
   const int lane = threadIdx.x & 31, slices = blockDim.x / kShare;
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
-  const int h = int(blockIdx.x / blocks_a_head % p.H);
-  const long long n = blockIdx.x / blocks_a_head / p.H;
-  const int end = row_end(p, n), chunks = (end + kChunk - 1) / kChunk;
-  const int first = int(blockIdx.x % blocks_a_head) * slices * 16;   // the block's first value channel
+  const int stages = run.stages, made = run.ends != nullptr ? run.segments - 1 : run.segments;
+  const int segment = int(blockIdx.x / run.blocks_a_head % made), h = int(blockIdx.x / run.blocks_a_head / made % p.H);
+  const long long n = blockIdx.x / run.blocks_a_head / made / p.H;
+  // the segment's tokens begin at `begin`, and are `end` (of the row's, which may be fewer)
+  const int begin = int(min((long long)segment * run.per * kChunk, (long long)p.L)), row_tokens = row_end(p, n);
+  const int end = max(0, min(row_tokens - begin, run.per * kChunk)), chunks = (end + kChunk - 1) / kChunk;
+  const int chunk0 = segment * run.per;
   const int pitch = value_pitch<T>(slices), stage_bytes = W::kStage + kChunk * pitch;
   const uint32_t smem = smem_u32(smem_raw);
   const int g = lane >> 2, t = lane & 3, m = lane >> 3, r = lane & 7;
   const bool outputs = warp >= 2 * slices;
   const int slice = outputs ? (warp - 2 * slices) / kOuts : warp >> 1, half = warp & 1;
-  const int row0 = first + slice * 16, channels = min(16, p.V - row0);
+  // 16 rows: value channels, or behind them (where the segments' ends are made) the rows of what the segment makes of a state, a unit's
+  // each, which meet no values
+  const int number = int(blockIdx.x % run.blocks_a_head) * slices + slice, value_slices = (p.V + 15) / 16;
+  const bool transition = run.ends != nullptr && number >= value_slices;
+  const int row0 = (transition ? number - value_slices : number) * 16, rows = min(16, (transition ? p.K : p.V) - row0);
+  const int channels = transition ? 0 : rows;
   uint8_t* const exchange = smem_raw + stages * stage_bytes + slice * E::kBytes;
   // named barriers of the slice's own: slices run at their own pace, `stages` chunks apart at most
   const int top_id = slice, pair_id = kMostSlices + slice, state_id = 2 * kMostSlices + slice, written_id = 3 * kMostSlices + slice;
   // The slice's warps, at the top of chunk c: it is there, and they are done with chunk c - 1.
   auto arrive_at = [&](int c) {
     barrier<kShare>(top_id);
-    mbar_wait_warp(&full[c % stages], uint32_t(c / stages) & 1u, &abort_word, status, kIncidentDeltaWait, wait_limit);
+    mbar_wait_warp(&full[c % stages], uint32_t(c / stages) & 1u, &abort_word, run.status, kIncidentDeltaWait, run.wait_limit);
   };
   auto leave = [&](int c) {
     __syncwarp();
@@ -685,15 +705,15 @@ delta_chunks_kernel(const DeltaParams p, int blocks_a_head, int stages, uint32_t
     const int tid = kOuts == 2 ? threadIdx.x & 63 : lane;
     constexpr int kStep = 32 * kOuts;
     const bool loader = threadIdx.x == 2u * slices * 32;
-    const uint8_t* keys_from = w.keys + (n * p.G + h / (p.H / p.G)) * w.chunks * (2ll * W::kKeyBytes);
-    const uint8_t* heads_from = w.heads + (n * p.H + h) * w.chunks * (long long)W::kHeadBytes;
-    const T* v0 = static_cast<const T*>(p.v) + n * p.v_s[0] + h * p.v_s[2] + row0 * p.v_s[3];
+    const uint8_t* keys_from = w.keys + ((n * p.G + h / (p.H / p.G)) * w.chunks + chunk0) * (2ll * W::kKeyBytes);
+    const uint8_t* heads_from = w.heads + ((n * p.H + h) * w.chunks + chunk0) * (long long)W::kHeadBytes;
+    const T* v0 = static_cast<const T*>(p.v) + n * p.v_s[0] + begin * p.v_s[1] + h * p.v_s[2] + row0 * p.v_s[3];
     int asked = 0;   // chunks, by the loader
     auto ask = [&](int c) {
       uint8_t* const to = smem_raw + (c % stages) * stage_bytes;
       if (loader && asked == c) {
         uint64_t* bar = &full[c % stages];
-        if (c < stages || mbar_wait_bounded(&empty[c % stages], uint32_t(c / stages - 1) & 1u, &abort_word, status, kIncidentDeltaWait, wait_limit)) {
+        if (c < stages || mbar_wait_bounded(&empty[c % stages], uint32_t(c / stages - 1) & 1u, &abort_word, run.status, kIncidentDeltaWait, run.wait_limit)) {
           mbar_arrive_expect_tx(bar, W::kStage);
           bulk_load_1d(to, keys_from + c * (2ll * W::kKeyBytes), 2 * W::kKeyBytes, bar);
           bulk_load_1d(to + 2 * W::kKeyBytes, heads_from + c * (long long)W::kHeadBytes, W::kHeadBytes, bar);
@@ -721,7 +741,8 @@ delta_chunks_kernel(const DeltaParams p, int blocks_a_head, int stages, uint32_t
       }
       async_commit();
     };
-    T* y = static_cast<T*>(p.y) + n * p.y_s[0] + h * p.y_s[2] + row0 * p.y_s[3];
+    T* const y_row = static_cast<T*>(p.y) + n * p.y_s[0] + h * p.y_s[2] + row0 * p.y_s[3];
+    T* const y = y_row + begin * p.y_s[1];
     for (int c = 0; c < stages - 1; ++c) {
       if (c < chunks) ask(c);
       else async_commit();
@@ -732,6 +753,12 @@ delta_chunks_kernel(const DeltaParams p, int blocks_a_head, int stages, uint32_t
       arrive_at(c);
       if (c + stages - 1 < chunks) ask(c + stages - 1);
       else async_commit();
+      if (run.ends != nullptr) {   // (the state alone)
+        barrier<kShare>(state_id);
+        barrier<kShare>(written_id);
+        leave(c);
+        continue;
+      }
       const uint8_t* const base = smem_raw + (c % stages) * stage_bytes;
       // this warp's tokens: all of the chunk's, or its first or last 32
       constexpr int kTiles = 8 / kOuts;
@@ -832,18 +859,28 @@ delta_chunks_kernel(const DeltaParams p, int blocks_a_head, int stages, uint32_t
       leave(c);
     }
     // tokens behind the row's end
-    for (long long i = end * 16ll + (kOuts == 2 ? (warp & 1) * 32 : 0) + lane; i < p.L * 16ll; i += 32 * kOuts)
-      if (i % 16 < channels) y[i / 16 * p.y_s[1] + i % 16 * p.y_s[3]] = from_f32<T>(0.0f);
+    if (run.ends == nullptr && segment == run.segments - 1)
+      for (long long i = row_tokens * 16ll + (kOuts == 2 ? (warp & 1) * 32 : 0) + lane; i < p.L * 16ll; i += 32 * kOuts)
+        if (i % 16 < channels) y_row[i / 16 * p.y_s[1] + i % 16 * p.y_s[3]] = from_f32<T>(0.0f);
     if (loader && *static_cast<volatile uint32_t*>(&abort_word) != 0) {   // after an incident: give the copies in flight time to land
       volatile uint32_t never = 0;
       for (int c = max(0, asked - stages); c < asked; ++c)
-        mbar_wait_bounded(&full[c % stages], uint32_t(c / stages) & 1u, &never, status, kIncidentDrainWait, kWaitLimitCycles / 16);
+        mbar_wait_bounded(&full[c % stages], uint32_t(c / stages) & 1u, &never, run.status, kIncidentDrainWait, kWaitLimitCycles / 16);
     }
     return;
   }
 
   // ---- two warps hold 16 rows of the state, half of the keys' channels each: s[j] rows lane / 4, + 8, channels 8 j + 2 (lane % 4), + 1
-  const long long state_at = ((n * p.H + h) * p.V + row0) * (long long)p.K;
+  const long long head = n * p.H + h;
+  const float* from = nullptr;   // the state before the first token: zeros, or a unit a row
+  float* to = nullptr;
+  if (run.ends != nullptr) {
+    to = run.ends + ((head * (run.segments - 1) + segment) * (value_slices * 16 + p.K) + (transition ? value_slices * 16 : 0) + row0) * p.K;
+  } else {
+    if (segment > 0) from = run.starts + ((head * (run.segments - 1) + segment - 1) * p.V + row0) * p.K;
+    else if (p.initial != nullptr) from = p.initial + (head * p.V + row0) * p.K;
+    if (segment == run.segments - 1 && p.final_state != nullptr) to = p.final_state + (head * p.V + row0) * p.K;
+  }
   float4 *const mine = reinterpret_cast<float4*>(exchange + half * 8 * 512) + lane, *const theirs = reinterpret_cast<float4*>(exchange + (half ^ 1) * 8 * 512) + lane;
   float s[kHalf / 8][4];
 #pragma unroll
@@ -851,7 +888,7 @@ delta_chunks_kernel(const DeltaParams p, int blocks_a_head, int stages, uint32_t
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int row = g + (i >> 1) * 8, at = half * kHalf + j * 8 + 2 * t + (i & 1);
-      s[j][i] = p.initial != nullptr && row < channels && at < p.K ? p.initial[state_at + (long long)row * p.K + at] : 0.0f;
+      s[j][i] = from != nullptr && row < rows && at < p.K ? from[(long long)row * p.K + at] : transition && row0 + row == at ? 1.0f : 0.0f;
     }
 
   for (int c = 0; c < chunks; ++c) {
@@ -1014,13 +1051,98 @@ delta_chunks_kernel(const DeltaParams p, int blocks_a_head, int stages, uint32_t
     leave(c);
   }
 
-  if (p.final_state != nullptr) {
+  if (to != nullptr) {
 #pragma unroll
     for (int j = 0; j < kHalf / 8; ++j)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int row = g + (i >> 1) * 8, at = half * kHalf + j * 8 + 2 * t + (i & 1);
-        if (row < channels && at < p.K) p.final_state[state_at + (long long)row * p.K + at] = s[j][i];
+        if (row < rows && at < p.K) to[(long long)row * p.K + at] = s[j][i];
+      }
+  }
+}
+
+// ---- segments put together -----------------------------------------------------------------------------------------
+
+constexpr int kJoinRows = 8, kJoinThreads = 256;
+constexpr int kJoinSmem = (2 * kChunkKeys + kJoinRows) * kChunkKeys * 4;
+// start[j + 1] = start[j] unit_end[j] + end[j], from the row's initial state on: eight rows of the state to a block, two of them at two columns
+// to a thread.  The next segment's ends are on their way meanwhile (64 KB of unit ends: read from L2 by each product they took 17 us
+// a segment).
+__global__ void __launch_bounds__(kJoinThreads)
+delta_join_kernel(const DeltaParams p, const float* ends, float* starts, int segments) {
+  extern __shared__ __align__(128) uint8_t smem_raw[];
+  constexpr int kPlace = kChunkKeys * kChunkKeys;
+  float* const units = reinterpret_cast<float*>(smem_raw);   // two of [K][K rounded up to 2]
+  float* const s = units + 2 * kPlace;                       // [kJoinRows][kChunkKeys]
+  chained();
+  const int parts = (p.V + kJoinRows - 1) / kJoinRows, row0 = int(blockIdx.x % parts) * kJoinRows + threadIdx.x / 64 * 2;
+  const long long head = blockIdx.x / parts;
+  const int col = threadIdx.x % 64 * 2, tall = (p.V + 15) / 16 * 16 + p.K, wide = (p.K + 1) / 2 * 2;
+  float* const mine = s + threadIdx.x / 64 * 2 * kChunkKeys;
+  auto ask = [&](int j) {
+    if (j < segments - 1) {
+      const float* unit = ends + ((head * (segments - 1) + j) * tall + tall - p.K) * p.K;
+      const uint32_t to = smem_u32(units + (j & 1) * kPlace);
+      if (p.K % 4 == 0) {   // (as the workspace's addresses)
+#pragma unroll 4
+        for (int i = threadIdx.x; i < p.K * p.K / 4; i += kJoinThreads) copy16(to + i * 16, unit + i * 4, 16);
+      } else {
+        for (int i = threadIdx.x; i < p.K * p.K; i += kJoinThreads)
+          asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to + (i / p.K * wide + i % p.K) * 4), "l"(unit + i) : "memory");
+      }
+    }
+    async_commit();
+  };
+  auto load = [&](float (&x)[2][2], const float* from) {   // rows of a state, or of an end
+#pragma unroll
+    for (int r = 0; r < 2; ++r)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) x[r][c] = from != nullptr && row0 + r < p.V && col + c < p.K ? from[(long long)(row0 + r) * p.K + col + c] : 0.0f;
+  };
+  float x[2][2], next[2][2];
+  ask(0);
+  load(x, p.initial != nullptr ? p.initial + head * p.V * p.K : nullptr);
+  load(next, ends + head * (segments - 1) * tall * p.K);
+  for (int j = 0; j < segments - 1; ++j) {
+    async_wait<0>();
+    __syncthreads();   // the ends are there; all are done with the last segment's start
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      *reinterpret_cast<float2*>(mine + r * kChunkKeys + col) = make_float2(x[r][0], x[r][1]);   // (zeros behind K)
+      x[r][0] = next[r][0];
+      x[r][1] = next[r][1];
+    }
+    __syncthreads();
+    ask(j + 1);
+    if (j + 1 < segments - 1) load(next, ends + (head * (segments - 1) + j + 1) * tall * p.K);
+    const float* unit = units + (j & 1) * kPlace + (col < p.K ? col : 0);
+    int k = 0;
+#pragma unroll 4
+    for (; k + 4 <= p.K; k += 4) {
+      float2 u[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) u[i] = *reinterpret_cast<const float2*>(unit + (k + i) * wide);
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const float4 v = *reinterpret_cast<const float4*>(mine + r * kChunkKeys + k);
+        x[r][0] = fmaf(v.w, u[3].x, fmaf(v.z, u[2].x, fmaf(v.y, u[1].x, fmaf(v.x, u[0].x, x[r][0]))));
+        x[r][1] = fmaf(v.w, u[3].y, fmaf(v.z, u[2].y, fmaf(v.y, u[1].y, fmaf(v.x, u[0].y, x[r][1]))));
+      }
+    }
+    for (; k < p.K; ++k)
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const float2 u = *reinterpret_cast<const float2*>(unit + k * wide);
+        x[r][0] = fmaf(mine[r * kChunkKeys + k], u.x, x[r][0]);
+        x[r][1] = fmaf(mine[r * kChunkKeys + k], u.y, x[r][1]);
+      }
+#pragma unroll
+    for (int r = 0; r < 2; ++r)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        if (col + c >= p.K) x[r][c] = 0.0f;
+        else if (row0 + r < p.V) starts[((head * (segments - 1) + j) * p.V + row0 + r) * p.K + col + c] = x[r][c];
       }
   }
 }
@@ -1037,6 +1159,51 @@ bool eights(const void* q, const long long* s) {
   return (reinterpret_cast<uintptr_t>(q) & 15u) == 0 && s[0] % kV == 0 && s[1] % kV == 0 && s[2] % kV == 0 && s[3] == 1;
 }
 
+constexpr int kMostSmem = 227 * 1024 - 256;   // (and the barriers)
+template <typename T, int KEYS>
+constexpr int smem_of(int slices, int stages) {
+  return stages * (Work<T, KEYS>::kStage + kChunk * value_pitch<T>(slices)) + slices * Exchange<T, KEYS>::kBytes;
+}
+
+// Rounds of blocks of so many slices, for a number of slices to a head and of segments to a row.
+long long rounds_of(const DeltaParams& p, int slices_a_head, int segments, int slices) {
+  const long long blocks = (long long)p.N * p.H * segments * ((slices_a_head + slices - 1) / slices), sms = current_sm_count();
+  return (blocks + sms - 1) / sms;
+}
+// Slices to a block.  Four take 1.7 times as long for a chunk as two (4100 and 7000 clocks: 128 x 128, bf16).
+template <typename T, int KEYS>
+int slices_of(const DeltaParams& p, int slices_a_head, int segments) {
+  static_assert(smem_of<T, KEYS>(1, 2) <= kMostSmem, "one slice has two stages");
+  int slices = slices_a_head < 2 ? slices_a_head : 2;
+  if (slices_a_head > 2 && 17 * rounds_of(p, slices_a_head, segments, 4) < 10 * rounds_of(p, slices_a_head, segments, 2))
+    slices = slices_a_head < 4 ? slices_a_head : 4;
+  while (slices > 1 && smem_of<T, KEYS>(slices, 2) > kMostSmem) --slices;
+  return slices;
+}
+// Segments to a row: the count with the least time, in chunks of two slices (2.2 us).  Two walks and what joins them, some 8 us and 2.4 us a
+// segment and round of blocks, against one: worth it where a tenth is won.
+struct Segments {
+  int count, per;
+};
+template <typename T, int KEYS>
+Segments segments_of(const DeltaParams& p) {
+  const int chunks = int(((long long)p.L + kChunk - 1) / kChunk), values = (p.V + 15) / 16, keys = (p.K + 15) / 16;
+  auto walk = [&](int slices_a_head, int segments, int per) {
+    const int slices = slices_of<T, KEYS>(p, slices_a_head, segments);
+    return per * (slices > 2 ? 1.7 : 1.0) * double(rounds_of(p, slices_a_head, segments, slices));
+  };
+  const long long join_blocks = (long long)p.N * p.H * ((p.V + 7) / 8), joins = (join_blocks + current_sm_count() - 1) / current_sm_count();
+  Segments best = {1, chunks};
+  double least = 0.9 * walk(values, 1, chunks);
+  for (int count = 2; count <= kMostSegments && 2 * count <= chunks; ++count) {
+    const int per = (chunks + count - 1) / count;
+    if ((chunks + per - 1) / per != count) continue;   // (as many segments in pieces as long)
+    const double time = walk(values + keys, count - 1, per) + walk(values, count, per) + (8.0 + 2.4 * count * double(joins)) / 2.2;
+    if (time < least) least = time, best = {count, per};
+  }
+  return best;
+}
+
 template <typename T, int KEYS>
 cudaError_t run(const DeltaParams& p, cudaStream_t stream) {
   const long long chunks = (p.L + kChunk - 1) / kChunk;
@@ -1051,37 +1218,46 @@ cudaError_t run(const DeltaParams& p, cudaStream_t stream) {
   e = launch_seq(prep, dim3(unsigned(prep_blocks)), kPrepThreads, kPrepSmem, 1, stream, p);
   if (e != cudaSuccess) return e;
 
-  const int most = (p.V + 15) / 16;
-  auto blocks_of = [&](int slices) { return (long long)p.N * p.H * ((most + slices - 1) / slices); };
-  auto smem_of = [&](int slices, int stages) {
-    return stages * (Work<T, KEYS>::kStage + kChunk * value_pitch<T>(slices)) + slices * Exchange<T, KEYS>::kBytes;
-  };
-  constexpr int kMostSmem = 227 * 1024 - 256;   // (and the barriers)
-  // Four slices to a block: a chunk takes half as long again as with two, for twice the rows
-  const int sms = current_sm_count();
-  auto rounds = [&](int slices) { return (blocks_of(slices) + sms - 1) / sms; };
-  int slices = most < 2 ? most : 2;
-  if (most > 2 && 3 * rounds(4) < 2 * rounds(2)) slices = most < 4 ? most : 4;
-  while (slices > 1 && smem_of(slices, 2) > kMostSmem) --slices;
-  const int stages = smem_of(slices, 3) <= kMostSmem ? 3 : 2;
-  static_assert(2 * (Work<T, KEYS>::kStage + kChunk * value_pitch<T>(1)) + Exchange<T, KEYS>::kBytes <= kMostSmem, "one slice has two stages");
-  const long long blocks = blocks_of(slices);
-  if (blocks > 0x7fffffffll) return cudaErrorInvalidConfiguration;
   const bool values_whole = p.V % (16 / int(sizeof(T))) == 0 && eights<T>(p.v, p.v_s) && eights<T>(p.y, p.y_s);
-  auto go = [&](auto* kernel, std::atomic<uint64_t>& allowed, int most_slices) -> cudaError_t {
-    cudaError_t err = allow_smem(kernel, kMostSmem, allowed);
+  Run r = {};
+  bounded_wait_of(&r.status, &r.wait_limit);
+  if (r.status == nullptr) return cudaErrorInvalidSymbol;
+  auto go = [&](auto* kernel, std::atomic<uint64_t>& allowed, int slices, long long blocks) -> cudaError_t {
+    const cudaError_t err = allow_smem(kernel, kMostSmem, allowed);
     if (err != cudaSuccess) return err;
-    uint32_t* status;
-    long long wait_limit;
-    bounded_wait_of(&status, &wait_limit);
-    if (status == nullptr) return cudaErrorInvalidSymbol;
-    return launch_seq(kernel, dim3(unsigned(blocks)), (2 + outs_of(most_slices)) * slices * 32, smem_of(slices, stages), 1, stream, p,
-                      (most + slices - 1) / slices, stages, status, wait_limit);
+    if (blocks > 0x7fffffffll) return cudaErrorInvalidConfiguration;
+    return launch_seq(kernel, dim3(unsigned(blocks)), (2 + outs_of(slices)) * slices * 32, smem_of<T, KEYS>(slices, r.stages), 1, stream, p, r);
   };
   static std::atomic<uint64_t> allowed[4];
-  if (slices <= 2)
-    return values_whole ? go(delta_chunks_kernel<T, KEYS, 2, true>, allowed[0], 2) : go(delta_chunks_kernel<T, KEYS, 2, false>, allowed[1], 2);
-  return values_whole ? go(delta_chunks_kernel<T, KEYS, 4, true>, allowed[2], 4) : go(delta_chunks_kernel<T, KEYS, 4, false>, allowed[3], 4);
+  auto walk = [&](int slices_a_head, int segments) -> cudaError_t {   // of each row
+    const int slices = slices_of<T, KEYS>(p, slices_a_head, segments);
+    r.blocks_a_head = (slices_a_head + slices - 1) / slices;
+    r.stages = smem_of<T, KEYS>(slices, 3) <= kMostSmem ? 3 : 2;
+    const long long blocks = (long long)p.N * p.H * segments * r.blocks_a_head;
+    if (slices <= 2)
+      return values_whole ? go(delta_chunks_kernel<T, KEYS, 2, true>, allowed[0], slices, blocks) : go(delta_chunks_kernel<T, KEYS, 2, false>, allowed[1], slices, blocks);
+    return values_whole ? go(delta_chunks_kernel<T, KEYS, 4, true>, allowed[2], slices, blocks) : go(delta_chunks_kernel<T, KEYS, 4, false>, allowed[3], slices, blocks);
+  };
+  const Segments cut = segments_of<T, KEYS>(p);
+  r.segments = cut.count;
+  r.per = cut.per;
+  if (cut.count > 1) {
+    float* const ends = reinterpret_cast<float*>(static_cast<uint8_t*>(p.workspace) + bytes_of<T, KEYS>(p));
+    float* const starts = ends + (long long)p.N * p.H * (cut.count - 1) * ((p.V + 15) / 16 * 16 + p.K) * p.K;
+    r.ends = ends;
+    e = walk((p.V + 15) / 16 + (p.K + 15) / 16, cut.count - 1);
+    if (e != cudaSuccess) return e;
+    const long long joins = (long long)p.N * p.H * ((p.V + kJoinRows - 1) / kJoinRows);
+    if (joins > 0x7fffffffll) return cudaErrorInvalidConfiguration;
+    static std::atomic<uint64_t> allowed_join;
+    e = allow_smem(delta_join_kernel, kJoinSmem, allowed_join);
+    if (e != cudaSuccess) return e;
+    e = launch_seq(delta_join_kernel, dim3(unsigned(joins)), kJoinThreads, kJoinSmem, 1, stream, p, ends, starts, cut.count);
+    if (e != cudaSuccess) return e;
+    r.ends = nullptr;
+    r.starts = starts;
+  }
+  return walk((p.V + 15) / 16, cut.count);
 }
 
 // f(TypeOf<T>, integral_constant<int, KEYS>)
@@ -1100,7 +1276,12 @@ auto by_type(int dtype, const DeltaParams& p, F&& f) {
 
 long long delta_rule_workspace(int dtype, const DeltaParams& p) {
   if (!in_chunks(p)) return 0;
-  return by_type(dtype, p, [&](auto type, auto keys) -> long long { return bytes_of<typename decltype(type)::type, decltype(keys)::value>(p); });
+  return by_type(dtype, p, [&](auto type, auto keys) -> long long {
+    using T = typename decltype(type)::type;
+    constexpr int kKeys = decltype(keys)::value;
+    const long long cuts = segments_of<T, kKeys>(p).count - 1;
+    return bytes_of<T, kKeys>(p) + (long long)p.N * p.H * cuts * ((p.V + 15) / 16 * 16 + p.K + p.V) * p.K * 4;
+  });
 }
 
 cudaError_t launch_delta_rule(int dtype, const DeltaParams& p, cudaStream_t stream) {

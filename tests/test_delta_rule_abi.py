@@ -68,15 +68,16 @@ def test_missing_rule_tensors_and_workspaces(native_lib):
 
 
 def test_the_workspace_grows_with_the_chunks(native_lib):
-    size = []
-    for length in (64, 128, 128 * 64):
-        d, nbytes = _rule(l=length), ctypes.c_int64()
+    def size(**kw):
+        d, nbytes = _rule(**kw), ctypes.c_int64()
         nat.check(native_lib.fdnn_gated_delta_rule_workspace_bytes(ctypes.byref(d), ctypes.byref(nbytes)))
-        size.append(nbytes.value)
-    assert size[1] == 2 * size[0] and size[2] == 128 * size[0]
-    d, nbytes = _rule(n=1 << 14, l=1 << 20), ctypes.c_int64()            # counted in 64 bits
-    nat.check(native_lib.fdnn_gated_delta_rule_workspace_bytes(ctypes.byref(d), ctypes.byref(nbytes)))
-    assert nbytes.value == size[0] // 2 * (1 << 28)
+        return nbytes.value
+
+    one = size(l=64)
+    assert size(l=128) == 2 * one and size(l=10) == 0 and size(l=64, dk=129) == 0
+    assert size(l=128 * 64, n=2000) == 1000 * 128 * one                 # rows enough for all SMs: whole
+    assert size(l=128 * 64) > 128 * one                                  # few rows in segments, whose ends and starts are kept
+    assert size(n=1 << 14, l=1 << 20) == one // 2 * (1 << 28)            # counted in 64 bits
 
 
 @pytest.mark.parametrize("change,status", [

@@ -102,6 +102,35 @@ def test_prompts(fd, case, dtype, raw, norm):
                 assert not y[i, end:].any()
 
 
+LONG = [   # few rows of many chunks: in segments
+    (2, 1500, 1, 2, 64, 48, "dense", [1500, 700]),
+    (1, 2300, 1, 1, 128, 100, "dense", None),
+    (3, 1300, 1, 1, 40, 20, "odd", [0, 1300, 65]),
+    (1, 1100, 1, 3, 72, 24, "slice", [1031]),
+    (2, 780, 2, 2, 128, 128, "dense", None),
+]
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("case", LONG, ids=[f"{n}x{l}h{g}-{h}k{dk}v{dv}{lay}" for n, l, g, h, dk, dv, lay, _ in LONG])
+def test_long_prompts(fd, case, dtype):
+    test_prompts(fd, case, dtype, True, True)
+
+
+def test_long_prompts_of_few_and_of_many_rows(fd):
+    """A row by itself, cut into segments, and among others, whole: the same but for roundings; where it forgets nothing, too."""
+    g = torch.Generator().manual_seed(13)
+    v, options = inputs(g, 40, 1000, 1, 2, 128, 128, torch.bfloat16, False, True)
+    v["delta"][3] *= 1e-4
+    before = torch.randn(40, 2, 128, 128, generator=g).cuda()
+    y, state = fd.gated_delta_rule(**v, **options, initial_state=before, return_final_state=True)
+    for i in (0, 3):
+        alone = {name: t[i:i + 1] for name, t in v.items()}
+        y1, state1 = fd.gated_delta_rule(**alone, **options, initial_state=before[i:i + 1], return_final_state=True)
+        torch.testing.assert_close(state1, state[i:i + 1], rtol=1e-4, atol=2e-5 * float(state[i].abs().max()))
+        torch.testing.assert_close(y1.float(), y[i:i + 1].float(), rtol=2.0 ** -7, atol=2.0 ** -10 * float(y[i].abs().max()))
+
+
 STEPS = [   # n, key heads, heads, dk, dv, slots
     (1, 1, 1, 16, 16, None), (3, 2, 4, 64, 32, [4, 0, 2]), (4, 1, 3, 33, 17, [1, -1, 9, 0]), (2, 2, 2, 128, 128, None), (70, 1, 2, 72, 100, "all"),
     (5, 4, 4, 200, 48, "all"), (2, 1, 1, 256, 3, None), (3, 1, 2, 128, 1024, "all"), (2, 1, 1, 1, 1, None), (9, 2, 2, 32, 64, "all")]
