@@ -62,7 +62,23 @@ __device__ __forceinline__ float cluster_f32(uint32_t at) {
   return v;
 }
 
-enum class Order { kReduction, kColumns, kAny };   // what lies together in b, in 16-byte pieces; kAny: value by value
+enum class Order { kReduction, kColumns, kAny };   // what lies together in b, in 16-byte pieces; kAny: in pieces of four bytes or value by value
+
+// ACROSS x LINES values to shared memory in pieces of UNIT, neighbouring threads across: a thread keeps its place across, and walks lines.
+// `across_step` and `line_step` are the strides of the source, the bytes those of shared memory; zeros from the bounds on.
+template <typename T, int ACROSS, int LINES, int UNIT>
+__device__ __forceinline__ void few_bytes(uint8_t* smem, int at, int line_bytes, int across_bytes, const T* src, const T* safe, long long line_step,
+                                          long long across_step, int lines, int across) {
+  constexpr int kAcross = ACROSS / UNIT, kBy = kThreads / kAcross;
+  const int place = threadIdx.x % kAcross * UNIT, first = threadIdx.x / kAcross, most = place < across ? lines : 0;
+  src += place * across_step + first * line_step;
+  at += place * across_bytes + first * line_bytes;
+#pragma unroll 8
+  for (int i = first; i < LINES; i += kBy, src += kBy * line_step, at += kBy * line_bytes) {
+    if constexpr (sizeof(T) * UNIT == 4) copy4(smem_u32(smem + at), i < most ? src : safe, i < most);
+    else *reinterpret_cast<T*>(smem + at) = i < most ? *src : from_f32<T>(0.0f);
+  }
+}
 
 // ROWS: of a, 16, 32 or 64 to a block.  WIDE: 16 columns to a warp, times this.  A_WHOLE: 16 bytes of a row of a are copied at once.
 template <typename T, int ROWS, int WIDE, Order ORDER, bool A_WHOLE>
@@ -71,6 +87,7 @@ mm_rows_kernel(const MmRowsParams p, int split) {
   extern __shared__ __align__(128) uint8_t smem_raw[];
   chained();
   constexpr int kV = 16 / int(sizeof(T)), kStep = kTileBytes / int(sizeof(T)), kCols = 16 * WIDE * kWarps, kStages = stages_of(ROWS, kCols);
+  constexpr int kPair = sizeof(T) == 2 ? 2 : 1;
   constexpr int kColTile = kCols * kPitch, kStage = kColTile + ROWS * kPitch;   // (b's tile takes that in either order)
   // columns together: rows of 64 columns, a step of the reduction apart
   constexpr int kColPitch = ORDER == Order::kColumns ? kCols * int(sizeof(T)) + (sizeof(T) == 2 ? 16 : 32) : kPitch;
@@ -101,22 +118,10 @@ mm_rows_kernel(const MmRowsParams p, int split) {
           copy16(smem + at + k * kColPitch + i % kPieces * 16, there ? b0 + (k0 + k) * p.b_s[0] + c : b0, there ? 16 : 0);
         }
       } else {
-        // value by value, threads side by side along what lies together: each keeps its column, or its place in the step
-        const bool along = p.b_s[0] != 1;
-        const int fixed = along ? tid % kCols : tid % kStep, first = along ? tid / kCols : tid / kStep, by = kThreads / (along ? kCols : kStep);
-        const int c0 = along ? fixed : first, kk0 = along ? first : fixed;
-        const bool in = along ? col0 + fixed < p.N : k0 + fixed < p.K;
-        const int most = along ? p.K - k0 : p.N - col0;
-        const T* src = b0 + c0 * p.b_s[1] + (k0 + kk0) * p.b_s[0];
-        const long long next = by * (along ? p.b_s[0] : p.b_s[1]);
-        int dst = at + c0 * kPitch + kk0 * int(sizeof(T));
-        const int dst_next = by * (along ? int(sizeof(T)) : kPitch);
-#pragma unroll 8
-        for (int i = first; i < (along ? kStep : kCols); i += by, src += next, dst += dst_next) {
-          const bool there = in && i < most;
-          if constexpr (sizeof(T) == 4) copy4(smem + dst, there ? src : b0, there);
-          else *reinterpret_cast<T*>(smem_raw + dst) = there ? *src : from_f32<T>(0.0f);
-        }
+        // threads side by side along what lies together; 16-bit pairs go as four bytes where they lie along the reduction at even places
+        if (p.b_s[0] != 1) few_bytes<T, kCols, kStep, 1>(smem_raw, at, int(sizeof(T)), kPitch, b0 + k0 * p.b_s[0], b0, p.b_s[0], p.b_s[1], p.K - k0, p.N - col0);
+        else if (p.b_pairs) few_bytes<T, kStep, kCols, kPair>(smem_raw, at, kPitch, int(sizeof(T)), b0 + k0, b0, p.b_s[1], 1, p.N - col0, p.K - k0);
+        else few_bytes<T, kStep, kCols, 1>(smem_raw, at, kPitch, int(sizeof(T)), b0 + k0, b0, p.b_s[1], 1, p.N - col0, p.K - k0);
       }
       const int a_at = at + kColTile;
       if constexpr (A_WHOLE) {
@@ -127,15 +132,9 @@ mm_rows_kernel(const MmRowsParams p, int split) {
           copy16(smem + a_at + row * kPitch + i % 8 * 16, there ? a0 + row * p.a_s[0] + k : static_cast<const T*>(p.a), there ? 16 : 0);
         }
       } else {
-        const int kk = tid % kStep, by = kThreads / kStep, most = k0 + kk < p.K ? p.M - row0 : 0;
-        const T* src = a0 + tid / kStep * p.a_s[0] + (k0 + kk) * p.a_s[1];
-        int dst = a_at + tid / kStep * kPitch + kk * int(sizeof(T));
-#pragma unroll 8
-        for (int i = tid / kStep; i < ROWS; i += by, src += by * p.a_s[0], dst += by * kPitch) {
-          const bool there = i < most;
-          if constexpr (sizeof(T) == 4) copy4(smem + dst, there ? src : static_cast<const T*>(p.a), there);
-          else *reinterpret_cast<T*>(smem_raw + dst) = there ? *src : from_f32<T>(0.0f);
-        }
+        const T* safe = static_cast<const T*>(p.a);
+        if (p.a_pairs) few_bytes<T, kStep, ROWS, kPair>(smem_raw, a_at, kPitch, int(sizeof(T)), a0 + k0, safe, p.a_s[0], 1, p.M - row0, p.K - k0);
+        else few_bytes<T, kStep, ROWS, 1>(smem_raw, a_at, kPitch, int(sizeof(T)), a0 + k0 * p.a_s[1], safe, p.a_s[0], p.a_s[1], p.M - row0, p.K - k0);
       }
     }
     async_commit();
@@ -258,13 +257,18 @@ cudaError_t go(const MmRowsParams& p, cudaStream_t stream) {
 }
 
 template <typename T>
-cudaError_t by_layout(const MmRowsParams& p, cudaStream_t stream) {
+cudaError_t by_layout(MmRowsParams p, cudaStream_t stream) {
   constexpr int kV = 16 / int(sizeof(T));
   auto whole = [&](const void* q, long long along, long long across, long long extent) {
     return along == 1 && (reinterpret_cast<uintptr_t>(q) & 15u) == 0 && across % kV == 0 && extent % kV == 0;
   };
   const bool a_whole = whole(p.a, p.a_s[1], p.a_s[0], p.K);
   const Order order = whole(p.b, p.b_s[0], p.b_s[1], p.K) ? Order::kReduction : whole(p.b, p.b_s[1], p.b_s[0], p.N) ? Order::kColumns : Order::kAny;
+  auto pairs = [&](const void* q, long long along, long long across) {
+    return sizeof(T) == 2 && along == 1 && (reinterpret_cast<uintptr_t>(q) & 3u) == 0 && across % 2 == 0 && p.K % 2 == 0;
+  };
+  p.a_pairs = pairs(p.a, p.a_s[1], p.a_s[0]);
+  p.b_pairs = pairs(p.b, p.b_s[0], p.b_s[1]);
   auto rows = [&](auto count, auto wide) -> cudaError_t {
     constexpr int R = decltype(count)::value, W = decltype(wide)::value;
     if (order == Order::kReduction) return a_whole ? go<T, R, W, Order::kReduction, true>(p, stream) : go<T, R, W, Order::kReduction, false>(p, stream);
@@ -277,7 +281,8 @@ cudaError_t by_layout(const MmRowsParams& p, cudaStream_t stream) {
   if constexpr (sizeof(T) == 4) {
     // 128 columns split rows of a half as often, 64 spread short reductions over more blocks: us with 64 and with 128, 100 x 2048 x 4096 76 and
     // 53, 1000 x 4096 x 1024 273 and 186, 8192 x 4096 x 4096 5140 and 4370; 3000 x 500 x 500 52 and 62, 300 x 1000 x 777 26 and 31
-    if (p.M > 64 && p.K > 1024) return rows(std::integral_constant<int, 64>{}, std::integral_constant<int, 2>{});
+    const bool many = (p.M + 63ll) / 64 * ((p.N + 127ll) / 128) >= 2 * current_sm_count();
+    if (p.M > 64 && (p.K > 1024 || many)) return rows(std::integral_constant<int, 64>{}, std::integral_constant<int, 2>{});
   }
   return rows(std::integral_constant<int, 64>{}, one);
 }
@@ -285,12 +290,14 @@ cudaError_t by_layout(const MmRowsParams& p, cudaStream_t stream) {
 }  // namespace
 
 // Its time goes with N K and, slowly, with M; the convolution's, on tiles of 128 rows, with K alone as long as they run at once.  16-bit,
-// us here and there: 4096 x 2048 64 rows 12.4 and 15.6, 96 rows 22.3 and 15.6; 2048 x 4096 16 rows 7.9 and 14.0, 32 rows 9.5 and
-// 9.6; 4096 x 8192 16 rows 18.9 and 17.6; 1024 x 1024 32 rows 5.4 and 6.1, 48 rows 6.6 and 6.1; 512 x 4096 16 rows 5.3 and 5.5, 32
-// rows 6.5 and 5.4.  Fewer than eight terms fill no 16 bytes: its paths for few channels add a residual in a step of its own.  Its fp32
-// sums stay in one accumulator (see above).
+// us here and there: K = 4096, N = 2048 64 rows 12.4 and 15.6, 96 rows 22.3 and 15.6; N = 1024 128 rows 12.1 and 15.5, 192 rows 19.4 and
+// 15.5; N = 512 256 rows 12.0 and 15.4, 512 rows 19.4 and 15.5; N = 8192 16 rows 18.9 and 17.6.  K = 8192, N = 1024 128 rows 18.7 and
+// 27.7, 192 rows 32.4 and 27.6.  K = 2048, N = 4096 16 rows 7.9 and 14.0, 32 rows 9.5 and 9.6; N = 256 256 rows 8.5 and 9.3.  K = 1024,
+// N = 1024 32 rows 5.4 and 6.1, 48 rows 6.6 and 6.1; N = 512 64 rows 6.0 and 5.7.  K = 512, N = 4096 16 rows 5.3 and 5.5, 32 rows 6.5 and
+// 5.4.  Fewer than eight terms fill no 16 bytes: the convolution's paths for few channels add a residual in a step of its own.  Its
+// fp32 sums stay in one accumulator (see above).
 bool mm_rows_preferred(int dtype, const MmRowsParams& p) {
-  return p.K < 8 || p.M <= 16 || dtype == FDNN_F32 || (p.M <= 64 && (long long)p.M * p.N <= 32ll * p.K);
+  return p.K < 8 || p.M <= 16 || dtype == FDNN_F32 || (p.M <= (p.K < 4096 ? 512 : 1024) && (long long)p.M * p.N <= (p.K < 4096 ? 32ll * p.K : 131072));
 }
 
 cudaError_t launch_mm_rows(int dtype, const MmRowsParams& p, cudaStream_t stream) {
