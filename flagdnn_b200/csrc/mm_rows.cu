@@ -20,14 +20,19 @@ constexpr int kThreads = 128;
 constexpr int kWarps = kThreads / 32;
 constexpr int kTileBytes = 128;           // of the reduction, a step of the ring
 constexpr int kPitch = kTileBytes + 16;   // eight rows of 16 bytes lie in different banks
-// Steps of the ring: some 90 KB, two blocks to an SM.
-__host__ __device__ constexpr int stages_of(int rows, int cols) { return cols == 128 ? 4 : rows <= 16 ? 8 : rows <= 32 ? 6 : 5; }
+// Steps of the ring: some 90 KB, two blocks to an SM; three of 64 fp32 rows, whose products are what bounds them (3000 x 500 x 500 78 us
+// with two, 52 with three).
+template <typename T>
+__host__ __device__ constexpr int stages_of(int rows, int cols) {
+  return cols == 128 ? 4 : rows <= 16 ? 8 : rows <= 32 ? 6 : sizeof(T) == 4 ? 4 : 5;
+}
 
 __device__ __forceinline__ void copy16(uint32_t to, const void* from, int bytes) {   // the rest of the 16 is zeros
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
 }
-__device__ __forceinline__ void copy4(uint32_t to, const void* from, bool there) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(from), "r"(there ? 4 : 0) : "memory");
+template <int BYTES>
+__device__ __forceinline__ void copy_few(uint32_t to, const void* from, bool there) {   // 4 or 8, or as many zeros
+  asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(to), "l"(from), "n"(BYTES), "r"(there ? BYTES : 0) : "memory");
 }
 template <bool TRANS>
 __device__ __forceinline__ void ldmatrix(uint32_t (&r)[4], uint32_t at) {
@@ -62,7 +67,7 @@ __device__ __forceinline__ float cluster_f32(uint32_t at) {
   return v;
 }
 
-enum class Order { kReduction, kColumns, kAny };   // what lies together in b, in 16-byte pieces; kAny: in pieces of four bytes or value by value
+enum class Order { kReduction, kColumns, kAny };   // what lies together in b, in 16-byte pieces; kAny: in fewer bytes, or value by value
 
 // ACROSS x LINES values to shared memory in pieces of UNIT, neighbouring threads across: a thread keeps its place across, and walks lines.
 // `across_step` and `line_step` are the strides of the source, the bytes those of shared memory; zeros from the bounds on.
@@ -70,12 +75,13 @@ template <typename T, int ACROSS, int LINES, int UNIT>
 __device__ __forceinline__ void few_bytes(uint8_t* smem, int at, int line_bytes, int across_bytes, const T* src, const T* safe, long long line_step,
                                           long long across_step, int lines, int across) {
   constexpr int kAcross = ACROSS / UNIT, kBy = kThreads / kAcross;
+  const uint32_t base = smem_u32(smem);
   const int place = threadIdx.x % kAcross * UNIT, first = threadIdx.x / kAcross, most = place < across ? lines : 0;
   src += place * across_step + first * line_step;
   at += place * across_bytes + first * line_bytes;
 #pragma unroll 8
   for (int i = first; i < LINES; i += kBy, src += kBy * line_step, at += kBy * line_bytes) {
-    if constexpr (sizeof(T) * UNIT == 4) copy4(smem_u32(smem + at), i < most ? src : safe, i < most);
+    if constexpr (sizeof(T) * UNIT >= 4) copy_few<int(sizeof(T)) * UNIT>(base + at, i < most ? src : safe, i < most);
     else *reinterpret_cast<T*>(smem + at) = i < most ? *src : from_f32<T>(0.0f);
   }
 }
@@ -86,8 +92,8 @@ __global__ void __launch_bounds__(kThreads)
 mm_rows_kernel(const MmRowsParams p, int split) {
   extern __shared__ __align__(128) uint8_t smem_raw[];
   chained();
-  constexpr int kV = 16 / int(sizeof(T)), kStep = kTileBytes / int(sizeof(T)), kCols = 16 * WIDE * kWarps, kStages = stages_of(ROWS, kCols);
-  constexpr int kPair = sizeof(T) == 2 ? 2 : 1;
+  constexpr int kV = 16 / int(sizeof(T)), kStep = kTileBytes / int(sizeof(T)), kCols = 16 * WIDE * kWarps, kStages = stages_of<T>(ROWS, kCols);
+  constexpr int kWord = sizeof(T) == 2 ? 2 : 1;   // values in four bytes
   constexpr int kColTile = kCols * kPitch, kStage = kColTile + ROWS * kPitch;   // (b's tile takes that in either order)
   // columns together: rows of 64 columns, a step of the reduction apart
   constexpr int kColPitch = ORDER == Order::kColumns ? kCols * int(sizeof(T)) + (sizeof(T) == 2 ? 16 : 32) : kPitch;
@@ -118,9 +124,10 @@ mm_rows_kernel(const MmRowsParams p, int split) {
           copy16(smem + at + k * kColPitch + i % kPieces * 16, there ? b0 + (k0 + k) * p.b_s[0] + c : b0, there ? 16 : 0);
         }
       } else {
-        // threads side by side along what lies together; 16-bit pairs go as four bytes where they lie along the reduction at even places
+        // threads side by side along what lies together; along the reduction eight or four bytes at once, where all places allow it
         if (p.b_s[0] != 1) few_bytes<T, kCols, kStep, 1>(smem_raw, at, int(sizeof(T)), kPitch, b0 + k0 * p.b_s[0], b0, p.b_s[0], p.b_s[1], p.K - k0, p.N - col0);
-        else if (p.b_pairs) few_bytes<T, kStep, kCols, kPair>(smem_raw, at, kPitch, int(sizeof(T)), b0 + k0, b0, p.b_s[1], 1, p.N - col0, p.K - k0);
+        else if (p.b_bytes == 8) few_bytes<T, kStep, kCols, 2 * kWord>(smem_raw, at, kPitch, int(sizeof(T)), b0 + k0, b0, p.b_s[1], 1, p.N - col0, p.K - k0);
+        else if (p.b_bytes == 4) few_bytes<T, kStep, kCols, kWord>(smem_raw, at, kPitch, int(sizeof(T)), b0 + k0, b0, p.b_s[1], 1, p.N - col0, p.K - k0);
         else few_bytes<T, kStep, kCols, 1>(smem_raw, at, kPitch, int(sizeof(T)), b0 + k0, b0, p.b_s[1], 1, p.N - col0, p.K - k0);
       }
       const int a_at = at + kColTile;
@@ -133,7 +140,8 @@ mm_rows_kernel(const MmRowsParams p, int split) {
         }
       } else {
         const T* safe = static_cast<const T*>(p.a);
-        if (p.a_pairs) few_bytes<T, kStep, ROWS, kPair>(smem_raw, a_at, kPitch, int(sizeof(T)), a0 + k0, safe, p.a_s[0], 1, p.M - row0, p.K - k0);
+        if (p.a_bytes == 8) few_bytes<T, kStep, ROWS, 2 * kWord>(smem_raw, a_at, kPitch, int(sizeof(T)), a0 + k0, safe, p.a_s[0], 1, p.M - row0, p.K - k0);
+        else if (p.a_bytes == 4) few_bytes<T, kStep, ROWS, kWord>(smem_raw, a_at, kPitch, int(sizeof(T)), a0 + k0, safe, p.a_s[0], 1, p.M - row0, p.K - k0);
         else few_bytes<T, kStep, ROWS, 1>(smem_raw, a_at, kPitch, int(sizeof(T)), a0 + k0 * p.a_s[1], safe, p.a_s[0], p.a_s[1], p.M - row0, p.K - k0);
       }
     }
@@ -240,7 +248,7 @@ uint32_t b[ROWS / 8][2], bl[ROWS / 8][2];
 
 template <typename T, int ROWS, int WIDE, Order ORDER, bool A_WHOLE>
 cudaError_t go(const MmRowsParams& p, cudaStream_t stream) {
-  constexpr int kCols = 16 * WIDE * kWarps, kSmem = stages_of(ROWS, kCols) * (kCols + ROWS) * kPitch;
+  constexpr int kCols = 16 * WIDE * kWarps, kSmem = stages_of<T>(ROWS, kCols) * (kCols + ROWS) * kPitch;
   static_assert(ROWS * (kCols + 4) * 4 <= kSmem, "the sums fit");
   static std::atomic<uint64_t> done;
   auto* kernel = mm_rows_kernel<T, ROWS, WIDE, ORDER, A_WHOLE>;
@@ -264,11 +272,14 @@ cudaError_t by_layout(MmRowsParams p, cudaStream_t stream) {
   };
   const bool a_whole = whole(p.a, p.a_s[1], p.a_s[0], p.K);
   const Order order = whole(p.b, p.b_s[0], p.b_s[1], p.K) ? Order::kReduction : whole(p.b, p.b_s[1], p.b_s[0], p.N) ? Order::kColumns : Order::kAny;
-  auto pairs = [&](const void* q, long long along, long long across) {
-    return sizeof(T) == 2 && along == 1 && (reinterpret_cast<uintptr_t>(q) & 3u) == 0 && across % 2 == 0 && p.K % 2 == 0;
+  auto bytes = [&](const void* q, long long along, long long across) {   // that can be copied at once along the reduction
+    if (along != 1) return 0;
+    for (int n = 8; n >= 4; n /= 2)
+      if (reinterpret_cast<uintptr_t>(q) % n == 0 && across * int(sizeof(T)) % n == 0 && (long long)p.K * int(sizeof(T)) % n == 0) return n;
+    return 0;
   };
-  p.a_pairs = pairs(p.a, p.a_s[1], p.a_s[0]);
-  p.b_pairs = pairs(p.b, p.b_s[0], p.b_s[1]);
+  p.a_bytes = bytes(p.a, p.a_s[1], p.a_s[0]);
+  p.b_bytes = bytes(p.b, p.b_s[0], p.b_s[1]);
   auto rows = [&](auto count, auto wide) -> cudaError_t {
     constexpr int R = decltype(count)::value, W = decltype(wide)::value;
     if (order == Order::kReduction) return a_whole ? go<T, R, W, Order::kReduction, true>(p, stream) : go<T, R, W, Order::kReduction, false>(p, stream);

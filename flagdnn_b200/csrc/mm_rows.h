@@ -6,7 +6,7 @@ namespace fdnn {
 
 struct MmRowsParams {
   int M, N, K, act;                                  // a [M, K], b [K, N]
-  bool a_pairs, b_pairs;                             // set by the launcher: 16-bit values lie in aligned pairs along the reduction
+  int a_bytes, b_bytes;                              // set by the launcher: 8, 4, or 0, that lie together and aligned along the reduction
   long long a_s[2], b_s[2], residual_s[2], y_s[2];   // element strides
   const void *a, *b, *bias, *residual;               // bias [N] or null; residual [M, N] or null
   void* y;
