@@ -23,9 +23,10 @@ constexpr int kPitch = kTileBytes + 16;   // eight rows of 16 bytes lie in diffe
 // Steps of the ring: some 90 KB, two blocks to an SM; three of 64 fp32 rows, whose products are what bounds them (3000 x 500 x 500 78 us
 // with two, 52 with three).
 template <typename T>
-__host__ __device__ constexpr int stages_of(int rows, int cols) {
+constexpr int stages_of(int rows, int cols) {
   return cols == 128 ? 4 : rows <= 16 ? 8 : rows <= 32 ? 6 : sizeof(T) == 4 ? 4 : 5;
 }
+constexpr int kShortRing = 4;   // .. four blocks to an SM
 
 __device__ __forceinline__ void copy16(uint32_t to, const void* from, int bytes) {   // the rest of the 16 is zeros
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
@@ -79,20 +80,29 @@ __device__ __forceinline__ void few_bytes(uint8_t* smem, int at, int line_bytes,
   const int place = threadIdx.x % kAcross * UNIT, first = threadIdx.x / kAcross, most = place < across ? lines : 0;
   src += place * across_step + first * line_step;
   at += place * across_bytes + first * line_bytes;
-#pragma unroll 8
-  for (int i = first; i < LINES; i += kBy, src += kBy * line_step, at += kBy * line_bytes) {
-    if constexpr (sizeof(T) * UNIT >= 4) copy_few<int(sizeof(T)) * UNIT>(base + at, i < most ? src : safe, i < most);
-    else *reinterpret_cast<T*>(smem + at) = i < most ? *src : from_f32<T>(0.0f);
+  constexpr int kCount = LINES / kBy;
+  if constexpr (sizeof(T) * UNIT >= 4) {
+#pragma unroll
+    for (int n = 0; n < kCount; ++n, src += kBy * line_step, at += kBy * line_bytes) {
+      const bool there = first + n * kBy < most;
+      copy_few<int(sizeof(T)) * UNIT>(base + at, there ? src : safe, there);
+    }
+  } else {   // (two bytes cannot be copied asynchronously: all on their way before the first is stored)
+    T v[kCount];
+#pragma unroll
+    for (int n = 0; n < kCount; ++n, src += kBy * line_step) v[n] = first + n * kBy < most ? *src : from_f32<T>(0.0f);
+#pragma unroll
+    for (int n = 0; n < kCount; ++n, at += kBy * line_bytes) *reinterpret_cast<T*>(smem + at) = v[n];
   }
 }
 
 // ROWS: of a, 16, 32 or 64 to a block.  WIDE: 16 columns to a warp, times this.  A_WHOLE: 16 bytes of a row of a are copied at once.
-template <typename T, int ROWS, int WIDE, Order ORDER, bool A_WHOLE>
+template <typename T, int ROWS, int WIDE, Order ORDER, bool A_WHOLE, int STAGES>
 __global__ void __launch_bounds__(kThreads)
 mm_rows_kernel(const MmRowsParams p, int split) {
   extern __shared__ __align__(128) uint8_t smem_raw[];
   chained();
-  constexpr int kV = 16 / int(sizeof(T)), kStep = kTileBytes / int(sizeof(T)), kCols = 16 * WIDE * kWarps, kStages = stages_of<T>(ROWS, kCols);
+  constexpr int kV = 16 / int(sizeof(T)), kStep = kTileBytes / int(sizeof(T)), kCols = 16 * WIDE * kWarps;
   constexpr int kWord = sizeof(T) == 2 ? 2 : 1;   // values in four bytes
   constexpr int kColTile = kCols * kPitch, kStage = kColTile + ROWS * kPitch;   // (b's tile takes that in either order)
   // columns together: rows of 64 columns, a step of the reduction apart
@@ -107,7 +117,7 @@ mm_rows_kernel(const MmRowsParams p, int split) {
 
   auto ask = [&](int step) {
     if (step < to) {
-      const int at = (step - from) % kStages * kStage, k0 = step * kStep;
+      const int at = (step - from) % STAGES * kStage, k0 = step * kStep;
       if constexpr (ORDER == Order::kReduction) {
 #pragma unroll
         for (int i = tid; i < kCols * 8; i += kThreads) {
@@ -150,12 +160,12 @@ mm_rows_kernel(const MmRowsParams p, int split) {
 
   float sum[WIDE][ROWS / 8][4] = {};
 #pragma unroll
-  for (int i = 0; i < kStages - 1; ++i) ask(from + i);
+  for (int i = 0; i < STAGES - 1; ++i) ask(from + i);
   for (int step = from; step < to; ++step) {
-    async_wait<kStages - 2>();
+    async_wait<STAGES - 2>();
     __syncthreads();
-    ask(step + kStages - 1);
-    const int at = (step - from) % kStages * kStage;
+    ask(step + STAGES - 1);
+    const int at = (step - from) % STAGES * kStage;
     float d[WIDE][ROWS / 8][4] = {};
     if constexpr (sizeof(T) == 2) {
       static_assert(WIDE == 1, "wide blocks are fp32's");
@@ -225,10 +235,10 @@ uint32_t b[ROWS / 8][2], bl[ROWS / 8][2];
       for (int i = 0; i < 4; ++i) sums[(j * 8 + 2 * t + (i & 1)) * kSumPitch + (warp * WIDE + n) * 16 + g + (i >> 1) * 8] = sum[n][j][i];
   if (split > 1) cluster_sync_all();
   else __syncthreads();
-  const int share = kCols / split, rows = min(ROWS, p.M - row0);
+  const int share = kCols / split, c0 = rank * share, rows = min(ROWS, p.M - row0);
   with_activation(p.act, [&](auto act) {
     for (int i = tid; i < rows * share; i += kThreads) {
-      const int row = i / share, c = rank * share + i % share;
+      const int row = i / share, c = c0 + i % share;
       const uint32_t at = smem + uint32_t(row * kSumPitch + c) * 4;
       float v = 0.0f;
       if (split > 1) {
@@ -248,20 +258,36 @@ uint32_t b[ROWS / 8][2], bl[ROWS / 8][2];
 
 template <typename T, int ROWS, int WIDE, Order ORDER, bool A_WHOLE>
 cudaError_t go(const MmRowsParams& p, cudaStream_t stream) {
-  constexpr int kCols = 16 * WIDE * kWarps, kSmem = stages_of<T>(ROWS, kCols) * (kCols + ROWS) * kPitch;
-  static_assert(ROWS * (kCols + 4) * 4 <= kSmem, "the sums fit");
-  static std::atomic<uint64_t> done;
-  auto* kernel = mm_rows_kernel<T, ROWS, WIDE, ORDER, A_WHOLE>;
-  const cudaError_t e = allow_smem(kernel, kSmem, done);
-  if (e != cudaSuccess) return e;
+  constexpr int kCols = 16 * WIDE * kWarps, kStep = kTileBytes / int(sizeof(T));
   const long long tiles = (p.N + kCols - 1) / kCols, row_blocks = (p.M + ROWS - 1) / ROWS;
-  const int steps = (p.K + kTileBytes / int(sizeof(T)) - 1) / (kTileBytes / int(sizeof(T)));
-  // up to two blocks an SM, which all run at once, as long as each has two steps: 2048 x 4096 bf16, one row, 9.8 / 8.1 / 6.1 / 9.0 us in
-  // 1 / 2 / 4 / 8 parts (64 to 512 blocks), 4096 x 8192 20.8 / 16.0 / 18.5 / 23.4 (128 to 1024)
-  int split = 1;
-  while (split < 8 && tiles * row_blocks * split <= current_sm_count() && steps >= 4 * split) split *= 2;
-  if (tiles * split > 0x7fffffffll || row_blocks > 65535) return cudaErrorInvalidConfiguration;
-  return launch_seq(kernel, dim3(unsigned(tiles * split), unsigned(row_blocks)), kThreads, kSmem, split, stream, p, split);
+  const int steps = (p.K + kStep - 1) / kStep;
+  if (tiles > 0x7fffffffll / 8 || row_blocks > 65535) return cudaErrorInvalidConfiguration;
+  // parts of the reduction: as many blocks as run at once, as long as each has two steps
+  auto split_of = [&](int at_once) {
+    int split = 1;
+    while (split < 8 && 2 * split * tiles * row_blocks <= (long long)at_once * current_sm_count() && steps >= 4 * split) split *= 2;
+    return split;
+  };
+  auto run = [&](auto stages, int split) -> cudaError_t {
+    constexpr int kStages = decltype(stages)::value, kSmem = kStages * (kCols + ROWS) * kPitch;
+    static_assert(ROWS * (kCols + 4) * 4 <= kSmem, "the sums fit");
+    static std::atomic<uint64_t> done;
+    auto* kernel = mm_rows_kernel<T, ROWS, WIDE, ORDER, A_WHOLE, kStages>;
+    const cudaError_t e = allow_smem(kernel, kSmem, done);
+    if (e != cudaSuccess) return e;
+    return launch_seq(kernel, dim3(unsigned(tiles * split), unsigned(row_blocks)), kThreads, kSmem, split, stream, p, split);
+  };
+  // One row, bf16, two blocks to an SM, 2048 x 4096 9.8 / 8.1 / 6.1 / 9.0 us in 1 / 2 / 4 / 8 parts (64 to 512 blocks), 4096 x 8192 20.8 / 16.0 /
+  // 18.5 / 23.4 (128 to 1024).  Where two parts too many would not run at once (7264 x 2432: 152 blocks of 4 parts 15.5 us), blocks of half the
+  // ring do, four to an SM (304 of 8 parts 12.7; 4096 x 2048, 256 blocks either way, 6.3 and 7.9).
+  constexpr int kStages = stages_of<T>(ROWS, kCols);
+  constexpr int kAtOnce = 227 * 1024 / (kStages * (kCols + ROWS) * kPitch + 1024);
+  const int split = split_of(kAtOnce);
+  if constexpr (kStages > 2 * kShortRing - 1) {
+    const int more = split_of(2 * kAtOnce);
+    if (more > split && 4 * split * tiles * row_blocks < 3ll * kAtOnce * current_sm_count()) return run(std::integral_constant<int, kShortRing>{}, more);
+  }
+  return run(std::integral_constant<int, kStages>{}, split);
 }
 
 template <typename T>
