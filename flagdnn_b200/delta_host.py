@@ -65,7 +65,9 @@ def gated_delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, delta: t
     ``q`` and ``k`` [N, L, G, K]: each key head serves ``H / G`` neighbouring heads; with ``qk_norm`` they are divided by
     ``sqrt(sum of squares + 1e-6)``.  ``delta`` and ``beta`` [N, L, H] are of ``v``'s type or float32, ``A`` and ``delta_bias`` [H]
     float32; ``scale`` is ``K ** -0.5`` if None.  ``initial_state`` and the returned state are float32 [N, H, V, K].
-    Prompts are taken in chunks of 64 tokens: an input that is not finite can make its whole chunk not finite."""
+    Prompts are taken in chunks of 64 tokens: an input that is not finite can make its whole chunk not finite, and decays above one are
+    taken as long as a chunk's product of them is an fp32 number. Long rows are cut into segments where few rows and heads run: a
+    row's last bits can depend on its batch."""
     what = "gated_delta_rule"
     fast = _conv._fast or _conv.native_host()
     if fast:

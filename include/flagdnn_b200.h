@@ -359,7 +359,8 @@ int fdnn_selective_scan_step(const fdnn_scan_desc* desc, const void* u, const vo
  * sqrt(sum of their squares + 1e-6) first.  A and delta_bias [heads] and the states [N, heads, dv, dk] are dense float32;
  * delta_bias, A, initial_state (zeros), lengths (see above) and final_state may be NULL.  final_state must not overlap
  * initial_state.  Longer prompts are taken in chunks of 64 tokens: a q, k, v, delta or beta that is not finite can make the whole chunk
- * that it lies in not finite, its earlier tokens too. */
+ * that it lies in not finite, its earlier tokens too; decays above one are taken as long as a chunk's product of them is an fp32 number.
+ * Long rows are cut into segments where few rows and heads run: a row's last bits can depend on its batch. */
 #define FDNN_DELTA_RULE_MAX_DK 256
 #define FDNN_DELTA_RULE_MAX_DV 1024
 #define FDNN_DELTA_RULE_MAX_HEADS 65535
@@ -391,7 +392,8 @@ int fdnn_gated_delta_rule_step(const fdnn_delta_rule_desc* desc, const void* q, 
                                int32_t n_slots, const int32_t* slots, void* y, void* stream);
 
 /* A product of few rows with its epilogue: y = act(a b + bias + residual), a [m, k], b [k, n] of any strides, bias [n] dense or NULL,
- * residual [m, n] or NULL; fp32 sums, one rounding.  fdnn_mm_rows_fwd takes any m (at most 2^22), but is made for a reading of b:
+ * residual [m, n] or NULL; fp32 sums, one rounding (an infinite fp32 operand makes NaN: it goes in as two parts).  fdnn_mm_rows_fwd
+ * takes any m (at most 2^22), but is made for a reading of b:
  * fdnn_mm_rows_preferred says whether it is ahead of the product as a 1x1 convolution (fdnn_conv2d_fwd_residual on a row of m pixels). */
 typedef struct fdnn_mm_desc {
   int32_t dtype;               /* FDNN_F16, FDNN_BF16 or FDNN_F32: every tensor */
