@@ -1202,10 +1202,11 @@ uint32_t* device_status_word() {
   return static_cast<uint32_t*>(p);
 }
 
-void bounded_wait_of(uint32_t** status, long long* limit) {
+void bounded_wait_of(uint32_t** status, long long* limit, int* skip_copies) {
   static std::atomic<uint32_t*> words[64];
   const long long set = g_wait_limit.load(std::memory_order_relaxed);
   *limit = set > 0 ? set : default_wait_limit_cycles();
+  *skip_copies = g_skip_copies.load(std::memory_order_relaxed);
   *status = nullptr;
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return;

@@ -179,8 +179,9 @@ bool encode_depthwise_map(CUtensorMap* tm, int dtype, const DirectParams& p, int
 bool depthwise_ring_ok(int dtype, const DirectParams& p);
 cudaError_t launch_depthwise_ring(int dtype, const DirectParams& d, uint32_t* status, long long wait_limit, cudaStream_t stream);
 int current_sm_count();   // of the current device (148 when none is visible)
-// What a kernel with bounded waits needs: the current device's status word (null if it cannot be had) and the limit in force.
-void bounded_wait_of(uint32_t** status, long long* limit);
+// What a kernel with bounded waits needs: the current device's status word (null if it cannot be had), the limit in force, and whether its copies
+// are skipped (fdnn_debug_set_wait_limit).
+void bounded_wait_of(uint32_t** status, long long* limit, int* skip_copies);
 cudaError_t launch_depthwise(int dtype, const DirectParams& p, int kind, cudaStream_t stream);
 
 // Pooling (pool.cu): element strides of x and y in (n, c, h, w) order; idx (max pooling only) may be null.

@@ -7,9 +7,9 @@
 //   S    <- e^(G_64) S + sum over j of e^(G_64 - G_j) U_j k_j^T
 // delta_prepare_kernel makes, for all chunks side by side, what does not need S: T, P_ij = scale D_ij (q_i . k_j), the keys and queries as
 // 16-bit operands and the factors of each token.  delta_chunks_kernel then walks a head's chunks in order.  A state's rows do
-// not meet, so a warp keeps 16 of them in registers, for the whole prompt, as the transposed accumulators of its own products: with rows
-// as the M side, S, v - S k, U and e^.. U are in turn the accumulators of one product and the A operand of the next, without a
-// word of shared memory between them, and no warp waits for another but for operands.
+// not meet, so two warps keep 16 of them in registers for the whole prompt, half of the keys' channels each, as the accumulators of their own
+// products: with rows as the M side, S, v - S k, U and e^.. U are in turn the accumulators of one product and the A operand of the next.
+// Through shared memory go only the halves of S k and of U, to each other, and S and U, to the warps that make y beside them.
 //
 // Precision.  The tensor cores take 16 bits.  Keys and queries that come as f16 or bf16 are f16 operands exactly: each token's is
 // scaled by a power of two to a largest value of 2^14 .. 2^15 (a bf16 value below 2^-29 of that loses bits that fp32 sums do not see).
@@ -644,6 +644,7 @@ struct Run {
   float* ends;           // null, or [N, H, segments - 1, V rounded up to 16 + K, K]: of all but the last
   uint32_t* status;
   long long wait_limit;
+  int skip_copies;       // a test of the bounded waits
 };
 
 // WHOLE: 16 bytes of neighbouring value channels are copied and stored at once.
@@ -711,7 +712,7 @@ delta_chunks_kernel(const DeltaParams p, const Run run) {
     int asked = 0;   // chunks, by the loader
     auto ask = [&](int c) {
       uint8_t* const to = smem_raw + (c % stages) * stage_bytes;
-      if (loader && asked == c) {
+      if (loader && asked == c && !run.skip_copies) {
         uint64_t* bar = &full[c % stages];
         if (c < stages || mbar_wait_bounded(&empty[c % stages], uint32_t(c / stages - 1) & 1u, &abort_word, run.status, kIncidentDeltaWait, run.wait_limit)) {
           mbar_arrive_expect_tx(bar, W::kStage);
@@ -1220,7 +1221,7 @@ cudaError_t run(const DeltaParams& p, cudaStream_t stream) {
 
   const bool values_whole = p.V % (16 / int(sizeof(T))) == 0 && eights<T>(p.v, p.v_s) && eights<T>(p.y, p.y_s);
   Run r = {};
-  bounded_wait_of(&r.status, &r.wait_limit);
+  bounded_wait_of(&r.status, &r.wait_limit, &r.skip_copies);
   if (r.status == nullptr) return cudaErrorInvalidSymbol;
   auto go = [&](auto* kernel, std::atomic<uint64_t>& allowed, int slices, long long blocks) -> cudaError_t {
     const cudaError_t err = allow_smem(kernel, kMostSmem, allowed);

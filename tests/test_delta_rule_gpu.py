@@ -299,6 +299,31 @@ def test_the_python_route_gives_the_same(fd, monkeypatch):
     assert torch.equal(*states) and states[1]._version > version and states[0]._version > 0
 
 
+def test_a_wait_that_runs_out_is_reported_and_the_device_stays_usable(fd, native_lib):
+    """No copy is issued: the first wait for a chunk's operands runs out after some 0.1 ms of clocks, the launches return, and the next
+    call is as before. A whole row and one in segments."""
+    import ctypes
+
+    from flagdnn_b200 import _native as nat
+
+    g = torch.Generator().manual_seed(14)
+    for rows, length in ((40, 130), (1, 1200)):
+        v, options = inputs(g, rows, length, 1, 2, 64, 64, torch.bfloat16, True, True)
+        good = fd.gated_delta_rule(**v, **options)
+        torch.cuda.synchronize()
+        assert fd.device_status() == 0
+        nat.check(native_lib.fdnn_debug_set_wait_limit(200_000, 1))
+        try:
+            fd.gated_delta_rule(**v, **options)
+            torch.cuda.synchronize()
+        finally:
+            nat.check(native_lib.fdnn_debug_set_wait_limit(0, 0))
+        word = ctypes.c_uint32(0)
+        assert native_lib.fdnn_device_status(ctypes.byref(word)) == nat.FDNN_DEVICE_TIMEOUT and word.value == 9
+        assert native_lib.fdnn_device_status(ctypes.byref(word)) == nat.FDNN_OK
+        assert torch.equal(fd.gated_delta_rule(**v, **options), good) and fd.device_status() == 0
+
+
 def test_refusals(fd):
     g = torch.Generator().manual_seed(12)
     v, options = inputs(g, 2, 10, 1, 2, 16, 16, torch.float16, True, True)
