@@ -73,6 +73,11 @@ __device__ __forceinline__ void copy16(uint32_t to, const void* from, int bytes)
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
 }
 
+template <int THREADS>
+__device__ __forceinline__ void barrier(int id) { asm volatile("bar.sync %0, %1;" ::"r"(id), "n"(THREADS) : "memory"); }
+template <int THREADS>
+__device__ __forceinline__ void barrier_arrive(int id) { asm volatile("bar.arrive %0, %1;" ::"r"(id), "n"(THREADS) : "memory"); }
+
 // A power of two that takes `most` to 2^14 .. 2^15 (an exponent that it cannot have is cut; of infinity or NaN, some power).
 __device__ __forceinline__ float raise(float most) {
   const int e = 268 - int((__float_as_uint(most) >> 23) & 255u);
@@ -180,7 +185,8 @@ __device__ __forceinline__ int row_end(const DeltaParams& p, long long n) {
 
 // ---- what does not need the state ----------------------------------------------------------------------------------
 
-constexpr int kPrepThreads = 128;
+// Eight warps to a chunk of a key head: four make a and solve it, four make P meanwhile.
+constexpr int kPrepThreads = 256, kSolvers = 128, kSolveId = 1;
 constexpr int kPitch = kChunk + 4;   // floats between rows of A, T
 
 struct HeadGates {
@@ -198,63 +204,58 @@ struct PrepShared {
   HeadGates gates[4];
 };
 
-// Keys or queries of a chunk, on their way to shared memory.  A warp takes 8 rows at once, four lanes a row, so that what they write is 128
-// bytes in a run; two passes make 64 rows.  All loads of a chunk are on their way before the first is waited for.
+// Keys or queries of a chunk, on their way to shared memory.  A warp takes 8 rows, four lanes a row, so that what they write is 128 bytes
+// in a run.  All loads of a chunk are on their way before the first is waited for.
 template <typename T, int KEYS, bool WHOLE>
 struct Rows {
   static constexpr int kPieces = KEYS / 32, kV = WHOLE ? 16 / int(sizeof(T)) : 1;   // pieces of eight channels, to a lane
-  Pack<T, kV> raw[2][kPieces][8 / kV];
-  static __device__ __forceinline__ int row(int pass) { return (pass * 4 + (threadIdx.x >> 5)) * 8 + (threadIdx.x & 7); }
+  Pack<T, kV> raw[kPieces][8 / kV];
+  static __device__ __forceinline__ int row() { return (threadIdx.x >> 5) * 8 + (threadIdx.x & 7); }
   static __device__ __forceinline__ int channel(int n) { return (n * 4 + ((threadIdx.x & 31) >> 3)) * 8; }
   __device__ __forceinline__ void load(const T* x, const long long* s, int tokens, int K) {
 #pragma unroll
-    for (int pass = 0; pass < 2; ++pass)
+    for (int n = 0; n < kPieces; ++n)
 #pragma unroll
-      for (int n = 0; n < kPieces; ++n)
-#pragma unroll
-        for (int i = 0; i < 8 / kV; ++i) {
-          const int at = channel(n) + i * kV;
-          raw[pass][n][i].clear();
-          if (row(pass) < tokens && at < K) raw[pass][n][i].load(x + row(pass) * s[1] + (WHOLE ? (long long)at : at * s[3]));
-        }
+      for (int i = 0; i < 8 / kV; ++i) {
+        const int at = channel(n) + i * kV;
+        raw[n][i].clear();
+        if (row() < tokens && at < K) raw[n][i].load(x + row() * s[1] + (WHOLE ? (long long)at : at * s[3]));
+      }
   }
   // To their places, as parts, scaled; the factors that take the operands back (with the norm, if asked, and `scale`).
   __device__ __forceinline__ void stage(uint8_t* to, float* factor, int tokens, bool norm, float scale) const {
+    float most = 0.0f, squares = 0.0f;
 #pragma unroll
-    for (int pass = 0; pass < 2; ++pass) {
-      float most = 0.0f, squares = 0.0f;
+    for (int n = 0; n < kPieces; ++n)
 #pragma unroll
-      for (int n = 0; n < kPieces; ++n)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float v = raw[pass][n][j / kV].at(j % kV);
-          most = fmaxf(most, fabsf(v));
-          squares += v * v;
-        }
-#pragma unroll
-      for (int o = 8; o < 32; o <<= 1) {
-        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-        squares += __shfl_xor_sync(0xffffffffu, squares, o);
+      for (int j = 0; j < 8; ++j) {
+        const float v = raw[n][j / kV].at(j % kV);
+        most = fmaxf(most, fabsf(v));
+        squares += v * v;
       }
-      const float up = raise(most);
-      const int r = row(pass);
 #pragma unroll
-      for (int n = 0; n < kPieces; ++n) {
-        uint4 hi, lo;
-        uint32_t* h = reinterpret_cast<uint32_t*>(&hi);
-        uint32_t* l = reinterpret_cast<uint32_t*>(&lo);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const F2 x = f2_mul(f2_pack(raw[pass][n][2 * j / kV].at(2 * j % kV), raw[pass][n][(2 * j + 1) / kV].at((2 * j + 1) % kV)), f2_both(up));
-          h[j] = high(x);
-          if constexpr (Parts<T>::kKey == 2) l[j] = low(x, h[j]);
-        }
-        const int at = piece(r, channel(n) / 8, KEYS / 16);
-        *reinterpret_cast<uint4*>(to + at) = hi;
-        if constexpr (Parts<T>::kKey == 2) *reinterpret_cast<uint4*>(to + kChunk * KEYS * 2 + at) = lo;
-      }
-      if ((threadIdx.x & 31) < 8) factor[r] = r < tokens ? scale * inverse_of_power(up) * (norm ? 1.0f / sqrtf(squares + kKeyEps) : 1.0f) : 0.0f;
+    for (int o = 8; o < 32; o <<= 1) {
+      most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+      squares += __shfl_xor_sync(0xffffffffu, squares, o);
     }
+    const float up = raise(most);
+    const int r = row();
+#pragma unroll
+    for (int n = 0; n < kPieces; ++n) {
+      uint4 hi, lo;
+      uint32_t* h = reinterpret_cast<uint32_t*>(&hi);
+      uint32_t* l = reinterpret_cast<uint32_t*>(&lo);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const F2 x = f2_mul(f2_pack(raw[n][2 * j / kV].at(2 * j % kV), raw[n][(2 * j + 1) / kV].at((2 * j + 1) % kV)), f2_both(up));
+        h[j] = high(x);
+        if constexpr (Parts<T>::kKey == 2) l[j] = low(x, h[j]);
+      }
+      const int at = piece(r, channel(n) / 8, KEYS / 16);
+      *reinterpret_cast<uint4*>(to + at) = hi;
+      if constexpr (Parts<T>::kKey == 2) *reinterpret_cast<uint4*>(to + kChunk * KEYS * 2 + at) = lo;
+    }
+    if ((threadIdx.x & 31) < 8) factor[r] = r < tokens ? scale * inverse_of_power(up) * (norm ? 1.0f / sqrtf(squares + kKeyEps) : 1.0f) : 0.0f;
   }
 };
 
@@ -386,7 +387,7 @@ __device__ __forceinline__ void invert(const float (&a)[kChunk][kPitch], float (
       for (int i = 0; i < 16; ++i) t[at + i][at + c] = x[i];
     }
   }
-  __syncthreads();
+  barrier<kSolvers>(kSolveId);
   if (warp < 2) {   // blocks (1, 0) and (3, 2)
     const int i = warp * 32 + 16, j = warp * 32;
     float d[2][4] = {};
@@ -397,22 +398,22 @@ __device__ __forceinline__ void invert(const float (&a)[kChunk][kPitch], float (
     block_product(e, &t[i][i], kPitch, &part[warp][0][0], 20);
     put_block(&t[i][j], kPitch, e, -1.0f);
   }
-  __syncthreads();
+  barrier<kSolvers>(kSolveId);
   {   // the lower left 32 x 32: part = a t, then t part
     const int i = 32 + (warp >> 1) * 16, j = (warp & 1) * 16;
     float d[2][4] = {};
     for (int m = j; m < 32; m += 16) block_product(d, &a[i][m], kPitch, &t[m][j], kPitch);
     put_block(&part[warp][0][0], 20, d, 1.0f);
-    __syncthreads();
+    barrier<kSolvers>(kSolveId);
     float e[2][4] = {};
     for (int m = 32; m <= i; m += 16) block_product(e, &t[i][m], kPitch, &part[(m - 32) / 16 * 2 + (warp & 1)][0][0], 20);
     put_block(&t[i][j], kPitch, e, -1.0f);
   }
-  __syncthreads();
+  barrier<kSolvers>(kSolveId);
 }
 
 template <typename T, int KEYS, bool WHOLE>
-__global__ void __launch_bounds__(kPrepThreads, 3)
+__global__ void __launch_bounds__(kPrepThreads, 2)
 delta_prepare_kernel(const DeltaParams p) {
   extern __shared__ __align__(128) uint8_t smem_raw[];
   PrepShared<T, KEYS>& s = *reinterpret_cast<PrepShared<T, KEYS>*>(smem_raw);
@@ -423,28 +424,20 @@ delta_prepare_kernel(const DeltaParams p) {
   const long long n = blockIdx.x / p.G / w.chunks;
   const int begin = c * kChunk, tokens = min(row_end(p, n) - begin, kChunk);
   if (tokens <= 0) return;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, q = lane >> 2, t = lane & 3;
+  const int tid = threadIdx.x, lane = tid & 31, q = lane >> 2, t = lane & 3;
+  const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0), block = warp & 3;   // of 16 tokens
+  const bool solver = warp < 4;
   uint8_t* const queries = s.keys + W::kKeyBytes;
   const int group = p.H / p.G, h0 = g * group;
   {
-    const T* kp = static_cast<const T*>(p.k) + n * p.k_s[0] + begin * p.k_s[1] + g * p.k_s[2];
-    const T* qp = static_cast<const T*>(p.q) + n * p.q_s[0] + begin * p.q_s[1] + g * p.q_s[2];
     RawGates gates;
-    if (warp < group) load_gates<T>(p, gates, n, begin, tokens, h0 + warp);
-    Rows<T, KEYS, WHOLE> rows;
-    rows.load(kp, p.k_s, tokens, p.K);
-    if constexpr (sizeof(T) == 2 && WHOLE) {   // (the queries' registers, too)
-      Rows<T, KEYS, WHOLE> more;
-      more.load(qp, p.q_s, tokens, p.K);
-      if (warp < group) sum_gates(p, gates, s.gates[warp], tokens);
-      rows.stage(s.keys, s.key_scale, tokens, p.norm, 1.0f);
-      more.stage(queries, s.query_scale, tokens, p.norm, p.scale);
-    } else {
-      if (warp < group) sum_gates(p, gates, s.gates[warp], tokens);
-      rows.stage(s.keys, s.key_scale, tokens, p.norm, 1.0f);
-      rows.load(qp, p.q_s, tokens, p.K);
-      rows.stage(queries, s.query_scale, tokens, p.norm, p.scale);
-    }
+    if (warp < 4 && warp < group) load_gates<T>(p, gates, n, begin, tokens, h0 + warp);
+    Rows<T, KEYS, WHOLE> rows, more;
+    rows.load(static_cast<const T*>(p.k) + n * p.k_s[0] + begin * p.k_s[1] + g * p.k_s[2], p.k_s, tokens, p.K);
+    more.load(static_cast<const T*>(p.q) + n * p.q_s[0] + begin * p.q_s[1] + g * p.q_s[2], p.q_s, tokens, p.K);
+    if (warp < 4 && warp < group) sum_gates(p, gates, s.gates[warp], tokens);
+    rows.stage(s.keys, s.key_scale, tokens, p.norm, 1.0f);
+    more.stage(queries, s.query_scale, tokens, p.norm, p.scale);
   }
   fence_proxy_async_smem();
   __syncthreads();
@@ -452,17 +445,16 @@ delta_prepare_kernel(const DeltaParams p) {
     bulk_store_1d(w.keys + ((n * p.G + g) * w.chunks + c) * (2ll * W::kKeyBytes), s.keys, 2 * W::kKeyBytes);
     bulk_commit_group();
   }
-  float kk[8][4] = {}, qk[8][4] = {};
-  dots<T, KEYS>(kk, s.keys, s.keys, warp);
-  dots<T, KEYS>(qk, queries, s.keys, warp);
-  const int r0 = warp * 16 + q;
+  float dot[8][4] = {};   // k_i . k_j of these 16 tokens, or q_i . k_j
+  dots<T, KEYS>(dot, solver ? s.keys : queries, s.keys, block);
+  const int r0 = block * 16 + q;
   {   // the factors of the rows and columns
-    const float k0 = s.key_scale[r0], k1 = s.key_scale[r0 + 8], q0 = s.query_scale[r0], q1 = s.query_scale[r0 + 8];
+    const float* of_row = solver ? s.key_scale : s.query_scale;
+    const float f0 = of_row[r0], f1 = of_row[r0 + 8];
 #pragma unroll
     for (int m = 0; m < 8; ++m) {
       const float2 f = *reinterpret_cast<const float2*>(&s.key_scale[m * 8 + 2 * t]);
-      kk[m][0] *= k0 * f.x, kk[m][1] *= k0 * f.y, kk[m][2] *= k1 * f.x, kk[m][3] *= k1 * f.y;
-      qk[m][0] *= q0 * f.x, qk[m][1] *= q0 * f.y, qk[m][2] *= q1 * f.x, qk[m][3] *= q1 * f.y;
+      dot[m][0] *= f0 * f.x, dot[m][1] *= f0 * f.y, dot[m][2] *= f1 * f.x, dot[m][3] *= f1 * f.y;
     }
   }
   if (tid == 0) bulk_wait_group_read0();
@@ -470,7 +462,8 @@ delta_prepare_kernel(const DeltaParams p) {
 
   for (int i = 0; i < group; ++i) {
     if (i > 0 && (i & 3) == 0) {
-      if (i + warp < group) {
+      __syncthreads();
+      if (warp < 4 && i + warp < group) {
         RawGates raw;
         load_gates<T>(p, raw, n, begin, tokens, h0 + i + warp);
         sum_gates(p, raw, s.gates[warp], tokens);
@@ -480,87 +473,72 @@ delta_prepare_kernel(const DeltaParams p) {
     const HeadGates& gates = s.gates[i & 3];
     uint8_t* out = w.heads + ((n * p.H + h0 + i) * w.chunks + c) * (long long)W::kHeadBytes;
     float* factors = reinterpret_cast<float*>(out + (2 + Parts<T>::kOut) * kLower);
-    if (tid < kChunk) {
-      const float hi = gates.hi[tid], lo = gates.lo[tid], since = exp2_of(hi, lo);
-      factors[tid] = -since * s.key_scale[tid];
-      factors[kChunk + tid] = since * s.query_scale[tid];
-      factors[2 * kChunk + tid] = exp2_of(gates.hi[kChunk - 1] - hi, gates.lo[kChunk - 1] - lo) * s.key_scale[tid];
-      if (tid == kChunk - 1) factors[5 * kChunk] = since;
+    // a or P, of this warp's 16 tokens
+    float hi[2], lo[2], beta[2], most[2] = {0.0f, 0.0f}, v[8][4];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      hi[j] = gates.hi[r0 + 8 * j];
+      lo[j] = gates.lo[r0 + 8 * j];
+      beta[j] = solver ? gates.beta[r0 + 8 * j] : 1.0f;
     }
-    // a and P, from this warp's 16 rows
-    {
-      float hi[2], lo[2], beta[2], most[2] = {0.0f, 0.0f}, pm[8][4];
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        hi[j] = gates.hi[r0 + 8 * j];
-        lo[j] = gates.lo[r0 + 8 * j];
-        beta[j] = gates.beta[r0 + 8 * j];
-      }
+    for (int m = 0; m < 8; ++m)
+      if (m < 2 * (block + 1)) {
+        const int col = m * 8 + 2 * t;
+        const float2 chi = *reinterpret_cast<const float2*>(&gates.hi[col]), clo = *reinterpret_cast<const float2*>(&gates.lo[col]);
 #pragma unroll
-      for (int m = 0; m < 8; ++m)
-        if (m < 2 * (warp + 1)) {
-          const int col = m * 8 + 2 * t;
-          const float2 chi = *reinterpret_cast<const float2*>(&gates.hi[col]), clo = *reinterpret_cast<const float2*>(&gates.lo[col]);
-          float av[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int row = r0 + (j >> 1) * 8, at = col + (j & 1);
-            const float d = ex2((hi[j >> 1] - ((j & 1) ? chi.y : chi.x)) + (lo[j >> 1] - ((j & 1) ? clo.y : clo.x)));
-            av[j] = at < row ? kk[m][j] * (beta[j >> 1] * d) : 0.0f;
-            pm[m][j] = at <= row ? qk[m][j] * d : 0.0f;
-            most[j >> 1] = fmaxf(most[j >> 1], fabsf(pm[m][j]));
-          }
-          *reinterpret_cast<float2*>(&s.solve.a[r0][col]) = make_float2(av[0], av[1]);
-          *reinterpret_cast<float2*>(&s.solve.a[r0 + 8][col]) = make_float2(av[2], av[3]);
+        for (int j = 0; j < 4; ++j) {
+          const int row = r0 + (j >> 1) * 8, at = col + (j & 1);
+          const float d = ex2((hi[j >> 1] - ((j & 1) ? chi.y : chi.x)) + (lo[j >> 1] - ((j & 1) ? clo.y : clo.x)));
+          v[m][j] = at < row || (at == row && !solver) ? dot[m][j] * (beta[j >> 1] * d) : 0.0f;
+          most[j >> 1] = fmaxf(most[j >> 1], fabsf(v[m][j]));
         }
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const float up = raise(quad_max(most[j]));
-        if (t == 0) factors[4 * kChunk + r0 + 8 * j] = inverse_of_power(up);
-#pragma unroll
-        for (int m = 0; m < 8; ++m)
-          if (m < 2 * (warp + 1)) {
-            const F2 x = f2_mul(f2_pack(pm[m][2 * j], pm[m][2 * j + 1]), f2_both(up));
-            const uint32_t h16 = high(x);
-            uint8_t* at = out + 2 * kLower + lower_block(warp, m >> 1) * kBlock + (j * 2 + (m & 1)) * 128 + lane * 4;
-            *reinterpret_cast<uint32_t*>(at) = h16;
-            if constexpr (Parts<T>::kOut == 2) *reinterpret_cast<uint32_t*>(at + kLower) = low(x, h16);
-          }
+        if (solver) {
+          *reinterpret_cast<float2*>(&s.solve.a[r0][col]) = make_float2(v[m][0], v[m][1]);
+          *reinterpret_cast<float2*>(&s.solve.a[r0 + 8][col]) = make_float2(v[m][2], v[m][3]);
+        }
       }
-    }
-    __syncthreads();
-    invert(s.solve.a, s.solve.t, s.solve.part);
-    {   // T = t diag(beta), this warp's 16 rows
-      float v[8][4], most[2] = {0.0f, 0.0f};
+    if (solver) {
+      barrier<kSolvers>(kSolveId);
+      invert(s.solve.a, s.solve.t, s.solve.part);
+      most[0] = most[1] = 0.0f;   // T = t diag(beta)
 #pragma unroll
       for (int m = 0; m < 8; ++m)
-        if (m < 2 * (warp + 1)) {
+        if (m < 2 * (block + 1)) {
           const int col = m * 8 + 2 * t;
-          const float2 beta = *reinterpret_cast<const float2*>(&gates.beta[col]);
+          const float2 b = *reinterpret_cast<const float2*>(&gates.beta[col]);
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
             const float2 x = *reinterpret_cast<const float2*>(&s.solve.t[r0 + 8 * j][col]);
-            v[m][2 * j] = x.x * beta.x;
-            v[m][2 * j + 1] = x.y * beta.y;
+            v[m][2 * j] = x.x * b.x;
+            v[m][2 * j + 1] = x.y * b.y;
             most[j] = fmaxf(most[j], fmaxf(fabsf(v[m][2 * j]), fabsf(v[m][2 * j + 1])));
           }
         }
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const float up = raise(quad_max(most[j]));
-        if (t == 0) factors[3 * kChunk + r0 + 8 * j] = inverse_of_power(up);
-#pragma unroll
-        for (int m = 0; m < 8; ++m)
-          if (m < 2 * (warp + 1)) {
-            const F2 x = f2_mul(f2_pack(v[m][2 * j], v[m][2 * j + 1]), f2_both(up));
-            const uint32_t h16 = high(x);
-            uint8_t* at = out + lower_block(warp, m >> 1) * kBlock + (j * 2 + (m & 1)) * 128 + lane * 4;
-            *reinterpret_cast<uint32_t*>(at) = h16;
-            *reinterpret_cast<uint32_t*>(at + kLower) = low(x, h16);
-          }
-      }
+    } else if (tid - kSolvers < kChunk) {
+      const int at = tid - kSolvers;
+      const float h = gates.hi[at], l = gates.lo[at], since = exp2_of(h, l);
+      factors[at] = -since * s.key_scale[at];
+      factors[kChunk + at] = since * s.query_scale[at];
+      factors[2 * kChunk + at] = exp2_of(gates.hi[kChunk - 1] - h, gates.lo[kChunk - 1] - l) * s.key_scale[at];
+      if (at == kChunk - 1) factors[5 * kChunk] = since;
     }
-    __syncthreads();
+    uint8_t* const parts = out + (solver ? 0 : 2 * kLower);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const float up = raise(quad_max(most[j]));
+      if (t == 0) factors[(solver ? 3 : 4) * kChunk + r0 + 8 * j] = inverse_of_power(up);
+#pragma unroll
+      for (int m = 0; m < 8; ++m)
+        if (m < 2 * (block + 1)) {
+          const F2 x = f2_mul(f2_pack(v[m][2 * j], v[m][2 * j + 1]), f2_both(up));
+          const uint32_t h16 = high(x);
+          uint8_t* at = parts + lower_block(block, m >> 1) * kBlock + (j * 2 + (m & 1)) * 128 + lane * 4;
+          *reinterpret_cast<uint32_t*>(at) = h16;
+          if (Parts<T>::kOut == 2 || solver) *reinterpret_cast<uint32_t*>(at + kLower) = low(x, h16);
+        }
+    }
+    if (solver) barrier<kSolvers>(kSolveId);   // (t is read before the next head's a is solved)
   }
   if (tid == 0) bulk_wait_group0();
 }
@@ -583,10 +561,6 @@ struct Exchange {
 template <typename T>
 __host__ __device__ constexpr int value_pitch(int slices) { return 16 * slices * int(sizeof(T)) + 16; }   // bytes; eight rows in different banks
 
-template <int THREADS>
-__device__ __forceinline__ void barrier(int id) { asm volatile("bar.sync %0, %1;" ::"r"(id), "n"(THREADS) : "memory"); }
-template <int THREADS>
-__device__ __forceinline__ void barrier_arrive(int id) { asm volatile("bar.arrive %0, %1;" ::"r"(id), "n"(THREADS) : "memory"); }
 __device__ __forceinline__ F2 pair_at(const float* p) { return *reinterpret_cast<const F2*>(p); }
 
 // Outputs of BLOCKS x 16 tokens: o[i][..] holds rows (value channels) lane / 4, + 8 and tokens 8 i + 2 (lane % 4), + 1; `y` is at the first
