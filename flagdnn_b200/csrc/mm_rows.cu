@@ -273,13 +273,32 @@ cudaError_t go(const MmRowsParams& p, cudaStream_t stream) {
     static_assert(ROWS * (kCols + 4) * 4 <= kSmem, "the sums fit");
     static std::atomic<uint64_t> done;
     auto* kernel = mm_rows_kernel<T, ROWS, WIDE, ORDER, A_WHOLE, kStages>;
-    const cudaError_t e = allow_smem(kernel, kSmem, done);
+    constexpr int kRoom = 227 * 1024, kAlone = 5;   // (five blocks leave no room to spread)
+    const cudaError_t e = allow_smem(kernel, kRoom, done);
     if (e != cudaSuccess) return e;
-    return launch_seq(kernel, dim3(unsigned(tiles * split), unsigned(row_blocks)), kThreads, kSmem, split, stream, p, split);
+    // No more blocks to an SM than an even spread has, where all of them still run at once: three blocks on some SMs and one on others take
+    // 44.8 us, two on each 35.3 (fp32, 64 x 2048 x 4096).  Clusters need their blocks in one group of SMs, so fewer fit than SMs would
+    // hold: sixteen clusters of eight with an SM to a block ran in two waves (bf16, 16 x 1024 x 1024: 7.1 us for 4.4).
+    // Not where two steps read the same 128 bytes of a row, which shorter rings leave in the L1 cache (2 x 7260 x 2432: 16.5 us, 21.2 with
+    // it); values one by one across columns lose there at times (fp32, 7 x 792 x 7905: 14.8 to 17.3) and gain more often (bf16,
+    // 33 x 7295 x 726: 37.3 to 33.0).
+    const long long blocks = tiles * split * row_blocks, each = (blocks + current_sm_count() - 1) / current_sm_count();
+    int smem = kSmem;
+    if (!(ORDER == Order::kAny && p.b_s[0] == 1) && each < kAlone && int(kRoom / each) - 2048 > kSmem) {
+      const int even = int(kRoom / each) - 2048, of = split == 1 ? 0 : split == 2 ? 1 : split == 4 ? 2 : 3;
+      static std::atomic<int> at_once[kAlone][4];   // one more than the clusters that run at once; 0: not asked yet
+      int n = at_once[each][of].load(std::memory_order_relaxed);
+      if (n == 0) {
+        n = 1 + clusters_at_once(kernel, kThreads, even, split);
+        at_once[each][of].store(n, std::memory_order_relaxed);
+      }
+      if (tiles * row_blocks < n) smem = even;
+    }
+    return launch_seq(kernel, dim3(unsigned(tiles * split), unsigned(row_blocks)), kThreads, smem, split, stream, p, split);
   };
   // One row, bf16, two blocks to an SM, 2048 x 4096 9.8 / 8.1 / 6.1 / 9.0 us in 1 / 2 / 4 / 8 parts (64 to 512 blocks), 4096 x 8192 20.8 / 16.0 /
   // 18.5 / 23.4 (128 to 1024).  Where two parts too many would not run at once (7264 x 2432: 152 blocks of 4 parts 15.5 us), blocks of half the
-  // ring do, four to an SM (304 of 8 parts 12.7; 4096 x 2048, 256 blocks either way, 6.3 and 7.9).
+  // ring do, four to an SM (304 of 8 parts 12.7, 11.5 evenly spread; 4096 x 2048, 256 blocks either way, 6.3 and 7.9).
   constexpr int kStages = stages_of<T>(ROWS, kCols);
   constexpr int kAtOnce = 227 * 1024 / (kStages * (kCols + ROWS) * kPitch + 1024);
   const int split = split_of(kAtOnce);

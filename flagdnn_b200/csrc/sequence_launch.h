@@ -48,4 +48,25 @@ cudaError_t allow_smem(K* kernel, int bytes, std::atomic<uint64_t>& done) {
   return e;
 }
 
+// Clusters of `cluster` blocks that run at once on an idle device; 0 if that cannot be had.
+template <typename K>
+int clusters_at_once(K* kernel, int threads, size_t smem, int cluster) {
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = unsigned(cluster);
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(unsigned(cluster));
+  cfg.blockDim = dim3(unsigned(threads));
+  cfg.dynamicSmemBytes = smem;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  int n = 0;
+  if (cudaOccupancyMaxActiveClusters(&n, reinterpret_cast<const void*>(kernel), &cfg) != cudaSuccess) {
+    cudaGetLastError();
+    return 0;
+  }
+  return n;
+}
+
 }  // namespace fdnn
