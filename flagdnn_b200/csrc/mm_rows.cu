@@ -348,7 +348,7 @@ cudaError_t by_layout(MmRowsParams p, cudaStream_t stream) {
 // Its time goes with N K and, slowly, with M; the convolution's, on tiles of 128 rows, with K alone as long as they run at once.  16-bit,
 // us here and there: K = 4096, N = 2048 64 rows 12.4 and 15.6, 96 rows 22.3 and 15.6; N = 1024 128 rows 12.1 and 15.5, 192 rows 19.4 and
 // 15.5; N = 512 256 rows 12.0 and 15.4, 512 rows 19.4 and 15.5; N = 8192 16 rows 18.9 and 17.6.  K = 8192, N = 1024 128 rows 18.7 and
-// 27.7, 192 rows 32.4 and 27.6.  K = 2048, N = 4096 16 rows 7.9 and 14.0, 32 rows 9.5 and 9.6; N = 256 256 rows 8.5 and 9.3.  K = 1024,
+// 27.7, 192 rows 32.4 and 27.6; N = 128 513 rows 17.5 and 27.4, 1024 rows 17.9 and 27.5, 1200 rows 30.1 and 27.6.  K = 2048, N = 4096 16 rows 7.9 and 14.0, 32 rows 9.5 and 9.6; N = 256 256 rows 8.5 and 9.3.  K = 1024,
 // N = 1024 32 rows 5.4 and 6.1, 48 rows 6.6 and 6.1; N = 512 64 rows 6.0 and 5.7.  K = 512, N = 4096 16 rows 5.3 and 5.5, 32 rows 6.5 and
 // 5.4.  Fewer than eight terms fill no 16 bytes: the convolution's paths for few channels add a residual in a step of its own.  Its
 // fp32 sums stay in one accumulator (see above).

@@ -108,7 +108,8 @@ def test_which_products_are_of_few_rows(native_lib):
 
     assert preferred(m=1, n=8192, k=64) and preferred(m=16, n=8192, k=64) and preferred(m=500, n=8192, k=7)
     assert preferred(m=64, n=2048, k=4096) and not preferred(m=65, n=2048, k=4096) and preferred(m=256, n=512, k=8192)
-    assert not preferred(m=64, n=4096, k=2048) and not preferred(m=48, n=1024, k=1024) and not preferred(m=513, n=16, k=8192)
+    assert not preferred(m=64, n=4096, k=2048) and not preferred(m=48, n=1024, k=1024)
+    assert preferred(m=1024, n=16, k=8192) and not preferred(m=1025, n=16, k=8192) and not preferred(m=513, n=16, k=2048)
     assert preferred(m=5000, n=8192, k=64, dtype=nat.F32)      # whose sums a convolution keeps in one accumulator
 
 
