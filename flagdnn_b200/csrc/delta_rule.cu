@@ -331,8 +331,12 @@ __device__ __forceinline__ void sum_gates(const DeltaParams& p, const RawGates& 
     to.lo[2 * lane + j] = float(each[j] - double(hi));
   }
 }
-// 2^(hi + lo) to fp32's last place but two: what a state keeps over many chunks has no drift.
-__device__ __forceinline__ float exp2_of(float hi, float lo) { return exp2f(hi) * fmaf(lo, 0.6931471805599453f, 1.0f); }
+// 2^d to fp32's last place but two: what a state keeps over many chunks has no drift.  (What fp32 leaves of a d whose power is not zero is
+// at most 2^-17.  The parts of a sum that has passed a token which forgets all are not: of 32 such tokens, 0.25.)
+__device__ __forceinline__ float exp2_of(double d) {
+  const float hi = float(d);
+  return exp2f(hi) * fmaf(float(d - double(hi)), 0.6931471805599453f, 1.0f);
+}
 
 // fp32 as a TF32 number, rounded to nearest, and what it leaves.
 __device__ __forceinline__ void two_parts(float v, uint32_t& hi, uint32_t& lo) {
@@ -517,10 +521,11 @@ delta_prepare_kernel(const DeltaParams p) {
         }
     } else if (tid - kSolvers < kChunk) {
       const int at = tid - kSolvers;
-      const float h = gates.hi[at], l = gates.lo[at], since = exp2_of(h, l);
+      const double sum = double(gates.hi[at]) + double(gates.lo[at]), all = double(gates.hi[kChunk - 1]) + double(gates.lo[kChunk - 1]);
+      const float since = exp2_of(sum);
       factors[at] = -since * s.key_scale[at];
       factors[kChunk + at] = since * s.query_scale[at];
-      factors[2 * kChunk + at] = exp2_of(gates.hi[kChunk - 1] - h, gates.lo[kChunk - 1] - l) * s.key_scale[at];
+      factors[2 * kChunk + at] = exp2_of(all - sum) * s.key_scale[at];
       if (at == kChunk - 1) factors[5 * kChunk] = since;
     }
     uint8_t* const parts = out + (solver ? 0 : 2 * kLower);
