@@ -78,10 +78,16 @@ __device__ __forceinline__ void barrier(int id) { asm volatile("bar.sync %0, %1;
 template <int THREADS>
 __device__ __forceinline__ void barrier_arrive(int id) { asm volatile("bar.arrive %0, %1;" ::"r"(id), "n"(THREADS) : "memory"); }
 
-// A power of two that takes `most` to 2^14 .. 2^15 (an exponent that it cannot have is cut; of infinity or NaN, some power).
+// A power of two that takes `most` to 2^14 .. 2^15 (an exponent that it cannot have is cut).  Beside an infinity nothing else would be left of a
+// row, as finite numbers that depend on a later token: its scale is NaN, and so is all that is made of the row.
 __device__ __forceinline__ float raise(float most) {
   const int e = 268 - int((__float_as_uint(most) >> 23) & 255u);
-  return __uint_as_float(uint32_t(min(max(e, 1), 253)) << 23);
+  return __uint_as_float(e == 13 ? 0x7fffffffu : uint32_t(min(max(e, 1), 253)) << 23);
+}
+__device__ __forceinline__ float lower_of(float x, float y) {   // of two scales
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(y));
+  return r;
 }
 __device__ __forceinline__ float inverse_of_power(float s) { return __uint_as_float((254u << 23) - __float_as_uint(s)); }
 
@@ -798,8 +804,8 @@ delta_chunks_kernel(const DeltaParams p, const Run run) {
 #pragma unroll
           for (int j = 0; j < 8 - kTiles; ++j) load(v[j], j);
           row_scales<8 - kTiles + 1>(v, v0, v1);
-          u0 = fminf(u0, v0);
-          u1 = fminf(u1, v1);
+          u0 = lower_of(u0, v0);
+          u1 = lower_of(u1, v1);
         }
         const F2 up0 = f2_both(u0), up1 = f2_both(u1);
         auto products = [&](const float (&x)[4], const float (&y)[4], int k, auto from) {   // tokens 16 k ..: what they wrote, to blocks from .. on

@@ -1,4 +1,4 @@
-"""gated_delta_rule where its inputs reach their ends: tokens that forget all.
+"""gated_delta_rule where its inputs reach their ends: tokens that forget all, infinities.
 
 Tolerances as in test_delta_rule_gpu.py."""
 import pytest
@@ -29,3 +29,47 @@ def test_several_tokens_of_a_chunk_forget_all(fd, dtype, resets, forget):  # noq
         y, state = fd.gated_delta_rule(**part, **options, initial_state=before, return_final_state=True)
         near(state, want.state, want.state_size, torch.float32)
         near(y, want.y, want.y_size, dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("name", ["v", "k", "q", "beta", "delta"])
+@pytest.mark.parametrize("length,at", [(130, 40), (64, 63), (130, 64), (2304, 1400)])
+def test_an_infinite_input_is_seen(fd, dtype, name, length, at):  # noqa: F811
+    """Tokens before it in its chunk are right or not finite, never finite and wrong; those before the chunk are right."""
+    g = torch.Generator().manual_seed(at)
+    v, options = inputs(g, 1, length, 1, 2, 64, 40, dtype, False, False)
+    v[name][0, at, 0, ...] = float("inf") if v[name].dim() == 3 else v[name][0, at, 0]
+    if v[name].dim() == 4:
+        v[name][0, at, 0, 7] = float("inf")
+    y, state = fd.gated_delta_rule(**v, **options, return_final_state=True)
+    y, state = y.double().cpu(), state.double().cpu()
+    want = do.gated_delta_rule(**{n: t[:, :at] for n, t in v.items()}, **options)
+    chunk = at // 64 * 64
+    heads = 1 if name in ("beta", "delta") or (name == "v") else 2          # the two heads share keys and queries
+    channels = slice(7, 8) if name == "v" else slice(0, 40)
+    assert y[0, :chunk].isfinite().all()
+    near(torch.where(y[0, :at].isfinite(), y[0, :at], want.y[0]), want.y[0], want.y_size[0], dtype)
+    assert not y[0, at, :heads, channels].isfinite().any()
+    others = torch.ones(2, 40, dtype=torch.bool)
+    others[:heads, channels] = False
+    assert y[0, :, others].isfinite().all()
+    if name != "q":
+        assert not y[0, at:, :heads, channels].isfinite().any() and not state[0, :heads, channels].isfinite().any()
+        assert state[0][others].isfinite().all()
+    else:
+        assert y[0, at + 1:].isfinite().all() and state.isfinite().all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("length", [9, 130, 2304])
+def test_an_infinite_state_is_seen(fd, dtype, length):  # noqa: F811
+    g = torch.Generator().manual_seed(length)
+    v, options = inputs(g, 1, length, 1, 2, 64, 40, dtype, False, False)
+    before = torch.randn(1, 2, 40, 64, generator=g).cuda()
+    want = do.gated_delta_rule(**v, **options, initial_state=before)
+    before[0, 1, 5, 3] = float("inf")
+    y, state = fd.gated_delta_rule(**v, **options, initial_state=before, return_final_state=True)
+    assert not y[0, :, 1, 5].isfinite().any() and not state[0, 1, 5].isfinite().any()
+    keep = [i for i in range(80) if i != 45]
+    near(y.flatten(2)[..., keep], want.y.flatten(2)[..., keep], want.y_size.flatten(2)[..., keep], dtype)
+    near(state.flatten(1, 2)[:, keep], want.state.flatten(1, 2)[:, keep], want.state_size.flatten(1, 2)[:, keep], torch.float32)
