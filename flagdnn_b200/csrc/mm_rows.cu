@@ -109,7 +109,9 @@ mm_rows_kernel(const MmRowsParams p, int split) {
   constexpr int kColPitch = ORDER == Order::kColumns ? kCols * int(sizeof(T)) + (sizeof(T) == 2 ? 16 : 32) : kPitch;
   static_assert(ORDER != Order::kColumns || kStep * kColPitch <= kColTile, "fits the tile's place");
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3, m = lane >> 3, r = lane & 7;
-  const int rank = int(blockIdx.x % split), col0 = int(blockIdx.x / split) * kCols, row0 = int(blockIdx.y) * ROWS;
+  const int rank = int(blockIdx.x % split), col0 = int(blockIdx.x / split) * kCols;
+  const int row0 = int(blockIdx.z * gridDim.y + blockIdx.y) * ROWS;   // (as many layers of blocks as 65535 to a layer ask for)
+  if (row0 >= p.M) return;
   const int steps = (p.K + kStep - 1) / kStep;
   const int from = int((long long)steps * rank / split), to = int((long long)steps * (rank + 1) / split);
   const uint32_t smem = smem_u32(smem_raw);
@@ -261,7 +263,8 @@ cudaError_t go(const MmRowsParams& p, cudaStream_t stream) {
   constexpr int kCols = 16 * WIDE * kWarps, kStep = kTileBytes / int(sizeof(T));
   const long long tiles = (p.N + kCols - 1) / kCols, row_blocks = (p.M + ROWS - 1) / ROWS;
   const int steps = (p.K + kStep - 1) / kStep;
-  if (tiles > 0x7fffffffll / 8 || row_blocks > 65535) return cudaErrorInvalidConfiguration;
+  const long long layers = (row_blocks + 65534) / 65535;
+  if (tiles > 0x7fffffffll / 8 || layers > 65535) return cudaErrorInvalidConfiguration;
   // parts of the reduction: as many blocks as run at once, as long as each has two steps
   auto split_of = [&](int at_once) {
     int split = 1;
@@ -294,7 +297,7 @@ cudaError_t go(const MmRowsParams& p, cudaStream_t stream) {
       }
       if (tiles * row_blocks < n) smem = even;
     }
-    return launch_seq(kernel, dim3(unsigned(tiles * split), unsigned(row_blocks)), kThreads, smem, split, stream, p, split);
+    return launch_seq(kernel, dim3(unsigned(tiles * split), unsigned((row_blocks + layers - 1) / layers), unsigned(layers)), kThreads, smem, split, stream, p, split);
   };
   // One row, bf16, two blocks to an SM, 2048 x 4096 9.8 / 8.1 / 6.1 / 9.0 us in 1 / 2 / 4 / 8 parts (64 to 512 blocks), 4096 x 8192 20.8 / 16.0 /
   // 18.5 / 23.4 (128 to 1024).  Where two parts too many would not run at once (7264 x 2432: 152 blocks of 4 parts 15.5 us), blocks of half the
