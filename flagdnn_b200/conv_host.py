@@ -717,8 +717,8 @@ def mm_bias_act(
     """``activation(input @ mat2 + bias + residual)``, summed in fp32 and rounded once: ``mm`` with the epilogue of
     ``conv2d_bias_act``.  ``input`` [M, K] and ``mat2`` [K, N] may have any strides (a linear layer's weight [N, K] goes in as
     ``weight.t()``), ``bias`` is [N], ``residual`` [M, N]; all fp16, bf16 or fp32.  Few rows are a reading of ``mat2`` by a kernel of
-    their own, as are fp32 products (an infinite operand makes NaN); others run as a 1x1 convolution.  It computes no gradients: tensors
-    that ask for one are refused."""
+    their own, as are fp32 products (an infinite operand, or products past fp32's range, give infinity or NaN); others run as a
+    1x1 convolution.  It computes no gradients: tensors that ask for one are refused."""
     if activation not in _ACTIVATIONS:
         raise RuntimeError(f"activation must be one of {', '.join(_ACTIVATIONS)}, got {activation!r}")
     act = _ACTIVATIONS[activation]

@@ -57,10 +57,14 @@ __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint3
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 // fp32 as a TF32 number, rounded to nearest (by the integer unit: the conversion's instruction takes as long as the products), and what it
-// leaves, of either sign, whose last bits the tensor core does not read.
+// leaves, of either sign, whose last bits the tensor core does not read.  The first part is finite: the largest numbers do not become infinite,
+// and an infinity or NaN is all in the second.
 __device__ __forceinline__ void two_parts(float v, uint32_t& hi, uint32_t& lo) {
-  hi = (__float_as_uint(v) + 0x1000u) & 0xffffe000u;
-  lo = __float_as_uint(v - __uint_as_float(hi));
+  constexpr float kLargest = 3.4011621342146535e38f;   // of TF32: 2^127 (2 - 2^-10)
+  float h;
+  asm("min.xorsign.abs.f32 %0, %1, %2;" : "=f"(h) : "f"(__uint_as_float((__float_as_uint(v) + 0x1000u) & 0xffffe000u)), "f"(kLargest));
+  hi = __float_as_uint(h);
+  lo = __float_as_uint(v - h);
 }
 __device__ __forceinline__ float cluster_f32(uint32_t at) {
   float v;

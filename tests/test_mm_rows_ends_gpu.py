@@ -1,10 +1,12 @@
-"""mm_bias_act at the ends of its range: the most rows.
+"""mm_bias_act at the ends of its range: the most rows, the largest numbers.
 
 Tolerances as in test_mm_bias_act_gpu.py."""
 import pytest
 import torch
 
+from oracle import delta_oracle as do
 from test_mm_bias_act_gpu import check, fd, matrix  # noqa: F401
+from test_sequence_gpu import DTYPES, IDS
 
 pytestmark = pytest.mark.gpu
 
@@ -17,3 +19,33 @@ def test_the_most_rows(fd, m, dtype, k, n):  # noqa: F811
     a, b = torch.randn(m, k, generator=g).to(dtype).cuda(), torch.randn(k, n, generator=g).to(dtype).cuda()
     bias = torch.randn(n, generator=g).to(dtype).cuda()
     check(fd, a, b, bias, None, "none")
+
+
+LARGEST = torch.finfo(torch.float32).max
+
+
+@pytest.mark.parametrize("m,k,n", [(1, 64, 64), (3, 1000, 72), (40, 130, 64), (130, 1100, 300)])
+@pytest.mark.parametrize("layout", ["dense", "t"])
+def test_the_largest_numbers(fd, m, k, n, layout):  # noqa: F811
+    """fp32 operands up to the largest finite one have finite products with small ones, of either sign and in either operand."""
+    g = torch.Generator().manual_seed(m)
+    for swap in (False, True):
+        big, small = (k, n) if swap else (m, k), (m, k) if swap else (k, n)
+        x = matrix(g, *big, torch.float32, layout)
+        x.copy_(torch.where(torch.rand(big, generator=g).cuda() < 0.5, LARGEST, -LARGEST) * (1 - 2.0 ** -24 * torch.randint(0, 5000, big, generator=g).cuda()))
+        w = matrix(g, *small, torch.float32, layout, 2.0 ** -30 / k)
+        check(fd, *((w, x) if swap else (x, w)), None, None, "none")
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("m,k,n", [(1, 64, 64), (3, 200, 72), (130, 1100, 300)])
+def test_infinite_operands(fd, m, k, n, dtype):  # noqa: F811
+    """An infinity times a number of ordinary size is one, of the product's sign; times zero, or with its opposite beside it, NaN."""
+    g = torch.Generator().manual_seed(m)
+    a, b = matrix(g, m, k, dtype, "dense"), matrix(g, k, n, dtype, "dense")
+    a[m // 2, 5] = float("inf")
+    b[9, 3] = -float("inf")
+    b[5, 7] = 0.0
+    a[m // 2, 11] = 2.0
+    got, want = fd.mm_bias_act(a, b).double().cpu(), do.mm_bias_act(a, b)
+    assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got[got.isinf()], want[want.isinf()]) and torch.equal(got.isinf(), want.isinf())
