@@ -293,13 +293,8 @@ cudaError_t go(const MmRowsParams& p, cudaStream_t stream) {
     int smem = kSmem;
     if (!(ORDER == Order::kAny && p.b_s[0] == 1) && each < kAlone && int(kRoom / each) - 2048 > kSmem) {
       const int even = int(kRoom / each) - 2048, of = split == 1 ? 0 : split == 2 ? 1 : split == 4 ? 2 : 3;
-      static std::atomic<int> at_once[kAlone][4];   // one more than the clusters that run at once; 0: not asked yet
-      int n = at_once[each][of].load(std::memory_order_relaxed);
-      if (n == 0) {
-        n = 1 + clusters_at_once(kernel, kThreads, even, split);
-        at_once[each][of].store(n, std::memory_order_relaxed);
-      }
-      if (tiles * row_blocks < n) smem = even;
+      static ClusterCounts known[kAlone][4];
+      if (tiles * row_blocks <= clusters_at_once(kernel, kThreads, even, split, known[each][of])) smem = even;
     }
     return launch_seq(kernel, dim3(unsigned(tiles * split), unsigned((row_blocks + layers - 1) / layers), unsigned(layers)), kThreads, smem, split, stream, p, split);
   };

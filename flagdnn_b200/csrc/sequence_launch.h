@@ -48,9 +48,20 @@ cudaError_t allow_smem(K* kernel, int bytes, std::atomic<uint64_t>& done) {
   return e;
 }
 
-// Clusters of `cluster` blocks that run at once on an idle device; 0 if that cannot be had.
+// Clusters of `cluster` blocks that run at once on an idle device; 0 if that cannot be had.  `known`: what each device has answered for this
+// kernel, shared memory and cluster, one more than it, so that it is asked once.
+struct ClusterCounts {
+  std::atomic<int> of_device[64];
+};
 template <typename K>
-int clusters_at_once(K* kernel, int threads, size_t smem, int cluster) {
+int clusters_at_once(K* kernel, int threads, size_t smem, int cluster, ClusterCounts& known) {
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) {
+    cudaGetLastError();
+    return 0;
+  }
+  std::atomic<int>* place = dev >= 0 && dev < 64 ? &known.of_device[dev] : nullptr;
+  if (place != nullptr && (n = place->load(std::memory_order_relaxed)) > 0) return n - 1;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = unsigned(cluster);
@@ -61,11 +72,11 @@ int clusters_at_once(K* kernel, int threads, size_t smem, int cluster) {
   cfg.dynamicSmemBytes = smem;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  int n = 0;
   if (cudaOccupancyMaxActiveClusters(&n, reinterpret_cast<const void*>(kernel), &cfg) != cudaSuccess) {
     cudaGetLastError();
     return 0;
   }
+  if (place != nullptr) place->store(n + 1, std::memory_order_relaxed);
   return n;
 }
 
