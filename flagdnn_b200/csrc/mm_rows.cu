@@ -349,13 +349,26 @@ cudaError_t by_layout(MmRowsParams p, cudaStream_t stream) {
 
 // Its time goes with N K and, slowly, with M; the convolution's, on tiles of 128 rows, with K alone as long as they run at once.  16-bit,
 // us here and there: K = 4096, N = 2048 64 rows 12.4 and 15.6, 96 rows 22.3 and 15.6; N = 1024 128 rows 12.1 and 15.5, 192 rows 19.4 and
-// 15.5; N = 512 256 rows 12.0 and 15.4, 512 rows 19.4 and 15.5; N = 8192 16 rows 18.9 and 17.6.  K = 8192, N = 1024 128 rows 18.7 and
-// 27.7, 192 rows 32.4 and 27.6; N = 128 513 rows 17.5 and 27.4, 1024 rows 17.9 and 27.5, 1200 rows 30.1 and 27.6.  K = 2048, N = 4096 16 rows 7.9 and 14.0, 32 rows 9.5 and 9.6; N = 256 256 rows 8.5 and 9.3.  K = 1024,
-// N = 1024 32 rows 5.4 and 6.1, 48 rows 6.6 and 6.1; N = 512 64 rows 6.0 and 5.7.  K = 512, N = 4096 16 rows 5.3 and 5.5, 32 rows 6.5 and
-// 5.4.  Fewer than eight terms fill no 16 bytes: the convolution's paths for few channels add a residual in a step of its own.  Its
-// fp32 sums stay in one accumulator (see above).
+// 15.5; N = 512 256 rows 12.0 and 15.4, 512 rows 19.4 and 15.5.  K = 8192, N = 1024 128 rows 18.7 and 27.7, 192 rows 32.4 and 27.6; N = 128
+// 513 rows 17.5 and 27.4, 1024 rows 17.9 and 27.5, 1200 rows 30.1 and 27.6.  K = 2048, N = 4096 16 rows 7.9 and 14.0, 32 rows 9.5 and 9.6;
+// N = 256 256 rows 8.5 and 9.3.  K = 1024, N = 1024 32 rows 5.4 and 6.1, 48 rows 6.6 and 6.1; N = 512 64 rows 6.0 and 5.7.  K = 512, N = 4096
+// 16 rows 5.3 and 5.5, 32 rows 6.5 and 5.4.  Fewer than eight terms fill no 16 bytes: the convolution's paths for few channels add a residual
+// in a step of its own.  Its fp32 sums stay in one accumulator (see above).
+//
+// Up to 16 rows, 16-bit, us here and there.  K = 4096: 8 rows N = 8192 18.2 and 30.2, 16 rows N = 6144 14.9 and 17.1, 8192 20.4 and 18.6 (b's
+// columns together 20.6 and 17.9; with GELU 20.4 and 20.9, 20.9 and 20.2), 12288 28.6 and 31.3, 14336 31.9 and 32.4 (36.0 and 31.2): from 16 rows
+// on the convolution takes a round of 74 tiles of 128 columns, full or not, in about 17 us.  K = 512, N = 18944 8 rows 8.5 and 8.8, N = 24576
+// 4 rows 11.0 and 10.8, 8 rows 12.2 and 10.7, 16 rows 14.7 and 10.6 (K = 1024: 8 rows 18.6 and 21.2, 16 rows 20.9 and 20.2): more blocks than run
+// at once, of few steps each.  (Left as it is: K = 256, N = 8192 16 rows 6.0 and 5.0.)
 bool mm_rows_preferred(int dtype, const MmRowsParams& p) {
-  return p.K < 8 || p.M <= 16 || dtype == FDNN_F32 || (p.M <= (p.K < 4096 ? 512 : 1024) && (long long)p.M * p.N <= (p.K < 4096 ? 32ll * p.K : 131072));
+  if (p.K < 8 || dtype == FDNN_F32) return true;
+  if (p.M > 16) return p.M <= (p.K < 4096 ? 512 : 1024) && (long long)p.M * p.N <= (p.K < 4096 ? 32ll * p.K : 131072);
+  // (operands that are not copied 16 bytes at a time are laid out anew for the convolution)
+  auto whole = [](long long along, long long across, int extent) { return along == 1 && across % 8 == 0 && extent % 8 == 0; };
+  if (!whole(p.a_s[1], p.a_s[0], p.K) || !(whole(p.b_s[0], p.b_s[1], p.K) || whole(p.b_s[1], p.b_s[0], p.N))) return true;
+  const long long sms = current_sm_count(), tiles = (p.N + 127ll) / 128, at_once = sms / 2, rounds = (tiles + at_once - 1) / at_once;
+  if (p.M == 16 && p.K >= 4096 && p.act <= FDNN_ACT_RELU) return 4 * tiles < 3 * rounds * at_once;
+  return !(p.M > 4 && p.K < 1024 && p.N > 128 * sms);
 }
 
 cudaError_t launch_mm_rows(int dtype, const MmRowsParams& p, cudaStream_t stream) {

@@ -49,3 +49,15 @@ def test_infinite_operands(fd, m, k, n, dtype):  # noqa: F811
     a[m // 2, 11] = 2.0
     got, want = fd.mm_bias_act(a, b).double().cpu(), do.mm_bias_act(a, b)
     assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got[got.isinf()], want[want.isinf()]) and torch.equal(got.isinf(), want.isinf())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "f16"])
+@pytest.mark.parametrize("m,k,n", [(16, 4096, 8192), (15, 4096, 8192), (16, 4104, 7176), (8, 512, 18952), (4, 512, 18952)])
+@pytest.mark.parametrize("layout", ["dense", "t", "ragged"])
+def test_few_rows_of_wide_layers(fd, m, k, n, dtype, layout):  # noqa: F811
+    """On either side of where the convolution is ahead."""
+    g = torch.Generator().manual_seed(k + m)
+    a, b = matrix(g, m, k, dtype, "dense"), matrix(g, k, n, dtype, layout, k ** -0.5)
+    bias = torch.randn(n, generator=g).to(dtype).cuda()
+    check(fd, a, b, bias, matrix(g, m, n, dtype, "dense"), "none")
+    check(fd, a, b, bias, None, "gelu")
