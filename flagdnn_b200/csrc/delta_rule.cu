@@ -1135,9 +1135,11 @@ delta_join_kernel(const DeltaParams p, const float* ends, float* starts, int seg
 
 // ---- launching -----------------------------------------------------------------------------------------------------
 
-// Prompts that the chunks' kernels take.  Token by token a prompt of 8 / 12 / 16 tokens takes 9.2 / 12.9 / 16.3 us (4 heads of 64 x 64), 10.5 /
-// 14.4 / 17.8 (32 of 128 x 128), 54 / 77 / 100 (16 rows of those); a chunk takes 14, 17 and 68.
-bool in_chunks(const DeltaParams& p) { return p.K <= kChunkKeys && p.L > 10; }
+// Prompts that the chunks' kernels take.  Token by token prompts of 10 / 12 / 16 tokens take, in us, and a chunk:
+//   16-bit   4 heads of 64 x 64 10.9 / 12.6 / 16.2, 12.6; 8 of them 11.0 / 12.9 / 16.6, 10.5; 100 rows of 4 17.9 / 20.9 / 26.9, 31.8
+//            one of 128 x 128 9.2 / 10.6 / 13.5, 12.0; 32 of them 13.1 / 14.9 / 19.4, 15.5; 4 rows of 32 23.6 / 28.5 / 38.3, 28.3; 16 rows 66 / 78 / 101, 68
+//   fp32     4 heads of 64 x 64 10.5 / 12.2 / 15.6, 11.5; 32 of 128 x 128 13.8 / 16.0 / 20.7, 22.2; 8 rows of 8 of them 15.4 / 18.1 / 23.1, 30.1
+bool in_chunks(int dtype, const DeltaParams& p) { return p.K <= kChunkKeys && p.L > (dtype == FDNN_F32 && p.K > 64 ? 16 : 11); }
 
 template <typename T>
 bool eights(const void* q, const long long* s) {
@@ -1261,7 +1263,7 @@ auto by_type(int dtype, const DeltaParams& p, F&& f) {
 }  // namespace
 
 long long delta_rule_workspace(int dtype, const DeltaParams& p) {
-  if (!in_chunks(p)) return 0;
+  if (!in_chunks(dtype, p)) return 0;
   return by_type(dtype, p, [&](auto type, auto keys) -> long long {
     using T = typename decltype(type)::type;
     constexpr int kKeys = decltype(keys)::value;
@@ -1271,7 +1273,7 @@ long long delta_rule_workspace(int dtype, const DeltaParams& p) {
 }
 
 cudaError_t launch_delta_rule(int dtype, const DeltaParams& p, cudaStream_t stream) {
-  if (!in_chunks(p)) return launch_delta_rule_tokens(dtype, p, stream);
+  if (!in_chunks(dtype, p)) return launch_delta_rule_tokens(dtype, p, stream);
   return by_type(dtype, p, [&](auto type, auto keys) -> cudaError_t { return run<typename decltype(type)::type, decltype(keys)::value>(p, stream); });
 }
 

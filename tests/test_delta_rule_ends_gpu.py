@@ -1,4 +1,4 @@
-"""gated_delta_rule where its inputs reach their ends: tokens that forget all, infinities.
+"""gated_delta_rule where its inputs reach their ends: tokens that forget all, infinities, lengths.
 
 Tolerances as in test_delta_rule_gpu.py."""
 import pytest
@@ -73,3 +73,18 @@ def test_an_infinite_state_is_seen(fd, dtype, length):  # noqa: F811
     keep = [i for i in range(80) if i != 45]
     near(y.flatten(2)[..., keep], want.y.flatten(2)[..., keep], want.y_size.flatten(2)[..., keep], dtype)
     near(state.flatten(1, 2)[:, keep], want.state.flatten(1, 2)[:, keep], want.state_size.flatten(1, 2)[:, keep], torch.float32)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("length", [10, 11, 12, 13, 16, 17])
+@pytest.mark.parametrize("dk", [64, 128])
+def test_lengths_between_the_two_ways(fd, dtype, length, dk):  # noqa: F811
+    g = torch.Generator().manual_seed(length)
+    v, options = inputs(g, 3, length, 1, 2, dk, 40, dtype, True, True)
+    before = torch.randn(3, 2, 40, dk, generator=g).cuda()
+    lengths = [length, 0, length - 3]
+    want = do.gated_delta_rule(**v, **options, initial_state=before, lengths=lengths)
+    y, state = fd.gated_delta_rule(**v, **options, initial_state=before, lengths=torch.tensor(lengths, dtype=torch.int32).cuda(),
+                                   return_final_state=True)
+    near(y, want.y, want.y_size, dtype)
+    near(state, want.state, want.state_size, torch.float32)
