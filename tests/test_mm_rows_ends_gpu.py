@@ -1,11 +1,11 @@
-"""mm_bias_act at the ends of its range: the most rows, the largest numbers.
+"""mm_bias_act at the ends of its range: the most rows, the largest numbers, wide blocks.
 
 Tolerances as in test_mm_bias_act_gpu.py."""
 import pytest
 import torch
 
 from oracle import delta_oracle as do
-from test_mm_bias_act_gpu import check, fd, matrix  # noqa: F401
+from test_mm_bias_act_gpu import ACTS, check, fd, matrix  # noqa: F401
 from test_sequence_gpu import DTYPES, IDS
 
 pytestmark = pytest.mark.gpu
@@ -61,3 +61,20 @@ def test_few_rows_of_wide_layers(fd, m, k, n, dtype, layout):  # noqa: F811
     bias = torch.randn(n, generator=g).to(dtype).cuda()
     check(fd, a, b, bias, matrix(g, m, n, dtype, "dense"), "none")
     check(fd, a, b, bias, None, "gelu")
+
+
+WIDE = [   # m, k, n, layout of a, of b: fp32 blocks of 64 x 128, several of them across, the last a part
+    (70, 1100, 300, "dense", "dense"), (130, 1101, 333, "dense", "dense"), (70, 1100, 300, "slice", "t"), (130, 1101, 333, "odd", "ragged"),
+    (96, 1100, 260, "t", "t"), (200, 1028, 516, "ragged", "slice"), (65, 4096, 130, "dense", "t"), (128, 1030, 257, "ragged", "t"),
+    (1300, 64, 2000, "dense", "dense"), (5000, 33, 520, "dense", "t"),     # by the count of blocks
+]
+
+
+@pytest.mark.parametrize("case", WIDE, ids=[f"{m}x{k}x{n}{a}-{b}" for m, k, n, a, b in WIDE])
+def test_wide_blocks(fd, case):  # noqa: F811
+    m, k, n, la, lb = case
+    g = torch.Generator().manual_seed(m + k)
+    a, b = matrix(g, m, k, torch.float32, la), matrix(g, k, n, torch.float32, lb, k ** -0.5)
+    bias = torch.randn(n, generator=g).cuda()
+    for i, act in enumerate(ACTS):
+        check(fd, a, b, bias if i % 2 else None, matrix(g, m, n, torch.float32, ("dense", "ragged", "t", "odd")[i]) if i < 3 else None, act)
