@@ -15,7 +15,9 @@
 // scaled by a power of two to a largest value of 2^14 .. 2^15 (a bf16 value below 2^-29 of that loses bits that fp32 sums do not see).
 // Everything made in fp32 (S, T, v - S k, U) goes in as two f16 parts, high and low, 22 bits below the row's largest value, which is
 // scaled to 2^14 .. 2^15 as well; so do fp32 inputs.  Products of low parts are left out (2^-22).  For bf16 outputs (2^-8) S q and P U
-// take the high parts alone, 11 bits each.  Sums are fp32; decays are differences of sums kept in 48 bits.
+// take the high parts alone, 11 bits each.  Sums are fp32; decays are differences of sums kept in 48 bits.  A row's values have one scale
+// and f16's steps end at 2^-24, so what a token writes is held to 2^-39 of the most that one of its chunk does; decays above one let it grow: up to
+// 2^18 within a chunk it keeps its 22 bits, and a chunk with a larger product of decays is NaN.
 #include <cuda_fp16.h>
 
 #include "delta_rule.cuh"
@@ -26,6 +28,7 @@ namespace {
 constexpr int kChunk = 64;
 constexpr int kChunkKeys = 128;      // the widest key that the chunks' kernels take
 constexpr int kMostSegments = 32;    // that a row is cut into
+constexpr float kMostGrowth = 18.0f; // log2 of a product of decays within a chunk
 constexpr int kFactors = 6 * kChunk; // floats a chunk and head: -a, b, d, t, p, and e^(G_64)
 constexpr int kLower = 10 * 512;     // bytes of a part of T or P
 
@@ -195,8 +198,9 @@ __device__ __forceinline__ int row_end(const DeltaParams& p, long long n) {
 constexpr int kPrepThreads = 256, kSolvers = 128, kSolveId = 1;
 constexpr int kPitch = kChunk + 4;   // floats between rows of A, T
 
-struct HeadGates {
+struct alignas(16) HeadGates {   // (pairs of each are read at once)
   float hi[kChunk], lo[kChunk], beta[kChunk];   // sums of log2 decays in two parts
+  float whole;                                  // 1, or NaN where a product of decays is past kMostGrowth
 };
 template <typename T, int KEYS>
 struct PrepShared {
@@ -330,6 +334,14 @@ __device__ __forceinline__ void sum_gates(const DeltaParams& p, const RawGates& 
     if (lane >= o) sum += other;
   }
   const double each[2] = {sum - v[1], sum};
+  // how far a later sum is above an earlier one
+  const float first = float(each[0]), second = float(each[1]);
+  float most = fmaxf(first, second);
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) most = fmaxf(most, __shfl_down_sync(0xffffffffu, most, o));   // (the last lanes' own again)
+  const float later = fmaxf(second, __shfl_down_sync(0xffffffffu, most, 1)), behind = lane < 31 ? later : second;
+  const bool grown = __any_sync(0xffffffffu, fmaxf(behind - first, behind - second) > kMostGrowth);
+  if (lane == 0) to.whole = grown ? __uint_as_float(0x7fffffffu) : 1.0f;
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
     const float hi = float(each[j]);
@@ -528,7 +540,7 @@ delta_prepare_kernel(const DeltaParams p) {
     } else if (tid - kSolvers < kChunk) {
       const int at = tid - kSolvers;
       const double sum = double(gates.hi[at]) + double(gates.lo[at]), all = double(gates.hi[kChunk - 1]) + double(gates.lo[kChunk - 1]);
-      const float since = exp2_of(sum);
+      const float since = exp2_of(sum) * gates.whole;
       factors[at] = -since * s.key_scale[at];
       factors[kChunk + at] = since * s.query_scale[at];
       factors[2 * kChunk + at] = exp2_of(all - sum) * s.key_scale[at];

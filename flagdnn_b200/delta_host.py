@@ -65,9 +65,11 @@ def gated_delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, delta: t
     ``q`` and ``k`` [N, L, G, K]: each key head serves ``H / G`` neighbouring heads; with ``qk_norm`` they are divided by
     ``sqrt(sum of squares + 1e-6)``.  ``delta`` and ``beta`` [N, L, H] are of ``v``'s type or float32, ``A`` and ``delta_bias`` [H]
     float32; ``scale`` is ``K ** -0.5`` if None.  ``initial_state`` and the returned state are float32 [N, H, V, K].
-    Prompts are taken in chunks of 64 tokens: an input that is not finite can make its whole chunk not finite, and decays above one are
-    taken as long as a chunk's product of them is an fp32 number. Long rows are cut into segments where few rows and heads run: a
-    row's last bits can depend on its batch."""
+    Prompts are taken in chunks of 64 tokens: an input that is not finite can make its whole chunk not finite, and what a token
+    brings to a value channel is held to 2^-22 of itself or 2^-39 of the most that one of its chunk does. Long rows are cut into
+    segments where few rows and heads run: a row's last bits can depend on its batch. Decays above one are taken as long as their
+    product is at most 2^18 over any stretch of a chunk (past that the chunk and what follows are NaN) and an fp32 number over any
+    stretch of the row, also where the state stays small or zero."""
     what = "gated_delta_rule"
     fast = _conv._fast or _conv.native_host()
     if fast:

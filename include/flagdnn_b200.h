@@ -359,8 +359,11 @@ int fdnn_selective_scan_step(const fdnn_scan_desc* desc, const void* u, const vo
  * sqrt(sum of their squares + 1e-6) first.  A and delta_bias [heads] and the states [N, heads, dv, dk] are dense float32;
  * delta_bias, A, initial_state (zeros), lengths (see above) and final_state may be NULL.  final_state must not overlap
  * initial_state.  Longer prompts are taken in chunks of 64 tokens: a q, k, v, delta or beta that is not finite can make the whole chunk
- * that it lies in not finite, its earlier tokens too; decays above one are taken as long as a chunk's product of them is an fp32 number.
- * Long rows are cut into segments where few rows and heads run: a row's last bits can depend on its batch. */
+ * that it lies in not finite, its earlier tokens too, and what a token brings to a value channel is held to 2^-22 of itself or 2^-39 of the
+ * most that one of its chunk does.  Long rows are cut into segments where few rows and heads run: a row's last bits can
+ * depend on its batch.  Decays above one are taken as long as their product is at most 2^18 over any stretch of a chunk (past that the
+ * chunk and what follows are NaN) and an fp32 number over any stretch of the row, also where the state stays small or zero: what a segment
+ * makes of a unit matrix has to be finite. */
 #define FDNN_DELTA_RULE_MAX_DK 256
 #define FDNN_DELTA_RULE_MAX_DV 1024
 #define FDNN_DELTA_RULE_MAX_HEADS 65535

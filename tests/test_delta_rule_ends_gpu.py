@@ -1,15 +1,16 @@
-"""gated_delta_rule where its inputs reach their ends: tokens that forget all, infinities, lengths; and rows that
+"""gated_delta_rule where its inputs reach their ends: tokens that forget all, infinities, lengths, decays above one; and rows that
 are cut into segments, as their workspace tells.
 
 Tolerances as in test_delta_rule_gpu.py."""
 import ctypes
+import math
 
 import pytest
 import torch
 
 from flagdnn_b200 import _native as nat
 from oracle import delta_oracle as do
-from test_delta_rule_gpu import fd, inputs, near  # noqa: F401
+from test_delta_rule_gpu import STATE_TOL, fd, inputs, near  # noqa: F401
 from test_sequence_gpu import DTYPES, IDS
 
 pytestmark = pytest.mark.gpu
@@ -155,3 +156,90 @@ def test_a_row_in_segments_and_among_others(fd, native_lib):  # noqa: F811
         for a, b in ((y1, state1), (y[i:i + 1], state[i:i + 1])):
             near(a, want.y, want.y_size, torch.bfloat16)
             near(b, want.state, want.state_size, torch.float32)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("length,grow", [(64, 0.19), (64, 1.3), (130, 0.19), (130, 0.6), (2304, 0.036)])
+def test_decays_above_one(fd, native_lib, dtype, length, grow):  # noqa: F811
+    """Products of decays up to 2^17.3 over chunks, and to e^83 over segments, next to the largest fp32 number; key channels that no key touches and
+    states of zeros in them. What grows is the state; values are small. Past 2^18 within a chunk it is NaN, by the step it is not."""
+    g = torch.Generator().manual_seed(length)
+    v, options = inputs(g, 1, length, 1, 2, 64, 40, dtype, False, True)
+    v["delta"].fill_(grow)
+    for name in ("k", "q"):
+        v[name][..., 40:] = 0.0
+    assert (segments(native_lib, v) > 1) == (length == 2304)
+    before = torch.randn(1, 2, 40, 64, generator=g).cuda() * 1e-6
+    before[:, :, ::2, 40:] = 0.0
+    v["v"] *= 1e-4
+    y, state = fd.gated_delta_rule(**v, **options, initial_state=before, return_final_state=True)
+    if grow > 0.2:
+        assert y.isnan().all() and state.isnan().all()
+        length = 10                                          # token by token
+        v = {name: t[:, :length] for name, t in v.items()}
+        y, state = fd.gated_delta_rule(**v, **options, initial_state=before, return_final_state=True)
+    want = do.gated_delta_rule(**v, **options, initial_state=before)
+    near(state, want.state, want.state_size, torch.float32)
+    if dtype != torch.float16:
+        near(y, want.y, want.y_size, dtype)
+
+
+def least_steps(v, options, before):
+    """What y can be off by because a channel's values of a chunk share a scale. Their largest is taken to 2^14 .. 2^15, and the second f16 part of
+    one of them is off by half of f16's least step, 2^-25: by 2^-39 of the largest. That goes for v - e^G S k and for what is written, U. An
+    error of the first is one of v; an error e of U does no more to y than a v of e / beta adds to the sums of sizes."""
+    x = {name: t.double().cpu() for name, t in v.items()}
+    norm = lambda t: t / (t.square().sum(-1, keepdim=True) + 1e-6).sqrt() if options["qk_norm"] else t  # noqa: E731
+    heads, length = x["v"].shape[2], x["v"].shape[1]
+    keys = norm(x["k"])[0].repeat_interleave(heads // x["k"].shape[2], 1)
+    most, state = torch.zeros_like(x["v"]), before.double().cpu()
+    for c in range(0, length, 64):
+        part = slice(c, min(length, c + 64))
+        for h in range(heads):
+            k, b, total = keys[part, h], x["beta"][0, part, h], x["delta"][0, part, h].clamp_min(-1e5).cumsum(0)
+            rest = x["v"][0, part, h] - total.exp()[:, None] * (k @ state[0, h].T)
+            a = b[:, None] * torch.exp((total[:, None] - total).clamp_max(700)).tril(-1) * (k @ k.T)
+            written = torch.linalg.solve_triangular(torch.eye(len(k), dtype=k.dtype) + a.tril(-1), b[:, None] * rest, upper=False)
+            most[0, part, h] = rest.abs().amax(0) + written.abs().amax(0) / b[:, None]
+        state = do.gated_delta_rule(**{n: t[:, part] for n, t in x.items()}, **options, initial_state=state).state
+    return 2.0 ** -39 * do.gated_delta_rule(**dict(x, v=most), **options).y_size
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("length", [200, 2304])
+def test_decays_on_both_sides_of_one(fd, dtype, length):  # noqa: F811
+    """Heads whose decays wander, grow within a chunk (too far in some) and shrink again, and forget all in between."""
+    g = torch.Generator().manual_seed(length + 1)
+    v, options = inputs(g, 1, length, 1, 6, 64, 24, dtype, False, True)
+    t = torch.arange(length)
+    v["delta"][0, :, 0] = torch.randn(length, generator=g).cuda() * 0.3
+    v["delta"][0, :, 1] = torch.where(t % 40 < 20, 1.0, -1.0).cuda()
+    v["delta"][0, :, 2] = torch.where(t % 64 == 31, -float("inf"), 0.3).cuda()
+    v["delta"][0, :, 3] = torch.where(t % 64 < 63, 0.3, -19.0).cuda()
+    v["delta"][0, :, 4] = torch.where(t % 40 < 20, 0.6, -0.6).cuda()
+    v["delta"][0, :, 5] = torch.where(t % 64 == 31, -float("inf"), 0.18).cuda()
+    before = torch.randn(1, 6, 24, 64, generator=g).cuda()
+    total = (v["delta"][0].double().clamp_min(-1e5) / math.log(2)).cumsum(0).cpu()
+    growth = [max(float((c[None] - c[:, None]).triu().max()) for c in total[:, h].split(64)) for h in range(6)]
+    assert [x > 18 for x in growth] == [False, True, False, True, False, False]
+    want = do.gated_delta_rule(**v, **options, initial_state=before)
+    y, state = fd.gated_delta_rule(**v, **options, initial_state=before, return_final_state=True)
+    y_size = want.y_size + least_steps(v, options, before) / STATE_TOL
+    for h in range(6):
+        if growth[h] > 18:
+            assert y[0, :, h].isnan().all() and state[0, h].isnan().all()
+            continue
+        near(state[0, h], want.state[0, h], want.state_size[0, h], torch.float32)
+        fits = want.y[0, :, h].abs() < 6e4                   # (past 65504 f16 has infinity)
+        near(y[0, :, h].cpu()[fits], want.y[0, :, h][fits], y_size[0, :, h][fits], dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "f32"])
+def test_values_far_below_their_chunks_largest(fd, dtype):  # noqa: F811
+    """A token whose values are 2^24 times its neighbours'."""
+    g = torch.Generator().manual_seed(21)
+    v, options = inputs(g, 1, 64, 1, 2, 64, 40, dtype, False, True)
+    v["v"][:, 50] *= 2.0 ** 24
+    want = do.gated_delta_rule(**v, **options)
+    y = fd.gated_delta_rule(**v, **options)
+    near(y, want.y, want.y_size + least_steps(v, options, torch.zeros(1, 2, 40, 64)) / STATE_TOL, dtype)
