@@ -21,6 +21,7 @@
 #include <cuda_fp16.h>
 
 #include "delta_rule.cuh"
+#include "mma_sync.cuh"
 
 namespace fdnn {
 namespace {
@@ -41,41 +42,16 @@ struct Parts {
 
 // ---- small things --------------------------------------------------------------------------------------------------
 
-// D += A B, 16 x 8 x 16.  A: rows lane / 4 (+ 8 in a[1], a[3]), pairs of k at 2 (lane % 4) (+ 8 in a[2], a[3]); B: column lane / 4, pairs
-// of k likewise; D: rows lane / 4 (+ 8 in d[2], d[3]), columns 2 (lane % 4) and the next.
-__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-// D = A B.
+// D = A B of f16 operands.
 __device__ __forceinline__ void mma_first(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
                : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
 }
-// The same of 16 x 8 x 8 in TF32: A at (row, k = lane % 4), (row + 8, k), (row, k + 4), (row + 8, k + 4), B at k = lane % 4, + 4.
-__device__ __forceinline__ void mma_tf32(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ void ldmatrix(uint32_t (&r)[4], uint32_t at) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
-}
-__device__ __forceinline__ void ldmatrix_t(uint32_t (&r)[4], uint32_t at) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
-}
 // Four 8 x 8 matrices of 16-bit values, held as accumulators are, transposed to shared memory: 16-byte rows at each lane's address.
 __device__ __forceinline__ void stmatrix_t(uint32_t at, uint32_t r0, uint32_t r1, uint32_t r2, uint32_t r3) {
   asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(r0), "r"(r1), "r"(r2), "r"(r3) : "memory");
 }
-__device__ __forceinline__ void copy16(uint32_t to, const void* from, int bytes) {   // the rest of the 16 is zeros
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
-}
-
 template <int THREADS>
 __device__ __forceinline__ void barrier(int id) { asm volatile("bar.sync %0, %1;" ::"r"(id), "n"(THREADS) : "memory"); }
 template <int THREADS>
@@ -279,19 +255,19 @@ __device__ __forceinline__ void dots(float (&c)[8][4], const uint8_t* x, const u
   for (int s = 0; s < KEYS / 16; ++s) {
     uint32_t a[Parts<T>::kKey][4];
 #pragma unroll
-    for (int k = 0; k < Parts<T>::kKey; ++k) ldmatrix(a[k], xs + k * kPart + s * kBlock);
+    for (int k = 0; k < Parts<T>::kKey; ++k) ldmatrix<false>(a[k], xs + k * kPart + s * kBlock);
 #pragma unroll
     for (int n = 0; n < 4; ++n)
       if (n <= i) {
         uint32_t b[Parts<T>::kKey][4];
 #pragma unroll
-        for (int k = 0; k < Parts<T>::kKey; ++k) ldmatrix(b[k], ys + k * kPart + (n * (KEYS / 16) + s) * kBlock);
+        for (int k = 0; k < Parts<T>::kKey; ++k) ldmatrix<false>(b[k], ys + k * kPart + (n * (KEYS / 16) + s) * kBlock);
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          mma(c[2 * n + j], a[0], b[0][2 * j], b[0][2 * j + 1]);
+          mma<__half>(c[2 * n + j], a[0], b[0][2 * j], b[0][2 * j + 1]);
           if constexpr (Parts<T>::kKey == 2) {
-            mma(c[2 * n + j], a[0], b[1][2 * j], b[1][2 * j + 1]);
-            mma(c[2 * n + j], a[1], b[0][2 * j], b[0][2 * j + 1]);
+            mma<__half>(c[2 * n + j], a[0], b[1][2 * j], b[1][2 * j + 1]);
+            mma<__half>(c[2 * n + j], a[1], b[0][2 * j], b[0][2 * j + 1]);
           }
         }
       }
@@ -356,11 +332,6 @@ __device__ __forceinline__ float exp2_of(double d) {
   return exp2f(hi) * fmaf(float(d - double(hi)), 0.6931471805599453f, 1.0f);
 }
 
-// fp32 as a TF32 number, rounded to nearest, and what it leaves.
-__device__ __forceinline__ void two_parts(float v, uint32_t& hi, uint32_t& lo) {
-  hi = (__float_as_uint(v) + 0x1000u) & 0xffffe000u;
-  lo = __float_as_uint(v - __uint_as_float(hi));
-}
 // d += x y of 16 x 16 blocks in fp32, by 3 x TF32 (2^-22).
 __device__ __forceinline__ void block_product(float (&d)[2][4], const float* x, int x_pitch, const float* y, int y_pitch) {
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -376,9 +347,9 @@ __device__ __forceinline__ void block_product(float (&d)[2][4], const float* x, 
       uint32_t b[2], bl[2];
 #pragma unroll
       for (int i = 0; i < 2; ++i) two_parts(y[(s * 8 + t + i * 4) * y_pitch + n * 8 + g], b[i], bl[i]);
-      mma_tf32(d[n], a, bl[0], bl[1]);
-      mma_tf32(d[n], al, b[0], b[1]);
-      mma_tf32(d[n], a, b[0], b[1]);
+      mma<float>(d[n], a, bl[0], bl[1]);
+      mma<float>(d[n], al, b[0], b[1]);
+      mma<float>(d[n], a, b[0], b[1]);
     }
   }
 }
@@ -628,7 +599,7 @@ __device__ __forceinline__ void mma_row(float (&d)[TILES][4], const uint32_t (&a
 #pragma unroll
   for (int j = FROM; j < TILES; ++j) {
     if (first) mma_first(d[j], a, b[j >> 1][2 * (j & 1)], b[j >> 1][2 * (j & 1) + 1]);
-    else mma(d[j], a, b[j >> 1][2 * (j & 1)], b[j >> 1][2 * (j & 1) + 1]);
+    else mma<__half>(d[j], a, b[j >> 1][2 * (j & 1)], b[j >> 1][2 * (j & 1) + 1]);
   }
 }
 
@@ -780,12 +751,12 @@ delta_chunks_kernel(const DeltaParams p, const Run run) {
             lo[0] = l.x, lo[1] = l.y, lo[2] = l.z, lo[3] = l.w;
           }
 #pragma unroll
-          for (int j = 0; j < kTiles / 2; ++j) ldmatrix(b[j], queries + (j * kSteps + half * (kSteps / 2) + k) * kBlock);
+          for (int j = 0; j < kTiles / 2; ++j) ldmatrix<false>(b[j], queries + (j * kSteps + half * (kSteps / 2) + k) * kBlock);
           mma_row<kTiles>(z, hi, b, k == 0);
           if constexpr (Parts<T>::kOut == 2) mma_row<kTiles>(z, lo, b);
           if constexpr (Parts<T>::kKey == 2) {
 #pragma unroll
-            for (int j = 0; j < kTiles / 2; ++j) ldmatrix(b[j], queries + kKeyPart + (j * kSteps + half * (kSteps / 2) + k) * kBlock);
+            for (int j = 0; j < kTiles / 2; ++j) ldmatrix<false>(b[j], queries + kKeyPart + (j * kSteps + half * (kSteps / 2) + k) * kBlock);
             mma_row<kTiles>(z, hi, b);
           }
         }
@@ -826,12 +797,12 @@ delta_chunks_kernel(const DeltaParams p, const Run run) {
           if constexpr (Parts<T>::kOut == 2) operand(x, y, up0, up1, hi, lo);
           else operand(x, y, up0, up1, hi);
 #pragma unroll
-          for (int j = j0; j < kTiles / 2; ++j) ldmatrix(b[j], weights + lower_block(tile0 / 2 + j, k) * kBlock);
+          for (int j = j0; j < kTiles / 2; ++j) ldmatrix<false>(b[j], weights + lower_block(tile0 / 2 + j, k) * kBlock);
           mma_row<kTiles, 2 * j0>(z, hi, b);
           if constexpr (Parts<T>::kOut == 2) {
             mma_row<kTiles, 2 * j0>(z, lo, b);
 #pragma unroll
-            for (int j = j0; j < kTiles / 2; ++j) ldmatrix(b[j], weights + kLower + lower_block(tile0 / 2 + j, k) * kBlock);
+            for (int j = j0; j < kTiles / 2; ++j) ldmatrix<false>(b[j], weights + kLower + lower_block(tile0 / 2 + j, k) * kBlock);
             mma_row<kTiles, 2 * j0>(z, hi, b);
           }
         };
@@ -896,7 +867,7 @@ delta_chunks_kernel(const DeltaParams p, const Run run) {
     const float* factors = reinterpret_cast<const float*>(base + 2 * W::kKeyBytes + (2 + Parts<T>::kOut) * kLower) + 2 * t;
     auto load_keys = [&](uint32_t (&b)[4][4], int k, int part) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) ldmatrix(b[j], keys + part * kKeyPart + lane * 16 + (j * kSteps + k) * kBlock);
+      for (int j = 0; j < 4; ++j) ldmatrix<false>(b[j], keys + part * kKeyPart + lane * 16 + (j * kSteps + k) * kBlock);
     };
     float x[8][4];
     uint32_t values[4][4];   // 16-bit: channels 0 .. 7 and 8 .. 15 of tokens 16 i .., then of 16 i + 8 ..
@@ -924,7 +895,7 @@ delta_chunks_kernel(const DeltaParams p, const Run run) {
       if constexpr (sizeof(T) == 2) {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          ldmatrix_t(values[i], smem_u32(base) + W::kStage + (i * 16 + (m >> 1) * 8 + r) * pitch + (slice * 16 + (m & 1) * 8) * 2);
+          ldmatrix<true>(values[i], smem_u32(base) + W::kStage + (i * 16 + (m >> 1) * 8 + r) * pitch + (slice * 16 + (m & 1) * 8) * 2);
       }
       const float i0 = inverse_of_power(s0), i1 = inverse_of_power(s1);
       reinterpret_cast<float2*>(exchange + E::kScales)[half * 32 + lane] = make_float2(i0, i1);
@@ -963,8 +934,8 @@ delta_chunks_kernel(const DeltaParams p, const Run run) {
       float z[2][2][4], z2[2][2][4], r0, r1;
       uint32_t b[2][4], bl[2][4];
       auto load = [&](int i, int k) {
-        ldmatrix(b[i], rows[i] + k * kBlock);
-        ldmatrix(bl[i], rows[i] + kLower + k * kBlock);
+        ldmatrix<false>(b[i], rows[i] + k * kBlock);
+        ldmatrix<false>(bl[i], rows[i] + kLower + k * kBlock);
       };
       load(0, 0);
       load(1, 0);
@@ -974,15 +945,15 @@ delta_chunks_kernel(const DeltaParams p, const Run run) {
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           if (k == 0) mma_first(z[i][j], hi, b[i][2 * j], b[i][2 * j + 1]);
-          else mma(z[i][j], hi, b[i][2 * j], b[i][2 * j + 1]);
+          else mma<__half>(z[i][j], hi, b[i][2 * j], b[i][2 * j + 1]);
         }
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           if (k == 0) mma_first(z2[i][j], lo, b[i][2 * j], b[i][2 * j + 1]);
-          else mma(z2[i][j], lo, b[i][2 * j], b[i][2 * j + 1]);
+          else mma<__half>(z2[i][j], lo, b[i][2 * j], b[i][2 * j + 1]);
         }
 #pragma unroll
-        for (int j = 0; j < 2; ++j) mma(z[i][j], hi, bl[i][2 * j], bl[i][2 * j + 1]);
+        for (int j = 0; j < 2; ++j) mma<__half>(z[i][j], hi, bl[i][2 * j], bl[i][2 * j + 1]);
       };
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
@@ -1011,7 +982,7 @@ delta_chunks_kernel(const DeltaParams p, const Run run) {
       const uint32_t columns = keys + ((m & 1) * 2 + (m >> 1)) * 128 + r * 16;
       auto load_columns = [&](uint32_t (&b)[kSteps / 2][4], int k, int part) {
 #pragma unroll
-        for (int j = 0; j < kSteps / 2; ++j) ldmatrix_t(b[j], columns + part * kKeyPart + (k * kSteps + j) * kBlock);
+        for (int j = 0; j < kSteps / 2; ++j) ldmatrix<true>(b[j], columns + part * kKeyPart + (k * kSteps + j) * kBlock);
       };
       uint32_t b[2][kSteps / 2][4];
       load_columns(b[0], 0, 0);

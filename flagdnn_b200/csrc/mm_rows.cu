@@ -11,6 +11,7 @@
 // ring (32 or 64 products) therefore has accumulators of its own, which are added to the sums in fp32 (5e-7).  That is why fp32 products
 // of any size come here: many rows in blocks of 64 x 128, whose operands are split once for eight or four products each.
 #include "group_norm.cuh"
+#include "mma_sync.cuh"
 #include "mm_rows.h"
 
 namespace fdnn {
@@ -28,43 +29,9 @@ constexpr int stages_of(int rows, int cols) {
 }
 constexpr int kShortRing = 4;   // .. four blocks to an SM
 
-__device__ __forceinline__ void copy16(uint32_t to, const void* from, int bytes) {   // the rest of the 16 is zeros
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
-}
 template <int BYTES>
 __device__ __forceinline__ void copy_few(uint32_t to, const void* from, bool there) {   // 4 or 8, or as many zeros
   asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(to), "l"(from), "n"(BYTES), "r"(there ? BYTES : 0) : "memory");
-}
-template <bool TRANS>
-__device__ __forceinline__ void ldmatrix(uint32_t (&r)[4], uint32_t at) {
-  if constexpr (TRANS)
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
-  else
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
-}
-template <typename T>
-__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  if constexpr (std::is_same<T, __half>::value)
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  else if constexpr (std::is_same<T, __nv_bfloat16>::value)
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  else
-    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-// fp32 as a TF32 number, rounded to nearest (by the integer unit: the conversion's instruction takes as long as the products), and what it
-// leaves, of either sign, whose last bits the tensor core does not read.  The first part is finite: the largest numbers do not become infinite,
-// and an infinity or NaN is all in the second.
-__device__ __forceinline__ void two_parts(float v, uint32_t& hi, uint32_t& lo) {
-  constexpr float kLargest = 3.4011621342146535e38f;   // of TF32: 2^127 (2 - 2^-10)
-  float h;
-  asm("min.xorsign.abs.f32 %0, %1, %2;" : "=f"(h) : "f"(__uint_as_float((__float_as_uint(v) + 0x1000u) & 0xffffe000u)), "f"(kLargest));
-  hi = __float_as_uint(h);
-  lo = __float_as_uint(v - h);
 }
 __device__ __forceinline__ float cluster_f32(uint32_t at) {
   float v;
@@ -201,7 +168,7 @@ mm_rows_kernel(const MmRowsParams p, int split) {
             const int c = (warp * WIDE + n) * 16 + g + (i & 1) * 8, kk = k * 8 + t + (i >> 1) * 4;
             two_parts(ORDER == Order::kColumns ? cols[kk * (kColPitch / 4) + c] : cols[c * (kPitch / 4) + kk], a[n][i], al[n][i]);
           }
-uint32_t b[ROWS / 8][2], bl[ROWS / 8][2];
+        uint32_t b[ROWS / 8][2], bl[ROWS / 8][2];
 #pragma unroll
         for (int j = 0; j < ROWS / 8; ++j)
 #pragma unroll
