@@ -281,6 +281,9 @@ cudaError_t go(const MmRowsParams& p, cudaStream_t stream) {
 template <typename T>
 cudaError_t by_layout(MmRowsParams p, cudaStream_t stream) {
   constexpr int kV = 16 / int(sizeof(T));
+  // a stride over an extent of one says nothing (a vector as b, 16 x 4096 x 1 in bf16: 10.2 us as if it did, 4.7 so)
+  if (p.M == 1) p.a_s[0] = 0;
+  if (p.N == 1) p.b_s[1] = 0;
   auto whole = [&](const void* q, long long along, long long across, long long extent) {
     return along == 1 && (reinterpret_cast<uintptr_t>(q) & 15u) == 0 && across % kV == 0 && extent % kV == 0;
   };

@@ -1,4 +1,4 @@
-"""mm_bias_act at the ends of its range: the most rows, the largest numbers, wide blocks.
+"""mm_bias_act at the ends of its range: the most rows, the largest numbers, wide blocks, vectors.
 
 Tolerances as in test_mm_bias_act_gpu.py."""
 import pytest
@@ -78,3 +78,19 @@ def test_wide_blocks(fd, case):  # noqa: F811
     bias = torch.randn(n, generator=g).cuda()
     for i, act in enumerate(ACTS):
         check(fd, a, b, bias if i % 2 else None, matrix(g, m, n, torch.float32, ("dense", "ragged", "t", "odd")[i]) if i < 3 else None, act)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("m,k,n", [(1, 4096, 1), (100, 4096, 1), (1, 520, 72), (5, 1, 1), (1, 1, 40), (300, 128, 1), (1, 129, 1)])
+def test_vectors(fd, m, k, n, dtype):  # noqa: F811
+    """Extents of one, whose strides say nothing."""
+    g = torch.Generator().manual_seed(m + k)
+    a, b = matrix(g, m, k, dtype, "dense"), matrix(g, k, n, dtype, "dense", k ** -0.5)
+    bias = torch.randn(n, generator=g).to(dtype).cuda()
+    want = check(fd, a, b, bias, matrix(g, m, n, dtype, "t"), "gelu_tanh")
+    if n == 1:
+        b = torch.as_strided(b, (k, 1), (1, 7))
+    if m == 1:
+        a = torch.as_strided(a, (1, k), (12345, 1))
+    assert torch.equal(check(fd, a, b, bias, None, "none"), check(fd, a.clone(), b.clone(), bias, None, "none"))
+    assert want.shape == (m, n)
