@@ -11,7 +11,9 @@ template <typename T>
 __device__ __forceinline__ float gate_at(const DeltaParams& p, const void* gates, long long i) {
   return p.gate_f32 ? static_cast<const float*>(gates)[i] : to_f32<T>(static_cast<const T*>(gates)[i]);
 }
-// The logarithm of the decay.  (One value a token and head: expf, not the special function unit's, whose results are cut downwards.)
+// The logarithm of the decay.  Its softplus takes a power from the special function unit, of a rounded argument: below 4e-7 + 8e-8 |dt| of
+// itself off (3.7e-7 measured at dt = -8 .. -6).  By expf in its place 2.5e-7, and the next tokens of 128 rows of 32 heads took 97 us in
+// place of 90.5: registers, four blocks to an SM.  (Held to five: 94.5, and 57 for 43 with keys of 256 channels.)
 __device__ __forceinline__ float log_decay(const DeltaParams& p, float delta, float bias, float A) {
   const float dt = delta + bias;
   return A * (p.softplus ? softplus(dt) : dt);

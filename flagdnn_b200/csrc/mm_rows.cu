@@ -8,7 +8,7 @@
 //
 // Sums are fp32; fp32 operands go in as 3 x TF32 (a high part, and what it leaves: 2^-22); one rounding at the end.  The tensor cores cut
 // what they add to an accumulator, always towards zero: a sum of 4096 fp32 products that stays in one is 3e-5 too small.  Each step of the
-// ring (32 or 64 products) therefore has accumulators of its own, which are added to the sums in fp32 (5e-7).  That is why fp32 products
+// ring (32 or 64 products) therefore has accumulators of its own, which are added to the sums in fp32 (at most 4e-7, 2e-7 in the mean).  That is why fp32 products
 // of any size come here: many rows in blocks of 64 x 128, whose operands are split once for eight or four products each.
 #include "group_norm.cuh"
 #include "mma_sync.cuh"

@@ -1,5 +1,5 @@
-"""gated_delta_rule where its inputs reach their ends: tokens that forget all, infinities, lengths, decays above one; and rows that
-are cut into segments, as their workspace tells.
+"""gated_delta_rule where its inputs reach their ends: tokens that forget all, infinities, lengths, decays above one, long
+sums of decays; and rows that are cut into segments, as their workspace tells.
 
 Tolerances as in test_delta_rule_gpu.py."""
 import ctypes
@@ -243,3 +243,32 @@ def test_values_far_below_their_chunks_largest(fd, dtype):  # noqa: F811
     want = do.gated_delta_rule(**v, **options)
     y = fd.gated_delta_rule(**v, **options)
     near(y, want.y, want.y_size + least_steps(v, options, torch.zeros(1, 2, 40, 64)) / STATE_TOL, dtype)
+
+
+@pytest.mark.parametrize("low,high", [(-8.0, -6.0), (-6.0, -4.0), (-4.0, -2.0), (-2.0, 0.0), (0.0, 2.0), (2.0, 6.0)])
+def test_raw_decays_add_up(fd, low, high):  # noqa: F811
+    """A state that forgets to e^-80 of itself, with nothing written, by tokens that are alike. A log decay's relative error: its softplus is a
+    polynomial (1.3e-7) of a power by the special function unit (2^-22), whose argument, log2 e times |dt|, is rounded (2^-24, and 1.3e-8 of the
+    constant: (2^-24 + 1.3e-8) |dt| of the power), then a product (2^-24). The state takes 2^-22 with a chunk's power and product, 3 * 2^-24
+    with a token's."""
+    g = torch.Generator().manual_seed(int(low) + 9)
+    n, heads = 8, 16
+    for length, by_step in ((1024, False), (64, True), (9, False)):
+        rows = torch.rand(n, heads, generator=g).cuda() * (high - low) + low
+        soft = torch.nn.functional.softplus(rows.double(), threshold=1000)
+        A = -(80.0 / (soft.mean(0) * length)).float()
+        total = soft * A.double() * length
+        q, v = torch.zeros(n, length, 1, 8, device="cuda"), torch.zeros(n, length, heads, 8, device="cuda")
+        delta, beta = rows[:, None].expand(n, length, heads).contiguous(), torch.full((n, length, heads), -200.0, device="cuda")
+        state = torch.ones(n, heads, 8, 8, device="cuda")
+        options = {"A": A, "delta_softplus": True, "beta_sigmoid": True}
+        if by_step:
+            for t in range(length):
+                fd.gated_delta_rule_step(q[:, t], q[:, t], v[:, t], delta[:, t], beta[:, t], state, **options)
+        else:
+            _, state = fd.gated_delta_rule(q, q, v, delta, beta, **options, initial_state=state, return_final_state=True)
+        want = total.exp()                                   # (of rates above the mean past fp32's normal numbers: steps of 2^-149 a product)
+        off = (state.double() - want[..., None, None]).abs().amax((2, 3))
+        each = 1.3e-7 + 2.0 ** -22 + (2.0 ** -24 + 1.3e-8) * rows.double().abs() + 2.0 ** -24
+        bound = each * total.abs() + (length // 64 * 2.0 ** -22 if length == 1024 else length * 3 * 2.0 ** -24)
+        assert (off <= bound * want + length * 2.0 ** -150).all(), float((off / (bound * want + length * 2.0 ** -150)).max())
