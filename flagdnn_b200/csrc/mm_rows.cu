@@ -8,8 +8,8 @@
 //
 // Sums are fp32; fp32 operands go in as 3 x TF32 (a high part, and what it leaves: 2^-22); one rounding at the end.  The tensor cores cut
 // what they add to an accumulator, always towards zero: a sum of 4096 fp32 products that stays in one is 3e-5 too small.  Each step of the
-// ring (32 or 64 products) therefore has accumulators of its own, which are added to the sums in fp32 (at most 4e-7, 2e-7 in the mean).  That is why fp32 products
-// of any size come here: many rows in blocks of 64 x 128, whose operands are split once for eight or four products each.
+// ring (32 or 64 products) therefore has accumulators of its own, which are added to the sums in fp32 (at most 4e-7, 2e-7 in the mean).  That
+// is why fp32 products of any size come here: many rows in blocks of 64 x 128, whose operands are split once for eight or four products each.
 #include "group_norm.cuh"
 #include "mma_sync.cuh"
 #include "mm_rows.h"
@@ -21,8 +21,8 @@ constexpr int kThreads = 128;
 constexpr int kWarps = kThreads / 32;
 constexpr int kTileBytes = 128;           // of the reduction, a step of the ring
 constexpr int kPitch = kTileBytes + 16;   // eight rows of 16 bytes lie in different banks
-// Steps of the ring: some 90 KB, two blocks to an SM; three of 64 fp32 rows, whose products are what bounds them (3000 x 500 x 500 78 us
-// with two, 52 with three).
+// Steps of the ring: some 90 KB, two blocks to an SM; four of 64 fp32 rows (300 x 1000 x 777 28.3 us with three steps, 21.0 with four;
+// 64 x 2048 x 4096 33.0 and 34.9).
 template <typename T>
 constexpr int stages_of(int rows, int cols) {
   return cols == 128 ? 4 : rows <= 16 ? 8 : rows <= 32 ? 6 : sizeof(T) == 4 ? 4 : 5;
@@ -251,11 +251,11 @@ cudaError_t go(const MmRowsParams& p, cudaStream_t stream) {
     const cudaError_t e = allow_smem(kernel, kRoom, done);
     if (e != cudaSuccess) return e;
     // No more blocks to an SM than an even spread has, where all of them still run at once: three blocks on some SMs and one on others take
-    // 44.8 us, two on each 35.3 (fp32, 64 x 2048 x 4096).  Clusters need their blocks in one group of SMs, so fewer fit than SMs would
+    // 44.9 us, two on each 35.0 (fp32, 64 x 2048 x 4096).  Clusters need their blocks in one group of SMs, so fewer fit than SMs would
     // hold: sixteen clusters of eight with an SM to a block ran in two waves (bf16, 16 x 1024 x 1024: 7.1 us for 4.4).
     // Not where two steps read the same 128 bytes of a row, which shorter rings leave in the L1 cache (2 x 7260 x 2432: 16.5 us, 21.2 with
-    // it); values one by one across columns lose there at times (fp32, 7 x 792 x 7905: 14.8 to 17.3) and gain more often (bf16,
-    // 33 x 7295 x 726: 37.3 to 33.0).
+    // it); values one by one across columns lose there at times (fp32, 7 x 792 x 7905: 15.7 to 18.0) and gain more often (bf16,
+    // 33 x 7295 x 726: 36.9 to 32.7).
     const long long blocks = tiles * split * row_blocks, each = (blocks + current_sm_count() - 1) / current_sm_count();
     int smem = kSmem;
     if (!(ORDER == Order::kAny && p.b_s[0] == 1) && each < kAlone && int(kRoom / each) - 2048 > kSmem) {
@@ -307,8 +307,8 @@ cudaError_t by_layout(MmRowsParams p, cudaStream_t stream) {
   if (p.M <= 16) return rows(std::integral_constant<int, 16>{}, one);
   if (p.M <= 32) return rows(std::integral_constant<int, 32>{}, one);
   if constexpr (sizeof(T) == 4) {
-    // 128 columns split rows of a half as often, 64 spread short reductions over more blocks: us with 64 and with 128, 100 x 2048 x 4096 76 and
-    // 53, 1000 x 4096 x 1024 273 and 186, 8192 x 4096 x 4096 5140 and 4370; 3000 x 500 x 500 52 and 62, 300 x 1000 x 777 26 and 31
+    // 128 columns split rows of a half as often, 64 spread short reductions over more blocks: us with 64 and with 128, 100 x 2048 x 4096 65 and
+    // 52, 1000 x 4096 x 1024 229 and 181, 8192 x 4096 x 4096 5850 and 4540; 3000 x 500 x 500 51 and 59, 300 x 1000 x 777 21 and 31
     const bool many = (p.M + 63ll) / 64 * ((p.N + 127ll) / 128) >= 2 * current_sm_count();
     if (p.M > 64 && (p.K > 1024 || many)) return rows(std::integral_constant<int, 64>{}, std::integral_constant<int, 2>{});
   }

@@ -397,7 +397,8 @@ int fdnn_gated_delta_rule_step(const fdnn_delta_rule_desc* desc, const void* q, 
 /* A product of few rows with its epilogue: y = act(a b + bias + residual), a [m, k], b [k, n] of any strides, bias [n] dense or NULL,
  * residual [m, n] or NULL; fp32 sums, one rounding (fp32 operands go in as two parts: an infinite one, or products past fp32's
  * range, give infinity or NaN).  fdnn_mm_rows_fwd takes any m (at most 2^22), but is made for a reading of b:
- * fdnn_mm_rows_preferred says whether it is ahead of the product as a 1x1 convolution (fdnn_conv2d_fwd_residual on a row of m pixels). */
+ * fdnn_mm_rows_preferred says, by sizes, strides and activation, whether it is ahead of the product as a 1x1 convolution
+ * (fdnn_conv2d_fwd_residual on a row of m pixels). */
 typedef struct fdnn_mm_desc {
   int32_t dtype;               /* FDNN_F16, FDNN_BF16 or FDNN_F32: every tensor */
   int32_t m, n, k;
