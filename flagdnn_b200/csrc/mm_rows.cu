@@ -333,9 +333,9 @@ cudaError_t by_layout(MmRowsParams p, cudaStream_t stream) {
 bool mm_rows_preferred(int dtype, const MmRowsParams& p) {
   if (p.K < 8 || dtype == FDNN_F32) return true;
   if (p.M > 16) return p.M <= (p.K < 4096 ? 512 : 1024) && (long long)p.M * p.N <= (p.K < 4096 ? 32ll * p.K : 131072);
-  // (operands that are not copied 16 bytes at a time are laid out anew for the convolution)
+  // (operands that are not copied 16 bytes at a time are laid out anew for the convolution; rows of y off 16 bytes cost it 1 to 4 us)
   auto whole = [](long long along, long long across, int extent) { return along == 1 && across % 8 == 0 && extent % 8 == 0; };
-  if (!whole(p.a_s[1], p.a_s[0], p.K) || !(whole(p.b_s[0], p.b_s[1], p.K) || whole(p.b_s[1], p.b_s[0], p.N))) return true;
+  if (p.N % 8 != 0 || !whole(p.a_s[1], p.a_s[0], p.K) || !(whole(p.b_s[0], p.b_s[1], p.K) || whole(p.b_s[1], p.b_s[0], p.N))) return true;
   const long long sms = current_sm_count(), tiles = (p.N + 127ll) / 128, at_once = sms / 2, rounds = (tiles + at_once - 1) / at_once;
   if (p.M == 16 && p.K >= 4096 && p.act <= FDNN_ACT_RELU) return 4 * tiles < 3 * rounds * at_once;
   return !(p.M > 4 && p.K < 1024 && p.N > 128 * sms);

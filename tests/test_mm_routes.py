@@ -11,7 +11,7 @@ from flagdnn_b200 import _native as nat
     (16, 4096, 8192, nat.ACT_NONE, False), (16, 4096, 8192, nat.ACT_RELU, False), (16, 4096, 8192, nat.ACT_GELU, True),
     (16, 4096, 8192, nat.ACT_GELU_TANH, True), (16, 4096, 12288, nat.ACT_NONE, True), (16, 8192, 8192, nat.ACT_NONE, False),
     (16, 2048, 8192, nat.ACT_NONE, True), (4, 512, 24576, nat.ACT_NONE, True), (8, 512, 24576, nat.ACT_NONE, False),
-    (16, 256, 18944, nat.ACT_GELU, True), (16, 256, 18952, nat.ACT_GELU, False), (8, 1024, 24576, nat.ACT_NONE, True)])
+    (16, 4096, 8188, nat.ACT_NONE, True), (8, 512, 24577, nat.ACT_NONE, True), (16, 256, 18944, nat.ACT_GELU, True), (16, 256, 18952, nat.ACT_GELU, False), (8, 1024, 24576, nat.ACT_NONE, True)])
 def test_up_to_sixteen_rows(native_lib, m, k, n, act, few):
     def preferred(dtype=nat.BF16, a=(k, 1), b=(n, 1)):
         d, yes = nat.MmDesc(), ctypes.c_int32()
